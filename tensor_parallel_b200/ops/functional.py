@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import math
 import os
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -117,6 +117,68 @@ def relative_bias_table_grad_ref(grad, buckets, rows: int):
     j = torch.arange(keys, device=buckets.device)[None, :]
     pairs = grad[0].permute(1, 2, 0).reshape(queries * keys, heads).float()
     return torch.zeros(rows, heads, dtype=torch.float32, device=grad.device).index_add(0, buckets[j - i + queries - 1].reshape(-1), pairs)
+
+
+class Int8Rows(NamedTuple):
+    """Rows in 8-bit integers with a scale each: ``values`` int8 ``[..., cols]``, ``scales`` fp32 ``[...]``; row ``r`` stands for
+    ``values[r] * scales[r]``.  An activation has a row per token, a weight a row per output channel.  Rows made here lie a multiple of 16 bytes apart,
+    as the matrix product reads them; what lies between is not written."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        return (self.values.float() * self.scales[..., None]).to(dtype)
+
+
+INT8_LEAST = 1e-30  # least maximum of a row, so that a row of zeros has a finite factor
+INT8_MAX_K = 131071  # longest contraction whose sum stays below 2^31 whatever the integers are
+
+
+def _int8_rows_ref(v: torch.Tensor, factor: Optional[torch.Tensor] = None) -> Int8Rows:
+    most = v.abs().amax(-1, keepdim=True).clamp_min(INT8_LEAST)
+    full = torch.full_like(most, 127.0)  # (with a plain number, PyTorch multiplies by a rounded reciprocal)
+    values = torch.round(v * (full / most))
+    scales = (most / full)[..., 0]
+    finite = torch.isfinite(most)
+    scales = torch.where(finite[..., 0], scales if factor is None else scales * factor, torch.full_like(scales, float("nan")))
+    return Int8Rows(torch.where(finite, values, torch.zeros_like(values)).to(torch.int8), scales)
+
+
+def quantize_int8_ref(x) -> Int8Rows:
+    return _int8_rows_ref(x.float())
+
+
+def _add_ref(x, residual):
+    return x if residual is None else (x.float() + residual.float()).to(x.dtype)
+
+
+def rms_norm_int8_ref(x, weight, eps: float, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
+    h = _add_ref(x, residual)
+    hf = h.float()
+    rstd = torch.rsqrt(hf.pow(2).mean(-1) + eps)
+    return _int8_rows_ref(hf if weight is None else hf * weight.to(x.dtype).float(), rstd), h
+
+
+def layer_norm_int8_ref(x, weight, bias, eps: float, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
+    h = _add_ref(x, residual)
+    w, b = (None if t is None else t.to(x.dtype).float() for t in (weight, bias))
+    return _int8_rows_ref(F.layer_norm(h.float(), h.shape[-1:], w, b, eps)), h
+
+
+def linear_int8_ref(x: Int8Rows, weight: Int8Rows, bias=None, act: Optional[str] = None, residual=None):
+    # (64 bits hold the sums of products exactly)
+    v = torch.matmul(x.values.double(), weight.values.double().t()).float() * x.scales[..., None] * weight.scales
+    if bias is not None:
+        v = v + bias.float()
+    if act == "swiglu16":
+        pairs = v.unflatten(-1, (-1, 2, 16))
+        v = (F.silu(pairs[..., 0, :]) * pairs[..., 1, :]).flatten(-2)
+    elif act is not None:
+        v = {"relu": F.relu, "silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh")}[act](v)
+    if residual is not None:
+        v = v + residual.float()
+    return v.to(torch.bfloat16)
 
 
 # -- dispatching front-end ---------------------------------------------------------------------
@@ -236,6 +298,88 @@ def geglu(gate, up, approximate: str = "tanh"):
     if nat is not None and nat.elementwise_supported(gate):
         return nat.geglu(gate, up, approximate)
     return geglu_ref(gate, up, approximate)
+
+
+# -- 8-bit integers (serving) --------------------------------------------------------------------
+
+
+def _serving_only(what: str, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+
+
+def _check_rows(what: str, x, weight=None, bias=None, residual=None):
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{what} takes bf16 or fp32 rows, got {x.dtype}")
+    if x.ndim < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{what} takes rows of at least one column, got {tuple(x.shape)}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != x.shape[-1:] or t.device != x.device):
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} on {t.device} does not fit rows {tuple(x.shape)} on {x.device}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError(f"{what}: the residual has to be like x ({tuple(x.shape)}, {x.dtype}, {x.device}), got {tuple(residual.shape)}, {residual.dtype}, {residual.device}")
+    _serving_only(what, x, weight, bias, residual)
+
+
+def quantize_int8(x) -> Int8Rows:
+    """The rows of ``x`` (bf16 or fp32, ``[..., cols]``) in 8 bits: ``rint(x * (127 / max |x|))`` and ``max |x| / 127``, ties to even.  For an activation
+    in front of :func:`linear_int8`, and for its weight (a row per output channel).  A row with a value that is not finite gets the scale NaN.
+    Serving only: there is no gradient."""
+    _check_rows("quantize_int8", x)
+    nat = _native(x)
+    return nat.quantize_int8(x) if nat is not None else quantize_int8_ref(x)
+
+
+def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
+    """``(rows, h)``: ``h = x + residual``, rounded to the type of ``x`` (``x`` itself without a residual), and its RMSNorm in 8 bits, as
+    :func:`quantize_int8` gives them.  ``weight`` may be None."""
+    _check_rows("rms_norm_int8", x, weight, residual=residual)
+    nat = _native(x)
+    return nat.norm_int8(x, weight, None, eps, 0, residual) if nat is not None else rms_norm_int8_ref(x, weight, eps, residual)
+
+
+def layer_norm_int8(x, weight, bias, eps: float = 1e-5, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
+    """Like :func:`rms_norm_int8`, with a LayerNorm; ``weight`` and ``bias`` may be None."""
+    _check_rows("layer_norm_int8", x, weight, bias, residual)
+    nat = _native(x)
+    return nat.norm_int8(x, weight, bias, eps, 1, residual) if nat is not None else layer_norm_int8_ref(x, weight, bias, eps, residual)
+
+
+_INT8_ACTS = (None, "relu", "gelu", "gelu_tanh", "silu", "swiglu16")
+
+
+def _check_linear_int8(x, weight, bias, act, residual):
+    for name, rows in (("x", x), ("weight", weight)):
+        v, s = rows
+        if v.dtype != torch.int8 or s.dtype != torch.float32 or s.shape != v.shape[:-1] or s.device != v.device:
+            raise ValueError(f"linear_int8: {name} takes int8 values with one fp32 scale per row, got {v.dtype} {tuple(v.shape)} and {s.dtype} {tuple(s.shape)}")
+    xv, wv = x[0], weight[0]
+    if xv.ndim < 2 or wv.ndim != 2 or xv.shape[-1] != wv.shape[1] or xv.device != wv.device:
+        raise ValueError(f"linear_int8: rows {tuple(xv.shape)} on {xv.device} and a weight {tuple(wv.shape)} on {wv.device} do not contract")
+    features, k = wv.shape
+    if not 0 < k <= INT8_MAX_K or features == 0:
+        raise ValueError(f"linear_int8 contracts 1 to {INT8_MAX_K} columns into at least one feature, got a weight {tuple(wv.shape)}")
+    if act not in _INT8_ACTS:
+        raise ValueError(f"linear_int8: unknown activation {act!r}")
+    if act == "swiglu16" and (features % 32 or residual is not None):
+        raise ValueError("linear_int8: swiglu16 takes weight rows in groups of 16 gate and 16 up rows, and no residual")
+    if bias is not None and (bias.shape != (features,) or bias.dtype != torch.bfloat16 or bias.device != xv.device):
+        raise ValueError(f"linear_int8: the bias has to be bf16 [{features}] on {xv.device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+    if residual is not None and (residual.shape != (*xv.shape[:-1], features) or residual.dtype != torch.bfloat16 or residual.device != xv.device):
+        raise ValueError(f"linear_int8: the residual has to be bf16 {(*xv.shape[:-1], features)} on {xv.device}, got {residual.dtype} {tuple(residual.shape)} on {residual.device}")
+    _serving_only("linear_int8", x[1], weight[1], bias, residual)
+
+
+def linear_int8(x: Int8Rows, weight: Int8Rows, bias=None, act: Optional[str] = None, residual=None):
+    """``act(x @ weight.T + bias) + residual`` in bf16, for rows and a weight in 8 bits (:class:`Int8Rows`, ``[..., k]`` and ``[features, k]``): the sums of
+    products are exact integers, scales, bias, activation and residual are fp32.  ``act``: None, ``"relu"``, ``"gelu"``, ``"gelu_tanh"``, ``"silu"``, or
+    ``"swiglu16"`` for a weight whose rows alternate in groups of 16 gate and 16 up rows (``silu(gate) * up``, half as many columns).  Serving only:
+    there is no gradient."""
+    _check_linear_int8(x, weight, bias, act, residual)
+    nat = _native(x[0])
+    if nat is not None:
+        return nat.linear_int8(x, weight, bias, act, residual)
+    return linear_int8_ref(Int8Rows(*x), Int8Rows(*weight), bias, act, residual)
 
 
 def cross_entropy(logits, labels, ignore_index: int = -100):

@@ -960,4 +960,108 @@ def adamw_step(param, grad, exp_avg, exp_avg_sq, step, lr, beta1, beta2, eps, we
     _launches += 1
 
 
+# ------------------------------------------------------------------------------------------------
+# 8-bit integers: rows with a scale each, and their matrix product (serving)
+# ------------------------------------------------------------------------------------------------
+
+LIB.tpb_rows_int8.argtypes = [c_void_p] * 7 + [c_int] * 2 + [c_ll] * 4 + [c_float] + [c_int] * 3 + [c_void_p]
+LIB.tpb_gemm_int8.argtypes = [c_void_p] * 7 + [c_int] * 3 + [c_ll] * 4 + [c_int] * 2 + [c_void_p] * 2
+
+
+def int8_rows_empty(rows: int, cols: int, device) -> OF.Int8Rows:
+    """Room for 8-bit rows that lie a multiple of 16 bytes apart."""
+    pitch = (cols + 15) // 16 * 16
+    values = torch.empty(rows, pitch, dtype=torch.int8, device=device)
+    return OF.Int8Rows(values if pitch == cols else values[:, :cols], torch.empty(rows, dtype=torch.float32, device=device))
+
+
+def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, sum_out=None, out=None, early=False) -> OF.Int8Rows:
+    """8-bit rows of ``x2d`` (rows of any pitch with unit inner stride) as they are, or (``norm`` 0 / 1) of the RMSNorm / LayerNorm of ``x2d + residual``, which is
+    also stored to ``sum_out`` (may be ``x2d``).  ``weight`` and ``bias`` have the type of ``x2d``.  ``out``: rows to write (:func:`int8_rows_empty`).  ``early``: see
+    :func:`gemm_nt` (nothing is read before the previous kernel has finished)."""
+    global _launches
+    rows, cols = x2d.shape
+    out = int8_rows_empty(rows, cols, x2d.device) if out is None else out
+    if rows == 0:
+        return out
+    check(LIB.tpb_rows_int8(_ptr(x2d), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(sum_out), _ptr(out[0]), _ptr(out[1]), rows, cols, _pitch(x2d),
+                            _pitch(residual), _pitch(sum_out), _pitch(out[0]), eps,
+                            0 if norm is None else norm + 1, _dtype_code(x2d), int(early), _stream()), "tpb_rows_int8")
+    _launches += 1
+    return out
+
+
+def _rows_view(t):
+    """``t`` as rows with unit inner stride: a view where its strides allow it."""
+    t = t if t.ndim == 2 else t.reshape(-1, t.shape[-1])
+    rows, cols = t.shape
+    return t if (t.stride(1) == 1 or cols == 1) and (t.stride(0) >= cols or rows == 1) else t.contiguous()
+
+
+def _pitch(t) -> int:
+    """Row pitch of ``t`` (that of a single row, which its stride need not say, is its padded length)."""
+    return 0 if t is None else t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
+def _int8_shaped(rows: OF.Int8Rows, shape) -> OF.Int8Rows:
+    if len(shape) == 2:
+        return rows
+    values, scales = rows
+    # (a split of the row dimension of padded rows is a view too)
+    return OF.Int8Rows(values.unflatten(0, shape[:-1]) if len(shape) > 2 else values[0], scales.view(shape[:-1]))
+
+
+def quantize_int8(x) -> OF.Int8Rows:
+    with torch.cuda.device(x.device):
+        return _int8_shaped(rows_int8(_rows_view(x)), x.shape)
+
+
+def norm_int8(x, weight, bias, eps, mode, residual=None):
+    with torch.cuda.device(x.device):
+        x2d = _rows_view(x)
+        w, b = (None if t is None else t.to(x.dtype).contiguous() for t in (weight, bias))
+        res = None if residual is None else _rows_view(residual)
+        summed = None if residual is None else torch.empty(x2d.shape, dtype=x.dtype, device=x.device)
+        rows = rows_int8(x2d, w, b, eps, mode, res, summed)
+        return _int8_shaped(rows, x.shape), x if summed is None else summed.view(x.shape)
+
+
+def gemm_int8(x: OF.Int8Rows, weight: OF.Int8Rows, bias=None, act=None, residual=None, out=None, early=False):
+    """``act(x @ weight.T + bias) + residual`` of 8-bit rows ``[tokens, k]`` and ``[features, k]``, bf16.  ``residual`` may be ``out``.  ``early``: see :func:`gemm_nt`."""
+    global _launches
+    (xv, sx), (given, sw) = x, weight
+    tokens, k = xv.shape
+    features = given.shape[0]
+    xv, wv = _int8_ready(xv), _int8_ready(given)
+    cols = features // 2 if act == "swiglu16" else features
+    out = torch.empty(tokens, cols, dtype=torch.bfloat16, device=xv.device) if out is None else out
+    if tokens == 0:
+        return out
+    check(LIB.tpb_gemm_int8(_ptr(xv), _ptr(sx), _ptr(wv), _ptr(sw), _ptr(out), _ptr(bias), _ptr(residual), tokens, features, k, _pitch(xv), _pitch(wv),
+                            _pitch(out), _pitch(residual), ACT_CODES[act], int(early and wv is given),
+                            _ptr(device_state(xv.device).status), _stream()), "tpb_gemm_int8")
+    _launches += 1
+    return out
+
+
+def _int8_ready(t: torch.Tensor) -> torch.Tensor:
+    """TMA's rules (see :func:`_tma_ready`) for 8-bit rows."""
+    rows, k = t.shape
+    if (t.stride(1) == 1 or k == 1) and (rows == 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= k)) and t.data_ptr() % 16 == 0:
+        return t
+    buf = int8_rows_empty(*t.shape, t.device).values
+    buf.copy_(t)
+    return buf
+
+
+def linear_int8(x: OF.Int8Rows, weight: OF.Int8Rows, bias=None, act=None, residual=None):
+    (xv, sx), (wv, sw) = x, weight
+    with torch.cuda.device(xv.device):
+        shape = xv.shape
+        x2d = xv if xv.ndim == 2 else xv.reshape(-1, shape[-1])
+        res = None if residual is None else _rows_view(residual)
+        out = gemm_int8((x2d, sx.reshape(-1).contiguous()), (wv, sw.contiguous()), None if bias is None else bias.contiguous(), act, res)
+        return out if len(shape) == 2 else out.view(*shape[:-1], out.shape[1])
+
+
 LIB.tpb_last_cuda_error.argtypes = [ctypes.c_char_p, c_int]
