@@ -1,93 +1,315 @@
-// Matrix product of 8-bit integers with a scale per token and per output channel:
-//   out[t, f] = act(sx[t] sw[f] sum_k x[t, k] w[f, k] + bias[f]) + residual[t, f]
-// The sum is exact (32-bit integers; k <= 131071, so that even rows of -128 stay below 2^31), the rest is fp32, rounded once to bf16.
+// Product of 8-bit integers: the entry point, and the kernel for many tokens on CTA pairs (see gemm_i8.cuh; few tokens: gemm_i8_stream_sm100.cu).
+//
+// The decomposition is that of the bf16 kernel (gemm_pair_sm100.cu): two CTAs on neighbouring SMs work on one tile of 256 tokens x BN features with
+// tcgen05.mma.cta_group::2, each loads 128 token rows and BN / 2 feature rows, the leader issues for both.  A k-block is 128 bytes of every row there
+// and here: 128 columns, 512 clocks of the tensor core at BN = 256.  Sums are 32-bit integers, the epilogue scales them.
+//
+// One CTA (192 threads), persistent over the pair's tiles:
+//   warp 0    : TMA producer of this CTA's operand rows; completion is counted on the LEADER's barrier (no multicast)
+//   warp 1    : leader only: one thread issues the MMAs; the commits signal the barriers of both CTAs
+//   warps 2-5 : epilogue of this CTA's 128 rows, two TMEM accumulators so that it runs under the next tile's MMAs
+// Every mbarrier wait is bounded; on expiry the CTA records a status code and drains.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
 
+#include <atomic>
+
+#include "gemm_i8.cuh"
 #include "launch.cuh"
 #include "ptx_sm100.cuh"
 #include "tpb_api.h"
 
 namespace tpb {
 
-constexpr int I8_MAX_K = 131071;
-constexpr int I8_GATED = 5;  // act: 16 gate rows of the weight, then their 16 up rows
+constexpr int I8_MAX_K = 131071;  // rows of -128 that long sum up to 2^31 - 2^14
+constexpr int IP_BM = 256;        // tokens of a pair tile (128 per CTA = TMEM lanes)
+constexpr int IP_THREADS = 192;
+constexpr int IP_MAX_STAGES = 8;
+constexpr int IP_BAND = 8;        // tiles are walked in bands of 8 token tiles x all feature tiles
 
-struct I8Gemm {
-  const int8_t *x, *w;
-  const float *sx, *sw;
-  __nv_bfloat16* out;
-  const __nv_bfloat16 *bias, *residual;
-  long long ldx, ldw, ld_out, ld_res;
-  int tokens, features, k, act;
+struct IpParams {
+  I8Gemm g;
+  int k_blocks, m_tiles, n_tiles;
 };
 
-__device__ __forceinline__ float i8_act(float x, int act) {
-  switch (act) {
-    case 1: return fmaxf(x, 0.f);
-    case 2: return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-    case 3: return 0.5f * x * (1.f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
-    case 4: return x / (1.f + expf(-x));
-    default: return x;
-  }
-}
+template <int BN>
+struct IpShape {
+  static constexpr int STAGES = BN == 256 ? 6 : 8;
+  static constexpr uint32_t A_BYTES = 128 * I8_BK;
+  static constexpr uint32_t B_BYTES = BN / 2 * I8_BK;
+  static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr size_t SMEM = size_t(STAGES) * STAGE_BYTES + 1024 /*align*/ + (2 * IP_MAX_STAGES + 4) * 8 + 16;
+};
 
-// 64 x 64 outputs per CTA on the integer dot products of the CUDA cores, 4 x 4 per thread: columns ty, ty + 16, .. of the tokens and tx,
-// tx + 16, .. of the features, so that a gate column and its up column are one thread's.
-constexpr int I8_TILE = 64, I8_STEP = 64;
-__global__ void __launch_bounds__(256)
-gemm_i8_kernel(const I8Gemm p) {
-  __shared__ int xs[I8_TILE][I8_STEP / 4 + 1], ws[I8_TILE][I8_STEP / 4 + 1];
+template <int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(IP_THREADS, 1)
+gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const IpParams p) {
+  using S = IpShape<BN>;
+  constexpr uint32_t TMEM_COLS = 2 * BN;
+  const I8Gemm& g = p.g;
+  extern __shared__ uint8_t ip_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ip_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + size_t(S::STAGES) * S::STAGE_BYTES);  // used in the leader
+  uint64_t* empty_bar = full_bar + IP_MAX_STAGES;
+  uint64_t* acc_full = empty_bar + IP_MAX_STAGES;  // [2]
+  uint64_t* acc_empty = acc_full + 2;              // [2], used in the leader
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();  // 0 = leader
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = p.m_tiles * p.n_tiles;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 8);  // one arrival per epilogue warp of either CTA
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
   pdl_trigger();
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int t0 = blockIdx.y * I8_TILE, f0 = blockIdx.x * I8_TILE;
-  int acc[4][4] = {};
-  auto word = [&](const int8_t* rows, long long ld, int row, int count, int k0) {  // 4 bytes of a row, zero where it has ended
-    uint32_t v = 0;
-    if (row < count) {
-      const int8_t* at = rows + row * ld + k0;
-      for (int i = 0; i < 4; ++i)
-        if (k0 + i < p.k) v |= uint32_t(uint8_t(at[i])) << (8 * i);
-    }
-    return int(v);
+
+  auto tile_at = [&](int t, int& mt, int& nt) {
+    const int band = t / (IP_BAND * p.n_tiles), r = t - band * IP_BAND * p.n_tiles;
+    const int rows = min(IP_BAND, p.m_tiles - band * IP_BAND);
+    mt = band * IP_BAND + r % rows;
+    nt = r / rows;
   };
-  for (int k0 = 0; k0 < p.k; k0 += I8_STEP) {
-    for (int i = threadIdx.x; i < I8_TILE * I8_STEP / 4; i += 256) {
-      const int r = i / (I8_STEP / 4), c = i % (I8_STEP / 4);
-      xs[r][c] = word(p.x, p.ldx, t0 + r, p.tokens, k0 + 4 * c);
-      ws[r][c] = word(p.w, p.ldw, f0 + r, p.features, k0 + 4 * c);
+  auto give_up = [&]() {
+    atomicMax(g.status, STATUS_TIMEOUT_MBAR);
+    *abort_flag = 1;
+  };
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += pairs) {
+        int mt, nt;
+        tile_at(t, mt, nt);
+        const int m0 = mt * IP_BM + int(rank) * 128, n0 = nt * BN + int(rank) * (BN / 2);
+        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+          const int s = it % S::STAGES;
+          if (*abort_flag || !mbar_wait(&empty_bar[s], ((it / S::STAGES) & 1) ^ 1)) {
+            give_up();
+            ok = false;
+            break;
+          }
+          uint8_t* a_dst = smem + size_t(s) * S::STAGE_BYTES;
+          const uint32_t bar = mapa_u32(smem_u32(&full_bar[s]), 0);
+          if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * S::STAGE_BYTES);  // both CTAs' bytes
+          tma_load_2d_pair(a_dst, &tmap_a, bar, kb * I8_BK, m0);
+          tma_load_2d_pair(a_dst + S::A_BYTES, &tmap_b, bar, kb * I8_BK, n0);
+        }
+      }
+      // the leader's last commits still arrive on this CTA's barriers: stay until each used stage has been released
+      for (uint32_t i = it > uint32_t(S::STAGES) ? it - S::STAGES : 0; ok && i < it; ++i) {
+        if (!mbar_wait(&empty_bar[i % S::STAGES], (i / S::STAGES) & 1)) {
+          give_up();
+          ok = false;
+        }
+      }
     }
-    __syncthreads();
-    for (int c = 0; c < I8_STEP / 4; ++c) {
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = make_idesc_i8(IP_BM, BN);
+      uint32_t it = 0, local = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += pairs, ++local) {
+        const int acc = local & 1;
+        if (*abort_flag || !mbar_wait(&acc_empty[acc], ((local >> 1) & 1) ^ 1)) {
+          give_up();
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+          const int s = it % S::STAGES;
+          if (!mbar_wait(&full_bar[s], (it / S::STAGES) & 1)) {
+            give_up();
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + size_t(s) * S::STAGE_BYTES), b_addr = a_addr + S::A_BYTES;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(xs[ty + 16 * i][c], ws[tx + 16 * j][c], acc[i][j]);
+          for (int kk = 0; kk < I8_BK / 32; ++kk)
+            umma_i8_pair(d_tmem, make_desc_kmajor_sw128(a_addr + kk * 32), make_desc_kmajor_sw128(b_addr + kk * 32), idesc, (kb | kk) ? 1u : 0u);
+          umma_commit_pair(&empty_bar[s]);
+        }
+        if (ok) umma_commit_pair(&acc_full[acc]);
+      }
     }
-    __syncthreads();
+  } else {
+    const int quarter = warp & 3;  // TMEM lane quarter this warp may access
+    const int row = quarter * 32 + lane;
+    const uint32_t acc_empty_leader[2] = {mapa_u32(smem_u32(&acc_empty[0]), 0), mapa_u32(smem_u32(&acc_empty[1]), 0)};
+    const bool gated = g.act == I8_GATED;
+    auto aligned = [](const void* ptr, long long ld) { return !(reinterpret_cast<uintptr_t>(ptr) & 15) && (ld & 7) == 0; };
+    const bool vec = aligned(g.out, g.ld_out) && aligned(g.bias, 0) && (!g.residual || aligned(g.residual, g.ld_res)) && !(reinterpret_cast<uintptr_t>(g.sw) & 15);
+    const bool sectors = vec && (g.ld_out & 15) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 31);
+    uint32_t local = 0;
+    for (int t = pair; t < tiles; t += pairs, ++local) {
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const int m = mt * IP_BM + int(rank) * 128 + row;
+      const int acc = local & 1;
+      const float sx = m < g.tokens ? g.sx[m] : 0.f;
+      const bool ready = !*abort_flag && mbar_wait(&acc_full[acc], (local >> 1) & 1);
+      if (!__all_sync(0xffffffffu, ready)) {
+        if (lane == 0) give_up();
+        break;
+      }
+      tc_fence_after();
+      const uint32_t t_lane = tmem_base + (uint32_t(quarter * 32) << 16) + acc * BN;
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += 32) {
+        const int n0 = nt * BN + c0;
+        if (n0 >= g.features) break;
+        uint32_t r[32];
+        __syncwarp();  // (rows past the end skip the rest of a chunk)
+        tmem_ld_x32(t_lane + c0, r);
+        tmem_ld_wait();
+        if (m >= g.tokens) continue;
+        __nv_bfloat16* out = g.out + m * g.ld_out + (gated ? n0 >> 1 : n0);
+        const __nv_bfloat16* residual = g.residual ? g.residual + m * g.ld_res + n0 : nullptr;
+        if (vec && n0 + 32 <= g.features) {
+          float v[32];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 s = __ldg(reinterpret_cast<const float4*>(g.sw + n0) + q);
+            float b[4] = {0.f, 0.f, 0.f, 0.f};
+            if (g.bias) {
+              const uint2 b2 = __ldg(reinterpret_cast<const uint2*>(g.bias + n0) + q);
+              b[0] = bf16_bits_to_float(b2.x & 0xFFFF);
+              b[1] = bf16_bits_to_float(b2.x >> 16);
+              b[2] = bf16_bits_to_float(b2.y & 0xFFFF);
+              b[3] = bf16_bits_to_float(b2.y >> 16);
+            }
+            v[4 * q] = i8_value(int(r[4 * q]), sx, s.x, b[0]);
+            v[4 * q + 1] = i8_value(int(r[4 * q + 1]), sx, s.y, b[1]);
+            v[4 * q + 2] = i8_value(int(r[4 * q + 2]), sx, s.z, b[2]);
+            v[4 * q + 3] = i8_value(int(r[4 * q + 3]), sx, s.w, b[3]);
+          }
+          if (gated) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = i8_silu(v[j]) * v[16 + j];
+          } else if (g.act) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = i8_act(v[j], g.act);
+          }
+          if (residual) {
+            const uint4* rp = reinterpret_cast<const uint4*>(residual);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint4 r4 = rp[q];
+              const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                v[8 * q + 2 * j] += bf16_bits_to_float(rw[j] & 0xFFFF);
+                v[8 * q + 2 * j + 1] += bf16_bits_to_float(rw[j] >> 16);
+              }
+            }
+          }
+          uint32_t w[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+          if (sectors) {  // whole 32-byte sectors
+            st_global_v8(out, w);
+            if (!gated) st_global_v8(out + 16, w + 8);
+          } else {
+            uint4* op = reinterpret_cast<uint4*>(out);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (q < 2 || !gated) op[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+          }
+        } else if (gated) {  // (the feature count is a multiple of 32: only alignment can be missing)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float gate = i8_value(int(r[j]), sx, g.sw[n0 + j], g.bias ? __bfloat162float(g.bias[n0 + j]) : 0.f);
+            const float up = i8_value(int(r[16 + j]), sx, g.sw[n0 + 16 + j], g.bias ? __bfloat162float(g.bias[n0 + 16 + j]) : 0.f);
+            out[j] = __float2bfloat16(i8_silu(gate) * up);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (n0 + j < g.features) {
+              float x = i8_value(int(r[j]), sx, g.sw[n0 + j], g.bias ? __bfloat162float(g.bias[n0 + j]) : 0.f);
+              if (g.act) x = i8_act(x, g.act);
+              if (residual) x += __bfloat162float(residual[j]);
+              out[j] = __float2bfloat16(x);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty_leader[acc]);  // both accumulator halves may be overwritten after 8 of these
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = t0 + ty + 16 * i;
-    if (t >= p.tokens) continue;
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int f = f0 + tx + 16 * j;
-      v[j] = f < p.features ? float(acc[i][j]) * (p.sx[t] * p.sw[f]) + (p.bias ? __bfloat162float(p.bias[f]) : 0.f) : 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int f = f0 + tx + 16 * j;
-      if (f >= p.features || (p.act == I8_GATED && (j & 1))) continue;
-      const int c = p.act == I8_GATED ? (f >> 5) * 16 + (f & 15) : f;
-      float r = p.act == I8_GATED ? i8_act(v[j], 4) * v[(j + 1) & 3] : i8_act(v[j], p.act);
-      if (p.residual) r += __bfloat162float(p.residual[t * p.ld_res + c]);
-      p.out[t * p.ld_out + c] = __float2bfloat16(r);
-    }
+
+  // both CTAs stay until nobody can touch the other's barriers or TMEM any more
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+}
+
+template <int BN>
+static int ip_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
+  using S = IpShape<BN>;
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TPB_ERR_CUDA;
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(gemm_i8_pair_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::SMEM)) != cudaSuccess) return TPB_ERR_CUDA;
+    configured[dev].store(true, std::memory_order_release);
   }
+  CUtensorMap ta, tb;
+  int rc = i8_tmap(&ta, g.x, g.tokens, g.k, g.ldx, 128);
+  if (rc == TPB_OK) rc = i8_tmap(&tb, g.w, g.features, g.k, g.ldw, BN / 2);
+  if (rc != TPB_OK) return rc;
+  IpParams p;
+  memset(&p, 0, sizeof(p));
+  p.g = g;
+  p.k_blocks = (g.k + I8_BK - 1) / I8_BK;
+  p.m_tiles = (g.tokens + IP_BM - 1) / IP_BM;
+  p.n_tiles = (g.features + BN - 1) / BN;
+  const long long tiles = (long long)p.m_tiles * p.n_tiles;
+  if (tiles > 0x7fffffffLL - sms) return TPB_ERR_SIZE;
+  const int pairs = int(tiles < sms / 2 ? tiles : sms / 2);
+  return launch_dependent(gemm_i8_pair_kernel<BN>, dim3(2 * pairs), dim3(IP_THREADS), S::SMEM, stream, g.early != 0, ta, tb, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+}
+
+// Columns of the pair tile: rounds of tiles x time of a k-block, in clocks (as gemm_pair_tile has them).
+static int ip_tile(int tokens, int features, int sms) {
+  auto rounds = [&](int bn) {
+    const long long tiles = (long long)((tokens + IP_BM - 1) / IP_BM) * ((features + bn - 1) / bn);
+    return (tiles + sms / 2 - 1) / (sms / 2);
+  };
+  return rounds(256) * 512 <= rounds(128) * 351 ? 256 : 128;
 }
 
 }  // namespace tpb
@@ -102,9 +324,14 @@ extern "C" int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, 
   if (act == tpb::I8_GATED && (features % 32 || residual)) return TPB_ERR_ARG;
   if (ldx < k || ldw < k || ld_out < cols || (residual && ld_res < cols)) return TPB_ERR_ARG;
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) || ldx % 16 || ldw % 16) return TPB_ERR_ALIGN;
-  tpb::I8Gemm p = {x, w, sx, sw, static_cast<bf16*>(out), static_cast<const bf16*>(bias), static_cast<const bf16*>(residual), ldx, ldw, ld_out, ld_res,
-                   tokens, features, k, act};
-  const dim3 grid((features + tpb::I8_TILE - 1) / tpb::I8_TILE, (tokens + tpb::I8_TILE - 1) / tpb::I8_TILE);
-  if (grid.y > 65535) return TPB_ERR_SIZE;
-  return tpb::launch_dependent(tpb::gemm_i8_kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), early != 0, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  if (((reinterpret_cast<uintptr_t>(sx) | reinterpret_cast<uintptr_t>(sw)) & 3) ||
+      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(residual)) & 1))
+    return TPB_ERR_ALIGN;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return TPB_ERR_CUDA;
+  const tpb::I8Gemm g = {x, w, sx, sw, static_cast<bf16*>(out), static_cast<const bf16*>(bias), static_cast<const bf16*>(residual), ldx, ldw, ld_out, ld_res,
+                         tokens, features, k, act, early, static_cast<uint32_t*>(status)};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (tokens <= 64) return tpb::gemm_i8_stream_launch(g, sms, s);
+  return tpb::ip_tile(tokens, features, sms) == 256 ? tpb::ip_launch<256>(g, sms, s) : tpb::ip_launch<128>(g, sms, s);
 }
