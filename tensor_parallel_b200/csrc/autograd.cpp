@@ -1,4 +1,5 @@
-// Autograd nodes of the layers whose training calls are bound by the host at ordinary sizes: linear and norms.
+// Autograd nodes of the layers whose training calls are bound by the host at ordinary sizes: linear and norms.  And, without nodes, the calls of
+// 8-bit serving, whose kernels take a few microseconds each at decode sizes.
 //
 // A small call (100 tokens through a 768 x 3072 projection with bias, forward and backward) keeps the GPU busy for 37 us.  As Python
 // autograd functions over ctypes it took 176 us: each of its launches cost 10 to 20 us of interpreter work, and the backward nodes
@@ -9,7 +10,9 @@
 // (a variant with index checks, for instance), and the two callbacks that need Python objects.
 #include <torch/extension.h>
 
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <atomic>
 #include <stdexcept>
@@ -30,6 +33,8 @@ struct Library {
   decltype(&tpb_norm_bwd_parts) norm_bwd_parts = nullptr;
   decltype(&tpb_col_sum_parts) col_sum_parts = nullptr;
   decltype(&tpb_col_sum) col_sum = nullptr;
+  decltype(&tpb_rows_int8) rows_int8 = nullptr;
+  decltype(&tpb_gemm_int8) gemm_int8 = nullptr;
 };
 Library lib;
 PyObject* error_text = nullptr;     // (code, what) -> message
@@ -274,6 +279,100 @@ Tensor norm(const Tensor& x, const std::optional<Tensor>& weight, const std::opt
   return NormFn::apply(x, weight, bias, eps, mode);
 }
 
+// ---- 8-bit serving ----
+// The ordinary calls: plain CUDA tensors that fit together and lie as the kernels read them, nothing that takes a gradient, no tracing.  Every other call
+// gets no value here and goes on in Python, which says what is wrong with it, or makes the copies that it needs.
+
+bool plain(const Tensor& t, at::ScalarType dtype, const c10::Device& device) {
+  return t.scalar_type() == dtype && t.device() == device && t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() &&
+         !(at::GradMode::is_enabled() && t.requires_grad());
+}
+// Rows that lie one pitch apart: their number, and the pitch (of a single row, its length rounded up).
+bool rows_apart(const Tensor& t, int64_t* rows, int64_t* pitch) {
+  const int64_t dims = t.dim(), cols = dims ? t.size(-1) : 0;
+  if (dims < 1 || cols == 0 || (t.stride(-1) != 1 && cols != 1)) return false;
+  *rows = 1;
+  *pitch = (cols + 15) / 16 * 16;
+  for (int64_t d = dims - 2; d >= 0; --d) {
+    const int64_t n = t.size(d);
+    if (n != 1) {
+      if (*rows == 1) *pitch = t.stride(d);
+      else if (t.stride(d) != *pitch * *rows) return false;
+    }
+    *rows *= n;
+  }
+  return *rows > 0 && *pitch >= cols && *rows < (int64_t(1) << 31) && cols < (int64_t(1) << 31);
+}
+bool vector_of(const Tensor& t, int64_t n) { return t.dim() == 1 && t.size(0) == n && (t.stride(0) == 1 || n == 1); }
+
+struct Int8Out {
+  Tensor values, scales;
+};
+Int8Out int8_out(const Tensor& x) {
+  const int64_t cols = x.size(-1), pitch = (cols + 15) / 16 * 16;
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  std::vector<int64_t> shape(lead.begin(), lead.end());
+  Tensor scales = at::empty(shape, x.options().dtype(at::kFloat));
+  shape.push_back(pitch);
+  Tensor values = at::empty(shape, x.options().dtype(at::kChar));
+  return {pitch == cols ? values : values.slice(-1, 0, cols), scales};
+}
+
+using MaybeRows = std::optional<std::tuple<Tensor, Tensor, std::optional<Tensor>>>;
+
+// norm: -1 the rows as they are, 0 RMSNorm, 1 LayerNorm.
+MaybeRows rows_int8(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, int64_t norm, const std::optional<Tensor>& residual_) {
+  const Tensor weight = or_undefined(weight_), bias = or_undefined(bias_), residual = or_undefined(residual_);
+  const auto dtype = x.scalar_type();
+  int64_t rows, pitch, residual_rows, residual_pitch = 0;
+  if (!lib.rows_int8 || !x.is_cuda() || (dtype != at::kBFloat16 && dtype != at::kFloat) || torch::jit::tracer::isTracing() || !plain(x, dtype, x.device()) ||
+      !rows_apart(x, &rows, &pitch))
+    return std::nullopt;
+  const int64_t cols = x.size(-1);
+  for (const Tensor& t : {weight, bias})
+    if (t.defined() && (!plain(t, dtype, x.device()) || !vector_of(t, cols))) return std::nullopt;
+  if (residual.defined() && (!plain(residual, dtype, x.device()) || residual.sizes() != x.sizes() || !rows_apart(residual, &residual_rows, &residual_pitch)))
+    return std::nullopt;
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Int8Out out = int8_out(x);
+  std::optional<Tensor> sum;
+  if (residual.defined()) sum = at::empty(x.sizes(), x.options());
+  check(lib.rows_int8(x.const_data_ptr(), data(residual), data(weight), data(bias), sum ? sum->mutable_data_ptr() : nullptr,
+                      static_cast<int8_t*>(out.values.mutable_data_ptr()), out.scales.mutable_data_ptr<float>(), int(rows), int(cols), pitch, residual_pitch, cols,
+                      (cols + 15) / 16 * 16, float(eps), int(norm) + 1, dtype == at::kFloat, 0, context(x, 0)->status, stream_of(x)),
+        "tpb_rows_int8");
+  launched.fetch_add(1, std::memory_order_relaxed);
+  return std::make_tuple(out.values, out.scales, sum);
+}
+
+std::optional<Tensor> linear_int8(const Tensor& x, const Tensor& sx, const Tensor& w, const Tensor& sw, const std::optional<Tensor>& bias_, int64_t act,
+                                  const std::optional<Tensor>& residual_) {
+  const Tensor bias = or_undefined(bias_), residual = or_undefined(residual_);
+  int64_t tokens, ldx, features, ldw, residual_rows, ld_res = 0;
+  const auto device = x.device();
+  if (!lib.gemm_int8 || !x.is_cuda() || torch::jit::tracer::isTracing() || !plain(x, at::kChar, device) || !plain(w, at::kChar, device) ||
+      !plain(sx, at::kFloat, device) || !plain(sw, at::kFloat, device) || x.dim() < 2 || w.dim() != 2 || !rows_apart(x, &tokens, &ldx) ||
+      !rows_apart(w, &features, &ldw) || x.size(-1) != w.size(1) || !vector_of(sw, features) || sx.sizes() != x.sizes().slice(0, x.dim() - 1) ||
+      !sx.is_contiguous())
+    return std::nullopt;
+  const int64_t k = w.size(1), cols = act == 5 ? features / 2 : features;
+  auto aligned = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; };
+  if (k > 131071 || ldx % 16 || ldw % 16 || !aligned(x) || !aligned(w) || (act == 5 && (features % 32 || residual.defined()))) return std::nullopt;
+  if (bias.defined() && (!plain(bias, at::kBFloat16, device) || !vector_of(bias, features))) return std::nullopt;
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = cols;
+  if (residual.defined() && (!plain(residual, at::kBFloat16, device) || residual.sizes() != at::IntArrayRef(shape) || !rows_apart(residual, &residual_rows, &ld_res)))
+    return std::nullopt;
+  const c10::cuda::CUDAGuard guard(device);
+  Tensor out = at::empty(shape, x.options().dtype(at::kBFloat16));
+  check(lib.gemm_int8(static_cast<const int8_t*>(x.const_data_ptr()), sx.const_data_ptr<float>(), static_cast<const int8_t*>(w.const_data_ptr()),
+                      sw.const_data_ptr<float>(), out.mutable_data_ptr(), data(bias), data(residual), int(tokens), int(features), int(k), ldx, ldw, cols, ld_res,
+                      int(act), 0, context(x, 0)->status, stream_of(x)),
+        "tpb_gemm_int8");
+  launched.fetch_add(1, std::memory_order_relaxed);
+  return out;
+}
+
 template <typename F>
 void entry(F& f, const py::dict& addresses, const char* name) {
   f = reinterpret_cast<F>(addresses[name].cast<uintptr_t>());
@@ -290,6 +389,12 @@ void bind(const py::dict& addresses, py::function text, py::function reserve) {
     entry(lib.col_sum, addresses, "tpb_col_sum");
   } else {
     lib.col_sum = nullptr;
+  }
+  lib.rows_int8 = nullptr;
+  lib.gemm_int8 = nullptr;
+  if (addresses.contains("tpb_gemm_int8")) {
+    entry(lib.rows_int8, addresses, "tpb_rows_int8");
+    entry(lib.gemm_int8, addresses, "tpb_gemm_int8");
   }
   Py_XDECREF(error_text);
   Py_XDECREF(reserve_slots);
@@ -308,4 +413,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear, unlocked);
   m.def("linears", &linears, unlocked);
   m.def("norm", &norm, unlocked);
+  m.def("rows_int8", &rows_int8, unlocked);
+  m.def("linear_int8", &linear_int8, unlocked);
 }

@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "attention_sm100.cuh"
 #include "launch.cuh"
 #include "ptx_sm100.cuh"
 #include "tpb_api.h"
@@ -32,6 +33,7 @@ struct RiParams {
   long long ldx, ldr, lds, ldq;  // row pitches in elements
   int rows, cols;
   float eps;
+  uint32_t* status;
 };
 
 __device__ __forceinline__ float ri_float(bf16 x) { return __bfloat162float(x); }
@@ -40,7 +42,42 @@ template <typename T> __device__ __forceinline__ T ri_round(float x);
 template <> __device__ __forceinline__ bf16 ri_round<bf16>(float x) { return __float2bfloat16(x); }
 template <> __device__ __forceinline__ float ri_round<float>(float x) { return x; }
 
-template <typename T> struct __align__(16) Ri8 { T e[8]; };  // 8 elements of a thread
+// 8 elements of a thread as they lie in memory (in words: one instruction takes an element out of its word).
+template <typename T> struct Ri8 {};
+template <> struct Ri8<bf16> {
+  static constexpr int WORDS = 4;
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int j) const { return __uint_as_float(j & 1 ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16); }
+  __device__ __forceinline__ void set2(int j, float a, float b) { w[j >> 1] = pack_bf16x2(a, b); }
+  __device__ __forceinline__ bf16 element(int j) const { return __ushort_as_bfloat16(uint16_t(w[j >> 1] >> (16 * (j & 1)))); }
+  __device__ __forceinline__ void pair(int j, bf16 a, bf16 b) { w[j >> 1] = uint32_t(__bfloat16_as_ushort(a)) | uint32_t(__bfloat16_as_ushort(b)) << 16; }
+};
+template <> struct Ri8<float> {
+  static constexpr int WORDS = 8;
+  uint32_t w[8];
+  __device__ __forceinline__ float get(int j) const { return __uint_as_float(w[j]); }
+  __device__ __forceinline__ void set2(int j, float a, float b) { w[j] = __float_as_uint(a); w[j + 1] = __float_as_uint(b); }
+  __device__ __forceinline__ float element(int j) const { return __uint_as_float(w[j]); }
+  __device__ __forceinline__ void pair(int j, float a, float b) { set2(j, a, b); }
+};
+template <typename T>
+__device__ __forceinline__ Ri8<T> ri_load8(const T* at, bool ok) {  // 16-byte aligned
+  Ri8<T> r;
+#pragma unroll
+  for (int u = 0; u < Ri8<T>::WORDS / 4; ++u) {
+    const uint4 q = ok ? reinterpret_cast<const uint4*>(at)[u] : make_uint4(0, 0, 0, 0);
+    r.w[4 * u] = q.x;
+    r.w[4 * u + 1] = q.y;
+    r.w[4 * u + 2] = q.z;
+    r.w[4 * u + 3] = q.w;
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void ri_store8(T* at, const Ri8<T>& r) {
+#pragma unroll
+  for (int u = 0; u < Ri8<T>::WORDS / 4; ++u) reinterpret_cast<uint4*>(at)[u] = make_uint4(r.w[4 * u], r.w[4 * u + 1], r.w[4 * u + 2], r.w[4 * u + 3]);
+}
 
 // Columns of a thread: V groups of 8.  VEC: 8 consecutive columns each, rows on 16-byte boundaries; else the lanes of a warp own consecutive
 // columns, so that rows of any width and alignment are read and written in whole sectors.
@@ -50,34 +87,29 @@ __device__ __forceinline__ int ri_col(int base, int i, int j) {
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ Ri8<T> ri_load(const T* row, int base, int i, int cols) {
-  Ri8<T> r;
   if constexpr (VEC) {
     const int c = ri_col<true>(base, i, 0);
-#pragma unroll
-    for (int u = 0; u < int(sizeof(T) / 2); ++u)
-      reinterpret_cast<uint4*>(&r)[u] = c < cols ? reinterpret_cast<const uint4*>(row + c)[u] : make_uint4(0, 0, 0, 0);
+    return ri_load8(row + c, c < cols);
   } else {
+    Ri8<T> r;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = ri_col<false>(base, i, j);
-      r.e[j] = c < cols ? row[c] : ri_round<T>(0.f);
+    for (int j = 0; j < 8; j += 2) {
+      const int c = ri_col<false>(base, i, j), d = ri_col<false>(base, i, j + 1);
+      r.pair(j, c < cols ? row[c] : ri_round<T>(0.f), d < cols ? row[d] : ri_round<T>(0.f));
     }
+    return r;
   }
-  return r;
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void ri_store(T* row, int base, int i, int cols, const Ri8<T>& r) {
   if constexpr (VEC) {
     const int c = ri_col<true>(base, i, 0);
-    if (c < cols) {
-#pragma unroll
-      for (int u = 0; u < int(sizeof(T) / 2); ++u) reinterpret_cast<uint4*>(row + c)[u] = reinterpret_cast<const uint4*>(&r)[u];
-    }
+    if (c < cols) ri_store8(row + c, r);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int c = ri_col<false>(base, i, j);
-      if (c < cols) row[c] = r.e[j];
+      if (c < cols) row[c] = r.element(j);
     }
   }
 }
@@ -108,10 +140,27 @@ __device__ __forceinline__ void ri_reduce(float& a, uint32_t& b, float* sums, ui
   if (MAX) b = __reduce_max_sync(0xffffffffu, lane < warps ? maxima[lane] : 0u);
 }
 
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// An integer in [-127, 127] stands in the low bits of x + 1.5 2^23, in two's complement, where that sum is rounded to nearest (ties to even).  The four integers
+// of v * inv.  `one` is 1, which the compiler does not know: y * one + 1.5 2^23 rounds like the sum, which it would contract with the product in front of it.
+constexpr float RI_MAGIC = 12582912.f;
+__device__ __forceinline__ uint32_t ri_integers(float2 v0, float2 v1, float inv, float one) {
+  const float2 a = __ffma2_rn(__fmul2_rn(v0, both(inv)), both(one), both(RI_MAGIC));
+  const float2 b = __ffma2_rn(__fmul2_rn(v1, both(inv)), both(one), both(RI_MAGIC));
+  return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+}
+
+// Blocks that an SM is to hold.
+template <int MODE, int V, bool VEC>
+constexpr int ri_blocks(int threads) {
+  return threads == 256 && VEC && MODE != RI_LAYER ? (V == 1 || MODE == RI_ROWS ? 8 : 6) : 1;
+}
+
 // A block of blockDim.y rows, blockDim.x threads each.  WIDE: rows of more than 8 V blockDim.x columns, read again from memory for every pass.
-template <typename T, int MODE, int V, bool VEC, bool WIDE>
-__global__ void __launch_bounds__(RI_MAX_THREADS)
-rows_int8_kernel(const RiParams p) {
+template <typename T, int MODE, int V, bool VEC, bool WIDE, int THREADS>
+__global__ void __launch_bounds__(THREADS, ri_blocks<MODE, V, VEC>(THREADS))
+rows_int8_kernel(const RiParams p, float one) {
   __shared__ float sums[32];
   __shared__ uint32_t maxima[32];
   const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
@@ -123,176 +172,441 @@ rows_int8_kernel(const RiParams p) {
   const T* weight = static_cast<const T*>(p.weight);
   const T* bias = static_cast<const T*>(p.bias);
 
-  Ri8<T> h[V];
-  auto fetch = [&](int base) {
+  Ri8<T> w[V];
+  float2 v[V][4];  // the row: h, then the values to be rounded
+  auto fetch = [&](int base, bool again) {
+    Ri8<T> raw[V];
+    // (x may be overwritten by the sum: a second pass reads what this thread stored)
+    const bool summed = again && residual && sum_out;
 #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = ri_load<T, VEC>(x, base, i, cols);
-    if (MODE != RI_ROWS && residual) {
+    for (int i = 0; i < V; ++i) raw[i] = ri_load<T, VEC>(summed ? sum_out : x, base, i, cols);
+    if (MODE != RI_ROWS && residual && !summed) {
+      Ri8<T> add[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) add[i] = ri_load<T, VEC>(residual, base, i, cols);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const Ri8<T> r = ri_load<T, VEC>(residual, base, i, cols);
         // rounded to the type it is stored in: the norm is taken of what later kernels read
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[i].e[j] = ri_round<T>(ri_float(h[i].e[j]) + ri_float(r.e[j]));
-        if (sum_out) ri_store<T, VEC>(sum_out, base, i, cols, h[i]);
+        for (int j = 0; j < 8; j += 2) raw[i].set2(j, raw[i].get(j) + add[i].get(j), raw[i].get(j + 1) + add[i].get(j + 1));
+        if (sum_out) ri_store<T, VEC>(sum_out, base, i, cols, raw[i]);
       }
     }
-  };
-  auto fetch_again = [&](int base) {
-    if (!WIDE) return;  // (still in registers)
-    if (MODE != RI_ROWS && residual && sum_out) {  // (x may have been overwritten by the sum: what this thread stored)
+    if (MODE != RI_ROWS && weight) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) h[i] = ri_load<T, VEC>(sum_out, base, i, cols);
-    } else {
-      fetch(base);
+      for (int i = 0; i < V; ++i) w[i] = ri_load<T, VEC>(weight, base, i, cols);
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = make_float2(raw[i].get(2 * j), raw[i].get(2 * j + 1));
   };
   const int end = WIDE ? cols : 1;
 
-  float mean = 0.f, rstd = 0.f, sum = 0.f;
-  uint32_t most = 0;
-  auto values = [&](int base, int i, float (&v)[8]) {
+  // v times the weight (and plus the bias, of a LayerNorm's (h - mean) rstd), and the largest |v|
+  float most0 = 0.f, most1 = 0.f;
+  auto finish_values = [&](int base, float mean, float rstd) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = ri_float(h[i].e[j]);
-    if (MODE == RI_RMS && weight) {
-      const Ri8<T> w = ri_load<T, VEC>(weight, base, i, cols);
+    for (int i = 0; i < V; ++i) {
+      if (MODE == RI_LAYER) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], ri_float(w.e[j]));
-    }
-    if (MODE == RI_LAYER) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean) * rstd;
-      if (weight) {
-        const Ri8<T> w = ri_load<T, VEC>(weight, base, i, cols);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= ri_float(w.e[j]);
+        for (int j = 0; j < 4; ++j) v[i][j] = __fmul2_rn(__fadd2_rn(v[i][j], both(-mean)), both(rstd));
       }
-      if (bias) {
-        const Ri8<T> b = ri_load<T, VEC>(bias, base, i, cols);
+      if (MODE != RI_ROWS && weight) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += ri_float(b.e[j]);
+        for (int j = 0; j < 4; ++j) v[i][j] = __fmul2_rn(v[i][j], make_float2(w[i].get(2 * j), w[i].get(2 * j + 1)));
+      }
+      if (MODE == RI_LAYER) {
+        if (bias) {
+          const Ri8<T> b = ri_load<T, VEC>(bias, base, i, cols);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[i][j] = __fadd2_rn(v[i][j], make_float2(b.get(2 * j), b.get(2 * j + 1)));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (ri_col<VEC>(base, i, 2 * j) >= cols) v[i][j].x = 0.f;
+          if (ri_col<VEC>(base, i, 2 * j + 1) >= cols) v[i][j].y = 0.f;
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (ri_col<VEC>(base, i, j) >= cols) v[j] = 0.f;
+      for (int j = 0; j < 4; j += 2) {
+        most0 = fmax3_abs_nan(most0, v[i][j].x, v[i][j].y);
+        most1 = fmax3_abs_nan(most1, v[i][j + 1].x, v[i][j + 1].y);
+      }
     }
-  };
-  auto raise = [&](const float (&v)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(fabsf(v[j])));
   };
 
   pdl_wait();
   pdl_trigger();
+  float sum = 0.f, rstd = 1.f, mean = 0.f;
   for (int base = 0; base < end; base += chunk) {
-    fetch(base);
+    fetch(base, false);
+    if (MODE == RI_RMS) {
+      float2 squares = both(0.f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (MODE == RI_RMS) {
+      for (int i = 0; i < V; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { const float f = ri_float(h[i].e[j]); sum += f * f; }
-      }
-      if (MODE == RI_LAYER) {
+        for (int j = 0; j < 4; ++j) squares = __ffma2_rn(v[i][j], v[i][j], squares);
+      sum += squares.x + squares.y;
+    }
+    if (MODE == RI_LAYER) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += ri_float(h[i].e[j]);
-      } else {
-        float v[8];
-        values(base, i, v);
-        raise(v);
-      }
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += v[i][j].x + v[i][j].y;
+    } else {
+      finish_values(base, 0.f, 1.f);
     }
   }
-  if (MODE == RI_ROWS) {
-    ri_reduce<false, true>(sum, most, sums, maxima);
-  } else if (MODE == RI_RMS) {
-    ri_reduce<true, true>(sum, most, sums, maxima);
-    rstd = rsqrtf(sum / float(p.cols) + p.eps);
-  } else {
+  uint32_t most = 0;
+  if (MODE == RI_LAYER) {
     // (the deviations are summed up around the mean: a difference of two sums would lose the digits that they share)
     ri_reduce<true, false>(sum, most, sums, maxima);
     mean = sum / float(p.cols);
     float squares = 0.f;
     for (int base = 0; base < end; base += chunk) {
-      fetch_again(base);
+      if (WIDE) fetch(base, true);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float d = ri_float(h[i].e[j]) - mean;
-          if (ri_col<VEC>(base, i, j) < cols) squares += d * d;
+        for (int j = 0; j < 4; ++j) {
+          const float a = v[i][j].x - mean, b = v[i][j].y - mean;
+          if (ri_col<VEC>(base, i, 2 * j) < cols) squares += a * a;
+          if (ri_col<VEC>(base, i, 2 * j + 1) < cols) squares += b * b;
         }
       }
     }
     ri_reduce<true, false>(squares, most, sums, maxima);
     rstd = rsqrtf(squares / float(p.cols) + p.eps);
     for (int base = 0; base < end; base += chunk) {
-      fetch_again(base);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float v[8];
-        values(base, i, v);
-        raise(v);
-      }
+      if (WIDE) fetch(base, true);
+      finish_values(base, mean, rstd);
     }
-    ri_reduce<false, true>(sum, most, sums, maxima);
   }
+  most = __float_as_uint(fmax3_abs_nan(most0, most1, 0.f));
+  ri_reduce<MODE == RI_RMS, true>(sum, most, sums, maxima);
 
   const bool finite = most < 0x7F800000u;
   const float amax = fmaxf(__uint_as_float(most), RI_LEAST);
   const float inv = __fdiv_rn(127.f, amax);
-  if (threadIdx.x == 0 && row < p.rows) p.scales[row] = finite ? amax / 127.f * (MODE == RI_RMS ? rstd : 1.f) : __int_as_float(0x7FC00000);
+  if (threadIdx.x == 0 && row < p.rows) {
+    const float scale = amax / 127.f * (MODE == RI_RMS ? rsqrtf(sum / float(p.cols) + p.eps) : 1.f);
+    p.scales[row] = finite ? scale : __int_as_float(0x7FC00000);
+  }
   int8_t* q = p.q + row * p.ldq;
   for (int base = 0; base < end; base += chunk) {
-    fetch_again(base);
+    if (WIDE) {
+      fetch(base, true);
+      finish_values(base, mean, rstd);
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      float v[8];
-      values(base, i, v);
-      uint32_t b[8];
-      // v inv is rounded to fp32, then, by the addition of 1.5 2^23, to the nearest integer (ties to even), whose two's complement the low bits are
-#pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = finite ? __float_as_uint(__fadd_rn(__fmul_rn(v[j], inv), 12582912.f)) : 0u;
+      uint2 u = make_uint2(ri_integers(v[i][0], v[i][1], inv, one), ri_integers(v[i][2], v[i][3], inv, one));
+      if (!finite) u = make_uint2(0, 0);
       if constexpr (VEC) {
         const int c = ri_col<true>(base, i, 0);
-        if (c < cols) {
-          uint2 w;
-          w.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-          w.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
-          *reinterpret_cast<uint2*>(q + c) = w;
-        }
+        if (c < cols) *reinterpret_cast<uint2*>(q + c) = u;
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int c = ri_col<false>(base, i, j);
-          if (c < cols) q[c] = int8_t(b[j] & 0xFFu);
+          if (c < cols) q[c] = int8_t((j < 4 ? u.x : u.y) >> (8 * (j & 3)));
         }
       }
     }
   }
 }
 
+// ---- many rows: persistent groups of threads, rows arriving by bulk copies several ahead -------------------------------------------------------
+
+__device__ __forceinline__ void ri_bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+// The whole 16-byte blocks that hold `cols` elements at `row` (at most 15 bytes more on either side, in the same blocks as the row's own): first
+// byte, and how far behind it the row begins.
+template <typename T>
+__device__ __forceinline__ uint32_t ri_span(const T* row, int cols, const void** first, uint32_t* bytes) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row), begin = at & ~uintptr_t(15);
+  *first = reinterpret_cast<const void*>(begin);
+  *bytes = uint32_t(((at + size_t(cols) * sizeof(T) + 15) & ~uintptr_t(15)) - begin);
+  return uint32_t(at - begin) / uint32_t(sizeof(T));
+}
+
+constexpr int RI_RING_BARS = 64;                 // slots of all groups
+constexpr size_t RI_RING_BYTES = 222 * 1024;     // dynamic shared memory of the one block of an SM
+
+// A quad: 4 consecutive columns.  Its integers are a word, its fp32 weights 16 bytes; neighbouring threads have neighbouring quads.
+template <typename T> struct Ri4 {};
+template <> struct Ri4<bf16> {
+  uint2 w;
+  __device__ __forceinline__ float2 low() const { return make_float2(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u)); }
+  __device__ __forceinline__ float2 high() const { return make_float2(__uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u)); }
+  __device__ __forceinline__ void set(float2 a, float2 b) { w = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(b.x, b.y)); }
+};
+template <> struct Ri4<float> {
+  float4 w;
+  __device__ __forceinline__ float2 low() const { return make_float2(w.x, w.y); }
+  __device__ __forceinline__ float2 high() const { return make_float2(w.z, w.w); }
+  __device__ __forceinline__ void set(float2 a, float2 b) { w = make_float4(a.x, a.y, b.x, b.y); }
+};
+// blockDim.y groups of blockDim.x threads; a group walks rows and has a ring of `stages` slots (x, and the residual behind it) of its own, which one thread
+// fills by bulk copies.  A row is read from its slot once for its statistics and once for its integers, so that registers limit neither its width nor the
+// rows in flight.  What bounds the kernel beside the bytes is instructions, a third of which are a row's and not an element's: few threads per row (one warp,
+// without barriers, where the slots of a block suffice for a dozen), fp32 arithmetic on two values at a time, weights as fp32 in shared memory.
+// ODD: rows that begin or end within a quad are read and written element by element.  `one` is 1: y * one + 1.5 2^23 rounds like a sum, which the compiler
+// would contract with the product in front of it.
+template <typename T, int MODE, bool ODD>
+__global__ void __launch_bounds__(RI_MAX_THREADS, 1)
+rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
+  extern __shared__ __align__(128) uint8_t ri_smem[];
+  __shared__ uint64_t full_bars[RI_RING_BARS];
+  __shared__ float sums[3][32];
+  __shared__ uint32_t maxima[32];
+  __shared__ uint32_t abort_word;
+  volatile uint32_t* abort_flag = &abort_word;
+  const int group = threadIdx.y, groups = blockDim.y, tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+  const int quads = (p.cols + 3) / 4;
+  uint64_t* full = full_bars + group * stages;
+  const bool two = MODE != RI_ROWS && p.residual;
+  const int stage_bytes = slot_bytes * (two ? 2 : 1);
+  float* weights = reinterpret_cast<float*>(ri_smem);
+  float* biases = weights + 4 * quads;
+  uint8_t* ring = ri_smem + size_t(MODE == RI_ROWS ? 0 : MODE == RI_RMS ? 16 : 32) * quads + size_t(group) * stages * stage_bytes;
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    if (group == 0) *abort_flag = 0;
+    fence_mbar_init();
+  }
+  pdl_wait();
+  pdl_trigger();
+  const long long step = (long long)gridDim.x * groups;
+  auto load = [&](long long row, int s) {
+    const uint32_t dst = smem_u32(ring + s * stage_bytes);
+    const void *from, *from2 = nullptr;
+    uint32_t bytes, bytes2 = 0;
+    ri_span(static_cast<const T*>(p.x) + row * p.ldx, p.cols, &from, &bytes);
+    if (two) ri_span(static_cast<const T*>(p.residual) + row * p.ldr, p.cols, &from2, &bytes2);
+    mbar_expect_tx(&full[s], bytes + bytes2);
+    ri_bulk_load(dst, from, bytes, &full[s]);
+    if (two) ri_bulk_load(dst + slot_bytes, from2, bytes2, &full[s]);
+  };
+  auto meet = [&]() {
+    if (warps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+  };
+  auto total = [&](float a, int which) {  // over the group
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if (warps == 1) return a;
+    float* at = sums[which] + group * warps;
+    if (lane == 0) at[warp] = a;
+    meet();
+    a = lane < warps ? at[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    return a;
+  };
+  // f(quad) for the thread's quads, four at a time
+  auto each = [&](auto f) {
+    int q = tid;
+    for (; q + 3 * threads < quads; q += 4 * threads) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f(q + k * threads);
+    }
+    for (; q < quads; q += threads) f(q);
+  };
+
+  long long row = (long long)blockIdx.x * groups + group;
+  long long issued = 0;
+  if (tid == 0)
+    for (; issued < stages && row + issued * step < p.rows; ++issued) load(row + issued * step, int(issued));
+  if (MODE != RI_ROWS) {
+    const T* weight = static_cast<const T*>(p.weight);
+    const T* bias = static_cast<const T*>(p.bias);
+    for (int c = group * threads + tid; c < 4 * quads; c += groups * threads) {
+      weights[c] = c >= p.cols ? 0.f : weight ? ri_float(weight[c]) : 1.f;
+      if (MODE == RI_LAYER) biases[c] = c < p.cols && bias ? ri_float(bias[c]) : 0.f;
+    }
+  }
+  __syncthreads();
+  int s = 0;
+  uint32_t parity = 0;
+  for (; row < p.rows; row += step) {
+    if (!*abort_flag && !mbar_wait(&full[s], parity)) {  // (the row's results are not valid then; the group stays together)
+      atomicMax(p.status, STATUS_TIMEOUT_MBAR);
+      *abort_flag = 1;
+    }
+    uint8_t* slot = ring + s * stage_bytes;
+    const void* unused;
+    uint32_t n;
+    T* xs = reinterpret_cast<T*>(slot) + ri_span(static_cast<const T*>(p.x) + row * p.ldx, p.cols, &unused, &n);
+    const T* rs = two ? reinterpret_cast<const T*>(slot + slot_bytes) + ri_span(static_cast<const T*>(p.residual) + row * p.ldr, p.cols, &unused, &n) : nullptr;
+    T* sum_out = two && p.sum_out ? static_cast<T*>(p.sum_out) + row * p.lds : nullptr;
+    struct Quad { float2 a, b; };
+    auto element = [&](int c) { return c < p.cols ? ri_float(xs[c]) : 0.f; };
+    auto get = [&](int q) -> Quad {
+      if constexpr (ODD) return {make_float2(element(4 * q), element(4 * q + 1)), make_float2(element(4 * q + 2), element(4 * q + 3))};
+      const Ri4<T> x = *reinterpret_cast<const Ri4<T>*>(xs + 4 * q);
+      return {x.low(), x.high()};
+    };
+    auto get_sum = [&](int q) -> Quad {  // h, which takes the place of x
+      if constexpr (ODD) {
+#pragma unroll
+        for (int c = 4 * q; c < 4 * q + 4; ++c) {
+          if (c >= p.cols) break;
+          const T h = ri_round<T>(ri_float(xs[c]) + ri_float(rs[c]));
+          xs[c] = h;
+          if (sum_out) sum_out[c] = h;
+        }
+        return get(q);
+      }
+      Ri4<T> x = *reinterpret_cast<const Ri4<T>*>(xs + 4 * q);
+      const Ri4<T> r = *reinterpret_cast<const Ri4<T>*>(rs + 4 * q);
+      // rounded to the type it is stored in: the norm is taken of what later kernels read
+      x.set(__fadd2_rn(x.low(), r.low()), __fadd2_rn(x.high(), r.high()));
+      *reinterpret_cast<Ri4<T>*>(xs + 4 * q) = x;
+      if (sum_out) *reinterpret_cast<Ri4<T>*>(sum_out + 4 * q) = x;
+      return {x.low(), x.high()};
+    };
+    float mean = 0.f, rstd = 1.f;
+    auto value = [&](int q, Quad h) -> Quad {  // what is rounded
+      if (MODE == RI_LAYER) {
+        h.a = __fmul2_rn(__fadd2_rn(h.a, both(-mean)), both(rstd));
+        h.b = __fmul2_rn(__fadd2_rn(h.b, both(-mean)), both(rstd));
+      }
+      if (MODE != RI_ROWS) {
+        const float4 w = *reinterpret_cast<const float4*>(weights + 4 * q);
+        h.a = __fmul2_rn(h.a, make_float2(w.x, w.y));
+        h.b = __fmul2_rn(h.b, make_float2(w.z, w.w));
+      }
+      if (MODE == RI_LAYER) {
+        const float4 b = *reinterpret_cast<const float4*>(biases + 4 * q);
+        h.a = __fadd2_rn(h.a, make_float2(b.x, b.y));
+        h.b = __fadd2_rn(h.b, make_float2(b.z, b.w));
+      }
+      return h;
+    };
+    float most0 = 0.f, most1 = 0.f;
+    float2 squares = both(0.f);
+    auto raise = [&](const Quad& v) {
+      most0 = fmax3_abs_nan(most0, v.a.x, v.a.y);
+      most1 = fmax3_abs_nan(most1, v.b.x, v.b.y);
+    };
+    auto statistics = [&](int q, const Quad& h) {
+      if (MODE == RI_RMS) squares = __ffma2_rn(h.b, h.b, __ffma2_rn(h.a, h.a, squares));
+      if (MODE == RI_LAYER) squares = __fadd2_rn(squares, __fadd2_rn(h.a, h.b));
+      else raise(value(q, h));
+    };
+    if (two) each([&](int q) { statistics(q, get_sum(q)); });
+    else each([&](int q) { statistics(q, get(q)); });
+    float sum = squares.x + squares.y;
+    if (MODE == RI_LAYER) {
+      // (the deviations are summed up around the mean: a difference of two sums would lose the digits that they share)
+      mean = total(sum, 0) / float(p.cols);
+      squares = both(0.f);
+      each([&](int q) {
+        Quad h = get(q);
+        h.a = __fadd2_rn(h.a, both(-mean));
+        h.b = __fadd2_rn(h.b, both(-mean));
+        if (ODD) {
+          if (4 * q + 1 >= p.cols) h.a.y = 0.f;
+          if (4 * q + 2 >= p.cols) h.b.x = 0.f;
+          if (4 * q + 3 >= p.cols) h.b.y = 0.f;
+        }
+        squares = __ffma2_rn(h.b, h.b, __ffma2_rn(h.a, h.a, squares));
+      });
+      rstd = rsqrtf(total(squares.x + squares.y, 1) / float(p.cols) + p.eps);
+      each([&](int q) { raise(value(q, get(q))); });  // (past the end the weight and the bias are zero)
+    }
+    uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(fmax3_abs_nan(most0, most1, 0.f)));
+    if (warps > 1 && lane == 0) maxima[group * warps + warp] = most;
+    if (MODE == RI_RMS) sum = total(sum, 2);
+    else meet();
+    if (warps > 1) most = __reduce_max_sync(0xffffffffu, lane < warps ? maxima[group * warps + lane] : 0u);
+    const bool finite = most < 0x7F800000u;
+    const float amax = fmaxf(__uint_as_float(most), RI_LEAST);
+    const float inv = __fdiv_rn(127.f, amax);
+    if (tid == 0) {
+      const float scale = amax / 127.f * (MODE == RI_RMS ? rsqrtf(sum / float(p.cols) + p.eps) : 1.f);
+      p.scales[row] = finite ? scale : __int_as_float(0x7FC00000);
+    }
+    int8_t* out = p.q + row * p.ldq;
+    each([&](int q) {
+      const Quad v = value(q, get(q));
+      uint32_t four = ri_integers(v.a, v.b, inv, one);
+      if (!finite) four = 0;
+      if (!ODD || 4 * q + 4 <= p.cols) {
+        *reinterpret_cast<uint32_t*>(out + 4 * q) = four;
+      } else {
+        for (int c = 4 * q; c < p.cols; ++c, four >>= 8) out[c] = int8_t(four & 0xFFu);
+      }
+    });
+    if (two) fence_proxy_async_smem();  // (h was written to the slot that a bulk copy fills next)
+    meet();
+    if (tid == 0 && row + stages * step < p.rows && !*abort_flag) {
+      load(row + stages * step, s);
+      ++issued;
+    }
+    if (++s == stages) { s = 0; parity ^= 1; }
+  }
+  if (tid == 0 && *abort_flag) {  // copies that are still on their way arrive before the block's memory goes
+    for (int i = 0; i < stages && i < issued; ++i) mbar_wait(&full[(issued - 1 - i) % stages], uint32_t((issued - 1 - i) / stages) & 1);
+  }
+}
+
+// True if the ring kernel was launched (or its launch failed: *e): there are rows for several turns of its groups, and room for two of them.
+template <typename T, int MODE>
+static bool ri_ring_launch(const RiParams& p, int sms, bool early, cudaStream_t stream, cudaError_t* e) {
+  const size_t slot = (size_t(p.cols) * sizeof(T) + 15) / 16 * 16 + 16;  // (a row may begin in the middle of 16 bytes)
+  const size_t stage = slot * (p.residual ? 2 : 1);
+  const size_t params = size_t(MODE == RI_ROWS ? 0 : MODE == RI_RMS ? 1 : 2) * size_t((p.cols + 3) / 4) * 16;
+  if (params + 2 * stage > RI_RING_BYTES || p.rows < 2 * sms) return false;
+  size_t slots = (RI_RING_BYTES - params) / stage;
+  if (slots > RI_RING_BARS) slots = RI_RING_BARS;
+  int groups = int(slots / 2);
+  if (groups < 1) groups = 1;
+  if (groups > (p.rows + sms - 1) / sms) groups = (p.rows + sms - 1) / sms;
+  int warps = 1;
+  while (warps < 8 && warps * groups < 16) warps *= 2;
+  if (groups * warps > 32) groups = 32 / warps;
+  if (warps > 1 && groups > 15) groups = 15;  // (named barriers)
+  int stages = int(slots / groups);
+  if (stages > 4) stages = 4;
+  auto whole = [](const void* base, long long ld) { return reinterpret_cast<uintptr_t>(base) % (4 * sizeof(T)) == 0 && ld % 4 == 0; };
+  const bool odd = p.cols % 4 || !whole(p.x, p.ldx) || !whole(p.residual, p.ldr) || !whole(p.sum_out, p.lds) || (reinterpret_cast<uintptr_t>(p.q) & 3) || p.ldq % 4;
+  auto go = [&](auto kernel) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(RI_RING_BYTES));
+    return err != cudaSuccess ? err
+                              : launch_dependent(kernel, dim3(sms), dim3(32 * warps, groups), params + groups * stages * stage, stream, early, p, stages, int(slot), 1.f);
+  };
+  *e = odd ? go(rows_int8_ring_kernel<T, MODE, true>) : go(rows_int8_ring_kernel<T, MODE, false>);
+  return true;
+}
+
 template <typename T, int MODE, bool VEC>
-static cudaError_t ri_launch(const RiParams& p, bool early, cudaStream_t stream) {
+static cudaError_t ri_launch(const RiParams& p, int sms, bool early, cudaStream_t stream) {
+  cudaError_t e;
+  if (!(VEC && p.cols <= (p.residual ? 8192 : 4096)) && ri_ring_launch<T, MODE>(p, sms, early, stream, &e)) return e;
   const int groups = (p.cols + 7) / 8;
-  const int v = groups <= 256 ? 1 : groups <= 2048 ? 2 : 4;
+  const int v = groups <= 32 ? 1 : 2;
   int threads = ((groups + v - 1) / v + 31) / 32 * 32;
   const bool wide = threads > RI_MAX_THREADS;
   if (wide) threads = RI_MAX_THREADS;
   const int rows_per_block = threads >= 256 ? 1 : 256 / threads;
   const dim3 block(threads, rows_per_block), grid((unsigned(p.rows) + rows_per_block - 1) / rows_per_block);
-  auto go = [&](auto kernel) { return launch_dependent(kernel, grid, block, 0, stream, early, p); };
-  if (wide) return go(rows_int8_kernel<T, MODE, 4, VEC, true>);
-  if (v == 1) return go(rows_int8_kernel<T, MODE, 1, VEC, false>);
-  if (v == 2) return go(rows_int8_kernel<T, MODE, 2, VEC, false>);
-  return go(rows_int8_kernel<T, MODE, 4, VEC, false>);
+  auto go = [&](auto kernel) { return launch_dependent(kernel, grid, block, 0, stream, early, p, 1.f); };
+  if (wide) return go(rows_int8_kernel<T, MODE, 2, VEC, true, 1024>);
+  if (v == 1) return go(rows_int8_kernel<T, MODE, 1, VEC, false, 256>);
+  return threads <= 256 ? go(rows_int8_kernel<T, MODE, 2, VEC, false, 256>) : go(rows_int8_kernel<T, MODE, 2, VEC, false, 1024>);
 }
 
 template <typename T>
-static cudaError_t ri_dispatch(const RiParams& p, int mode, bool early, cudaStream_t stream) {
+static cudaError_t ri_dispatch(const RiParams& p, int sms, int mode, bool early, cudaStream_t stream) {
   auto rows_aligned = [](const void* base, long long ld) { return !(reinterpret_cast<uintptr_t>(base) & 15) && (ld * sizeof(T)) % 16 == 0; };
   const bool vec = p.cols % 8 == 0 && rows_aligned(p.x, p.ldx) && rows_aligned(p.residual, p.ldr) && rows_aligned(p.sum_out, p.lds) &&
                    rows_aligned(p.weight, 0) && rows_aligned(p.bias, 0) && !(reinterpret_cast<uintptr_t>(p.q) & 7) && p.ldq % 8 == 0;
-#define RI_GO(MODE) (vec ? ri_launch<T, MODE, true>(p, early, stream) : ri_launch<T, MODE, false>(p, early, stream))
+#define RI_GO(MODE) (vec ? ri_launch<T, MODE, true>(p, sms, early, stream) : ri_launch<T, MODE, false>(p, sms, early, stream))
   return mode == RI_ROWS ? RI_GO(RI_ROWS) : mode == RI_RMS ? RI_GO(RI_RMS) : RI_GO(RI_LAYER);
 #undef RI_GO
 }
@@ -300,13 +614,15 @@ static cudaError_t ri_dispatch(const RiParams& p, int mode, bool early, cudaStre
 }  // namespace tpb
 
 extern "C" int tpb_rows_int8(const void* x, const void* residual, const void* weight, const void* bias, void* sum_out, int8_t* q, float* scales, int rows,
-                             int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, int early, void* stream) {
-  if (!x || !q || !scales || rows <= 0 || cols <= 0 || mode < 0 || mode > 2 || dtype < 0 || dtype > 1) return TPB_ERR_ARG;
+                             int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, int early, void* status, void* stream) {
+  if (!x || !q || !scales || !status || rows <= 0 || cols <= 0 || mode < 0 || mode > 2 || dtype < 0 || dtype > 1) return TPB_ERR_ARG;
   if (mode == tpb::RI_ROWS && (residual || weight || bias || sum_out)) return TPB_ERR_ARG;
   if ((bias && mode != tpb::RI_LAYER) || (sum_out && !residual)) return TPB_ERR_ARG;
   if (ldx < cols || ldq < cols || (residual && ldr < cols) || (sum_out && lds < cols)) return TPB_ERR_ARG;
-  tpb::RiParams p = {x, residual, weight, bias, sum_out, q, scales, ldx, residual ? ldr : 0, sum_out ? lds : 0, ldq, rows, cols, eps};
+  tpb::RiParams p = {x, residual, weight, bias, sum_out, q, scales, ldx, residual ? ldr : 0, sum_out ? lds : 0, ldq, rows, cols, eps, static_cast<uint32_t*>(status)};
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return TPB_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == 0 ? tpb::ri_dispatch<tpb::bf16>(p, mode, early != 0, s) : tpb::ri_dispatch<float>(p, mode, early != 0, s);
+  const cudaError_t e = dtype == 0 ? tpb::ri_dispatch<tpb::bf16>(p, sms, mode, early != 0, s) : tpb::ri_dispatch<float>(p, sms, mode, early != 0, s);
   return e == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }

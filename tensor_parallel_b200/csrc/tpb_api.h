@@ -136,7 +136,7 @@ int tpb_col_sum(const void* g, void* out, float* partials, int rows, int cols, i
 // (LayerNorm) and residual may be null; with residual, x + residual rounded to the type of x is normalised and stored to sum_out (may be null, or x).
 // early: launch as a programmatic dependent of the previous kernel of the stream.
 int tpb_rows_int8(const void* x, const void* residual, const void* weight, const void* bias, void* sum_out, int8_t* q, float* scales, int rows,
-                  int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, int early, void* stream);
+                  int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, int early, void* status, void* stream);
 
 // out[t, f] = act(sx[t] sw[f] sum_k x[t, k] w[f, k] + bias[f]) + residual[t, f]: x [tokens, k] and w [features, k] 8-bit integers (16-byte aligned, row pitches
 // multiples of 16; what lies between k and the pitch is not read), sums in 32 bits, bf16 bias, residual (may be out) and out.  act as in tpb_gemm_bf16; 5

@@ -325,24 +325,33 @@ def quantize_int8(x) -> Int8Rows:
     """The rows of ``x`` (bf16 or fp32, ``[..., cols]``) in 8 bits: ``rint(x * (127 / max |x|))`` and ``max |x| / 127``, ties to even.  For an activation
     in front of :func:`linear_int8`, and for its weight (a row per output channel).  A row with a value that is not finite gets the scale NaN.
     Serving only: there is no gradient."""
-    _check_rows("quantize_int8", x)
     nat = _native(x)
-    return nat.quantize_int8(x) if nat is not None else quantize_int8_ref(x)
+    out = None if nat is None else nat.quantize_int8_directly(x)
+    if out is not None:
+        return out
+    _check_rows("quantize_int8", x)
+    return quantize_int8_ref(x) if nat is None or torch._C._is_tracing() else nat.quantize_int8(x)
 
 
 def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
     """``(rows, h)``: ``h = x + residual``, rounded to the type of ``x`` (``x`` itself without a residual), and its RMSNorm in 8 bits, as
     :func:`quantize_int8` gives them.  ``weight`` may be None."""
-    _check_rows("rms_norm_int8", x, weight, residual=residual)
     nat = _native(x)
-    return nat.norm_int8(x, weight, None, eps, 0, residual) if nat is not None else rms_norm_int8_ref(x, weight, eps, residual)
+    out = None if nat is None else nat.norm_int8_directly(x, weight, None, eps, 0, residual)
+    if out is not None:
+        return out
+    _check_rows("rms_norm_int8", x, weight, residual=residual)
+    return rms_norm_int8_ref(x, weight, eps, residual) if nat is None or torch._C._is_tracing() else nat.norm_int8(x, weight, None, eps, 0, residual)
 
 
 def layer_norm_int8(x, weight, bias, eps: float = 1e-5, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
     """Like :func:`rms_norm_int8`, with a LayerNorm; ``weight`` and ``bias`` may be None."""
-    _check_rows("layer_norm_int8", x, weight, bias, residual)
     nat = _native(x)
-    return nat.norm_int8(x, weight, bias, eps, 1, residual) if nat is not None else layer_norm_int8_ref(x, weight, bias, eps, residual)
+    out = None if nat is None else nat.norm_int8_directly(x, weight, bias, eps, 1, residual)
+    if out is not None:
+        return out
+    _check_rows("layer_norm_int8", x, weight, bias, residual)
+    return layer_norm_int8_ref(x, weight, bias, eps, residual) if nat is None or torch._C._is_tracing() else nat.norm_int8(x, weight, bias, eps, 1, residual)
 
 
 _INT8_ACTS = (None, "relu", "gelu", "gelu_tanh", "silu", "swiglu16")
@@ -375,11 +384,14 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias=None, act: Optional[str] = N
     products are exact integers, scales, bias, activation and residual are fp32.  ``act``: None, ``"relu"``, ``"gelu"``, ``"gelu_tanh"``, ``"silu"``, or
     ``"swiglu16"`` for a weight whose rows alternate in groups of 16 gate and 16 up rows (``silu(gate) * up``, half as many columns).  Serving only:
     there is no gradient."""
-    _check_linear_int8(x, weight, bias, act, residual)
     nat = _native(x[0])
-    if nat is not None:
-        return nat.linear_int8(x, weight, bias, act, residual)
-    return linear_int8_ref(Int8Rows(*x), Int8Rows(*weight), bias, act, residual)
+    out = None if nat is None else nat.linear_int8_directly(x, weight, bias, act, residual)
+    if out is not None:
+        return out
+    _check_linear_int8(x, weight, bias, act, residual)
+    if nat is None or torch._C._is_tracing():
+        return linear_int8_ref(Int8Rows(*x), Int8Rows(*weight), bias, act, residual)
+    return nat.linear_int8(x, weight, bias, act, residual)
 
 
 def cross_entropy(logits, labels, ignore_index: int = -100):

@@ -214,7 +214,8 @@ def _reserve_slots(index: int, elems: int) -> int:
 
 
 def _bind_autograd():
-    names = ("tpb_gemm_plan_ex", "tpb_gemm_bf16_ex", "tpb_norm_fwd", "tpb_norm_bwd", "tpb_norm_bwd_parts", "tpb_col_sum_parts", "tpb_col_sum")
+    names = ("tpb_gemm_plan_ex", "tpb_gemm_bf16_ex", "tpb_norm_fwd", "tpb_norm_bwd", "tpb_norm_bwd_parts", "tpb_col_sum_parts", "tpb_col_sum",
+             "tpb_rows_int8", "tpb_gemm_int8")
     AUTOGRAD.bind({n: ctypes.cast(getattr(LIB, n), c_void_p).value for n in names if hasattr(LIB, n)}, _error_text, _reserve_slots)
 
 
@@ -964,7 +965,7 @@ def adamw_step(param, grad, exp_avg, exp_avg_sq, step, lr, beta1, beta2, eps, we
 # 8-bit integers: rows with a scale each, and their matrix product (serving)
 # ------------------------------------------------------------------------------------------------
 
-LIB.tpb_rows_int8.argtypes = [c_void_p] * 7 + [c_int] * 2 + [c_ll] * 4 + [c_float] + [c_int] * 3 + [c_void_p]
+LIB.tpb_rows_int8.argtypes = [c_void_p] * 7 + [c_int] * 2 + [c_ll] * 4 + [c_float] + [c_int] * 3 + [c_void_p] * 2
 LIB.tpb_gemm_int8.argtypes = [c_void_p] * 7 + [c_int] * 3 + [c_ll] * 4 + [c_int] * 2 + [c_void_p] * 2
 
 
@@ -986,7 +987,7 @@ def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, su
         return out
     check(LIB.tpb_rows_int8(_ptr(x2d), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(sum_out), _ptr(out[0]), _ptr(out[1]), rows, cols, _pitch(x2d),
                             _pitch(residual), _pitch(sum_out), _pitch(out[0]), eps,
-                            0 if norm is None else norm + 1, _dtype_code(x2d), int(early), _stream()), "tpb_rows_int8")
+                            0 if norm is None else norm + 1, _dtype_code(x2d), int(early), _ptr(device_state(x2d.device).status), _stream()), "tpb_rows_int8")
     _launches += 1
     return out
 
@@ -1024,6 +1025,24 @@ def norm_int8(x, weight, bias, eps, mode, residual=None):
         summed = None if residual is None else torch.empty(x2d.shape, dtype=x.dtype, device=x.device)
         rows = rows_int8(x2d, w, b, eps, mode, res, summed)
         return _int8_shaped(rows, x.shape), x if summed is None else summed.view(x.shape)
+
+
+# The calls that need neither a check's words nor a copy, by the C++ module (which leaves all others: None).
+
+
+def quantize_int8_directly(x):
+    out = None if AUTOGRAD is None else AUTOGRAD.rows_int8(x, None, None, 0.0, -1, None)
+    return None if out is None else OF.Int8Rows(out[0], out[1])
+
+
+def norm_int8_directly(x, weight, bias, eps, mode, residual):
+    out = None if AUTOGRAD is None else AUTOGRAD.rows_int8(x, weight, bias, eps, mode, residual)
+    return None if out is None else (OF.Int8Rows(out[0], out[1]), x if residual is None else out[2])
+
+
+def linear_int8_directly(x, weight, bias, act, residual):
+    code = ACT_CODES.get(act)
+    return None if AUTOGRAD is None or code is None else AUTOGRAD.linear_int8(x[0], x[1], weight[0], weight[1], bias, code, residual)
 
 
 def gemm_int8(x: OF.Int8Rows, weight: OF.Int8Rows, bias=None, act=None, residual=None, out=None, early=False):
