@@ -28,15 +28,65 @@ struct I8Gemm {
 __device__ __forceinline__ float i8_value(int sum, float sx, float sw, float bias) {
   return __fadd_rn(__fmul_rn(__int2float_rn(sum), __fmul_rn(sx, sw)), bias);
 }
-__device__ __forceinline__ float i8_silu(float x) { return x / (1.f + expf(-x)); }
-__device__ __forceinline__ float i8_act(float x, int act) {
+// x sigmoid(u).  The hardware's exponential and quotient are off by about 2^-21 (|u| 2^-24 more for large |u|), far below the rounding to bf16 that follows;
+// expf and the IEEE division made the epilogue of a 256 x 256 tile longer than its products (8192 x 22016 x 4096, gated: 732 us).
+__device__ __forceinline__ float i8_gate(float x, float u) { return __fdividef(x, 1.f + __expf(-u)); }
+// act = 1 relu, 2 gelu, 3 gelu (tanh form: 0.5 x (1 + tanh(u)) = x sigmoid(2u)), 4 silu
+template <int N>
+__device__ __forceinline__ void i8_activate(float (&v)[N], int act) {
   switch (act) {
-    case 1: return fmaxf(x, 0.f);
-    case 2: return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-    case 3: return 0.5f * x * (1.f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
-    case 4: return i8_silu(x);
-    default: return x;
+    case 1:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];  // (NaN stays)
+      break;
+    case 2:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = 0.5f * v[j] * (1.f + erff(v[j] * 0.70710678118654752f));
+      break;
+    case 3:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = i8_gate(v[j], 1.5957691216057308f * (v[j] + 0.044715f * v[j] * v[j] * v[j]));
+      break;
+    case 4:
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = i8_gate(v[j], v[j]);
+      break;
   }
+}
+
+// Tokens t0 .. t0 + N of feature m, for the kernels whose lanes are features: neighbouring lanes of a warp have neighbouring features, m_ok says whether this lane's
+// exists, sx points to the scales of the tokens, res are the residual's values.  Called by whole warps.
+template <int N>
+__device__ __forceinline__ void i8_finish(const I8Gemm& g, const int (&sum)[N], const float* sx, int t0, int m, bool m_ok, float sw, float bias, const float (&res)[N]) {
+  float v[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = i8_value(sum[j], sx[j], sw, bias);
+  int col = m;
+  if (g.act == I8_GATED) {  // lanes 0-15 hold gate rows, lanes 16-31 the matching up rows
+    col = (m >> 5) * 16 + (m & 15);
+    m_ok = m_ok && !(m & 16);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float up = __shfl_xor_sync(0xffffffffu, v[j], 16);
+      v[j] = i8_gate(v[j], v[j]) * up;
+    }
+  } else {
+    i8_activate(v, g.act);
+    if (g.residual) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] += res[j];
+    }
+  }
+  if (!m_ok) return;
+  __nv_bfloat16* out = g.out + t0 * g.ld_out + col;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (t0 + j < g.tokens) out[j * g.ld_out] = __float2bfloat16(v[j]);
+}
+template <int N>
+__device__ __forceinline__ void i8_residual(const I8Gemm& g, float (&res)[N], int t0, int m, bool m_ok) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) res[j] = g.residual && m_ok && t0 + j < g.tokens ? __bfloat162float(g.residual[(t0 + j) * g.ld_res + m]) : 0.f;
 }
 
 // [rows, k] bytes, row pitch ld; box = [box_rows][128 columns], 128-byte swizzle.  What lies past k is not read: it arrives as zeros.

@@ -4,10 +4,10 @@
 // tcgen05.mma.cta_group::2, each loads 128 token rows and BN / 2 feature rows, the leader issues for both.  A k-block is 128 bytes of every row there
 // and here: 128 columns, 512 clocks of the tensor core at BN = 256.  Sums are 32-bit integers, the epilogue scales them.
 //
-// One CTA (192 threads), persistent over the pair's tiles:
+// One CTA (320 threads), persistent over the pair's tiles:
 //   warp 0    : TMA producer of this CTA's operand rows; completion is counted on the LEADER's barrier (no multicast)
 //   warp 1    : leader only: one thread issues the MMAs; the commits signal the barriers of both CTAs
-//   warps 2-5 : epilogue of this CTA's 128 rows, two TMEM accumulators so that it runs under the next tile's MMAs
+//   warps 2-9 : epilogue of this CTA's 128 rows, two TMEM accumulators so that it runs under the next tile's MMAs
 // Every mbarrier wait is bounded; on expiry the CTA records a status code and drains.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -26,9 +26,12 @@ namespace tpb {
 
 constexpr int I8_MAX_K = 131071;  // rows of -128 that long sum up to 2^31 - 2^14
 constexpr int IP_BM = 256;        // tokens of a pair tile (128 per CTA = TMEM lanes)
-constexpr int IP_THREADS = 192;
+constexpr int IP_EPI_WARPS = 8;   // two per quarter of the TMEM lanes: one for each half of the columns
+constexpr int IP_THREADS = 64 + 32 * IP_EPI_WARPS;
 constexpr int IP_MAX_STAGES = 8;
 constexpr int IP_BAND = 8;        // tiles are walked in bands of 8 token tiles x all feature tiles
+
+constexpr int IP_TURN_PITCH = 17; // 16 columns of a chunk, turned in shared memory
 
 struct IpParams {
   I8Gemm g;
@@ -41,7 +44,9 @@ struct IpShape {
   static constexpr uint32_t A_BYTES = 128 * I8_BK;
   static constexpr uint32_t B_BYTES = BN / 2 * I8_BK;
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr size_t SMEM = size_t(STAGES) * STAGE_BYTES + 1024 /*align*/ + (2 * IP_MAX_STAGES + 4) * 8 + 16;
+  static constexpr size_t PARAM_BYTES = 2 * 2 * BN * sizeof(float);                         // scales and biases of the features of two tiles
+  static constexpr size_t TURN_BYTES = size_t(IP_EPI_WARPS) * 32 * IP_TURN_PITCH * sizeof(float);  // where rows of `out` are not aligned
+  static constexpr size_t SMEM = size_t(STAGES) * STAGE_BYTES + 1024 /*align*/ + PARAM_BYTES + TURN_BYTES + (2 * IP_MAX_STAGES + 4) * 8 + 16;
 };
 
 template <int BN>
@@ -52,7 +57,9 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   const I8Gemm& g = p.g;
   extern __shared__ uint8_t ip_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ip_smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + size_t(S::STAGES) * S::STAGE_BYTES);  // used in the leader
+  float* params = reinterpret_cast<float*>(smem + size_t(S::STAGES) * S::STAGE_BYTES);  // [2 tiles][scales, biases][BN]
+  float* turn = params + S::PARAM_BYTES / sizeof(float);                               // [epilogue warp][32 tokens][IP_TURN_PITCH]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(turn + S::TURN_BYTES / sizeof(float));  // used in the leader
   uint64_t* empty_bar = full_bar + IP_MAX_STAGES;
   uint64_t* acc_full = empty_bar + IP_MAX_STAGES;  // [2]
   uint64_t* acc_empty = acc_full + 2;              // [2], used in the leader
@@ -73,7 +80,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8);  // one arrival per epilogue warp of either CTA
+      mbar_init(&acc_empty[a], 2 * IP_EPI_WARPS);  // one arrival per epilogue warp of either CTA
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -163,64 +170,66 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     }
   } else {
     const int quarter = warp & 3;  // TMEM lane quarter this warp may access
+    const int half = (warp - 2) >> 2, col0 = half * (BN / 2);
     const int row = quarter * 32 + lane;
     const uint32_t acc_empty_leader[2] = {mapa_u32(smem_u32(&acc_empty[0]), 0), mapa_u32(smem_u32(&acc_empty[1]), 0)};
     const bool gated = g.act == I8_GATED;
     auto aligned = [](const void* ptr, long long ld) { return !(reinterpret_cast<uintptr_t>(ptr) & 15) && (ld & 7) == 0; };
-    const bool vec = aligned(g.out, g.ld_out) && aligned(g.bias, 0) && (!g.residual || aligned(g.residual, g.ld_res)) && !(reinterpret_cast<uintptr_t>(g.sw) & 15);
+    const bool vec = aligned(g.out, g.ld_out) && (!g.residual || aligned(g.residual, g.ld_res));
     const bool sectors = vec && (g.ld_out & 15) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 31);
+    float* mine = turn + (warp - 2) * 32 * IP_TURN_PITCH;
+    bool gone = false;  // given up: on to the end without waits, through the barriers that the epilogue warps share
     uint32_t local = 0;
     for (int t = pair; t < tiles; t += pairs, ++local) {
       int mt, nt;
       tile_at(t, mt, nt);
-      const int m = mt * IP_BM + int(rank) * 128 + row;
+      const int m0 = mt * IP_BM + int(rank) * 128 + quarter * 32, m = m0 + lane;
       const int acc = local & 1;
+      float* sws = params + acc * 2 * BN;
+      const float* biases = sws + BN;
+      // (every warp has read what the tile before the last left there: it has passed the last tile's barrier)
+      for (int c = int(threadIdx.x) - 64; c < 2 * BN; c += 32 * IP_EPI_WARPS) {
+        const int f = nt * BN + (c & (BN - 1));
+        sws[c] = f >= g.features ? 0.f : c < BN ? g.sw[f] : g.bias ? __bfloat162float(g.bias[f]) : 0.f;
+      }
       const float sx = m < g.tokens ? g.sx[m] : 0.f;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * IP_EPI_WARPS) : "memory");
       const bool ready = !*abort_flag && mbar_wait(&acc_full[acc], (local >> 1) & 1);
       if (!__all_sync(0xffffffffu, ready)) {
         if (lane == 0) give_up();
-        break;
+        gone = true;
       }
       tc_fence_after();
       const uint32_t t_lane = tmem_base + (uint32_t(quarter * 32) << 16) + acc * BN;
 #pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += 32) {
+      for (int c0 = col0; c0 < col0 + BN / 2; c0 += 32) {
         const int n0 = nt * BN + c0;
-        if (n0 >= g.features) break;
+        if (gone || n0 >= g.features) break;
         uint32_t r[32];
-        __syncwarp();  // (rows past the end skip the rest of a chunk)
+        __syncwarp();
         tmem_ld_x32(t_lane + c0, r);
         tmem_ld_wait();
-        if (m >= g.tokens) continue;
-        __nv_bfloat16* out = g.out + m * g.ld_out + (gated ? n0 >> 1 : n0);
-        const __nv_bfloat16* residual = g.residual ? g.residual + m * g.ld_res + n0 : nullptr;
+        float v[32];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 s = *reinterpret_cast<const float4*>(sws + c0 + 4 * q), b = *reinterpret_cast<const float4*>(biases + c0 + 4 * q);
+          v[4 * q] = i8_value(int(r[4 * q]), sx, s.x, b.x);
+          v[4 * q + 1] = i8_value(int(r[4 * q + 1]), sx, s.y, b.y);
+          v[4 * q + 2] = i8_value(int(r[4 * q + 2]), sx, s.z, b.z);
+          v[4 * q + 3] = i8_value(int(r[4 * q + 3]), sx, s.w, b.w);
+        }
+        if (gated) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = i8_gate(v[j], v[j]) * v[16 + j];
+        } else {
+          i8_activate(v, g.act);
+        }
+        const int cols = gated ? 16 : 32, at = gated ? n0 >> 1 : n0;  // output columns of the chunk
         if (vec && n0 + 32 <= g.features) {
-          float v[32];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const float4 s = __ldg(reinterpret_cast<const float4*>(g.sw + n0) + q);
-            float b[4] = {0.f, 0.f, 0.f, 0.f};
-            if (g.bias) {
-              const uint2 b2 = __ldg(reinterpret_cast<const uint2*>(g.bias + n0) + q);
-              b[0] = bf16_bits_to_float(b2.x & 0xFFFF);
-              b[1] = bf16_bits_to_float(b2.x >> 16);
-              b[2] = bf16_bits_to_float(b2.y & 0xFFFF);
-              b[3] = bf16_bits_to_float(b2.y >> 16);
-            }
-            v[4 * q] = i8_value(int(r[4 * q]), sx, s.x, b[0]);
-            v[4 * q + 1] = i8_value(int(r[4 * q + 1]), sx, s.y, b[1]);
-            v[4 * q + 2] = i8_value(int(r[4 * q + 2]), sx, s.z, b[2]);
-            v[4 * q + 3] = i8_value(int(r[4 * q + 3]), sx, s.w, b[3]);
-          }
-          if (gated) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = i8_silu(v[j]) * v[16 + j];
-          } else if (g.act) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = i8_act(v[j], g.act);
-          }
-          if (residual) {
-            const uint4* rp = reinterpret_cast<const uint4*>(residual);
+          if (m >= g.tokens) continue;
+          __nv_bfloat16* out = g.out + m * g.ld_out + at;
+          if (g.residual) {
+            const uint4* rp = reinterpret_cast<const uint4*>(g.residual + m * g.ld_res + n0);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               const uint4 r4 = rp[q];
@@ -244,28 +253,30 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
             for (int q = 0; q < 4; ++q)
               if (q < 2 || !gated) op[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
           }
-        } else if (gated) {  // (the feature count is a multiple of 32: only alignment can be missing)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float gate = i8_value(int(r[j]), sx, g.sw[n0 + j], g.bias ? __bfloat162float(g.bias[n0 + j]) : 0.f);
-            const float up = i8_value(int(r[16 + j]), sx, g.sw[n0 + 16 + j], g.bias ? __bfloat162float(g.bias[n0 + 16 + j]) : 0.f);
-            out[j] = __float2bfloat16(i8_silu(gate) * up);
-          }
         } else {
+          // 16 columns at a time through shared memory, so that neighbouring lanes store neighbouring columns
+          const int last = gated ? g.features >> 1 : g.features;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (n0 + j < g.features) {
-              float x = i8_value(int(r[j]), sx, g.sw[n0 + j], g.bias ? __bfloat162float(g.bias[n0 + j]) : 0.f);
-              if (g.act) x = i8_act(x, g.act);
-              if (residual) x += __bfloat162float(residual[j]);
-              out[j] = __float2bfloat16(x);
+          for (int h = 0; h < 2; ++h) {
+            if (16 * h >= cols) break;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mine[lane * IP_TURN_PITCH + j] = v[16 * h + j];
+            __syncwarp();
+            const int c = at + 16 * h + (lane & 15);
+#pragma unroll 4
+            for (int i = lane >> 4; i < 32; i += 2) {
+              if (m0 + i >= g.tokens || c >= last) continue;
+              float x = mine[i * IP_TURN_PITCH + (lane & 15)];
+              if (g.residual) x += __bfloat162float(g.residual[(m0 + i) * g.ld_res + c]);
+              g.out[(m0 + i) * g.ld_out + c] = __float2bfloat16(x);
             }
           }
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(acc_empty_leader[acc]);  // both accumulator halves may be overwritten after 8 of these
+      if (lane == 0) mbar_arrive_cluster(acc_empty_leader[acc]);  // both accumulator halves may be overwritten after all of these
     }
   }
 

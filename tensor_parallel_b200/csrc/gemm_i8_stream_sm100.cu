@@ -38,9 +38,6 @@ struct IsParams {
   int stages;
 };
 
-// (out of line: the epilogue runs once or twice per CTA, from a cold instruction cache)
-__device__ __noinline__ float is_act(float x, int act) { return i8_act(x, act); }
-
 // NACC accumulators per pass: consecutive MMAs into the same TMEM columns serialise, so k-steps are dealt round-robin and the epilogue adds the
 // accumulators up.  KBOX boxes of 128 columns per stage and unit.
 // KS > 1 (every CTA has one unit): the contraction is cut into KS slices that run side by side: weight slice s fills rows 32 s .. of the tile, token
@@ -212,32 +209,9 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     pdl_wait();
     {
       const int t = int(threadIdx.x) - (IS_THREADS - IS_EPI);
-      if (t < g.tokens) sx[t] = g.sx[t];  // (at most 64 tokens)
+      if (t < 64) sx[t] = t < g.tokens ? g.sx[t] : 0.f;
       asm volatile("bar.sync 1, %0;" ::"n"(IS_EPI) : "memory");
     }
-    const bool pitch_even = (g.ld_out & 1) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 3) == 0;
-    // Finishes the sum of (token t, feature m) and stores it; called by a whole warp, neighbouring lanes own neighbouring features.
-    auto finish = [&](int sum, int t, int m, bool m_ok, float sw, float bias, float res) {
-      float x = i8_value(sum, sx[t], sw, bias);
-      if (gated) {
-        // lanes 0-15 of a warp hold gate rows, lanes 16-31 the matching up rows
-        const float partner = __shfl_xor_sync(0xffffffffu, x, 16);
-        if (m_ok && lane < 16) g.out[t * g.ld_out + (m >> 5) * 16 + (m & 15)] = __float2bfloat16(i8_silu(x) * partner);
-        return;
-      }
-      if (g.act) x = is_act(x, g.act);
-      x += res;
-      // pairs of neighbouring lanes store two features (4 bytes) at a time
-      const bool writes_pair = pitch_even && !(lane & 1) && m + 1 < g.features;
-      const bool covered = pitch_even && (lane & 1);  // the even neighbour stores this lane's value
-      const float up = __shfl_down_sync(0xffffffffu, x, 1);
-      __nv_bfloat16* at = g.out + t * g.ld_out + m;
-      if (m_ok) {
-        if (writes_pair) *reinterpret_cast<uint32_t*>(at) = pack_bf16x2(x, up);
-        else if (!covered) *at = __float2bfloat16(x);
-      }
-    };
-    auto residual_at = [&](int t, int m, bool ok) { return g.residual && ok && t < g.tokens ? __bfloat162float(g.residual[t * g.ld_res + m]) : 0.f; };
     const int n_acc = min(NACC, p.k_stages * STEPS);
     if constexpr (KS > 1) {
       constexpr int MINE = TOK / KS;  // tokens this warp finishes: the slices' sums are exchanged, then each warp takes a share
@@ -246,8 +220,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const float sw = m_ok ? g.sw[m] : 0.f;
       const float bias = (g.bias && m_ok) ? __bfloat162float(g.bias[m]) : 0.f;
       float res[MINE];
-#pragma unroll
-      for (int j = 0; j < MINE; ++j) res[j] = residual_at(quarter * MINE + j, m, m_ok);
+      i8_residual(g, res, quarter * MINE, m, m_ok);
       const bool ready = !*abort_flag && mbar_wait(&acc_full[0], 0);
       if (!ready) give_up();
       tc_fence_after();
@@ -268,15 +241,14 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       }
       asm volatile("bar.sync 1, %0;" ::"n"(IS_EPI) : "memory");
       if (!*abort_flag) {
+        int sum[MINE];
 #pragma unroll
         for (int j = 0; j < MINE; ++j) {
-          const int t = quarter * MINE + j;
-          if (t >= g.tokens) break;  // (uniform)
-          int sum = 0;
+          sum[j] = 0;
 #pragma unroll
-          for (int sl = 0; sl < KS; ++sl) sum += slices[(sl * 32 + lane) * (TOK + 1) + t];
-          finish(sum, t, m, m_ok, sw, bias, res[j]);
+          for (int sl = 0; sl < KS; ++sl) sum[j] += slices[(sl * 32 + lane) * (TOK + 1) + quarter * MINE + j];
         }
+        i8_finish(g, sum, sx + quarter * MINE, quarter * MINE, m, m_ok, sw, bias, res);
       }
     } else {
       for (int pass = 0; pass < passes; ++pass) {
@@ -290,8 +262,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         const float sw = m_ok ? g.sw[m] : 0.f;
         const float bias = (g.bias && m_ok) ? __bfloat162float(g.bias[m]) : 0.f;
         float res[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) res[j] = residual_at(j, m, m_ok);
+        i8_residual(g, res, 0, m, m_ok);
         const bool ready = !*abort_flag && mbar_wait(&acc_full[acc], (pass >> 1) & 1);
         if (!__all_sync(0xffffffffu, ready)) {
           if (lane == 0) give_up();
@@ -314,15 +285,8 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] += int(r[j]);
           }
-          if (n0 > 0) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) res[j] = residual_at(n0 + j, m, m_ok);
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (n0 + j >= g.tokens) break;  // (uniform)
-            finish(v[j], n0 + j, m, m_ok, sw, bias, res[j]);
-          }
+          if (n0 > 0) i8_residual(g, res, n0, m, m_ok);
+          i8_finish(g, v, sx + n0, n0, m, m_ok, sw, bias, res);
         }
         tc_fence_before();
         __syncwarp();
