@@ -1,4 +1,5 @@
-// Shared by the kernels of the 8-bit integer product (gemm_i8_sm100.cu: entry point and many tokens, gemm_i8_stream_sm100.cu: few tokens):
+// Shared by the kernels of the 8-bit integer product (gemm_i8_sm100.cu: entry point and many tokens, gemm_i8_stream_sm100.cu: few tokens,
+// gemm_i8_split_sm100.cu: in between):
 //   out[t, f] = act(sx[t] sw[f] sum_k x[t, k] w[f, k] + bias[f]) + residual[t, f]
 #pragma once
 #include <cuda.h>
@@ -7,6 +8,7 @@
 #include <stdint.h>
 
 #include "attention_sm100.cuh"
+#include "ptx_sm100.cuh"
 #include "tpb_api.h"
 
 namespace tpb {
@@ -57,7 +59,7 @@ __device__ __forceinline__ void i8_activate(float (&v)[N], int act) {
 // Tokens t0 .. t0 + N of feature m, for the kernels whose lanes are features: neighbouring lanes of a warp have neighbouring features, m_ok says whether this lane's
 // exists, sx points to the scales of the tokens, res are the residual's values.  Called by whole warps.
 template <int N>
-__device__ __forceinline__ void i8_finish(const I8Gemm& g, const int (&sum)[N], const float* sx, int t0, int m, bool m_ok, float sw, float bias, const float (&res)[N]) {
+__device__ __forceinline__ void i8_finish(const I8Gemm& g, const int (&sum)[N], const float* sx, int t0, int m, bool m_ok, float sw, float bias, const float* res) {
   float v[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) v[j] = i8_value(sum[j], sx[j], sw, bias);
@@ -83,10 +85,20 @@ __device__ __forceinline__ void i8_finish(const I8Gemm& g, const int (&sum)[N], 
   for (int j = 0; j < N; ++j)
     if (t0 + j < g.tokens) out[j * g.ld_out] = __float2bfloat16(v[j]);
 }
+// The residual of those tokens (zeros without one).  Addresses past the end are drawn back into the matrix: loads that no branch keeps apart are in flight together.
 template <int N>
-__device__ __forceinline__ void i8_residual(const I8Gemm& g, float (&res)[N], int t0, int m, bool m_ok) {
+__device__ __forceinline__ void i8_residual(const I8Gemm& g, float (&res)[N], int t0, int m) {
+  if (!g.residual) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) res[j] = g.residual && m_ok && t0 + j < g.tokens ? __bfloat162float(g.residual[(t0 + j) * g.ld_res + m]) : 0.f;
+    for (int j = 0; j < N; ++j) res[j] = 0.f;
+    return;
+  }
+  const uint16_t* at = reinterpret_cast<const uint16_t*>(g.residual) + min(m, g.features - 1);
+  uint16_t raw[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) raw[j] = at[min(t0 + j, g.tokens - 1) * g.ld_res];
+#pragma unroll
+  for (int j = 0; j < N; ++j) res[j] = bf16_bits_to_float(raw[j]);
 }
 
 // [rows, k] bytes, row pitch ld; box = [box_rows][128 columns], 128-byte swizzle.  What lies past k is not read: it arrives as zeros.
@@ -102,5 +114,8 @@ inline int i8_tmap(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t k,
 }
 
 int gemm_i8_stream_launch(const I8Gemm& g, int sms, cudaStream_t stream);  // at most 64 tokens
+// bn tokens of a tile (32, 64, 128), CTAs that share its contraction (1, 2, 4, 8; at most one per k-block of 128 columns; bn / splits at least 8)
+bool gemm_i8_split_pick(int tokens, int features, int k, int sms, int* bn, int* splits);  // false: another kernel is faster
+int gemm_i8_split_launch(const I8Gemm& g, int bn, int splits, cudaStream_t stream);
 
 }  // namespace tpb

@@ -314,13 +314,14 @@ static int ip_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
   return launch_dependent(gemm_i8_pair_kernel<BN>, dim3(2 * pairs), dim3(IP_THREADS), S::SMEM, stream, g.early != 0, ta, tb, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
-// Columns of the pair tile: rounds of tiles x time of a k-block, in clocks (as gemm_pair_tile has them).
+// Columns of the pair tile: rounds of tiles x time of a k-block, in clocks (256 x 22016 x 4096 with 256 / 128 columns 31.9 / 29.3 us, 512 x 12288 x 4096
+// 28.3 / 26.7, 512 x 22016 x 4096 40.5 / 43.1, 768 x 12288 x 4096 30.6 / 35.0, 1024 x 4096 x 11008 35.2 / 39.3).
 static int ip_tile(int tokens, int features, int sms) {
   auto rounds = [&](int bn) {
     const long long tiles = (long long)((tokens + IP_BM - 1) / IP_BM) * ((features + bn - 1) / bn);
     return (tiles + sms / 2 - 1) / (sms / 2);
   };
-  return rounds(256) * 512 <= rounds(128) * 351 ? 256 : 128;
+  return rounds(256) * 512 <= rounds(128) * 325 ? 256 : 128;
 }
 
 }  // namespace tpb
@@ -343,6 +344,8 @@ extern "C" int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, 
   const tpb::I8Gemm g = {x, w, sx, sw, static_cast<bf16*>(out), static_cast<const bf16*>(bias), static_cast<const bf16*>(residual), ldx, ldw, ld_out, ld_res,
                          tokens, features, k, act, early, static_cast<uint32_t*>(status)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int bn = 0, splits = 0;
+  if (tpb::gemm_i8_split_pick(tokens, features, k, sms, &bn, &splits)) return tpb::gemm_i8_split_launch(g, bn, splits, s);
   if (tokens <= 64) return tpb::gemm_i8_stream_launch(g, sms, s);
   return tpb::ip_tile(tokens, features, sms) == 256 ? tpb::ip_launch<256>(g, sms, s) : tpb::ip_launch<128>(g, sms, s);
 }

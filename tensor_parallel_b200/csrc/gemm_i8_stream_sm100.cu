@@ -5,7 +5,7 @@
 // tokens are the N side; with `early` the ring fills with weights before griddepcontrol.wait.  A box is 128 bytes wide there and here, so that
 // what differs is the number of columns in it (128), the MMA (kind::i8, 32 columns a step, exact 32-bit sums) and the epilogue, which scales.
 //
-// One CTA (192 threads): warp 0 = TMA producer, warp 1 = MMA issuer, warps 2-5 = epilogue.  Rows of the MMA past the pass multiply whatever lies
+// One CTA: warp 0 = TMA producer, warp 1 = MMA issuer, then 4 epilogue warps (8 from 64 tokens on, each with half of them).  Rows of the MMA past the pass multiply whatever lies
 // behind it in shared memory; their results are never read.  Every mbarrier wait is bounded; on expiry the CTA records a status code and drains.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -24,8 +24,8 @@
 namespace tpb {
 
 constexpr int IS_UNIT = StreamRows::UNIT;
-constexpr int IS_THREADS = 192;
-constexpr int IS_EPI = 128;
+__host__ __device__ constexpr int IS_EPI(int bn, int ks) { return bn >= 64 && ks == 1 ? 256 : 128; }  // epilogue threads
+constexpr int IS_CONTROL = 2048;  // barriers, scales of the tokens
 constexpr int IS_MAX_STAGES = 16;
 constexpr size_t IS_RING_BYTES = 204 * 1024;
 __host__ __device__ constexpr size_t IS_SLICE_BYTES(int ks) { return ks > 1 ? 9 * 1024 : 0; }
@@ -43,7 +43,7 @@ struct IsParams {
 // KS > 1 (every CTA has one unit): the contraction is cut into KS slices that run side by side: weight slice s fills rows 32 s .. of the tile, token
 // slice s columns TOK s .., the diagonal blocks of the product are the slices' sums (the other blocks are never read), added up through shared memory.
 template <int BN, int NACC, int KBOX, int KS>
-__global__ void __launch_bounds__(IS_THREADS, 1)
+__global__ void __launch_bounds__(64 + IS_EPI(BN, KS), 1)
 gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_w1, const __grid_constant__ CUtensorMap tmap_x,
                       const IsParams p) {
   constexpr uint32_t X_BOX = BN * I8_BK, X_BYTES = KBOX * X_BOX;
@@ -51,6 +51,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   constexpr int STEPS = KBOX * (I8_BK / 32);  // MMAs of a stage; step n of the pass goes to accumulator n % NACC
   static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0 && TMEM_COLS >= 32, "TMEM allocation");
   constexpr int TOK = BN / KS;  // token columns of a slice
+  constexpr int EPI = IS_EPI(BN, KS);
   const I8Gemm& g = p.g;
   const uint32_t w_box = uint32_t(KS > 1 ? KS : p.rows.pass_units) * IS_UNIT * 128;  // [rows of a pass, or of all slices][128 columns]
   const uint32_t w_bytes = KBOX * w_box, stage_bytes = w_bytes + X_BYTES;
@@ -64,9 +65,9 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   uint64_t* acc_empty = acc_full + 2;              // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  float* sx = reinterpret_cast<float*>(tmem_slot + 4);    // [64] scales of the tokens
-  int* slices = reinterpret_cast<int*>(smem + 1024);      // KS > 1: [KS][32 rows][TOK + 1] partial sums
-  uint8_t* ring = smem + 1024 + IS_SLICE_BYTES(KS);
+  float* sx = reinterpret_cast<float*>(tmem_slot + 4);    // [BN] scales of the tokens
+  int* slices = reinterpret_cast<int*>(smem + IS_CONTROL);     // KS > 1: [KS][32 rows][TOK + 1] partial sums
+  uint8_t* ring = smem + IS_CONTROL + IS_SLICE_BYTES(KS);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
   const int unit0 = p.rows.first(blockIdx.x), my_units = p.rows.first(blockIdx.x + 1) - unit0, passes = p.rows.passes;
@@ -83,7 +84,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], IS_EPI / 32);
+      mbar_init(&acc_empty[a], EPI / 32);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -207,11 +208,8 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     const int quarter = warp & 3;
     const bool gated = g.act == I8_GATED;
     pdl_wait();
-    {
-      const int t = int(threadIdx.x) - (IS_THREADS - IS_EPI);
-      if (t < 64) sx[t] = t < g.tokens ? g.sx[t] : 0.f;
-      asm volatile("bar.sync 1, %0;" ::"n"(IS_EPI) : "memory");
-    }
+    for (int t = int(threadIdx.x) - 64; t < BN; t += EPI) sx[t] = t < g.tokens ? g.sx[t] : 0.f;
+    asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
     const int n_acc = min(NACC, p.k_stages * STEPS);
     if constexpr (KS > 1) {
       constexpr int MINE = TOK / KS;  // tokens this warp finishes: the slices' sums are exchanged, then each warp takes a share
@@ -220,7 +218,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const float sw = m_ok ? g.sw[m] : 0.f;
       const float bias = (g.bias && m_ok) ? __bfloat162float(g.bias[m]) : 0.f;
       float res[MINE];
-      i8_residual(g, res, quarter * MINE, m, m_ok);
+      i8_residual(g, res, quarter * MINE, m);
       const bool ready = !*abort_flag && mbar_wait(&acc_full[0], 0);
       if (!ready) give_up();
       tc_fence_after();
@@ -239,7 +237,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 #pragma unroll
         for (int j = 0; j < TOK; ++j) slices[(quarter * 32 + lane) * (TOK + 1) + j] = v[j];
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(IS_EPI) : "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
       if (!*abort_flag) {
         int sum[MINE];
 #pragma unroll
@@ -251,6 +249,8 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         i8_finish(g, sum, sx + quarter * MINE, quarter * MINE, m, m_ok, sw, bias, res);
       }
     } else {
+      constexpr int SHARE = BN / (EPI / 128);  // tokens of this warp
+      const int first = (warp - 2) / 4 * SHARE;
       for (int pass = 0; pass < passes; ++pass) {
         const int acc = pass & 1, rows = pass_units(pass) * IS_UNIT;
         const bool m64 = rows <= 64 && !gated;
@@ -261,8 +261,8 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         // fetched while the weights are still streaming: a load behind the accumulators would add a full round trip
         const float sw = m_ok ? g.sw[m] : 0.f;
         const float bias = (g.bias && m_ok) ? __bfloat162float(g.bias[m]) : 0.f;
-        float res[16];
-        i8_residual(g, res, 0, m, m_ok);
+        float res[SHARE];
+        i8_residual(g, res, first, m);
         const bool ready = !*abort_flag && mbar_wait(&acc_full[acc], (pass >> 1) & 1);
         if (!__all_sync(0xffffffffu, ready)) {
           if (lane == 0) give_up();
@@ -270,8 +270,8 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         }
         tc_fence_after();
         const uint32_t t_lane = tmem_base + (uint32_t(quarter * 32) << 16) + acc * ACC_COLS;
-#pragma unroll 1
-        for (int n0 = 0; n0 < BN; n0 += 16) {
+#pragma unroll
+        for (int n0 = first; n0 < first + SHARE; n0 += 16) {
           if (n0 >= g.tokens) break;
           int v[16];
 #pragma unroll
@@ -285,8 +285,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] += int(r[j]);
           }
-          if (n0 > 0) i8_residual(g, res, n0, m, m_ok);
-          i8_finish(g, v, sx + n0, n0, m, m_ok, sw, bias, res);
+          i8_finish(g, v, sx + n0, n0, m, m_ok, sw, bias, res + (n0 - first));
         }
         tc_fence_before();
         __syncwarp();
@@ -317,7 +316,7 @@ static int is_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
   int stages = int(IS_RING_BYTES / stage_bytes);
   if (stages > IS_MAX_STAGES) stages = IS_MAX_STAGES;
   p.stages = stages;
-  const size_t smem = 1024 + 1024 + IS_SLICE_BYTES(KS) + stages * stage_bytes + over;
+  const size_t smem = 1024 + IS_CONTROL + IS_SLICE_BYTES(KS) + stages * stage_bytes + over;
   static std::atomic<bool> configured[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TPB_ERR_CUDA;
@@ -330,7 +329,7 @@ static int is_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
   if (rc == TPB_OK) rc = i8_tmap(&tw1, g.w, g.features, g.k, g.ldw, IS_UNIT);
   if (rc == TPB_OK) rc = i8_tmap(&tx, g.x, g.tokens, g.k, g.ldx, BN / KS);
   if (rc != TPB_OK) return rc;
-  return launch_dependent(gemm_i8_stream_kernel<BN, NACC, KBOX, KS>, dim3(p.rows.grid), dim3(IS_THREADS), smem, stream, g.early != 0, tw, tw1, tx, p) == cudaSuccess
+  return launch_dependent(gemm_i8_stream_kernel<BN, NACC, KBOX, KS>, dim3(p.rows.grid), dim3(64 + IS_EPI(BN, KS)), smem, stream, g.early != 0, tw, tw1, tx, p) == cudaSuccess
              ? TPB_OK
              : TPB_ERR_CUDA;
 }
