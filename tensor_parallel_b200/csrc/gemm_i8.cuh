@@ -118,4 +118,8 @@ int gemm_i8_stream_launch(const I8Gemm& g, int sms, cudaStream_t stream);  // at
 bool gemm_i8_split_pick(int tokens, int features, int k, int sms, int* bn, int* splits);  // false: another kernel is faster
 int gemm_i8_split_launch(const I8Gemm& g, int bn, int splits, cudaStream_t stream);
 
+cudaError_t gemm_i8_stream_preload();
+cudaError_t gemm_i8_split_preload();
+cudaError_t rows_int8_preload();
+
 }  // namespace tpb

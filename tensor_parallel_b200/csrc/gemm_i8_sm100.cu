@@ -349,3 +349,14 @@ extern "C" int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, 
   if (tokens <= 64) return tpb::gemm_i8_stream_launch(g, sms, s);
   return tpb::ip_tile(tokens, features, sms) == 256 ? tpb::ip_launch<256>(g, sms, s) : tpb::ip_launch<128>(g, sms, s);
 }
+
+// Loads every kernel of the 8-bit operators on the current device: a single host thread that drives several GPUs does so before the first of them waits for a peer.
+extern "C" int tpb_int8_preload(void) {
+  cudaFuncAttributes attr;
+  cudaError_t e = cudaFuncGetAttributes(&attr, tpb::gemm_i8_pair_kernel<256>);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, tpb::gemm_i8_pair_kernel<128>);
+  if (e == cudaSuccess) e = tpb::gemm_i8_stream_preload();
+  if (e == cudaSuccess) e = tpb::gemm_i8_split_preload();
+  if (e == cudaSuccess) e = tpb::rows_int8_preload();
+  return e == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+}

@@ -293,13 +293,21 @@ bool gemm_i8_split_pick(int tokens, int features, int k, int sms, int* bn, int* 
   return *splits > 1 ? k_blocks >= 16 : tokens <= 128 && tiles(128) <= sms;
 }
 
+#define IX_FORMS(GO) GO(32, 1) GO(32, 2) GO(32, 4) GO(64, 1) GO(64, 2) GO(64, 4) GO(64, 8) GO(128, 1) GO(128, 2)
 int gemm_i8_split_launch(const I8Gemm& g, int bn, int splits, cudaStream_t stream) {
-#define GO(BN, S) if (bn == BN && splits == S) return ix_launch<BN, S>(g, stream)
-  GO(32, 1); GO(32, 2); GO(32, 4);
-  GO(64, 1); GO(64, 2); GO(64, 4); GO(64, 8);
-  GO(128, 1); GO(128, 2); GO(128, 4); GO(128, 8);
+#define GO(BN, S) if (bn == BN && splits == S) return ix_launch<BN, S>(g, stream);
+  IX_FORMS(GO)
 #undef GO
   return TPB_ERR_ARG;
+}
+
+cudaError_t gemm_i8_split_preload() {
+  cudaFuncAttributes attr;
+  cudaError_t e = cudaSuccess;
+#define LOAD(BN, S) if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, gemm_i8_split_kernel<BN, S>);
+  IX_FORMS(LOAD)
+#undef LOAD
+  return e;
 }
 
 }  // namespace tpb

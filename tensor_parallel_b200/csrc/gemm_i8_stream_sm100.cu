@@ -345,4 +345,13 @@ int gemm_i8_stream_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
   return TPB_ERR_ARG;
 }
 
+cudaError_t gemm_i8_stream_preload() {
+  cudaFuncAttributes attr;
+  cudaError_t e = cudaSuccess;
+#define LOAD(BN, NACC, KBOX, KS) if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, gemm_i8_stream_kernel<BN, NACC, KBOX, KS>)
+  LOAD(32, 4, 2, 4); LOAD(64, 2, 2, 4); LOAD(16, 8, 2, 1); LOAD(32, 8, 2, 1); LOAD(64, 2, 2, 1);
+#undef LOAD
+  return e;
+}
+
 }  // namespace tpb

@@ -13,6 +13,7 @@
 #include <stdint.h>
 
 #include "attention_sm100.cuh"
+#include "gemm_i8.cuh"
 #include "launch.cuh"
 #include "ptx_sm100.cuh"
 #include "tpb_api.h"
@@ -609,6 +610,32 @@ static cudaError_t ri_dispatch(const RiParams& p, int sms, int mode, bool early,
 #define RI_GO(MODE) (vec ? ri_launch<T, MODE, true>(p, sms, early, stream) : ri_launch<T, MODE, false>(p, sms, early, stream))
   return mode == RI_ROWS ? RI_GO(RI_ROWS) : mode == RI_RMS ? RI_GO(RI_RMS) : RI_GO(RI_LAYER);
 #undef RI_GO
+}
+
+template <typename T, int MODE>
+static cudaError_t ri_preload() {
+  cudaFuncAttributes attr;
+  cudaError_t e = cudaSuccess;
+#define LOAD(...) if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, __VA_ARGS__)
+  LOAD(rows_int8_ring_kernel<T, MODE, true>);
+  LOAD(rows_int8_ring_kernel<T, MODE, false>);
+  LOAD(rows_int8_kernel<T, MODE, 2, true, true, 1024>);
+  LOAD(rows_int8_kernel<T, MODE, 2, false, true, 1024>);
+  LOAD(rows_int8_kernel<T, MODE, 1, true, false, 256>);
+  LOAD(rows_int8_kernel<T, MODE, 1, false, false, 256>);
+  LOAD(rows_int8_kernel<T, MODE, 2, true, false, 256>);
+  LOAD(rows_int8_kernel<T, MODE, 2, false, false, 256>);
+  LOAD(rows_int8_kernel<T, MODE, 2, true, false, 1024>);
+  LOAD(rows_int8_kernel<T, MODE, 2, false, false, 1024>);
+#undef LOAD
+  return e;
+}
+cudaError_t rows_int8_preload() {
+  const cudaError_t all[6] = {ri_preload<bf16, RI_ROWS>(), ri_preload<bf16, RI_RMS>(), ri_preload<bf16, RI_LAYER>(),
+                              ri_preload<float, RI_ROWS>(), ri_preload<float, RI_RMS>(), ri_preload<float, RI_LAYER>()};
+  for (const cudaError_t e : all)
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
 }
 
 }  // namespace tpb

@@ -23,9 +23,17 @@ Kernels per layer of a decode step::
     parallel block     qkv GEMM(+norm) -> attention -> MLP-in GEMM(+norm +activation) -> [o | down] GEMM(+all-reduce
                        +residual)                                                                                   = 4
 
+``quantize="int8"`` serves the projections of all layers with 8-bit integer weights (a scale per output channel) and activations (a scale per
+token); embedding, attention, cache and head stay bf16.  The norms then run as kernels that write 8-bit rows, and nothing is folded into a
+weight::
+
+    sequential block   norm -> qkv -> attention -> rows -> o_proj (+residual) -> norm -> MLP-in (+activation) -> rows -> MLP-out (+residual)  = 9
+    parallel block     norm (two, where the MLP has its own) -> qkv -> attention -> rows -> MLP-in -> o_proj -> rows -> MLP-out      = 8 or 9
+
 With several ranks the row-parallel GEMMs push their partial tiles to every peer from the epilogue and reduce
 them in the same kernel (decode), or write into symmetric memory and run the device all-reduce (prefill);
-nothing goes through NCCL.  The reference reaches the same maths through Python wrappers, host barriers and
+nothing goes through NCCL.  (8-bit projections leave their partial results in symmetric memory for the device all-reduce, whose sum the next norm
+kernel adds to the residual stream.)  The reference reaches the same maths through Python wrappers, host barriers and
 one NCCL call per collective (``src/tensor_parallel/tensor_parallel.py:139-161``,
 ``src/tensor_parallel/communications.py:34-52``).
 """
@@ -67,7 +75,10 @@ def _cat_bias(parts, sizes, device) -> Optional[torch.Tensor]:
 class DecoderEngine:
     def __init__(self, shard, comm=None, max_batch: int = 8, max_seq: int = 2560, use_graph: bool = True, embed_table=None,
                  process_group=None, replicate_embedding: bool = True, spec: Optional[engine_spec.DecoderSpec] = None,
-                 pipeline_prefill: Optional[bool] = None):
+                 pipeline_prefill: Optional[bool] = None, quantize: Optional[str] = None):
+        if quantize not in (None, "int8"):
+            raise ValueError(f"quantize={quantize!r}: the engine serves bf16 (None) or 8-bit integer projections ('int8')")
+        self.quantize = quantize
         spec = spec if spec is not None else engine_spec.describe(shard, max_seq)
         if spec is None:
             raise ValueError("no serving description for this model (see tensor_parallel_b200.engine_spec)")
@@ -116,6 +127,9 @@ class DecoderEngine:
             raise ValueError("gated MLPs are served with the SiLU gate only")
         for L in spec.layers:
             nq, nk = L.wq.shape[0] // D, L.wk.shape[0] // D
+            if quantize:
+                self.layers.append(self._int8_layer_weights(L, gated, nq, nk))
+                continue
             wqkv_raw = torch.cat([L.wq, L.wk, L.wv], dim=0)
             wqkv = _fold(wqkv_raw, L.ln1_w)
             bqkv = _cat_bias([L.bq, L.bk, L.bv], [L.wq.shape[0], L.wk.shape[0], L.wv.shape[0]], dev)
@@ -165,6 +179,7 @@ class DecoderEngine:
                 entry["wo"], entry["bo"] = L.wo, L.bo
                 entry["wd"], entry["bd"] = (w_down if w_down is L.w_down else w_down.contiguous()), L.b_down
             self.layers.append(entry)
+        self._summed: Optional[torch.Tensor] = None  # 8-bit layers of several ranks: what the next norm adds to the residual stream
         self.nq, self.nkv, self.ff = self.layers[0]["nq"], self.layers[0]["nkv"], self.layers[0]["ff"]
 
         # -- head -----------------------------------------------------------------------------------
@@ -212,6 +227,28 @@ class DecoderEngine:
 
     # -- helpers ------------------------------------------------------------------------------------
 
+    def _int8_layer_weights(self, L, gated: bool, nq: int, nk: int) -> dict:
+        """The serving layout of a layer with 8-bit projections: weights as ``Int8Rows``, norm parameters and biases as they are."""
+        rows = native.quantize_int8
+
+        def plain(t):
+            return None if t is None else t.to(torch.bfloat16).contiguous()
+
+        bqkv = _cat_bias([L.bq, L.bk, L.bv], [L.wq.shape[0], L.wk.shape[0], L.wv.shape[0]], self.device)
+        ff, w_up, w_gate, w_down, b1 = L.w_up.shape[0], L.w_up, L.w_gate, L.w_down, L.b_up
+        if gated:
+            pad = -ff % 16  # rows of zeros (and columns of the down projection) fill the last group of 16: silu(0) * 0 = 0
+            w_gate, w_up = (torch.cat([w, w.new_zeros(pad, w.shape[1])]) if pad else w for w in (w_gate, w_up))
+            w_down = torch.cat([w_down, w_down.new_zeros(w_down.shape[0], pad)], dim=1) if pad else w_down
+            w_up = native.interleave_gate_up(w_gate, w_up)
+            if L.b_gate is not None or L.b_up is not None:
+                bg, bu = (torch.zeros(ff + pad, device=self.device) if b is None else torch.nn.functional.pad(b.float(), (0, pad)) for b in (L.b_gate, L.b_up))
+                b1 = torch.stack((bg.reshape(-1, 16), bu.reshape(-1, 16)), dim=1).reshape(-1)
+            ff += pad
+        return dict(wqkv=rows(torch.cat([L.wq, L.wk, L.wv], dim=0)), bqkv=plain(bqkv), ln1=(plain(L.ln1_w), plain(L.ln1_b)),
+                    ln2=None if L.ln2_w is None else (plain(L.ln2_w), plain(L.ln2_b)), w1=rows(w_up), b1=plain(b1), wo=rows(L.wo), bo=L.bo, wd=rows(w_down),
+                    bd=L.b_down, nq=nq, nkv=nk, ff=ff)
+
     def _gather_columns(self, local: torch.Tensor) -> torch.Tensor:
         import torch.distributed as dist
 
@@ -229,7 +266,8 @@ class DecoderEngine:
     def _own_tensors(self):
         seen = [self.embed, self.embed_local, self.pos_embed, self.pos_local, self.lm_head, self.head_bias, self.head_rowsum]
         for entry in self.layers:
-            seen.extend(entry.values())
+            for value in entry.values():
+                seen.extend(value if isinstance(value, tuple) else (value,))  # (8-bit rows and norm parameters are pairs)
         return [t for t in seen if isinstance(t, torch.Tensor)]
 
     @torch.no_grad()
@@ -312,6 +350,8 @@ class DecoderEngine:
             # what the passes above did not launch: the kernels of the multi-rank projections, whose forms depend on rank count and batch
             native.check(native.LIB.tpb_gemm_preload(), "tpb_gemm_preload")
             native.check(native.LIB.tpb_comm_preload(), "tpb_comm_preload")
+            if self.quantize:
+                native.check(native.LIB.tpb_int8_preload(), "tpb_int8_preload")
 
     # -- building blocks --------------------------------------------------------------------------
 
@@ -336,17 +376,52 @@ class DecoderEngine:
             return native.gemm_nt(x, weight, bias=bias, act=act, out=out, norm=(self.mode, self.eps, rowsum), early=early)
         return native.gemm_nt(n, weight, bias=bias, act=act, out=out)
 
-    def _layer(self, i, x, n, qkv, q_rot, cat, act_buf, batch, seq, decode: bool):
+    def _int8_norm(self, x, norm, early):
+        """8-bit rows of the norm of the residual stream ``x``, which is brought up to date first: what the ranks' last sum left is added."""
+        summed, self._summed = self._summed, None
+        return native.rows_int8(x, norm[0], norm[1], self.eps, self.mode - 1, residual=summed, sum_out=None if summed is None else x, early=early)
+
+    def _int8_row_parallel(self, parts, x, early):
+        """``x += all-reduce(sum of the projections) + biases`` for ``parts`` of (rows, weight, bias; the shard's copy, bias / world).  With several ranks the
+        sum is left for the next norm to add."""
+        if self.world == 1:
+            for rows, weight, bias in parts:
+                native.gemm_int8(rows, weight, bias, residual=x, out=x, early=early)
+            return
+        staged = self.comm.staging_view("in", tuple(x.shape), torch.bfloat16)
+        for n, (rows, weight, bias) in enumerate(parts):
+            native.gemm_int8(rows, weight, residual=staged if n else None, out=staged)
+            if bias is not None:
+                x.add_(bias * self.world)
+        self._summed = self.comm.all_reduce(staged)
+
+    def _int8_settle(self, x):
+        """Adds what the last layer left for a norm that does not come."""
+        if self._summed is not None:
+            x.add_(self._summed)
+            self._summed = None
+
+    def _int8_layer(self, i, x, qkv, q_rot, cat, act_buf, batch, seq, decode: bool):
         L = self.layers[i]
+        early = decode and self.world == 1  # (see _layer)
+        rows = self._int8_norm(x, L["ln1"], early)
+        mlp_rows = None
+        if self.parallel:  # the MLP reads the block input as well
+            mlp_rows = rows if L["ln2"] is None else self._int8_norm(x, L["ln2"], early)
+        native.gemm_int8(rows, L["wqkv"], L["bqkv"], out=qkv, early=early)
+        attn = self._attend(i, qkv, q_rot, cat, batch, seq, decode, early)
+        attn_rows = native.rows_int8(attn, early=early)
+        if not self.parallel:
+            self._int8_row_parallel([(attn_rows, L["wo"], L["bo"])], x, early)
+            mlp_rows = self._int8_norm(x, L["ln2"], early)
+        hidden = cat[:, self.nq * self.head_dim :] if self.parallel else act_buf
+        native.gemm_int8(mlp_rows, L["w1"], L["b1"], act=self.act, out=hidden, early=early)
+        down = (native.rows_int8(hidden, early=early), L["wd"], L["bd"])
+        self._int8_row_parallel([(attn_rows, L["wo"], L["bo"]), down] if self.parallel else [down], x, early)
+
+    def _attend(self, i, qkv, q_rot, cat, batch, seq, decode: bool, early: bool):
+        """Rotary embedding, cache and attention of layer ``i`` on its projection ``qkv``; the result is the first columns of ``cat``."""
         D, spec = self.head_dim, self.spec
-        fold = n is None
-        # A decode step on one GPU is a chain of kernels that each stream megabytes nothing in the chain writes (weights, older
-        # cache rows): every kernel may start while its predecessor drains and fetch those first.  With several ranks a
-        # predecessor may be waiting for a peer, and kernels parked behind it take the SMs it needs: not there.
-        early = decode and fold and self.world == 1
-        if not fold:
-            native.norm_forward(x, None, None, self.eps, self.mode - 1, out=n)
-        self._projection(x, n, L["wqkv"], L["bqkv"], L["sqkv"], qkv, early=early)
         nq_w, nk_w = self.nq * D, self.nkv * D
         q2, k2, v2 = qkv[:, :nq_w], qkv[:, nq_w : nq_w + nk_w], qkv[:, nq_w + nk_w :]
         attn = cat[:, :nq_w]
@@ -363,6 +438,23 @@ class DecoderEngine:
             v = self.vcache[i][:batch, :, :total].transpose(1, 2)
             native.attention_forward(q_rot.view(batch, seq, self.nq, D), k, v, True, None,
                                      out=attn.unflatten(0, (batch, seq)).unflatten(2, (self.nq, D)))
+        return attn
+
+    def _layer(self, i, x, n, qkv, q_rot, cat, act_buf, batch, seq, decode: bool):
+        if self.quantize:
+            return self._int8_layer(i, x, qkv, q_rot, cat, act_buf, batch, seq, decode)
+        L = self.layers[i]
+        D = self.head_dim
+        fold = n is None
+        # A decode step on one GPU is a chain of kernels that each stream megabytes nothing in the chain writes (weights, older
+        # cache rows): every kernel may start while its predecessor drains and fetch those first.  With several ranks a
+        # predecessor may be waiting for a peer, and kernels parked behind it take the SMs it needs: not there.
+        early = decode and fold and self.world == 1
+        if not fold:
+            native.norm_forward(x, None, None, self.eps, self.mode - 1, out=n)
+        self._projection(x, n, L["wqkv"], L["bqkv"], L["sqkv"], qkv, early=early)
+        nq_w = self.nq * D
+        attn = self._attend(i, qkv, q_rot, cat, batch, seq, decode, early)
         if self.parallel:
             # the MLP reads the block input as well (through its own norm weights, folded into w1; the statistics are
             # the same rows'), and both partial results leave through one row-parallel GEMM
@@ -416,7 +508,7 @@ class DecoderEngine:
         if self.spec.pos_embed is not None:
             positions = torch.arange(base, base + seq, device=dev).repeat(batch)
         x = self._embed_tokens(input_ids.to(dev).reshape(-1), positions)
-        n = torch.empty(tokens, self.hidden, **bf) if tokens > 64 else None
+        n = torch.empty(tokens, self.hidden, **bf) if tokens > 64 and not self.quantize else None
         qkv = torch.empty(tokens, (self.nq + 2 * self.nkv) * D, **bf)
         q_rot = torch.empty(tokens, self.nq, D, **bf)
         cat = torch.empty(tokens, self.cat.shape[1], **bf)
@@ -426,6 +518,7 @@ class DecoderEngine:
         else:
             for i in range(len(self.layers)):
                 self._layer(i, x, n, qkv, q_rot, cat, act_buf, batch, seq, decode=False)
+            self._int8_settle(x)
         last = x.view(batch, seq, self.hidden)[:, -1].contiguous()
         logits_local = torch.empty(batch, self.vocab_local, **bf)
         logits = self._head(last, logits_local, batch)
@@ -433,7 +526,7 @@ class DecoderEngine:
         return logits.float()
 
     def _can_pipeline(self, batch: int, seq: int) -> bool:
-        if not self.pipeline_prefill or self.world == 1 or batch < 2 or batch * seq < 1024:
+        if self.quantize or not self.pipeline_prefill or self.world == 1 or batch < 2 or batch * seq < 1024:
             return False
         region = -(-((batch + 1) // 2 * seq * self.hidden * 2) // 1024) * 1024
         return 2 * region <= self.comm.staging_in.numel()
@@ -537,6 +630,7 @@ class DecoderEngine:
         for i in range(len(self.layers)):
             self._layer(i, x, self.n[:batch] if batch > 64 else None, self.qkv[:batch], None, self.cat[:batch],
                         None if self.parallel else self.act_buf[:batch], batch, 1, decode=True)
+        self._int8_settle(x)
         logits = self._head(x, self.logits_local[:batch], batch, decode=True)
         native.greedy_pick(logits, self.next_ids[:batch], self.ids[:batch], self.pos, early=self.world == 1)
         self.kernels_per_step = native.launch_count - before
@@ -635,7 +729,7 @@ class EngineGroup:
     own), whereas eager launches of the same kernels in the same order overlap as expected.  One process per GPU
     (:class:`DecoderEngine` with a graph per process) remains the fast path."""
 
-    def __init__(self, shards, comms, max_batch: int = 8, max_seq: int = 2560):
+    def __init__(self, shards, comms, max_batch: int = 8, max_seq: int = 2560, quantize: Optional[str] = None):
         specs = [engine_spec.describe(s, max_seq) for s in shards]
         if any(s is None for s in specs):
             raise ValueError("no serving description for this model")
@@ -648,11 +742,12 @@ class EngineGroup:
                 table = (torch.cat([s.embed.to(dev) for s in specs], dim=1).contiguous(),
                          None if spec.pos_embed is None else torch.cat([s.pos_embed.to(dev) for s in specs], dim=1).contiguous())
             with torch.cuda.device(spec.embed.device):
-                engine = DecoderEngine(shard, comm, max_batch=max_batch, max_seq=max_seq, use_graph=False, embed_table=table, spec=spec)
+                engine = DecoderEngine(shard, comm, max_batch=max_batch, max_seq=max_seq, use_graph=False, embed_table=table, spec=spec, quantize=quantize)
                 engine.preload()
                 self.engines.append(engine)
         first = self.engines[0]
         self.max_batch, self.max_seq, self.world, self.device = first.max_batch, first.max_seq, len(self.engines), first.device
+        self.quantize = first.quantize
         self.comm = first.comm
 
     @property

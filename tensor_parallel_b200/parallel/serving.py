@@ -20,14 +20,20 @@ class ServingMixin:
         backend = getattr(self, "_device_backend", None)
         return getattr(backend, "comm", None)
 
-    def serving_engine(self, max_batch: int = 8, max_seq: int = 2560):
+    def serving_engine(self, max_batch: int = 8, max_seq: int = 2560, quantize: Optional[str] = None):
         """The kernel-level engine of this model, or ``None`` when it does not apply: the shards must be CUDA bf16
         causal LMs of a family that ``tensor_parallel_b200.engine_spec`` can describe (Llama / Mistral / Qwen2, OPT,
         Falcon - self-contained or Hugging Face classes).
 
         The engine keeps its own serving-layout copies of the projection weights.  It notices through the tensors'
         version counters when the shard's parameters have been written to since it was built (an optimizer step,
-        ``load_state_dict``, a merged adapter) and is rebuilt then; with ZeRO-3 the flat shards are gathered first."""
+        ``load_state_dict``, a merged adapter) and is rebuilt then; with ZeRO-3 the flat shards are gathered first.
+
+        ``quantize``: ``"int8"`` serves the projections with 8-bit integer weights and activations (a scale per output channel and per token:
+        half of the weight bytes of a decode step, twice the tensor-core rate of a prompt), ``"bf16"`` as they are, ``None`` as the engine
+        that is there does (bf16 at first)."""
+        if quantize not in (None, "bf16", "int8"):
+            raise ValueError(f"quantize={quantize!r}: 'int8', 'bf16', or None for the present engine's")
         from tensor_parallel_b200 import engine_spec
 
         shard = self.module_shards[0]
@@ -39,14 +45,16 @@ class ServingMixin:
             with torch.no_grad():
                 manager.synchronize_weights(getattr(self, "all_cuda", True))
         eng = self._engine
+        form = None if quantize == "bf16" else "int8" if quantize == "int8" else getattr(eng, "quantize", None)
         if eng is not None and eng.stale():
             self._engine = eng = None
-        fits = eng is not None and eng.max_batch >= max_batch and eng.max_seq >= max_seq
+        fits = eng is not None and eng.max_batch >= max_batch and eng.max_seq >= max_seq and eng.quantize == form
         if fits:
             return eng
         if eng is not None and any(e._versions is None for e in getattr(eng, "engines", [eng])):
             raise RuntimeError("the training-layout weights were released (release_training_weights): the engine cannot be "
-                               f"rebuilt for max_batch={max_batch}, max_seq={max_seq}; it serves up to {eng.max_batch} x {eng.max_seq}")
+                               f"rebuilt for max_batch={max_batch}, max_seq={max_seq}, quantize={form}; it serves up to {eng.max_batch} x {eng.max_seq} "
+                               f"with quantize={eng.quantize}")
         if eng is not None:
             max_batch, max_seq = max(max_batch, eng.max_batch), max(max_seq, eng.max_seq)
         spec = engine_spec.describe(shard, max_seq)
@@ -62,7 +70,7 @@ class ServingMixin:
 
             self._engine = None  # (frees the old caches before the new ones are allocated)
             try:
-                self._engine = EngineGroup(list(self.module_shards), comms, max_batch=max_batch, max_seq=max_seq)
+                self._engine = EngineGroup(list(self.module_shards), comms, max_batch=max_batch, max_seq=max_seq, quantize=form)
             except ValueError:
                 return None
             return self._engine
@@ -73,7 +81,7 @@ class ServingMixin:
 
         self._engine = None
         self._engine = DecoderEngine(shard, comm if world > 1 else None, max_batch=max_batch, max_seq=max_seq, spec=spec,
-                                     process_group=getattr(self, "process_group", None))
+                                     process_group=getattr(self, "process_group", None), quantize=form)
         return self._engine
 
     def release_training_weights(self) -> int:
@@ -89,20 +97,23 @@ class ServingMixin:
         return sum(e.release_source_weights(shard) for e, shard in zip(engines, self.module_shards))
 
     @torch.no_grad()
-    def generate(self, input_ids: Optional[torch.Tensor] = None, max_new_tokens: int = 20, **kwargs):
+    def generate(self, input_ids: Optional[torch.Tensor] = None, max_new_tokens: int = 20, quantize: Optional[str] = None, **kwargs):
+        """``quantize``: see :meth:`serving_engine`; ``"int8"`` is for greedy decoding on the engine only."""
         greedy = not kwargs.get("do_sample", False) and kwargs.get("num_beams", 1) == 1 and not kwargs.get("output_scores", False)
         if input_ids is not None and greedy and set(kwargs) <= {"do_sample", "num_beams", "output_scores"}:
-            engine = self.serving_engine(input_ids.shape[0], input_ids.shape[1] + max_new_tokens + 4)
+            engine = self.serving_engine(input_ids.shape[0], input_ids.shape[1] + max_new_tokens + 4, quantize)
             if engine is not None:
                 return engine.generate(input_ids, max_new_tokens)
+        if quantize == "int8":
+            raise ValueError("quantize='int8' needs the CUDA serving engine and greedy decoding (bf16 shards of a served family, a prompt of ids)")
         from tensor_parallel_b200.models.generation import generate
 
         return generate(self, input_ids, max_new_tokens=max_new_tokens, **kwargs)
 
     @torch.no_grad()
-    def prefill(self, input_ids: torch.Tensor, max_new_tokens: int = 256) -> torch.Tensor:
-        """Engine-backed prompt pass; returns last-position logits ``[batch, vocab]``."""
-        engine = self.serving_engine(input_ids.shape[0], input_ids.shape[1] + max_new_tokens + 4)
+    def prefill(self, input_ids: torch.Tensor, max_new_tokens: int = 256, quantize: Optional[str] = None) -> torch.Tensor:
+        """Engine-backed prompt pass; returns last-position logits ``[batch, vocab]``.  ``quantize``: see :meth:`serving_engine`."""
+        engine = self.serving_engine(input_ids.shape[0], input_ids.shape[1] + max_new_tokens + 4, quantize)
         if engine is None:
             raise RuntimeError("prefill()/decode_step() need the CUDA serving engine (bf16 shards of a served family)")
         return engine.prefill(input_ids)

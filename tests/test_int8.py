@@ -167,3 +167,17 @@ def test_no_tokens():
     assert OF.linear_int8(OF.Int8Rows(x.values[:0], x.scales[:0]), w).shape == (0, 32)
     q, s = OF.quantize_int8(torch.empty(0, 3, 64))
     assert q.shape == (0, 3, 64) and s.shape == (0, 3)
+
+
+def test_generation_in_8_bits_needs_the_engine():
+    import tensor_parallel_b200 as tp
+    from tensor_parallel_b200.models.llama import LlamaConfig, LlamaForCausalLM
+
+    model = LlamaForCausalLM(LlamaConfig(vocab_size=64, hidden_size=32, intermediate_size=48, num_hidden_layers=1, num_attention_heads=4)).eval()
+    wrapped = tp.tensor_parallel(model, ["cpu"])
+    ids = torch.randint(0, 64, (1, 5))
+    with pytest.raises(ValueError, match="serving engine"):
+        wrapped.generate(ids, max_new_tokens=2, quantize="int8")
+    with pytest.raises(ValueError, match="quantize"):
+        wrapped.generate(ids, max_new_tokens=2, quantize="fp4")
+    assert wrapped.generate(ids, max_new_tokens=2, quantize="bf16").shape == (1, 7)
