@@ -308,14 +308,23 @@ bool vector_of(const Tensor& t, int64_t n) { return t.dim() == 1 && t.size(0) ==
 struct Int8Out {
   Tensor values, scales;
 };
-Int8Out int8_out(const Tensor& x) {
+// Both in one allocation (an allocation and its release cost as much as a third of a launch): values a multiple of 16 bytes apart, scales behind them.
+Int8Out int8_out(const Tensor& x, int64_t rows) {
   const int64_t cols = x.size(-1), pitch = (cols + 15) / 16 * 16;
-  const auto lead = x.sizes().slice(0, x.dim() - 1);
-  std::vector<int64_t> shape(lead.begin(), lead.end());
-  Tensor scales = at::empty(shape, x.options().dtype(at::kFloat));
-  shape.push_back(pitch);
-  Tensor values = at::empty(shape, x.options().dtype(at::kChar));
-  return {pitch == cols ? values : values.slice(-1, 0, cols), scales};
+  const Tensor room = at::empty({rows * (pitch + int64_t(sizeof(float)))}, x.options().dtype(at::kByte));
+  auto part = [&](at::ScalarType dtype, int64_t offset, at::IntArrayRef sizes, int64_t step) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(room.storage()), room.key_set(), c10::scalarTypeToTypeMeta(dtype));
+    std::vector<int64_t> strides(sizes.size(), 1);
+    for (int64_t d = int64_t(sizes.size()) - 1, next = step; d >= 0; --d) {
+      if (step > 1 && d == int64_t(sizes.size()) - 1) continue;  // (the columns of the values)
+      strides[d] = next;
+      next *= std::max<int64_t>(sizes[d], 1);
+    }
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides);
+    return t;
+  };
+  return {part(at::kChar, 0, x.sizes(), pitch), part(at::kFloat, rows * pitch / int64_t(sizeof(float)), x.sizes().slice(0, x.dim() - 1), 1)};
 }
 
 using MaybeRows = std::optional<std::tuple<Tensor, Tensor, std::optional<Tensor>>>;
@@ -334,12 +343,12 @@ MaybeRows rows_int8(const Tensor& x, const std::optional<Tensor>& weight_, const
   if (residual.defined() && (!plain(residual, dtype, x.device()) || residual.sizes() != x.sizes() || !rows_apart(residual, &residual_rows, &residual_pitch)))
     return std::nullopt;
   const c10::cuda::CUDAGuard guard(x.device());
-  const Int8Out out = int8_out(x);
+  const Int8Out out = int8_out(x, rows);
   std::optional<Tensor> sum;
   if (residual.defined()) sum = at::empty(x.sizes(), x.options());
   check(lib.rows_int8(x.const_data_ptr(), data(residual), data(weight), data(bias), sum ? sum->mutable_data_ptr() : nullptr,
                       static_cast<int8_t*>(out.values.mutable_data_ptr()), out.scales.mutable_data_ptr<float>(), int(rows), int(cols), pitch, residual_pitch, cols,
-                      (cols + 15) / 16 * 16, float(eps), int(norm) + 1, dtype == at::kFloat, 0, context(x, 0)->status, stream_of(x)),
+                      (cols + 15) / 16 * 16, float(eps), int(norm) + 1, dtype == at::kFloat, context(x, 0)->status, stream_of(x)),
         "tpb_rows_int8");
   launched.fetch_add(1, std::memory_order_relaxed);
   return std::make_tuple(out.values, out.scales, sum);

@@ -311,7 +311,7 @@ static int ip_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
   const long long tiles = (long long)p.m_tiles * p.n_tiles;
   if (tiles > 0x7fffffffLL - sms) return TPB_ERR_SIZE;
   const int pairs = int(tiles < sms / 2 ? tiles : sms / 2);
-  return launch_dependent(gemm_i8_pair_kernel<BN>, dim3(2 * pairs), dim3(IP_THREADS), S::SMEM, stream, g.early != 0, ta, tb, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  return launch_dependent(gemm_i8_pair_kernel<BN>, dim3(2 * pairs), dim3(IP_THREADS), S::SMEM, stream, true, ta, tb, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
 // Columns of the pair tile: rounds of tiles x time of a k-block, in clocks (256 x 22016 x 4096 with 256 / 128 columns 31.9 / 29.3 us, 512 x 12288 x 4096

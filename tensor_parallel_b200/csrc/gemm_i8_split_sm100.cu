@@ -264,7 +264,7 @@ static int ix_launch(const I8Gemm& g, cudaStream_t stream) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = g.early ? 2 : 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<BN, S>, tw, tx, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 

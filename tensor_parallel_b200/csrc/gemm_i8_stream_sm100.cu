@@ -329,7 +329,7 @@ static int is_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
   if (rc == TPB_OK) rc = i8_tmap(&tw1, g.w, g.features, g.k, g.ldw, IS_UNIT);
   if (rc == TPB_OK) rc = i8_tmap(&tx, g.x, g.tokens, g.k, g.ldx, BN / KS);
   if (rc != TPB_OK) return rc;
-  return launch_dependent(gemm_i8_stream_kernel<BN, NACC, KBOX, KS>, dim3(p.rows.grid), dim3(64 + IS_EPI(BN, KS)), smem, stream, g.early != 0, tw, tw1, tx, p) == cudaSuccess
+  return launch_dependent(gemm_i8_stream_kernel<BN, NACC, KBOX, KS>, dim3(p.rows.grid), dim3(64 + IS_EPI(BN, KS)), smem, stream, true, tw, tw1, tx, p) == cudaSuccess
              ? TPB_OK
              : TPB_ERR_CUDA;
 }

@@ -558,7 +558,7 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
 
 // True if the ring kernel was launched (or its launch failed: *e): there are rows for several turns of its groups, and room for two of them.
 template <typename T, int MODE>
-static bool ri_ring_launch(const RiParams& p, int sms, bool early, cudaStream_t stream, cudaError_t* e) {
+static bool ri_ring_launch(const RiParams& p, int sms, cudaStream_t stream, cudaError_t* e) {
   const size_t slot = (size_t(p.cols) * sizeof(T) + 15) / 16 * 16 + 16;  // (a row may begin in the middle of 16 bytes)
   const size_t stage = slot * (p.residual ? 2 : 1);
   const size_t params = size_t(MODE == RI_ROWS ? 0 : MODE == RI_RMS ? 1 : 2) * size_t((p.cols + 3) / 4) * 16;
@@ -579,16 +579,16 @@ static bool ri_ring_launch(const RiParams& p, int sms, bool early, cudaStream_t 
   auto go = [&](auto kernel) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(RI_RING_BYTES));
     return err != cudaSuccess ? err
-                              : launch_dependent(kernel, dim3(sms), dim3(32 * warps, groups), params + groups * stages * stage, stream, early, p, stages, int(slot), 1.f);
+                              : launch_dependent(kernel, dim3(sms), dim3(32 * warps, groups), params + groups * stages * stage, stream, true, p, stages, int(slot), 1.f);
   };
   *e = odd ? go(rows_int8_ring_kernel<T, MODE, true>) : go(rows_int8_ring_kernel<T, MODE, false>);
   return true;
 }
 
 template <typename T, int MODE, bool VEC>
-static cudaError_t ri_launch(const RiParams& p, int sms, bool early, cudaStream_t stream) {
+static cudaError_t ri_launch(const RiParams& p, int sms, cudaStream_t stream) {
   cudaError_t e;
-  if (!(VEC && p.cols <= (p.residual ? 8192 : 4096)) && ri_ring_launch<T, MODE>(p, sms, early, stream, &e)) return e;
+  if (!(VEC && p.cols <= (p.residual ? 8192 : 4096)) && ri_ring_launch<T, MODE>(p, sms, stream, &e)) return e;
   const int groups = (p.cols + 7) / 8;
   const int v = groups <= 32 ? 1 : 2;
   int threads = ((groups + v - 1) / v + 31) / 32 * 32;
@@ -596,18 +596,18 @@ static cudaError_t ri_launch(const RiParams& p, int sms, bool early, cudaStream_
   if (wide) threads = RI_MAX_THREADS;
   const int rows_per_block = threads >= 256 ? 1 : 256 / threads;
   const dim3 block(threads, rows_per_block), grid((unsigned(p.rows) + rows_per_block - 1) / rows_per_block);
-  auto go = [&](auto kernel) { return launch_dependent(kernel, grid, block, 0, stream, early, p, 1.f); };
+  auto go = [&](auto kernel) { return launch_dependent(kernel, grid, block, 0, stream, true, p, 1.f); };
   if (wide) return go(rows_int8_kernel<T, MODE, 2, VEC, true, 1024>);
   if (v == 1) return go(rows_int8_kernel<T, MODE, 1, VEC, false, 256>);
   return threads <= 256 ? go(rows_int8_kernel<T, MODE, 2, VEC, false, 256>) : go(rows_int8_kernel<T, MODE, 2, VEC, false, 1024>);
 }
 
 template <typename T>
-static cudaError_t ri_dispatch(const RiParams& p, int sms, int mode, bool early, cudaStream_t stream) {
+static cudaError_t ri_dispatch(const RiParams& p, int sms, int mode, cudaStream_t stream) {
   auto rows_aligned = [](const void* base, long long ld) { return !(reinterpret_cast<uintptr_t>(base) & 15) && (ld * sizeof(T)) % 16 == 0; };
   const bool vec = p.cols % 8 == 0 && rows_aligned(p.x, p.ldx) && rows_aligned(p.residual, p.ldr) && rows_aligned(p.sum_out, p.lds) &&
                    rows_aligned(p.weight, 0) && rows_aligned(p.bias, 0) && !(reinterpret_cast<uintptr_t>(p.q) & 7) && p.ldq % 8 == 0;
-#define RI_GO(MODE) (vec ? ri_launch<T, MODE, true>(p, sms, early, stream) : ri_launch<T, MODE, false>(p, sms, early, stream))
+#define RI_GO(MODE) (vec ? ri_launch<T, MODE, true>(p, sms, stream) : ri_launch<T, MODE, false>(p, sms, stream))
   return mode == RI_ROWS ? RI_GO(RI_ROWS) : mode == RI_RMS ? RI_GO(RI_RMS) : RI_GO(RI_LAYER);
 #undef RI_GO
 }
@@ -641,7 +641,7 @@ cudaError_t rows_int8_preload() {
 }  // namespace tpb
 
 extern "C" int tpb_rows_int8(const void* x, const void* residual, const void* weight, const void* bias, void* sum_out, int8_t* q, float* scales, int rows,
-                             int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, int early, void* status, void* stream) {
+                             int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, void* status, void* stream) {
   if (!x || !q || !scales || !status || rows <= 0 || cols <= 0 || mode < 0 || mode > 2 || dtype < 0 || dtype > 1) return TPB_ERR_ARG;
   if (mode == tpb::RI_ROWS && (residual || weight || bias || sum_out)) return TPB_ERR_ARG;
   if ((bias && mode != tpb::RI_LAYER) || (sum_out && !residual)) return TPB_ERR_ARG;
@@ -650,6 +650,6 @@ extern "C" int tpb_rows_int8(const void* x, const void* residual, const void* we
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return TPB_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == 0 ? tpb::ri_dispatch<tpb::bf16>(p, sms, mode, early != 0, s) : tpb::ri_dispatch<float>(p, sms, mode, early != 0, s);
+  const cudaError_t e = dtype == 0 ? tpb::ri_dispatch<tpb::bf16>(p, sms, mode, s) : tpb::ri_dispatch<float>(p, sms, mode, s);
   return e == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }

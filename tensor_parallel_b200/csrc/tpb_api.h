@@ -134,14 +134,14 @@ int tpb_col_sum(const void* g, void* out, float* partials, int rows, int cols, i
 // row, q * scale being x (mode 0), or the RMSNorm (1) or LayerNorm (2) of x.  q = rint(v * (127 / amax)), amax = max(max |v|, 1e-30), where v is x, x * weight
 // (RMSNorm, whose 1 / rms is in the scale alone) or the normalised row.  A row with a value that is not finite: integers 0, scale NaN.  Modes 1 and 2: weight, bias
 // (LayerNorm) and residual may be null; with residual, x + residual rounded to the type of x is normalised and stored to sum_out (may be null, or x).
-// early: launch as a programmatic dependent of the previous kernel of the stream.
+// Launched, like the product below, as a programmatic dependent of the previous kernel of the stream, and touches no memory before that kernel has finished.
 int tpb_rows_int8(const void* x, const void* residual, const void* weight, const void* bias, void* sum_out, int8_t* q, float* scales, int rows,
-                  int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, int early, void* status, void* stream);
+                  int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, void* status, void* stream);
 
 // out[t, f] = act(sx[t] sw[f] sum_k x[t, k] w[f, k] + bias[f]) + residual[t, f]: x [tokens, k] and w [features, k] 8-bit integers (16-byte aligned, row pitches
 // multiples of 16; what lies between k and the pitch is not read), sums in 32 bits, bf16 bias, residual (may be out) and out.  act as in tpb_gemm_bf16; 5
-// (rows of w: 16 gate, 16 up in turn; out has features / 2 columns) takes no residual.  k <= 131071.  early: launch as a programmatic dependent of
-// the previous kernel of the stream and read w before that kernel has finished, which must not write it.
+// (rows of w: 16 gate, 16 up in turn; out has features / 2 columns) takes no residual.  k <= 131071.  early: read w before the
+// previous kernel of the stream has finished, which must not write it.
 int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, const float* sw, void* out, const void* bias, const void* residual, int tokens,
                   int features, int k, long long ldx, long long ldw, long long ld_out, long long ld_res, int act, int early, void* status, void* stream);
 

@@ -965,7 +965,7 @@ def adamw_step(param, grad, exp_avg, exp_avg_sq, step, lr, beta1, beta2, eps, we
 # 8-bit integers: rows with a scale each, and their matrix product (serving)
 # ------------------------------------------------------------------------------------------------
 
-LIB.tpb_rows_int8.argtypes = [c_void_p] * 7 + [c_int] * 2 + [c_ll] * 4 + [c_float] + [c_int] * 3 + [c_void_p] * 2
+LIB.tpb_rows_int8.argtypes = [c_void_p] * 7 + [c_int] * 2 + [c_ll] * 4 + [c_float] + [c_int] * 2 + [c_void_p] * 2
 LIB.tpb_gemm_int8.argtypes = [c_void_p] * 7 + [c_int] * 3 + [c_ll] * 4 + [c_int] * 2 + [c_void_p] * 2
 
 
@@ -976,10 +976,9 @@ def int8_rows_empty(rows: int, cols: int, device) -> OF.Int8Rows:
     return OF.Int8Rows(values if pitch == cols else values[:, :cols], torch.empty(rows, dtype=torch.float32, device=device))
 
 
-def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, sum_out=None, out=None, early=False) -> OF.Int8Rows:
+def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, sum_out=None, out=None) -> OF.Int8Rows:
     """8-bit rows of ``x2d`` (rows of any pitch with unit inner stride) as they are, or (``norm`` 0 / 1) of the RMSNorm / LayerNorm of ``x2d + residual``, which is
-    also stored to ``sum_out`` (may be ``x2d``).  ``weight`` and ``bias`` have the type of ``x2d``.  ``out``: rows to write (:func:`int8_rows_empty`).  ``early``: see
-    :func:`gemm_nt` (nothing is read before the previous kernel has finished)."""
+    also stored to ``sum_out`` (may be ``x2d``).  ``weight`` and ``bias`` have the type of ``x2d``.  ``out``: rows to write (:func:`int8_rows_empty`)."""
     global _launches
     rows, cols = x2d.shape
     out = int8_rows_empty(rows, cols, x2d.device) if out is None else out
@@ -987,7 +986,7 @@ def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, su
         return out
     check(LIB.tpb_rows_int8(_ptr(x2d), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(sum_out), _ptr(out[0]), _ptr(out[1]), rows, cols, _pitch(x2d),
                             _pitch(residual), _pitch(sum_out), _pitch(out[0]), eps,
-                            0 if norm is None else norm + 1, _dtype_code(x2d), int(early), _ptr(device_state(x2d.device).status), _stream()), "tpb_rows_int8")
+                            0 if norm is None else norm + 1, _dtype_code(x2d), _ptr(device_state(x2d.device).status), _stream()), "tpb_rows_int8")
     _launches += 1
     return out
 
