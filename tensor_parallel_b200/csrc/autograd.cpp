@@ -280,12 +280,12 @@ Tensor norm(const Tensor& x, const std::optional<Tensor>& weight, const std::opt
 }
 
 // ---- 8-bit serving ----
-// The ordinary calls: plain CUDA tensors that fit together and lie as the kernels read them, nothing that takes a gradient, no tracing.  Every other call
+// The ordinary calls: plain CUDA tensors that fit together and lie as the kernels read them, nothing that takes a gradient or has a tangent, no tracing.  Every other call
 // gets no value here and goes on in Python, which says what is wrong with it, or makes the copies that it needs.
 
 bool plain(const Tensor& t, at::ScalarType dtype, const c10::Device& device) {
   return t.scalar_type() == dtype && t.device() == device && t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() &&
-         !(at::GradMode::is_enabled() && t.requires_grad());
+         !(at::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined();
 }
 // Rows that lie one pitch apart: their number, and the pitch (of a single row, its length rounded up).
 bool rows_apart(const Tensor& t, int64_t* rows, int64_t* pitch) {

@@ -115,30 +115,30 @@ __device__ __forceinline__ void ri_store(T* row, int base, int i, int cols, cons
   }
 }
 
-// Over the threads of a row: the sum of a, and the maximum of b (non-negative floats order as their bits do, with NaN above infinity).
+// Over the threads of a row: the sum of a, and the maximum of b (non-negative floats order as their bits do, with NaN above infinity).  `sums` and `maxima`
+// have not been used yet, or not since the last barrier.  With both, only the row's first warp gets the sum.
 template <bool SUM, bool MAX>
 __device__ __forceinline__ void ri_reduce(float& a, uint32_t& b, float* sums, uint32_t* maxima) {
+  if (MAX) b = __reduce_max_sync(0xffffffffu, b);
   if (SUM) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
   }
-  if (MAX) b = __reduce_max_sync(0xffffffffu, b);
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warps == 1) return;
   sums += threadIdx.y * warps;
   maxima += threadIdx.y * warps;
-  __syncthreads();
   if (lane == 0) {
     if (SUM) sums[warp] = a;
     if (MAX) maxima[warp] = b;
   }
   __syncthreads();
-  if (SUM) {
+  if (MAX) b = __reduce_max_sync(0xffffffffu, lane < warps ? maxima[lane] : 0u);
+  if (SUM && (!MAX || warp == 0)) {
     a = lane < warps ? sums[lane] : 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
   }
-  if (MAX) b = __reduce_max_sync(0xffffffffu, lane < warps ? maxima[lane] : 0u);
 }
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
@@ -153,16 +153,16 @@ __device__ __forceinline__ uint32_t ri_integers(float2 v0, float2 v1, float inv,
 }
 
 // Blocks that an SM is to hold.
-template <int MODE, int V, bool VEC>
+template <typename T, int MODE, int V, bool VEC>
 constexpr int ri_blocks(int threads) {
-  return threads == 256 && VEC && MODE != RI_LAYER ? (V == 1 || MODE == RI_ROWS ? 8 : 6) : 1;
+  return threads != 256 || !VEC || MODE == RI_LAYER ? 1 : V == 1 ? 6 : sizeof(T) == 4 ? 4 : MODE == RI_ROWS ? 8 : 6;
 }
 
 // A block of blockDim.y rows, blockDim.x threads each.  WIDE: rows of more than 8 V blockDim.x columns, read again from memory for every pass.
 template <typename T, int MODE, int V, bool VEC, bool WIDE, int THREADS>
-__global__ void __launch_bounds__(THREADS, ri_blocks<MODE, V, VEC>(THREADS))
+__global__ void __launch_bounds__(THREADS, ri_blocks<T, MODE, V, VEC>(THREADS))
 rows_int8_kernel(const RiParams p, float one) {
-  __shared__ float sums[32];
+  __shared__ float sums[2][32];
   __shared__ uint32_t maxima[32];
   const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
   const int cols = row < p.rows ? p.cols : 0;  // (a row past the end still takes part in the block's barriers)
@@ -262,7 +262,7 @@ rows_int8_kernel(const RiParams p, float one) {
   uint32_t most = 0;
   if (MODE == RI_LAYER) {
     // (the deviations are summed up around the mean: a difference of two sums would lose the digits that they share)
-    ri_reduce<true, false>(sum, most, sums, maxima);
+    ri_reduce<true, false>(sum, most, sums[0], maxima);
     mean = sum / float(p.cols);
     float squares = 0.f;
     for (int base = 0; base < end; base += chunk) {
@@ -277,7 +277,7 @@ rows_int8_kernel(const RiParams p, float one) {
         }
       }
     }
-    ri_reduce<true, false>(squares, most, sums, maxima);
+    ri_reduce<true, false>(squares, most, sums[1], maxima);
     rstd = rsqrtf(squares / float(p.cols) + p.eps);
     for (int base = 0; base < end; base += chunk) {
       if (WIDE) fetch(base, true);
@@ -285,7 +285,7 @@ rows_int8_kernel(const RiParams p, float one) {
     }
   }
   most = __float_as_uint(fmax3_abs_nan(most0, most1, 0.f));
-  ri_reduce<MODE == RI_RMS, true>(sum, most, sums, maxima);
+  ri_reduce<MODE == RI_RMS, true>(sum, most, sums[0], maxima);
 
   const bool finite = most < 0x7F800000u;
   const float amax = fmaxf(__uint_as_float(most), RI_LEAST);
@@ -643,6 +643,7 @@ cudaError_t rows_int8_preload() {
 extern "C" int tpb_rows_int8(const void* x, const void* residual, const void* weight, const void* bias, void* sum_out, int8_t* q, float* scales, int rows,
                              int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, void* status, void* stream) {
   if (!x || !q || !scales || !status || rows <= 0 || cols <= 0 || mode < 0 || mode > 2 || dtype < 0 || dtype > 1) return TPB_ERR_ARG;
+  if (cols > 1 << 30) return TPB_ERR_SIZE;
   if (mode == tpb::RI_ROWS && (residual || weight || bias || sum_out)) return TPB_ERR_ARG;
   if ((bias && mode != tpb::RI_LAYER) || (sum_out && !residual)) return TPB_ERR_ARG;
   if (ldx < cols || ldq < cols || (residual && ldr < cols) || (sum_out && lds < cols)) return TPB_ERR_ARG;

@@ -306,6 +306,8 @@ def geglu(gate, up, approximate: str = "tanh"):
 def _serving_only(what: str, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+    if any(t is not None and t.is_floating_point() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no derivative, in forward mode neither")
 
 
 def _check_rows(what: str, x, weight=None, bias=None, residual=None):
@@ -330,7 +332,7 @@ def quantize_int8(x) -> Int8Rows:
     if out is not None:
         return out
     _check_rows("quantize_int8", x)
-    return quantize_int8_ref(x) if nat is None or torch._C._is_tracing() else nat.quantize_int8(x)
+    return quantize_int8_ref(x) if nat is None or transformed(x) else nat.quantize_int8(x)
 
 
 def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
@@ -341,7 +343,7 @@ def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows
     if out is not None:
         return out
     _check_rows("rms_norm_int8", x, weight, residual=residual)
-    return rms_norm_int8_ref(x, weight, eps, residual) if nat is None or torch._C._is_tracing() else nat.norm_int8(x, weight, None, eps, 0, residual)
+    return rms_norm_int8_ref(x, weight, eps, residual) if nat is None or transformed(x) else nat.norm_int8(x, weight, None, eps, 0, residual)
 
 
 def layer_norm_int8(x, weight, bias, eps: float = 1e-5, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
@@ -351,7 +353,7 @@ def layer_norm_int8(x, weight, bias, eps: float = 1e-5, residual=None) -> Tuple[
     if out is not None:
         return out
     _check_rows("layer_norm_int8", x, weight, bias, residual)
-    return layer_norm_int8_ref(x, weight, bias, eps, residual) if nat is None or torch._C._is_tracing() else nat.norm_int8(x, weight, bias, eps, 1, residual)
+    return layer_norm_int8_ref(x, weight, bias, eps, residual) if nat is None or transformed(x) else nat.norm_int8(x, weight, bias, eps, 1, residual)
 
 
 _INT8_ACTS = (None, "relu", "gelu", "gelu_tanh", "silu", "swiglu16")
@@ -389,7 +391,7 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias=None, act: Optional[str] = N
     if out is not None:
         return out
     _check_linear_int8(x, weight, bias, act, residual)
-    if nat is None or torch._C._is_tracing():
+    if nat is None or transformed(x[0]) or transformed(x[1]):
         return linear_int8_ref(Int8Rows(*x), Int8Rows(*weight), bias, act, residual)
     return nat.linear_int8(x, weight, bias, act, residual)
 

@@ -969,6 +969,12 @@ LIB.tpb_rows_int8.argtypes = [c_void_p] * 7 + [c_int] * 2 + [c_ll] * 4 + [c_floa
 LIB.tpb_gemm_int8.argtypes = [c_void_p] * 7 + [c_int] * 3 + [c_ll] * 4 + [c_int] * 2 + [c_void_p] * 2
 
 
+def _int32(what: str, *sizes):
+    if max(sizes) >= 2 ** 31:
+        raise ValueError(f"{what}: sizes {sizes} beyond 2^31")
+    return sizes
+
+
 def int8_rows_empty(rows: int, cols: int, device) -> OF.Int8Rows:
     """Room for 8-bit rows that lie a multiple of 16 bytes apart."""
     pitch = (cols + 15) // 16 * 16
@@ -980,7 +986,7 @@ def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, su
     """8-bit rows of ``x2d`` (rows of any pitch with unit inner stride) as they are, or (``norm`` 0 / 1) of the RMSNorm / LayerNorm of ``x2d + residual``, which is
     also stored to ``sum_out`` (may be ``x2d``).  ``weight`` and ``bias`` have the type of ``x2d``.  ``out``: rows to write (:func:`int8_rows_empty`)."""
     global _launches
-    rows, cols = x2d.shape
+    rows, cols = _int32("rows_int8", *x2d.shape)
     out = int8_rows_empty(rows, cols, x2d.device) if out is None else out
     if rows == 0:
         return out
@@ -1048,8 +1054,7 @@ def gemm_int8(x: OF.Int8Rows, weight: OF.Int8Rows, bias=None, act=None, residual
     """``act(x @ weight.T + bias) + residual`` of 8-bit rows ``[tokens, k]`` and ``[features, k]``, bf16.  ``residual`` may be ``out``.  ``early``: see :func:`gemm_nt`."""
     global _launches
     (xv, sx), (given, sw) = x, weight
-    tokens, k = xv.shape
-    features = given.shape[0]
+    tokens, k, features = _int32("gemm_int8", *xv.shape, given.shape[0])
     xv, wv = _int8_ready(xv), _int8_ready(given)
     cols = features // 2 if act == "swiglu16" else features
     out = torch.empty(tokens, cols, dtype=torch.bfloat16, device=xv.device) if out is None else out

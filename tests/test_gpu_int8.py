@@ -395,3 +395,88 @@ def test_a_gated_mlp_in_8_bits():
     n = OF.rms_norm_ref(h, gamma, 1e-5).double()
     exact = (torch.nn.functional.silu(n @ wg.double().t()) * (n @ wu.double().t())) @ wd.double().t() + h.double()
     assert (out.double() - exact).norm() < 0.25 * (exact - h.double()).norm()
+
+
+def test_offsets_beyond_32_bits():
+    rows, cols = 70001, 32768  # 2.3 G elements
+    x = torch.zeros(rows, cols, dtype=BF16, device="cuda")
+    some = torch.tensor([0, 1, 65535, 65536, 65537, 69999, 70000], device="cuda")
+    x[some] = _wave(len(some), cols, BF16, 100)
+    q, s = OF.quantize_int8(x)
+    want = OF.quantize_int8_ref(x[some])
+    assert torch.equal(q[some], want.values) and torch.equal(s[some], want.scales)
+    assert not q[2:65535:4099].any()
+    (nq, ns), h = OF.rms_norm_int8(x, None, 1e-6, x)
+    (wq, ws), wh = OF.rms_norm_int8_ref(x[some], None, 1e-6, x[some])
+    assert torch.equal(nq[some], wq) and torch.equal(h[some], wh)
+    torch.testing.assert_close(ns[some], ws, rtol=64 * 2.0 ** -24, atol=0)
+    del h, nq, ns
+    w = OF.quantize_int8_ref(torch.randn(40, cols, device="cuda", generator=_gen(101)))
+    out = OF.linear_int8(OF.Int8Rows(q, s), w)
+    assert torch.equal(out[some], OF.linear_int8(OF.Int8Rows(q[some].contiguous(), s[some]), w)) and not out[2:65535:4099].any()
+    del q, s, x, out
+    tokens, features, k = 131077, 20000, 64  # 2.6 G results
+    x, w = _operands(tokens, features, k, 102)
+    out = OF.linear_int8(x, w)
+    some = torch.tensor([0, 127, 107373, 107374, 107375, 131071, 131072, 131076], device="cuda")
+    assert torch.equal(out[some], OF.linear_int8(OF.Int8Rows(x.values[some].contiguous(), x.scales[some]), w))
+
+
+def test_strided_leading_dimensions():
+    x = _wave(40, 96, BF16, 110).view(4, 10, 96)
+    for t in (x[:, ::2], x.transpose(0, 1), x[::2], x[:, 3:4], x[1:2, :, :], x[..., 16:80], x[..., 5:70]):
+        got, want = OF.quantize_int8(t), OF.quantize_int8_ref(t)
+        assert got.values.shape == t.shape and torch.equal(got.values, want.values) and torch.equal(got.scales, want.scales)
+        (q, s), h = OF.rms_norm_int8(t, None, 1e-6, t)
+        assert torch.equal(h, (t.float() * 2).to(BF16)) and torch.equal(q, want.values)
+    w = OF.quantize_int8(_wave(64, 96, BF16, 111))
+    r = OF.quantize_int8(x)
+    for at in ((slice(None), slice(None, None, 2)), (slice(1, 3),), (slice(None), slice(4, 5))):
+        part = OF.Int8Rows(r.values[at], r.scales[at])
+        residual = _wave(part.scales.numel(), 64, BF16, 112).view(*part.scales.shape, 64)
+        assert torch.equal(OF.linear_int8(part, w), OF.linear_int8(r, w)[at])
+        want = OF.linear_int8_ref(part, w, residual=residual).float()
+        torch.testing.assert_close(OF.linear_int8(part, w, residual=residual).float(), want, rtol=2.0 ** -7, atol=1e-4)  # a rounding to bf16 on either side
+
+
+def test_under_transforms_tracing_and_tangents():
+    x = _wave(6, 64, BF16, 120)
+    want = OF.quantize_int8_ref(x)
+    got = torch.vmap(lambda t: tuple(OF.quantize_int8(t)))(x.view(2, 3, 64))
+    assert torch.equal(got[0].reshape(6, 64), want.values) and torch.equal(got[1].reshape(6), want.scales)
+    traced = torch.jit.trace(lambda t: tuple(OF.quantize_int8(t)), (x,))
+    y = _wave(6, 64, BF16, 121)
+    assert torch.equal(traced(y)[0], OF.quantize_int8_ref(y).values)  # (its steps, not its first result)
+    import torch.autograd.forward_ad as fwd
+
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="no derivative"):
+            OF.quantize_int8(dual)
+        with pytest.raises(RuntimeError, match="no derivative"):
+            OF.rms_norm_int8(x, None, 1e-6, residual=dual)
+    with torch.inference_mode():
+        got = OF.quantize_int8(x)
+        assert torch.equal(got.values, want.values) and got.values.is_inference()
+        got.values.zero_()
+
+
+def test_a_weight_of_another_type_and_rows_as_a_plain_pair():
+    x = _wave(5, 64, BF16, 130)
+    w = 1 + 0.1 * torch.randn(64, device="cuda", generator=_gen(131))
+    (q, s), _ = OF.rms_norm_int8(x, w, 1e-6)
+    (wq, ws), _ = OF.rms_norm_int8_ref(x, w, 1e-6)
+    assert torch.equal(q, wq)
+    rows, weight = OF.quantize_int8(x), OF.quantize_int8(_wave(32, 64, BF16, 132))
+    assert torch.equal(OF.linear_int8(tuple(rows), tuple(weight)), OF.linear_int8(rows, weight))
+
+
+@pytest.mark.multigpu
+def test_tensors_on_another_device_than_the_current_one():
+    x, w = _operands(9, 64, 128, 140)
+    y = _wave(9, 128, BF16, 141)
+    want, rows = OF.linear_int8(x, w), OF.quantize_int8(y)
+    with torch.cuda.device(0):
+        far = [OF.Int8Rows(t.values.to("cuda:1"), t.scales.to("cuda:1")) for t in (x, w)]
+        out, got = OF.linear_int8(*far), OF.quantize_int8(y.to("cuda:1"))
+    assert out.device.index == 1 and torch.equal(out.cpu(), want.cpu()) and torch.equal(got.values.cpu(), rows.values.cpu())

@@ -169,6 +169,16 @@ def test_no_tokens():
     assert q.shape == (0, 3, 64) and s.shape == (0, 3)
 
 
+def test_tangents_are_refused_and_batches_go_through_the_steps():
+    import torch.autograd.forward_ad as fwd
+
+    x = torch.randn(4, 8)
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="no derivative"):
+        OF.quantize_int8(fwd.make_dual(x, torch.ones_like(x)))
+    got = torch.vmap(lambda t: tuple(OF.quantize_int8(t)))(x)
+    assert torch.equal(got[0], OF.quantize_int8(x).values)
+
+
 def test_generation_in_8_bits_needs_the_engine():
     import tensor_parallel_b200 as tp
     from tensor_parallel_b200.models.llama import LlamaConfig, LlamaForCausalLM
