@@ -51,7 +51,7 @@ template <> struct Ri8<bf16> {
   __device__ __forceinline__ float get(int j) const { return __uint_as_float(j & 1 ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16); }
   __device__ __forceinline__ void set2(int j, float a, float b) { w[j >> 1] = pack_bf16x2(a, b); }
   __device__ __forceinline__ bf16 element(int j) const { return __ushort_as_bfloat16(uint16_t(w[j >> 1] >> (16 * (j & 1)))); }
-  __device__ __forceinline__ void pair(int j, bf16 a, bf16 b) { w[j >> 1] = uint32_t(__bfloat16_as_ushort(a)) | uint32_t(__bfloat16_as_ushort(b)) << 16; }
+  __device__ __forceinline__ void clear(int j) { w[j >> 1] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u; }
 };
 template <> struct Ri8<float> {
   static constexpr int WORDS = 8;
@@ -59,7 +59,7 @@ template <> struct Ri8<float> {
   __device__ __forceinline__ float get(int j) const { return __uint_as_float(w[j]); }
   __device__ __forceinline__ void set2(int j, float a, float b) { w[j] = __float_as_uint(a); w[j + 1] = __float_as_uint(b); }
   __device__ __forceinline__ float element(int j) const { return __uint_as_float(w[j]); }
-  __device__ __forceinline__ void pair(int j, float a, float b) { set2(j, a, b); }
+  __device__ __forceinline__ void clear(int j) { w[j] = 0; }
 };
 template <typename T>
 __device__ __forceinline__ Ri8<T> ri_load8(const T* at, bool ok) {  // 16-byte aligned
@@ -80,38 +80,53 @@ __device__ __forceinline__ void ri_store8(T* at, const Ri8<T>& r) {
   for (int u = 0; u < Ri8<T>::WORDS / 4; ++u) reinterpret_cast<uint4*>(at)[u] = make_uint4(r.w[4 * u], r.w[4 * u + 1], r.w[4 * u + 2], r.w[4 * u + 3]);
 }
 
-// Columns of a thread: V groups of 8.  VEC: 8 consecutive columns each, rows on 16-byte boundaries; else the lanes of a warp own consecutive
-// columns, so that rows of any width and alignment are read and written in whole sectors.
-template <bool VEC>
-__device__ __forceinline__ int ri_col(int base, int i, int j) {
-  return VEC ? base + (int(threadIdx.x) + i * int(blockDim.x)) * 8 + j : base + int(threadIdx.x) + (i * 8 + j) * int(blockDim.x);
-}
+// Columns of a thread: V groups of 8 consecutive ones.
+__device__ __forceinline__ int ri_col(int base, int i) { return base + (int(threadIdx.x) + i * int(blockDim.x)) * 8; }
+
+// 8 columns of a row from column c on, zeros past its end.  VEC: rows begin on 16 bytes and have a multiple of 8 columns.  Else the columns are taken out of the
+// aligned 16-byte blocks that hold them (and a few bytes of their neighbours, which lie in the same blocks), which costs two instructions per element.
 template <typename T, bool VEC>
-__device__ __forceinline__ Ri8<T> ri_load(const T* row, int base, int i, int cols) {
-  if constexpr (VEC) {
-    const int c = ri_col<true>(base, i, 0);
-    return ri_load8(row + c, c < cols);
-  } else {
-    Ri8<T> r;
+__device__ __forceinline__ Ri8<T> ri_load(const T* row, int c, int cols) {
+  if constexpr (VEC) return ri_load8(row + c, c < cols);
+  constexpr int BLOCKS = sizeof(T) / 2 + 1, WORDS = Ri8<T>::WORDS;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + c), end = reinterpret_cast<uintptr_t>(row + cols);
+  const uint32_t skip = uint32_t(at) & 15;  // (the same for all groups of a row)
+  uint32_t w[4 * BLOCKS];
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const int c = ri_col<false>(base, i, j), d = ri_col<false>(base, i, j + 1);
-      r.pair(j, c < cols ? row[c] : ri_round<T>(0.f), d < cols ? row[d] : ri_round<T>(0.f));
-    }
-    return r;
+  for (int u = 0; u < BLOCKS; ++u) {
+    const uintptr_t block = at - skip + 16 * u;
+    const uint4 q = c < cols && block < end ? *reinterpret_cast<const uint4*>(block) : make_uint4(0, 0, 0, 0);
+    w[4 * u] = q.x;
+    w[4 * u + 1] = q.y;
+    w[4 * u + 2] = q.z;
+    w[4 * u + 3] = q.w;
   }
+  if (skip & 4) {
+#pragma unroll
+    for (int i = 0; i + 1 < 4 * BLOCKS; ++i) w[i] = w[i + 1];
+  }
+  if (skip & 8) {
+#pragma unroll
+    for (int i = 0; i + 2 < 4 * BLOCKS; ++i) w[i] = w[i + 2];
+  }
+  Ri8<T> r;
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) r.w[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], (skip & 2) * 8);
+  if (c + 8 > cols) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j >= cols) r.clear(j);
+  }
+  return r;
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void ri_store(T* row, int base, int i, int cols, const Ri8<T>& r) {
+__device__ __forceinline__ void ri_store(T* row, int c, int cols, const Ri8<T>& r) {
   if constexpr (VEC) {
-    const int c = ri_col<true>(base, i, 0);
     if (c < cols) ri_store8(row + c, r);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = ri_col<false>(base, i, j);
-      if (c < cols) row[c] = r.element(j);
-    }
+    for (int j = 0; j < 8; ++j)
+      if (c + j < cols) row[c + j] = r.element(j);
   }
 }
 
@@ -155,7 +170,7 @@ __device__ __forceinline__ uint32_t ri_integers(float2 v0, float2 v1, float inv,
 // Blocks that an SM is to hold.
 template <typename T, int MODE, int V, bool VEC>
 constexpr int ri_blocks(int threads) {
-  return threads != 256 || !VEC || MODE == RI_LAYER ? 1 : V == 1 ? 6 : sizeof(T) == 4 ? 4 : MODE == RI_ROWS ? 8 : 6;
+  return threads != 256 || !VEC ? 1 : MODE == RI_LAYER ? 4 : V == 1 ? 6 : sizeof(T) == 4 ? 4 : MODE == RI_ROWS ? 8 : 6;
 }
 
 // A block of blockDim.y rows, blockDim.x threads each.  WIDE: rows of more than 8 V blockDim.x columns, read again from memory for every pass.
@@ -180,22 +195,22 @@ rows_int8_kernel(const RiParams p, float one) {
     // (x may be overwritten by the sum: a second pass reads what this thread stored)
     const bool summed = again && residual && sum_out;
 #pragma unroll
-    for (int i = 0; i < V; ++i) raw[i] = ri_load<T, VEC>(summed ? sum_out : x, base, i, cols);
+    for (int i = 0; i < V; ++i) raw[i] = ri_load<T, VEC>(summed ? sum_out : x, ri_col(base, i), cols);
     if (MODE != RI_ROWS && residual && !summed) {
       Ri8<T> add[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) add[i] = ri_load<T, VEC>(residual, base, i, cols);
+      for (int i = 0; i < V; ++i) add[i] = ri_load<T, VEC>(residual, ri_col(base, i), cols);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         // rounded to the type it is stored in: the norm is taken of what later kernels read
 #pragma unroll
         for (int j = 0; j < 8; j += 2) raw[i].set2(j, raw[i].get(j) + add[i].get(j), raw[i].get(j + 1) + add[i].get(j + 1));
-        if (sum_out) ri_store<T, VEC>(sum_out, base, i, cols, raw[i]);
+        if (sum_out) ri_store<T, VEC>(sum_out, ri_col(base, i), cols, raw[i]);
       }
     }
     if (MODE != RI_ROWS && weight) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = ri_load<T, VEC>(weight, base, i, cols);
+      for (int i = 0; i < V; ++i) w[i] = ri_load<T, VEC>(weight, ri_col(base, i), cols);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -219,14 +234,14 @@ rows_int8_kernel(const RiParams p, float one) {
       }
       if (MODE == RI_LAYER) {
         if (bias) {
-          const Ri8<T> b = ri_load<T, VEC>(bias, base, i, cols);
+          const Ri8<T> b = ri_load<T, VEC>(bias, ri_col(base, i), cols);
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[i][j] = __fadd2_rn(v[i][j], make_float2(b.get(2 * j), b.get(2 * j + 1)));
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (ri_col<VEC>(base, i, 2 * j) >= cols) v[i][j].x = 0.f;
-          if (ri_col<VEC>(base, i, 2 * j + 1) >= cols) v[i][j].y = 0.f;
+          if (ri_col(base, i) + 2 * j >= cols) v[i][j].x = 0.f;
+          if (ri_col(base, i) + 2 * j + 1 >= cols) v[i][j].y = 0.f;
         }
       }
 #pragma unroll
@@ -272,8 +287,8 @@ rows_int8_kernel(const RiParams p, float one) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float a = v[i][j].x - mean, b = v[i][j].y - mean;
-          if (ri_col<VEC>(base, i, 2 * j) < cols) squares += a * a;
-          if (ri_col<VEC>(base, i, 2 * j + 1) < cols) squares += b * b;
+          if (ri_col(base, i) + 2 * j < cols) squares += a * a;
+          if (ri_col(base, i) + 2 * j + 1 < cols) squares += b * b;
         }
       }
     }
@@ -295,6 +310,7 @@ rows_int8_kernel(const RiParams p, float one) {
     p.scales[row] = finite ? scale : __int_as_float(0x7FC00000);
   }
   int8_t* q = p.q + row * p.ldq;
+  const bool whole = VEC || !((reinterpret_cast<uintptr_t>(p.q) | uintptr_t(p.ldq)) & 7);  // 8 integers may be stored at once
   for (int base = 0; base < end; base += chunk) {
     if (WIDE) {
       fetch(base, true);
@@ -304,15 +320,13 @@ rows_int8_kernel(const RiParams p, float one) {
     for (int i = 0; i < V; ++i) {
       uint2 u = make_uint2(ri_integers(v[i][0], v[i][1], inv, one), ri_integers(v[i][2], v[i][3], inv, one));
       if (!finite) u = make_uint2(0, 0);
-      if constexpr (VEC) {
-        const int c = ri_col<true>(base, i, 0);
+      const int c = ri_col(base, i);
+      if (VEC || (whole && c + 8 <= cols)) {
         if (c < cols) *reinterpret_cast<uint2*>(q + c) = u;
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = ri_col<false>(base, i, j);
-          if (c < cols) q[c] = int8_t((j < 4 ? u.x : u.y) >> (8 * (j & 3)));
-        }
+        for (int j = 0; j < 8; ++j)
+          if (c + j < cols) q[c + j] = int8_t((j < 4 ? u.x : u.y) >> (8 * (j & 3)));
       }
     }
   }
@@ -355,9 +369,7 @@ template <> struct Ri4<float> {
 // fills by bulk copies.  A row is read from its slot once for its statistics and once for its integers, so that registers limit neither its width nor the
 // rows in flight.  What bounds the kernel beside the bytes is instructions, a third of which are a row's and not an element's: few threads per row (one warp,
 // without barriers, where the slots of a block suffice for a dozen), fp32 arithmetic on two values at a time, weights as fp32 in shared memory.
-// ODD: rows that begin or end within a quad are read and written element by element.  `one` is 1: y * one + 1.5 2^23 rounds like a sum, which the compiler
-// would contract with the product in front of it.
-template <typename T, int MODE, bool ODD>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(RI_MAX_THREADS, 1)
 rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
   extern __shared__ __align__(128) uint8_t ri_smem[];
@@ -367,7 +379,7 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
   __shared__ uint32_t abort_word;
   volatile uint32_t* abort_flag = &abort_word;
   const int group = threadIdx.y, groups = blockDim.y, tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
-  const int quads = (p.cols + 3) / 4;
+  const int quads = p.cols / 4;
   uint64_t* full = full_bars + group * stages;
   const bool two = MODE != RI_ROWS && p.residual;
   const int stage_bytes = slot_bytes * (two ? 2 : 1);
@@ -426,8 +438,8 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
     const T* weight = static_cast<const T*>(p.weight);
     const T* bias = static_cast<const T*>(p.bias);
     for (int c = group * threads + tid; c < 4 * quads; c += groups * threads) {
-      weights[c] = c >= p.cols ? 0.f : weight ? ri_float(weight[c]) : 1.f;
-      if (MODE == RI_LAYER) biases[c] = c < p.cols && bias ? ri_float(bias[c]) : 0.f;
+      weights[c] = weight ? ri_float(weight[c]) : 1.f;
+      if (MODE == RI_LAYER) biases[c] = bias ? ri_float(bias[c]) : 0.f;
     }
   }
   __syncthreads();
@@ -445,23 +457,11 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
     const T* rs = two ? reinterpret_cast<const T*>(slot + slot_bytes) + ri_span(static_cast<const T*>(p.residual) + row * p.ldr, p.cols, &unused, &n) : nullptr;
     T* sum_out = two && p.sum_out ? static_cast<T*>(p.sum_out) + row * p.lds : nullptr;
     struct Quad { float2 a, b; };
-    auto element = [&](int c) { return c < p.cols ? ri_float(xs[c]) : 0.f; };
     auto get = [&](int q) -> Quad {
-      if constexpr (ODD) return {make_float2(element(4 * q), element(4 * q + 1)), make_float2(element(4 * q + 2), element(4 * q + 3))};
       const Ri4<T> x = *reinterpret_cast<const Ri4<T>*>(xs + 4 * q);
       return {x.low(), x.high()};
     };
     auto get_sum = [&](int q) -> Quad {  // h, which takes the place of x
-      if constexpr (ODD) {
-#pragma unroll
-        for (int c = 4 * q; c < 4 * q + 4; ++c) {
-          if (c >= p.cols) break;
-          const T h = ri_round<T>(ri_float(xs[c]) + ri_float(rs[c]));
-          xs[c] = h;
-          if (sum_out) sum_out[c] = h;
-        }
-        return get(q);
-      }
       Ri4<T> x = *reinterpret_cast<const Ri4<T>*>(xs + 4 * q);
       const Ri4<T> r = *reinterpret_cast<const Ri4<T>*>(rs + 4 * q);
       // rounded to the type it is stored in: the norm is taken of what later kernels read
@@ -510,15 +510,10 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
         Quad h = get(q);
         h.a = __fadd2_rn(h.a, both(-mean));
         h.b = __fadd2_rn(h.b, both(-mean));
-        if (ODD) {
-          if (4 * q + 1 >= p.cols) h.a.y = 0.f;
-          if (4 * q + 2 >= p.cols) h.b.x = 0.f;
-          if (4 * q + 3 >= p.cols) h.b.y = 0.f;
-        }
         squares = __ffma2_rn(h.b, h.b, __ffma2_rn(h.a, h.a, squares));
       });
       rstd = rsqrtf(total(squares.x + squares.y, 1) / float(p.cols) + p.eps);
-      each([&](int q) { raise(value(q, get(q))); });  // (past the end the weight and the bias are zero)
+      each([&](int q) { raise(value(q, get(q))); });
     }
     uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(fmax3_abs_nan(most0, most1, 0.f)));
     if (warps > 1 && lane == 0) maxima[group * warps + warp] = most;
@@ -537,11 +532,7 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
       const Quad v = value(q, get(q));
       uint32_t four = ri_integers(v.a, v.b, inv, one);
       if (!finite) four = 0;
-      if (!ODD || 4 * q + 4 <= p.cols) {
-        *reinterpret_cast<uint32_t*>(out + 4 * q) = four;
-      } else {
-        for (int c = 4 * q; c < p.cols; ++c, four >>= 8) out[c] = int8_t(four & 0xFFu);
-      }
+      *reinterpret_cast<uint32_t*>(out + 4 * q) = four;
     });
     if (two) fence_proxy_async_smem();  // (h was written to the slot that a bulk copy fills next)
     meet();
@@ -556,13 +547,18 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
   }
 }
 
-// True if the ring kernel was launched (or its launch failed: *e): there are rows for several turns of its groups, and room for two of them.
+// True if the ring kernel was launched (or its launch failed: *e): rows that begin and end on a quad's boundary, enough of them for every SM, and room for two.
+// For rows wide enough; narrower ones have more of them in flight with a block each (us, ring / block per row: 8192 x 4096 24.1 / 17.9, RMSNorm 26.1 / 24.8, with a
+// residual 4096 x 8192 45.2 / 42.7; 4096 x 11008 25.9 / 30.7, RMSNorm 35 / 58, 4096 x 16384 35 / 56).
 template <typename T, int MODE>
 static bool ri_ring_launch(const RiParams& p, int sms, cudaStream_t stream, cudaError_t* e) {
   const size_t slot = (size_t(p.cols) * sizeof(T) + 15) / 16 * 16 + 16;  // (a row may begin in the middle of 16 bytes)
   const size_t stage = slot * (p.residual ? 2 : 1);
   const size_t params = size_t(MODE == RI_ROWS ? 0 : MODE == RI_RMS ? 1 : 2) * size_t((p.cols + 3) / 4) * 16;
-  if (params + 2 * stage > RI_RING_BYTES || p.rows < 2 * sms) return false;
+  auto whole = [](const void* base, long long ld) { return reinterpret_cast<uintptr_t>(base) % (4 * sizeof(T)) == 0 && ld % 4 == 0; };
+  if (p.cols <= (p.residual || MODE == RI_LAYER ? 8192 : 4096) || p.rows < 2 * sms || params + 2 * stage > RI_RING_BYTES || p.cols % 4 || !whole(p.x, p.ldx) ||
+      !whole(p.residual, p.ldr) || !whole(p.sum_out, p.lds) || (reinterpret_cast<uintptr_t>(p.q) & 3) || p.ldq % 4)
+    return false;
   size_t slots = (RI_RING_BYTES - params) / stage;
   if (slots > RI_RING_BARS) slots = RI_RING_BARS;
   int groups = int(slots / 2);
@@ -574,21 +570,19 @@ static bool ri_ring_launch(const RiParams& p, int sms, cudaStream_t stream, cuda
   if (warps > 1 && groups > 15) groups = 15;  // (named barriers)
   int stages = int(slots / groups);
   if (stages > 4) stages = 4;
-  auto whole = [](const void* base, long long ld) { return reinterpret_cast<uintptr_t>(base) % (4 * sizeof(T)) == 0 && ld % 4 == 0; };
-  const bool odd = p.cols % 4 || !whole(p.x, p.ldx) || !whole(p.residual, p.ldr) || !whole(p.sum_out, p.lds) || (reinterpret_cast<uintptr_t>(p.q) & 3) || p.ldq % 4;
   auto go = [&](auto kernel) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(RI_RING_BYTES));
     return err != cudaSuccess ? err
                               : launch_dependent(kernel, dim3(sms), dim3(32 * warps, groups), params + groups * stages * stage, stream, true, p, stages, int(slot), 1.f);
   };
-  *e = odd ? go(rows_int8_ring_kernel<T, MODE, true>) : go(rows_int8_ring_kernel<T, MODE, false>);
+  *e = go(rows_int8_ring_kernel<T, MODE>);
   return true;
 }
 
 template <typename T, int MODE, bool VEC>
 static cudaError_t ri_launch(const RiParams& p, int sms, cudaStream_t stream) {
   cudaError_t e;
-  if (!(VEC && p.cols <= (p.residual ? 8192 : 4096)) && ri_ring_launch<T, MODE>(p, sms, stream, &e)) return e;
+  if (ri_ring_launch<T, MODE>(p, sms, stream, &e)) return e;
   const int groups = (p.cols + 7) / 8;
   const int v = groups <= 32 ? 1 : 2;
   int threads = ((groups + v - 1) / v + 31) / 32 * 32;
@@ -617,8 +611,7 @@ static cudaError_t ri_preload() {
   cudaFuncAttributes attr;
   cudaError_t e = cudaSuccess;
 #define LOAD(...) if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, __VA_ARGS__)
-  LOAD(rows_int8_ring_kernel<T, MODE, true>);
-  LOAD(rows_int8_ring_kernel<T, MODE, false>);
+  LOAD(rows_int8_ring_kernel<T, MODE>);
   LOAD(rows_int8_kernel<T, MODE, 2, true, true, 1024>);
   LOAD(rows_int8_kernel<T, MODE, 2, false, true, 1024>);
   LOAD(rows_int8_kernel<T, MODE, 1, true, false, 256>);
