@@ -50,7 +50,6 @@ template <> struct Ri8<bf16> {
   uint32_t w[4];
   __device__ __forceinline__ float get(int j) const { return __uint_as_float(j & 1 ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16); }
   __device__ __forceinline__ void set2(int j, float a, float b) { w[j >> 1] = pack_bf16x2(a, b); }
-  __device__ __forceinline__ bf16 element(int j) const { return __ushort_as_bfloat16(uint16_t(w[j >> 1] >> (16 * (j & 1)))); }
   __device__ __forceinline__ void clear(int j) { w[j >> 1] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u; }
 };
 template <> struct Ri8<float> {
@@ -58,7 +57,6 @@ template <> struct Ri8<float> {
   uint32_t w[8];
   __device__ __forceinline__ float get(int j) const { return __uint_as_float(w[j]); }
   __device__ __forceinline__ void set2(int j, float a, float b) { w[j] = __float_as_uint(a); w[j + 1] = __float_as_uint(b); }
-  __device__ __forceinline__ float element(int j) const { return __uint_as_float(w[j]); }
   __device__ __forceinline__ void clear(int j) { w[j] = 0; }
 };
 template <typename T>
@@ -119,14 +117,21 @@ __device__ __forceinline__ Ri8<T> ri_load(const T* row, int c, int cols) {
   }
   return r;
 }
+// The same 8 columns back.  Rows of any alignment are turned in the warp's part of shared memory, so that neighbouring lanes store neighbouring columns.
 template <typename T, bool VEC>
-__device__ __forceinline__ void ri_store(T* row, int c, int cols, const Ri8<T>& r) {
+__device__ __forceinline__ void ri_store(T* row, int c, int cols, const Ri8<T>& r, T* stage) {
   if constexpr (VEC) {
     if (c < cols) ri_store8(row + c, r);
   } else {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    ri_store8(stage + lane * 8, r);
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < cols) row[c + j] = r.element(j);
+    for (int j = 0; j < 8; ++j) {
+      const int d = c - lane * 8 + 32 * j + lane;
+      if (d < cols) row[d] = stage[32 * j + lane];
+    }
   }
 }
 
@@ -179,6 +184,8 @@ __global__ void __launch_bounds__(THREADS, ri_blocks<T, MODE, V, VEC>(THREADS))
 rows_int8_kernel(const RiParams p, float one) {
   __shared__ float sums[2][32];
   __shared__ uint32_t maxima[32];
+  __shared__ __align__(16) T turned[VEC || MODE == RI_ROWS ? 1 : THREADS * 8];
+  T* stage = turned + (VEC || MODE == RI_ROWS ? 0 : (threadIdx.y * blockDim.x + threadIdx.x) / 32 * 256);
   const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
   const int cols = row < p.rows ? p.cols : 0;  // (a row past the end still takes part in the block's barriers)
   const int chunk = 8 * V * int(blockDim.x);
@@ -192,7 +199,7 @@ rows_int8_kernel(const RiParams p, float one) {
   float2 v[V][4];  // the row: h, then the values to be rounded
   auto fetch = [&](int base, bool again) {
     Ri8<T> raw[V];
-    // (x may be overwritten by the sum: a second pass reads what this thread stored)
+    // (x may be overwritten by the sum: a second pass reads what its warp stored)
     const bool summed = again && residual && sum_out;
 #pragma unroll
     for (int i = 0; i < V; ++i) raw[i] = ri_load<T, VEC>(summed ? sum_out : x, ri_col(base, i), cols);
@@ -205,7 +212,7 @@ rows_int8_kernel(const RiParams p, float one) {
         // rounded to the type it is stored in: the norm is taken of what later kernels read
 #pragma unroll
         for (int j = 0; j < 8; j += 2) raw[i].set2(j, raw[i].get(j) + add[i].get(j), raw[i].get(j + 1) + add[i].get(j + 1));
-        if (sum_out) ri_store<T, VEC>(sum_out, ri_col(base, i), cols, raw[i]);
+        if (sum_out) ri_store<T, VEC>(sum_out, ri_col(base, i), cols, raw[i], stage);
       }
     }
     if (MODE != RI_ROWS && weight) {
