@@ -350,7 +350,7 @@ class DecoderEngine:
             # what the passes above did not launch: the kernels of the multi-rank projections, whose forms depend on rank count and batch
             native.check(native.LIB.tpb_gemm_preload(), "tpb_gemm_preload")
             native.check(native.LIB.tpb_comm_preload(), "tpb_comm_preload")
-            if self.quantize:
+            if getattr(self, "quantize", None):
                 native.check(native.LIB.tpb_int8_preload(), "tpb_int8_preload")
 
     # -- building blocks --------------------------------------------------------------------------
