@@ -171,7 +171,6 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   } else {
     const int quarter = warp & 3;  // TMEM lane quarter this warp may access
     const int half = (warp - 2) >> 2, col0 = half * (BN / 2);
-    const int row = quarter * 32 + lane;
     const uint32_t acc_empty_leader[2] = {mapa_u32(smem_u32(&acc_empty[0]), 0), mapa_u32(smem_u32(&acc_empty[1]), 0)};
     const bool gated = g.act == I8_GATED;
     auto aligned = [](const void* ptr, long long ld) { return !(reinterpret_cast<uintptr_t>(ptr) & 15) && (ld & 7) == 0; };
@@ -348,6 +347,17 @@ extern "C" int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, 
   if (tpb::gemm_i8_split_pick(tokens, features, k, sms, &bn, &splits)) return tpb::gemm_i8_split_launch(g, bn, splits, s);
   if (tokens <= 64) return tpb::gemm_i8_stream_launch(g, sms, s);
   return tpb::ip_tile(tokens, features, sms) == 256 ? tpb::ip_launch<256>(g, sms, s) : tpb::ip_launch<128>(g, sms, s);
+}
+
+// The kernel that takes a product of these sizes, for tests: 0 streaming, 1 shared contraction (form: tokens of a tile, CTAs that share it), 2 CTA pairs (columns
+// of a tile).
+extern "C" int tpb_gemm_int8_form(int tokens, int features, int k, int sms, int* form) {
+  if (tokens <= 0 || features <= 0 || k <= 0 || k > tpb::I8_MAX_K || sms < 2 || !form) return -1;
+  form[0] = form[1] = 0;
+  if (tpb::gemm_i8_split_pick(tokens, features, k, sms, &form[0], &form[1])) return 1;
+  form[1] = 0;
+  form[0] = tokens <= 64 ? 0 : tpb::ip_tile(tokens, features, sms);
+  return tokens <= 64 ? 0 : 2;
 }
 
 // Loads every kernel of the 8-bit operators on the current device: a single host thread that drives several GPUs does so before the first of them waits for a peer.

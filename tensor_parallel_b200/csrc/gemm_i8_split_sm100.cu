@@ -1,4 +1,4 @@
-// Product of 8-bit integers for a middling number of tokens, 17 to about a thousand: see gemm_i8.cuh.
+// Product of 8-bit integers for a middling number of tokens, up to about a thousand, or a small weight: see gemm_i8.cuh.
 //
 // A tile is 128 features (the lanes of TMEM) x BN tokens, and the CTAs of a cluster of S share its contraction: there are too few tiles to occupy
 // the SMs, and each SM can only bring in so many bytes per clock.  Every CTA accumulates its range of k-blocks, then hands the partial sums of each
@@ -268,25 +268,28 @@ static int ix_launch(const I8Gemm& g, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<BN, S>, tw, tx, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
-// Where sharing the contraction pays, from a sweep over 17 to 1024 tokens and nine sizes from 768 x 4096 to 22016 x 4096 (us; stream / pair / this):
-//   17 x 4096 x 4096    11.4 / 13.1 / 8.3     17 x 768 x 4096    10.7 / 10.5 / 5.9     17 x 22016 x 4096   20.9 / 31.8 / 25.6
-//   64 x 4096 x 4096    11.1 / 11.7 / 9.0     64 x 4096 x 11008  19.8 / 20.9 / 13.8    64 x 12288 x 4096   15.1 / 18.3 / 15.2
+// Where this kernel pays, from sweeps over 1 to 1024 tokens and sizes from 256 x 1024 to 22016 x 4096 (us; stream / pair / this):
+//   1 x 4096 x 1024     4.5 / - / 3.9         1 x 2048 x 512     3.0 / - / 2.8         1 x 5120 x 8192     14.6 / - / 11.5     8 x 4096 x 4096   5.5 / - / 6.9
+//   1 x 8192 x 4096     10.3 / - / 9.6        16 x 12288 x 4096  12.2 / - / 12.4       17 x 4096 x 4096    11.4 / 13.1 / 8.3   17 x 768 x 4096   10.7 / 10.5 / 5.9
+//   64 x 4096 x 4096    11.1 / 11.7 / 9.0     64 x 4096 x 11008  19.8 / 20.9 / 13.8    64 x 22016 x 4096   21.9 / 26.7 / 28.1
 //   100 x 4096 x 11008  - / 21.7 / 15.3       100 x 2999 x 1001  - / 10.8 / 6.5        100 x 12288 x 4096  - / 18.9 / 17.5
-//   257 x 2999 x 1001   - / 11.1 / 8.0      256 x 4096 x 1024   - / 7.9 / 7.7         1024 x 1024 x 1024  - / 7.2 / 7.0
+//   257 x 2999 x 1001   - / 11.1 / 8.0        256 x 4096 x 1024  - / 7.9 / 7.7         1024 x 1024 x 1024  - / 7.2 / 7.0
 //   256 x 4096 x 11008  - / 22.1 / 18.6       256 x 4096 x 4096  - / 12.4 / 12.1       300 x 12288 x 4096  - / 25.8 / 30.2
-// A tile takes as many CTAs as there are idle SMs (clusters of 8 find room in a GPU's groups of SMs up to about 96 CTAs, of 4 up to 128).
+// A tile takes as many CTAs as there are idle SMs, two k-blocks each at least (clusters of 8 find room in a GPU's groups of SMs up to about 96 CTAs, of 4 up to
+// 128).  Up to 16 tokens the streaming kernel is ahead where it can cut long rows into slices itself, one unit of rows per CTA.
 bool gemm_i8_split_pick(int tokens, int features, int k, int sms, int* bn, int* splits) {
   const int k_blocks = (k + I8_BK - 1) / I8_BK;
   auto tiles = [&](int n) { return (long long)((features + 127) / 128) * ((tokens + n - 1) / n); };
   auto most = [&](int n) {
     int s = 1;
     for (int c = 2; c <= 8; c *= 2)
-      if (tiles(n) * c <= (c == 8 ? sms * 96 / 148 : c == 4 ? sms * 128 / 148 : sms) && c <= k_blocks && n / c >= 8) s = c;
+      if (tiles(n) * c <= (c == 8 ? sms * 96 / 148 : c == 4 ? sms * 128 / 148 : sms) && 2 * c <= k_blocks && n / c >= 8) s = c;
     return s;
   };
   *bn = tokens <= 32 ? 32 : 64;
   *splits = most(*bn);
-  if (tokens <= 64) return tokens > 16 && tiles(*bn) <= sms;
+  if (tokens <= 16) return k_blocks < 16 ? tiles(32) * (k_blocks <= 4 ? 1 : 2) <= sms : (features + 31) / 32 > sms && tiles(32) * 2 <= sms;
+  if (tokens <= 64) return tiles(*bn) <= sms;
   if (*splits > 1 || (k_blocks < 16 && tiles(64) <= sms)) return true;
   *bn = 128;
   *splits = most(128);

@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from tensor_parallel_b200 import build
 from tensor_parallel_b200.ops import functional as OF
 
 BF16 = torch.bfloat16
@@ -191,3 +192,30 @@ def test_generation_in_8_bits_needs_the_engine():
     with pytest.raises(ValueError, match="quantize"):
         wrapped.generate(ids, max_new_tokens=2, quantize="fp4")
     assert wrapped.generate(ids, max_new_tokens=2, quantize="bf16").shape == (1, 7)
+
+
+def _form(tokens, features, k, sms=148):
+    import ctypes
+
+    from tensor_parallel_b200.ops import native
+
+    form = (ctypes.c_int * 2)()
+    return native.LIB.tpb_gemm_int8_form(tokens, features, k, sms, form), form[0], form[1]
+
+
+@pytest.mark.skipif(not build.LIB_PATH.exists(), reason="native library not built")
+@pytest.mark.parametrize("sms", [148, 132, 20, 2])
+def test_every_size_has_a_kernel_that_takes_it(sms):
+    for tokens in (1, 2, 16, 17, 32, 33, 64, 65, 128, 129, 300, 512, 1000, 8192, 200000):
+        for features in (1, 32, 33, 768, 4096, 4736, 4737, 12288, 22016, 151936):
+            for k in (1, 128, 129, 500, 1024, 2048, 4096, 11008, OF.INT8_MAX_K):
+                kind, bn, splits = _form(tokens, features, k, sms)
+                if kind == 0:
+                    assert tokens <= 64
+                elif kind == 1:
+                    tiles = -(-features // 128) * -(-tokens // bn)
+                    assert (bn, splits) in {(32, 1), (32, 2), (32, 4), (64, 1), (64, 2), (64, 4), (64, 8), (128, 1), (128, 2)}
+                    assert splits <= -(-k // 128) and tiles * splits <= sms  # (a k-block for every CTA, and one round of CTAs)
+                else:
+                    assert kind == 2 and tokens > 64 and bn in (128, 256)
+    assert _form(0, 1, 1)[0] == _form(1, 1, OF.INT8_MAX_K + 1)[0] == -1
