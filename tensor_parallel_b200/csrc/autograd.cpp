@@ -10,6 +10,8 @@
 // (a variant with index checks, for instance), and the two callbacks that need Python objects.
 #include <torch/extension.h>
 
+#include <ATen/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -305,13 +307,18 @@ bool rows_apart(const Tensor& t, int64_t* rows, int64_t* pitch) {
 }
 bool vector_of(const Tensor& t, int64_t n) { return t.dim() == 1 && t.size(0) == n && (t.stride(0) == 1 || n == 1); }
 
+// Uninitialised memory of the current device, without the detour through the dispatcher.
+Tensor room_for(at::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::detail::empty_generic(sizes, c10::cuda::CUDACachingAllocator::get(), c10::DispatchKeySet(c10::DispatchKey::CUDA), dtype, std::nullopt);
+}
+
 struct Int8Out {
   Tensor values, scales;
 };
 // Both in one allocation (an allocation and its release cost as much as a third of a launch): values a multiple of 16 bytes apart, scales behind them.
 Int8Out int8_out(const Tensor& x, int64_t rows) {
   const int64_t cols = x.size(-1), pitch = (cols + 15) / 16 * 16;
-  const Tensor room = at::empty({rows * (pitch + int64_t(sizeof(float)))}, x.options().dtype(at::kByte));
+  const Tensor room = room_for({rows * (pitch + int64_t(sizeof(float)))}, at::kByte);
   auto part = [&](at::ScalarType dtype, int64_t offset, at::IntArrayRef sizes, int64_t step) {
     Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(room.storage()), room.key_set(), c10::scalarTypeToTypeMeta(dtype));
     std::vector<int64_t> strides(sizes.size(), 1);
@@ -327,10 +334,9 @@ Int8Out int8_out(const Tensor& x, int64_t rows) {
   return {part(at::kChar, 0, x.sizes(), pitch), part(at::kFloat, rows * pitch / int64_t(sizeof(float)), x.sizes().slice(0, x.dim() - 1), 1)};
 }
 
-using MaybeRows = std::optional<std::tuple<Tensor, Tensor, std::optional<Tensor>>>;
-
-// norm: -1 the rows as they are, 0 RMSNorm, 1 LayerNorm.
-MaybeRows rows_int8(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, int64_t norm, const std::optional<Tensor>& residual_) {
+// norm: -1 the rows as they are, 0 RMSNorm, 1 LayerNorm.  Values, scales, and with a residual the sum (else x).
+std::optional<std::tuple<Tensor, Tensor, Tensor>> rows_int8(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, int64_t norm,
+                                                            const std::optional<Tensor>& residual_) {
   const Tensor weight = or_undefined(weight_), bias = or_undefined(bias_), residual = or_undefined(residual_);
   const auto dtype = x.scalar_type();
   int64_t rows, pitch, residual_rows, residual_pitch = 0;
@@ -344,14 +350,18 @@ MaybeRows rows_int8(const Tensor& x, const std::optional<Tensor>& weight_, const
     return std::nullopt;
   const c10::cuda::CUDAGuard guard(x.device());
   const Int8Out out = int8_out(x, rows);
-  std::optional<Tensor> sum;
-  if (residual.defined()) sum = at::empty(x.sizes(), x.options());
-  check(lib.rows_int8(x.const_data_ptr(), data(residual), data(weight), data(bias), sum ? sum->mutable_data_ptr() : nullptr,
+  const Tensor sum = residual.defined() ? room_for(x.sizes(), dtype) : Tensor();
+  check(lib.rows_int8(x.const_data_ptr(), data(residual), data(weight), data(bias), sum.defined() ? sum.mutable_data_ptr() : nullptr,
                       static_cast<int8_t*>(out.values.mutable_data_ptr()), out.scales.mutable_data_ptr<float>(), int(rows), int(cols), pitch, residual_pitch, cols,
                       (cols + 15) / 16 * 16, float(eps), int(norm) + 1, dtype == at::kFloat, context(x, 0)->status, stream_of(x)),
         "tpb_rows_int8");
   launched.fetch_add(1, std::memory_order_relaxed);
-  return std::make_tuple(out.values, out.scales, sum);
+  return std::make_tuple(out.values, out.scales, sum.defined() ? sum : x);
+}
+std::optional<std::tuple<Tensor, Tensor>> quantize_int8(const Tensor& x) {
+  const auto out = rows_int8(x, std::nullopt, std::nullopt, 0., -1, std::nullopt);
+  if (!out) return std::nullopt;
+  return std::make_tuple(std::get<0>(*out), std::get<1>(*out));
 }
 
 std::optional<Tensor> linear_int8(const Tensor& x, const Tensor& sx, const Tensor& w, const Tensor& sw, const std::optional<Tensor>& bias_, int64_t act,
@@ -373,7 +383,7 @@ std::optional<Tensor> linear_int8(const Tensor& x, const Tensor& sx, const Tenso
   if (residual.defined() && (!plain(residual, at::kBFloat16, device) || residual.sizes() != at::IntArrayRef(shape) || !rows_apart(residual, &residual_rows, &ld_res)))
     return std::nullopt;
   const c10::cuda::CUDAGuard guard(device);
-  Tensor out = at::empty(shape, x.options().dtype(at::kBFloat16));
+  Tensor out = room_for(shape, at::kBFloat16);
   check(lib.gemm_int8(static_cast<const int8_t*>(x.const_data_ptr()), sx.const_data_ptr<float>(), static_cast<const int8_t*>(w.const_data_ptr()),
                       sw.const_data_ptr<float>(), out.mutable_data_ptr(), data(bias), data(residual), int(tokens), int(features), int(k), ldx, ldw, cols, ld_res,
                       int(act), 0, context(x, 0)->status, stream_of(x)),
@@ -422,6 +432,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear, unlocked);
   m.def("linears", &linears, unlocked);
   m.def("norm", &norm, unlocked);
-  m.def("rows_int8", &rows_int8, unlocked);
+  m.def("norm_int8", &rows_int8, unlocked);
+  m.def("quantize_int8", &quantize_int8, unlocked);
   m.def("linear_int8", &linear_int8, unlocked);
 }

@@ -356,7 +356,7 @@ def layer_norm_int8(x, weight, bias, eps: float = 1e-5, residual=None) -> Tuple[
     return layer_norm_int8_ref(x, weight, bias, eps, residual) if nat is None or transformed(x) else nat.norm_int8(x, weight, bias, eps, 1, residual)
 
 
-_INT8_ACTS = (None, "relu", "gelu", "gelu_tanh", "silu", "swiglu16")
+INT8_ACTS = (None, "relu", "gelu", "gelu_tanh", "silu", "swiglu16")
 
 
 def _check_linear_int8(x, weight, bias, act, residual):
@@ -370,7 +370,7 @@ def _check_linear_int8(x, weight, bias, act, residual):
     features, k = wv.shape
     if not 0 < k <= INT8_MAX_K or features == 0:
         raise ValueError(f"linear_int8 contracts 1 to {INT8_MAX_K} columns into at least one feature, got a weight {tuple(wv.shape)}")
-    if act not in _INT8_ACTS:
+    if act not in INT8_ACTS:
         raise ValueError(f"linear_int8: unknown activation {act!r}")
     if act == "swiglu16" and (features % 32 or residual is not None):
         raise ValueError("linear_int8: swiglu16 takes weight rows in groups of 16 gate and 16 up rows, and no residual")

@@ -1035,18 +1035,24 @@ def norm_int8(x, weight, bias, eps, mode, residual=None):
 # The calls that need neither a check's words nor a copy, by the C++ module (which leaves all others: None).
 
 
+_tuple = tuple.__new__  # (a named tuple's own constructor is a Python function)
+
+
 def quantize_int8_directly(x):
-    out = None if AUTOGRAD is None else AUTOGRAD.rows_int8(x, None, None, 0.0, -1, None)
-    return None if out is None else OF.Int8Rows(out[0], out[1])
+    out = None if AUTOGRAD is None else AUTOGRAD.quantize_int8(x)
+    return None if out is None else _tuple(OF.Int8Rows, out)
 
 
 def norm_int8_directly(x, weight, bias, eps, mode, residual):
-    out = None if AUTOGRAD is None else AUTOGRAD.rows_int8(x, weight, bias, eps, mode, residual)
-    return None if out is None else (OF.Int8Rows(out[0], out[1]), x if residual is None else out[2])
+    out = None if AUTOGRAD is None else AUTOGRAD.norm_int8(x, weight, bias, eps, mode, residual)
+    return None if out is None else (_tuple(OF.Int8Rows, out[:2]), out[2])
+
+
+_INT8_ACTS = {act: ACT_CODES[act] for act in OF.INT8_ACTS}
 
 
 def linear_int8_directly(x, weight, bias, act, residual):
-    code = ACT_CODES.get(act)
+    code = _INT8_ACTS.get(act) if act is None or type(act) is str else None
     return None if AUTOGRAD is None or code is None else AUTOGRAD.linear_int8(x[0], x[1], weight[0], weight[1], bias, code, residual)
 
 
