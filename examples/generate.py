@@ -2,6 +2,7 @@
 
     python examples/generate.py                                      # two CPU ranks, tiny model, generic path
     python examples/generate.py --devices cuda:0 --dtype bfloat16    # kernel-level serving engine, CUDA-graph decode
+    python examples/generate.py --devices cuda:0 --dtype bfloat16 --quantize int8   # the same with 8-bit projections
     torchrun --standalone --nproc-per-node 8 examples/generate.py --devices cuda --dtype bfloat16 --size 7b
 
 On CUDA with bf16 Llama-shaped shards ``generate()`` runs the serving engine (prefill + one CUDA graph per decode step,
@@ -25,6 +26,7 @@ def main():
     ap.add_argument("--dtype", default="float32")
     ap.add_argument("--size", default="tiny", choices=["tiny", "7b"])
     ap.add_argument("--new-tokens", type=int, default=8)
+    ap.add_argument("--quantize", choices=["bf16", "int8"])
     args = ap.parse_args()
     devices = args.devices
     if "LOCAL_RANK" in os.environ:
@@ -42,7 +44,7 @@ def main():
         model = LlamaForCausalLM(cfg).to(getattr(torch, args.dtype)).eval()
     model = tp.tensor_parallel(model, devices)
     prompt = torch.randint(0, cfg.vocab_size, (2, 12))
-    greedy = model.generate(prompt, max_new_tokens=args.new_tokens)
+    greedy = model.generate(prompt, max_new_tokens=args.new_tokens, quantize=args.quantize)
     print("greedy :", greedy[0, 12:].tolist())
     if build_on == "cpu":  # (beam search and sampling use the generic path; fine on any device, shown here on CPU)
         beams = model.generate(prompt, max_new_tokens=args.new_tokens, num_beams=3)

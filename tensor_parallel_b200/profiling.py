@@ -141,6 +141,27 @@ def case_norm(rows, cols, iters):
     return {"us": us, "tbps": 2.0 * rows * cols * 2 / us / 1e6}
 
 
+def case_int8_rows(rows, cols, iters, norm=None, residual=False):
+    """8-bit rows of activations, or of their RMSNorm with the residual's addition."""
+    xs = [torch.randn(rows, cols, device="cuda").to(torch.bfloat16) for _ in range(3)]
+    w = torch.ones(cols, device="cuda", dtype=torch.bfloat16) if norm is not None else None
+    summed, out = torch.empty_like(xs[0]) if residual else None, native.int8_rows_empty(rows, cols, "cuda")
+    res = _timed(lambda i: native.rows_int8(xs[i % 3], w, None, 1e-6, norm, xs[(i + 1) % 3] if residual else None, summed, out), iters)
+    return {**res, "tbps": rows * cols * (7.0 if residual else 3.0) / res.get("graph_us", res["us"]) / 1e6}
+
+
+def case_int8_product(tokens, features, k, iters, act=None):
+    def rows(n):
+        return torch.randint(-127, 128, (n, k), dtype=torch.int8, device="cuda"), torch.rand(n, device="cuda") * 1e-3
+
+    ring = max(2, int(300e6 // (features * k)) + 1)
+    x, ws = rows(tokens), [rows(features) for _ in range(ring)]
+    out = torch.empty(tokens, features // 2 if act == "swiglu16" else features, device="cuda", dtype=torch.bfloat16)
+    res = _timed(lambda i: native.gemm_int8(x, ws[i % ring], act=act, out=out), iters)
+    us = res.get("graph_us", res["us"])
+    return {**res, "tops": 2.0 * tokens * features * k / us / 1e6, "tbps": (float(features) * k + tokens * k + 2.0 * out.numel()) / us / 1e6}
+
+
 def case_swiglu(rows, cols, iters):
     gus = [torch.randn(rows, 2 * cols, device="cuda", dtype=torch.bfloat16) for _ in range(3)]
     out = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
@@ -183,6 +204,11 @@ CASES = {
     "attn_backward": lambda it: case_attn_backward(4, 2048, 32, 128, it),
     "head_cross_entropy": lambda it: case_cross_entropy(8192, 32000, 4096, it),
     "rmsnorm": lambda it: case_norm(32768, 4096, it),
+    "int8_norm": lambda it: case_int8_rows(8192, 4096, it, norm=0, residual=True),
+    "int8_rows": lambda it: case_int8_rows(8192, 11008, it),
+    "int8_decode_gate_up": lambda it: case_int8_product(8, 22016, 4096, it, act="swiglu16"),
+    "int8_short_down": lambda it: case_int8_product(100, 4096, 11008, it),
+    "int8_prompt_up": lambda it: case_int8_product(2048, 11008, 4096, it),
     "swiglu": lambda it: case_swiglu(16384, 11008, it),
     "rope_append": lambda it: case_rope_append(8, 2048, 32, it),
     "adamw": lambda it: case_adamw(64 * 1024 * 1024, it),
