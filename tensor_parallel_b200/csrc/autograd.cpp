@@ -315,23 +315,14 @@ Tensor room_for(at::IntArrayRef sizes, at::ScalarType dtype) {
 struct Int8Out {
   Tensor values, scales;
 };
-// Both in one allocation (an allocation and its release cost as much as a third of a launch): values a multiple of 16 bytes apart, scales behind them.
+// Values a multiple of 16 bytes apart.  An allocation each: two types over one storage cannot be saved.
 Int8Out int8_out(const Tensor& x, int64_t rows) {
-  const int64_t cols = x.size(-1), pitch = (cols + 15) / 16 * 16;
-  const Tensor room = room_for({rows * (pitch + int64_t(sizeof(float)))}, at::kByte);
-  auto part = [&](at::ScalarType dtype, int64_t offset, at::IntArrayRef sizes, int64_t step) {
-    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(room.storage()), room.key_set(), c10::scalarTypeToTypeMeta(dtype));
-    std::vector<int64_t> strides(sizes.size(), 1);
-    for (int64_t d = int64_t(sizes.size()) - 1, next = step; d >= 0; --d) {
-      if (step > 1 && d == int64_t(sizes.size()) - 1) continue;  // (the columns of the values)
-      strides[d] = next;
-      next *= std::max<int64_t>(sizes[d], 1);
-    }
-    t.unsafeGetTensorImpl()->set_storage_offset(offset);
-    t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides);
-    return t;
-  };
-  return {part(at::kChar, 0, x.sizes(), pitch), part(at::kFloat, rows * pitch / int64_t(sizeof(float)), x.sizes().slice(0, x.dim() - 1), 1)};
+  const int64_t dims = x.dim(), pitch = (x.size(-1) + 15) / 16 * 16;
+  Tensor values = room_for({rows * pitch}, at::kChar);
+  std::vector<int64_t> strides(dims, 1);
+  for (int64_t d = dims - 2, next = pitch; d >= 0; next *= x.size(d--)) strides[d] = next;
+  values.unsafeGetTensorImpl()->set_sizes_and_strides(x.sizes(), strides);
+  return {values, room_for(x.sizes().slice(0, dims - 1), at::kFloat)};
 }
 
 // norm: -1 the rows as they are, 0 RMSNorm, 1 LayerNorm.  Values, scales, and with a residual the sum (else x).

@@ -25,6 +25,7 @@
 namespace tpb {
 
 constexpr int I8_MAX_K = 131071;  // rows of -128 that long sum up to 2^31 - 2^14
+constexpr int I8_MAX_ROWS = 0x7fffffff - 511;  // (rows of the last tile are counted in 32 bits)
 constexpr int IP_BM = 256;        // tokens of a pair tile (128 per CTA = TMEM lanes)
 constexpr int IP_EPI_WARPS = 8;   // two per quarter of the TMEM lanes: one for each half of the columns
 constexpr int IP_THREADS = 64 + 32 * IP_EPI_WARPS;
@@ -330,7 +331,7 @@ extern "C" int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, 
                              void* stream) {
   using bf16 = __nv_bfloat16;
   if (!x || !sx || !w || !sw || !out || !status || tokens <= 0 || features <= 0 || k <= 0 || act < 0 || act > tpb::I8_GATED) return TPB_ERR_ARG;
-  if (k > tpb::I8_MAX_K) return TPB_ERR_SIZE;
+  if (k > tpb::I8_MAX_K || tokens > tpb::I8_MAX_ROWS || features > tpb::I8_MAX_ROWS) return TPB_ERR_SIZE;
   const int cols = act == tpb::I8_GATED ? features / 2 : features;
   if (act == tpb::I8_GATED && (features % 32 || residual)) return TPB_ERR_ARG;
   if (ldx < k || ldw < k || ld_out < cols || (residual && ld_res < cols)) return TPB_ERR_ARG;
@@ -352,7 +353,7 @@ extern "C" int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, 
 // The kernel that takes a product of these sizes, for tests: 0 streaming, 1 shared contraction (form: tokens of a tile, CTAs that share it), 2 CTA pairs (columns
 // of a tile).
 extern "C" int tpb_gemm_int8_form(int tokens, int features, int k, int sms, int* form) {
-  if (tokens <= 0 || features <= 0 || k <= 0 || k > tpb::I8_MAX_K || sms < 2 || !form) return -1;
+  if (tokens <= 0 || features <= 0 || k <= 0 || k > tpb::I8_MAX_K || tokens > tpb::I8_MAX_ROWS || features > tpb::I8_MAX_ROWS || sms < 2 || !form) return -1;
   form[0] = form[1] = 0;
   if (tpb::gemm_i8_split_pick(tokens, features, k, sms, &form[0], &form[1])) return 1;
   form[1] = 0;

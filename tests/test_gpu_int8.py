@@ -480,3 +480,18 @@ def test_tensors_on_another_device_than_the_current_one():
         far = [OF.Int8Rows(t.values.to("cuda:1"), t.scales.to("cuda:1")) for t in (x, w)]
         out, got = OF.linear_int8(*far), OF.quantize_int8(y.to("cuda:1"))
     assert out.device.index == 1 and torch.equal(out.cpu(), want.cpu()) and torch.equal(got.values.cpu(), rows.values.cpu())
+
+
+@pytest.mark.parametrize("shape", [(5, 40), (2, 3, 64), (33,)])
+def test_rows_are_saved_and_copied_like_other_tensors(shape, tmp_path):
+    import copy
+
+    rows = OF.quantize_int8(_wave(1, torch.Size(shape).numel(), BF16, 95).view(shape))
+    torch.save({"weight": rows.values, "scales": rows.scales}, tmp_path / "rows.pt")
+    read = torch.load(tmp_path / "rows.pt", weights_only=True)
+    assert torch.equal(read["weight"], rows.values) and torch.equal(read["scales"], rows.scales)
+    twin = copy.deepcopy(rows)
+    twin.values.zero_()
+    twin.scales.zero_()
+    again = OF.quantize_int8(_wave(1, torch.Size(shape).numel(), BF16, 95).view(shape))
+    assert torch.equal(again.values, rows.values) and torch.equal(again.scales, rows.scales)

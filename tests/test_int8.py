@@ -219,3 +219,9 @@ def test_every_size_has_a_kernel_that_takes_it(sms):
                 else:
                     assert kind == 2 and tokens > 64 and bn in (128, 256)
     assert _form(0, 1, 1)[0] == _form(1, 1, OF.INT8_MAX_K + 1)[0] == -1
+
+
+@pytest.mark.skipif(not build.LIB_PATH.exists(), reason="native library not built")
+def test_sizes_whose_last_tile_would_not_count_in_32_bits_are_refused():
+    assert _form(2 ** 31 - 1, 1, 1)[0] == _form(1, 2 ** 31 - 1, 1)[0] == -1
+    assert _form(2 ** 31 - 512, 1, 1)[0] == 2 and _form(1, 2 ** 31 - 512, 1)[0] == 0
