@@ -14,6 +14,8 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <atomic>
@@ -325,54 +327,48 @@ Int8Out int8_out(const Tensor& x, int64_t rows) {
   return {values, room_for(x.sizes().slice(0, dims - 1), at::kFloat)};
 }
 
-// norm: -1 the rows as they are, 0 RMSNorm, 1 LayerNorm.  Values, scales, and with a residual the sum (else x).
-std::optional<std::tuple<Tensor, Tensor, Tensor>> rows_int8(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, int64_t norm,
-                                                            const std::optional<Tensor>& residual_) {
-  const Tensor weight = or_undefined(weight_), bias = or_undefined(bias_), residual = or_undefined(residual_);
+// norm: -1 the rows as they are, 0 RMSNorm, 1 LayerNorm.  Values, scales, and with a residual the sum (`out` and `sum` stay as they are where it returns false).
+bool rows_int8(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, int64_t norm, const Tensor& residual, Int8Out* out, Tensor* sum) {
   const auto dtype = x.scalar_type();
   int64_t rows, pitch, residual_rows, residual_pitch = 0;
   if (!lib.rows_int8 || !x.is_cuda() || (dtype != at::kBFloat16 && dtype != at::kFloat) || torch::jit::tracer::isTracing() || !plain(x, dtype, x.device()) ||
       !rows_apart(x, &rows, &pitch))
-    return std::nullopt;
+    return false;
   const int64_t cols = x.size(-1);
-  for (const Tensor& t : {weight, bias})
-    if (t.defined() && (!plain(t, dtype, x.device()) || !vector_of(t, cols))) return std::nullopt;
+  for (const Tensor* t : {&weight, &bias})
+    if (t->defined() && (!plain(*t, dtype, x.device()) || !vector_of(*t, cols))) return false;
   if (residual.defined() && (!plain(residual, dtype, x.device()) || residual.sizes() != x.sizes() || !rows_apart(residual, &residual_rows, &residual_pitch)))
-    return std::nullopt;
+    return false;
+  const py::gil_scoped_release unlocked;
   const c10::cuda::CUDAGuard guard(x.device());
-  const Int8Out out = int8_out(x, rows);
-  const Tensor sum = residual.defined() ? room_for(x.sizes(), dtype) : Tensor();
-  check(lib.rows_int8(x.const_data_ptr(), data(residual), data(weight), data(bias), sum.defined() ? sum.mutable_data_ptr() : nullptr,
-                      static_cast<int8_t*>(out.values.mutable_data_ptr()), out.scales.mutable_data_ptr<float>(), int(rows), int(cols), pitch, residual_pitch, cols,
+  *out = int8_out(x, rows);
+  if (residual.defined()) *sum = room_for(x.sizes(), dtype);
+  check(lib.rows_int8(x.const_data_ptr(), data(residual), data(weight), data(bias), sum && sum->defined() ? sum->mutable_data_ptr() : nullptr,
+                      static_cast<int8_t*>(out->values.mutable_data_ptr()), out->scales.mutable_data_ptr<float>(), int(rows), int(cols), pitch, residual_pitch, cols,
                       (cols + 15) / 16 * 16, float(eps), int(norm) + 1, dtype == at::kFloat, context(x, 0)->status, stream_of(x)),
         "tpb_rows_int8");
   launched.fetch_add(1, std::memory_order_relaxed);
-  return std::make_tuple(out.values, out.scales, sum.defined() ? sum : x);
-}
-std::optional<std::tuple<Tensor, Tensor>> quantize_int8(const Tensor& x) {
-  const auto out = rows_int8(x, std::nullopt, std::nullopt, 0., -1, std::nullopt);
-  if (!out) return std::nullopt;
-  return std::make_tuple(std::get<0>(*out), std::get<1>(*out));
+  return true;
 }
 
-std::optional<Tensor> linear_int8(const Tensor& x, const Tensor& sx, const Tensor& w, const Tensor& sw, const std::optional<Tensor>& bias_, int64_t act,
-                                  const std::optional<Tensor>& residual_) {
-  const Tensor bias = or_undefined(bias_), residual = or_undefined(residual_);
+// The product, or no tensor.
+Tensor linear_int8(const Tensor& x, const Tensor& sx, const Tensor& w, const Tensor& sw, const Tensor& bias, int64_t act, const Tensor& residual) {
   int64_t tokens, ldx, features, ldw, residual_rows, ld_res = 0;
   const auto device = x.device();
   if (!lib.gemm_int8 || !x.is_cuda() || torch::jit::tracer::isTracing() || !plain(x, at::kChar, device) || !plain(w, at::kChar, device) ||
       !plain(sx, at::kFloat, device) || !plain(sw, at::kFloat, device) || x.dim() < 2 || w.dim() != 2 || !rows_apart(x, &tokens, &ldx) ||
       !rows_apart(w, &features, &ldw) || x.size(-1) != w.size(1) || !vector_of(sw, features) || sx.sizes() != x.sizes().slice(0, x.dim() - 1) ||
       !sx.is_contiguous())
-    return std::nullopt;
+    return {};
   const int64_t k = w.size(1), cols = act == 5 ? features / 2 : features;
   auto aligned = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; };
-  if (k > 131071 || ldx % 16 || ldw % 16 || !aligned(x) || !aligned(w) || (act == 5 && (features % 32 || residual.defined()))) return std::nullopt;
-  if (bias.defined() && (!plain(bias, at::kBFloat16, device) || !vector_of(bias, features))) return std::nullopt;
-  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  if (k > 131071 || ldx % 16 || ldw % 16 || !aligned(x) || !aligned(w) || (act == 5 && (features % 32 || residual.defined()))) return {};
+  if (bias.defined() && (!plain(bias, at::kBFloat16, device) || !vector_of(bias, features))) return {};
+  c10::DimVector shape(x.sizes().begin(), x.sizes().end());
   shape.back() = cols;
   if (residual.defined() && (!plain(residual, at::kBFloat16, device) || residual.sizes() != at::IntArrayRef(shape) || !rows_apart(residual, &residual_rows, &ld_res)))
-    return std::nullopt;
+    return {};
+  const py::gil_scoped_release unlocked;
   const c10::cuda::CUDAGuard guard(device);
   Tensor out = room_for(shape, at::kBFloat16);
   check(lib.gemm_int8(static_cast<const int8_t*>(x.const_data_ptr()), sx.const_data_ptr<float>(), static_cast<const int8_t*>(w.const_data_ptr()),
@@ -381,6 +377,87 @@ std::optional<Tensor> linear_int8(const Tensor& x, const Tensor& sx, const Tenso
         "tpb_gemm_int8");
   launched.fetch_add(1, std::memory_order_relaxed);
   return out;
+}
+
+// The interpreter's side of these calls, without pybind11's conversions, which cost 0.6 us of a call's 4.5.
+PyObject* rows_type = nullptr;  // the named tuple (values, scales)
+PyObject* act_codes = nullptr;  // activation -> code
+
+const Tensor nothing;
+// The tensor behind an argument (None: an undefined one), or null if it is neither.
+const Tensor* tensor_of(PyObject* o) { return o == Py_None ? &nothing : THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
+const Tensor* a_tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
+
+PyObject* tuple_of(PyTypeObject* type, PyObject* a, PyObject* b) {  // takes the references
+  PyObject* t = a && b ? type->tp_alloc(type, 2) : nullptr;
+  if (!t) {
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    return nullptr;
+  }
+  PyTuple_SET_ITEM(t, 0, a);
+  PyTuple_SET_ITEM(t, 1, b);
+  return t;
+}
+PyObject* rows_object(const Int8Out& r) { return tuple_of(reinterpret_cast<PyTypeObject*>(rows_type), THPVariable_Wrap(r.values), THPVariable_Wrap(r.scales)); }
+
+// (x) -> rows
+PyObject* py_quantize_int8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor* x = n == 1 && rows_type ? a_tensor(args[0]) : nullptr;
+  Int8Out out;
+  if (!x || !rows_int8(*x, nothing, nothing, 0., -1, nothing, &out, nullptr)) Py_RETURN_NONE;
+  return rows_object(out);
+  END_HANDLE_TH_ERRORS
+}
+// (x, weight, bias, eps, 0 RMSNorm / 1 LayerNorm, residual) -> (rows, sum)
+PyObject* py_norm_int8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !rows_type) Py_RETURN_NONE;
+  const Tensor *x = a_tensor(args[0]), *weight = tensor_of(args[1]), *bias = tensor_of(args[2]), *residual = tensor_of(args[5]);
+  if (!x || !weight || !bias || !residual) Py_RETURN_NONE;
+  const double eps = PyFloat_AsDouble(args[3]);
+  const long norm = PyLong_AsLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  Int8Out out;
+  Tensor sum;
+  if (norm < 0 || norm > 1 || !rows_int8(*x, *weight, *bias, eps, norm, *residual, &out, &sum)) Py_RETURN_NONE;
+  PyObject* rows = rows_object(out);
+  return rows ? tuple_of(&PyTuple_Type, rows, sum.defined() ? THPVariable_Wrap(sum) : Py_NewRef(args[0])) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+// (rows, weight's rows, bias, activation, residual) -> product
+PyObject* py_linear_int8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !act_codes) Py_RETURN_NONE;
+  const Tensor *part[4], *bias = tensor_of(args[2]), *residual = tensor_of(args[4]);
+  for (int i = 0; i < 2; ++i) {
+    if (!PyTuple_Check(args[i]) || PyTuple_GET_SIZE(args[i]) != 2) Py_RETURN_NONE;
+    for (int j = 0; j < 2; ++j)
+      if (!(part[2 * i + j] = a_tensor(PyTuple_GET_ITEM(args[i], j)))) Py_RETURN_NONE;
+  }
+  if (!bias || !residual || (args[3] != Py_None && !PyUnicode_CheckExact(args[3]))) Py_RETURN_NONE;
+  PyObject* code = PyDict_GetItemWithError(act_codes, args[3]);
+  if (!code) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  const Tensor out = linear_int8(*part[0], *part[1], *part[2], *part[3], *bias, PyLong_AsLong(code), *residual);
+  if (!out.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+PyMethodDef int8_calls[] = {
+    {"quantize_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_quantize_int8)), METH_FASTCALL, nullptr},
+    {"norm_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_int8)), METH_FASTCALL, nullptr},
+    {"linear_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_int8)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+
+void bind_int8(py::object type, py::dict codes) {
+  Py_XDECREF(rows_type);
+  Py_XDECREF(act_codes);
+  rows_type = type.release().ptr();  // (kept like the callbacks above)
+  act_codes = codes.release().ptr();
 }
 
 template <typename F>
@@ -423,7 +500,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear, unlocked);
   m.def("linears", &linears, unlocked);
   m.def("norm", &norm, unlocked);
-  m.def("norm_int8", &rows_int8, unlocked);
-  m.def("quantize_int8", &quantize_int8, unlocked);
-  m.def("linear_int8", &linear_int8, unlocked);
+  m.def("bind_int8", &bind_int8);
+  if (PyModule_AddFunctions(m.ptr(), int8_calls) != 0) throw py::error_already_set();
 }

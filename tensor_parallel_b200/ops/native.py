@@ -1035,25 +1035,15 @@ def norm_int8(x, weight, bias, eps, mode, residual=None):
 # The calls that need neither a check's words nor a copy, by the C++ module (which leaves all others: None).
 
 
-_tuple = tuple.__new__  # (a named tuple's own constructor is a Python function)
+def _left(*args):
+    return None
 
 
-def quantize_int8_directly(x):
-    out = None if AUTOGRAD is None else AUTOGRAD.quantize_int8(x)
-    return None if out is None else _tuple(OF.Int8Rows, out)
-
-
-def norm_int8_directly(x, weight, bias, eps, mode, residual):
-    out = None if AUTOGRAD is None else AUTOGRAD.norm_int8(x, weight, bias, eps, mode, residual)
-    return None if out is None else (_tuple(OF.Int8Rows, out[:2]), out[2])
-
-
-_INT8_ACTS = {act: ACT_CODES[act] for act in OF.INT8_ACTS}
-
-
-def linear_int8_directly(x, weight, bias, act, residual):
-    code = _INT8_ACTS.get(act) if act is None or type(act) is str else None
-    return None if AUTOGRAD is None or code is None else AUTOGRAD.linear_int8(x[0], x[1], weight[0], weight[1], bias, code, residual)
+if AUTOGRAD is None:
+    quantize_int8_directly = norm_int8_directly = linear_int8_directly = _left
+else:
+    AUTOGRAD.bind_int8(OF.Int8Rows, {act: ACT_CODES[act] for act in OF.INT8_ACTS})
+    quantize_int8_directly, norm_int8_directly, linear_int8_directly = AUTOGRAD.quantize_int8, AUTOGRAD.norm_int8, AUTOGRAD.linear_int8
 
 
 def gemm_int8(x: OF.Int8Rows, weight: OF.Int8Rows, bias=None, act=None, residual=None, out=None, early=False):
