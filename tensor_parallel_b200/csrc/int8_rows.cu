@@ -6,8 +6,10 @@
 // the scale: the integers depend on no order of summation, and a row needs one exchange (sum of squares and maximum together) instead of two.
 // A row with a value that is not finite gets integers 0 and the scale NaN, so that everything computed from it is NaN.
 //
-// Memory-bound: x and the residual are read once, h and the integers written once; a row waits in registers, in its own type, for its
-// statistics.
+// Memory-bound: x and the residual are read once, h and the integers written once; a row waits for its statistics in the registers of a block as fp32, or, where
+// many wide rows need more of them in flight than registers hold, in shared memory.  Measured (us, and of the floor at 6549 GB/s): 8192 x 4096 bf16 17.8 (0.86),
+// its RMSNorm 24.8 (0.62), with a residual 37.4 (0.96), LayerNorm with a residual 41 (0.87); 8192 x 11008 46.8 (0.88).  What is above is instructions (unpacking,
+// maxima, the integers: about 20 per element with a row's own share, most on the half-rate pipe), and 2 us of launch and first latency.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -172,9 +174,11 @@ __device__ __forceinline__ uint32_t ri_integers(float2 v0, float2 v1, float inv,
   return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
 }
 
-// Blocks that an SM is to hold.
+// Blocks that an SM is to hold: as many registers as the row and its raw words take, without spills to speak of (8192 x 4096, RMSNorm with 8 blocks 28.6 us
+// instead of 24.8; with 32 columns a thread, 11008 wide, two blocks of 512 instead of one 76 us instead of 116).
 template <typename T, int MODE, int V, bool VEC>
 constexpr int ri_blocks(int threads) {
+  if (V == 4) return threads > 256 ? 1024 / threads : 768 / threads;
   return threads != 256 || !VEC ? 1 : MODE == RI_LAYER ? 4 : V == 1 ? 6 : sizeof(T) == 4 ? 4 : MODE == RI_ROWS ? 8 : 6;
 }
 
@@ -226,6 +230,14 @@ rows_int8_kernel(const RiParams p, float one) {
   };
   const int end = WIDE ? cols : 1;
 
+  auto clear_past = [&](int c, float2 (&g)[4]) {  // the columns past the end, of a group at column c
+    if (VEC ? c < cols : c + 8 <= cols) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (VEC || c + 2 * j >= cols) g[j].x = 0.f;
+      if (VEC || c + 2 * j + 1 >= cols) g[j].y = 0.f;
+    }
+  };
   // v times the weight (and plus the bias, of a LayerNorm's (h - mean) rstd), and the largest |v|
   float most0 = 0.f, most1 = 0.f;
   auto finish_values = [&](int base, float mean, float rstd) {
@@ -233,7 +245,7 @@ rows_int8_kernel(const RiParams p, float one) {
     for (int i = 0; i < V; ++i) {
       if (MODE == RI_LAYER) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = __fmul2_rn(__fadd2_rn(v[i][j], both(-mean)), both(rstd));
+        for (int j = 0; j < 4; ++j) v[i][j] = __fmul2_rn(WIDE ? __fadd2_rn(v[i][j], both(-mean)) : v[i][j], both(rstd));
       }
       if (MODE != RI_ROWS && weight) {
 #pragma unroll
@@ -245,11 +257,7 @@ rows_int8_kernel(const RiParams p, float one) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[i][j] = __fadd2_rn(v[i][j], make_float2(b.get(2 * j), b.get(2 * j + 1)));
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (ri_col(base, i) + 2 * j >= cols) v[i][j].x = 0.f;
-          if (ri_col(base, i) + 2 * j + 1 >= cols) v[i][j].y = 0.f;
-        }
+        if (WIDE) clear_past(ri_col(base, i), v[i]);
       }
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
@@ -275,10 +283,12 @@ rows_int8_kernel(const RiParams p, float one) {
       sum += squares.x + squares.y;
     }
     if (MODE == RI_LAYER) {
+      float2 total = both(0.f);
 #pragma unroll
       for (int i = 0; i < V; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum += v[i][j].x + v[i][j].y;
+        for (int j = 0; j < 4; ++j) total = __fadd2_rn(total, v[i][j]);
+      sum += total.x + total.y;
     } else {
       finish_values(base, 0.f, 1.f);
     }
@@ -288,19 +298,19 @@ rows_int8_kernel(const RiParams p, float one) {
     // (the deviations are summed up around the mean: a difference of two sums would lose the digits that they share)
     ri_reduce<true, false>(sum, most, sums[0], maxima);
     mean = sum / float(p.cols);
-    float squares = 0.f;
+    float2 around = both(0.f);
     for (int base = 0; base < end; base += chunk) {
       if (WIDE) fetch(base, true);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = v[i][j].x - mean, b = v[i][j].y - mean;
-          if (ri_col(base, i) + 2 * j < cols) squares += a * a;
-          if (ri_col(base, i) + 2 * j + 1 < cols) squares += b * b;
-        }
+        for (int j = 0; j < 4; ++j) v[i][j] = __fadd2_rn(v[i][j], both(-mean));
+        clear_past(ri_col(base, i), v[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) around = __ffma2_rn(v[i][j], v[i][j], around);
       }
     }
+    float squares = around.x + around.y;
     ri_reduce<true, false>(squares, most, sums[1], maxima);
     rstd = rsqrtf(squares / float(p.cols) + p.eps);
     for (int base = 0; base < end; base += chunk) {
@@ -341,7 +351,7 @@ rows_int8_kernel(const RiParams p, float one) {
   }
 }
 
-// ---- many rows: persistent groups of threads, rows arriving by bulk copies several ahead -------------------------------------------------------
+// ---- many wide rows: persistent groups of threads, rows arriving by bulk copies several ahead -------------------------------------------------------
 
 __device__ __forceinline__ void ri_bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(smem_u32(bar))
@@ -556,17 +566,15 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
   }
 }
 
-// True if the ring kernel was launched (or its launch failed: *e): rows that begin and end on a quad's boundary, enough of them for every SM, and room for two.
-// For rows wide enough; narrower ones have more of them in flight with a block each (us, ring / block per row: 8192 x 4096 24.1 / 17.9, RMSNorm 26.1 / 24.8, with a
-// residual 4096 x 8192 45.2 / 42.7; 4096 x 11008 25.9 / 30.7, RMSNorm 35 / 58, 4096 x 16384 35 / 56).
+// True if the ring kernel was launched (or its launch failed: *e): rows that begin and end on a quad's boundary, and room for two.
 template <typename T, int MODE>
 static bool ri_ring_launch(const RiParams& p, int sms, cudaStream_t stream, cudaError_t* e) {
   const size_t slot = (size_t(p.cols) * sizeof(T) + 15) / 16 * 16 + 16;  // (a row may begin in the middle of 16 bytes)
   const size_t stage = slot * (p.residual ? 2 : 1);
   const size_t params = size_t(MODE == RI_ROWS ? 0 : MODE == RI_RMS ? 1 : 2) * size_t((p.cols + 3) / 4) * 16;
   auto whole = [](const void* base, long long ld) { return reinterpret_cast<uintptr_t>(base) % (4 * sizeof(T)) == 0 && ld % 4 == 0; };
-  if (p.cols <= (p.residual || MODE == RI_LAYER ? 8192 : 4096) || p.rows < 2 * sms || params + 2 * stage > RI_RING_BYTES || p.cols % 4 || !whole(p.x, p.ldx) ||
-      !whole(p.residual, p.ldr) || !whole(p.sum_out, p.lds) || (reinterpret_cast<uintptr_t>(p.q) & 3) || p.ldq % 4)
+  if (params + 2 * stage > RI_RING_BYTES || p.cols % 4 || !whole(p.x, p.ldx) || !whole(p.residual, p.ldr) || !whole(p.sum_out, p.lds) ||
+      (reinterpret_cast<uintptr_t>(p.q) & 3) || p.ldq % 4)
     return false;
   size_t slots = (RI_RING_BYTES - params) / stage;
   if (slots > RI_RING_BARS) slots = RI_RING_BARS;
@@ -588,18 +596,48 @@ static bool ri_ring_launch(const RiParams& p, int sms, cudaStream_t stream, cuda
   return true;
 }
 
+// Which rows go by the ring, and which by 32 columns a thread instead of 16 (aligned bf16 rows of at most 32768 columns: the fp32 ones do not fit the registers).
+// Fewer threads a row cost latency, which few rows do not hide, and save the row's own share of the instructions.  us, 16 columns / 32 columns / ring:
+//   rows       8192 x 5120 - / 22.1 / 24.9     1024 x 8192 - / 6.1 / 9.0      8192 x 11008 - / 56 / 46.8    2048 x 11008 - / 16.2 / 15.0   1024 x 11008 - / 9.3 / 10.5
+//              592 x 20000 - / 10.5 / 9.6      2048 x 20000 - / 31.0 / 23.2
+//   RMSNorm    8192 x 4096 24.8 / 25.2 / 26.1  8192 x 5120 - / 34.6 / 31.4    8192 x 8192 - / 50.1 / 46.9   2048 x 8192 - / 14.8 / 16.8    2048 x 16384 - / 26.2 / 28.7
+//   + residual 8192 x 4096 37.4 / 37.8 / -     8192 x 8192 81 / 72 / -        8192 x 11008 - / 109 / 112    300 x 5120 4.0 / 4.5 / -       300 x 8192 6.0 / 5.4 / -
+//              8192 x 16392 - / 205 / 163      8192 x 20000 - / 222 / 312     8 x 16392 5.0 / 3.6 / -
+//   LayerNorm  8192 x 2560 22.5 / 22.9 / -     8192 x 3584 31.6 / 29.6 / -    8192 x 4096 37.2 / 30.3 / -   8192 x 8192 78 / 60 / -        8192 x 11008 - / 94 / 107
+// Other rows (fp32, or of any alignment), 16 columns / ring: RMSNorm with a residual 4096 x 8192 42.7 / 45.2; 4096 x 11008 30.7 / 25.9, RMSNorm 58 / 35.
+template <typename T, int MODE, bool VEC>
+static bool ri_ring(const RiParams& p, int sms) {
+  if (!VEC || sizeof(T) != 2 || p.cols > 32768) return p.rows >= 2 * sms && p.cols > (p.residual || MODE == RI_LAYER ? 8192 : 4096);
+  if (MODE == RI_ROWS) return p.cols > 8192 && p.rows >= (p.cols > 16384 ? 4 : 12) * sms;
+  return MODE == RI_RMS && !p.residual && p.cols > 4096 && p.rows >= 16 * sms;
+}
+template <typename T, int MODE, bool VEC>
+static bool ri_four(const RiParams& p, int sms) {
+  if (!VEC || sizeof(T) != 2 || p.cols > 32768) return false;
+  return p.cols > 16384 || (p.rows >= (p.cols > 6144 ? 2 : 4) * sms && p.cols >= (MODE == RI_LAYER ? 3584 : 4097));
+}
+
 template <typename T, int MODE, bool VEC>
 static cudaError_t ri_launch(const RiParams& p, int sms, cudaStream_t stream) {
   cudaError_t e;
-  if (ri_ring_launch<T, MODE>(p, sms, stream, &e)) return e;
+  if (ri_ring<T, MODE, VEC>(p, sms) && ri_ring_launch<T, MODE>(p, sms, stream, &e)) return e;
   const int groups = (p.cols + 7) / 8;
-  const int v = groups <= 32 ? 1 : 2;
+  const int v = groups <= 32 ? 1 : ri_four<T, MODE, VEC>(p, sms) ? 4 : 2;
   int threads = ((groups + v - 1) / v + 31) / 32 * 32;
   const bool wide = threads > RI_MAX_THREADS;
   if (wide) threads = RI_MAX_THREADS;
-  const int rows_per_block = threads >= 256 ? 1 : 256 / threads;
+  const int rows_per_block = threads >= 256 || v == 4 ? 1 : 256 / threads;
   const dim3 block(threads, rows_per_block), grid((unsigned(p.rows) + rows_per_block - 1) / rows_per_block);
   auto go = [&](auto kernel) { return launch_dependent(kernel, grid, block, 0, stream, true, p, 1.f); };
+  if constexpr (VEC && sizeof(T) == 2) {
+    if constexpr (MODE == RI_LAYER) {
+      if (v == 4 && threads <= 128) return go(rows_int8_kernel<T, MODE, 4, true, false, 128>);
+    }
+    if (v == 4)
+      return threads <= 256   ? go(rows_int8_kernel<T, MODE, 4, true, false, 256>)
+             : threads <= 512 ? go(rows_int8_kernel<T, MODE, 4, true, false, 512>)
+                              : go(rows_int8_kernel<T, MODE, 4, true, false, 1024>);
+  }
   if (wide) return go(rows_int8_kernel<T, MODE, 2, VEC, true, 1024>);
   if (v == 1) return go(rows_int8_kernel<T, MODE, 1, VEC, false, 256>);
   return threads <= 256 ? go(rows_int8_kernel<T, MODE, 2, VEC, false, 256>) : go(rows_int8_kernel<T, MODE, 2, VEC, false, 1024>);
@@ -629,6 +667,12 @@ static cudaError_t ri_preload() {
   LOAD(rows_int8_kernel<T, MODE, 2, false, false, 256>);
   LOAD(rows_int8_kernel<T, MODE, 2, true, false, 1024>);
   LOAD(rows_int8_kernel<T, MODE, 2, false, false, 1024>);
+  if constexpr (sizeof(T) == 2) {
+    LOAD(rows_int8_kernel<T, MODE, 4, true, false, 256>);
+    LOAD(rows_int8_kernel<T, MODE, 4, true, false, 512>);
+    LOAD(rows_int8_kernel<T, MODE, 4, true, false, 1024>);
+    if constexpr (MODE == RI_LAYER) LOAD(rows_int8_kernel<T, MODE, 4, true, false, 128>);
+  }
 #undef LOAD
   return e;
 }

@@ -495,3 +495,64 @@ def test_rows_are_saved_and_copied_like_other_tensors(shape, tmp_path):
     twin.scales.zero_()
     again = OF.quantize_int8(_wave(1, torch.Size(shape).numel(), BF16, 95).view(shape))
     assert torch.equal(again.values, rows.values) and torch.equal(again.scales, rows.scales)
+
+
+# Rows of these widths and numbers (in SMs) reach every division of a row among threads, and the kernel that has rows on their way ahead.
+MANY = [(3584, 5), (4096, 5), (4100, 3), (4104, 17), (5120, 5), (6152, 3), (8192, 17), (8196, 3), (8200, 5), (11008, 3), (11008, 17), (16384, 13), (16392, 5), (20000, 2), (32768, 3), (32776, 3)]
+
+
+def _many(cols, sms, dtype, seed):
+    rows = sms * torch.cuda.get_device_properties(0).multi_processor_count + 3
+    x = _wave(rows, cols, dtype, seed)
+    x[1] = 0
+    x[2, cols - 1] = float("nan")
+    return x
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("cols,sms", MANY)
+def test_many_wide_rows(cols, sms, dtype):
+    x = _many(cols, sms, dtype, cols)
+    q, s = OF.quantize_int8(x)
+    want = OF.quantize_int8_ref(x)
+    assert torch.equal(q, want.values)
+    torch.testing.assert_close(s, want.scales, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("cols,sms", MANY)
+def test_rms_norm_of_many_wide_rows(cols, sms, with_residual, dtype):
+    x = _many(cols, sms, dtype, cols)
+    res = _wave(*x.shape, dtype, cols + 1) if with_residual else None
+    w = (1 + 0.1 * torch.randn(cols, device="cuda", generator=_gen(3))).to(dtype)
+    (q, s), h = OF.rms_norm_int8(x, w, 1e-5, res)
+    (wq, ws), wh = OF.rms_norm_int8_ref(x, w, 1e-5, res)
+    assert torch.equal(q, wq)
+    torch.testing.assert_close(h, wh, rtol=0, atol=0, equal_nan=True)
+    most = (wh.float() * w.float()).abs().amax(1).clamp_min(1e-30)
+    scale = most.double() / 127 * torch.rsqrt((wh.float() * wh.float()).sum(1, dtype=torch.float64) / cols + 1e-5)
+    # fp32: a square, then at most 80 sums one after the other (halved by the root), the root, five more roundings, and the squares' above
+    torch.testing.assert_close(s.double(), scale, rtol=64 * 2.0 ** -24, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("cols,sms", MANY)
+def test_layer_norm_of_many_wide_rows(cols, sms, with_residual, dtype):
+    x = (_many(cols, sms, dtype, cols).float() + 50).to(dtype)
+    res = _wave(*x.shape, dtype, cols + 1) if with_residual else None
+    w = (1 + 0.1 * torch.randn(cols, device="cuda", generator=_gen(3))).to(dtype)
+    b = (0.1 * torch.randn(cols, device="cuda", generator=_gen(4))).to(dtype)
+    (q, s), h = OF.layer_norm_int8(x, w, b, 1e-5, res)
+    torch.testing.assert_close(h, x if res is None else (x.float() + res.float()).to(dtype), rtol=0, atol=0, equal_nan=True)
+    assert s[2].isnan() and not q[2].any()
+    for lo in range(0, x.shape[0], 512):
+        part = slice(lo, lo + 512)
+        hd = h[part].double()
+        y = torch.nn.functional.layer_norm(hd, (cols,), w.double(), b.double(), 1e-5)
+        step = y.abs().amax(1, keepdim=True).clamp_min(1e-30) / 127
+        back = q[part].double() * s[part].double()[:, None]
+        slack = 80 * 2.0 ** -24 * hd.abs().amax(1, keepdim=True) * torch.rsqrt(hd.var(1, unbiased=False, keepdim=True) + 1e-5) * 1.5
+        near = (back - y).abs() <= 0.501 * step + slack  # (as in test_layer_norm_rows)
+        assert (near | ~hd.isfinite().all(1, keepdim=True)).all()
