@@ -5,6 +5,8 @@
 // and here: 128 columns, 512 clocks of the tensor core at BN = 256.  Sums are 32-bit integers, the epilogue scales them.
 //
 // One CTA (320 threads), persistent over the pair's tiles:
+// Measured (us, of twice the bf16 rate of a library product in short runs, 1647 TFLOP/s): 2048 x 11008 x 4096 63.0 (0.89, tensor pipe busy for 0.81 at 1.64 GHz), 4000 x 12288 x 4096 136
+// (0.90), 8192 x 22016 x 4096 gated 440 (1.02); in long runs the power limit bounds them.  About 5 to 7 us of a call are prologue, first bytes and the last epilogue.
 //   warp 0    : TMA producer of this CTA's operand rows; completion is counted on the LEADER's barrier (no multicast)
 //   warp 1    : leader only: one thread issues the MMAs; the commits signal the barriers of both CTAs
 //   warps 2-9 : epilogue of this CTA's 128 rows, two TMEM accumulators so that it runs under the next tile's MMAs
@@ -41,7 +43,9 @@ struct IpParams {
 
 template <int BN>
 struct IpShape {
-  static constexpr int STAGES = BN == 256 ? 6 : 8;
+  static constexpr int STAGES = BN > 192 ? 6 : BN > 128 ? 7 : 8;
+  static constexpr int ACC_COLS = BN > 128 ? 256 : 128;  // TMEM columns of an accumulator
+  static constexpr int SPLIT = (BN / 2 + 31) / 32 * 32;  // columns that the first epilogue warp of a quarter takes
   static constexpr uint32_t A_BYTES = 128 * I8_BK;
   static constexpr uint32_t B_BYTES = BN / 2 * I8_BK;
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
@@ -54,7 +58,7 @@ template <int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(IP_THREADS, 1)
 gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const IpParams p) {
   using S = IpShape<BN>;
-  constexpr uint32_t TMEM_COLS = 2 * BN;
+  constexpr uint32_t TMEM_COLS = 2 * S::ACC_COLS;
   const I8Gemm& g = p.g;
   extern __shared__ uint8_t ip_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ip_smem_raw) + 1023) & ~uintptr_t(1023));
@@ -151,7 +155,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           break;
         }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * BN;
+        const uint32_t d_tmem = tmem_base + acc * S::ACC_COLS;
         for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
           const int s = it % S::STAGES;
           if (!mbar_wait(&full_bar[s], (it / S::STAGES) & 1)) {
@@ -171,7 +175,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     }
   } else {
     const int quarter = warp & 3;  // TMEM lane quarter this warp may access
-    const int half = (warp - 2) >> 2, col0 = half * (BN / 2);
+    const int half = (warp - 2) >> 2, col0 = half * S::SPLIT, col1 = half ? BN : S::SPLIT;
     const uint32_t acc_empty_leader[2] = {mapa_u32(smem_u32(&acc_empty[0]), 0), mapa_u32(smem_u32(&acc_empty[1]), 0)};
     const bool gated = g.act == I8_GATED;
     auto aligned = [](const void* ptr, long long ld) { return !(reinterpret_cast<uintptr_t>(ptr) & 15) && (ld & 7) == 0; };
@@ -189,7 +193,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       const float* biases = sws + BN;
       // (every warp has read what the tile before the last left there: it has passed the last tile's barrier)
       for (int c = int(threadIdx.x) - 64; c < 2 * BN; c += 32 * IP_EPI_WARPS) {
-        const int f = nt * BN + (c & (BN - 1));
+        const int f = nt * BN + (c < BN ? c : c - BN);
         sws[c] = f >= g.features ? 0.f : c < BN ? g.sw[f] : g.bias ? __bfloat162float(g.bias[f]) : 0.f;
       }
       const float sx = m < g.tokens ? g.sx[m] : 0.f;
@@ -200,9 +204,9 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         gone = true;
       }
       tc_fence_after();
-      const uint32_t t_lane = tmem_base + (uint32_t(quarter * 32) << 16) + acc * BN;
+      const uint32_t t_lane = tmem_base + (uint32_t(quarter * 32) << 16) + acc * S::ACC_COLS;
 #pragma unroll 1
-      for (int c0 = col0; c0 < col0 + BN / 2; c0 += 32) {
+      for (int c0 = col0; c0 < col1; c0 += 32) {
         const int n0 = nt * BN + c0;
         if (gone || n0 >= g.features) break;
         uint32_t r[32];
@@ -314,15 +318,27 @@ static int ip_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
   return launch_dependent(gemm_i8_pair_kernel<BN>, dim3(2 * pairs), dim3(IP_THREADS), S::SMEM, stream, true, ta, tb, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
-// Columns of the pair tile: rounds of tiles x time of a k-block, in clocks (256 x 22016 x 4096 with 256 / 128 columns 31.9 / 29.3 us, 512 x 12288 x 4096
-// 28.3 / 26.7, 512 x 22016 x 4096 40.5 / 43.1, 768 x 12288 x 4096 30.6 / 35.0, 1024 x 4096 x 11008 35.2 / 39.3).
+// Columns of the pair tile: the least rounds of tiles x clocks of a k-block, which is bound by the products at 256 columns and by what an SM gets from L2 at 128.
+// A narrower tile has to win 4.5 %: it moves more bytes per product, which costs where the card is at its power limit.  us with 256 / 224 / 192 / 160 / 128 columns:
+//   256 x 12288 x 4096 18.3 17.6 16.2 21.8 19.7    300 x 12288 x 4096 26.5 24.4 22.3 26.8 24.3     512 x 4096 x 4096 17.2 15.5 14.2 12.9 11.8
+//   300 x 11008 x 4096 26.7 24.6 22.3 20.7 24.1    300 x 22016 x 4096 38.6 36.0 39.0 37.2 39.5     768 x 12288 x 4096 30.5 34.8 33.0 36.1 35.0
+//   2048 x 12288 x 4096 74 71 74 80 86             2048 x 4096 x 11008 63 74 70 66 74              8192 x 22016 x 4096 (gated) 443 468 615 607 653
 static int ip_tile(int tokens, int features, int sms) {
-  auto rounds = [&](int bn) {
-    const long long tiles = (long long)((tokens + IP_BM - 1) / IP_BM) * ((features + bn - 1) / bn);
-    return (tiles + sms / 2 - 1) / (sms / 2);
-  };
-  return rounds(256) * 512 <= rounds(128) * 325 ? 256 : 128;
+  struct Shape { int bn, clocks; };
+  constexpr Shape SHAPES[] = {{256, 512}, {224, 450}, {192, 412}, {160, 365}, {128, 325}};
+  int bn = 0;
+  double least = 0;
+  for (const Shape& shape : SHAPES) {
+    const long long tiles = (long long)((tokens + IP_BM - 1) / IP_BM) * ((features + shape.bn - 1) / shape.bn);
+    const double clocks = double((tiles + sms / 2 - 1) / (sms / 2)) * shape.clocks;
+    if (bn && clocks * 1.045 >= least) continue;
+    bn = shape.bn;
+    least = clocks;
+  }
+  return bn;
 }
+
+#define IP_FORMS(GO) GO(128) GO(160) GO(192) GO(224) GO(256)
 
 }  // namespace tpb
 
@@ -347,7 +363,11 @@ extern "C" int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, 
   int bn = 0, splits = 0;
   if (tpb::gemm_i8_split_pick(tokens, features, k, sms, &bn, &splits)) return tpb::gemm_i8_split_launch(g, bn, splits, s);
   if (tokens <= 64) return tpb::gemm_i8_stream_launch(g, sms, s);
-  return tpb::ip_tile(tokens, features, sms) == 256 ? tpb::ip_launch<256>(g, sms, s) : tpb::ip_launch<128>(g, sms, s);
+  bn = tpb::ip_tile(tokens, features, sms);
+#define GO(BN) if (bn == BN) return tpb::ip_launch<BN>(g, sms, s);
+  IP_FORMS(GO)
+#undef GO
+  return TPB_ERR_ARG;
 }
 
 // The kernel that takes a product of these sizes, for tests: 0 streaming, 1 shared contraction (form: tokens of a tile, CTAs that share it), 2 CTA pairs (columns
@@ -364,8 +384,10 @@ extern "C" int tpb_gemm_int8_form(int tokens, int features, int k, int sms, int*
 // Loads every kernel of the 8-bit operators on the current device: a single host thread that drives several GPUs does so before the first of them waits for a peer.
 extern "C" int tpb_int8_preload(void) {
   cudaFuncAttributes attr;
-  cudaError_t e = cudaFuncGetAttributes(&attr, tpb::gemm_i8_pair_kernel<256>);
-  if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, tpb::gemm_i8_pair_kernel<128>);
+  cudaError_t e = cudaSuccess;
+#define LOAD(BN) if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, tpb::gemm_i8_pair_kernel<BN>);
+  IP_FORMS(LOAD)
+#undef LOAD
   if (e == cudaSuccess) e = tpb::gemm_i8_stream_preload();
   if (e == cudaSuccess) e = tpb::gemm_i8_split_preload();
   if (e == cudaSuccess) e = tpb::rows_int8_preload();

@@ -272,9 +272,9 @@ static int ix_launch(const I8Gemm& g, cudaStream_t stream) {
 //   1 x 4096 x 1024     4.5 / - / 3.9         1 x 2048 x 512     3.0 / - / 2.8         1 x 5120 x 8192     14.6 / - / 11.5     8 x 4096 x 4096   5.5 / - / 6.9
 //   1 x 8192 x 4096     10.3 / - / 9.6        16 x 12288 x 4096  12.2 / - / 12.4       17 x 4096 x 4096    11.4 / 13.1 / 8.3   17 x 768 x 4096   10.7 / 10.5 / 5.9
 //   64 x 4096 x 4096    11.1 / 11.7 / 9.0     64 x 4096 x 11008  19.8 / 20.9 / 13.8    64 x 22016 x 4096   21.9 / 26.7 / 28.1
-//   100 x 4096 x 11008  - / 21.7 / 15.3       100 x 2999 x 1001  - / 10.8 / 6.5        100 x 12288 x 4096  - / 18.9 / 17.5
+//   100 x 4096 x 11008  - / 21.7 / 15.3       100 x 2999 x 1001  - / 10.8 / 6.5        100 x 12288 x 4096  - / 15.9 / 15.0
 //   257 x 2999 x 1001   - / 11.1 / 8.0        256 x 4096 x 1024  - / 7.9 / 7.7         1024 x 1024 x 1024  - / 7.2 / 7.0
-//   256 x 4096 x 11008  - / 22.1 / 18.6       256 x 4096 x 4096  - / 12.4 / 12.1       300 x 12288 x 4096  - / 25.8 / 30.2
+//   256 x 4096 x 11008  - / 22.1 / 18.6       256 x 4096 x 4096  - / 12.4 / 12.1       300 x 12288 x 4096  - / 22.6 / 30.2
 // A tile takes as many CTAs as there are idle SMs, two k-blocks each at least (clusters of 8 find room in a GPU's groups of SMs up to about 96 CTAs, of 4 up to
 // 128).  Up to 16 tokens the streaming kernel is ahead where it can cut long rows into slices itself, one unit of rows per CTA.
 bool gemm_i8_split_pick(int tokens, int features, int k, int sms, int* bn, int* splits) {

@@ -556,3 +556,23 @@ def test_layer_norm_of_many_wide_rows(cols, sms, with_residual, dtype):
         slack = 80 * 2.0 ** -24 * hd.abs().amax(1, keepdim=True) * torch.rsqrt(hd.var(1, unbiased=False, keepdim=True) + 1e-5) * 1.5
         near = (back - y).abs() <= 0.501 * step + slack  # (as in test_layer_norm_rows)
         assert (near | ~hd.isfinite().all(1, keepdim=True)).all()
+
+
+# tokens, features that the widths of the pair kernel's tile take on a GPU of 148 SMs
+PAIRS = {128: [(512, 4096), (500, 4095)], 160: [(300, 11008), (290, 11009)], 192: [(300, 12288), (511, 12285)], 224: [(300, 22016), (2048, 12288)], 256: [(768, 12288), (1000, 4090)]}
+
+
+@pytest.mark.parametrize("act", [None, "gelu", "swiglu16"])
+@pytest.mark.parametrize("width", list(PAIRS))
+def test_every_width_of_the_pair_tile(width, act):
+    import ctypes
+
+    for tokens, features in PAIRS[width]:
+        features = features // 32 * 32 if act == "swiglu16" else features
+        form = (ctypes.c_int * 2)()
+        if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+            assert _native().LIB.tpb_gemm_int8_form(tokens, features, 400, 148, form) == 2 and form[0] == width, (tokens, features, form[0])
+        x, w = _operands(tokens, features, 400, width + tokens)
+        bias = torch.randn(features, device="cuda", generator=_gen(5)).to(BF16)
+        residual = None if act else torch.randn(tokens, features, device="cuda", generator=_gen(6)).to(BF16)
+        _check_product(x, w, bias, act, residual)
