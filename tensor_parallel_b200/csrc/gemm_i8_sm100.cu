@@ -4,9 +4,11 @@
 // tcgen05.mma.cta_group::2, each loads 128 token rows and BN / 2 feature rows, the leader issues for both.  A k-block is 128 bytes of every row there
 // and here: 128 columns, 512 clocks of the tensor core at BN = 256.  Sums are 32-bit integers, the epilogue scales them.
 //
+// Measured (us, of twice the bf16 rate of a library product in short runs, 1647 TFLOP/s): 2048 x 11008 x 4096 63.0 (0.89, tensor pipe busy for 0.81 at
+// 1.64 GHz), 4000 x 12288 x 4096 136 (0.90), 8192 x 22016 x 4096 gated 440 (1.02); in long runs the power limit bounds them.  About 5 to 7 us of a call
+// are prologue, first bytes and the last epilogue.
+//
 // One CTA (320 threads), persistent over the pair's tiles:
-// Measured (us, of twice the bf16 rate of a library product in short runs, 1647 TFLOP/s): 2048 x 11008 x 4096 63.0 (0.89, tensor pipe busy for 0.81 at 1.64 GHz), 4000 x 12288 x 4096 136
-// (0.90), 8192 x 22016 x 4096 gated 440 (1.02); in long runs the power limit bounds them.  About 5 to 7 us of a call are prologue, first bytes and the last epilogue.
 //   warp 0    : TMA producer of this CTA's operand rows; completion is counted on the LEADER's barrier (no multicast)
 //   warp 1    : leader only: one thread issues the MMAs; the commits signal the barriers of both CTAs
 //   warps 2-9 : epilogue of this CTA's 128 rows, two TMEM accumulators so that it runs under the next tile's MMAs
