@@ -199,6 +199,16 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         sws[c] = f >= g.features ? 0.f : c < BN ? g.sw[f] : g.bias ? __bfloat162float(g.bias[f]) : 0.f;
       }
       const float sx = m < g.tokens ? g.sx[m] : 0.f;
+      // the residual of a chunk, a chunk ahead
+      uint4 res[4];
+      auto fetch = [&](int c0) {
+        const int n0 = nt * BN + c0;
+        if (!g.residual || !vec || c0 >= col1 || n0 + 32 > g.features || m >= g.tokens) return;
+        const uint4* rp = reinterpret_cast<const uint4*>(g.residual + m * g.ld_res + n0);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) res[q] = rp[q];
+      };
+      fetch(col0);
       asm volatile("bar.sync 1, %0;" ::"n"(32 * IP_EPI_WARPS) : "memory");
       const bool ready = !*abort_flag && mbar_wait(&acc_full[acc], (local >> 1) & 1);
       if (!__all_sync(0xffffffffu, ready)) {
@@ -207,6 +217,13 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       }
       tc_fence_after();
       const uint32_t t_lane = tmem_base + (uint32_t(quarter * 32) << 16) + acc * S::ACC_COLS;
+      // Both accumulator halves may be overwritten after all of these.  Nothing but the tcgen05 loads, which have completed, has to come before (a release would
+      // wait for the stores, about 1 us), and only a tile that waits for it is told, so that no arrival is on its way to a CTA that has left.
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0 && t + 2 * pairs < tiles) mbar_arrive_cluster_relaxed(acc_empty_leader[acc]);
+      };
 #pragma unroll 1
       for (int c0 = col0; c0 < col1; c0 += 32) {
         const int n0 = nt * BN + c0;
@@ -215,6 +232,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         __syncwarp();
         tmem_ld_x32(t_lane + c0, r);
         tmem_ld_wait();
+        if (c0 + 32 >= col1 || n0 + 32 >= g.features) release();
         float v[32];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
@@ -235,11 +253,9 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           if (m >= g.tokens) continue;
           __nv_bfloat16* out = g.out + m * g.ld_out + at;
           if (g.residual) {
-            const uint4* rp = reinterpret_cast<const uint4*>(g.residual + m * g.ld_res + n0);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const uint4 r4 = rp[q];
-              const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
+              const uint32_t rw[4] = {res[q].x, res[q].y, res[q].z, res[q].w};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 v[8 * q + 2 * j] += bf16_bits_to_float(rw[j] & 0xFFFF);
@@ -247,6 +263,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
               }
             }
           }
+          fetch(c0 + 32);
           uint32_t w[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
@@ -280,16 +297,14 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(acc_empty_leader[acc]);  // both accumulator halves may be overwritten after all of these
+      if (!gone && nt * BN + col0 >= g.features) release();  // (nothing of the tile is this warp's)
     }
   }
 
   // both CTAs stay until nobody can touch the other's barriers or TMEM any more
   __syncwarp();
   tc_fence_before();
-  cluster_sync_all();
+  cluster_meet();
   tc_fence_after();
   if (warp == 1) tmem_dealloc_pair(tmem_base, TMEM_COLS);
 }
