@@ -8,7 +8,7 @@
 //
 // Memory-bound: x and the residual are read once, h and the integers written once; a row waits for its statistics in the registers of a block as fp32, or, where
 // many wide rows need more of them in flight than registers hold, in shared memory.  Measured (us, and of the floor at 6549 GB/s): 8192 x 4096 bf16 17.8 (0.86),
-// its RMSNorm 24.8 (0.62), with a residual 37.4 (0.96), LayerNorm with a residual 41 (0.87); 8192 x 11008 46.8 (0.88).  What is above is instructions (unpacking,
+// its RMSNorm 20.6 (0.75), with a residual 37.4 (0.96), LayerNorm 27.8 (0.55), with a residual 41 (0.87); 8192 x 11008 46.8 (0.88).  What is above is instructions (unpacking,
 // maxima, the integers: about 20 per element with a row's own share, most on the half-rate pipe), and 2 us of launch and first latency.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -351,6 +351,115 @@ rows_int8_kernel(const RiParams p, float one) {
   }
 }
 
+// Norms of many aligned bf16 rows without a residual: persistent blocks that keep the weights in registers and have the next row on its way while they work on
+// one.  The exchanges alternate between two sets of shared memory, so that a row of an RMSNorm has one barrier.  At most as many blocks as rows.
+constexpr int ri_walk_threads(int v, int threads) { return v == 2 ? 1024 : threads <= 128 ? 640 : 512; }  // of an SM, by what a thread needs in registers
+template <int MODE, int V, int THREADS>
+__global__ void __launch_bounds__(THREADS, ri_walk_threads(V, THREADS) / THREADS)
+rows_int8_walk_kernel(const RiParams p, float one) {
+  __shared__ float sums[2][2][32];
+  __shared__ uint32_t maxima[2][32];
+  const bf16* weight = static_cast<const bf16*>(p.weight);
+  const bf16* bias = static_cast<const bf16*>(p.bias);
+  pdl_trigger();  // (see rows_int8_kernel)
+  pdl_wait();
+  Ri8<bf16> next[V], w[V];
+  const bf16* x = static_cast<const bf16*>(p.x) + blockIdx.x * p.ldx;  // (of the row on its way)
+  const long long step_x = (long long)gridDim.x * p.ldx, step_q = (long long)gridDim.x * p.ldq;
+  int8_t* q = p.q + blockIdx.x * p.ldq;
+#pragma unroll
+  for (int i = 0; i < V; ++i) next[i] = ri_load<bf16, true>(x, ri_col(0, i), p.cols);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (weight) {
+      w[i] = ri_load<bf16, true>(weight, ri_col(0, i), p.cols);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[i].w[j] = 0x3F803F80u;  // ones
+    }
+  }
+  int buffer = 0;
+  for (int row = blockIdx.x; row < p.rows; row += gridDim.x, q += step_q, buffer ^= 1) {
+    float2 v[V][4];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = make_float2(next[i].get(2 * j), next[i].get(2 * j + 1));
+    x += step_x;
+    if (row + int(gridDim.x) < p.rows) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) next[i] = ri_load<bf16, true>(x, ri_col(0, i), p.cols);
+    }
+    float sum = 0.f, rstd = 1.f;
+    uint32_t most = 0;
+    if (MODE == RI_RMS) {
+      float2 squares = both(0.f);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) squares = __ffma2_rn(v[i][j], v[i][j], squares);
+      sum = squares.x + squares.y;
+    }
+    if (MODE == RI_LAYER) {
+      float2 total = both(0.f);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) total = __fadd2_rn(total, v[i][j]);
+      sum = total.x + total.y;
+      // (the deviations are summed up around the mean: a difference of two sums would lose the digits that they share)
+      ri_reduce<true, false>(sum, most, sums[0][buffer], maxima[buffer]);
+      const float mean = sum / float(p.cols);
+      float2 around = both(0.f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool in = ri_col(0, i) < p.cols;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[i][j] = in ? __fadd2_rn(v[i][j], both(-mean)) : both(0.f);
+          around = __ffma2_rn(v[i][j], v[i][j], around);
+        }
+      }
+      float squares = around.x + around.y;
+      ri_reduce<true, false>(squares, most, sums[1][buffer], maxima[buffer]);
+      rstd = rsqrtf(squares / float(p.cols) + p.eps);
+    }
+    float most0 = 0.f, most1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      Ri8<bf16> b;
+      if (MODE == RI_LAYER && bias) b = ri_load<bf16, true>(bias, ri_col(0, i), p.cols);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (MODE == RI_LAYER) v[i][j] = __fmul2_rn(v[i][j], both(rstd));
+        v[i][j] = __fmul2_rn(v[i][j], make_float2(w[i].get(2 * j), w[i].get(2 * j + 1)));
+        if (MODE == RI_LAYER && bias) v[i][j] = __fadd2_rn(v[i][j], make_float2(b.get(2 * j), b.get(2 * j + 1)));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        most0 = fmax3_abs_nan(most0, v[i][j].x, v[i][j].y);
+        most1 = fmax3_abs_nan(most1, v[i][j + 1].x, v[i][j + 1].y);
+      }
+    }
+    most = __float_as_uint(fmax3_abs_nan(most0, most1, 0.f));
+    ri_reduce<MODE == RI_RMS, true>(sum, most, sums[0][buffer], maxima[buffer]);
+    const bool finite = most < 0x7F800000u;
+    const float amax = fmaxf(__uint_as_float(most), RI_LEAST);
+    const float inv = __fdiv_rn(127.f, amax);
+    if (threadIdx.x == 0) {
+      const float scale = amax / 127.f * (MODE == RI_RMS ? rsqrtf(sum / float(p.cols) + p.eps) : 1.f);
+      p.scales[row] = finite ? scale : __int_as_float(0x7FC00000);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      uint2 u = make_uint2(ri_integers(v[i][0], v[i][1], inv, one), ri_integers(v[i][2], v[i][3], inv, one));
+      if (!finite) u = make_uint2(0, 0);
+      const int c = ri_col(0, i);
+      if (c < p.cols) *reinterpret_cast<uint2*>(q + c) = u;
+    }
+  }
+}
+
 // ---- many wide rows: persistent groups of threads, rows arriving by bulk copies several ahead -------------------------------------------------------
 
 __device__ __forceinline__ void ri_bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -604,12 +713,16 @@ static bool ri_ring_launch(const RiParams& p, int sms, cudaStream_t stream, cuda
 //   + residual 8192 x 4096 37.4 / 37.8 / -     8192 x 8192 81 / 72 / -        8192 x 11008 - / 109 / 112    300 x 5120 4.0 / 4.5 / -       300 x 8192 6.0 / 5.4 / -
 //              8192 x 16392 - / 205 / 163      8192 x 20000 - / 222 / 312     8 x 16392 5.0 / 3.6 / -
 //   LayerNorm  8192 x 2560 22.5 / 22.9 / -     8192 x 3584 31.6 / 29.6 / -    8192 x 4096 37.2 / 30.3 / -   8192 x 8192 78 / 60 / -        8192 x 11008 - / 94 / 107
+// Norms without a residual of many rows, a block a row / persistent blocks with 16 columns a thread / with 32 (rows_int8_walk_kernel):
+//   RMSNorm    16384 x 512 7.2 / 7.7 / 8.5     16384 x 1024 13.7 / 12.3 / 10.5   2400 x 1024 3.8 / 4.0 / 4.0    8192 x 2048 13.6 / 11.2 / 11.8   8192 x 4096 25.0 / 20.6 / 21.0
+//              8192 x 5120 31.4 / 25.3 / 25.8  8192 x 8192 46.7 / 38.2 / 38.6    8192 x 11008 60 / 75 / 58      8192 x 16384 87 / 90 / 74
+//   LayerNorm  16384 x 1024 20.0 / 15.7 / 12.1 8192 x 2560 22.5 / 19.8 / 22.3    8192 x 4096 30.6 / 29.8 / 27.8 8192 x 8192 61 / 60 / 47         8192 x 16384 122 / 122 / 98
 // Other rows (fp32, or of any alignment), 16 columns / ring: RMSNorm with a residual 4096 x 8192 42.7 / 45.2; 4096 x 11008 30.7 / 25.9, RMSNorm 58 / 35.
 template <typename T, int MODE, bool VEC>
 static bool ri_ring(const RiParams& p, int sms) {
   if (!VEC || sizeof(T) != 2 || p.cols > 32768) return p.rows >= 2 * sms && p.cols > (p.residual || MODE == RI_LAYER ? 8192 : 4096);
   if (MODE == RI_ROWS) return p.cols > 8192 && p.rows >= (p.cols > 16384 ? 4 : 12) * sms;
-  return MODE == RI_RMS && !p.residual && p.cols > 4096 && p.rows >= 16 * sms;
+  return MODE == RI_RMS && !p.residual && p.cols > 16384 && p.rows >= 16 * sms;
 }
 template <typename T, int MODE, bool VEC>
 static bool ri_four(const RiParams& p, int sms) {
@@ -622,6 +735,21 @@ static cudaError_t ri_launch(const RiParams& p, int sms, cudaStream_t stream) {
   cudaError_t e;
   if (ri_ring<T, MODE, VEC>(p, sms) && ri_ring_launch<T, MODE>(p, sms, stream, &e)) return e;
   const int groups = (p.cols + 7) / 8;
+  if constexpr (VEC && sizeof(T) == 2 && MODE != RI_ROWS) {
+    if (!p.residual && p.cols >= 768 && p.cols <= 16384 && p.rows >= (p.cols > 1024 ? 16 : 32) * sms) {
+      auto walk = [&](auto kernel, int v, int most) {
+        const int threads = ((groups + v - 1) / v + 31) / 32 * 32, blocks = ri_walk_threads(v, most) / threads * sms;
+        return launch_dependent(kernel, dim3(blocks < p.rows ? blocks : p.rows), dim3(threads), 0, stream, true, p, 1.f);
+      };
+      if (p.cols <= 1024) return walk(rows_int8_walk_kernel<MODE, 4, 32>, 4, 32);
+      if (p.cols <= 2048) return walk(rows_int8_walk_kernel<MODE, 2, 128>, 2, 128);
+      if constexpr (MODE == RI_LAYER) {
+        if (p.cols > 3584 && p.cols <= 4096) return walk(rows_int8_walk_kernel<MODE, 4, 128>, 4, 128);
+      }
+      if (p.cols <= 4096) return walk(rows_int8_walk_kernel<MODE, 2, 256>, 2, 256);
+      return p.cols <= 8192 ? walk(rows_int8_walk_kernel<MODE, 4, 256>, 4, 256) : walk(rows_int8_walk_kernel<MODE, 4, 512>, 4, 512);
+    }
+  }
   const int v = groups <= 32 ? 1 : ri_four<T, MODE, VEC>(p, sms) ? 4 : 2;
   int threads = ((groups + v - 1) / v + 31) / 32 * 32;
   const bool wide = threads > RI_MAX_THREADS;
@@ -671,7 +799,17 @@ static cudaError_t ri_preload() {
     LOAD(rows_int8_kernel<T, MODE, 4, true, false, 256>);
     LOAD(rows_int8_kernel<T, MODE, 4, true, false, 512>);
     LOAD(rows_int8_kernel<T, MODE, 4, true, false, 1024>);
-    if constexpr (MODE == RI_LAYER) LOAD(rows_int8_kernel<T, MODE, 4, true, false, 128>);
+    if constexpr (MODE == RI_LAYER) {
+      LOAD(rows_int8_kernel<T, MODE, 4, true, false, 128>);
+      LOAD(rows_int8_walk_kernel<MODE, 4, 128>);
+    }
+    if constexpr (MODE != RI_ROWS) {
+      LOAD(rows_int8_walk_kernel<MODE, 4, 32>);
+      LOAD(rows_int8_walk_kernel<MODE, 2, 128>);
+      LOAD(rows_int8_walk_kernel<MODE, 2, 256>);
+      LOAD(rows_int8_walk_kernel<MODE, 4, 256>);
+      LOAD(rows_int8_walk_kernel<MODE, 4, 512>);
+    }
   }
 #undef LOAD
   return e;

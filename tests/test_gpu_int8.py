@@ -576,3 +576,29 @@ def test_every_width_of_the_pair_tile(width, act):
         bias = torch.randn(features, device="cuda", generator=_gen(5)).to(BF16)
         residual = None if act else torch.randn(tokens, features, device="cuda", generator=_gen(6)).to(BF16)
         _check_product(x, w, bias, act, residual)
+
+
+@pytest.mark.parametrize("weighted", [True, False])
+@pytest.mark.parametrize("cols,sms", [(768, 33), (1000, 33), (1024, 40), (1032, 17), (1536, 17), (2048, 70), (2056, 17), (3584, 17), (3592, 17), (4096, 40), (4104, 17), (8192, 17), (8200, 17), (16384, 17)])
+def test_norms_without_a_residual_of_many_rows(cols, sms, weighted):
+    rows = sms * torch.cuda.get_device_properties(0).multi_processor_count + 1
+    pitch = cols + 24
+    x = _wave(rows, pitch, BF16, cols).as_strided((rows, cols), (pitch, 1), 8)
+    x[1], x[rows - 1, 0], x[2, cols - 1] = 0, float("inf"), float("nan")
+    w, b = ((1 + 0.1 * torch.randn(cols, device="cuda", generator=_gen(3))).to(BF16), (0.1 * torch.randn(cols, device="cuda", generator=_gen(4))).to(BF16)) if weighted else (None, None)
+    (q, s), _ = OF.rms_norm_int8(x, w, 1e-5)
+    v = x.float() if w is None else x.float() * w.float()
+    want = OF.rms_norm_int8_ref(x, w, 1e-5)[0]
+    assert torch.equal(q, want.values)
+    scale = v.abs().amax(1).clamp_min(1e-30).double() / 127 * torch.rsqrt((x.float() * x.float()).sum(1, dtype=torch.float64) / cols + 1e-5)
+    finite = scale.isfinite()
+    assert finite.sum() == rows - 2 and s[~finite].isnan().all() and not q[~finite].any()
+    torch.testing.assert_close(s[finite].double(), scale[finite], rtol=64 * 2.0 ** -24, atol=0)  # (as in test_rms_norm_of_many_wide_rows)
+    (q, s), _ = OF.layer_norm_int8(x, w, b, 1e-5)
+    assert s[~finite].isnan().all() and not q[~finite].any()
+    xd = x[finite].double()
+    y = torch.nn.functional.layer_norm(xd, (cols,), None if w is None else w.double(), None if b is None else b.double(), 1e-5)
+    step = y.abs().amax(1, keepdim=True).clamp_min(1e-30) / 127
+    back = q[finite].double() * s[finite].double()[:, None]
+    slack = 80 * 2.0 ** -24 * xd.abs().amax(1, keepdim=True) * torch.rsqrt(xd.var(1, unbiased=False, keepdim=True) + 1e-5) * 1.5
+    assert ((back - y).abs() <= 0.501 * step + slack).all()  # (as in test_layer_norm_rows)
