@@ -6,10 +6,11 @@
 // the scale: the integers depend on no order of summation, and a row needs one exchange (sum of squares and maximum together) instead of two.
 // A row with a value that is not finite gets integers 0 and the scale NaN, so that everything computed from it is NaN.
 //
-// Memory-bound: x and the residual are read once, h and the integers written once; a row waits for its statistics in the registers of a block as fp32, or, where
-// many wide rows need more of them in flight than registers hold, in shared memory.  Measured (us, and of the floor at 6549 GB/s): 8192 x 4096 bf16 17.8 (0.86),
-// its RMSNorm 20.6 (0.75), with a residual 37.4 (0.96), LayerNorm 27.8 (0.55), with a residual 41 (0.87); 8192 x 11008 46.8 (0.88).  What is above is instructions (unpacking,
-// maxima, the integers: about 20 per element with a row's own share, most on the half-rate pipe), and 2 us of launch and first latency.
+// Memory-bound: x and the residual are read once, h and the integers written once.  A row waits for its statistics in registers as fp32: in a block of its own, in
+// a persistent block that has the next row on its way (norms of many rows), or, where many wide rows need more of them in flight than registers hold, in shared
+// memory.  Measured (us, and of the floor at 6549 GB/s), 8192 x 4096 bf16: rows 17.8 (0.86), RMSNorm 20.6 (0.75), with a residual 37.3 (0.96), LayerNorm 27.8 (0.55),
+// with a residual 39.0 (0.92); 8192 x 11008 rows 46.8 (0.88).  What is above is instructions (unpacking, maxima, the integers, most of them on the half-rate
+// pipe; a LayerNorm meets three times), and 2 us of launch and first latency.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -178,7 +179,7 @@ __device__ __forceinline__ uint32_t ri_integers(float2 v0, float2 v1, float inv,
 // instead of 24.8; with 32 columns a thread, 11008 wide, two blocks of 512 instead of one 76 us instead of 116).
 template <typename T, int MODE, int V, bool VEC>
 constexpr int ri_blocks(int threads) {
-  if (V == 4) return threads > 256 ? 1024 / threads : 768 / threads;
+  if (V == 4) return threads > 256 ? 1024 / threads : 3;
   return threads != 256 || !VEC ? 1 : MODE == RI_LAYER ? 4 : V == 1 ? 6 : sizeof(T) == 4 ? 4 : MODE == RI_ROWS ? 8 : 6;
 }
 
@@ -351,11 +352,13 @@ rows_int8_kernel(const RiParams p, float one) {
   }
 }
 
-// Norms of many aligned bf16 rows without a residual: persistent blocks that keep the weights in registers and have the next row on its way while they work on
+// Norms of many aligned bf16 rows: persistent blocks that keep the weights in registers and have the next row (TWO: and its residual) on its way while they work on
 // one.  The exchanges alternate between two sets of shared memory, so that a row of an RMSNorm has one barrier.  At most as many blocks as rows.
-constexpr int ri_walk_threads(int v, int threads) { return v == 2 ? 1024 : threads <= 128 ? 640 : 512; }  // of an SM, by what a thread needs in registers
-template <int MODE, int V, int THREADS>
-__global__ void __launch_bounds__(THREADS, ri_walk_threads(V, THREADS) / THREADS)
+constexpr int ri_walk_threads(int v, int threads, bool two) {  // of an SM, by what a thread needs in registers
+  return v == 2 ? (two ? 768 : 1024) : threads <= 128 && !two ? 640 : 512;
+}
+template <int MODE, int V, int THREADS, bool TWO>
+__global__ void __launch_bounds__(THREADS, ri_walk_threads(V, THREADS, TWO) / THREADS)
 rows_int8_walk_kernel(const RiParams p, float one) {
   __shared__ float sums[2][2][32];
   __shared__ uint32_t maxima[2][32];
@@ -363,12 +366,17 @@ rows_int8_walk_kernel(const RiParams p, float one) {
   const bf16* bias = static_cast<const bf16*>(p.bias);
   pdl_trigger();  // (see rows_int8_kernel)
   pdl_wait();
-  Ri8<bf16> next[V], w[V];
+  Ri8<bf16> next[V], next2[TWO ? V : 1], w[V];
   const bf16* x = static_cast<const bf16*>(p.x) + blockIdx.x * p.ldx;  // (of the row on its way)
   const long long step_x = (long long)gridDim.x * p.ldx, step_q = (long long)gridDim.x * p.ldq;
   int8_t* q = p.q + blockIdx.x * p.ldq;
+  const bf16* r = TWO ? static_cast<const bf16*>(p.residual) + blockIdx.x * p.ldr : nullptr;
+  bf16* h = TWO && p.sum_out ? static_cast<bf16*>(p.sum_out) + blockIdx.x * p.lds : nullptr;
 #pragma unroll
-  for (int i = 0; i < V; ++i) next[i] = ri_load<bf16, true>(x, ri_col(0, i), p.cols);
+  for (int i = 0; i < V; ++i) {
+    next[i] = ri_load<bf16, true>(x, ri_col(0, i), p.cols);
+    if (TWO) next2[i] = ri_load<bf16, true>(r, ri_col(0, i), p.cols);
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (weight) {
@@ -381,6 +389,17 @@ rows_int8_walk_kernel(const RiParams p, float one) {
   int buffer = 0;
   for (int row = blockIdx.x; row < p.rows; row += gridDim.x, q += step_q, buffer ^= 1) {
     float2 v[V][4];
+    if (TWO) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        // rounded to the type it is stored in: the norm is taken of what later kernels read
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) next[i].set2(j, next[i].get(j) + next2[i].get(j), next[i].get(j + 1) + next2[i].get(j + 1));
+        if (h) ri_store<bf16, true>(h, ri_col(0, i), p.cols, next[i], nullptr);
+      }
+      if (h) h += (long long)gridDim.x * p.lds;
+      r += (long long)gridDim.x * p.ldr;
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
@@ -388,7 +407,10 @@ rows_int8_walk_kernel(const RiParams p, float one) {
     x += step_x;
     if (row + int(gridDim.x) < p.rows) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) next[i] = ri_load<bf16, true>(x, ri_col(0, i), p.cols);
+      for (int i = 0; i < V; ++i) {
+        next[i] = ri_load<bf16, true>(x, ri_col(0, i), p.cols);
+        if (TWO) next2[i] = ri_load<bf16, true>(r, ri_col(0, i), p.cols);
+      }
     }
     float sum = 0.f, rstd = 1.f;
     uint32_t most = 0;
@@ -713,10 +735,13 @@ static bool ri_ring_launch(const RiParams& p, int sms, cudaStream_t stream, cuda
 //   + residual 8192 x 4096 37.4 / 37.8 / -     8192 x 8192 81 / 72 / -        8192 x 11008 - / 109 / 112    300 x 5120 4.0 / 4.5 / -       300 x 8192 6.0 / 5.4 / -
 //              8192 x 16392 - / 205 / 163      8192 x 20000 - / 222 / 312     8 x 16392 5.0 / 3.6 / -
 //   LayerNorm  8192 x 2560 22.5 / 22.9 / -     8192 x 3584 31.6 / 29.6 / -    8192 x 4096 37.2 / 30.3 / -   8192 x 8192 78 / 60 / -        8192 x 11008 - / 94 / 107
-// Norms without a residual of many rows, a block a row / persistent blocks with 16 columns a thread / with 32 (rows_int8_walk_kernel):
+// Norms of many rows, a block a row / persistent blocks with 16 columns a thread / with 32 (rows_int8_walk_kernel; the better of both in the last two lines):
 //   RMSNorm    16384 x 512 7.2 / 7.7 / 8.5     16384 x 1024 13.7 / 12.3 / 10.5   2400 x 1024 3.8 / 4.0 / 4.0    8192 x 2048 13.6 / 11.2 / 11.8   8192 x 4096 25.0 / 20.6 / 21.0
 //              8192 x 5120 31.4 / 25.3 / 25.8  8192 x 8192 46.7 / 38.2 / 38.6    8192 x 11008 60 / 75 / 58      8192 x 16384 87 / 90 / 74
 //   LayerNorm  16384 x 1024 20.0 / 15.7 / 12.1 8192 x 2560 22.5 / 19.8 / 22.3    8192 x 4096 30.6 / 29.8 / 27.8 8192 x 8192 61 / 60 / 47         8192 x 16384 122 / 122 / 98
+//   fewer rows 1200 x 2048 3.8 / 3.4 / -       1200 x 5120 7.4 / - / 5.5         600 x 11008 8.4 / - / 6.5
+//   + residual 600 x 2048 4.2 / 3.5, 1200 x 8192 14.1 / 13.0, 8192 x 4096 37.5 / 37.9, 8192 x 8192 72.6 / 77.5; LayerNorm 8192 x 1024 14.3 / 11.7, 8192 x 5120 55 / 49,
+//              16384 x 4096 76.7 / 80.1, 2400 x 16384 60 / 48
 // Other rows (fp32, or of any alignment), 16 columns / ring: RMSNorm with a residual 4096 x 8192 42.7 / 45.2; 4096 x 11008 30.7 / 25.9, RMSNorm 58 / 35.
 template <typename T, int MODE, bool VEC>
 static bool ri_ring(const RiParams& p, int sms) {
@@ -727,7 +752,13 @@ static bool ri_ring(const RiParams& p, int sms) {
 template <typename T, int MODE, bool VEC>
 static bool ri_four(const RiParams& p, int sms) {
   if (!VEC || sizeof(T) != 2 || p.cols > 32768) return false;
-  return p.cols > 16384 || (p.rows >= (p.cols > 6144 ? 2 : 4) * sms && p.cols >= (MODE == RI_LAYER ? 3584 : 4097));
+  return p.cols > 16384 || (p.rows >= (p.cols > 6144 ? 2 : 4) * sms && p.cols > 4096);
+}
+
+template <int MODE>
+static bool ri_walk(const RiParams& p, int sms) {
+  if (p.cols < 768 || p.cols > 16384 || p.rows < (p.cols > 1024 ? 4 : 32) * sms) return false;
+  return MODE == RI_LAYER || !p.residual || p.cols <= 1024 || p.rows <= 32 * sms;
 }
 
 template <typename T, int MODE, bool VEC>
@@ -736,18 +767,20 @@ static cudaError_t ri_launch(const RiParams& p, int sms, cudaStream_t stream) {
   if (ri_ring<T, MODE, VEC>(p, sms) && ri_ring_launch<T, MODE>(p, sms, stream, &e)) return e;
   const int groups = (p.cols + 7) / 8;
   if constexpr (VEC && sizeof(T) == 2 && MODE != RI_ROWS) {
-    if (!p.residual && p.cols >= 768 && p.cols <= 16384 && p.rows >= (p.cols > 1024 ? 16 : 32) * sms) {
+    if (ri_walk<MODE>(p, sms)) {
       auto walk = [&](auto kernel, int v, int most) {
-        const int threads = ((groups + v - 1) / v + 31) / 32 * 32, blocks = ri_walk_threads(v, most) / threads * sms;
+        const int threads = ((groups + v - 1) / v + 31) / 32 * 32, blocks = ri_walk_threads(v, most, p.residual) / threads * sms;
         return launch_dependent(kernel, dim3(blocks < p.rows ? blocks : p.rows), dim3(threads), 0, stream, true, p, 1.f);
       };
-      if (p.cols <= 1024) return walk(rows_int8_walk_kernel<MODE, 4, 32>, 4, 32);
-      if (p.cols <= 2048) return walk(rows_int8_walk_kernel<MODE, 2, 128>, 2, 128);
+#define WALK(V, N) (p.residual ? walk(rows_int8_walk_kernel<MODE, V, N, true>, V, N) : walk(rows_int8_walk_kernel<MODE, V, N, false>, V, N))
+      if (p.cols <= 1024) return WALK(4, 32);
+      if (p.cols <= 2048) return WALK(2, 128);
       if constexpr (MODE == RI_LAYER) {
-        if (p.cols > 3584 && p.cols <= 4096) return walk(rows_int8_walk_kernel<MODE, 4, 128>, 4, 128);
+        if (p.cols > 3584 && p.cols <= 4096) return WALK(4, 128);
       }
-      if (p.cols <= 4096) return walk(rows_int8_walk_kernel<MODE, 2, 256>, 2, 256);
-      return p.cols <= 8192 ? walk(rows_int8_walk_kernel<MODE, 4, 256>, 4, 256) : walk(rows_int8_walk_kernel<MODE, 4, 512>, 4, 512);
+      if (p.cols <= 4096) return WALK(2, 256);
+      return p.cols <= 8192 ? WALK(4, 256) : WALK(4, 512);
+#undef WALK
     }
   }
   const int v = groups <= 32 ? 1 : ri_four<T, MODE, VEC>(p, sms) ? 4 : 2;
@@ -758,9 +791,6 @@ static cudaError_t ri_launch(const RiParams& p, int sms, cudaStream_t stream) {
   const dim3 block(threads, rows_per_block), grid((unsigned(p.rows) + rows_per_block - 1) / rows_per_block);
   auto go = [&](auto kernel) { return launch_dependent(kernel, grid, block, 0, stream, true, p, 1.f); };
   if constexpr (VEC && sizeof(T) == 2) {
-    if constexpr (MODE == RI_LAYER) {
-      if (v == 4 && threads <= 128) return go(rows_int8_kernel<T, MODE, 4, true, false, 128>);
-    }
     if (v == 4)
       return threads <= 256   ? go(rows_int8_kernel<T, MODE, 4, true, false, 256>)
              : threads <= 512 ? go(rows_int8_kernel<T, MODE, 4, true, false, 512>)
@@ -799,16 +829,17 @@ static cudaError_t ri_preload() {
     LOAD(rows_int8_kernel<T, MODE, 4, true, false, 256>);
     LOAD(rows_int8_kernel<T, MODE, 4, true, false, 512>);
     LOAD(rows_int8_kernel<T, MODE, 4, true, false, 1024>);
-    if constexpr (MODE == RI_LAYER) {
-      LOAD(rows_int8_kernel<T, MODE, 4, true, false, 128>);
-      LOAD(rows_int8_walk_kernel<MODE, 4, 128>);
-    }
     if constexpr (MODE != RI_ROWS) {
-      LOAD(rows_int8_walk_kernel<MODE, 4, 32>);
-      LOAD(rows_int8_walk_kernel<MODE, 2, 128>);
-      LOAD(rows_int8_walk_kernel<MODE, 2, 256>);
-      LOAD(rows_int8_walk_kernel<MODE, 4, 256>);
-      LOAD(rows_int8_walk_kernel<MODE, 4, 512>);
+#define LOAD_WALK(V, N) LOAD(rows_int8_walk_kernel<MODE, V, N, false>); LOAD(rows_int8_walk_kernel<MODE, V, N, true>)
+      LOAD_WALK(4, 32);
+      LOAD_WALK(2, 128);
+      LOAD_WALK(2, 256);
+      LOAD_WALK(4, 256);
+      LOAD_WALK(4, 512);
+      if constexpr (MODE == RI_LAYER) {
+        LOAD_WALK(4, 128);
+      }
+#undef LOAD_WALK
     }
   }
 #undef LOAD

@@ -602,3 +602,18 @@ def test_norms_without_a_residual_of_many_rows(cols, sms, weighted):
     back = q[finite].double() * s[finite].double()[:, None]
     slack = 80 * 2.0 ** -24 * xd.abs().amax(1, keepdim=True) * torch.rsqrt(xd.var(1, unbiased=False, keepdim=True) + 1e-5) * 1.5
     assert ((back - y).abs() <= 0.501 * step + slack).all()  # (as in test_layer_norm_rows)
+
+
+@pytest.mark.parametrize("cols,sms", [(1024, 33), (2048, 5), (4096, 5), (8192, 5), (11008, 5), (4096, 40), (20000, 3)])
+def test_the_sum_of_many_rows_in_place(cols, sms):
+    nat = _native()
+    x = _many(cols, sms, BF16, cols)
+    res = _wave(*x.shape, BF16, cols + 1)
+    for norm, ref in ((0, lambda: OF.rms_norm_int8_ref(x, None, 1e-5, res)), (1, lambda: OF.layer_norm_int8(x, None, None, 1e-5, res))):
+        (wq, _), wh = ref()
+        for target in ("x", "residual"):
+            a, b = x.clone(), res.clone()
+            into = a if target == "x" else b
+            q, _ = nat.rows_int8(a, eps=1e-5, norm=norm, residual=b, sum_out=into)
+            assert torch.equal(q, wq)
+            torch.testing.assert_close(into, wh, rtol=0, atol=0, equal_nan=True)
