@@ -303,6 +303,14 @@ def geglu(gate, up, approximate: str = "tanh"):
 # -- 8-bit integers (serving) --------------------------------------------------------------------
 
 
+def _not_taken(*args):
+    return None
+
+
+# The ordinary calls, as the native module takes them once it is loaded: its results, or None for a call that needs a check's words or a copy.
+quantize_int8_directly = norm_int8_directly = linear_int8_directly = _not_taken
+
+
 def _serving_only(what: str, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
@@ -327,10 +335,10 @@ def quantize_int8(x) -> Int8Rows:
     """The rows of ``x`` (bf16 or fp32, ``[..., cols]``) in 8 bits: ``rint(x * (127 / max |x|))`` and ``max |x| / 127``, ties to even.  For an activation
     in front of :func:`linear_int8`, and for its weight (a row per output channel).  A row with a value that is not finite gets the scale NaN.
     Serving only: there is no gradient."""
-    nat = _native(x)
-    out = None if nat is None else nat.quantize_int8_directly(x)
+    out = quantize_int8_directly(x)
     if out is not None:
         return out
+    nat = _native(x)
     _check_rows("quantize_int8", x)
     return quantize_int8_ref(x) if nat is None or transformed(x) else nat.quantize_int8(x)
 
@@ -338,20 +346,20 @@ def quantize_int8(x) -> Int8Rows:
 def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
     """``(rows, h)``: ``h = x + residual``, rounded to the type of ``x`` (``x`` itself without a residual), and its RMSNorm in 8 bits, as
     :func:`quantize_int8` gives them.  ``weight`` may be None."""
-    nat = _native(x)
-    out = None if nat is None else nat.norm_int8_directly(x, weight, None, eps, 0, residual)
+    out = norm_int8_directly(x, weight, None, eps, 0, residual)
     if out is not None:
         return out
+    nat = _native(x)
     _check_rows("rms_norm_int8", x, weight, residual=residual)
     return rms_norm_int8_ref(x, weight, eps, residual) if nat is None or transformed(x) else nat.norm_int8(x, weight, None, eps, 0, residual)
 
 
 def layer_norm_int8(x, weight, bias, eps: float = 1e-5, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
     """Like :func:`rms_norm_int8`, with a LayerNorm; ``weight`` and ``bias`` may be None."""
-    nat = _native(x)
-    out = None if nat is None else nat.norm_int8_directly(x, weight, bias, eps, 1, residual)
+    out = norm_int8_directly(x, weight, bias, eps, 1, residual)
     if out is not None:
         return out
+    nat = _native(x)
     _check_rows("layer_norm_int8", x, weight, bias, residual)
     return layer_norm_int8_ref(x, weight, bias, eps, residual) if nat is None or transformed(x) else nat.norm_int8(x, weight, bias, eps, 1, residual)
 
@@ -386,10 +394,10 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias=None, act: Optional[str] = N
     products are exact integers, scales, bias, activation and residual are fp32.  ``act``: None, ``"relu"``, ``"gelu"``, ``"gelu_tanh"``, ``"silu"``, or
     ``"swiglu16"`` for a weight whose rows alternate in groups of 16 gate and 16 up rows (``silu(gate) * up``, half as many columns).  Serving only:
     there is no gradient."""
-    nat = _native(x[0])
-    out = None if nat is None else nat.linear_int8_directly(x, weight, bias, act, residual)
+    out = linear_int8_directly(x, weight, bias, act, residual)
     if out is not None:
         return out
+    nat = _native(x[0])
     _check_linear_int8(x, weight, bias, act, residual)
     if nat is None or transformed(x[0]) or transformed(x[1]):
         return linear_int8_ref(Int8Rows(*x), Int8Rows(*weight), bias, act, residual)

@@ -1033,17 +1033,10 @@ def norm_int8(x, weight, bias, eps, mode, residual=None):
 
 
 # The calls that need neither a check's words nor a copy, by the C++ module (which leaves all others: None).
-
-
-def _left(*args):
-    return None
-
-
-if AUTOGRAD is None:
-    quantize_int8_directly = norm_int8_directly = linear_int8_directly = _left
-else:
+if AUTOGRAD is not None:
     AUTOGRAD.bind_int8(OF.Int8Rows, {act: ACT_CODES[act] for act in OF.INT8_ACTS})
-    quantize_int8_directly, norm_int8_directly, linear_int8_directly = AUTOGRAD.quantize_int8, AUTOGRAD.norm_int8, AUTOGRAD.linear_int8
+    if not OF._FORCE_TORCH:
+        OF.quantize_int8_directly, OF.norm_int8_directly, OF.linear_int8_directly = AUTOGRAD.quantize_int8, AUTOGRAD.norm_int8, AUTOGRAD.linear_int8
 
 
 def gemm_int8(x: OF.Int8Rows, weight: OF.Int8Rows, bias=None, act=None, residual=None, out=None, early=False):
