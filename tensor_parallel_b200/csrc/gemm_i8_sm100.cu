@@ -208,7 +208,16 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
 #pragma unroll
         for (int q = 0; q < 4; ++q) res[q] = rp[q];
       };
-      fetch(col0);
+      // of half a chunk, where it leaves through shared memory: rows lane / 16, + 2, .. of one column (addresses past the end are drawn back, see i8_residual)
+      uint16_t turned[16];
+      auto fetch_turned = [&](int c) {
+        if (!g.residual || nt * BN + c >= g.features) return;
+        const uint16_t* rp = reinterpret_cast<const uint16_t*>(g.residual) + min(nt * BN + c + (lane & 15), g.features - 1);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) turned[i] = rp[min(m0 + (lane >> 4) + 2 * i, g.tokens - 1) * g.ld_res];
+      };
+      if (vec) fetch(col0);
+      else fetch_turned(col0);
       asm volatile("bar.sync 1, %0;" ::"n"(32 * IP_EPI_WARPS) : "memory");
       const bool ready = !*abort_flag && mbar_wait(&acc_full[acc], (local >> 1) & 1);
       if (!__all_sync(0xffffffffu, ready)) {
@@ -282,18 +291,20 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (16 * h >= cols) break;
+            if (vec) fetch_turned(c0 + 16 * h);
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < 16; ++j) mine[lane * IP_TURN_PITCH + j] = v[16 * h + j];
             __syncwarp();
             const int c = at + 16 * h + (lane & 15);
-#pragma unroll 4
-            for (int i = lane >> 4; i < 32; i += 2) {
-              if (m0 + i >= g.tokens || c >= last) continue;
-              float x = mine[i * IP_TURN_PITCH + (lane & 15)];
-              if (g.residual) x += __bfloat162float(g.residual[(m0 + i) * g.ld_res + c]);
-              g.out[(m0 + i) * g.ld_out + c] = __float2bfloat16(x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int row = (lane >> 4) + 2 * i;
+              float x = mine[row * IP_TURN_PITCH + (lane & 15)];
+              if (g.residual) x += bf16_bits_to_float(turned[i]);
+              if (m0 + row < g.tokens && c < last) g.out[(m0 + row) * g.ld_out + c] = __float2bfloat16(x);
             }
+            if (!vec && c0 + 16 * h + 16 < col1) fetch_turned(c0 + 16 * h + 16);
           }
         }
       }
