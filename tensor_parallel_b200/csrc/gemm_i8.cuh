@@ -33,6 +33,21 @@ __device__ __forceinline__ float i8_value(int sum, float sx, float sw, float bia
 // x sigmoid(u).  The hardware's exponential and quotient are off by about 2^-21 (|u| 2^-24 more for large |u|), far below the rounding to bf16 that follows;
 // expf and the IEEE division made the epilogue of a 256 x 256 tile longer than its products (8192 x 22016 x 4096, gated: 732 us).
 __device__ __forceinline__ float i8_gate(float x, float u) { return __fdividef(x, 1.f + __expf(-u)); }
+// v Phi(v).  Half of erfc(v / sqrt 2), v >= 0, as a polynomial in t = 1 / (1 + 0.245 v) times exp(-v^2 / 2): coefficients of the least greatest error in units of
+// (value + 0.001), found by reweighted least squares over 0 .. 14.  Off by 4e-9 (6e-6 of it up to v = 5), in fp32 by 2.2e-7.  With erff, whose two branches a warp walks
+// one after the other, the epilogue of 2820 x 11648 x 1088 took longer than its products.
+__device__ __forceinline__ float i8_gelu(float v) {
+  const float t = __fdividef(1.f, __fmaf_rn(0.245f, fabsf(v), 1.f));
+  float s = -0.109306395f;
+  s = __fmaf_rn(s, t, 0.447354406f);
+  s = __fmaf_rn(s, t, -0.449595600f);
+  s = __fmaf_rn(s, t, 0.443083793f);
+  s = __fmaf_rn(s, t, -0.0574047603f);
+  s = __fmaf_rn(s, t, 0.131341979f);
+  s = __fmaf_rn(s, t, 0.0945266038f);
+  const float q = s * t * __expf(-0.5f * v * v);
+  return v * (v < 0.f ? q : 1.f - q);
+}
 // act = 1 relu, 2 gelu, 3 gelu (tanh form: 0.5 x (1 + tanh(u)) = x sigmoid(2u)), 4 silu
 template <int N>
 __device__ __forceinline__ void i8_activate(float (&v)[N], int act) {
@@ -43,7 +58,7 @@ __device__ __forceinline__ void i8_activate(float (&v)[N], int act) {
       break;
     case 2:
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = 0.5f * v[j] * (1.f + erff(v[j] * 0.70710678118654752f));
+      for (int j = 0; j < N; ++j) v[j] = i8_gelu(v[j]);
       break;
     case 3:
 #pragma unroll
