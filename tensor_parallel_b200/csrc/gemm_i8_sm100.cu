@@ -366,6 +366,16 @@ static int ip_tile(int tokens, int features, int sms) {
   return bn;
 }
 
+// Results (or residuals) whose rows are not aligned leave a pair's tile 2 bytes at a time through shared memory, which costs about as much as 20 k-blocks: the shared
+// contraction's kernel stores as fast as ever, tiles of 128 x 128, but brings in more per product (looked at up to three rounds of tiles).  us, pairs / 128 x 128: 150 x 6370 x 512 9.5 / 6.2, x 2048
+// 11.2 / 8.7, x 6000 22.4 / 22.9; 600 x 6370 x 2048 (2 rounds of either) 22.9 / 17.8; 1000 x 3043 x 512 (1 / 2 rounds) 12.1 / 11.7, x 2048 14.9 / 17.0.
+static bool ip_yields(int tokens, int features, int k, int sms) {
+  const int bn = ip_tile(tokens, features, sms), k_blocks = (k + I8_BK - 1) / I8_BK;
+  const long long pairs = (long long)((tokens + IP_BM - 1) / IP_BM) * ((features + bn - 1) / bn), tiles = (long long)((tokens + 127) / 128) * ((features + 127) / 128);
+  const long long pair_rounds = (pairs + sms / 2 - 1) / (sms / 2), rounds = (tiles + sms - 1) / sms;
+  return k_blocks < 32 && rounds <= 3 && rounds <= (k_blocks <= 4 ? 2 : 1) * pair_rounds;
+}
+
 #define IP_FORMS(GO) GO(128) GO(160) GO(192) GO(224) GO(256)
 
 }  // namespace tpb
@@ -391,6 +401,9 @@ extern "C" int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, 
   int bn = 0, splits = 0;
   if (tpb::gemm_i8_split_pick(tokens, features, k, sms, &bn, &splits)) return tpb::gemm_i8_split_launch(g, bn, splits, s);
   if (tokens <= 64) return tpb::gemm_i8_stream_launch(g, sms, s);
+  auto aligned = [](const void* p, long long ld) { return !(reinterpret_cast<uintptr_t>(p) & 15) && ld % 8 == 0; };
+  if (!(aligned(out, ld_out) && (!residual || aligned(residual, ld_res))) && tpb::ip_yields(tokens, features, k, sms))
+    return tpb::gemm_i8_split_launch(g, 128, 1, s);
   bn = tpb::ip_tile(tokens, features, sms);
 #define GO(BN) if (bn == BN) return tpb::ip_launch<BN>(g, sms, s);
   IP_FORMS(GO)
@@ -398,12 +411,17 @@ extern "C" int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, 
   return TPB_ERR_ARG;
 }
 
-// The kernel that takes a product of these sizes, for tests: 0 streaming, 1 shared contraction (form: tokens of a tile, CTAs that share it), 2 CTA pairs (columns
+// The kernel that takes a product of these sizes (contiguous results, no activation that changes their number), for tests: 0 streaming, 1 shared contraction (form: tokens of a tile, CTAs that share it), 2 CTA pairs (columns
 // of a tile).
 extern "C" int tpb_gemm_int8_form(int tokens, int features, int k, int sms, int* form) {
   if (tokens <= 0 || features <= 0 || k <= 0 || k > tpb::I8_MAX_K || tokens > tpb::I8_MAX_ROWS || features > tpb::I8_MAX_ROWS || sms < 2 || !form) return -1;
   form[0] = form[1] = 0;
   if (tpb::gemm_i8_split_pick(tokens, features, k, sms, &form[0], &form[1])) return 1;
+  if (tokens > 64 && features % 8 && tpb::ip_yields(tokens, features, k, sms)) {
+    form[0] = 128;
+    form[1] = 1;
+    return 1;
+  }
   form[1] = 0;
   form[0] = tokens <= 64 ? 0 : tpb::ip_tile(tokens, features, sms);
   return tokens <= 64 ? 0 : 2;
