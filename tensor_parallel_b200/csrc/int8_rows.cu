@@ -727,7 +727,7 @@ static bool ri_ring_launch(const RiParams& p, int sms, cudaStream_t stream, cuda
   return true;
 }
 
-// Which rows go by the ring, and which by 32 columns a thread instead of 16 (aligned bf16 rows of at most 32768 columns: the fp32 ones do not fit the registers).
+// Which rows go by the ring, and which by 32 columns a thread instead of 16 (bf16 rows of at most 32768 columns: the fp32 ones do not fit the registers).
 // Fewer threads a row cost latency, which few rows do not hide, and save the row's own share of the instructions.  us, 16 columns / 32 columns / ring:
 //   rows       8192 x 5120 - / 22.1 / 24.9     1024 x 8192 - / 6.1 / 9.0      8192 x 11008 - / 56 / 46.8    2048 x 11008 - / 16.2 / 15.0   1024 x 11008 - / 9.3 / 10.5
 //              592 x 20000 - / 10.5 / 9.6      2048 x 20000 - / 31.0 / 23.2
@@ -742,6 +742,8 @@ static bool ri_ring_launch(const RiParams& p, int sms, cudaStream_t stream, cuda
 //   fewer rows 1200 x 2048 3.8 / 3.4 / -       1200 x 5120 7.4 / - / 5.5         600 x 11008 8.4 / - / 6.5
 //   + residual 600 x 2048 4.2 / 3.5, 1200 x 8192 14.1 / 13.0, 8192 x 4096 37.5 / 37.9, 8192 x 8192 72.6 / 77.5; LayerNorm 8192 x 1024 14.3 / 11.7, 8192 x 5120 55 / 49,
 //              16384 x 4096 76.7 / 80.1, 2400 x 16384 60 / 48
+// Rows of any alignment, bf16, 16 columns a thread / 32: rows 8192 x 5255 40.1 / 32.8, 300 x 5255 3.1 / 3.9, 2000 x 11007 29.9 / 19.9, 8 x 16610 5.2 / 2.5; RMSNorm 8192 x 4490
+// 41.1 / 46.2, 2000 x 11007 38.7 / 28.9, with a residual 59.2 / 55.2, 300 rows of it 12.6 / 14.0, 8192 x 16610 640 / 391; LayerNorm 8192 x 5255 92 / 70, 2000 x 16610 241 / 72.
 // Other rows (fp32, or of any alignment), 16 columns / ring: RMSNorm with a residual 4096 x 8192 42.7 / 45.2; 4096 x 11008 30.7 / 25.9, RMSNorm 58 / 35.
 template <typename T, int MODE, bool VEC>
 static bool ri_ring(const RiParams& p, int sms) {
@@ -751,7 +753,8 @@ static bool ri_ring(const RiParams& p, int sms) {
 }
 template <typename T, int MODE, bool VEC>
 static bool ri_four(const RiParams& p, int sms) {
-  if (!VEC || sizeof(T) != 2 || p.cols > 32768) return false;
+  if (sizeof(T) != 2 || p.cols > 32768) return false;
+  if (!VEC) return p.cols > 16384 || (p.cols > 6144 ? p.rows >= (p.residual ? 8 : 2) * sms : p.cols > 4096 && MODE != RI_RMS && p.rows >= 4 * sms);
   return p.cols > 16384 || (p.rows >= (p.cols > 6144 ? 2 : 4) * sms && p.cols > 4096);
 }
 
@@ -790,11 +793,11 @@ static cudaError_t ri_launch(const RiParams& p, int sms, cudaStream_t stream) {
   const int rows_per_block = threads >= 256 || v == 4 ? 1 : 256 / threads;
   const dim3 block(threads, rows_per_block), grid((unsigned(p.rows) + rows_per_block - 1) / rows_per_block);
   auto go = [&](auto kernel) { return launch_dependent(kernel, grid, block, 0, stream, true, p, 1.f); };
-  if constexpr (VEC && sizeof(T) == 2) {
+  if constexpr (sizeof(T) == 2) {
     if (v == 4)
-      return threads <= 256   ? go(rows_int8_kernel<T, MODE, 4, true, false, 256>)
-             : threads <= 512 ? go(rows_int8_kernel<T, MODE, 4, true, false, 512>)
-                              : go(rows_int8_kernel<T, MODE, 4, true, false, 1024>);
+      return threads <= 256   ? go(rows_int8_kernel<T, MODE, 4, VEC, false, 256>)
+             : threads <= 512 ? go(rows_int8_kernel<T, MODE, 4, VEC, false, 512>)
+                              : go(rows_int8_kernel<T, MODE, 4, VEC, false, 1024>);
   }
   if (wide) return go(rows_int8_kernel<T, MODE, 2, VEC, true, 1024>);
   if (v == 1) return go(rows_int8_kernel<T, MODE, 1, VEC, false, 256>);
@@ -829,6 +832,9 @@ static cudaError_t ri_preload() {
     LOAD(rows_int8_kernel<T, MODE, 4, true, false, 256>);
     LOAD(rows_int8_kernel<T, MODE, 4, true, false, 512>);
     LOAD(rows_int8_kernel<T, MODE, 4, true, false, 1024>);
+    LOAD(rows_int8_kernel<T, MODE, 4, false, false, 256>);
+    LOAD(rows_int8_kernel<T, MODE, 4, false, false, 512>);
+    LOAD(rows_int8_kernel<T, MODE, 4, false, false, 1024>);
     if constexpr (MODE != RI_ROWS) {
 #define LOAD_WALK(V, N) LOAD(rows_int8_walk_kernel<MODE, V, N, false>); LOAD(rows_int8_walk_kernel<MODE, V, N, true>)
       LOAD_WALK(4, 32);

@@ -629,3 +629,11 @@ def test_unaligned_results_of_short_contractions(tokens, features, k, act, resid
     if not residual:  # the same results in rows that are aligned: by another kernel, bit by bit
         room = torch.zeros(tokens, (features + 31) // 32 * 32, device="cuda", dtype=BF16)
         assert torch.equal(_native().gemm_int8(x, w, bias, act, out=room[:, :features]), out) and not room[:, features:].any()
+
+
+@pytest.mark.parametrize("cols,sms", [(4490, 5), (5255, 5), (8191, 3), (8191, 9), (11007, 3), (11007, 9), (16383, 9), (16610, 1), (32767, 1)])
+def test_many_rows_of_odd_widths(cols, sms):
+    test_many_wide_rows(cols, sms, BF16)
+    for with_residual in (False, True):
+        test_rms_norm_of_many_wide_rows(cols, sms, with_residual, BF16)
+        test_layer_norm_of_many_wide_rows(cols, sms, with_residual, BF16)
