@@ -11,6 +11,8 @@
 #include <torch/extension.h>
 
 #include <ATen/EmptyTensor.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -284,8 +286,16 @@ Tensor norm(const Tensor& x, const std::optional<Tensor>& weight, const std::opt
 }
 
 // ---- 8-bit serving ----
-// The ordinary calls: plain CUDA tensors that fit together and lie as the kernels read them, nothing that takes a gradient or has a tangent, no tracing.  Every other call
-// gets no value here and goes on in Python, which says what is wrong with it, or makes the copies that it needs.
+// The ordinary calls: plain CUDA tensors that fit together and lie as the kernels read them, nothing that takes a gradient or has a tangent, nothing around the call that
+// wants to see its steps.  Every other call gets no value here and goes on in Python, which says what is wrong with it, makes the copies that it needs, or takes the steps.
+
+// Whether something stands between a call and its kernels that they would drop out of: a dispatch mode (fake tensors, make_fx, which follows tensors without wrapping
+// them), its form ahead of dispatch, a functorch transform, functionalization, tracing.  The thread knows, not the tensors.
+bool interposed() {
+  constexpr c10::DispatchKeySet around({c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::Functionalize, c10::DispatchKey::PreDispatch});
+  return c10::impl::TorchDispatchModeTLS::any_modes_set() || (c10::impl::tls_local_dispatch_key_set().included_ & around).raw_repr() != 0 ||
+         torch::jit::tracer::isTracing();
+}
 
 bool plain(const Tensor& t, at::ScalarType dtype, const c10::Device& device) {
   return t.scalar_type() == dtype && t.device() == device && t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() &&
@@ -331,7 +341,7 @@ Int8Out int8_out(const Tensor& x, int64_t rows) {
 bool rows_int8(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, int64_t norm, const Tensor& residual, Int8Out* out, Tensor* sum) {
   const auto dtype = x.scalar_type();
   int64_t rows, pitch, residual_rows, residual_pitch = 0;
-  if (!lib.rows_int8 || !x.is_cuda() || (dtype != at::kBFloat16 && dtype != at::kFloat) || torch::jit::tracer::isTracing() || !plain(x, dtype, x.device()) ||
+  if (!lib.rows_int8 || !x.is_cuda() || (dtype != at::kBFloat16 && dtype != at::kFloat) || interposed() || !plain(x, dtype, x.device()) ||
       !rows_apart(x, &rows, &pitch))
     return false;
   const int64_t cols = x.size(-1);
@@ -355,7 +365,7 @@ bool rows_int8(const Tensor& x, const Tensor& weight, const Tensor& bias, double
 Tensor linear_int8(const Tensor& x, const Tensor& sx, const Tensor& w, const Tensor& sw, const Tensor& bias, int64_t act, const Tensor& residual) {
   int64_t tokens, ldx, features, ldw, residual_rows, ld_res = 0;
   const auto device = x.device();
-  if (!lib.gemm_int8 || !x.is_cuda() || torch::jit::tracer::isTracing() || !plain(x, at::kChar, device) || !plain(w, at::kChar, device) ||
+  if (!lib.gemm_int8 || !x.is_cuda() || interposed() || !plain(x, at::kChar, device) || !plain(w, at::kChar, device) ||
       !plain(sx, at::kFloat, device) || !plain(sw, at::kFloat, device) || x.dim() < 2 || w.dim() != 2 || !rows_apart(x, &tokens, &ldx) ||
       !rows_apart(w, &features, &ldw) || x.size(-1) != w.size(1) || !vector_of(sw, features) || sx.sizes() != x.sizes().slice(0, x.dim() - 1) ||
       !sx.is_contiguous())
@@ -447,7 +457,14 @@ PyObject* py_linear_int8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
+// () -> whether a call would go on in Python for what is around it
+PyObject* py_interposed(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  return PyBool_FromLong(interposed());
+  END_HANDLE_TH_ERRORS
+}
 PyMethodDef int8_calls[] = {
+    {"interposed", py_interposed, METH_NOARGS, nullptr},
     {"quantize_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_quantize_int8)), METH_FASTCALL, nullptr},
     {"norm_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_int8)), METH_FASTCALL, nullptr},
     {"linear_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_int8)), METH_FASTCALL, nullptr},

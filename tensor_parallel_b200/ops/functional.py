@@ -236,14 +236,17 @@ def _only_looks_rows_up(embedding: torch.nn.Module) -> bool:
             and embedding.max_norm is None and embedding.padding_idx is None and not embedding.sparse and not embedding.scale_grad_by_freq and not any(hooks))
 
 
+_AHEAD_OF_DISPATCH = torch._C.DispatchKey.PreDispatch
+
+
 def transformed(t: torch.Tensor) -> bool:
     """True where an autograd function over raw pointers would drop out of what is going on around it: a functorch transform (vmap,
-    grad, jvp), a batch of gradients (``is_grads_batched``), a forward-mode tangent, a dispatch mode (fake tensors, ``make_fx``), tracing
-    or compilation."""
+    grad, jvp), a batch of gradients (``is_grads_batched``), a forward-mode tangent, a dispatch mode (fake tensors, ``make_fx``, ahead of dispatch
+    too), tracing or compilation."""
     functorch = torch._C._functorch
     return (functorch.peek_interpreter_stack() is not None or functorch.is_functorch_wrapped_tensor(t) or functorch.is_legacy_batchedtensor(t)
-            or torch._C._len_torch_dispatch_stack() > 0 or torch.jit.is_tracing() or torch.compiler.is_compiling()
-            or torch.autograd.forward_ad.unpack_dual(t).tangent is not None)
+            or torch._C._len_torch_dispatch_stack() > 0 or torch._C._dispatch_tls_is_dispatch_key_included(_AHEAD_OF_DISPATCH)
+            or torch.jit.is_tracing() or torch.compiler.is_compiling() or torch.autograd.forward_ad.unpack_dual(t).tangent is not None)
 
 
 def relative_bias(embedding: torch.nn.Module, buckets, queries: int, keys: int):
