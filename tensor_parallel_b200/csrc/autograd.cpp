@@ -389,6 +389,17 @@ Tensor linear_int8(const Tensor& x, const Tensor& sx, const Tensor& w, const Ten
   return out;
 }
 
+// Whether operators are being captured or shapes followed (make_fx, fake tensors, capture ahead of dispatch): a kernel would leave nothing in the graph but the
+// allocation of its result.  Other dispatch modes (recomputation with a policy, counters) let kernels run.
+bool captured() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  if (c10::impl::tls_local_dispatch_key_set().included_.has(c10::DispatchKey::PreDispatch)) return true;
+  if (!Modes::any_modes_set()) return false;
+  for (const auto key : {c10::impl::TorchDispatchModeKey::PROXY, c10::impl::TorchDispatchModeKey::FAKE, c10::impl::TorchDispatchModeKey::FUNCTIONAL})
+    if (Modes::get_mode(key).has_value()) return true;
+  return false;
+}
+
 // The interpreter's side of these calls, without pybind11's conversions, which cost 0.6 us of a call's 4.5.
 PyObject* rows_type = nullptr;  // the named tuple (values, scales)
 PyObject* act_codes = nullptr;  // activation -> code
@@ -463,7 +474,14 @@ PyObject* py_interposed(PyObject*, PyObject*) {
   return PyBool_FromLong(interposed());
   END_HANDLE_TH_ERRORS
 }
-PyMethodDef int8_calls[] = {
+// () -> whether operators are being captured
+PyObject* py_captured(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  return PyBool_FromLong(captured());
+  END_HANDLE_TH_ERRORS
+}
+PyMethodDef plain_calls[] = {
+    {"captured", py_captured, METH_NOARGS, nullptr},
     {"interposed", py_interposed, METH_NOARGS, nullptr},
     {"quantize_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_quantize_int8)), METH_FASTCALL, nullptr},
     {"norm_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_int8)), METH_FASTCALL, nullptr},
@@ -518,5 +536,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linears", &linears, unlocked);
   m.def("norm", &norm, unlocked);
   m.def("bind_int8", &bind_int8);
-  if (PyModule_AddFunctions(m.ptr(), int8_calls) != 0) throw py::error_already_set();
+  if (PyModule_AddFunctions(m.ptr(), plain_calls) != 0) throw py::error_already_set();
 }

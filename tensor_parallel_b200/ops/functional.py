@@ -20,7 +20,8 @@ _native_module = None
 
 
 def _native(x: torch.Tensor):
-    """The native module if ``x`` should run on hand-written kernels, else ``None``."""
+    """The native module if ``x`` should run on hand-written kernels, else ``None``: on other devices, and where operators are being captured (``make_fx``,
+    fake tensors), since a kernel leaves nothing in the graph."""
     global _native_module
     if not x.is_cuda or _FORCE_TORCH:
         return None
@@ -28,7 +29,7 @@ def _native(x: torch.Tensor):
         from tensor_parallel_b200.ops import native  # raises if the library is missing on a GPU box
 
         _native_module = native
-    return _native_module
+    return _native_module if torch.compiler.is_dynamo_compiling() or not _native_module.captured() else None
 
 
 # -- reference definitions ---------------------------------------------------------------------
@@ -267,8 +268,8 @@ def relative_buckets(first: int, count: int, device, bidirectional: bool, bucket
     exact, device = buckets // (4 if bidirectional else 2), torch.device(device)
     if (device.type != "cuda" or _FORCE_TORCH or not 0 < count <= 2 ** 31 or type(buckets) is not int or type(max_distance) is not int
             or not 0 < exact < max_distance < 2 ** 31 or torch._C._functorch.peek_interpreter_stack() is not None
-            or torch._C._len_torch_dispatch_stack() > 0 or torch.jit.is_tracing() or torch.compiler.is_compiling()
-            or device.index not in (None, torch.cuda.current_device())):
+            or torch._C._len_torch_dispatch_stack() > 0 or torch._C._dispatch_tls_is_dispatch_key_included(_AHEAD_OF_DISPATCH)
+            or torch.jit.is_tracing() or torch.compiler.is_compiling() or device.index not in (None, torch.cuda.current_device())):
         return None
     from tensor_parallel_b200.ops import native
 

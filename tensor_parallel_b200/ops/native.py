@@ -59,6 +59,15 @@ AUTOGRAD = _load_autograd(LIB)  # autograd nodes of linear layers and norms in C
 _launches = 0
 
 
+def _captured() -> bool:
+    modes = torch._C._TorchDispatchModeKey
+    return torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch) or (
+        torch._C._len_torch_dispatch_stack() > 0 and any(torch._C._get_dispatch_mode(key) is not None for key in (modes.PROXY, modes.FAKE, modes.FUNCTIONAL)))
+
+
+captured = _captured if AUTOGRAD is None else AUTOGRAD.captured  # whether operators are being captured (make_fx, fake tensors)
+
+
 class _Module(types.ModuleType):
     @property
     def launch_count(self):

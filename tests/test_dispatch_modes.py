@@ -43,3 +43,52 @@ def test_the_native_calls_know_what_goes_on_around_them(around):
     SURROUNDINGS[around](f, torch.ones(2, 4))
     assert seen == [(True, True)]
     assert not native.AUTOGRAD.interposed() and not OF.transformed(plain)
+
+
+class _OnGpu:
+    is_cuda = True
+
+
+CAPTURES = {
+    "make_fx": lambda f, x: make_fx(f, tracing_mode="real")(x),
+    "make_fx, before dispatch": lambda f, x: make_fx(f, pre_dispatch=True)(x),
+    "fake tensors": lambda f, x: make_fx(f, tracing_mode="fake")(x),
+    "functionalized": lambda f, x: make_fx(torch.func.functionalize(f))(x),
+}
+
+
+@pytest.mark.skipif(not build.LIB_PATH.exists(), reason="native library not built")
+@pytest.mark.parametrize("asks", ["module", "python"])
+@pytest.mark.parametrize("around", list(CAPTURES))
+def test_no_kernel_is_taken_while_operators_are_captured(around, asks, monkeypatch):
+    from tensor_parallel_b200.ops import native
+
+    if asks == "python":  # (as without the C++ module)
+        monkeypatch.setattr(native, "captured", native._captured)
+    monkeypatch.setattr(OF, "_FORCE_TORCH", False)
+    seen = []
+
+    def f(x):
+        seen.append(OF._native(_OnGpu()))
+        return x + 1
+
+    CAPTURES[around](f, torch.ones(2, 4))
+    assert seen == [None]
+    with _Watch():  # (a mode that captures nothing)
+        assert OF._native(_OnGpu()) is native
+    assert OF._native(_OnGpu()) is native
+
+
+def test_no_kernel_is_taken_while_a_model_is_exported(monkeypatch):
+    if not build.LIB_PATH.exists():
+        pytest.skip("native library not built")
+    monkeypatch.setattr(OF, "_FORCE_TORCH", False)
+    seen = []
+
+    class Model(torch.nn.Module):
+        def forward(self, x):
+            seen.append(OF._native(_OnGpu()))
+            return x + 1
+
+    torch.export.export(Model(), (torch.ones(2, 4),), strict=False)
+    assert seen and set(seen) == {None}

@@ -68,3 +68,29 @@ def test_a_mode_sees_the_steps_of_the_8_bit_operators(name):
         got = call(*args)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert [n for n in watch.names if n in set(base.names)] == base.names
+
+
+OTHERS = {
+    "linear": lambda x, w, b, g: OF.linear(x, w, b),
+    "rms_norm": lambda x, w, b, g: OF.rms_norm(x, g, 1e-5),
+    "layer_norm": lambda x, w, b, g: OF.layer_norm(x, g, g, 1e-5),
+    "gelu": lambda x, w, b, g: OF.gelu(x),
+    "relu": lambda x, w, b, g: OF.relu(x),
+    "swiglu": lambda x, w, b, g: OF.swiglu(x, x * 2),
+    "geglu": lambda x, w, b, g: OF.geglu(x, x * 2),
+    "rope": lambda x, w, b, g: OF.apply_rope(x.view(1, -1, 1, 64), torch.arange(x.shape[0], device=x.device)[None]),
+    "attention": lambda x, w, b, g: OF.attention(*(x.view(1, -1, 1, 64) * s for s in (1, 2, 3)), True),
+}
+
+
+@pytest.mark.parametrize("capture", list(CAPTURES))
+@pytest.mark.parametrize("name", list(OTHERS))
+def test_a_captured_graph_holds_the_steps_of_the_other_operators(name, capture):
+    call = OTHERS[name]
+    graph = CAPTURES[capture](call, *_inputs(128, 10))
+    for seed in (11, 12):
+        args = _inputs(128, seed)
+        got, want = graph(*args).float(), call(*args).float()
+        # steps against the kernel: a rounding to bf16 on either side (2^-8 of a value each); terms of a sum and probabilities are rounded to bf16 in between, 2^-8 of
+        # values up to 16 each
+        torch.testing.assert_close(got, want, rtol=2.0 ** -7, atol=2.0 ** -4)
