@@ -447,8 +447,8 @@ attn_decode_fused_kernel(const bf16* q, const bf16* k, const bf16* v,
                          int splits, float scale_log2e, int rotary_dim, float log2_theta, int interleaved, long long q_ld,
                          long long k_ld, long long v_ld, const float2* __restrict__ rope_table, long long out_ld, int early) {
   constexpr int EPL = D / 8;
-  // early: the cache rows before `pos` and `pos` itself were written before the previous kernel of the stream began, so the
-  // first keys are on their way before that kernel (the q / k / v projection) has finished
+  // early: the cache rows before `pos` and `pos` itself were written before the previous kernel of the stream began (and that is no
+  // row kernel launched with `ahead`, see launch.cuh), so the first keys are on their way before that kernel (the q / k / v projection) has finished
   if (!early) pdl_wait();
   const int bh = blockIdx.x;
   const int b = bh / kv_heads, kvh = bh % kv_heads;
@@ -1407,7 +1407,7 @@ extern "C" int tpb_rope_table(void* table, int positions, int rotary_dim, float 
 // rope_table: optional output of tpb_rope_table covering every position < max_seq (null: angles are computed in place).
 // out: [batch][q_heads * head_dim] with a row pitch of out_ld elements (<= 0: dense).
 // early: launch as a programmatic dependent of the previous kernel of the stream and read pos_ptr and the cache rows before it
-// while that kernel still runs: it may produce q / k / v, but not those.
+// while that kernel still runs: it may produce q / k / v, but not those (row kernels launched with `ahead` in between: see `early` in tpb_gemm_opts_t).
 extern "C" int tpb_attn_decode_fused(const void* q, const void* k, const void* v, void* kcache, void* vcache, void* out,
                                      float* part_o, float* part_ml, void* counters, const int* pos_ptr, int batch, int q_heads,
                                      int kv_heads, int head_dim, int max_seq, int splits, float scale, int rotary_dim, float theta,

@@ -355,7 +355,7 @@ bool rows_int8(const Tensor& x, const Tensor& weight, const Tensor& bias, double
   if (residual.defined()) *sum = room_for(x.sizes(), dtype);
   check(lib.rows_int8(x.const_data_ptr(), data(residual), data(weight), data(bias), sum && sum->defined() ? sum->mutable_data_ptr() : nullptr,
                       static_cast<int8_t*>(out->values.mutable_data_ptr()), out->scales.mutable_data_ptr<float>(), int(rows), int(cols), pitch, residual_pitch, cols,
-                      (cols + 15) / 16 * 16, float(eps), int(norm) + 1, dtype == at::kFloat, context(x, 0)->status, stream_of(x)),
+                      (cols + 15) / 16 * 16, float(eps), int(norm) + 1, dtype == at::kFloat, 0, context(x, 0)->status, stream_of(x)),
         "tpb_rows_int8");
   launched.fetch_add(1, std::memory_order_relaxed);
   return true;

@@ -37,8 +37,18 @@ struct RiParams {
   long long ldx, ldr, lds, ldq;  // row pitches in elements
   int rows, cols;
   float eps;
+  int ahead;
   uint32_t* status;
 };
+
+// Waits for the kernel in front, and lets the one behind come in: as every kernel does (launch.cuh), or with `ahead` before the wait.  A product behind may then fetch
+// its weights while the kernel in front drains (decode step of four 7B layers, batch 8 x 2048, 484 -> 463 us, batch 8 x 64 291 -> 267); its CTAs leave no room for a third,
+// so no chain piles up.  What it reads early must then be older than the kernel in front of this one too, which only a caller that knows the chain can vouch for.
+__device__ __forceinline__ void ri_begin(int ahead) {
+  if (ahead) pdl_trigger();
+  pdl_wait();
+  pdl_trigger();
+}
 
 __device__ __forceinline__ float ri_float(bf16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float ri_float(float x) { return x; }
@@ -268,10 +278,7 @@ rows_int8_kernel(const RiParams p, float one) {
     }
   };
 
-  // (the other way round than in launch.cuh: a product behind this kernel may then come in while the one in front of it drains, and fetch its weights.  Its CTAs
-  // leave no room for a third, so no chain piles up; decode step of four 7B layers, batch 8 x 2048, 484 -> 463 us, batch 8 x 64 291 -> 267)
-  pdl_trigger();
-  pdl_wait();
+  ri_begin(p.ahead);
   float sum = 0.f, rstd = 1.f, mean = 0.f;
   for (int base = 0; base < end; base += chunk) {
     fetch(base, false);
@@ -364,8 +371,7 @@ rows_int8_walk_kernel(const RiParams p, float one) {
   __shared__ uint32_t maxima[2][32];
   const bf16* weight = static_cast<const bf16*>(p.weight);
   const bf16* bias = static_cast<const bf16*>(p.bias);
-  pdl_trigger();  // (see rows_int8_kernel)
-  pdl_wait();
+  ri_begin(p.ahead);
   Ri8<bf16> next[V], next2[TWO ? V : 1], w[V];
   const bf16* x = static_cast<const bf16*>(p.x) + blockIdx.x * p.ldx;  // (of the row on its way)
   const long long step_x = (long long)gridDim.x * p.ldx, step_q = (long long)gridDim.x * p.ldq;
@@ -541,8 +547,7 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
     if (group == 0) *abort_flag = 0;
     fence_mbar_init();
   }
-  pdl_trigger();  // (see rows_int8_kernel)
-  pdl_wait();
+  ri_begin(p.ahead);
   const long long step = (long long)gridDim.x * groups;
   auto load = [&](long long row, int s) {
     const uint32_t dst = smem_u32(ring + s * stage_bytes);
@@ -862,13 +867,13 @@ cudaError_t rows_int8_preload() {
 }  // namespace tpb
 
 extern "C" int tpb_rows_int8(const void* x, const void* residual, const void* weight, const void* bias, void* sum_out, int8_t* q, float* scales, int rows,
-                             int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, void* status, void* stream) {
+                             int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, int ahead, void* status, void* stream) {
   if (!x || !q || !scales || !status || rows <= 0 || cols <= 0 || mode < 0 || mode > 2 || dtype < 0 || dtype > 1) return TPB_ERR_ARG;
   if (cols > 1 << 30) return TPB_ERR_SIZE;
   if (mode == tpb::RI_ROWS && (residual || weight || bias || sum_out)) return TPB_ERR_ARG;
   if ((bias && mode != tpb::RI_LAYER) || (sum_out && !residual)) return TPB_ERR_ARG;
   if (ldx < cols || ldq < cols || (residual && ldr < cols) || (sum_out && lds < cols)) return TPB_ERR_ARG;
-  tpb::RiParams p = {x, residual, weight, bias, sum_out, q, scales, ldx, residual ? ldr : 0, sum_out ? lds : 0, ldq, rows, cols, eps, static_cast<uint32_t*>(status)};
+  tpb::RiParams p = {x, residual, weight, bias, sum_out, q, scales, ldx, residual ? ldr : 0, sum_out ? lds : 0, ldq, rows, cols, eps, ahead, static_cast<uint32_t*>(status)};
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return TPB_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

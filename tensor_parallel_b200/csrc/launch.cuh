@@ -9,8 +9,9 @@
 // allocation), then griddepcontrol.wait, and only THEN griddepcontrol.launch_dependents.  A successor is scheduled
 // once every CTA of this grid has passed that point, i.e. once the whole grid is resident and its predecessor has
 // completed: exactly one kernel is ever scheduled ahead, and its idle CTAs cannot take an SM from a CTA of the grid
-// they wait for.  (Triggering before the wait let a whole chain of future kernels pile up on the SMs and slowed the
-// Llama-7B decode step from 6.4 to 7.9 ms.)  The GEMM kernels trigger always, the decode attention when it is launched early itself: a
+// they wait for; what a kernel reads early only has to be older than the one kernel in front of it.  (Triggering before the wait let a whole chain of future kernels
+// pile up on the SMs and slowed the Llama-7B decode step from 6.4 to 7.9 ms.)  One exception, which a caller asks for: the 8-bit row kernels launched with `ahead`
+// trigger first (int8_rows.cu); early reads behind them have to be older than the kernel in front of all of them.  The GEMM kernels trigger always, the decode attention when it is launched early itself: a
 // GEMM that follows a GEMM gains about 1 us, whereas successors that only start ahead of time, scheduled into a running attention kernel
 // (many small CTAs, several per SM), end up unevenly spread over the SMs and cost more than the hidden launch latency (+1 to 2 us per
 // attention launch).

@@ -85,7 +85,8 @@ typedef struct {
   double wait_seconds;       // bound of the waits for peer GPUs; <= 0: the library default (tpb_set_wait_limit)
   size_t out_elems;          // extent of `out` in elements, for the index checks of a -DTPB_BOUNDS build; 0: derived from the shape
   int early;                 // launch as a programmatic dependent of the previous kernel of the stream and read w before that
-                             // kernel has finished (few-token streaming kernel only): w must not be an output of that kernel
+                             // kernel has finished (few-token streaming kernel only): w must not be an output of that kernel, nor, where it
+                             // is a tpb_rows_int8 with `ahead`, of the kernel in front of it, and so on through such calls
 } tpb_gemm_opts_t;
 
 // 1 if this library was built with -DTPB_BOUNDS (kernels check their store indices and report STATUS_BAD_ARG = 3 in the
@@ -135,19 +136,22 @@ int tpb_col_sum(const void* g, void* out, float* partials, int rows, int cols, i
 // (RMSNorm, whose 1 / rms is in the scale alone) or the normalised row.  A row with a value that is not finite: integers 0, scale NaN.  Modes 1 and 2: weight, bias
 // (LayerNorm) and residual may be null; with residual, x + residual rounded to the type of x is normalised and stored to sum_out (may be null, or x).
 // Launched, like the product below, as a programmatic dependent of the previous kernel of the stream, and touches no memory before that kernel has finished.
+// ahead: the next kernel of the stream may start before that; what it reads early (see `early`) must not be an output of that kernel either.
 int tpb_rows_int8(const void* x, const void* residual, const void* weight, const void* bias, void* sum_out, int8_t* q, float* scales, int rows,
-                  int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, void* status, void* stream);
+                  int cols, long long ldx, long long ldr, long long lds, long long ldq, float eps, int mode, int dtype, int ahead, void* status,
+                  void* stream);
 
 // out[t, f] = act(sx[t] sw[f] sum_k x[t, k] w[f, k] + bias[f]) + residual[t, f]: x [tokens, k] and w [features, k] 8-bit integers (16-byte aligned, row pitches
 // multiples of 16; what lies between k and the pitch is not read), sums in 32 bits, bf16 bias, residual (may be out) and out.  act as in tpb_gemm_bf16; 5
 // (rows of w: 16 gate, 16 up in turn; out has features / 2 columns) takes no residual.  k <= 131071.  early: read w before the
-// previous kernel of the stream has finished, which must not write it.
+// previous kernel of the stream has finished, which must not write it (as in tpb_gemm_opts_t).
 int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, const float* sw, void* out, const void* bias, const void* residual, int tokens,
                   int features, int k, long long ldx, long long ldw, long long ld_out, long long ld_res, int act, int early, void* status, void* stream);
 
-// Sizes of the structures above as this library was built, one byte-count per 16 bits (plan, reduction context, options), for callers that
-// are built apart from it.
-#define TPB_API_LAYOUT ((unsigned long long)sizeof(tpb_gemm_plan_t) | (unsigned long long)sizeof(tpb_reduce_ctx_t) << 16 | (unsigned long long)sizeof(tpb_gemm_opts_t) << 32)
+// Sizes of the structures above as this library was built, one byte-count per 16 bits (plan, reduction context, options), and the version of the
+// signatures that are called from elsewhere (1: tpb_rows_int8 takes `ahead`), for callers that are built apart from it.
+#define TPB_API_LAYOUT \
+  ((unsigned long long)sizeof(tpb_gemm_plan_t) | (unsigned long long)sizeof(tpb_reduce_ctx_t) << 16 | (unsigned long long)sizeof(tpb_gemm_opts_t) << 32 | 1ull << 48)
 unsigned long long tpb_api_layout(void);
 
 // Measurement aids.  tpb_gemm_debug caps the smem ring depth (0 restores the default).  Skipping the MMAs and the

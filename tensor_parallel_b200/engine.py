@@ -379,7 +379,7 @@ class DecoderEngine:
     def _int8_norm(self, x, norm):
         """8-bit rows of the norm of the residual stream ``x``, which is brought up to date first: what the ranks' last sum left is added."""
         summed, self._summed = self._summed, None
-        return native.rows_int8(x, norm[0], norm[1], self.eps, self.mode - 1, residual=summed, sum_out=None if summed is None else x)
+        return native.rows_int8(x, norm[0], norm[1], self.eps, self.mode - 1, residual=summed, sum_out=None if summed is None else x, ahead=self.world == 1)
 
     def _int8_row_parallel(self, parts, x, early):
         """``x += all-reduce(sum of the projections) + biases`` for ``parts`` of (rows, weight, bias; the shard's copy, bias / world).  With several ranks the
@@ -404,19 +404,20 @@ class DecoderEngine:
     def _int8_layer(self, i, x, qkv, q_rot, cat, act_buf, batch, seq, decode: bool):
         L = self.layers[i]
         early = decode and self.world == 1  # (see _layer)
+        # (the kernels behind the rows are products, which read early only weights: `ahead` on one rank, where nothing waits for a peer)
         rows = self._int8_norm(x, L["ln1"])
         mlp_rows = None
         if self.parallel:  # the MLP reads the block input as well
             mlp_rows = rows if L["ln2"] is None else self._int8_norm(x, L["ln2"])
         native.gemm_int8(rows, L["wqkv"], L["bqkv"], out=qkv, early=early)
         attn = self._attend(i, qkv, q_rot, cat, batch, seq, decode, early)
-        attn_rows = native.rows_int8(attn)
+        attn_rows = native.rows_int8(attn, ahead=self.world == 1)
         if not self.parallel:
             self._int8_row_parallel([(attn_rows, L["wo"], L["bo"])], x, early)
             mlp_rows = self._int8_norm(x, L["ln2"])
         hidden = cat[:, self.nq * self.head_dim :] if self.parallel else act_buf
         native.gemm_int8(mlp_rows, L["w1"], L["b1"], act=self.act, out=hidden, early=early)
-        down = (native.rows_int8(hidden), L["wd"], L["bd"])
+        down = (native.rows_int8(hidden, ahead=self.world == 1), L["wd"], L["bd"])
         self._int8_row_parallel([(attn_rows, L["wo"], L["bo"]), down] if self.parallel else [down], x, early)
 
     def _attend(self, i, qkv, q_rot, cat, batch, seq, decode: bool, early: bool):

@@ -292,8 +292,8 @@ def gemm_nt(x2d: torch.Tensor, w: torch.Tensor, bias=None, residual=None, act=No
     ``[tokens, n]`` are the rows the statistics are taken over when ``x2d`` is only a column slice of them.
     ``out_elems`` (a library built with ``-DTPB_BOUNDS`` only): extent of ``out`` that the kernel checks its store
     indices against; 0 derives it from the shape.  ``early``: the kernel may start, and read ``w``, while the previous kernel
-    of the stream is still running (that kernel must not write ``w``); everything else is read after it.  It has no effect on a
-    ``w`` that TMA cannot read in place."""
+    of the stream is still running (that kernel must not write ``w``, nor, where it is a :func:`rows_int8` with ``ahead``, the one in front of it, and so on);
+    everything else is read after it.  It has no effect on a ``w`` that TMA cannot read in place."""
     global _launches
     if x_t:
         k, tokens = x2d.shape
@@ -835,7 +835,8 @@ def attn_decode_fused(q, k, v, kcache, vcache, pos_ptr, rotary_dim, theta, inter
     projection output), append k, v to the cache at ``pos_ptr[0]``, attend over ``[0, pos]`` and merge the key splits.
     ``workspace = (part_o, part_ml, counters)`` with ``counters`` an int32 tensor of at least ``batch * kv_heads`` elements
     zeroed once (``batch * q_heads``: all query-head groups of a KV head share one launch).  ``early``: the kernel may start while
-    the previous kernel of the stream is still running and read ``pos_ptr`` and the cached rows, which that kernel must not write."""
+    the previous kernel of the stream is still running and read ``pos_ptr`` and the cached rows, which that kernel must not write (see
+    :func:`gemm_nt`)."""
     global _launches
     d = kcache.shape[3]
     b, hq, hkv, smax = q.shape[0], q.shape[1] // d, kcache.shape[1], kcache.shape[2]
@@ -974,7 +975,7 @@ def adamw_step(param, grad, exp_avg, exp_avg_sq, step, lr, beta1, beta2, eps, we
 # 8-bit integers: rows with a scale each, and their matrix product (serving)
 # ------------------------------------------------------------------------------------------------
 
-LIB.tpb_rows_int8.argtypes = [c_void_p] * 7 + [c_int] * 2 + [c_ll] * 4 + [c_float] + [c_int] * 2 + [c_void_p] * 2
+LIB.tpb_rows_int8.argtypes = [c_void_p] * 7 + [c_int] * 2 + [c_ll] * 4 + [c_float] + [c_int] * 3 + [c_void_p] * 2
 LIB.tpb_gemm_int8.argtypes = [c_void_p] * 7 + [c_int] * 3 + [c_ll] * 4 + [c_int] * 2 + [c_void_p] * 2
 
 
@@ -991,9 +992,11 @@ def int8_rows_empty(rows: int, cols: int, device) -> OF.Int8Rows:
     return OF.Int8Rows(values if pitch == cols else values[:, :cols], torch.empty(rows, dtype=torch.float32, device=device))
 
 
-def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, sum_out=None, out=None) -> OF.Int8Rows:
+def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, sum_out=None, out=None, ahead=False) -> OF.Int8Rows:
     """8-bit rows of ``x2d`` (rows of any pitch with unit inner stride) as they are, or (``norm`` 0 / 1) of the RMSNorm / LayerNorm of ``x2d + residual``, which is
-    also stored to ``sum_out`` (may be ``x2d``).  ``weight`` and ``bias`` have the type of ``x2d``.  ``out``: rows to write (:func:`int8_rows_empty`)."""
+    also stored to ``sum_out`` (may be ``x2d``).  ``weight`` and ``bias`` have the type of ``x2d``.  ``out``: rows to write (:func:`int8_rows_empty`).
+    ``ahead``: the kernel behind may start while the one in front of this is still running: what it reads early (see :func:`gemm_nt`) must not be written by
+    that one either."""
     global _launches
     rows, cols = _int32("rows_int8", *x2d.shape)
     out = int8_rows_empty(rows, cols, x2d.device) if out is None else out
@@ -1001,7 +1004,7 @@ def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, su
         return out
     check(LIB.tpb_rows_int8(_ptr(x2d), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(sum_out), _ptr(out[0]), _ptr(out[1]), rows, cols, _pitch(x2d),
                             _pitch(residual), _pitch(sum_out), _pitch(out[0]), eps,
-                            0 if norm is None else norm + 1, _dtype_code(x2d), _ptr(device_state(x2d.device).status), _stream()), "tpb_rows_int8")
+                            0 if norm is None else norm + 1, _dtype_code(x2d), int(ahead), _ptr(device_state(x2d.device).status), _stream()), "tpb_rows_int8")
     _launches += 1
     return out
 

@@ -1,0 +1,86 @@
+"""Order of programmatic launches, checked on the CPU: when a kernel lets the next one in, and who asks for the exception."""
+import re
+import types
+
+import pytest
+import torch
+
+from tensor_parallel_b200 import build
+from tensor_parallel_b200.engine import DecoderEngine
+
+needs_library = pytest.mark.skipif(not build.LIB_PATH.exists(), reason="native library not built")
+
+
+def _code(path):
+    return [line for line in (re.sub(r"//.*", "", raw).strip() for raw in path.read_text().splitlines()) if line]
+
+
+def test_kernels_let_the_next_one_in_behind_their_own_wait():
+    """A kernel that reads early promises that it reads nothing the one kernel in front of it writes: that is enough as long as no kernel lets its successor in
+    before its own wait, unless it was asked to."""
+    found = 0
+    for path in sorted(build.CSRC.glob("*.cu")):
+        lines = _code(path)
+        for before, line in zip(lines, lines[1:]):
+            if "pdl_trigger()" not in line:
+                continue
+            found += 1
+            assert before == "pdl_wait();" or line == "if (ahead) pdl_trigger();", f"{path.name}: {before} / {line}"
+    assert found >= 8
+
+
+@needs_library
+def test_rows_let_the_next_kernel_in_ahead_only_where_they_are_asked(monkeypatch):
+    from tensor_parallel_b200.ops import native
+
+    calls = []
+    argtypes = native.LIB.tpb_rows_int8.argtypes
+    monkeypatch.setattr(native, "LIB", types.SimpleNamespace(tpb_rows_int8=lambda *args: calls.append(args) or 0))
+    monkeypatch.setattr(native, "_stream", lambda: None)
+    monkeypatch.setattr(native, "device_state", lambda device: types.SimpleNamespace(status=torch.zeros(4, dtype=torch.int32)))
+    x = torch.ones(3, 32, dtype=torch.bfloat16)
+    native.rows_int8(x)
+    native.rows_int8(x, x[0], None, 1e-5, 0)
+    native.rows_int8(x, ahead=True)
+    assert all(len(args) == len(argtypes) for args in calls) and [args[-3] for args in calls] == [0, 0, 1]
+
+
+class _Chain:
+    """Stands in for the native module: writes down what an engine's layer asks for."""
+
+    def __init__(self):
+        self.rows, self.products = [], []
+
+    def rows_int8(self, x, *args, ahead=False, **kwargs):
+        self.rows.append(ahead)
+        return x, x
+
+    def gemm_int8(self, x, weight, bias=None, act=None, residual=None, out=None, early=False):
+        self.products.append(early)
+        return out
+
+
+def _layer_engine(world, parallel=False):
+    engine = DecoderEngine.__new__(DecoderEngine)
+    engine.world, engine.parallel, engine.nq, engine.head_dim, engine.mode, engine.eps, engine.act = world, parallel, 1, 8, 1, 1e-5, None
+    engine._summed = None
+    engine.layers = [dict(wqkv=None, bqkv=None, ln1=(None, None), ln2=(None, None), w1=None, b1=None, wo=None, bo=None, wd=None, bd=None)]
+    engine._attend = lambda i, qkv, q_rot, cat, *rest: cat[:, :8]
+    engine.comm = types.SimpleNamespace(staging_view=lambda which, shape, dtype: torch.zeros(shape, dtype=dtype), all_reduce=lambda t: t * world)
+    return engine
+
+
+@needs_library
+@pytest.mark.parametrize("parallel", [False, True])
+@pytest.mark.parametrize("decode", [False, True])
+@pytest.mark.parametrize("world", [1, 2])
+def test_the_engine_asks_for_it_on_one_rank_only(world, decode, parallel, monkeypatch):
+    from tensor_parallel_b200 import engine as module
+
+    chain = _Chain()
+    monkeypatch.setattr(module, "native", chain)
+    engine = _layer_engine(world, parallel)
+    x = torch.zeros(2, 8, dtype=torch.bfloat16)
+    engine._int8_layer(0, x, torch.zeros(2, 24), None, torch.zeros(2, 16), torch.zeros(2, 8), 2, 1, decode)
+    assert len(chain.rows) == 4 and set(chain.rows) == {world == 1}
+    assert set(chain.products) <= {decode and world == 1, False} and (not decode or world > 1 or all(chain.products))
