@@ -4,7 +4,9 @@
 //   v = (h - mean) rstd w + b         scale = amax / 127
 // with amax = max(max |v|, 1e-30) over the row and q = rint(v (127 / amax)).  An RMSNorm's rstd is common to the row, so it only enters
 // the scale: the integers depend on no order of summation, and a row needs one exchange (sum of squares and maximum together) instead of two.
-// A row with a value that is not finite gets integers 0 and the scale NaN, so that everything computed from it is NaN.
+// A row with a value that is not finite gets integers 0 and the scale NaN, so that everything computed from it is NaN.  So does the scale of a finite row whose sum of
+// squares passes the range of fp32 (a value above 2^64 is enough), instead of the zero that 1 / rms would be.  (Done again with a scaled sum, in the same kernel, such a
+// row cost the ordinary ones 2 to 27 % of their time: registers, or a branch per warp.)
 //
 // Memory-bound: x and the residual are read once, h and the integers written once.  A row waits for its statistics in registers as fp32: in a block of its own, in
 // a persistent block that has the next row on its way (norms of many rows), or, where many wide rows need more of them in flight than registers hold, in shared
@@ -185,6 +187,14 @@ __device__ __forceinline__ uint32_t ri_integers(float2 v0, float2 v1, float inv,
   return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
 }
 
+// The scale of a row, by its first thread: of an RMSNorm from the sum of squares, of a LayerNorm with 1 / deviation as it was used.
+template <int MODE>
+__device__ __forceinline__ float ri_scale(float amax, bool finite, float squares, float rstd, const RiParams& p) {
+  const bool in_range = MODE == RI_RMS ? squares <= 3.402823466e38f : MODE == RI_LAYER ? rstd > 0.f : true;
+  const float scale = amax / 127.f * (MODE == RI_RMS ? rsqrtf(squares / float(p.cols) + p.eps) : 1.f);
+  return finite && in_range ? scale : __int_as_float(0x7FC00000);
+}
+
 // Blocks that an SM is to hold: as many registers as the row and its raw words take, without spills to speak of (8192 x 4096, RMSNorm with 8 blocks 28.6 us
 // instead of 24.8; with 32 columns a thread, 11008 wide, two blocks of 512 instead of one 76 us instead of 116).
 template <typename T, int MODE, int V, bool VEC>
@@ -333,8 +343,7 @@ rows_int8_kernel(const RiParams p, float one) {
   const float amax = fmaxf(__uint_as_float(most), RI_LEAST);
   const float inv = __fdiv_rn(127.f, amax);
   if (threadIdx.x == 0 && row < p.rows) {
-    const float scale = amax / 127.f * (MODE == RI_RMS ? rsqrtf(sum / float(p.cols) + p.eps) : 1.f);
-    p.scales[row] = finite ? scale : __int_as_float(0x7FC00000);
+    p.scales[row] = ri_scale<MODE>(amax, finite, sum, rstd, p);
   }
   int8_t* q = p.q + row * p.ldq;
   const bool whole = VEC || !((reinterpret_cast<uintptr_t>(p.q) | uintptr_t(p.ldq)) & 7);  // 8 integers may be stored at once
@@ -475,8 +484,7 @@ rows_int8_walk_kernel(const RiParams p, float one) {
     const float amax = fmaxf(__uint_as_float(most), RI_LEAST);
     const float inv = __fdiv_rn(127.f, amax);
     if (threadIdx.x == 0) {
-      const float scale = amax / 127.f * (MODE == RI_RMS ? rsqrtf(sum / float(p.cols) + p.eps) : 1.f);
-      p.scales[row] = finite ? scale : __int_as_float(0x7FC00000);
+      p.scales[row] = ri_scale<MODE>(amax, finite, sum, rstd, p);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -679,8 +687,7 @@ rows_int8_ring_kernel(const RiParams p, int stages, int slot_bytes, float one) {
     const float amax = fmaxf(__uint_as_float(most), RI_LEAST);
     const float inv = __fdiv_rn(127.f, amax);
     if (tid == 0) {
-      const float scale = amax / 127.f * (MODE == RI_RMS ? rsqrtf(sum / float(p.cols) + p.eps) : 1.f);
-      p.scales[row] = finite ? scale : __int_as_float(0x7FC00000);
+      p.scales[row] = ri_scale<MODE>(amax, finite, sum, rstd, p);
     }
     int8_t* out = p.q + row * p.ldq;
     each([&](int q) {

@@ -133,7 +133,8 @@ int tpb_col_sum(const void* g, void* out, float* partials, int rows, int cols, i
 
 // Rows of x [rows, cols] (bf16: dtype 0, fp32: 1; row pitches ld* in elements) in 8-bit integers: q [rows, cols] (pitch ldq) and one fp32 scale per
 // row, q * scale being x (mode 0), or the RMSNorm (1) or LayerNorm (2) of x.  q = rint(v * (127 / amax)), amax = max(max |v|, 1e-30), where v is x, x * weight
-// (RMSNorm, whose 1 / rms is in the scale alone) or the normalised row.  A row with a value that is not finite: integers 0, scale NaN.  Modes 1 and 2: weight, bias
+// (RMSNorm, whose 1 / rms is in the scale alone) or the normalised row.  A row with a value that is not finite: integers 0, scale NaN; a finite one whose
+// sum of squares (of deviations) passes fp32, in modes 1 and 2: scale NaN.  Modes 1 and 2: weight, bias
 // (LayerNorm) and residual may be null; with residual, x + residual rounded to the type of x is normalised and stored to sum_out (may be null, or x).
 // Launched, like the product below, as a programmatic dependent of the previous kernel of the stream, and touches no memory before that kernel has finished.
 // ahead: the next kernel of the stream may start before that; what it reads early (see `early`) must not be an output of that kernel either.

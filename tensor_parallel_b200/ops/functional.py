@@ -154,17 +154,25 @@ def _add_ref(x, residual):
     return x if residual is None else (x.float() + residual.float()).to(x.dtype)
 
 
+def _in_range(rstd):
+    """NaN for the 1 / deviation of a row whose sum of squares passes the range of fp32 (a value above 2^64 is enough), which would come out as zero."""
+    return torch.where(rstd > 0, rstd, torch.full_like(rstd, float("nan")))
+
+
 def rms_norm_int8_ref(x, weight, eps: float, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
     h = _add_ref(x, residual)
     hf = h.float()
-    rstd = torch.rsqrt(hf.pow(2).mean(-1) + eps)
+    rstd = _in_range(torch.rsqrt(hf.pow(2).mean(-1) + eps))
     return _int8_rows_ref(hf if weight is None else hf * weight.to(x.dtype).float(), rstd), h
 
 
 def layer_norm_int8_ref(x, weight, bias, eps: float, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
     h = _add_ref(x, residual)
+    hf = h.float()
     w, b = (None if t is None else t.to(x.dtype).float() for t in (weight, bias))
-    return _int8_rows_ref(F.layer_norm(h.float(), h.shape[-1:], w, b, eps)), h
+    values, scales = _int8_rows_ref(F.layer_norm(hf, h.shape[-1:], w, b, eps))
+    rstd = torch.rsqrt((hf - hf.mean(-1, keepdim=True)).pow(2).mean(-1) + eps)
+    return Int8Rows(values, torch.where(_in_range(rstd).isnan(), rstd.new_full((), float("nan")), scales)), h
 
 
 def linear_int8_ref(x: Int8Rows, weight: Int8Rows, bias=None, act: Optional[str] = None, residual=None):
@@ -349,7 +357,8 @@ def quantize_int8(x) -> Int8Rows:
 
 def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
     """``(rows, h)``: ``h = x + residual``, rounded to the type of ``x`` (``x`` itself without a residual), and its RMSNorm in 8 bits, as
-    :func:`quantize_int8` gives them.  ``weight`` may be None."""
+    :func:`quantize_int8` gives them.  ``weight`` may be None.  A row whose sum of squares passes the range of fp32 (a value above 2^64 is enough) gets
+    the scale NaN."""
     out = norm_int8_directly(x, weight, None, eps, 0, residual)
     if out is not None:
         return out
@@ -359,7 +368,8 @@ def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows
 
 
 def layer_norm_int8(x, weight, bias, eps: float = 1e-5, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
-    """Like :func:`rms_norm_int8`, with a LayerNorm; ``weight`` and ``bias`` may be None."""
+    """Like :func:`rms_norm_int8`, with a LayerNorm (whose squares are those of the deviations, and whose sum of values has a part in it); ``weight`` and
+    ``bias`` may be None."""
     out = norm_int8_directly(x, weight, bias, eps, 1, residual)
     if out is not None:
         return out
