@@ -29,7 +29,7 @@ def _native(x: torch.Tensor):
         from tensor_parallel_b200.ops import native  # raises if the library is missing on a GPU box
 
         _native_module = native
-    return _native_module if torch.compiler.is_dynamo_compiling() or not _native_module.captured() else None
+    return _native_module if _compiling() or not _native_module.captured() else None
 
 
 # -- reference definitions ---------------------------------------------------------------------
@@ -245,6 +245,7 @@ def _only_looks_rows_up(embedding: torch.nn.Module) -> bool:
             and embedding.max_norm is None and embedding.padding_idx is None and not embedding.sparse and not embedding.scale_grad_by_freq and not any(hooks))
 
 
+_compiling = torch.compiler.is_dynamo_compiling
 _AHEAD_OF_DISPATCH = torch._C.DispatchKey.PreDispatch
 
 
@@ -319,7 +320,8 @@ def _not_taken(*args):
     return None
 
 
-# The ordinary calls, as the native module takes them once it is loaded: its results, or None for a call that needs a check's words or a copy.
+# The ordinary calls, as the native module takes them once it is loaded: its results, or None for a call that needs a check's words or a copy.  Not while a compiler
+# traces the front end, which would stop there: it gets the steps.
 quantize_int8_directly = norm_int8_directly = linear_int8_directly = _not_taken
 
 
@@ -347,10 +349,11 @@ def quantize_int8(x) -> Int8Rows:
     """The rows of ``x`` (bf16 or fp32, ``[..., cols]``) in 8 bits: ``rint(x * (127 / max |x|))`` and ``max |x| / 127``, ties to even.  For an activation
     in front of :func:`linear_int8`, and for its weight (a row per output channel).  A row with a value that is not finite gets the scale NaN.
     Serving only: there is no gradient."""
-    out = quantize_int8_directly(x)
-    if out is not None:
-        return out
-    nat = _native(x)
+    if not _compiling():
+        out = quantize_int8_directly(x)
+        if out is not None:
+            return out
+    nat = None if _compiling() else _native(x)
     _check_rows("quantize_int8", x)
     return quantize_int8_ref(x) if nat is None or transformed(x) else nat.quantize_int8(x)
 
@@ -359,10 +362,11 @@ def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows
     """``(rows, h)``: ``h = x + residual``, rounded to the type of ``x`` (``x`` itself without a residual), and its RMSNorm in 8 bits, as
     :func:`quantize_int8` gives them.  ``weight`` may be None.  A row whose sum of squares passes the range of fp32 (a value above 2^64 is enough) gets
     the scale NaN."""
-    out = norm_int8_directly(x, weight, None, eps, 0, residual)
-    if out is not None:
-        return out
-    nat = _native(x)
+    if not _compiling():
+        out = norm_int8_directly(x, weight, None, eps, 0, residual)
+        if out is not None:
+            return out
+    nat = None if _compiling() else _native(x)
     _check_rows("rms_norm_int8", x, weight, residual=residual)
     return rms_norm_int8_ref(x, weight, eps, residual) if nat is None or transformed(x) else nat.norm_int8(x, weight, None, eps, 0, residual)
 
@@ -370,10 +374,11 @@ def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows
 def layer_norm_int8(x, weight, bias, eps: float = 1e-5, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
     """Like :func:`rms_norm_int8`, with a LayerNorm (whose squares are those of the deviations, and whose sum of values has a part in it); ``weight`` and
     ``bias`` may be None."""
-    out = norm_int8_directly(x, weight, bias, eps, 1, residual)
-    if out is not None:
-        return out
-    nat = _native(x)
+    if not _compiling():
+        out = norm_int8_directly(x, weight, bias, eps, 1, residual)
+        if out is not None:
+            return out
+    nat = None if _compiling() else _native(x)
     _check_rows("layer_norm_int8", x, weight, bias, residual)
     return layer_norm_int8_ref(x, weight, bias, eps, residual) if nat is None or transformed(x) else nat.norm_int8(x, weight, bias, eps, 1, residual)
 
@@ -408,10 +413,11 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias=None, act: Optional[str] = N
     products are exact integers, scales, bias, activation and residual are fp32.  ``act``: None, ``"relu"``, ``"gelu"``, ``"gelu_tanh"``, ``"silu"``, or
     ``"swiglu16"`` for a weight whose rows alternate in groups of 16 gate and 16 up rows (``silu(gate) * up``, half as many columns).  Serving only:
     there is no gradient."""
-    out = linear_int8_directly(x, weight, bias, act, residual)
-    if out is not None:
-        return out
-    nat = _native(x[0])
+    if not _compiling():
+        out = linear_int8_directly(x, weight, bias, act, residual)
+        if out is not None:
+            return out
+    nat = None if _compiling() else _native(x[0])
     _check_linear_int8(x, weight, bias, act, residual)
     if nat is None or transformed(x[0]) or transformed(x[1]):
         return linear_int8_ref(Int8Rows(*x), Int8Rows(*weight), bias, act, residual)

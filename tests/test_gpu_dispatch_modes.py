@@ -94,3 +94,15 @@ def test_a_captured_graph_holds_the_steps_of_the_other_operators(name, capture):
         # steps against the kernel: a rounding to bf16 on either side (2^-8 of a value each); terms of a sum and probabilities are rounded to bf16 in between, 2^-8 of
         # values up to 16 each
         torch.testing.assert_close(got, want, rtol=2.0 ** -7, atol=2.0 ** -4)
+
+
+@pytest.mark.parametrize("name", list(INT8))
+def test_one_compiled_graph_of_the_8_bit_operators(name):
+    call, steps = INT8[name]
+    call(*_inputs(6, 14))  # (the native module is loaded)
+    torch._dynamo.reset()
+    compiled = torch.compile(call, fullgraph=True, backend="eager")
+    with torch.no_grad():
+        for seed in (15, 16):
+            args = _inputs(6, seed)
+            assert all(torch.equal(a, b) for a, b in zip(compiled(*args), steps(*args)))
