@@ -179,7 +179,6 @@ class DecoderEngine:
                 entry["wo"], entry["bo"] = L.wo, L.bo
                 entry["wd"], entry["bd"] = (w_down if w_down is L.w_down else w_down.contiguous()), L.b_down
             self.layers.append(entry)
-        self._summed: Optional[torch.Tensor] = None  # 8-bit layers of several ranks: what the next norm adds to the residual stream
         self.nq, self.nkv, self.ff = self.layers[0]["nq"], self.layers[0]["nkv"], self.layers[0]["ff"]
 
         # -- head -----------------------------------------------------------------------------------
@@ -376,36 +375,30 @@ class DecoderEngine:
             return native.gemm_nt(x, weight, bias=bias, act=act, out=out, norm=(self.mode, self.eps, rowsum), early=early)
         return native.gemm_nt(n, weight, bias=bias, act=act, out=out)
 
-    def _int8_norm(self, x, norm):
+    def _int8_norm(self, x, norm, summed=None):
         """8-bit rows of the norm of the residual stream ``x``, which is brought up to date first: what the ranks' last sum left is added."""
-        summed, self._summed = self._summed, None
         return native.rows_int8(x, norm[0], norm[1], self.eps, self.mode - 1, residual=summed, sum_out=None if summed is None else x, ahead=self.world == 1)
 
     def _int8_row_parallel(self, parts, x, early):
         """``x += all-reduce(sum of the projections) + biases`` for ``parts`` of (rows, weight, bias; the shard's copy, bias / world).  With several ranks the
-        sum is left for the next norm to add."""
+        sum is returned, for the next norm to add."""
         if self.world == 1:
             for rows, weight, bias in parts:
                 native.gemm_int8(rows, weight, bias, residual=x, out=x, early=early)
-            return
+            return None
         staged = self.comm.staging_view("in", tuple(x.shape), torch.bfloat16)
         for n, (rows, weight, bias) in enumerate(parts):
             native.gemm_int8(rows, weight, residual=staged if n else None, out=staged)
             if bias is not None:
                 x.add_(bias * self.world)
-        self._summed = self.comm.all_reduce(staged)
+        return self.comm.all_reduce(staged)
 
-    def _int8_settle(self, x):
-        """Adds what the last layer left for a norm that does not come."""
-        if self._summed is not None:
-            x.add_(self._summed)
-            self._summed = None
-
-    def _int8_layer(self, i, x, qkv, q_rot, cat, act_buf, batch, seq, decode: bool):
+    def _int8_layer(self, i, x, qkv, q_rot, cat, act_buf, batch, seq, decode: bool, summed=None):
+        """``summed``: what the layer before returned, the ranks' sum that the first norm adds to ``x``."""
         L = self.layers[i]
         early = decode and self.world == 1  # (see _layer)
         # (the kernels behind the rows are products, which read early only weights: `ahead` on one rank, where nothing waits for a peer)
-        rows = self._int8_norm(x, L["ln1"])
+        rows = self._int8_norm(x, L["ln1"], summed)
         mlp_rows = None
         if self.parallel:  # the MLP reads the block input as well
             mlp_rows = rows if L["ln2"] is None else self._int8_norm(x, L["ln2"])
@@ -413,12 +406,11 @@ class DecoderEngine:
         attn = self._attend(i, qkv, q_rot, cat, batch, seq, decode, early)
         attn_rows = native.rows_int8(attn, ahead=self.world == 1)
         if not self.parallel:
-            self._int8_row_parallel([(attn_rows, L["wo"], L["bo"])], x, early)
-            mlp_rows = self._int8_norm(x, L["ln2"])
+            mlp_rows = self._int8_norm(x, L["ln2"], self._int8_row_parallel([(attn_rows, L["wo"], L["bo"])], x, early))
         hidden = cat[:, self.nq * self.head_dim :] if self.parallel else act_buf
         native.gemm_int8(mlp_rows, L["w1"], L["b1"], act=self.act, out=hidden, early=early)
         down = (native.rows_int8(hidden, ahead=self.world == 1), L["wd"], L["bd"])
-        self._int8_row_parallel([(attn_rows, L["wo"], L["bo"]), down] if self.parallel else [down], x, early)
+        return self._int8_row_parallel([(attn_rows, L["wo"], L["bo"]), down] if self.parallel else [down], x, early)
 
     def _attend(self, i, qkv, q_rot, cat, batch, seq, decode: bool, early: bool):
         """Rotary embedding, cache and attention of layer ``i`` on its projection ``qkv``; the result is the first columns of ``cat``."""
@@ -441,9 +433,19 @@ class DecoderEngine:
                                      out=attn.unflatten(0, (batch, seq)).unflatten(2, (self.nq, D)))
         return attn
 
-    def _layer(self, i, x, n, qkv, q_rot, cat, act_buf, batch, seq, decode: bool):
+    def _layers(self, x, n, qkv, q_rot, cat, act_buf, batch, seq, decode: bool):
+        """All layers, on the residual stream ``x`` in place."""
         if self.quantize:
-            return self._int8_layer(i, x, qkv, q_rot, cat, act_buf, batch, seq, decode)
+            summed = None
+            for i in range(len(self.layers)):
+                summed = self._int8_layer(i, x, qkv, q_rot, cat, act_buf, batch, seq, decode, summed)
+            if summed is not None:
+                x.add_(summed)
+            return
+        for i in range(len(self.layers)):
+            self._layer(i, x, n, qkv, q_rot, cat, act_buf, batch, seq, decode)
+
+    def _layer(self, i, x, n, qkv, q_rot, cat, act_buf, batch, seq, decode: bool):
         L = self.layers[i]
         D = self.head_dim
         fold = n is None
@@ -517,9 +519,7 @@ class DecoderEngine:
         if self._can_pipeline(batch, seq):
             self._prefill_pipelined(x, n, qkv, q_rot, cat, act_buf, batch, seq)
         else:
-            for i in range(len(self.layers)):
-                self._layer(i, x, n, qkv, q_rot, cat, act_buf, batch, seq, decode=False)
-            self._int8_settle(x)
+            self._layers(x, n, qkv, q_rot, cat, act_buf, batch, seq, decode=False)
         last = x.view(batch, seq, self.hidden)[:, -1].contiguous()
         logits_local = torch.empty(batch, self.vocab_local, **bf)
         logits = self._head(last, logits_local, batch)
@@ -628,10 +628,8 @@ class DecoderEngine:
         positions = self.pos.to(torch.int64).expand(batch) if self.spec.pos_embed is not None else None
         self._embed_tokens(self.ids[:batch], positions, out=self.x[:batch])
         x = self.x[:batch]
-        for i in range(len(self.layers)):
-            self._layer(i, x, self.n[:batch] if batch > 64 else None, self.qkv[:batch], None, self.cat[:batch],
-                        None if self.parallel else self.act_buf[:batch], batch, 1, decode=True)
-        self._int8_settle(x)
+        self._layers(x, self.n[:batch] if batch > 64 else None, self.qkv[:batch], None, self.cat[:batch],
+                     None if self.parallel else self.act_buf[:batch], batch, 1, decode=True)
         logits = self._head(x, self.logits_local[:batch], batch, decode=True)
         native.greedy_pick(logits, self.next_ids[:batch], self.ids[:batch], self.pos, early=self.world == 1)
         self.kernels_per_step = native.launch_count - before

@@ -84,3 +84,34 @@ def test_the_engine_asks_for_it_on_one_rank_only(world, decode, parallel, monkey
     engine._int8_layer(0, x, torch.zeros(2, 24), None, torch.zeros(2, 16), torch.zeros(2, 8), 2, 1, decode)
     assert len(chain.rows) == 4 and set(chain.rows) == {world == 1}
     assert set(chain.products) <= {decode and world == 1, False} and (not decode or world > 1 or all(chain.products))
+
+
+@needs_library
+@pytest.mark.parametrize("parallel", [False, True])
+def test_a_pass_that_ends_early_leaves_nothing_for_the_next(parallel, monkeypatch):
+    """What the ranks' last sum leaves for the next norm belongs to the pass, not to the engine."""
+    from tensor_parallel_b200 import engine as module
+
+    class Chain(_Chain):
+        def rows_int8(self, x, *args, residual=None, **kwargs):
+            self.rows.append(residual is not None)
+            return x, x
+
+    class Two(list):  # (and the second is not there)
+        def __len__(self):
+            return 2
+
+    monkeypatch.setattr(module, "native", chain := Chain())
+    engine = _layer_engine(2, parallel)
+    one, engine.layers = engine.layers, Two(engine.layers)
+    engine.quantize, x = "int8", torch.zeros(2, 8, dtype=torch.bfloat16)
+    args = (torch.zeros(2, 24), None, torch.zeros(2, 16), torch.zeros(2, 8), 2, 1, False)
+    for _ in range(2):
+        chain.rows.clear()
+        with pytest.raises(IndexError):
+            engine._layers(x, None, *args)
+        assert chain.rows[0] is False and sum(chain.rows) == (0 if parallel else 1)
+    chain.rows.clear()
+    engine.layers = one
+    engine._layers(x, None, *args)
+    assert chain.rows[0] is False and not x.any()
