@@ -34,7 +34,8 @@ __device__ __forceinline__ float i8_value(int sum, float sx, float sw, float bia
 // expf and the IEEE division made the epilogue of a 256 x 256 tile longer than its products (8192 x 22016 x 4096, gated: 732 us).
 __device__ __forceinline__ float i8_gate(float x, float u) { return __fdividef(x, 1.f + __expf(-u)); }
 // v Phi(v).  Half of erfc(v / sqrt 2), v >= 0, as a polynomial in t = 1 / (1 + 0.245 v) times exp(-v^2 / 2): coefficients of the least greatest error in units of
-// (value + 0.001), found by reweighted least squares over 0 .. 14.  Off by 4e-9 (6e-6 of it up to v = 5), in fp32 by 2.2e-7.  With erff, whose two branches a warp walks
+// (value + 0.001), found by reweighted least squares over 0 .. 14.  With the coefficients as they stand half of erfc is off by 3.0e-8 (5.3e-6 of it up to v = 5, 1.5e-4 up
+// to 8, 1.2e-3 up to 13), v times it by 6.6e-9; fp32 adds a few 2^-24 of the terms.  With erff, whose two branches a warp walks
 // one after the other, the epilogue of 2820 x 11648 x 1088 took longer than its products.
 __device__ __forceinline__ float i8_gelu(float v) {
   const float t = __fdividef(1.f, __fmaf_rn(0.245f, fabsf(v), 1.f));
