@@ -333,9 +333,11 @@ class DecoderEngine:
                 self.prefill(torch.zeros(batch, min(seq, self.max_seq - 2), dtype=torch.int64, device=self.device))
             for _ in range(2):
                 self._decode_body(batch)
-            # the PyTorch kernels that only the multi-rank path uses (strided copies, in-place add)
+            # the PyTorch kernels that only the multi-rank path uses (strided copies, in-place add, of a bias to all rows)
             t = self.x[:batch]
             t.add_(t)
+            rows = self.x.new_zeros(2, self.x.shape[1])
+            rows.add_(rows[0] * world)
             g = self.logits_local[:batch, : max(8, self.vocab_local // 2)].contiguous()
             torch.stack([g, g]).permute(1, 0, 2).reshape(batch, -1).float().argmax(-1)
             self.pos.zero_()

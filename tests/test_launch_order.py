@@ -115,3 +115,27 @@ def test_a_pass_that_ends_early_leaves_nothing_for_the_next(parallel, monkeypatc
     engine.layers = one
     engine._layers(x, None, *args)
     assert chain.rows[0] is False and not x.any()
+
+
+@needs_library
+def test_a_rank_alone_runs_the_tensor_kernels_of_several(monkeypatch):
+    """A kernel that is launched for the first time may be loaded then, which may wait for the device: not behind a kernel that waits for a peer which the same thread has yet to
+    launch.  So a rank's own passes include the operations that only several ranks take: a bias times the number of ranks, added to all rows."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from tensor_parallel_b200.ops import native
+
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types_, args=(), kwargs=None):
+            seen.append((func, [tuple(a.shape) for a in args if isinstance(a, torch.Tensor)]))
+            return func(*args, **(kwargs or {}))
+
+    monkeypatch.setattr(native, "LIB", types.SimpleNamespace(tpb_gemm_preload=lambda: 0, tpb_comm_preload=lambda: 0, tpb_int8_preload=lambda: 0))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    engine = types.SimpleNamespace(comm=object(), world=2, head_split="vocab", embed_split=False, max_seq=80, device="cpu", vocab_local=32, x=torch.zeros(1, 8), quantize="int8",
+                                   logits_local=torch.zeros(1, 32), pos=torch.zeros(1), ids=torch.zeros(1), prefill=lambda ids: None, _decode_body=lambda batch: None)
+    with Watch():
+        DecoderEngine.preload(engine)
+    assert (torch.ops.aten.mul.Tensor, [(8,)]) in seen and (torch.ops.aten.add_.Tensor, [(2, 8), (8,)]) in seen
