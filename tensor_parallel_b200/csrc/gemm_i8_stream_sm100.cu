@@ -334,7 +334,7 @@ static int is_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
              : TPB_ERR_CUDA;
 }
 
-int gemm_i8_stream_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
+static int is_pick(const I8Gemm& g, int sms, cudaStream_t stream) {
   // one unit per CTA: slices of the contraction side by side, as long as each has a few stages
   const bool one_unit = (g.features + IS_UNIT - 1) / IS_UNIT <= sms && g.k >= 2048;
   if (one_unit && g.tokens <= 8) return is_launch<32, 4, 2, 4>(g, sms, stream);
@@ -343,6 +343,23 @@ int gemm_i8_stream_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
   if (g.tokens <= 32) return is_launch<32, 8, 2, 1>(g, sms, stream);
   if (g.tokens <= 64) return is_launch<64, 2, 2, 1>(g, sms, stream);
   return TPB_ERR_ARG;
+}
+
+// More rows than a launch counts (310 million on 148 SMs) go by several.
+int gemm_i8_stream_launch(const I8Gemm& g, int sms, cudaStream_t stream) {
+  const long long most = StreamRows::most_rows(sms);
+  int rc = TPB_OK;
+  for (long long f = 0; f < g.features && rc == TPB_OK; f += most) {
+    I8Gemm part = g;
+    part.features = int(g.features - f < most ? g.features - f : most);
+    part.w += f * g.ldw;
+    part.sw += f;
+    part.out += g.act == I8_GATED ? f / 2 : f;
+    if (g.bias) part.bias += f;
+    if (g.residual) part.residual += f;
+    rc = is_pick(part, sms, stream);
+  }
+  return rc;
 }
 
 cudaError_t gemm_i8_stream_preload() {

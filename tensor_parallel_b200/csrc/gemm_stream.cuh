@@ -34,6 +34,8 @@ struct StreamGemm {
 struct StreamRows {
   static constexpr int UNIT = 32;      // rows of a unit; the gated activation pairs 16 gate rows with their 16 up rows
   static constexpr int PASS_UNITS = 4;  // 128 rows: the lanes of TMEM
+  static constexpr int MOST_PASSES = 1 << 14;  // a range of 4 x 2^14 units times 2^14 passes fits 32 bits (in 64, pass_start made the kernels 30 % slower)
+  static long long most_rows(int sms) { return (long long)UNIT * PASS_UNITS * MOST_PASSES * sms; }  // of a launch
   int units, grid, passes;
   int pass_units;  // units of the longest pass of any CTA
   int box_units;   // of the shortest: every pass is at least one box of this many units
@@ -53,7 +55,7 @@ inline StreamRows gemm_stream_rows(int features, int sms) {
 }
 
 // True if a few-token (at most 64) GEMM of this shape streams its weights on one pass of row ranges, false if split-K tiles
-// are the better decomposition.
+// are the better decomposition, or the rows more than a launch of this kernel counts.
 bool gemm_stream_fits(int features, int k, int sms);
 int gemm_stream_launch(const StreamGemm& g, int sms, cudaStream_t stream);
 cudaError_t gemm_stream_preload();

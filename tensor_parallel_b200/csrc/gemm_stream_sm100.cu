@@ -473,7 +473,7 @@ static int gs_launch(const StreamGemm& g, int sms, cudaStream_t stream) {
 
 bool gemm_stream_fits(int features, int k, int sms) {
   const long long unit_bytes = 2LL * GS_UNIT * k;
-  return (features + GS_UNIT - 1) / GS_UNIT >= sms / 2 || unit_bytes <= 1024 * 1024;
+  return features <= StreamRows::most_rows(sms) && ((features + GS_UNIT - 1) / GS_UNIT >= sms / 2 || unit_bytes <= 1024 * 1024);
 }
 
 // 512 contiguous bytes of every weight row per stage where rows are long and a stage stays small, else 256 in twice as many stages:
@@ -513,6 +513,7 @@ cudaError_t gemm_stream_preload() {
 // units at which the passes of CTA `cta` begin and the last one ends (room for `capacity` of them).
 extern "C" int tpb_gemm_stream_rows(int features, int sms, int cta, int* shape, int* starts, int capacity) {
   if (features <= 0 || sms <= 0 || cta < 0 || !shape || !starts) return TPB_ERR_ARG;
+  if (features > tpb::StreamRows::most_rows(sms)) return TPB_ERR_SIZE;
   const tpb::StreamRows r = tpb::gemm_stream_rows(features, sms);
   if (cta >= r.grid || r.passes >= capacity) return TPB_ERR_ARG;
   const int values[5] = {r.units, r.grid, r.passes, r.pass_units, r.box_units};
