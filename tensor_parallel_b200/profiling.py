@@ -205,6 +205,7 @@ CASES = {
     "head_cross_entropy": lambda it: case_cross_entropy(8192, 32000, 4096, it),
     "rmsnorm": lambda it: case_norm(32768, 4096, it),
     "int8_norm": lambda it: case_int8_rows(8192, 4096, it, norm=0, residual=True),
+    "int8_norm_alone": lambda it: case_int8_rows(8192, 4096, it, norm=0),
     "int8_rows": lambda it: case_int8_rows(8192, 11008, it),
     "int8_decode_gate_up": lambda it: case_int8_product(8, 22016, 4096, it, act="swiglu16"),
     "int8_short_down": lambda it: case_int8_product(100, 4096, 11008, it),
