@@ -372,8 +372,8 @@ def rms_norm_int8(x, weight, eps: float = 1e-6, residual=None) -> Tuple[Int8Rows
 
 
 def layer_norm_int8(x, weight, bias, eps: float = 1e-5, residual=None) -> Tuple[Int8Rows, torch.Tensor]:
-    """Like :func:`rms_norm_int8`, with a LayerNorm (whose squares are those of the deviations, and whose sum of values has a part in it); ``weight`` and
-    ``bias`` may be None."""
+    """Like :func:`rms_norm_int8`, with a LayerNorm; ``weight`` and ``bias`` may be None.  A row gets the scale NaN where the sum of its values, or of the
+    squares of its deviations, passes the range of fp32."""
     if not _compiling():
         out = norm_int8_directly(x, weight, bias, eps, 1, residual)
         if out is not None:
