@@ -298,7 +298,7 @@ bool interposed() {
 }
 
 bool plain(const Tensor& t, at::ScalarType dtype, const c10::Device& device) {
-  return t.scalar_type() == dtype && t.device() == device && t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() &&
+  return t.scalar_type() == dtype && t.device() == device && t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.is_neg() &&
          !(at::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined();
 }
 // Rows that lie one pitch apart: their number, and the pitch (of a single row, its length rounded up).

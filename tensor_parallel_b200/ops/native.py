@@ -1010,7 +1010,8 @@ def rows_int8(x2d, weight=None, bias=None, eps=0.0, norm=None, residual=None, su
 
 
 def _rows_view(t):
-    """``t`` as rows with unit inner stride: a view where its strides allow it."""
+    """``t`` as rows with unit inner stride, whose memory holds its values (not their negatives): a view where its strides allow it."""
+    t = t.resolve_neg()
     t = t if t.ndim == 2 else t.reshape(-1, t.shape[-1])
     rows, cols = t.shape
     return t if (t.stride(1) == 1 or cols == 1) and (t.stride(0) >= cols or rows == 1) else t.contiguous()
@@ -1037,7 +1038,7 @@ def quantize_int8(x) -> OF.Int8Rows:
 def norm_int8(x, weight, bias, eps, mode, residual=None):
     with torch.cuda.device(x.device):
         x2d = _rows_view(x)
-        w, b = (None if t is None else t.to(x.dtype).contiguous() for t in (weight, bias))
+        w, b = (None if t is None else t.to(x.dtype).resolve_neg().contiguous() for t in (weight, bias))
         res = None if residual is None else _rows_view(residual)
         summed = None if residual is None else torch.empty(x2d.shape, dtype=x.dtype, device=x.device)
         rows = rows_int8(x2d, w, b, eps, mode, res, summed)
@@ -1079,12 +1080,12 @@ def _int8_ready(t: torch.Tensor) -> torch.Tensor:
 
 
 def linear_int8(x: OF.Int8Rows, weight: OF.Int8Rows, bias=None, act=None, residual=None):
-    (xv, sx), (wv, sw) = x, weight
+    (xv, sx), (wv, sw) = ((values.resolve_neg(), scales.resolve_neg()) for values, scales in (x, weight))
     with torch.cuda.device(xv.device):
         shape = xv.shape
         x2d = xv if xv.ndim == 2 else xv.reshape(-1, shape[-1])
         res = None if residual is None else _rows_view(residual)
-        out = gemm_int8((x2d, sx.reshape(-1).contiguous()), (wv, sw.contiguous()), None if bias is None else bias.contiguous(), act, res)
+        out = gemm_int8((x2d, sx.reshape(-1).contiguous()), (wv, sw.contiguous()), None if bias is None else bias.resolve_neg().contiguous(), act, res)
         return out if len(shape) == 2 else out.view(*shape[:-1], out.shape[1])
 
 
