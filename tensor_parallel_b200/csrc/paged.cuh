@@ -1,0 +1,50 @@
+// Shared by the kernels of a paged cache: what a sequence of the batch comes to, and the tensor maps over the pages.
+//
+// A cache holds keys and values as [pages][kv_heads][page_size][head_dim]; key j of a sequence is slot j % page_size of page table[sequence][j / page_size].
+// The batch is ragged: the new tokens of sequence s are the rows starts[s] .. starts[s + 1] of the queries, behind past[s] cached ones.  Lengths and
+// table live in device memory and change from step to step under a captured graph, so every kernel checks what it reads of them: a sequence that
+// does not fit the rows, the table or the cache is recorded as STATUS_BAD_ARG and answered with NaN, and nothing is read or written through its entries.
+#pragma once
+#include <cuda_bf16.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include "attention_sm100.cuh"
+#include "ptx_sm100.cuh"
+#include "tpb_api.h"
+
+namespace tpb {
+
+struct PagedBatch {
+  const int* starts;
+  const int* past;
+  const int* table;
+  long long table_ld;
+  int n, tokens, table_width, pages, page_shift;
+  int most_new;  // more new tokens than this are an error
+  uint32_t* status;
+};
+
+struct PagedSequence {
+  int token0, fresh, past;
+  bool bad;  // its rows are [token0, token0 + fresh) all the same
+};
+
+__device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch& b, int s) {
+  const int a = __ldg(b.starts + s), e = __ldg(b.starts + s + 1), past = __ldg(b.past + s);
+  PagedSequence q;
+  q.token0 = min(max(a, 0), b.tokens);
+  q.fresh = min(max(e, q.token0), b.tokens) - q.token0;
+  q.past = past;
+  q.bad = q.token0 != a || q.token0 + q.fresh != e || past < 0 || q.fresh > b.most_new ||
+          (q.fresh > 0 && (long long)past + q.fresh > ((long long)b.table_width << b.page_shift)) || (long long)past + q.fresh > INT_MAX - 256;
+  return q;
+}
+
+// A cache whose slots TMA can read: head_dim contiguous, the other strides multiples of 16 bytes.  Box: 64 elements of `rows` slots of one page.
+static int paged_tmap(CUtensorMap* map, const void* ptr, int head_dim, int page_size, int kv_heads, int pages, long long s_slot, long long s_head, long long s_page,
+                      int rows) {
+  return fa_tmap(map, ptr, head_dim, rows, page_size, kv_heads, pages, s_slot, s_head, s_page);
+}
+
+}  // namespace tpb

@@ -1,0 +1,685 @@
+// Attention of new tokens over a paged cache, for sequences with few query rows (a new token or a few of them, times the query heads of a KV head).
+//
+//   o[t, h] = sum_j softmax_j(scale * q[t, h] . k[j]) v[j],   j in (p - window, p],   p = past + t the token's own position
+//
+// What bounds it is reading the pages once: 4 * head_dim bytes per key and KV head, and two products of 16 rows with each.  One launch deals with every
+// sequence of the batch, whatever their lengths: the work (sequence, row tile, KV head, tile of 64 keys) lies on one line, cut into as many equal
+// ranges as there are CTAs.  A range may begin and end inside a row tile's keys; such pieces leave unnormalised sums with their maximum in a workspace, and a
+// second kernel, launched ahead, joins them in the order of the keys (no counters, no atomics: the result does not depend on timing, and calls on
+// other streams or captured graphs share nothing).
+//
+//   producer warp : walks the range; TMA boxes of up to 64 slots per page into a ring of stages (keys and values of 64 keys), up to 32 table entries
+//                   fetched at a time and 32 ahead; query rows by cp.async into one of two buffers, so that the next piece's are there when its first keys are
+//   compute warps : a warp holds 16 query rows and a part of the stage's keys (ROW_GROUPS x key groups): mma.sync m16n8k16 (what there is to multiply
+//                   here leaves the tensor cores idle; tcgen05 would fill 128 rows for 1 to 64), its own running maximum and sum; key groups meet at the end of a piece
+//
+// Keys outside a sequence (the rest of its last page, slots that left the window) may hold anything: their scores are replaced, not added to, and
+// their values are cut out of the fragments, so that neither NaN nor infinities get through.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "launch.cuh"
+#include "paged.cuh"
+
+namespace tpb {
+
+typedef __nv_bfloat16 bf16;
+
+constexpr int PA_TILE = 64;                 // keys of a stage
+constexpr int PA_BLOCK = PA_TILE * 128;     // bytes of a swizzled block of 64 keys x 64 elements
+constexpr int PA_MIN_SHARE = 2;             // tiles of a CTA's range, at least
+
+struct PagedAttnParams {
+  PagedBatch b;
+  const bf16* q;
+  bf16* out;
+  long long q_st, q_sh, o_st, o_sh;
+  int heads, kv_heads, group, window;
+  int rows_low, rows_high;  // sequences with rows (new tokens x group) in [rows_low, rows_high] are this launch's
+  int takes_bad;            // and those whose lengths are not possible
+  int fill_rest;            // rows outside all sequences become zeros
+  float scale_log2e;
+  float* part_o;            // [2 per CTA][16 * ROW_GROUPS][head_dim]
+  float2* part_ml;          // [2 per CTA][16 * ROW_GROUPS] maximum (of scaled scores, in powers of two) and sum
+  int4* joins;              // [2 per CTA]: the row tile whose keys begin in this CTA's range and end in another's
+};
+
+// A sequence as this launch deals with it.
+struct PagedUnits {
+  PagedSequence s;
+  int rows, row_tiles, first_tile, tiles;  // tiles of keys, from first_tile on
+  long long cost;                          // row_tiles * kv_heads * tiles, 0: not this launch's
+};
+
+template <int ROWS>
+__device__ __forceinline__ PagedUnits paged_units(const PagedAttnParams& p, int s) {
+  PagedUnits u;
+  u.s = paged_sequence(p.b, s);
+  u.rows = u.s.fresh * p.group;
+  u.row_tiles = (u.rows + ROWS - 1) / ROWS;
+  const bool mine = u.rows > 0 && (u.s.bad ? p.takes_bad : u.rows >= p.rows_low && u.rows <= p.rows_high);
+  u.first_tile = 0;
+  u.tiles = 1;  // (a bad sequence: one tile without keys)
+  if (!u.s.bad) {
+    u.first_tile = p.window ? max(0, u.s.past - p.window + 1) / PA_TILE : 0;
+    u.tiles = (u.s.past + u.s.fresh + PA_TILE - 1) / PA_TILE - u.first_tile;
+  }
+  u.cost = mine ? (long long)u.row_tiles * p.kv_heads * u.tiles : 0;
+  return u;
+}
+
+enum { PIECE_FIRST = 1, PIECE_LAST = 2, PIECE_POISON = 4 };
+
+struct PagedPiece {  // of a row tile's keys, as the producer hands it to the compute warps
+  int token0, row0, rows, past, total, low, kvh;  // low: first key that any row of the sequence sees
+  int slot;                                       // of the workspace, -1: the piece is the whole
+  int bad;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_wait_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pa_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <int D, int R>
+struct Few {
+  static constexpr int ROWS = 16 * R;
+  static constexpr int WARPS = R == 1 ? 4 : 8;
+  static constexpr int KEY_GROUPS = WARPS / R;
+  static constexpr int KEYS = PA_TILE / KEY_GROUPS;  // of a warp
+  static constexpr int CTAS = R == 1 ? 2 : 1;        // per SM
+  static constexpr int DB = D / 64;
+  static constexpr int STAGE_BYTES = 2 * DB * PA_BLOCK;
+  static constexpr int STAGES = (R == 1 ? 96 : 160) * 1024 / STAGE_BYTES;
+  static constexpr int Q_BYTES = ROWS * D * 2;
+  static constexpr int MERGE_FLOATS = WARPS * 2 * D;
+  static constexpr int THREADS = WARPS * 32 + 32;
+  static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 2 * Q_BYTES + MERGE_FLOATS * 4 + WARPS * 16 * 8 + STAGES * 8 + 2 * int(sizeof(PagedPiece)) +
+                              (2 * STAGES + 6) * 8 + 256;
+};
+
+template <int D, int R>
+__global__ void __launch_bounds__(Few<D, R>::THREADS, Few<D, R>::CTAS)
+paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const PagedAttnParams p) {
+  using C = Few<D, R>;
+  constexpr int DB = C::DB, STAGES = C::STAGES, WARPS = C::WARPS, ROWS = C::ROWS;
+
+  extern __shared__ uint8_t pa_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem;                                    // [STAGES][keys | values][DB][64 keys][128 bytes]
+  uint8_t* q_s = ring + STAGES * C::STAGE_BYTES;           // [2][DB][ROWS][128 bytes], swizzled like the ring
+  float* merge = reinterpret_cast<float*>(q_s + 2 * C::Q_BYTES);         // [WARPS][2 rows][D]
+  float2* stats = reinterpret_cast<float2*>(merge + C::MERGE_FLOATS);    // [WARPS][16 rows]
+  int2* stage_info = reinterpret_cast<int2*>(stats + WARPS * 16);        // [STAGES] first key, flags
+  PagedPiece* pieces = reinterpret_cast<PagedPiece*>(stage_info + STAGES);  // [2]
+  uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(pieces + 2) + 7) & ~uintptr_t(7));
+  uint64_t* full = bars;
+  uint64_t* empty = bars + STAGES;
+  uint64_t* q_full = bars + 2 * STAGES;       // [2]
+  uint64_t* q_empty = bars + 2 * STAGES + 2;  // [2]
+  uint64_t* meet = bars + 2 * STAGES + 4;     // the compute warps, phase by phase
+  volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+  __shared__ long long scan_s[C::THREADS / 32];
+  __shared__ long long found_begin;
+  __shared__ int found_seq;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmap_k);
+    prefetch_tmap(&tmap_v);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], WARPS);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 33);  // the lanes' copies and the piece
+      mbar_init(&q_empty[s], WARPS);
+    }
+    mbar_init(meet, WARPS);
+    *abort_flag = 0;
+    found_seq = p.b.n;
+    found_begin = 0;
+    fence_mbar_init();
+  }
+  pa_launch_next();  // (the whole grid is resident; the joining kernel waits for its end)
+
+  // ---- this CTA's range: all costs summed up, then the sequence in which the range begins ----
+  auto block_scan = [&](long long v, long long& before, long long& total) {
+    long long inc = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
+    }
+    __syncthreads();
+    if (lane == 31) scan_s[warp] = inc;
+    __syncthreads();
+    before = inc - v;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < C::THREADS / 32; ++w) {
+      if (w < warp) before += scan_s[w];
+      total += scan_s[w];
+    }
+  };
+  long long all = 0, mine_before = 0, mine = 0;
+  for (int base = 0; base < p.b.n; base += C::THREADS) {
+    const int s = base + threadIdx.x;
+    long long cost = 0, before, total;
+    if (s < p.b.n) {
+      const PagedUnits u = paged_units<ROWS>(p, s);
+      cost = u.cost;
+      if (u.s.bad && p.takes_bad && blockIdx.x == 0) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+    }
+    block_scan(cost, before, total);
+    mine_before = all + before;
+    mine = cost;
+    all += total;
+  }
+  const long long share = max((long long)PA_MIN_SHARE, (all + gridDim.x - 1) / gridDim.x);
+  const long long w0 = min(all, share * blockIdx.x), w1 = min(all, w0 + share);
+  if (p.b.n <= C::THREADS) {
+    if (mine > 0 && w0 >= mine_before && w0 < mine_before + mine) {
+      found_seq = threadIdx.x;
+      found_begin = mine_before;
+    }
+  } else {
+    long long so_far = 0;
+    for (int base = 0; base < p.b.n && so_far <= w0; base += C::THREADS) {
+      const int s = base + threadIdx.x;
+      long long before, total;
+      const long long cost = s < p.b.n ? paged_units<ROWS>(p, s).cost : 0;
+      block_scan(cost, before, total);
+      before += so_far;
+      if (cost > 0 && w0 >= before && w0 < before + cost) {
+        found_seq = s;
+        found_begin = before;
+      }
+      so_far += total;
+    }
+  }
+  if (threadIdx.x < 2) p.joins[2 * blockIdx.x + threadIdx.x] = make_int4(-1, 0, 0, 0);
+  __syncthreads();
+
+  if (p.fill_rest) {
+    const int used0 = p.b.n ? min(max(__ldg(p.b.starts), 0), p.b.tokens) : p.b.tokens;
+    const int used1 = p.b.n ? min(max(__ldg(p.b.starts + p.b.n), used0), p.b.tokens) : p.b.tokens;
+    const int rest = used0 + p.b.tokens - used1, chunks = p.heads * (D / 8);
+    for (int i = blockIdx.x; i < rest; i += gridDim.x) {
+      const long long t = i < used0 ? i : used1 + (i - used0);
+      for (int c = threadIdx.x; c < chunks; c += C::THREADS)
+        *reinterpret_cast<uint4*>(p.out + t * p.o_st + (c / (D / 8)) * p.o_sh + (c % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  auto give_up = [&]() {
+    atomicMax(p.b.status, uint32_t(STATUS_TIMEOUT_MBAR));
+    *abort_flag = 1;
+  };
+
+  if (warp == WARPS) {
+    // ---------------- producer ----------------
+    const int page_size = 1 << p.b.page_shift;
+    const int per_tile = max(1, PA_TILE >> p.b.page_shift);  // pages of a tile
+    const int box_rows = min(page_size, PA_TILE);
+    const int my_page = lane / (2 * DB), my_block = lane % (2 * DB);  // the box of this lane
+    int seq = found_seq, it = 0, piece = 0;
+    long long at = w0, seq_begin = found_begin;
+    bool ok = true;
+    while (ok && at < w1) {
+      ok = seq < p.b.n;  // (the costs add up to w1, unless somebody writes the lengths meanwhile)
+      if (!ok) break;
+      const PagedUnits u = paged_units<ROWS>(p, seq);
+      if (at >= seq_begin + u.cost) {
+        seq_begin += u.cost;
+        ++seq;
+        continue;
+      }
+      const long long unit = (at - seq_begin) / u.tiles;
+      const int t0 = int((at - seq_begin) - unit * u.tiles);
+      const int t1 = int(min((long long)u.tiles, t0 + (w1 - at)));
+      const int kvh = int(unit % p.kv_heads), row0 = int(unit / p.kv_heads) * ROWS;
+      const int total = u.s.bad ? 0 : u.s.past + u.s.fresh;
+      const int low = p.window && !u.s.bad ? max(0, u.s.past - p.window + 1) : 0;
+      const int qb = piece & 1;
+      // table entries, 32 at a time and 32 ahead
+      const int* row = p.b.table + (long long)seq * p.b.table_ld;
+      int entry0 = (u.first_tile + t0) * PA_TILE >> p.b.page_shift;
+      const int entries = total > 0 ? ((total - 1) >> p.b.page_shift) + 1 : 0;
+      auto fetch = [&](int e) { return e < entries ? __ldg(row + e) : -1; };
+      int now = fetch(entry0 + lane), next = fetch(entry0 + 32 + lane);
+      // ---- query rows ----
+      ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], ((piece >> 1) & 1) ^ 1));
+      if (!ok) break;
+      if (lane == 0) {
+        PagedPiece& o = pieces[qb];
+        o.token0 = u.s.token0;
+        o.row0 = row0;
+        o.rows = min(ROWS, u.rows - row0);
+        o.past = u.s.past;
+        o.total = total;
+        o.low = low;
+        o.kvh = kvh;
+        o.bad = u.s.bad;
+        // keys that begin in this range and end in another's are joined by the block of this CTA; its other piece continues the range in front
+        o.slot = t0 == 0 && t1 == u.tiles ? -1 : 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+        if (t0 == 0 && t1 < u.tiles) {
+          const long long unit_end = seq_begin + (unit + 1) * u.tiles;
+          p.joins[2 * blockIdx.x] = make_int4(o.token0, row0, o.rows, kvh);
+          p.joins[2 * blockIdx.x + 1] = make_int4(int((unit_end - 1) / share), 0, 0, 0);
+        }
+      }
+      {
+        const int chunks = ROWS * (D / 8), left = u.rows - row0;
+        for (int c = lane; c < chunks; c += 32) {
+          const int r = c / (D / 8), e = c % (D / 8);
+          const int t = (row0 + min(r, left - 1)) / p.group, g = (row0 + min(r, left - 1)) % p.group;
+          const bf16* src = p.q + (long long)(u.s.token0 + t) * p.q_st + (long long)(kvh * p.group + g) * p.q_sh + e * 8;
+          cp_async16(smem_u32(q_s + qb * C::Q_BYTES + (e >> 3) * (ROWS * 128) + r * 128 + (((e & 7) ^ (r & 7)) << 4)), src, r < left ? 16 : 0);
+        }
+        cp_async_arrive(&q_full[qb]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[qb]);
+      }
+      // ---- keys and values ----
+      for (int t = t0; t < t1; ++t, ++it) {
+        const int stage = it % STAGES;
+        const int key0 = (u.first_tile + t) * PA_TILE;
+        int e = (key0 >> p.b.page_shift) - entry0;
+        if (e >= 32) {
+          entry0 += 32;
+          e -= 32;
+          now = next;
+          next = fetch(entry0 + 32 + lane);
+        }
+        const int page = __shfl_sync(0xffffffffu, now, (e + my_page) & 31);
+        const int first = key0 + my_page * page_size;  // (of pages shorter than a tile; longer ones have one box, with keys of use in it)
+        const bool wanted = lane < per_tile * 2 * DB && (per_tile == 1 || (first < total && first + page_size > low)) && total > 0;
+        const bool good = wanted && page >= 0 && page < p.b.pages;
+        const uint32_t boxes = __ballot_sync(0xffffffffu, good), lost = __ballot_sync(0xffffffffu, wanted && !good);
+        ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait(&empty[stage], ((it / STAGES) & 1) ^ 1));
+        if (!ok) break;
+        if (lane == 0) {
+          if (lost) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+          stage_info[stage] = make_int2(key0, (t == t0 ? PIECE_FIRST : 0) | (t == t1 - 1 ? PIECE_LAST : 0) | (lost ? PIECE_POISON : 0));
+          mbar_expect_tx(&full[stage], __popc(boxes) * box_rows * 128);
+        }
+        __syncwarp();
+        if (good)
+          tma_load_4d(ring + stage * C::STAGE_BYTES + my_block * PA_BLOCK + my_page * box_rows * 128, my_block < DB ? &tmap_k : &tmap_v, &full[stage],
+                      (my_block % DB) * 64, per_tile == 1 ? key0 & (page_size - 1) : 0, kvh, page);
+      }
+      if (!ok) break;
+      at += t1 - t0;
+      ++piece;
+    }
+    if (!ok && lane == 0 && !*abort_flag) give_up();
+    return;
+  }
+
+  // ---------------- compute warps ----------------
+  constexpr int NT = C::KEYS / 8;  // blocks of 8 keys
+  const int rg = warp % R, kg = warp / R;
+  const int key_off = kg * C::KEYS;
+  const int g8 = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;
+  const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(q_s);
+  const int count = int(w1 - w0);
+  float o[D / 8][4];
+  float m[2], l[2];
+  uint32_t qf[R == 1 ? D / 16 : 1][4];
+  PagedPiece pc = {};
+  int pos[2] = {0, 0}, piece = 0;
+  uint32_t meet_phase = 0;
+  bool poisoned = false;
+  bool ok = true;
+  auto meet_all = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(meet);
+    ok = __all_sync(0xffffffffu, mbar_wait(meet, meet_phase));
+    meet_phase ^= 1;
+    return ok;
+  };
+  for (int it = 0; it < count; ++it) {
+    const int stage = it % STAGES;
+    ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait(&full[stage], (it / STAGES) & 1));
+    if (!ok) break;
+    const int2 info = stage_info[stage];
+    const int key0 = info.x + key_off;
+    if (info.y & PIECE_FIRST) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&q_full[piece & 1], (piece >> 1) & 1));
+      if (!ok) break;
+      pc = pieces[piece & 1];
+      poisoned = pc.bad;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        pos[i] = pc.past + (pc.row0 + rg * 16 + g8 + 8 * i) / p.group;
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+      if (R == 1) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const int r = (mi & 1) * 8 + mr, c = kk * 2 + (mi >> 1);
+          ldsm4(qf[R == 1 ? kk : 0], q_a + (piece & 1) * C::Q_BYTES + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        }
+      }
+    }
+    poisoned |= (info.y & PIECE_POISON) != 0;
+    // ---- scores ----
+    float sc[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
+    const uint32_t k_a = ring_a + stage * C::STAGE_BYTES, v_a = k_a + DB * PA_BLOCK;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      uint32_t a[4];
+      if (R == 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] = qf[R == 1 ? kk : 0][j];
+      } else {
+        const int r = rg * 16 + (mi & 1) * 8 + mr, c = kk * 2 + (mi >> 1);
+        ldsm4(a, q_a + (piece & 1) * C::Q_BYTES + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+      }
+#pragma unroll
+      for (int np = 0; np < NT / 2; ++np) {
+        uint32_t b[4];
+        const int r = key_off + np * 16 + (mi >> 1) * 8 + mr, c = kk * 2 + (mi & 1);
+        ldsm4(b, k_a + (c >> 3) * PA_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        mma16816(sc[2 * np], a, b[0], b[1]);
+        mma16816(sc[2 * np + 1], a, b[2], b[3]);
+      }
+    }
+    // ---- mask, maximum, probabilities ----
+    const int last_pos = pc.past + (pc.row0 + pc.rows - 1) / p.group;
+    const bool plain = key0 + C::KEYS - 1 <= pc.past + pc.row0 / p.group && (!p.window || key0 > last_pos - p.window);
+    float mt[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v = sc[i][j] * p.scale_log2e;
+        if (!plain) {
+          const int key = key0 + i * 8 + t4 * 2 + (j & 1), at = pos[j >> 1];
+          if (key > at || (p.window && key <= at - p.window)) v = -INFINITY;
+        }
+        sc[i][j] = v;
+        mt[j >> 1] = fmaxf(mt[j >> 1], v);
+      }
+    bool rises = false;
+    float base[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 1));
+      mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 2));
+      rises |= mt[i] > m[i];
+    }
+    if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float mn = fmaxf(m[i], mt[i]);
+        const float f = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - mn);
+        m[i] = mn;
+        l[i] *= f;
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) {
+          o[d][2 * i] *= f;
+          o[d][2 * i + 1] *= f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sc[i][j] = ex2_approx(sc[i][j] - base[j >> 1]);
+        l[j >> 1] += sc[i][j];
+      }
+    // ---- values ----
+    const bool cut = key0 < pc.low || key0 + C::KEYS > pc.total;
+#pragma unroll
+    for (int ks = 0; ks < NT / 2; ++ks) {
+      uint32_t a[4] = {pack_bf16x2(sc[2 * ks][0], sc[2 * ks][1]), pack_bf16x2(sc[2 * ks][2], sc[2 * ks][3]),
+                       pack_bf16x2(sc[2 * ks + 1][0], sc[2 * ks + 1][1]), pack_bf16x2(sc[2 * ks + 1][2], sc[2 * ks + 1][3])};
+      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+      if (cut) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int key = key0 + ks * 16 + i * 8 + t4 * 2;
+          keep[i] = (key >= pc.low && key < pc.total ? 0xffffu : 0u) | (key + 1 >= pc.low && key + 1 < pc.total ? 0xffff0000u : 0u);
+        }
+      }
+#pragma unroll
+      for (int dn = 0; dn < D / 16; ++dn) {
+        uint32_t b[4];
+        const int r = key_off + ks * 16 + (mi & 1) * 8 + mr, c = dn * 2 + (mi >> 1);
+        ldsm4_t(b, v_a + (c >> 3) * PA_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        mma16816(o[2 * dn], a, b[0] & keep[0], b[1] & keep[1]);
+        mma16816(o[2 * dn + 1], a, b[2] & keep[0], b[3] & keep[1]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[stage]);
+
+    if (info.y & PIECE_LAST) {
+      // ---- the key groups meet: a row (and the one eight below it) at a time ----
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if (t4 == 0) stats[warp * 16 + g8 + 8 * i] = make_float2(m[i], l[i]);
+      }
+      if (!meet_all()) break;
+      float f[2], top[2], sum[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = -INFINITY;
+        sum[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < C::KEY_GROUPS; ++k) top[i] = fmaxf(top[i], stats[(k * R + rg) * 16 + g8 + 8 * i].x);
+        const float b0 = top[i] == -INFINITY ? 0.f : top[i];
+#pragma unroll
+        for (int k = 0; k < C::KEY_GROUPS; ++k) {
+          const float2 st = stats[(k * R + rg) * 16 + g8 + 8 * i];
+          sum[i] += st.y * ex2_approx(st.x - b0);
+        }
+        f[i] = ex2_approx(m[i] - b0);
+        if (poisoned) sum[i] = __uint_as_float(0x7fc00000u);
+        if (pc.slot < 0) f[i] = sum[i] == 0.f ? 0.f : f[i] / sum[i];
+        if (pc.slot >= 0 && kg == 0 && t4 == 0) p.part_ml[(long long)pc.slot * ROWS + rg * 16 + g8 + 8 * i] = make_float2(top[i], sum[i]);
+      }
+      const int here = pc.rows;  // rows of the piece
+      for (int g = 0; g < min(8, here); ++g) {
+        if (g8 == g) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int d = 0; d < D / 8; ++d)
+              *reinterpret_cast<float2*>(merge + (warp * 2 + i) * D + d * 8 + t4 * 2) = make_float2(o[d][2 * i] * f[i], o[d][2 * i + 1] * f[i]);
+        }
+        if (!meet_all()) break;
+        // the warps of a row group share out its two rows
+        for (int c = kg * 32 + lane; c < D; c += C::KEY_GROUPS * 32) {
+          const int i = c / (D / 2), col = (c % (D / 2)) * 2;
+          const int r = rg * 16 + g + 8 * i;
+          if (r < here) {
+            float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < C::KEY_GROUPS; ++k) {
+              const float2 w = *reinterpret_cast<const float2*>(merge + ((k * R + rg) * 2 + i) * D + col);
+              v.x += w.x;
+              v.y += w.y;
+            }
+            if (pc.slot >= 0) {
+              *reinterpret_cast<float2*>(p.part_o + ((long long)pc.slot * ROWS + r) * D + col) = v;
+            } else {
+              const int t = (pc.row0 + r) / p.group, h = (pc.row0 + r) % p.group;
+              *reinterpret_cast<uint32_t*>(p.out + (long long)(pc.token0 + t) * p.o_st + (long long)(pc.kvh * p.group + h) * p.o_sh + col) = pack_bf16x2(v.x, v.y);
+            }
+          }
+        }
+        if (!meet_all()) break;
+      }
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(&q_empty[piece & 1]);
+      ++piece;
+    }
+  }
+  if (!ok && lane == 0 && !*abort_flag) give_up();
+}
+
+// Joins the pieces of the row tile whose keys begin in a CTA's range and end in another's: a block for each CTA, and most of them have nothing to do.
+constexpr int PA_JOIN_THREADS = 128;
+
+template <int D>
+__global__ void __launch_bounds__(PA_JOIN_THREADS)
+paged_attn_join_kernel(const PagedAttnParams p, int rows_of_slot) {
+  pa_wait_prior();
+  const int c = blockIdx.x;
+  const int4 unit = p.joins[2 * c];
+  if (unit.x < 0 || int(blockIdx.y) >= unit.z) return;
+  const int last = p.joins[2 * c + 1].x;
+  // the first piece is in slot 2c + 1, those of the CTAs behind it in their slots 2c'
+  for (int r = blockIdx.y; r < unit.z; r += gridDim.y) {
+    auto slot = [&](int i) { return (long long)(i == c ? 2 * c + 1 : 2 * i) * rows_of_slot + r; };
+    float top = -INFINITY;
+    for (int i = c; i <= last; ++i) top = fmaxf(top, p.part_ml[slot(i)].x);
+    const float b0 = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int i = c; i <= last; ++i) {
+      const float2 s = p.part_ml[slot(i)];
+      sum += s.y * ex2_approx(s.x - b0);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int t = (unit.y + r) / p.group, h = (unit.y + r) % p.group;
+    for (int col = threadIdx.x; col < D; col += PA_JOIN_THREADS) {
+      float v = 0.f;
+      for (int i = c; i <= last; ++i) v += p.part_o[slot(i) * D + col] * ex2_approx(p.part_ml[slot(i)].x - b0);
+      p.out[(long long)(unit.x + t) * p.o_st + (long long)(unit.w * p.group + h) * p.o_sh + col] = __float2bfloat16(v * inv);
+    }
+  }
+}
+
+static int pa_sms() {
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 148;
+  if (!sms[dev]) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+  return sms[dev];
+}
+
+template <int D, int R>
+static int pa_few_launch(const PagedAttnParams& p, const CUtensorMap& k, const CUtensorMap& v, int grid, bool joins, cudaStream_t stream) {
+  using C = Few<D, R>;
+  static int ready[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return TPB_ERR_CUDA;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(paged_attn_few_kernel<D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return TPB_ERR_CUDA;
+    ready[dev] = 1;
+  }
+  paged_attn_few_kernel<D, R><<<grid, C::THREADS, C::SMEM, stream>>>(k, v, p);
+  if (cudaGetLastError() != cudaSuccess) return TPB_ERR_CUDA;
+  if (!joins) return TPB_OK;
+  const dim3 join_grid(grid, min(C::ROWS, max(1, min(p.b.most_new, p.b.tokens)) * p.group));
+  return launch_dependent(paged_attn_join_kernel<D>, join_grid, dim3(PA_JOIN_THREADS), 0, stream, true, p, C::ROWS) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+}
+
+}  // namespace tpb
+
+using namespace tpb;
+
+// CTAs and workspace of a call (bytes, 16-byte aligned); see tpb_paged_attention.
+static void pa_plan(int n, int tokens, int table_width, int page_shift, int most_new, int kv_heads, int group, int head_dim, int* row_groups, int* grid, long long* floats) {
+  const long long most_rows = (long long)min(most_new, tokens) * group;
+  *row_groups = most_rows <= 16 ? 1 : most_rows <= 32 ? 2 : 4;
+  const int rows = 16 * *row_groups;
+  const long long key_tiles = (((long long)table_width << page_shift) + PA_TILE - 1) / PA_TILE;
+  const long long row_tiles = (long long)tokens * group / rows + n;  // (at most: one more than full ones per sequence)
+  const long long most = min(row_tiles, (long long)n * ((most_rows + rows - 1) / rows)) * kv_heads * key_tiles;
+  const int resident = pa_sms() * (*row_groups == 1 ? 2 : 1);
+  *grid = int(max(1LL, min((long long)resident, (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE)));
+  *floats = (long long)*grid * 2 * (rows * (head_dim + 2) + 4);
+}
+
+extern "C" long long tpb_paged_attention_workspace(int n, int tokens, int table_width, int page_size, int most_new, int kv_heads, int group, int head_dim) {
+  int row_groups, grid;
+  long long floats;
+  int shift = 0;
+  while ((1 << shift) < page_size) ++shift;
+  pa_plan(n, tokens, table_width, shift, most_new, kv_heads, group, head_dim, &row_groups, &grid, &floats);
+  return floats * 4;
+}
+
+extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
+  if (!a || !a->q || !a->out || !a->keys || !a->values || !a->table || !a->starts || !a->past || !a->status || !a->workspace) return TPB_ERR_ARG;
+  if (a->n < 0 || a->tokens <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || a->pages <= 0 || a->table_width <= 0 || a->window < 0 ||
+      a->most_new < 0)
+    return TPB_ERR_ARG;
+  if ((a->head_dim != 64 && a->head_dim != 128) || a->page_size < 16 || (a->page_size & (a->page_size - 1))) return TPB_ERR_ARG;
+  if ((long long)a->tokens * a->heads > INT_MAX / 2) return TPB_ERR_SIZE;
+  const uintptr_t addresses = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(a->keys) |
+                              reinterpret_cast<uintptr_t>(a->values) | reinterpret_cast<uintptr_t>(a->workspace);
+  if ((addresses & 15) || ((a->q_st | a->q_sh | a->o_st | a->o_sh | a->k_sp | a->k_sh | a->k_ss | a->v_sp | a->v_sh | a->v_ss) & 7)) return TPB_ERR_ALIGN;
+  int rc = fa_bind_thread();
+  if (rc != TPB_OK) return rc;
+  PagedAttnParams p = {};
+  int shift = 0;
+  while ((1 << shift) < a->page_size) ++shift;
+  p.b = {a->starts, a->past, a->table, a->table_ld, a->n, a->tokens, a->table_width, a->pages, shift, a->most_new, static_cast<uint32_t*>(a->status)};
+  p.q = static_cast<const bf16*>(a->q);
+  p.out = static_cast<bf16*>(a->out);
+  p.q_st = a->q_st, p.q_sh = a->q_sh, p.o_st = a->o_st, p.o_sh = a->o_sh;
+  p.heads = a->heads, p.kv_heads = a->kv_heads, p.group = a->heads / a->kv_heads, p.window = a->window;
+  p.fill_rest = a->fill_rest;
+  p.scale_log2e = a->scale * 1.4426950408889634f;
+  p.rows_low = 1;
+  p.rows_high = INT_MAX;
+  p.takes_bad = 1;
+  int row_groups, grid;
+  long long floats;
+  pa_plan(a->n, a->tokens, a->table_width, shift, a->most_new, p.kv_heads, p.group, a->head_dim, &row_groups, &grid, &floats);
+  if (a->workspace_bytes < floats * 4) return TPB_ERR_WORKSPACE;
+  const int rows = 16 * row_groups;
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (long long)grid * 2 * rows * a->head_dim);
+  p.joins = reinterpret_cast<int4*>(p.part_ml + (long long)grid * 2 * rows);
+  CUtensorMap k, v;
+  const int box = min(a->page_size, PA_TILE);
+  rc = paged_tmap(&k, a->keys, a->head_dim, a->page_size, a->kv_heads, a->pages, a->k_ss, a->k_sh, a->k_sp, box);
+  if (rc == TPB_OK) rc = paged_tmap(&v, a->values, a->head_dim, a->page_size, a->kv_heads, a->pages, a->v_ss, a->v_sh, a->v_sp, box);
+  if (rc != TPB_OK) return rc;
+  const bool joins = ((long long)a->table_width << shift) > PA_TILE;  // (a single tile of keys is never cut)
+  cudaStream_t s = static_cast<cudaStream_t>(stream_);
+#define PA_LAUNCH(D)                                                                                       \
+  return row_groups == 1 ? pa_few_launch<D, 1>(p, k, v, grid, joins, s)                                    \
+                         : row_groups == 2 ? pa_few_launch<D, 2>(p, k, v, grid, joins, s) : pa_few_launch<D, 4>(p, k, v, grid, joins, s)
+  if (a->head_dim == 64) PA_LAUNCH(64);
+  PA_LAUNCH(128);
+#undef PA_LAUNCH
+}

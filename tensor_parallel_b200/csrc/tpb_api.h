@@ -149,6 +149,77 @@ int tpb_rows_int8(const void* x, const void* residual, const void* weight, const
 int tpb_gemm_int8(const int8_t* x, const float* sx, const int8_t* w, const float* sw, void* out, const void* bias, const void* residual, int tokens,
                   int features, int k, long long ldx, long long ldw, long long ld_out, long long ld_res, int act, int early, void* status, void* stream);
 
+// A paged cache and the new tokens of a ragged batch (paged.cuh): keys and values [pages][kv_heads][page_size][head_dim] bf16 (element strides sp, sh, ss; head_dim
+// contiguous), table int32 [n][table_width] (row pitch table_ld), starts int32 [n + 1] and past int32 [n].  page_size a power of two from 16 up.
+// A sequence that does not fit the rows, the table or the cache, or has more than most_new new tokens: status 3.
+typedef struct {
+  const void* q;  // [tokens][heads][head_dim], strides q_st, q_sh
+  void* out;      // the same shape, strides o_st, o_sh; may be q itself
+  const void* keys;
+  const void* values;
+  const int* table;
+  const int* starts;
+  const int* past;
+  void* status;
+  void* workspace;  // tpb_paged_attention_workspace bytes, 16-byte aligned, of this call alone until it has finished
+  long long workspace_bytes;
+  long long q_st, q_sh, o_st, o_sh, k_sp, k_sh, k_ss, v_sp, v_sh, v_ss, table_ld;
+  int n, tokens, heads, kv_heads, head_dim, pages, page_size, table_width;
+  int window;     // keys that a token sees, itself the last; 0: all
+  int most_new;   // new tokens of a sequence, at most
+  int fill_rest;  // rows outside all sequences become zeros (else they stay as they are)
+  float scale;    // positive
+} tpb_paged_attn_t;
+long long tpb_paged_attention_workspace(int n, int tokens, int table_width, int page_size, int most_new, int kv_heads, int group, int head_dim);
+// out[t, h] = softmax over the keys up to t's own, window of them at most.  head_dim 64 or 128.
+int tpb_paged_attention(const tpb_paged_attn_t* args, void* stream);
+
+// New tokens into a paged cache: k, after an RMSNorm of each head (k_norm, may be null) and the rotation of its position, and v are written to the slots past[s],
+// past[s] + 1, ... of sequence s; q_out gets q, normed and rotated (may be q itself).  Rotation: pairs (i, i + rotary_dim / 2), interleaved (2i, 2i + 1),
+// by position * frequencies[i] radians, cosine and sine times `factor`; the other elements stay.  rotary_dim 0: none.
+typedef struct {
+  const void* q;  // [tokens][heads][head_dim] bf16, strides q_st, q_sh; null with q_out: nothing happens to q
+  const void* k;  // [tokens][kv_heads][head_dim]
+  const void* v;
+  void* q_out;
+  void* keys;
+  void* values;
+  const int* table;
+  const int* starts;
+  const int* past;
+  const void* q_norm;        // bf16 [head_dim] or null
+  const void* k_norm;
+  const float* frequencies;  // fp32 [rotary_dim / 2]
+  void* status;
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, k_sp, k_shead, k_ss, v_sp, v_shead, v_ss, table_ld;
+  int n, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, rotary_dim, interleaved;
+  int fill_rest;  // rows of q_out outside all sequences become zeros (else they stay as they are)
+  float factor, eps;
+} tpb_paged_append_t;
+int tpb_paged_append(const tpb_paged_append_t* args, void* stream);
+
+// Logits [rows][vocab] (bf16: dtype 0, fp32: 1) of sequences in front of the pick of a token: x of a token that is among the first `lengths` of its row's
+// tokens becomes x > 0 ? x / repetition : x * repetition; then frequency * count + presence * (count > 0) is subtracted, count being how often it is among those
+// behind the first `prompts`; bias is added; a token whose bit of `allowed` is clear becomes -inf.  Each of them may be null (per row: the number `*_all`
+// holds then).  out may be logits.
+typedef struct {
+  const void* logits;
+  void* out;
+  const long long* tokens;  // [rows][width], pitch tokens_ld; tokens outside [0, vocab) do not count
+  const int* lengths;       // [rows], null: width
+  const int* prompts;       // [rows], null: 0
+  const float* repetition;  // [rows]
+  const float* frequency;
+  const float* presence;
+  const void* bias;         // [vocab] (bias_ld 0) or [rows][vocab], bf16 (bias_dtype 0) or fp32 (1)
+  const int* allowed;       // [rows][words], bit i of word w: token 32 w + i; pitch allowed_ld (0: one row for all)
+  void* status;
+  long long logits_ld, out_ld, tokens_ld, bias_ld, allowed_ld;
+  int rows, vocab, width, dtype, bias_dtype;
+  float repetition_all, frequency_all, presence_all;
+} tpb_adjust_logits_t;
+int tpb_adjust_logits(const tpb_adjust_logits_t* args, void* stream);
+
 // Sizes of the structures above as this library was built, one byte-count per 16 bits (plan, reduction context, options), and the version of the
 // signatures that are called from elsewhere (1: tpb_rows_int8 takes `ahead`), for callers that are built apart from it.
 #define TPB_API_LAYOUT \

@@ -190,6 +190,162 @@ def linear_int8_ref(x: Int8Rows, weight: Int8Rows, bias=None, act: Optional[str]
     return v.to(torch.bfloat16)
 
 
+class PagedCache(NamedTuple):
+    """Keys and values of sequences of different lengths, ``[pages, kv_heads, page_size, head_dim]`` each, and the pages of every sequence, int32
+    ``[sequences, most pages of one]``: key ``j`` of sequence ``s`` is slot ``j % page_size`` of page ``table[s, j // page_size]``.  Pages may be in any order and
+    belong to several sequences (a common prefix); entries beyond a sequence's keys are not read.  Keys and values may be strided views (the layers
+    of one tensor, keys and values side by side, heads inside of slots)."""
+
+    keys: torch.Tensor
+    values: torch.Tensor
+    table: torch.Tensor
+
+
+class Rotary(NamedTuple):
+    """A position rotation: the pairs of the first ``2 * len(frequencies)`` elements of a head are turned by ``position * frequencies[i]`` radians and multiplied
+    by ``factor``.  Pairs are ``(2i, 2i + 1)`` if ``interleaved`` (GPT-J / CodeGen), else ``(i, i + len(frequencies))`` (Llama / NeoX / Falcon)."""
+
+    frequencies: torch.Tensor  # fp32 [rotary_dim / 2]
+    interleaved: bool = False
+    factor: float = 1.0
+
+
+def rotary(rotary_dim: int, theta: float = 10000.0, interleaved: bool = False, scaling: Optional[dict] = None, device=None) -> Rotary:
+    """The usual frequencies ``theta ** (-2i / rotary_dim)``, for contexts longer than a model was trained on scaled as ``scaling`` says (the dictionary of
+    a Hugging Face configuration): ``"linear"`` (all slower by ``factor``), ``"llama3"`` (slow ones slower by ``factor``, a ramp between) or ``"yarn"`` (a ramp over the
+    pairs, and a factor on cosine and sine)."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"a rotation takes an even number of elements, got {rotary_dim}")
+    f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    kind, factor = "default", 1.0
+    if scaling:
+        kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "linear":
+        f = f / scaling["factor"]
+    elif kind == "llama3":
+        low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
+        turns = scaling["original_max_position_embeddings"] * f / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        f = f * keep + f / scaling["factor"] * (1 - keep)
+    elif kind == "yarn":
+        def pair(turns):  # the pair that makes so many turns over the original context
+            return rotary_dim * math.log(scaling["original_max_position_embeddings"] / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        low, high = max(math.floor(pair(scaling.get("beta_fast", 32))), 0), min(math.ceil(pair(scaling.get("beta_slow", 1))), rotary_dim - 1)
+        slow = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+        f = f * (1 - slow) + f / scaling["factor"] * slow
+        factor = scaling.get("attention_factor") or (0.1 * math.log(scaling["factor"]) + 1.0 if scaling["factor"] > 1 else 1.0)
+    elif kind != "default":
+        raise ValueError(f"scaling of rotary frequencies: 'linear', 'llama3' or 'yarn', got {kind!r}")
+    return Rotary(f.float().to(device), interleaved, factor)
+
+
+def _spans(what: str, cache: PagedCache, tokens: int, starts, past, most_new: Optional[int] = None):
+    """``(start, new, past)`` of every sequence, from the device; what the kernels answer with NaN and a status is an error here."""
+    bounds, cached = starts.tolist(), past.tolist()
+    room = cache.table.shape[1] * cache.keys.shape[2]
+    spans = []
+    for s, p in enumerate(cached):
+        a, e = bounds[s], bounds[s + 1]
+        if not 0 <= a <= e <= tokens or p < 0 or (e > a and p + e - a > room) or (most_new is not None and e - a > most_new):
+            raise ValueError(f"{what}: sequence {s} has rows {a} to {e} of {tokens} behind {p} cached keys; its table has room for {room}"
+                             + ("" if most_new is None else f", most_new is {most_new}"))
+        spans.append((a, e - a, p))
+    return spans
+
+
+def _pages_of(what: str, cache: PagedCache, s: int, first: int, last: int):
+    pages = cache.table[s, first:last + 1].long()
+    if pages.numel() and not 0 <= int(pages.min()) <= int(pages.max()) < cache.keys.shape[0]:
+        raise ValueError(f"{what}: pages {pages.tolist()} of sequence {s} are not all among the {cache.keys.shape[0]} of the cache")
+    return pages
+
+
+def _normed_and_turned(x, weight, eps: float, positions, turn: Optional[Rotary]):
+    h = x.float()
+    if weight is not None:
+        h = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps) * weight.float()
+    if turn is not None:
+        half = turn.frequencies.shape[0]
+        angles = positions.double()[:, None] * turn.frequencies.double()  # (in 32 bits, far positions are off by hundredths of a radian)
+        c, s = ((fn(angles) * turn.factor).float()[:, None] for fn in (torch.cos, torch.sin))
+        rot, keep = h[..., :2 * half], h[..., 2 * half:]
+        if turn.interleaved:
+            a, b = rot[..., 0::2], rot[..., 1::2]
+            rot = torch.stack((a * c - b * s, b * c + a * s), dim=-1).flatten(-2)
+        else:
+            a, b = rot[..., :half], rot[..., half:]
+            rot = torch.cat((a * c - b * s, b * c + a * s), dim=-1)
+        h = torch.cat((rot, keep), dim=-1)
+    return h.to(x.dtype)
+
+
+def paged_append_ref(cache: PagedCache, q, k, v, starts, past, rotary=None, q_norm=None, k_norm=None, eps: float = 1e-6, out=None):
+    spans = _spans("paged_append", cache, k.shape[0], starts, past)
+    page = cache.keys.shape[2]
+    places = [_pages_of("paged_append", cache, s, p // page, (p + new - 1) // page) if new else None for s, (_, new, p) in enumerate(spans)]
+    given = out
+    if q is not None and (rotary is not None or q_norm is not None or out is not None):
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    for (start, new, p), pages in zip(spans, places):
+        if not new:
+            continue
+        at = torch.arange(p, p + new, device=k.device)
+        rows = slice(start, start + new)
+        into = pages[at // page - p // page]
+        cache.keys[into, :, at % page] = _normed_and_turned(k[rows], k_norm, eps, at, rotary)
+        cache.values[into, :, at % page] = v[rows]
+        if out is not None:
+            out[rows] = _normed_and_turned(q[rows], q_norm, eps, at, rotary)
+    return q if out is None and given is None else out
+
+
+def paged_attention_ref(q, cache: PagedCache, starts, past, scale: Optional[float] = None, window: Optional[int] = None, most_new: Optional[int] = None, out=None):
+    spans = _spans("paged_attention", cache, q.shape[0], starts, past, most_new)
+    page = cache.keys.shape[2]
+    result = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    for s, (start, new, p) in enumerate(spans):
+        if not new:
+            continue
+        total = p + new
+        first = 0 if window is None else max(0, p - window + 1)  # the first key that a token sees
+        pages = _pages_of("paged_attention", cache, s, first // page, (total - 1) // page)
+        k, v = (t[pages].transpose(1, 2).flatten(0, 1)[first - first // page * page:][:total - first] for t in (cache.keys, cache.values))
+        at, key = torch.arange(p, total, device=q.device)[:, None], torch.arange(first, total, device=q.device)[None]
+        hidden = key > at if window is None else (key > at) | (key <= at - window)
+        bias = torch.zeros(new, total - first, device=q.device).masked_fill_(hidden, float("-inf"))
+        result[start:start + new] = attention_ref(q[None, start:start + new], k[None], v[None], False, bias, scale)[0]
+    return result
+
+
+def adjust_logits_ref(logits, tokens=None, lengths=None, prompt_lengths=None, repetition=None, frequency=None, presence=None, bias=None, allowed=None):
+    x = logits.float()
+    rows, vocab = logits.shape
+
+    def per_row(value, neutral):
+        return neutral if value is None else value[:, None] if isinstance(value, torch.Tensor) else value
+
+    if tokens is not None:
+        at = torch.arange(tokens.shape[1], device=tokens.device)[None]
+        there = (tokens >= 0) & (tokens < vocab)
+        if lengths is not None:
+            there = there & (at < lengths[:, None])
+        said = there if prompt_lengths is None else there & (at >= prompt_lengths[:, None])
+        index = tokens.clamp(0, max(vocab - 1, 0))
+        seen = torch.zeros(rows, vocab, dtype=torch.int32, device=logits.device).scatter_add(1, index, there.int()) > 0
+        count = torch.zeros(rows, vocab, dtype=torch.int32, device=logits.device).scatter_add(1, index, said.int())
+        r = per_row(repetition, 1.0)
+        x = torch.where(seen, torch.where(x > 0, x / r, x * r), x)
+        x = torch.where(count > 0, x - (per_row(frequency, 0.0) * count.float() + per_row(presence, 0.0)), x)
+    if bias is not None:
+        x = x + bias.float()
+    if allowed is not None:
+        token = torch.arange(vocab, device=logits.device)
+        bits = allowed[..., token // 32] >> (token % 32).int() & 1
+        x = x.masked_fill(bits == 0, float("-inf"))
+    return x.to(logits.dtype)
+
+
 # -- dispatching front-end ---------------------------------------------------------------------
 
 
@@ -422,6 +578,170 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias=None, act: Optional[str] = N
     if nat is None or transformed(x[0]) or transformed(x[1]):
         return linear_int8_ref(Int8Rows(*x), Int8Rows(*weight), bias, act, residual)
     return nat.linear_int8(x, weight, bias, act, residual)
+
+
+# -- sequences of different lengths (serving) ------------------------------------------------------
+
+
+def _not_captured(what: str):
+    """A kernel would leave nothing in a captured graph, and the steps depend on lengths that are on the device."""
+    if (torch._C._functorch.peek_interpreter_stack() is not None or torch.jit.is_tracing()
+            or torch._C._dispatch_tls_is_dispatch_key_included(_AHEAD_OF_DISPATCH) or _capturing_modes()):
+        raise RuntimeError(f"{what} reads lengths on the device: it cannot be traced, captured as operators or transformed (CUDA graphs are fine)")
+
+
+def _capturing_modes() -> bool:
+    modes = torch._C._TorchDispatchModeKey
+    return torch._C._len_torch_dispatch_stack() > 0 and any(torch._C._get_dispatch_mode(key) is not None for key in (modes.PROXY, modes.FAKE, modes.FUNCTIONAL))
+
+
+def _check_paged(what: str, cache, starts, past, rows):
+    """``rows``: name -> ``[tokens, heads, head_dim]``."""
+    keys, values, table = cache
+    if keys.ndim != 4 or values.shape != keys.shape or values.dtype != keys.dtype or not keys.is_floating_point():
+        raise ValueError(f"{what}: keys and values have to be [pages, kv_heads, page_size, head_dim] of one type, got {keys.dtype} {tuple(keys.shape)} and "
+                         f"{values.dtype} {tuple(values.shape)}")
+    for name, t, shape in (("the table", table, (None, None)), ("starts", starts, (None,)), ("past", past, (None,))):
+        if t.dtype != torch.int32 or t.ndim != len(shape):
+            raise ValueError(f"{what}: {name} has to be int32 with {len(shape)} dimension{'s' * (len(shape) > 1)}, got {t.dtype} {tuple(t.shape)}")
+    n = past.shape[0]
+    if starts.shape[0] != n + 1 or table.shape[0] != n:
+        raise ValueError(f"{what}: {n} cached lengths go with {n + 1} starts and {n} rows of the table, got {starts.shape[0]} and {table.shape[0]}")
+    tokens = None
+    for name, t in rows.items():
+        if t is None:
+            continue
+        if t.ndim != 3 or t.dtype != keys.dtype or t.shape[2] != keys.shape[3] or (tokens is not None and t.shape[0] != tokens):
+            raise ValueError(f"{what}: {name} has to be [tokens, heads, {keys.shape[3]}] in {keys.dtype}, got {t.dtype} {tuple(t.shape)}")
+        tokens = t.shape[0]
+    for t in (values, table, starts, past, *rows.values()):
+        if t is not None and t.device != keys.device:
+            raise ValueError(f"{what}: all tensors have to be on {keys.device}, got one on {t.device}")
+    if tokens and n and (0 in keys.shape or table.shape[1] == 0):
+        raise ValueError(f"{what}: a cache of {tuple(keys.shape)} with a table of {tuple(table.shape)} has no place for {tokens} tokens")
+
+
+def _check_out(what: str, out, like):
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise ValueError(f"{what}: out has to be like q ({tuple(like.shape)}, {like.dtype}, {like.device}, no element twice), got {tuple(out.shape)}, {out.dtype}, {out.device}")
+
+
+def paged_append(cache: PagedCache, q, k, v, starts, past, rotary: Optional[Rotary] = None, q_norm=None, k_norm=None, eps: float = 1e-6, out=None):
+    """Writes the new keys and values of a ragged batch to a paged cache and returns its queries; keys and queries are normed and rotated on the way.
+
+    ``k`` and ``v`` are ``[tokens, kv_heads, head_dim]`` and ``q`` ``[tokens, heads, head_dim]`` (strided views of one projection are fine; ``q`` may be None): rows
+    ``starts[s]`` to ``starts[s + 1]`` belong to sequence ``s``, and follow its ``past[s]`` keys in the cache (int32, ``[sequences + 1]`` and ``[sequences]``).  ``q_norm`` and
+    ``k_norm``, ``[head_dim]``, ask for an RMSNorm of each head, ``rotary`` for the rotation by the token's position (its index in the sequence) behind it.
+    Angles are exact at any position; results are rounded once.
+
+    The queries come in a tensor of their own, in ``out`` (which may be ``q``), or as they are where nothing is done to them.  Rows in front of the first
+    sequence and behind the last (a batch padded to a captured size) are not stored; ``out`` keeps what it has there, and a new tensor holds zeros.
+    A sequence whose rows, table or pages do not fit is not stored: the CUDA kernel records status 3 (see ``native.device_state``), the steps over
+    tensors raise.  Two tokens for one slot (sequences that share the page that they write to) leave either.  Serving only: there is no gradient."""
+    if _compiling():
+        torch._dynamo.graph_break()
+    _check_paged("paged_append", cache, starts, past, dict(q=q, k=k, v=v))
+    d, kv_heads = cache[0].shape[3], cache[0].shape[1]
+    if k.shape[1] != kv_heads or v.shape[1] != kv_heads:
+        raise ValueError(f"paged_append: the cache has {kv_heads} heads, got keys {tuple(k.shape)} and values {tuple(v.shape)}")
+    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if t is not None and (t.shape != (d,) or t.dtype != k.dtype or t.device != k.device):
+            raise ValueError(f"paged_append: {name} has to be {k.dtype} [{d}] on {k.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if rotary is not None:
+        f = rotary[0]
+        if f.dtype != torch.float32 or f.ndim != 1 or f.device != k.device or not 0 < 2 * f.shape[0] <= d:
+            raise ValueError(f"paged_append: frequencies have to be fp32 on {k.device}, 1 to {d // 2} of them, got {f.dtype} {tuple(f.shape)} on {f.device}")
+    if out is not None:
+        if q is None:
+            raise ValueError("paged_append: out is for queries, and there are none")
+        _check_out("paged_append", out, q)
+    _serving_only("paged_append", cache[0], cache[1], q, k, v, q_norm, k_norm, out)
+    _not_captured("paged_append")
+    nat = _native(k)
+    if nat is not None and nat.paged_append_supported(cache, q, k, out):
+        return nat.paged_append(cache, q, k, v, starts, past, rotary, q_norm, k_norm, eps, out)
+    return paged_append_ref(PagedCache(*cache), q, k, v, starts, past, None if rotary is None else Rotary(*rotary), q_norm, k_norm, eps, out)
+
+
+def paged_attention(q, cache: PagedCache, starts, past, scale: Optional[float] = None, window: Optional[int] = None, most_new: Optional[int] = None, out=None):
+    """Causal attention of the new tokens of a ragged batch over a paged cache that holds their own keys and values already (:func:`paged_append`).
+
+    ``q`` is ``[tokens, heads, head_dim]``; ``starts`` and ``past`` as for :func:`paged_append`, ``past`` not counting the new tokens: row ``starts[s] + i`` sees keys ``0`` to
+    ``past[s] + i`` of sequence ``s``, or the last ``window`` of them.  One token of each sequence is a decode step, a whole prompt is a prefill, and
+    sequences of both kinds may be in one batch.  ``most_new`` says how many new tokens any sequence has at most, where the caller knows (the launch is
+    chosen by it).  What lies in the cache outside of a token's keys has no influence, whatever it is; pages that have left the window are not read.
+
+    The result is a new tensor, zero in rows outside all sequences, or ``out`` (which may be ``q``), left as it is there.  A sequence whose rows, table or
+    pages do not fit, or with more than ``most_new`` new tokens, gives NaN, and the CUDA kernel records status 3 (see ``native.device_state``); the steps over tensors
+    raise.  Serving only: there is no gradient."""
+    if _compiling():
+        torch._dynamo.graph_break()
+    _check_paged("paged_attention", cache, starts, past, dict(q=q))
+    if q.shape[1] == 0 or cache[0].shape[1] == 0 or q.shape[1] % cache[0].shape[1]:
+        raise ValueError(f"paged_attention: {q.shape[1]} query heads are no multiple of {cache[0].shape[1]} in the cache")
+    if window is not None and window < 1:
+        raise ValueError(f"paged_attention: a window holds at least the token itself, got {window}")
+    if most_new is not None and most_new < 0:
+        raise ValueError(f"paged_attention: most_new={most_new}")
+    if scale is not None and not 0 < scale < math.inf:
+        raise ValueError(f"paged_attention: the scale has to be positive, got {scale}")
+    if out is not None:
+        _check_out("paged_attention", out, q)
+    _serving_only("paged_attention", q, cache[0], cache[1], out)
+    _not_captured("paged_attention")
+    nat = _native(q)
+    if nat is not None and nat.paged_attention_supported(q, cache, out):
+        return nat.paged_attention(q, cache, starts, past, scale, window, most_new, out)
+    return paged_attention_ref(q, PagedCache(*cache), starts, past, scale, window, most_new, out)
+
+
+def _check_adjust(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed):
+    what = "adjust_logits"
+    if logits.ndim != 2 or not logits.is_floating_point():
+        raise ValueError(f"{what} takes logits [rows, vocabulary], got {logits.dtype} {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    if tokens is None and any(t is not None for t in (lengths, prompt_lengths, repetition, frequency, presence)):
+        raise ValueError(f"{what}: lengths and penalties are for the tokens that a sequence has had, and none are given")
+    if tokens is not None and (tokens.dtype != torch.int64 or tokens.ndim != 2 or tokens.shape[0] != rows):
+        raise ValueError(f"{what}: tokens have to be int64 [{rows}, width], got {tokens.dtype} {tuple(tokens.shape)}")
+    for name, t in (("lengths", lengths), ("prompt_lengths", prompt_lengths)):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (rows,)):
+            raise ValueError(f"{what}: {name} have to be int32 [{rows}], got {t.dtype} {tuple(t.shape)}")
+    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+        if isinstance(t, torch.Tensor):
+            if t.dtype != torch.float32 or t.shape != (rows,):
+                raise ValueError(f"{what}: {name} has to be a number or fp32 [{rows}], got {t.dtype} {tuple(t.shape)}")
+        elif name == "repetition" and t is not None and not t > 0:
+            raise ValueError(f"{what}: logits are divided by repetition, which has to be positive, got {t}")
+    if bias is not None and (bias.shape not in ((vocab,), (rows, vocab)) or bias.dtype not in (torch.bfloat16, torch.float32)):
+        raise ValueError(f"{what}: the bias has to be bf16 or fp32 [{vocab}] or [{rows}, {vocab}], got {bias.dtype} {tuple(bias.shape)}")
+    words = (vocab + 31) // 32
+    if allowed is not None and (allowed.shape not in ((words,), (rows, words)) or allowed.dtype != torch.int32):
+        raise ValueError(f"{what}: allowed tokens are bits of int32 [{words}] or [{rows}, {words}], got {allowed.dtype} {tuple(allowed.shape)}")
+    for t in (tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed):
+        if isinstance(t, torch.Tensor) and t.device != logits.device:
+            raise ValueError(f"{what}: all tensors have to be on {logits.device}, got one on {t.device}")
+    _serving_only(what, *(t if isinstance(t, torch.Tensor) else None for t in (logits, repetition, frequency, presence, bias)))
+
+
+def adjust_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repetition=None, frequency=None, presence=None, bias=None, allowed=None):
+    """Logits ``[rows, vocabulary]`` as they go into the pick of a token, in their own type (32 bits on the way), in this order:
+
+    * penalties for the tokens that a row has had, the first ``lengths[row]`` (None: all) of ``tokens[row]`` (int64 ``[rows, width]``; ids outside the vocabulary do not
+      count): a positive logit is divided by ``repetition`` and another multiplied by it; for those behind the first ``prompt_lengths[row]`` (None: 0), how often
+      one was said times ``frequency``, and ``presence`` once, are subtracted.  Each is None, a number, or fp32 ``[rows]``.
+    * ``bias``, fp32 or bf16, ``[vocabulary]`` or ``[rows, vocabulary]``, is added;
+    * tokens that ``allowed`` does not name become ``-inf``: bit ``i`` of word ``w`` stands for token ``32 w + i`` (int32 ``[words]`` or ``[rows, words]``).
+
+    Lengths beyond the width count as the width, below zero as zero (the CUDA kernel records status 3).  Serving only: there is no gradient."""
+    if not _compiling():
+        nat = _native(logits)
+        _check_adjust(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed)
+        if nat is not None and nat.adjust_logits_supported(logits) and not transformed(logits):
+            return nat.adjust_logits(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed)
+    else:
+        _check_adjust(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed)
+    return adjust_logits_ref(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed)
 
 
 def cross_entropy(logits, labels, ignore_index: int = -100):

@@ -870,6 +870,160 @@ def qkv_rope_append(q, k, v, q_out, kcache, vcache, base_pos, batch, seq, rotary
     _launches += 1
     return q_out
 
+# ------------------------------------------------------------------------------------------------
+# sequences of different lengths: paged cache, its attention, logits
+# ------------------------------------------------------------------------------------------------
+
+
+class PagedAttn(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("q", "out", "keys", "values", "table", "starts", "past", "status", "workspace")] + [("workspace_bytes", c_ll)]
+                + [(n, c_ll) for n in ("q_st", "q_sh", "o_st", "o_sh", "k_sp", "k_sh", "k_ss", "v_sp", "v_sh", "v_ss", "table_ld")]
+                + [(n, c_int) for n in ("n", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_size", "table_width", "window", "most_new", "fill_rest")]
+                + [("scale", c_float)])
+
+
+class PagedAppend(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "q_out", "keys", "values", "table", "starts", "past", "q_norm", "k_norm", "frequencies", "status")]
+                + [(n, c_ll) for n in ("q_st", "q_sh", "k_st", "k_sh", "v_st", "v_sh", "o_st", "o_sh", "k_sp", "k_shead", "k_ss", "v_sp", "v_shead", "v_ss", "table_ld")]
+                + [(n, c_int) for n in ("n", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_size", "table_width", "rotary_dim", "interleaved", "fill_rest")]
+                + [("factor", c_float), ("eps", c_float)])
+
+
+class AdjustLogits(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("logits", "out", "tokens", "lengths", "prompts", "repetition", "frequency", "presence", "bias", "allowed", "status")]
+                + [(n, c_ll) for n in ("logits_ld", "out_ld", "tokens_ld", "bias_ld", "allowed_ld")]
+                + [(n, c_int) for n in ("rows", "vocab", "width", "dtype", "bias_dtype")]
+                + [(n, c_float) for n in ("repetition_all", "frequency_all", "presence_all")])
+
+
+LIB.tpb_paged_attention_workspace.argtypes = [c_int] * 8
+LIB.tpb_paged_attention_workspace.restype = c_ll
+LIB.tpb_paged_attention.argtypes = [ctypes.POINTER(PagedAttn), c_void_p]
+LIB.tpb_paged_append.argtypes = [ctypes.POINTER(PagedAppend), c_void_p]
+LIB.tpb_adjust_logits.argtypes = [ctypes.POINTER(AdjustLogits), c_void_p]
+
+
+def _vector_rows(t: torch.Tensor) -> bool:
+    """Elements of a row together, and every row on a 16-byte boundary."""
+    return t.stride(-1) == 1 and not any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1) and t.data_ptr() % 16 == 0
+
+
+def _in_vectors(t: Optional[torch.Tensor]):
+    """``t``, or a copy that vectors can read (``contiguous()`` would leave a tensor that starts off a boundary as it is)."""
+    return t if t is None or _vector_rows(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t: torch.Tensor, dims: int):
+    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(dims))  # (a dimension of one may come with any stride)
+
+
+def _pages_supported(cache) -> bool:
+    keys, values, _ = cache
+    return (keys.dtype == torch.bfloat16 and keys.numel() > 0 and _vector_rows(keys) and _vector_rows(values)
+            and all(s > 0 for t in (keys, values) for s, n in zip(t.stride(), t.shape) if n > 1))
+
+
+def paged_append_supported(cache, q, k, out) -> bool:
+    page, d = cache[0].shape[2:]
+    return _pages_supported(cache) and page & (page - 1) == 0 and d % 8 == 0 and d <= 256 and k.shape[0] > 0 and cache[2].numel() > 0 and (out is None or _vector_rows(out))
+
+
+def paged_append(cache, q, k, v, starts, past, rotary, q_norm, k_norm, eps, out):
+    global _launches
+    keys, values, table = cache
+    with torch.cuda.device(keys.device):
+        given, kept = out, q
+        if q is not None and (rotary is not None or q_norm is not None or out is not None):
+            q = _in_vectors(q)
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        else:
+            q = None
+        k, v, q_norm, k_norm = (_in_vectors(t) for t in (k, v, q_norm, k_norm))
+        starts, past, table = starts.contiguous(), past.contiguous(), table if table.stride(1) == 1 or table.shape[1] == 1 else table.contiguous()
+        a = PagedAppend(q=_ptr(q), k=_ptr(k), v=_ptr(v), q_out=None if q is None else _ptr(out), keys=_ptr(keys), values=_ptr(values), table=_ptr(table), starts=_ptr(starts),
+                        past=_ptr(past), q_norm=_ptr(q_norm), k_norm=_ptr(k_norm), status=_ptr(device_state(keys.device).status), table_ld=table.stride(0),
+                        n=past.shape[0], tokens=k.shape[0], heads=0 if q is None else q.shape[1], kv_heads=k.shape[1], head_dim=k.shape[2], pages=keys.shape[0],
+                        page_size=keys.shape[2], table_width=table.shape[1], fill_rest=int(given is None), factor=1.0, eps=eps)
+        if rotary is not None:
+            f = rotary[0].contiguous()
+            a.frequencies, a.rotary_dim, a.interleaved, a.factor = _ptr(f), 2 * f.shape[0], int(bool(rotary[1])), float(rotary[2])
+        if q is not None:
+            a.q_st, a.q_sh = _strides(q, 2)
+            a.o_st, a.o_sh = _strides(out, 2)
+        (a.k_st, a.k_sh), (a.v_st, a.v_sh) = _strides(k, 2), _strides(v, 2)
+        (a.k_sp, a.k_shead, a.k_ss), (a.v_sp, a.v_shead, a.v_ss) = _strides(keys, 3), _strides(values, 3)
+        check(LIB.tpb_paged_append(ctypes.byref(a), _stream()), "tpb_paged_append")
+    _launches += 1
+    return kept if q is None else out
+
+
+def paged_attention_supported(q, cache, out) -> bool:
+    page, d = cache[0].shape[2:]
+    return (_pages_supported(cache) and page >= 16 and page & (page - 1) == 0 and d in (64, 128) and q.numel() > 0 and cache[2].numel() > 0
+            and (out is None or _vector_rows(out)))
+
+
+def paged_attention(q, cache, starts, past, scale, window, most_new, out):
+    global _launches
+    keys, values, table = cache
+    tokens, heads, d = q.shape
+    n, kv_heads, page, width = past.shape[0], keys.shape[1], keys.shape[2], table.shape[1]
+    with torch.cuda.device(keys.device):
+        q, given = _in_vectors(q), out
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        starts, past, table = starts.contiguous(), past.contiguous(), table if table.stride(1) == 1 or width == 1 else table.contiguous()
+        most = tokens if most_new is None else min(most_new, tokens)
+        need = LIB.tpb_paged_attention_workspace(n, tokens, width, page, most, kv_heads, heads // kv_heads, d)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a = PagedAttn(q=_ptr(q), out=_ptr(out), keys=_ptr(keys), values=_ptr(values), table=_ptr(table), starts=_ptr(starts), past=_ptr(past),
+                      status=_ptr(device_state(q.device).status), workspace=_ptr(workspace), workspace_bytes=need, table_ld=table.stride(0), n=n, tokens=tokens,
+                      heads=heads, kv_heads=kv_heads, head_dim=d, pages=keys.shape[0], page_size=page, table_width=width, window=min(window or 0, 2 ** 30),
+                      most_new=most, fill_rest=int(given is None), scale=1.0 / math.sqrt(d) if scale is None else scale)
+        (a.q_st, a.q_sh), (a.o_st, a.o_sh) = _strides(q, 2), _strides(out, 2)
+        (a.k_sp, a.k_sh, a.k_ss), (a.v_sp, a.v_sh, a.v_ss) = _strides(keys, 3), _strides(values, 3)
+        check(LIB.tpb_paged_attention(ctypes.byref(a), _stream()), "tpb_paged_attention")
+    _launches += 2
+    return out
+
+
+def adjust_logits_supported(logits) -> bool:
+    return logits.dtype in (torch.bfloat16, torch.float32) and logits.numel() > 0
+
+
+def adjust_logits(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed):
+    global _launches
+    rows, vocab = logits.shape
+    with torch.cuda.device(logits.device):
+        x = logits if logits.stride(1) == 1 or vocab == 1 else logits.contiguous()
+        out = torch.empty(rows, vocab, dtype=x.dtype, device=x.device)
+        a = AdjustLogits(logits=_ptr(x), out=_ptr(out), status=_ptr(device_state(x.device).status), logits_ld=x.stride(0), out_ld=vocab, rows=rows, vocab=vocab,
+                         dtype=_dtype_code(x), repetition_all=1.0)
+        held = []  # (copies live until the launch)
+
+        def dense(t, dims=1):
+            t = t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+            held.append(t)
+            return t
+
+        if tokens is not None and tokens.shape[1] > 0:
+            t = dense(tokens)
+            a.tokens, a.tokens_ld, a.width = _ptr(t), t.stride(0), t.shape[1]
+            a.lengths, a.prompts = (None if t is None else _ptr(dense(t)) for t in (lengths, prompt_lengths))
+            for name, value in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+                if isinstance(value, torch.Tensor):
+                    setattr(a, name, _ptr(dense(value)))
+                elif value is not None:
+                    setattr(a, name + "_all", float(value))
+        if bias is not None:
+            t = dense(bias)
+            a.bias, a.bias_ld, a.bias_dtype = _ptr(t), t.stride(0) if t.ndim == 2 else 0, _dtype_code(t)
+        if allowed is not None:
+            t = dense(allowed)
+            a.allowed, a.allowed_ld = _ptr(t), t.stride(0) if t.ndim == 2 else 0
+        check(LIB.tpb_adjust_logits(ctypes.byref(a), _stream()), "tpb_adjust_logits")
+    _launches += 1
+    return out
+
 
 LIB.tpb_relative_bias.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]
 LIB.tpb_relative_bias_bwd.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]
