@@ -1,5 +1,5 @@
 // Autograd nodes of the layers whose training calls are bound by the host at ordinary sizes: linear and norms.  And, without nodes, the calls of
-// 8-bit serving, whose kernels take a few microseconds each at decode sizes.
+// 8-bit serving and of ragged batches, whose kernels take a few microseconds each at decode sizes.
 //
 // A small call (100 tokens through a 768 x 3072 projection with bias, forward and backward) keeps the GPU busy for 37 us.  As Python
 // autograd functions over ctypes it took 176 us: each of its launches cost 10 to 20 us of interpreter work, and the backward nodes
@@ -20,7 +20,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <stdexcept>
 #include <string>
 
@@ -41,6 +43,10 @@ struct Library {
   decltype(&tpb_col_sum) col_sum = nullptr;
   decltype(&tpb_rows_int8) rows_int8 = nullptr;
   decltype(&tpb_gemm_int8) gemm_int8 = nullptr;
+  decltype(&tpb_paged_attention_workspace) paged_attention_workspace = nullptr;
+  decltype(&tpb_paged_attention) paged_attention = nullptr;
+  decltype(&tpb_paged_append) paged_append = nullptr;
+  decltype(&tpb_adjust_logits) adjust_logits = nullptr;
 };
 Library lib;
 PyObject* error_text = nullptr;     // (code, what) -> message
@@ -389,6 +395,167 @@ Tensor linear_int8(const Tensor& x, const Tensor& sx, const Tensor& w, const Ten
   return out;
 }
 
+// ---- sequences of different lengths ----
+// As the 8-bit calls: the ordinary ones are taken here, every other goes on in Python.
+
+bool ints(const Tensor& t, int64_t dims, const c10::Device& device) {
+  return plain(t, at::kInt, device) && t.dim() == dims && (t.stride(dims - 1) == 1 || t.size(dims - 1) <= 1);
+}
+// bf16 with the last dimension together and every row on a 16-byte boundary.
+bool vectors(const Tensor& t, int64_t dims, const c10::Device& device) {
+  if (!plain(t, at::kBFloat16, device) || t.dim() != dims || t.stride(dims - 1) != 1 || reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16) return false;
+  for (int64_t d = 0; d + 1 < dims; ++d)
+    if (t.size(d) > 1 && t.stride(d) % 8) return false;
+  return true;
+}
+long long step(const Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+struct Pages {
+  const Tensor *keys, *values, *table, *starts, *past;
+  int64_t n() const { return past->size(0); }
+};
+bool pages_fit(const Pages& p, int64_t least_page) {
+  const Tensor& k = *p.keys;
+  const auto device = k.device();
+  if (!k.is_cuda() || !vectors(k, 4, device) || !vectors(*p.values, 4, device) || k.sizes() != p.values->sizes() || k.numel() == 0) return false;
+  for (int64_t d = 0; d < 3; ++d)
+    if (k.size(d) > 1 && (k.stride(d) <= 0 || p.values->stride(d) <= 0)) return false;
+  const int64_t page = k.size(2), limit = int64_t(1) << 31;
+  return page >= least_page && (page & (page - 1)) == 0 && page < limit && k.size(0) < limit && ints(*p.table, 2, device) && ints(*p.starts, 1, device) &&
+         ints(*p.past, 1, device) && p.starts->size(0) == p.n() + 1 && p.table->size(0) == p.n() && p.n() > 0 && p.n() < limit - 1 && p.table->size(1) > 0 &&
+         p.table->size(1) < limit;
+}
+bool rows_like(const Tensor& t, int64_t heads, const Pages& p, int64_t tokens) {
+  return vectors(t, 3, p.keys->device()) && t.size(2) == p.keys->size(3) && t.size(0) == tokens && (heads < 0 || t.size(1) == heads);
+}
+bool written_once(const Tensor& t) {
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) == 0) return false;
+  return true;
+}
+
+// scale 0: the usual one.  The result, or no tensor.
+Tensor paged_attention(const Tensor& q, const Pages& p, double scale, int64_t window, int64_t most_new, const Tensor& given) {
+  if (!lib.paged_attention || interposed() || !pages_fit(p, 16) || q.dim() != 3) return {};
+  const int64_t tokens = q.size(0), heads = q.size(1), dim = q.size(2), kv_heads = p.keys->size(1);
+  if ((dim != 64 && dim != 128) || tokens <= 0 || heads <= 0 || heads % kv_heads || tokens * heads >= (int64_t(1) << 30) || !rows_like(q, -1, p, tokens)) return {};
+  if (given.defined() && (!rows_like(given, heads, p, tokens) || !written_once(given))) return {};
+  const py::gil_scoped_release unlocked;
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = given.defined() ? given : room_for(q.sizes(), at::kBFloat16);
+  tpb_paged_attn_t a = {};
+  const int64_t most = most_new < 0 ? tokens : std::min(most_new, tokens);
+  a.workspace_bytes = lib.paged_attention_workspace(int(p.n()), int(tokens), int(p.table->size(1)), int(p.keys->size(2)), int(most), int(kv_heads),
+                                                    int(heads / kv_heads), int(dim));
+  const Tensor workspace = room_for({a.workspace_bytes}, at::kByte);
+  a.q = q.const_data_ptr(), a.out = out.mutable_data_ptr(), a.keys = p.keys->const_data_ptr(), a.values = p.values->const_data_ptr();
+  a.table = p.table->const_data_ptr<int>(), a.starts = p.starts->const_data_ptr<int>(), a.past = p.past->const_data_ptr<int>();
+  a.status = context(q, 0)->status, a.workspace = workspace.mutable_data_ptr();
+  a.q_st = step(q, 0), a.q_sh = step(q, 1), a.o_st = step(out, 0), a.o_sh = step(out, 1);
+  a.k_sp = step(*p.keys, 0), a.k_sh = step(*p.keys, 1), a.k_ss = step(*p.keys, 2);
+  a.v_sp = step(*p.values, 0), a.v_sh = step(*p.values, 1), a.v_ss = step(*p.values, 2), a.table_ld = p.table->stride(0);
+  a.n = int(p.n()), a.tokens = int(tokens), a.heads = int(heads), a.kv_heads = int(kv_heads), a.head_dim = int(dim), a.pages = int(p.keys->size(0));
+  a.page_size = int(p.keys->size(2)), a.table_width = int(p.table->size(1)), a.window = int(std::min<int64_t>(window, 1 << 30)), a.most_new = int(most);
+  a.fill_rest = !given.defined(), a.scale = scale == 0. ? float(1. / std::sqrt(double(dim))) : float(scale);
+  check(lib.paged_attention(&a, stream_of(q)), "tpb_paged_attention");
+  launched.fetch_add(2, std::memory_order_relaxed);
+  return out;
+}
+
+struct Turn {
+  Tensor frequencies;
+  bool interleaved = false;
+  double factor = 1.;
+};
+enum class Queries { not_taken, kept, made };
+
+Queries paged_append(const Pages& p, const Tensor& q, const Tensor& k, const Tensor& v, const Turn& turn, const Tensor& q_norm, const Tensor& k_norm, double eps,
+                     const Tensor& given, Tensor* result) {
+  if (!lib.paged_append || interposed() || !pages_fit(p, 1) || k.dim() != 3) return Queries::not_taken;
+  const int64_t tokens = k.size(0), kv_heads = p.keys->size(1), dim = p.keys->size(3);
+  const auto device = p.keys->device();
+  if (dim % 8 || dim > 256 || tokens <= 0 || tokens >= (int64_t(1) << 31) || !rows_like(k, kv_heads, p, tokens) || !rows_like(v, kv_heads, p, tokens) ||
+      !written_once(*p.keys) || !written_once(*p.values))
+    return Queries::not_taken;
+  for (const Tensor* t : {&q_norm, &k_norm})
+    if (t->defined() && (!vectors(*t, 1, device) || t->size(0) != dim)) return Queries::not_taken;
+  if (turn.frequencies.defined() && (!plain(turn.frequencies, at::kFloat, device) || turn.frequencies.dim() != 1 || !turn.frequencies.is_contiguous() ||
+                                     turn.frequencies.size(0) == 0 || 2 * turn.frequencies.size(0) > dim))
+    return Queries::not_taken;
+  if (q.defined() && (!rows_like(q, -1, p, tokens) || q.size(1) == 0)) return Queries::not_taken;
+  if (given.defined() && (!q.defined() || !rows_like(given, q.size(1), p, tokens) || !written_once(given))) return Queries::not_taken;
+  const bool makes = q.defined() && (turn.frequencies.defined() || q_norm.defined() || given.defined());
+  const py::gil_scoped_release unlocked;
+  const c10::cuda::CUDAGuard guard(device);
+  tpb_paged_append_t a = {};
+  if (makes) {
+    *result = given.defined() ? given : room_for(q.sizes(), at::kBFloat16);
+    a.q = q.const_data_ptr(), a.q_out = result->mutable_data_ptr(), a.heads = int(q.size(1));
+    a.q_st = step(q, 0), a.q_sh = step(q, 1), a.o_st = step(*result, 0), a.o_sh = step(*result, 1);
+  }
+  a.k = k.const_data_ptr(), a.v = v.const_data_ptr(), a.keys = p.keys->mutable_data_ptr(), a.values = p.values->mutable_data_ptr();
+  a.table = p.table->const_data_ptr<int>(), a.starts = p.starts->const_data_ptr<int>(), a.past = p.past->const_data_ptr<int>();
+  a.q_norm = data(q_norm), a.k_norm = data(k_norm), a.status = context(k, 0)->status;
+  if (turn.frequencies.defined()) {
+    a.frequencies = turn.frequencies.const_data_ptr<float>();
+    a.rotary_dim = int(2 * turn.frequencies.size(0)), a.interleaved = turn.interleaved;
+  }
+  a.k_st = step(k, 0), a.k_sh = step(k, 1), a.v_st = step(v, 0), a.v_sh = step(v, 1);
+  a.k_sp = step(*p.keys, 0), a.k_shead = step(*p.keys, 1), a.k_ss = step(*p.keys, 2);
+  a.v_sp = step(*p.values, 0), a.v_shead = step(*p.values, 1), a.v_ss = step(*p.values, 2), a.table_ld = p.table->stride(0);
+  a.n = int(p.n()), a.tokens = int(tokens), a.kv_heads = int(kv_heads), a.head_dim = int(dim), a.pages = int(p.keys->size(0)), a.page_size = int(p.keys->size(2));
+  a.table_width = int(p.table->size(1)), a.fill_rest = !given.defined(), a.factor = float(turn.factor), a.eps = float(eps);
+  check(lib.paged_append(&a, stream_of(k)), "tpb_paged_append");
+  launched.fetch_add(1, std::memory_order_relaxed);
+  return makes ? Queries::made : Queries::kept;
+}
+
+struct PerRow {  // a penalty: fp32 [rows], or one number for all
+  Tensor rows;
+  double all;
+};
+Tensor adjust_logits(const Tensor& x, const Tensor& tokens, const Tensor& lengths, const Tensor& prompts, const PerRow& repetition, const PerRow& frequency,
+                     const PerRow& presence, const Tensor& bias, const Tensor& allowed) {
+  const auto device = x.device();
+  const auto dtype = x.scalar_type();
+  const int64_t limit = int64_t(1) << 31;
+  if (!lib.adjust_logits || !x.is_cuda() || (dtype != at::kBFloat16 && dtype != at::kFloat) || interposed() || !plain(x, dtype, device) || x.dim() != 2) return {};
+  const int64_t rows = x.size(0), vocab = x.size(1), words = (vocab + 31) / 32;
+  if (rows <= 0 || vocab <= 0 || rows >= limit || vocab >= limit || (x.stride(1) != 1 && vocab != 1)) return {};
+  if (!tokens.defined() && (lengths.defined() || prompts.defined() || repetition.rows.defined() || frequency.rows.defined() || presence.rows.defined())) return {};
+  if (tokens.defined() && (!plain(tokens, at::kLong, device) || tokens.dim() != 2 || tokens.size(0) != rows || tokens.size(1) >= limit ||
+                           (tokens.stride(1) != 1 && tokens.size(1) > 1)))
+    return {};
+  for (const Tensor* t : {&lengths, &prompts})
+    if (t->defined() && (!ints(*t, 1, device) || t->size(0) != rows)) return {};
+  for (const PerRow* t : {&repetition, &frequency, &presence})
+    if (t->rows.defined() && (!plain(t->rows, at::kFloat, device) || !vector_of(t->rows, rows))) return {};
+  if (bias.defined() && ((bias.scalar_type() != at::kFloat && bias.scalar_type() != at::kBFloat16) || !plain(bias, bias.scalar_type(), device) || bias.dim() < 1 ||
+                         bias.dim() > 2 || bias.size(-1) != vocab || (bias.dim() == 2 && bias.size(0) != rows) || (bias.stride(-1) != 1 && vocab != 1)))
+    return {};
+  if (allowed.defined() && (allowed.dim() < 1 || allowed.dim() > 2 || !ints(allowed, allowed.dim(), device) || allowed.size(-1) != words ||
+                            (allowed.dim() == 2 && allowed.size(0) != rows)))
+    return {};
+  const py::gil_scoped_release unlocked;
+  const c10::cuda::CUDAGuard guard(device);
+  Tensor out = room_for(x.sizes(), dtype);
+  tpb_adjust_logits_t a = {};
+  a.logits = x.const_data_ptr(), a.out = out.mutable_data_ptr(), a.status = context(x, 0)->status;
+  a.logits_ld = x.stride(0), a.out_ld = vocab, a.rows = int(rows), a.vocab = int(vocab), a.dtype = dtype == at::kFloat, a.repetition_all = 1.f;
+  if (tokens.defined() && tokens.size(1) > 0) {
+    auto numbers = [](const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; };
+    a.tokens = reinterpret_cast<const long long*>(tokens.const_data_ptr<int64_t>()), a.tokens_ld = tokens.stride(0), a.width = int(tokens.size(1));
+    a.lengths = lengths.defined() ? lengths.const_data_ptr<int>() : nullptr, a.prompts = prompts.defined() ? prompts.const_data_ptr<int>() : nullptr;
+    a.repetition = numbers(repetition.rows), a.frequency = numbers(frequency.rows), a.presence = numbers(presence.rows);
+    a.repetition_all = float(repetition.all), a.frequency_all = float(frequency.all), a.presence_all = float(presence.all);
+  }
+  if (bias.defined()) a.bias = bias.const_data_ptr(), a.bias_ld = bias.dim() == 2 ? bias.stride(0) : 0, a.bias_dtype = bias.scalar_type() == at::kFloat;
+  if (allowed.defined()) a.allowed = allowed.const_data_ptr<int>(), a.allowed_ld = allowed.dim() == 2 ? allowed.stride(0) : 0;
+  check(lib.adjust_logits(&a, stream_of(x)), "tpb_adjust_logits");
+  launched.fetch_add(1, std::memory_order_relaxed);
+  return out;
+}
+
 // Whether operators are being captured or shapes followed (make_fx, fake tensors, capture ahead of dispatch): a kernel would leave nothing in the graph but the
 // allocation of its result.  Other dispatch modes (recomputation with a policy, counters) let kernels run.
 bool captured() {
@@ -468,6 +635,92 @@ PyObject* py_linear_int8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
+// The tensors of a cache and of a batch's lengths.
+bool pages_of(PyObject* cache, PyObject* starts, PyObject* past, Pages* p) {
+  if (!PyTuple_Check(cache) || PyTuple_GET_SIZE(cache) != 3) return false;
+  p->keys = a_tensor(PyTuple_GET_ITEM(cache, 0));
+  p->values = a_tensor(PyTuple_GET_ITEM(cache, 1));
+  p->table = a_tensor(PyTuple_GET_ITEM(cache, 2));
+  p->starts = a_tensor(starts);
+  p->past = a_tensor(past);
+  return p->keys && p->values && p->table && p->starts && p->past && p->past->dim() == 1 && p->starts->dim() == 1 && p->table->dim() == 2;
+}
+// (q, cache, starts, past, scale, window, most_new, out) -> result
+PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages p;
+  const Tensor *q = n == 8 ? a_tensor(args[0]) : nullptr, *given = n == 8 ? tensor_of(args[7]) : nullptr;
+  if (!q || !given || !pages_of(args[1], args[2], args[3], &p)) Py_RETURN_NONE;
+  double scale = 0.;
+  int64_t window = 0, most_new = -1;
+  if (args[4] != Py_None) {
+    if (!PyFloat_CheckExact(args[4]) || !(PyFloat_AS_DOUBLE(args[4]) > 0.) || std::isinf(PyFloat_AS_DOUBLE(args[4]))) Py_RETURN_NONE;
+    scale = PyFloat_AS_DOUBLE(args[4]);
+  }
+  for (int i = 5; i < 7; ++i) {
+    if (args[i] == Py_None) continue;
+    if (!PyLong_CheckExact(args[i])) Py_RETURN_NONE;
+    int over = 0;
+    const long long value = PyLong_AsLongLongAndOverflow(args[i], &over);
+    if (over || value < (i == 5 ? 1 : 0)) Py_RETURN_NONE;
+    (i == 5 ? window : most_new) = value;
+  }
+  const Tensor out = paged_attention(*q, p, scale, window, most_new, *given);
+  if (!out.defined()) Py_RETURN_NONE;
+  return given->defined() ? Py_NewRef(args[7]) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+// (cache, q, k, v, starts, past, rotary, q_norm, k_norm, eps, out) -> (queries,)
+PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages p;
+  if (n != 11 || !pages_of(args[0], args[4], args[5], &p)) Py_RETURN_NONE;
+  const Tensor *q = tensor_of(args[1]), *k = a_tensor(args[2]), *v = a_tensor(args[3]), *q_norm = tensor_of(args[7]), *k_norm = tensor_of(args[8]), *given = tensor_of(args[10]);
+  if (!q || !k || !v || !q_norm || !k_norm || !given || !PyFloat_CheckExact(args[9])) Py_RETURN_NONE;
+  Turn turn;
+  if (args[6] != Py_None) {
+    PyObject* t = args[6];
+    const Tensor* f = PyTuple_Check(t) && PyTuple_GET_SIZE(t) == 3 ? a_tensor(PyTuple_GET_ITEM(t, 0)) : nullptr;
+    if (!f || !PyBool_Check(PyTuple_GET_ITEM(t, 1)) || !PyFloat_CheckExact(PyTuple_GET_ITEM(t, 2))) Py_RETURN_NONE;
+    turn = {*f, PyTuple_GET_ITEM(t, 1) == Py_True, PyFloat_AS_DOUBLE(PyTuple_GET_ITEM(t, 2))};
+  }
+  Tensor result;
+  const Queries done = paged_append(p, *q, *k, *v, turn, *q_norm, *k_norm, PyFloat_AS_DOUBLE(args[9]), *given, &result);
+  if (done == Queries::not_taken) Py_RETURN_NONE;
+  PyObject* queries = done == Queries::kept ? Py_NewRef(args[1]) : given->defined() ? Py_NewRef(args[10]) : THPVariable_Wrap(result);
+  if (!queries) return nullptr;
+  PyObject* one = PyTuple_New(1);  // (a call without queries is done as well)
+  if (!one) {
+    Py_DECREF(queries);
+    return nullptr;
+  }
+  PyTuple_SET_ITEM(one, 0, queries);
+  return one;
+  END_HANDLE_TH_ERRORS
+}
+// (logits, tokens, lengths, prompt lengths, repetition, frequency, presence, bias, allowed) -> logits
+PyObject* py_adjust_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor* x = n == 9 ? a_tensor(args[0]) : nullptr;
+  if (!x) Py_RETURN_NONE;
+  const Tensor *tokens = tensor_of(args[1]), *lengths = tensor_of(args[2]), *prompts = tensor_of(args[3]), *bias = tensor_of(args[7]), *allowed = tensor_of(args[8]);
+  if (!tokens || !lengths || !prompts || !bias || !allowed) Py_RETURN_NONE;
+  PerRow penalties[3] = {{Tensor(), 1.}, {Tensor(), 0.}, {Tensor(), 0.}};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* o = args[4 + i];
+    if (o == Py_None) continue;
+    if (THPVariable_Check(o)) {
+      penalties[i].rows = THPVariable_Unpack(o);
+    } else {
+      if (!PyFloat_CheckExact(o) || !tokens->defined() || (i == 0 && !(PyFloat_AS_DOUBLE(o) > 0.))) Py_RETURN_NONE;
+      penalties[i].all = PyFloat_AS_DOUBLE(o);
+    }
+  }
+  const Tensor out = adjust_logits(*x, *tokens, *lengths, *prompts, penalties[0], penalties[1], penalties[2], *bias, *allowed);
+  if (!out.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
 // () -> whether a call would go on in Python for what is around it
 PyObject* py_interposed(PyObject*, PyObject*) {
   HANDLE_TH_ERRORS
@@ -486,6 +739,9 @@ PyMethodDef plain_calls[] = {
     {"quantize_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_quantize_int8)), METH_FASTCALL, nullptr},
     {"norm_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_int8)), METH_FASTCALL, nullptr},
     {"linear_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_int8)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_attention)), METH_FASTCALL, nullptr},
+    {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_append)), METH_FASTCALL, nullptr},
+    {"adjust_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_adjust_logits)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 void bind_int8(py::object type, py::dict codes) {
@@ -517,6 +773,15 @@ void bind(const py::dict& addresses, py::function text, py::function reserve) {
   if (addresses.contains("tpb_gemm_int8")) {
     entry(lib.rows_int8, addresses, "tpb_rows_int8");
     entry(lib.gemm_int8, addresses, "tpb_gemm_int8");
+  }
+  lib.paged_attention = nullptr;
+  lib.paged_append = nullptr;
+  lib.adjust_logits = nullptr;
+  if (addresses.contains("tpb_paged_attention")) {
+    entry(lib.paged_attention_workspace, addresses, "tpb_paged_attention_workspace");
+    entry(lib.paged_attention, addresses, "tpb_paged_attention");
+    entry(lib.paged_append, addresses, "tpb_paged_append");
+    entry(lib.adjust_logits, addresses, "tpb_adjust_logits");
   }
   Py_XDECREF(error_text);
   Py_XDECREF(reserve_slots);

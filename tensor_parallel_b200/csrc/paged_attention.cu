@@ -30,7 +30,9 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int PA_TILE = 64;                 // keys of a stage
 constexpr int PA_BLOCK = PA_TILE * 128;     // bytes of a swizzled block of 64 keys x 64 elements
-constexpr int PA_MIN_SHARE = 2;             // tiles of a CTA's range, at least
+constexpr int PA_MIN_SHARE = 3;             // of a CTA's range, at least: a piece and two tiles
+// What a row tile costs beside its key tiles, in tiles: its query rows, the meeting of the key groups, its result.  It stands in front of them on the line.
+constexpr int PA_PIECE_COST = 1;
 
 struct PagedAttnParams {
   PagedBatch b;
@@ -51,7 +53,7 @@ struct PagedAttnParams {
 struct PagedUnits {
   PagedSequence s;
   int rows, row_tiles, first_tile, tiles;  // tiles of keys, from first_tile on
-  long long cost;                          // row_tiles * kv_heads * tiles, 0: not this launch's
+  long long cost;                          // row_tiles * kv_heads * (tiles + PA_PIECE_COST), 0: not this launch's
 };
 
 template <int ROWS>
@@ -67,11 +69,11 @@ __device__ __forceinline__ PagedUnits paged_units(const PagedAttnParams& p, int 
     u.first_tile = p.window ? max(0, u.s.past - p.window + 1) / PA_TILE : 0;
     u.tiles = (u.s.past + u.s.fresh + PA_TILE - 1) / PA_TILE - u.first_tile;
   }
-  u.cost = mine ? (long long)u.row_tiles * p.kv_heads * u.tiles : 0;
+  u.cost = mine ? (long long)u.row_tiles * p.kv_heads * (u.tiles + PA_PIECE_COST) : 0;
   return u;
 }
 
-enum { PIECE_FIRST = 1, PIECE_LAST = 2, PIECE_POISON = 4 };
+enum { PIECE_FIRST = 1, PIECE_LAST = 2, PIECE_POISON = 4, RANGE_END = 8 };
 
 struct PagedPiece {  // of a row tile's keys, as the producer hands it to the compute warps
   int token0, row0, rows, past, total, low, kvh;  // low: first key that any row of the sequence sees
@@ -110,9 +112,9 @@ struct Few {
   static constexpr int STAGE_BYTES = 2 * DB * PA_BLOCK;
   static constexpr int STAGES = (R == 1 ? 96 : 160) * 1024 / STAGE_BYTES;
   static constexpr int Q_BYTES = ROWS * D * 2;
-  static constexpr int MERGE_FLOATS = WARPS * 2 * D;
+  static constexpr int MERGE_COLS = STAGE_BYTES / (WARPS * 16 * 4) < D ? STAGE_BYTES / (WARPS * 16 * 4) : D;  // that the partial results of all warps fill a stage with
   static constexpr int THREADS = WARPS * 32 + 32;
-  static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 2 * Q_BYTES + MERGE_FLOATS * 4 + WARPS * 16 * 8 + STAGES * 8 + 2 * int(sizeof(PagedPiece)) +
+  static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 2 * Q_BYTES + WARPS * 16 * 8 + STAGES * 8 + 2 * int(sizeof(PagedPiece)) +
                               (2 * STAGES + 6) * 8 + 256;
 };
 
@@ -126,8 +128,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem;                                    // [STAGES][keys | values][DB][64 keys][128 bytes]
   uint8_t* q_s = ring + STAGES * C::STAGE_BYTES;           // [2][DB][ROWS][128 bytes], swizzled like the ring
-  float* merge = reinterpret_cast<float*>(q_s + 2 * C::Q_BYTES);         // [WARPS][2 rows][D]
-  float2* stats = reinterpret_cast<float2*>(merge + C::MERGE_FLOATS);    // [WARPS][16 rows]
+  float2* stats = reinterpret_cast<float2*>(q_s + 2 * C::Q_BYTES);       // [WARPS][16 rows]
   int2* stage_info = reinterpret_cast<int2*>(stats + WARPS * 16);        // [STAGES] first key, flags
   PagedPiece* pieces = reinterpret_cast<PagedPiece*>(stage_info + STAGES);  // [2]
   uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(pieces + 2) + 7) & ~uintptr_t(7));
@@ -253,9 +254,12 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         ++seq;
         continue;
       }
-      const long long unit = (at - seq_begin) / u.tiles;
-      const int t0 = int((at - seq_begin) - unit * u.tiles);
-      const int t1 = int(min((long long)u.tiles, t0 + (w1 - at)));
+      const int length = u.tiles + PA_PIECE_COST;
+      const long long unit = (at - seq_begin) / length;
+      const int from = int((at - seq_begin) - unit * length), to = int(min((long long)length, from + (w1 - at)));
+      const int t0 = max(0, from - PA_PIECE_COST), t1 = max(0, to - PA_PIECE_COST);
+      at += to - from;
+      if (t0 == t1) continue;  // (the range ends in front of the first tile)
       const int kvh = int(unit % p.kv_heads), row0 = int(unit / p.kv_heads) * ROWS;
       const int total = u.s.bad ? 0 : u.s.past + u.s.fresh;
       const int low = p.window && !u.s.bad ? max(0, u.s.past - p.window + 1) : 0;
@@ -282,7 +286,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         // keys that begin in this range and end in another's are joined by the block of this CTA; its other piece continues the range in front
         o.slot = t0 == 0 && t1 == u.tiles ? -1 : 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
         if (t0 == 0 && t1 < u.tiles) {
-          const long long unit_end = seq_begin + (unit + 1) * u.tiles;
+          const long long unit_end = seq_begin + (unit + 1) * length;
           p.joins[2 * blockIdx.x] = make_int4(o.token0, row0, o.rows, kvh);
           p.joins[2 * blockIdx.x + 1] = make_int4(int((unit_end - 1) / share), 0, 0, 0);
         }
@@ -328,8 +332,15 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                       (my_block % DB) * 64, per_tile == 1 ? key0 & (page_size - 1) : 0, kvh, page);
       }
       if (!ok) break;
-      at += t1 - t0;
       ++piece;
+    }
+    if (ok) {
+      const int stage = it % STAGES;
+      ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait(&empty[stage], ((it / STAGES) & 1) ^ 1));
+      if (ok && lane == 0) {
+        stage_info[stage] = make_int2(0, RANGE_END);
+        mbar_arrive(&full[stage]);
+      }
     }
     if (!ok && lane == 0 && !*abort_flag) give_up();
     return;
@@ -341,7 +352,6 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   const int key_off = kg * C::KEYS;
   const int g8 = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;
   const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(q_s);
-  const int count = int(w1 - w0);
   float o[D / 8][4];
   float m[2], l[2];
   uint32_t qf[R == 1 ? D / 16 : 1][4];
@@ -357,11 +367,12 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     meet_phase ^= 1;
     return ok;
   };
-  for (int it = 0; it < count; ++it) {
+  for (int it = 0;; ++it) {
     const int stage = it % STAGES;
     ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait(&full[stage], (it / STAGES) & 1));
     if (!ok) break;
     const int2 info = stage_info[stage];
+    if (info.y & RANGE_END) break;
     const int key0 = info.x + key_off;
     if (info.y & PIECE_FIRST) {
       ok = __all_sync(0xffffffffu, mbar_wait(&q_full[piece & 1], (piece >> 1) & 1));
@@ -479,110 +490,119 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         uint32_t b[4];
         const int r = key_off + ks * 16 + (mi & 1) * 8 + mr, c = dn * 2 + (mi >> 1);
         ldsm4_t(b, v_a + (c >> 3) * PA_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-        mma16816(o[2 * dn], a, b[0] & keep[0], b[1] & keep[1]);
-        mma16816(o[2 * dn + 1], a, b[2] & keep[0], b[3] & keep[1]);
+        if (cut) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] &= keep[j & 1];
+        }
+        mma16816(o[2 * dn], a, b[0], b[1]);
+        mma16816(o[2 * dn + 1], a, b[2], b[3]);
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[stage]);
-
-    if (info.y & PIECE_LAST) {
-      // ---- the key groups meet: a row (and the one eight below it) at a time ----
+    if (!(info.y & PIECE_LAST)) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+      continue;
+    }
+    // ---- the key groups meet, in the room of the stage that all of them have read: [warp][16 rows][COLS], blocks of eight columns swizzled by row ----
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (t4 == 0) stats[warp * 16 + g8 + 8 * i] = make_float2(m[i], l[i]);
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      if (t4 == 0) stats[warp * 16 + g8 + 8 * i] = make_float2(m[i], l[i]);
+    }
+    if (!meet_all()) break;
+    float f[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < C::KEY_GROUPS; ++k) top = fmaxf(top, stats[(k * R + rg) * 16 + g8 + 8 * i].x);
+      const float b0 = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int k = 0; k < C::KEY_GROUPS; ++k) {
+        const float2 st = stats[(k * R + rg) * 16 + g8 + 8 * i];
+        sum += st.y * ex2_approx(st.x - b0);
       }
+      f[i] = ex2_approx(m[i] - b0);
+      if (poisoned) sum = __uint_as_float(0x7fc00000u);
+      if (pc.slot < 0) f[i] = sum == 0.f ? 0.f : f[i] / sum;
+      if (pc.slot >= 0 && kg == 0 && t4 == 0) p.part_ml[(long long)pc.slot * ROWS + rg * 16 + g8 + 8 * i] = make_float2(top, sum);
+    }
+    float* merge = reinterpret_cast<float*>(ring + stage * C::STAGE_BYTES);
+    constexpr int COLS = C::MERGE_COLS;
+#pragma unroll
+    for (int c0 = 0; c0 < D; c0 += COLS) {
+      if (c0 && !meet_all()) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int d = 0; d < COLS / 8; ++d)
+          *reinterpret_cast<float2*>(merge + (warp * 16 + g8 + 8 * i) * COLS + ((d ^ (g8 & (COLS / 8 - 1))) * 8) + t4 * 2) =
+              make_float2(o[c0 / 8 + d][2 * i] * f[i], o[c0 / 8 + d][2 * i + 1] * f[i]);
       if (!meet_all()) break;
-      float f[2], top[2], sum[2];
+      for (int c = threadIdx.x; c < pc.rows * (COLS / 4); c += WARPS * 32) {
+        const int r = c / (COLS / 4), col = (c % (COLS / 4)) * 4;
+        const float* from = merge + ((r >> 4) * 16 + (r & 15)) * COLS + (((col >> 3) ^ (r & 7 & (COLS / 8 - 1))) * 8) + (col & 7);
+        float4 v = *reinterpret_cast<const float4*>(from);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[i] = -INFINITY;
-        sum[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < C::KEY_GROUPS; ++k) top[i] = fmaxf(top[i], stats[(k * R + rg) * 16 + g8 + 8 * i].x);
-        const float b0 = top[i] == -INFINITY ? 0.f : top[i];
-#pragma unroll
-        for (int k = 0; k < C::KEY_GROUPS; ++k) {
-          const float2 st = stats[(k * R + rg) * 16 + g8 + 8 * i];
-          sum[i] += st.y * ex2_approx(st.x - b0);
+        for (int k = 1; k < C::KEY_GROUPS; ++k) {
+          const float4 w = *reinterpret_cast<const float4*>(from + k * R * 16 * COLS);
+          v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
         }
-        f[i] = ex2_approx(m[i] - b0);
-        if (poisoned) sum[i] = __uint_as_float(0x7fc00000u);
-        if (pc.slot < 0) f[i] = sum[i] == 0.f ? 0.f : f[i] / sum[i];
-        if (pc.slot >= 0 && kg == 0 && t4 == 0) p.part_ml[(long long)pc.slot * ROWS + rg * 16 + g8 + 8 * i] = make_float2(top[i], sum[i]);
+        if (pc.slot >= 0) {
+          *reinterpret_cast<float4*>(p.part_o + ((long long)pc.slot * ROWS + r) * D + c0 + col) = v;
+        } else {
+          const int t = (pc.row0 + r) / p.group, h = (pc.row0 + r) % p.group;
+          *reinterpret_cast<uint2*>(p.out + (long long)(pc.token0 + t) * p.o_st + (long long)(pc.kvh * p.group + h) * p.o_sh + c0 + col) =
+              make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+        }
       }
-      const int here = pc.rows;  // rows of the piece
-      for (int g = 0; g < min(8, here); ++g) {
-        if (g8 == g) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int d = 0; d < D / 8; ++d)
-              *reinterpret_cast<float2*>(merge + (warp * 2 + i) * D + d * 8 + t4 * 2) = make_float2(o[d][2 * i] * f[i], o[d][2 * i + 1] * f[i]);
-        }
-        if (!meet_all()) break;
-        // the warps of a row group share out its two rows
-        for (int c = kg * 32 + lane; c < D; c += C::KEY_GROUPS * 32) {
-          const int i = c / (D / 2), col = (c % (D / 2)) * 2;
-          const int r = rg * 16 + g + 8 * i;
-          if (r < here) {
-            float2 v = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < C::KEY_GROUPS; ++k) {
-              const float2 w = *reinterpret_cast<const float2*>(merge + ((k * R + rg) * 2 + i) * D + col);
-              v.x += w.x;
-              v.y += w.y;
-            }
-            if (pc.slot >= 0) {
-              *reinterpret_cast<float2*>(p.part_o + ((long long)pc.slot * ROWS + r) * D + col) = v;
-            } else {
-              const int t = (pc.row0 + r) / p.group, h = (pc.row0 + r) % p.group;
-              *reinterpret_cast<uint32_t*>(p.out + (long long)(pc.token0 + t) * p.o_st + (long long)(pc.kvh * p.group + h) * p.o_sh + col) = pack_bf16x2(v.x, v.y);
-            }
-          }
-        }
-        if (!meet_all()) break;
-      }
-      if (!ok) break;
-      if (lane == 0) mbar_arrive(&q_empty[piece & 1]);
-      ++piece;
     }
+    if (!ok) break;
+    fence_proxy_async_smem();  // (the next bulk copies come behind these writes)
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&empty[stage]);
+      mbar_arrive(&q_empty[piece & 1]);
+    }
+    ++piece;
   }
   if (!ok && lane == 0 && !*abort_flag) give_up();
 }
 
-// Joins the pieces of the row tile whose keys begin in a CTA's range and end in another's: a block for each CTA, and most of them have nothing to do.
+// Joins the pieces of the row tile whose keys begin in a CTA's range and end in another's: blocks for each CTA, of which most have nothing to do, and a
+// thread for every four columns of a row.
 constexpr int PA_JOIN_THREADS = 128;
 
 template <int D>
 __global__ void __launch_bounds__(PA_JOIN_THREADS)
 paged_attn_join_kernel(const PagedAttnParams p, int rows_of_slot) {
+  const int item = blockIdx.y * PA_JOIN_THREADS + threadIdx.x, r = item / (D / 4), col = item % (D / 4) * 4, c = blockIdx.x;
   pa_wait_prior();
-  const int c = blockIdx.x;
   const int4 unit = p.joins[2 * c];
-  if (unit.x < 0 || int(blockIdx.y) >= unit.z) return;
   const int last = p.joins[2 * c + 1].x;
+  if (unit.x < 0 || r >= unit.z) return;
   // the first piece is in slot 2c + 1, those of the CTAs behind it in their slots 2c'
-  for (int r = blockIdx.y; r < unit.z; r += gridDim.y) {
-    auto slot = [&](int i) { return (long long)(i == c ? 2 * c + 1 : 2 * i) * rows_of_slot + r; };
-    float top = -INFINITY;
-    for (int i = c; i <= last; ++i) top = fmaxf(top, p.part_ml[slot(i)].x);
-    const float b0 = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int i = c; i <= last; ++i) {
-      const float2 s = p.part_ml[slot(i)];
-      sum += s.y * ex2_approx(s.x - b0);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int t = (unit.y + r) / p.group, h = (unit.y + r) % p.group;
-    for (int col = threadIdx.x; col < D; col += PA_JOIN_THREADS) {
-      float v = 0.f;
-      for (int i = c; i <= last; ++i) v += p.part_o[slot(i) * D + col] * ex2_approx(p.part_ml[slot(i)].x - b0);
-      p.out[(long long)(unit.x + t) * p.o_st + (long long)(unit.w * p.group + h) * p.o_sh + col] = __float2bfloat16(v * inv);
-    }
+  const float2* ml = p.part_ml + r;
+  const float* part = p.part_o + (long long)r * D + col;
+  auto slot = [&](int i) { return (long long)(i == c ? 2 * c + 1 : 2 * i) * rows_of_slot; };
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int i = c; i <= last; ++i) top = fmaxf(top, ml[slot(i)].x);
+  const float b0 = top == -INFINITY ? 0.f : top;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = c; i <= last; ++i) {
+    const float2 s = ml[slot(i)];
+    const float4 w = *reinterpret_cast<const float4*>(part + slot(i) * D);
+    const float f = ex2_approx(s.x - b0);
+    sum += s.y * f;
+    v.x += w.x * f, v.y += w.y * f, v.z += w.z * f, v.w += w.w * f;
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int t = (unit.y + r) / p.group, h = (unit.y + r) % p.group;
+  *reinterpret_cast<uint2*>(p.out + (long long)(unit.x + t) * p.o_st + (long long)(unit.w * p.group + h) * p.o_sh + col) =
+      make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
 }
 
 static int pa_sms() {
@@ -606,7 +626,8 @@ static int pa_few_launch(const PagedAttnParams& p, const CUtensorMap& k, const C
   paged_attn_few_kernel<D, R><<<grid, C::THREADS, C::SMEM, stream>>>(k, v, p);
   if (cudaGetLastError() != cudaSuccess) return TPB_ERR_CUDA;
   if (!joins) return TPB_OK;
-  const dim3 join_grid(grid, min(C::ROWS, max(1, min(p.b.most_new, p.b.tokens)) * p.group));
+  const int rows = min(C::ROWS, max(1, min(p.b.most_new, p.b.tokens)) * p.group);
+  const dim3 join_grid(grid, (rows * (D / 4) + PA_JOIN_THREADS - 1) / PA_JOIN_THREADS);
   return launch_dependent(paged_attn_join_kernel<D>, join_grid, dim3(PA_JOIN_THREADS), 0, stream, true, p, C::ROWS) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
@@ -621,7 +642,7 @@ static void pa_plan(int n, int tokens, int table_width, int page_shift, int most
   const int rows = 16 * *row_groups;
   const long long key_tiles = (((long long)table_width << page_shift) + PA_TILE - 1) / PA_TILE;
   const long long row_tiles = (long long)tokens * group / rows + n;  // (at most: one more than full ones per sequence)
-  const long long most = min(row_tiles, (long long)n * ((most_rows + rows - 1) / rows)) * kv_heads * key_tiles;
+  const long long most = min(row_tiles, (long long)n * ((most_rows + rows - 1) / rows)) * kv_heads * (key_tiles + PA_PIECE_COST);
   const int resident = pa_sms() * (*row_groups == 1 ? 2 : 1);
   *grid = int(max(1LL, min((long long)resident, (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE)));
   *floats = (long long)*grid * 2 * (rows * (head_dim + 2) + 4);

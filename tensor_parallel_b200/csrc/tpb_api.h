@@ -220,10 +220,11 @@ typedef struct {
 } tpb_adjust_logits_t;
 int tpb_adjust_logits(const tpb_adjust_logits_t* args, void* stream);
 
-// Sizes of the structures above as this library was built, one byte-count per 16 bits (plan, reduction context, options), and the version of the
-// signatures that are called from elsewhere (1: tpb_rows_int8 takes `ahead`), for callers that are built apart from it.
+// Sizes of the structures above as this library was built (plan, reduction context, options: one byte-count per 16 bits; the three of ragged batches in the
+// last, added up), and the version of the signatures that are called from elsewhere (1: tpb_rows_int8 takes `ahead`), for callers that are built apart from it.
 #define TPB_API_LAYOUT \
-  ((unsigned long long)sizeof(tpb_gemm_plan_t) | (unsigned long long)sizeof(tpb_reduce_ctx_t) << 16 | (unsigned long long)sizeof(tpb_gemm_opts_t) << 32 | 1ull << 48)
+  ((unsigned long long)sizeof(tpb_gemm_plan_t) | (unsigned long long)sizeof(tpb_reduce_ctx_t) << 16 | (unsigned long long)sizeof(tpb_gemm_opts_t) << 32 | \
+   (1ull + 2 * (sizeof(tpb_paged_attn_t) + sizeof(tpb_paged_append_t) + sizeof(tpb_adjust_logits_t))) << 48)
 unsigned long long tpb_api_layout(void);
 
 // Measurement aids.  tpb_gemm_debug caps the smem ring depth (0 restores the default).  Skipping the MMAs and the

@@ -479,6 +479,7 @@ def _not_taken(*args):
 # The ordinary calls, as the native module takes them once it is loaded: its results, or None for a call that needs a check's words or a copy.  Not while a compiler
 # traces the front end, which would stop there: it gets the steps.
 quantize_int8_directly = norm_int8_directly = linear_int8_directly = _not_taken
+paged_append_directly = paged_attention_directly = adjust_logits_directly = _not_taken
 
 
 def _serving_only(what: str, *tensors):
@@ -640,6 +641,9 @@ def paged_append(cache: PagedCache, q, k, v, starts, past, rotary: Optional[Rota
     tensors raise.  Two tokens for one slot (sequences that share the page that they write to) leave either.  Serving only: there is no gradient."""
     if _compiling():
         torch._dynamo.graph_break()
+    done = paged_append_directly(cache, q, k, v, starts, past, rotary, q_norm, k_norm, eps, out)
+    if done is not None:
+        return done[0]
     _check_paged("paged_append", cache, starts, past, dict(q=q, k=k, v=v))
     d, kv_heads = cache[0].shape[3], cache[0].shape[1]
     if k.shape[1] != kv_heads or v.shape[1] != kv_heads:
@@ -676,6 +680,9 @@ def paged_attention(q, cache: PagedCache, starts, past, scale: Optional[float] =
     raise.  Serving only: there is no gradient."""
     if _compiling():
         torch._dynamo.graph_break()
+    done = paged_attention_directly(q, cache, starts, past, scale, window, most_new, out)
+    if done is not None:
+        return done
     _check_paged("paged_attention", cache, starts, past, dict(q=q))
     if q.shape[1] == 0 or cache[0].shape[1] == 0 or q.shape[1] % cache[0].shape[1]:
         raise ValueError(f"paged_attention: {q.shape[1]} query heads are no multiple of {cache[0].shape[1]} in the cache")
@@ -735,6 +742,9 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repeti
 
     Lengths beyond the width count as the width, below zero as zero (the CUDA kernel records status 3).  Serving only: there is no gradient."""
     if not _compiling():
+        done = adjust_logits_directly(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed)
+        if done is not None:
+            return done
         nat = _native(logits)
         _check_adjust(logits, tokens, lengths, prompt_lengths, repetition, frequency, presence, bias, allowed)
         if nat is not None and nat.adjust_logits_supported(logits) and not transformed(logits):

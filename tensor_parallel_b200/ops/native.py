@@ -224,7 +224,7 @@ def _reserve_slots(index: int, elems: int) -> int:
 
 def _bind_autograd():
     names = ("tpb_gemm_plan_ex", "tpb_gemm_bf16_ex", "tpb_norm_fwd", "tpb_norm_bwd", "tpb_norm_bwd_parts", "tpb_col_sum_parts", "tpb_col_sum",
-             "tpb_rows_int8", "tpb_gemm_int8")
+             "tpb_rows_int8", "tpb_gemm_int8", "tpb_paged_attention_workspace", "tpb_paged_attention", "tpb_paged_append", "tpb_adjust_logits")
     AUTOGRAD.bind({n: ctypes.cast(getattr(LIB, n), c_void_p).value for n in names if hasattr(LIB, n)}, _error_text, _reserve_slots)
 
 
@@ -910,22 +910,28 @@ def _vector_rows(t: torch.Tensor) -> bool:
 
 def _in_vectors(t: Optional[torch.Tensor]):
     """``t``, or a copy that vectors can read (``contiguous()`` would leave a tensor that starts off a boundary as it is)."""
+    t = t if t is None else t.resolve_neg()
     return t if t is None or _vector_rows(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    t = t.resolve_neg()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _strides(t: torch.Tensor, dims: int):
     return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(dims))  # (a dimension of one may come with any stride)
 
 
-def _pages_supported(cache) -> bool:
+def _pages_supported(cache, *written) -> bool:
     keys, values, _ = cache
-    return (keys.dtype == torch.bfloat16 and keys.numel() > 0 and _vector_rows(keys) and _vector_rows(values)
+    return (not any(t is not None and (t.is_neg() or type(t) not in (torch.Tensor, torch.nn.Parameter)) for t in (keys, values, *written)) and keys.dtype == torch.bfloat16 and keys.numel() > 0 and _vector_rows(keys) and _vector_rows(values)
             and all(s > 0 for t in (keys, values) for s, n in zip(t.stride(), t.shape) if n > 1))
 
 
 def paged_append_supported(cache, q, k, out) -> bool:
     page, d = cache[0].shape[2:]
-    return _pages_supported(cache) and page & (page - 1) == 0 and d % 8 == 0 and d <= 256 and k.shape[0] > 0 and cache[2].numel() > 0 and (out is None or _vector_rows(out))
+    return _pages_supported(cache, out) and page & (page - 1) == 0 and d % 8 == 0 and d <= 256 and k.shape[0] > 0 and cache[2].numel() > 0 and (out is None or _vector_rows(out))
 
 
 def paged_append(cache, q, k, v, starts, past, rotary, q_norm, k_norm, eps, out):
@@ -939,13 +945,13 @@ def paged_append(cache, q, k, v, starts, past, rotary, q_norm, k_norm, eps, out)
         else:
             q = None
         k, v, q_norm, k_norm = (_in_vectors(t) for t in (k, v, q_norm, k_norm))
-        starts, past, table = starts.contiguous(), past.contiguous(), table if table.stride(1) == 1 or table.shape[1] == 1 else table.contiguous()
+        starts, past, table = _dense(starts), _dense(past), _dense(table)
         a = PagedAppend(q=_ptr(q), k=_ptr(k), v=_ptr(v), q_out=None if q is None else _ptr(out), keys=_ptr(keys), values=_ptr(values), table=_ptr(table), starts=_ptr(starts),
                         past=_ptr(past), q_norm=_ptr(q_norm), k_norm=_ptr(k_norm), status=_ptr(device_state(keys.device).status), table_ld=table.stride(0),
                         n=past.shape[0], tokens=k.shape[0], heads=0 if q is None else q.shape[1], kv_heads=k.shape[1], head_dim=k.shape[2], pages=keys.shape[0],
                         page_size=keys.shape[2], table_width=table.shape[1], fill_rest=int(given is None), factor=1.0, eps=eps)
         if rotary is not None:
-            f = rotary[0].contiguous()
+            f = _dense(rotary[0])
             a.frequencies, a.rotary_dim, a.interleaved, a.factor = _ptr(f), 2 * f.shape[0], int(bool(rotary[1])), float(rotary[2])
         if q is not None:
             a.q_st, a.q_sh = _strides(q, 2)
@@ -959,7 +965,7 @@ def paged_append(cache, q, k, v, starts, past, rotary, q_norm, k_norm, eps, out)
 
 def paged_attention_supported(q, cache, out) -> bool:
     page, d = cache[0].shape[2:]
-    return (_pages_supported(cache) and page >= 16 and page & (page - 1) == 0 and d in (64, 128) and q.numel() > 0 and cache[2].numel() > 0
+    return (_pages_supported(cache, out) and page >= 16 and page & (page - 1) == 0 and d in (64, 128) and q.numel() > 0 and cache[2].numel() > 0
             and (out is None or _vector_rows(out)))
 
 
@@ -971,7 +977,7 @@ def paged_attention(q, cache, starts, past, scale, window, most_new, out):
     with torch.cuda.device(keys.device):
         q, given = _in_vectors(q), out
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        starts, past, table = starts.contiguous(), past.contiguous(), table if table.stride(1) == 1 or width == 1 else table.contiguous()
+        starts, past, table = _dense(starts), _dense(past), _dense(table)
         most = tokens if most_new is None else min(most_new, tokens)
         need = LIB.tpb_paged_attention_workspace(n, tokens, width, page, most, kv_heads, heads // kv_heads, d)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
@@ -994,16 +1000,15 @@ def adjust_logits(logits, tokens, lengths, prompt_lengths, repetition, frequency
     global _launches
     rows, vocab = logits.shape
     with torch.cuda.device(logits.device):
-        x = logits if logits.stride(1) == 1 or vocab == 1 else logits.contiguous()
+        x = _dense(logits)
         out = torch.empty(rows, vocab, dtype=x.dtype, device=x.device)
         a = AdjustLogits(logits=_ptr(x), out=_ptr(out), status=_ptr(device_state(x.device).status), logits_ld=x.stride(0), out_ld=vocab, rows=rows, vocab=vocab,
                          dtype=_dtype_code(x), repetition_all=1.0)
         held = []  # (copies live until the launch)
 
-        def dense(t, dims=1):
-            t = t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-            held.append(t)
-            return t
+        def dense(t):
+            held.append(_dense(t))
+            return held[-1]
 
         if tokens is not None and tokens.shape[1] > 0:
             t = dense(tokens)
@@ -1204,6 +1209,7 @@ if AUTOGRAD is not None:
     AUTOGRAD.bind_int8(OF.Int8Rows, {act: ACT_CODES[act] for act in OF.INT8_ACTS})
     if not OF._FORCE_TORCH:
         OF.quantize_int8_directly, OF.norm_int8_directly, OF.linear_int8_directly = AUTOGRAD.quantize_int8, AUTOGRAD.norm_int8, AUTOGRAD.linear_int8
+        OF.paged_append_directly, OF.paged_attention_directly, OF.adjust_logits_directly = AUTOGRAD.paged_append, AUTOGRAD.paged_attention, AUTOGRAD.adjust_logits
 
 
 def gemm_int8(x: OF.Int8Rows, weight: OF.Int8Rows, bias=None, act=None, residual=None, out=None, early=False):
