@@ -21,33 +21,18 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "launch.cuh"
-#include "paged.cuh"
+#include "paged_attention.cuh"
 
 namespace tpb {
-
-typedef __nv_bfloat16 bf16;
 
 constexpr int PA_TILE = 64;                 // keys of a stage
 constexpr int PA_BLOCK = PA_TILE * 128;     // bytes of a swizzled block of 64 keys x 64 elements
 constexpr int PA_MIN_SHARE = 3;             // of a CTA's range, at least: a piece and two tiles
 // What a row tile costs beside its key tiles, in tiles: its query rows, the meeting of the key groups, its result.  It stands in front of them on the line.
 constexpr int PA_PIECE_COST = 1;
-
-struct PagedAttnParams {
-  PagedBatch b;
-  const bf16* q;
-  bf16* out;
-  long long q_st, q_sh, o_st, o_sh;
-  int heads, kv_heads, group, window;
-  int rows_low, rows_high;  // sequences with rows (new tokens x group) in [rows_low, rows_high] are this launch's
-  int takes_bad;            // and those whose lengths are not possible
-  int fill_rest;            // rows outside all sequences become zeros
-  float scale_log2e;
-  float* part_o;            // [2 per CTA][16 * ROW_GROUPS][head_dim]
-  float2* part_ml;          // [2 per CTA][16 * ROW_GROUPS] maximum (of scaled scores, in powers of two) and sum
-  int4* joins;              // [2 per CTA]: the row tile whose keys begin in this CTA's range and end in another's
-};
 
 // A sequence as this launch deals with it.
 struct PagedUnits {
@@ -81,9 +66,6 @@ struct PagedPiece {  // of a row tile's keys, as the producer hands it to the co
   int bad;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -98,9 +80,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void pa_wait_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pa_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 template <int D, int R>
 struct Few {
   static constexpr int ROWS = 16 * R;
@@ -138,9 +117,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   uint64_t* q_empty = bars + 2 * STAGES + 2;  // [2]
   uint64_t* meet = bars + 2 * STAGES + 4;     // the compute warps, phase by phase
   volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
-  __shared__ long long scan_s[C::THREADS / 32];
-  __shared__ long long found_begin;
-  __shared__ int found_seq;
+  __shared__ RangeSearch<C::THREADS> range;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -156,80 +133,18 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     }
     mbar_init(meet, WARPS);
     *abort_flag = 0;
-    found_seq = p.b.n;
-    found_begin = 0;
     fence_mbar_init();
   }
+  if (threadIdx.x < 2) p.parts.joins[2 * blockIdx.x + threadIdx.x] = make_int4(-1, 0, 0, 0);
   pa_launch_next();  // (the whole grid is resident; the joining kernel waits for its end)
 
-  // ---- this CTA's range: all costs summed up, then the sequence in which the range begins ----
-  auto block_scan = [&](long long v, long long& before, long long& total) {
-    long long inc = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += o;
-    }
-    __syncthreads();
-    if (lane == 31) scan_s[warp] = inc;
-    __syncthreads();
-    before = inc - v;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < C::THREADS / 32; ++w) {
-      if (w < warp) before += scan_s[w];
-      total += scan_s[w];
-    }
-  };
-  long long all = 0, mine_before = 0, mine = 0;
-  for (int base = 0; base < p.b.n; base += C::THREADS) {
-    const int s = base + threadIdx.x;
-    long long cost = 0, before, total;
-    if (s < p.b.n) {
-      const PagedUnits u = paged_units<ROWS>(p, s);
-      cost = u.cost;
-      if (u.s.bad && p.takes_bad && blockIdx.x == 0) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
-    }
-    block_scan(cost, before, total);
-    mine_before = all + before;
-    mine = cost;
-    all += total;
-  }
-  const long long share = max((long long)PA_MIN_SHARE, (all + gridDim.x - 1) / gridDim.x);
-  const long long w0 = min(all, share * blockIdx.x), w1 = min(all, w0 + share);
-  if (p.b.n <= C::THREADS) {
-    if (mine > 0 && w0 >= mine_before && w0 < mine_before + mine) {
-      found_seq = threadIdx.x;
-      found_begin = mine_before;
-    }
-  } else {
-    long long so_far = 0;
-    for (int base = 0; base < p.b.n && so_far <= w0; base += C::THREADS) {
-      const int s = base + threadIdx.x;
-      long long before, total;
-      const long long cost = s < p.b.n ? paged_units<ROWS>(p, s).cost : 0;
-      block_scan(cost, before, total);
-      before += so_far;
-      if (cost > 0 && w0 >= before && w0 < before + cost) {
-        found_seq = s;
-        found_begin = before;
-      }
-      so_far += total;
-    }
-  }
-  if (threadIdx.x < 2) p.joins[2 * blockIdx.x + threadIdx.x] = make_int4(-1, 0, 0, 0);
-  __syncthreads();
-
-  if (p.fill_rest) {
-    const int used0 = p.b.n ? min(max(__ldg(p.b.starts), 0), p.b.tokens) : p.b.tokens;
-    const int used1 = p.b.n ? min(max(__ldg(p.b.starts + p.b.n), used0), p.b.tokens) : p.b.tokens;
-    const int rest = used0 + p.b.tokens - used1, chunks = p.heads * (D / 8);
-    for (int i = blockIdx.x; i < rest; i += gridDim.x) {
-      const long long t = i < used0 ? i : used1 + (i - used0);
-      for (int c = threadIdx.x; c < chunks; c += C::THREADS)
-        *reinterpret_cast<uint4*>(p.out + t * p.o_st + (c / (D / 8)) * p.o_sh + (c % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
-    }
-  }
+  long long share, w0, w1;
+  share_out<C::THREADS>(p.b.n, PA_MIN_SHARE, range, [&](int i) {
+    const PagedUnits u = paged_units<ROWS>(p, i);
+    if (u.s.bad && p.takes_bad && blockIdx.x == 0) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+    return u.cost;
+  }, share, w0, w1);
+  if (p.fill_rest) fill_around<D, C::THREADS>(p);
 
   auto give_up = [&]() {
     atomicMax(p.b.status, uint32_t(STATUS_TIMEOUT_MBAR));
@@ -242,8 +157,8 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     const int per_tile = max(1, PA_TILE >> p.b.page_shift);  // pages of a tile
     const int box_rows = min(page_size, PA_TILE);
     const int my_page = lane / (2 * DB), my_block = lane % (2 * DB);  // the box of this lane
-    int seq = found_seq, it = 0, piece = 0;
-    long long at = w0, seq_begin = found_begin;
+    int seq = range.seq, it = 0, piece = 0;
+    long long at = w0, seq_begin = range.begin;
     bool ok = true;
     while (ok && at < w1) {
       ok = seq < p.b.n;  // (the costs add up to w1, unless somebody writes the lengths meanwhile)
@@ -287,8 +202,8 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         o.slot = t0 == 0 && t1 == u.tiles ? -1 : 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
         if (t0 == 0 && t1 < u.tiles) {
           const long long unit_end = seq_begin + (unit + 1) * length;
-          p.joins[2 * blockIdx.x] = make_int4(o.token0, row0, o.rows, kvh);
-          p.joins[2 * blockIdx.x + 1] = make_int4(int((unit_end - 1) / share), 0, 0, 0);
+          p.parts.joins[2 * blockIdx.x] = make_int4(o.token0, row0, o.rows, kvh);
+          p.parts.joins[2 * blockIdx.x + 1] = make_int4(int((unit_end - 1) / share), 0, 0, 0);
         }
       }
       {
@@ -524,9 +439,12 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         sum += st.y * ex2_approx(st.x - b0);
       }
       f[i] = ex2_approx(m[i] - b0);
-      if (poisoned) sum = __uint_as_float(0x7fc00000u);
+      if (poisoned) {
+        top = 0.f;
+        sum = __uint_as_float(0x7fc00000u);
+      }
       if (pc.slot < 0) f[i] = sum == 0.f ? 0.f : f[i] / sum;
-      if (pc.slot >= 0 && kg == 0 && t4 == 0) p.part_ml[(long long)pc.slot * ROWS + rg * 16 + g8 + 8 * i] = make_float2(top, sum);
+      if (pc.slot >= 0 && kg == 0 && t4 == 0) p.parts.ml[(long long)pc.slot * ROWS + rg * 16 + g8 + 8 * i] = make_float2(top, sum);
     }
     float* merge = reinterpret_cast<float*>(ring + stage * C::STAGE_BYTES);
     constexpr int COLS = C::MERGE_COLS;
@@ -550,7 +468,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
         }
         if (pc.slot >= 0) {
-          *reinterpret_cast<float4*>(p.part_o + ((long long)pc.slot * ROWS + r) * D + c0 + col) = v;
+          *reinterpret_cast<float4*>(p.parts.o + ((long long)pc.slot * ROWS + r) * D + c0 + col) = v;
         } else {
           const int t = (pc.row0 + r) / p.group, h = (pc.row0 + r) % p.group;
           *reinterpret_cast<uint2*>(p.out + (long long)(pc.token0 + t) * p.o_st + (long long)(pc.kvh * p.group + h) * p.o_sh + c0 + col) =
@@ -571,38 +489,42 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 }
 
 // Joins the pieces of the row tile whose keys begin in a CTA's range and end in another's: blocks for each CTA, of which most have nothing to do, and a
-// thread for every four columns of a row.
+// thread for every four columns of a row.  `wide`: of a second launch, with larger tiles, behind those of the first.
 constexpr int PA_JOIN_THREADS = 128;
 
 template <int D>
 __global__ void __launch_bounds__(PA_JOIN_THREADS)
-paged_attn_join_kernel(const PagedAttnParams p, int rows_of_slot) {
-  const int item = blockIdx.y * PA_JOIN_THREADS + threadIdx.x, r = item / (D / 4), col = item % (D / 4) * 4, c = blockIdx.x;
+paged_attn_join_kernel(const PagedAttnParams p, const PagedParts few, int few_grid, const PagedParts wide) {
+  const bool is_wide = int(blockIdx.x) >= few_grid;
+  const PagedParts parts = is_wide ? wide : few;
+  const int c = blockIdx.x - (is_wide ? few_grid : 0);
   pa_wait_prior();
-  const int4 unit = p.joins[2 * c];
-  const int last = p.joins[2 * c + 1].x;
-  if (unit.x < 0 || r >= unit.z) return;
-  // the first piece is in slot 2c + 1, those of the CTAs behind it in their slots 2c'
-  const float2* ml = p.part_ml + r;
-  const float* part = p.part_o + (long long)r * D + col;
-  auto slot = [&](int i) { return (long long)(i == c ? 2 * c + 1 : 2 * i) * rows_of_slot; };
-  float top = -INFINITY, sum = 0.f;
+  const int4 unit = parts.joins[2 * c];
+  const int last = parts.joins[2 * c + 1].x;
+  if (unit.x < 0) return;
+  for (int item = blockIdx.y * PA_JOIN_THREADS + threadIdx.x; item < unit.z * (D / 4); item += gridDim.y * PA_JOIN_THREADS) {
+    const int r = item / (D / 4), col = item % (D / 4) * 4;
+    const float2* ml = parts.ml + r;
+    const float* part = parts.o + (long long)r * D + col;
+    auto slot = [&](int i) { return (long long)(i == c ? 2 * c + 1 : 2 * i) * parts.rows; };
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll 4
-  for (int i = c; i <= last; ++i) top = fmaxf(top, ml[slot(i)].x);
-  const float b0 = top == -INFINITY ? 0.f : top;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = c; i <= last; ++i) top = fmaxf(top, ml[slot(i)].x);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int i = c; i <= last; ++i) {
-    const float2 s = ml[slot(i)];
-    const float4 w = *reinterpret_cast<const float4*>(part + slot(i) * D);
-    const float f = ex2_approx(s.x - b0);
-    sum += s.y * f;
-    v.x += w.x * f, v.y += w.y * f, v.z += w.z * f, v.w += w.w * f;
+    for (int i = c; i <= last; ++i) {
+      const float2 s = ml[slot(i)];
+      if (s.x == -INFINITY) continue;  // (no key of the piece is the row's)
+      const float4 w = *reinterpret_cast<const float4*>(part + slot(i) * D);
+      const float f = ex2_approx(s.x - top);
+      sum += s.y * f;
+      v.x += w.x * f, v.y += w.y * f, v.z += w.z * f, v.w += w.w * f;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int t = (unit.y + r) / p.group, h = (unit.y + r) % p.group;
+    *reinterpret_cast<uint2*>(p.out + (long long)(unit.x + t) * p.o_st + (long long)(unit.w * p.group + h) * p.o_sh + col) =
+        make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int t = (unit.y + r) / p.group, h = (unit.y + r) % p.group;
-  *reinterpret_cast<uint2*>(p.out + (long long)(unit.x + t) * p.o_st + (long long)(unit.w * p.group + h) * p.o_sh + col) =
-      make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
 }
 
 static int pa_sms() {
@@ -614,93 +536,130 @@ static int pa_sms() {
 }
 
 template <int D, int R>
-static int pa_few_launch(const PagedAttnParams& p, const CUtensorMap& k, const CUtensorMap& v, int grid, bool joins, cudaStream_t stream) {
+static int pa_few_launch(const PagedAttnParams& p, const CUtensorMap& k, const CUtensorMap& v, int grid, cudaStream_t stream) {
   using C = Few<D, R>;
-  static int ready[64] = {};
+  static std::atomic<bool> ready[64];
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return TPB_ERR_CUDA;
-  if (!ready[dev]) {
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TPB_ERR_CUDA;
+  if (!ready[dev].load(std::memory_order_acquire)) {
     if (cudaFuncSetAttribute(paged_attn_few_kernel<D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return TPB_ERR_CUDA;
-    ready[dev] = 1;
+    ready[dev].store(true, std::memory_order_release);
   }
   paged_attn_few_kernel<D, R><<<grid, C::THREADS, C::SMEM, stream>>>(k, v, p);
-  if (cudaGetLastError() != cudaSuccess) return TPB_ERR_CUDA;
-  if (!joins) return TPB_OK;
-  const int rows = min(C::ROWS, max(1, min(p.b.most_new, p.b.tokens)) * p.group);
-  const dim3 join_grid(grid, (rows * (D / 4) + PA_JOIN_THREADS - 1) / PA_JOIN_THREADS);
-  return launch_dependent(paged_attn_join_kernel<D>, join_grid, dim3(PA_JOIN_THREADS), 0, stream, true, p, C::ROWS) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+}
+
+// What a call launches.  Sequences with few query rows (new tokens x query heads of a KV head) go by the kernel above, bound by memory; those with more by the one
+// on the tensor cores of paged_attention_sm100.cu.  The host knows the rows of a sequence at most; where both kinds may be in the batch, both are launched.
+struct PagedPlan {
+  int row_groups, few_grid, few_high, wide_grid;  // grid 0: not launched; sequences up to few_high rows are the first's
+  bool joins;
+  long long few_floats, wide_floats;
+};
+static PagedPlan pa_plan(int n, int tokens, int table_width, int page_shift, int most_new, int kv_heads, int group, int head_dim) {
+  PagedPlan plan = {};
+  const long long most_rows = (long long)min(most_new, tokens) * group, keys = (long long)table_width << page_shift;
+  const bool wide = most_rows > 64, few = !wide || n > 1;
+  // rows of a tile of the first: all of a sequence's where there are no more than 64, else those of one token
+  const long long usual = wide ? group : most_rows;
+  plan.row_groups = usual <= 16 ? 1 : usual <= 32 ? 2 : 4;
+  const int rows = 16 * plan.row_groups;
+  plan.few_high = !few ? 0 : wide ? rows : INT_MAX;
+  if (few) {
+    const long long tiles = min((long long)tokens * group / rows + n, (long long)n * ((min(most_rows, (long long)plan.few_high) + rows - 1) / rows)) * kv_heads;
+    const long long most = tiles * ((keys + PA_TILE - 1) / PA_TILE + PA_PIECE_COST);
+    plan.few_grid = int(max(1LL, min((long long)pa_sms() * (plan.row_groups == 1 ? 2 : 1), (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE)));
+    plan.few_floats = (long long)plan.few_grid * 2 * (rows * (head_dim + 2) + 4);
+  }
+  if (wide) {
+    plan.wide_grid = pw_grid(head_dim);
+    plan.wide_floats = (long long)plan.wide_grid * 2 * (PW_ROWS * (head_dim + 2) + 4);
+  }
+  plan.joins = keys > PA_TILE;  // (a single tile of keys is never cut)
+  return plan;
+}
+static PagedParts pa_parts(float*& room, int grid, int rows, int head_dim) {
+  PagedParts parts;
+  parts.o = room;
+  parts.ml = reinterpret_cast<float2*>(room + (long long)grid * 2 * rows * head_dim);
+  parts.joins = reinterpret_cast<int4*>(parts.ml + (long long)grid * 2 * rows);
+  parts.rows = rows;
+  room += (long long)grid * 2 * (rows * (head_dim + 2) + 4);
+  return parts;
 }
 
 }  // namespace tpb
 
 using namespace tpb;
 
-// CTAs and workspace of a call (bytes, 16-byte aligned); see tpb_paged_attention.
-static void pa_plan(int n, int tokens, int table_width, int page_shift, int most_new, int kv_heads, int group, int head_dim, int* row_groups, int* grid, long long* floats) {
-  const long long most_rows = (long long)min(most_new, tokens) * group;
-  *row_groups = most_rows <= 16 ? 1 : most_rows <= 32 ? 2 : 4;
-  const int rows = 16 * *row_groups;
-  const long long key_tiles = (((long long)table_width << page_shift) + PA_TILE - 1) / PA_TILE;
-  const long long row_tiles = (long long)tokens * group / rows + n;  // (at most: one more than full ones per sequence)
-  const long long most = min(row_tiles, (long long)n * ((most_rows + rows - 1) / rows)) * kv_heads * (key_tiles + PA_PIECE_COST);
-  const int resident = pa_sms() * (*row_groups == 1 ? 2 : 1);
-  *grid = int(max(1LL, min((long long)resident, (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE)));
-  *floats = (long long)*grid * 2 * (rows * (head_dim + 2) + 4);
-}
-
 extern "C" long long tpb_paged_attention_workspace(int n, int tokens, int table_width, int page_size, int most_new, int kv_heads, int group, int head_dim) {
-  int row_groups, grid;
-  long long floats;
   int shift = 0;
   while ((1 << shift) < page_size) ++shift;
-  pa_plan(n, tokens, table_width, shift, most_new, kv_heads, group, head_dim, &row_groups, &grid, &floats);
-  return floats * 4;
+  const PagedPlan plan = pa_plan(n, tokens, table_width, shift, most_new, kv_heads, group, head_dim);
+  return (plan.few_floats + plan.wide_floats) * 4;
 }
 
 extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
   if (!a || !a->q || !a->out || !a->keys || !a->values || !a->table || !a->starts || !a->past || !a->status || !a->workspace) return TPB_ERR_ARG;
-  if (a->n < 0 || a->tokens <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || a->pages <= 0 || a->table_width <= 0 || a->window < 0 ||
+  if (a->n <= 0 || a->tokens <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || a->pages <= 0 || a->table_width <= 0 || a->window < 0 ||
       a->most_new < 0)
     return TPB_ERR_ARG;
   if ((a->head_dim != 64 && a->head_dim != 128) || a->page_size < 16 || (a->page_size & (a->page_size - 1))) return TPB_ERR_ARG;
-  if ((long long)a->tokens * a->heads > INT_MAX / 2) return TPB_ERR_SIZE;
+  if ((long long)a->tokens * a->heads >= 1 << 30) return TPB_ERR_SIZE;
   const uintptr_t addresses = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(a->keys) |
                               reinterpret_cast<uintptr_t>(a->values) | reinterpret_cast<uintptr_t>(a->workspace);
   if ((addresses & 15) || ((a->q_st | a->q_sh | a->o_st | a->o_sh | a->k_sp | a->k_sh | a->k_ss | a->v_sp | a->v_sh | a->v_ss) & 7)) return TPB_ERR_ALIGN;
   int rc = fa_bind_thread();
   if (rc != TPB_OK) return rc;
-  PagedAttnParams p = {};
   int shift = 0;
   while ((1 << shift) < a->page_size) ++shift;
+  const int group = a->heads / a->kv_heads;
+  const PagedPlan plan = pa_plan(a->n, a->tokens, a->table_width, shift, a->most_new, a->kv_heads, group, a->head_dim);
+  if (a->workspace_bytes < (plan.few_floats + plan.wide_floats) * 4) return TPB_ERR_WORKSPACE;
+  PagedAttnParams p = {};
   p.b = {a->starts, a->past, a->table, a->table_ld, a->n, a->tokens, a->table_width, a->pages, shift, a->most_new, static_cast<uint32_t*>(a->status)};
   p.q = static_cast<const bf16*>(a->q);
   p.out = static_cast<bf16*>(a->out);
   p.q_st = a->q_st, p.q_sh = a->q_sh, p.o_st = a->o_st, p.o_sh = a->o_sh;
-  p.heads = a->heads, p.kv_heads = a->kv_heads, p.group = a->heads / a->kv_heads, p.window = a->window;
-  p.fill_rest = a->fill_rest;
+  p.heads = a->heads, p.kv_heads = a->kv_heads, p.group = group, p.window = a->window;
   p.scale_log2e = a->scale * 1.4426950408889634f;
-  p.rows_low = 1;
-  p.rows_high = INT_MAX;
-  p.takes_bad = 1;
-  int row_groups, grid;
-  long long floats;
-  pa_plan(a->n, a->tokens, a->table_width, shift, a->most_new, p.kv_heads, p.group, a->head_dim, &row_groups, &grid, &floats);
-  if (a->workspace_bytes < floats * 4) return TPB_ERR_WORKSPACE;
-  const int rows = 16 * row_groups;
-  p.part_o = static_cast<float*>(a->workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (long long)grid * 2 * rows * a->head_dim);
-  p.joins = reinterpret_cast<int4*>(p.part_ml + (long long)grid * 2 * rows);
-  CUtensorMap k, v;
-  const int box = min(a->page_size, PA_TILE);
-  rc = paged_tmap(&k, a->keys, a->head_dim, a->page_size, a->kv_heads, a->pages, a->k_ss, a->k_sh, a->k_sp, box);
-  if (rc == TPB_OK) rc = paged_tmap(&v, a->values, a->head_dim, a->page_size, a->kv_heads, a->pages, a->v_ss, a->v_sh, a->v_sp, box);
-  if (rc != TPB_OK) return rc;
-  const bool joins = ((long long)a->table_width << shift) > PA_TILE;  // (a single tile of keys is never cut)
+  float* room = static_cast<float*>(a->workspace);
+  const PagedParts few = pa_parts(room, plan.few_grid, 16 * plan.row_groups, a->head_dim), wide = pa_parts(room, plan.wide_grid, PW_ROWS, a->head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
-#define PA_LAUNCH(D)                                                                                       \
-  return row_groups == 1 ? pa_few_launch<D, 1>(p, k, v, grid, joins, s)                                    \
-                         : row_groups == 2 ? pa_few_launch<D, 2>(p, k, v, grid, joins, s) : pa_few_launch<D, 4>(p, k, v, grid, joins, s)
-  if (a->head_dim == 64) PA_LAUNCH(64);
-  PA_LAUNCH(128);
+  auto maps = [&](CUtensorMap& k, CUtensorMap& v, int tile) {
+    const int box = min(a->page_size, tile);
+    const int r = paged_tmap(&k, a->keys, a->head_dim, a->page_size, a->kv_heads, a->pages, a->k_ss, a->k_sh, a->k_sp, box);
+    return r != TPB_OK ? r : paged_tmap(&v, a->values, a->head_dim, a->page_size, a->kv_heads, a->pages, a->v_ss, a->v_sh, a->v_sp, box);
+  };
+  CUtensorMap k, v;
+  if (plan.few_grid) {
+    rc = maps(k, v, PA_TILE);
+    if (rc != TPB_OK) return rc;
+    p.parts = few;
+    p.rows_low = 1, p.rows_high = plan.few_high;
+    p.takes_bad = 1;
+    p.fill_rest = a->fill_rest;
+#define PA_LAUNCH(D) \
+  (plan.row_groups == 1 ? pa_few_launch<D, 1>(p, k, v, plan.few_grid, s) : plan.row_groups == 2 ? pa_few_launch<D, 2>(p, k, v, plan.few_grid, s) : pa_few_launch<D, 4>(p, k, v, plan.few_grid, s))
+    rc = a->head_dim == 64 ? PA_LAUNCH(64) : PA_LAUNCH(128);
 #undef PA_LAUNCH
+    if (rc != TPB_OK) return rc;
+  }
+  if (plan.wide_grid) {
+    if (!plan.few_grid || a->page_size > PA_TILE) rc = maps(k, v, pw_tile(a->head_dim));
+    if (rc != TPB_OK) return rc;
+    p.parts = wide;
+    p.rows_low = plan.few_high + 1, p.rows_high = INT_MAX;
+    p.takes_bad = plan.few_grid == 0;
+    p.fill_rest = a->fill_rest && !plan.few_grid;
+    rc = pw_launch(a->head_dim, p, k, v, plan.wide_grid, plan.few_grid != 0, s);
+    if (rc != TPB_OK) return rc;
+  }
+  if (!plan.joins) return TPB_OK;
+  const int rows = plan.wide_grid ? PW_ROWS : int(min((long long)few.rows, max(1LL, (long long)min(a->most_new, a->tokens) * group)));
+  const dim3 grid(plan.few_grid + plan.wide_grid, min(16, (rows * (a->head_dim / 4) + PA_JOIN_THREADS - 1) / PA_JOIN_THREADS));
+  const cudaError_t launched =
+      a->head_dim == 64 ? launch_dependent(paged_attn_join_kernel<64>, grid, dim3(PA_JOIN_THREADS), 0, s, true, p, few, plan.few_grid, wide)
+                        : launch_dependent(paged_attn_join_kernel<128>, grid, dim3(PA_JOIN_THREADS), 0, s, true, p, few, plan.few_grid, wide);
+  return launched == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
