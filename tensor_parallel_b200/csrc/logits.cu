@@ -2,10 +2,10 @@
 //
 //   seen:  x = x > 0 ? x / repetition : x * repetition;   x -= frequency * count + presence * (count > 0);   x += bias;   not allowed: -inf
 //
-// Bound by memory: each logit is read once and written once.  A block has a slice of one row's vocabulary; it counts the tokens of that slice in shared memory
-// (a 32-bit word per entry: the top bit for a token that was seen at all, the rest for how often it was said) by walking the row's whole history, which
-// the other slices of the row find in L2, and then passes over its logits.  Integer atomics: the counts do not depend on their order.  Long slices walk
-// the history less often, short ones fill the GPU when there are few rows.
+// Bound by memory: each logit is read once and written once.  A block has a slice of one row's vocabulary, up to eight 16-byte vectors per thread, which are on
+// their way to registers while it counts the tokens of that slice in shared memory (a 32-bit word per entry: the top bit for a token that was seen at all, the
+// rest for how often it was said) by walking the row's whole history, which the other slices of the row find in L2.  Integer atomics: the counts do not depend
+// on their order.  Long slices walk the history less often, short ones fill the GPU when there are few rows.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -30,7 +30,7 @@ struct LogitsParams {
   const uint32_t* allowed;
   uint32_t* status;
   long long logits_ld, out_ld, tokens_ld, bias_ld, allowed_ld;
-  int vocab, width, slice, bias_fp32;
+  int vocab, width, bias_fp32;
   float repetition_all, frequency_all, presence_all;
 };
 
@@ -46,19 +46,62 @@ __device__ __forceinline__ float lg_load(const bf16* p) { return __bfloat162floa
 __device__ __forceinline__ void lg_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void lg_store(bf16* p, float v) { *p = __float2bfloat16(v); }
 
-// WIDE: logits and results of a row lie alike to a 16-byte boundary, and go in 16-byte vectors; else one by one.
-template <typename T, bool WIDE>
+// Elements at, at + 1, ... of a row of numbers, `n` of them in [0, limit); one vector where the address allows.
+template <int N>
+__device__ __forceinline__ void lg_numbers(const float* row, int at, int limit, float (&v)[N]) {
+  if (N > 1 && at >= 0 && at + N <= limit && !(reinterpret_cast<uintptr_t>(row + at) & 15)) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(row + at + i));
+      v[i] = f.x;
+      if (N > 1) v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = at + i >= 0 && at + i < limit ? __ldg(row + at + i) : 0.f;
+}
+
+// WIDE: logits and results of a row lie alike to a 16-byte boundary, and go in 16-byte vectors of the row's own grid, of which the first may begin in front of a
+// slice's row and the last end behind it; else one by one.
+template <typename T, bool WIDE, int VECTORS>
 __global__ void __launch_bounds__(LG_THREADS)
 adjust_logits_kernel(const LogitsParams p) {
   extern __shared__ uint32_t counts[];
-  constexpr int N = WIDE ? Vec<T>::N : 1;
+  constexpr int N = WIDE ? Vec<T>::N : 1, SLICE = LG_THREADS * N * VECTORS;
   const long long row = blockIdx.x;
-  const int begin = blockIdx.y * p.slice, end = min(p.vocab, begin + p.slice);
   const T* x = static_cast<const T*>(p.logits) + row * p.logits_ld;
   T* y = static_cast<T*>(p.out) + row * p.out_ld;
+  const int skew = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % N);
+  const int begin = blockIdx.y * SLICE - skew;  // (the first slice begins up to N - 1 in front of the row)
+  const int mine = begin + int(threadIdx.x) * N;
+  uint4 raw[WIDE ? VECTORS : 1];
+  float single[WIDE ? 1 : VECTORS];
+#pragma unroll
+  for (int j = 0; j < VECTORS; ++j) {
+    const int at = mine + j * (LG_THREADS * N);
+    if (WIDE) {
+      T* v = reinterpret_cast<T*>(&raw[WIDE ? j : 0]);
+      if (at >= 0 && at + N <= p.vocab) {
+        raw[WIDE ? j : 0] = *reinterpret_cast<const uint4*>(x + at);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (at + i >= 0 && at + i < p.vocab) v[i] = x[at + i];
+      }
+    } else if (at < p.vocab) {
+      single[WIDE ? 0 : j] = lg_load(x + at);
+    }
+  }
   const bool history = p.tokens != nullptr;
   if (history) {
-    for (int i = threadIdx.x; i < end - begin; i += LG_THREADS) counts[i] = 0;
+#pragma unroll
+    for (int i = 0; i < N * VECTORS; i += 4) {
+      if (N * VECTORS >= 4)
+        *reinterpret_cast<uint4*>(counts + (i * LG_THREADS + int(threadIdx.x) * 4)) = make_uint4(0, 0, 0, 0);
+    }
+    if (N * VECTORS < 4)
+      for (int i = threadIdx.x; i < SLICE; i += LG_THREADS) counts[i] = 0;
     int length = p.lengths ? __ldg(p.lengths + row) : p.width;
     const int prompt = p.prompts ? __ldg(p.prompts + row) : 0;
     if (length < 0 || length > p.width || prompt < 0) {
@@ -67,9 +110,10 @@ adjust_logits_kernel(const LogitsParams p) {
     }
     __syncthreads();
     const long long* said = p.tokens + row * p.tokens_ld;
-    for (int i = threadIdx.x; i < length; i += LG_THREADS) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.width; i += LG_THREADS) {
       const long long token = __ldg(said + i);
-      if (token >= begin && token < end) {
+      if (i < length && token >= max(begin, 0) && token < min((long long)p.vocab, (long long)begin + SLICE)) {
         if (i < prompt)
           atomicOr(&counts[token - begin], 0x80000000u);
         else
@@ -82,54 +126,96 @@ adjust_logits_kernel(const LogitsParams p) {
   const float frequency = p.frequency ? __ldg(p.frequency + row) : p.frequency_all;
   const float presence = p.presence ? __ldg(p.presence + row) : p.presence_all;
   const uint32_t* allowed = p.allowed ? p.allowed + row * p.allowed_ld : nullptr;
+  const int words = (p.vocab + 31) / 32;
 
-  auto adjust = [&](float v, int i) {
+#pragma unroll
+  for (int j = 0; j < VECTORS; ++j) {
+    const int at = mine + j * (LG_THREADS * N);
+    if (at >= p.vocab) continue;
+    T* packed = reinterpret_cast<T*>(&raw[WIDE ? j : 0]);
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = WIDE ? lg_load(packed + i) : single[WIDE ? 0 : j];
     if (history) {
-      const uint32_t seen = counts[i - begin];
-      if (seen) {
-        v = v > 0.f ? v / repetition : v * repetition;
-        const uint32_t count = seen & 0x7fffffffu;
-        if (count) v -= frequency * float(count) + presence;
+      uint32_t seen[N], any = 0;
+#pragma unroll
+      for (int i = 0; i < N; i += N < 4 ? 1 : 4) {
+        const uint32_t* from = counts + (at - begin) + i;
+        if (N < 4) {
+          seen[i] = *from;
+        } else {
+          const uint4 u = *reinterpret_cast<const uint4*>(from);
+          seen[i] = u.x, seen[i + (N > 1)] = u.y, seen[i + 2 * (N > 2)] = u.z, seen[i + 3 * (N > 3)] = u.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) any |= seen[i];
+      if (any) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (seen[i]) {
+            v[i] = v[i] > 0.f ? v[i] / repetition : v[i] * repetition;
+            const uint32_t count = seen[i] & 0x7fffffffu;
+            if (count) v[i] -= frequency * float(count) + presence;
+          }
       }
     }
-    if (p.bias) v += p.bias_fp32 ? __ldg(static_cast<const float*>(p.bias) + row * p.bias_ld + i) : __bfloat162float(static_cast<const bf16*>(p.bias)[row * p.bias_ld + i]);
-    if (allowed && !(__ldg(allowed + (i >> 5)) >> (i & 31) & 1u)) v = -INFINITY;
-    return v;
-  };
-  if (!WIDE) {
-    for (int i = begin + threadIdx.x; i < end; i += LG_THREADS) lg_store(y + i, adjust(lg_load(x + i), i));
-    return;
-  }
-  // vectors of the row's own 16-byte grid: the first may begin in front of the slice, the last end behind it
-  const int skew = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % N);
-  for (int at = (begin + skew) / N * N - skew + int(threadIdx.x) * N; at < end; at += LG_THREADS * N) {
-    if (at >= begin && at + N <= end) {
-      uint4 u = *reinterpret_cast<const uint4*>(x + at);
-      T* v = reinterpret_cast<T*>(&u);
+    if (p.bias) {
+      if (p.bias_fp32) {
+        float b[N];
+        lg_numbers<N>(static_cast<const float*>(p.bias) + row * p.bias_ld, at, p.vocab, b);
 #pragma unroll
-      for (int i = 0; i < N; ++i) lg_store(v + i, adjust(lg_load(v + i), at + i));
-      *reinterpret_cast<uint4*>(y + at) = u;
+        for (int i = 0; i < N; ++i) v[i] += b[i];
+      } else {
+        const bf16* b = static_cast<const bf16*>(p.bias) + row * p.bias_ld;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (at + i >= 0 && at + i < p.vocab) v[i] += __bfloat162float(b[at + i]);
+      }
+    }
+    if (allowed) {
+      // bits of tokens at, at + 1, ...: from two words (the vector may cross their border, and begin in front of the first)
+      const int word = at >> 5;
+      const uint32_t low = word >= 0 ? __ldg(allowed + word) : 0u, high = word + 1 < words ? __ldg(allowed + word + 1) : 0u;
+      const uint32_t bits = __funnelshift_r(low, high, at & 31);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (!(bits >> i & 1u)) v[i] = -INFINITY;
+    }
+    if (WIDE) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) lg_store(packed + i, v[i]);
+      if (at >= 0 && at + N <= p.vocab) {
+        *reinterpret_cast<uint4*>(y + at) = raw[WIDE ? j : 0];
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (at + i >= 0 && at + i < p.vocab) y[at + i] = packed[i];
+      }
     } else {
-      for (int i = max(at, begin); i < min(at + N, end); ++i) lg_store(y + i, adjust(lg_load(x + i), i));
+      lg_store(y + at, v[0]);
     }
   }
 }
 
-template <typename T>
-static int lg_launch(LogitsParams& p, int rows, cudaStream_t stream) {
-  auto grid_place = [](const void* t) { return reinterpret_cast<uintptr_t>(t) / sizeof(T) % Vec<T>::N; };
-  const bool wide = grid_place(p.logits) == grid_place(p.out) && (rows == 1 || p.logits_ld % Vec<T>::N == p.out_ld % Vec<T>::N) && p.logits_ld >= 0;
-  // slices: short enough for a few blocks per SM, long enough that walking the history (one read per 256 tokens and thread) stays below the logits' own
-  p.slice = 8192;
-  while (p.slice > 1024 && (long long)rows * ((p.vocab + p.slice - 1) / p.slice) < 148 * 4) p.slice /= 2;
-  const dim3 grid(rows, (p.vocab + p.slice - 1) / p.slice);
-  if (grid.y > 65535) return TPB_ERR_SIZE;
-  const size_t smem = p.tokens ? p.slice * 4 : 0;
-  if (wide)
-    adjust_logits_kernel<T, true><<<grid, LG_THREADS, smem, stream>>>(p);
-  else
-    adjust_logits_kernel<T, false><<<grid, LG_THREADS, smem, stream>>>(p);
+template <typename T, bool WIDE, int VECTORS>
+static int lg_go(const LogitsParams& p, int rows, cudaStream_t stream) {
+  constexpr int SLICE = LG_THREADS * (WIDE ? Vec<T>::N : 1) * VECTORS;
+  const long long slices = ((long long)p.vocab + (WIDE ? Vec<T>::N - 1 : 0) + SLICE - 1) / SLICE;
+  if (slices > 65535) return TPB_ERR_SIZE;
+  adjust_logits_kernel<T, WIDE, VECTORS><<<dim3(rows, unsigned(slices)), LG_THREADS, p.tokens ? SLICE * 4 : 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+}
+
+template <typename T>
+static int lg_launch(const LogitsParams& p, int rows, cudaStream_t stream) {
+  constexpr int N = Vec<T>::N;
+  auto place = [](const void* t) { return reinterpret_cast<uintptr_t>(t) / sizeof(T) % N; };
+  const bool wide = place(p.logits) == place(p.out) && (rows == 1 || (p.logits_ld - p.out_ld) % N == 0);
+  if (!wide) return lg_go<T, false, 8>(p, rows, stream);
+  const long long vectors = (long long)rows * ((p.vocab + N - 1) / N);
+  if (vectors >= 148LL * 4 * LG_THREADS * 4) return lg_go<T, true, 32 / N>(p, rows, stream);
+  return lg_go<T, true, 1>(p, rows, stream);
 }
 
 }  // namespace tpb
@@ -139,7 +225,7 @@ using namespace tpb;
 extern "C" int tpb_adjust_logits(const tpb_adjust_logits_t* a, void* stream_) {
   if (!a || !a->logits || !a->out || !a->status || a->rows <= 0 || a->vocab <= 0 || a->width < 0 || a->dtype < 0 || a->dtype > 1) return TPB_ERR_ARG;
   LogitsParams p = {a->logits, a->out, a->tokens, a->lengths, a->prompts, a->repetition, a->frequency, a->presence, a->bias, reinterpret_cast<const uint32_t*>(a->allowed),
-                    static_cast<uint32_t*>(a->status), a->logits_ld, a->out_ld, a->tokens_ld, a->bias_ld, a->allowed_ld, a->vocab, a->width, 0, a->bias_dtype,
+                    static_cast<uint32_t*>(a->status), a->logits_ld, a->out_ld, a->tokens_ld, a->bias_ld, a->allowed_ld, a->vocab, a->width, a->bias_dtype,
                     a->repetition_all, a->frequency_all, a->presence_all};
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
   return a->dtype ? lg_launch<float>(p, a->rows, s) : lg_launch<bf16>(p, a->rows, s);

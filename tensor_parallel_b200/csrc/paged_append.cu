@@ -3,10 +3,11 @@
 //   n = x * w / sqrt(mean(x^2) + eps)  (heads with a norm);   (a, b) -> (a cos - b sin, b cos + a sin) * factor  over the pairs of the first rotary_dim elements
 //
 // Bound by memory: every row is read once and written once, 4 bytes per element in all.  A row is a group of head_dim / 8 lanes (a power of two of them) with
-// eight elements each, so that the sum of squares and the partner of a pair come by shuffles; the rows of a token (query, key and value heads)
-// are dealt out to the groups of one block, or of several blocks where there are few tokens.  The angles are common to a token's heads: one thread per
-// frequency evaluates them into shared memory while the rows are on their way.  They are taken modulo a turn in 64 bits (position * frequency in
-// 32 bits is off by position * 2^-24 radians, 0.06 at a million), then by sincospif.  Rounded to bf16 once, at the end.
+// eight elements each, so that the sum of squares and the partner of a pair come by shuffles; the rows (query, key and value heads) of a block's tokens are
+// dealt out to its groups.  A token's place (a search for its sequence, its lengths, its page: four loads behind one another) and its angles are common to its
+// heads: a warp per token looks the place up and a thread per frequency evaluates the angle, while the first rows are on their way.  Many tokens go eight to a
+// block, so that this chain is paid once for 8 x 48 rows; few tokens have several blocks each.  Angles are taken modulo a turn in 64 bits (position *
+// frequency in 32 bits is off by position * 2^-24 radians, 0.06 at a million), then by sincospif.  Rounded to bf16 once, at the end.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -21,6 +22,7 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int AP_THREADS = 256;
 constexpr int AP_MAX_HALF = 128;  // rotary_dim / 2 at head_dim 256
+constexpr int AP_TOKENS = 8;      // of a block, at most: one per warp
 
 struct AppendParams {
   PagedBatch b;
@@ -56,82 +58,98 @@ __device__ __forceinline__ int sequence_of(const PagedBatch& b, int t, int lane)
   return low - 1;
 }
 
+struct AppendPlace {  // of a token
+  int position;
+  int inside;           // of a sequence
+  long long k_at, v_at; // -1: not stored
+};
+
 template <int LANES>
-__global__ void __launch_bounds__(AP_THREADS)
-paged_append_kernel(const AppendParams p) {
-  __shared__ float cos_s[AP_MAX_HALF], sin_s[AP_MAX_HALF];
+__global__ void __launch_bounds__(AP_THREADS, 4)
+paged_append_kernel(const AppendParams p, int tokens_of_block) {
+  __shared__ float cos_s[AP_TOKENS * AP_MAX_HALF], sin_s[AP_TOKENS * AP_MAX_HALF];
+  __shared__ AppendPlace places[AP_TOKENS];
   constexpr int GROUPS = AP_THREADS / LANES;  // rows at a time
-  const int lane = threadIdx.x & 31;
-  const int t = blockIdx.x;
-  const int c = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const int e0 = c * 8;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t0 = blockIdx.x * tokens_of_block, tokens = min(tokens_of_block, p.b.tokens - t0);
+  const int e0 = threadIdx.x % LANES * 8;
   const bool on = e0 < p.head_dim;
   const int rows = p.q_heads + 2 * p.kv_heads;
+  // rows of the block: (token, head), heads fastest, one to a group and round; every lane makes its warp's rounds (the shuffles are the whole warp's)
+  const int all = tokens * rows, stride = gridDim.y * GROUPS;
+  const int i0 = blockIdx.y * GROUPS + threadIdx.x / LANES, first = blockIdx.y * GROUPS + (threadIdx.x & ~31) / LANES;
 
-  auto source = [&](int r) {
+  auto source = [&](int i) {
+    const long long t = t0 + i / rows;
+    const int r = i % rows;
     return r < p.q_heads ? p.q + t * p.q_st + r * p.q_sh
                          : r < p.q_heads + p.kv_heads ? p.k + t * p.k_st + (r - p.q_heads) * p.k_sh : p.v + t * p.v_st + (r - p.q_heads - p.kv_heads) * p.v_sh;
   };
-  // the rows of the first rounds are on their way while the token's place is looked up
   constexpr int AHEAD = 4;
-  const int stride = gridDim.y * GROUPS, r0 = blockIdx.y * GROUPS + group;
   uint4 raw[AHEAD];
+  auto fetch = [&](int from) {
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i)
-    if (on && r0 + i * stride < rows) raw[i] = *reinterpret_cast<const uint4*>(source(r0 + i * stride) + e0);
-
-  const int seq = sequence_of(p.b, t, lane);
-  const bool outside = seq < 0 || seq >= p.b.n;
-  int position = 0;
-  long long k_at = -1, v_at = -1;
-  if (!outside) {
-    const PagedSequence s = paged_sequence(p.b, seq);
-    position = s.past + (t - s.token0);
-    int page = -1;
-    if (!s.bad && t >= s.token0 && t < s.token0 + s.fresh) page = __ldg(p.b.table + seq * p.b.table_ld + (position >> p.b.page_shift));
-    if (page >= 0 && page < p.b.pages) {
-      const int at = position & ((1 << p.b.page_shift) - 1);
-      k_at = page * p.k_sp + at * p.k_ss;
-      v_at = page * p.v_sp + at * p.v_ss;
-    } else if (threadIdx.x == 0 && blockIdx.y == 0) {
-      atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+    for (int j = 0; j < AHEAD; ++j) {
+      const int i = from + j * stride;
+      if (on && i < all) raw[j] = *reinterpret_cast<const uint4*>(source(i) + e0);
     }
+  };
+  fetch(i0);
+
+  if (warp < tokens) {
+    const int t = t0 + warp, seq = sequence_of(p.b, t, lane);
+    AppendPlace at = {0, seq >= 0 && seq < p.b.n, -1, -1};
+    if (at.inside) {
+      const PagedSequence s = paged_sequence(p.b, seq);
+      at.position = s.past + (t - s.token0);
+      int page = -1;
+      if (!s.bad && t >= s.token0 && t < s.token0 + s.fresh) page = __ldg(p.b.table + seq * p.b.table_ld + (at.position >> p.b.page_shift));
+      if (page >= 0 && page < p.b.pages) {
+        const int slot = at.position & ((1 << p.b.page_shift) - 1);
+        at.k_at = page * p.k_sp + slot * p.k_ss;
+        at.v_at = page * p.v_sp + slot * p.v_ss;
+      } else if (lane == 0 && blockIdx.y == 0) {
+        atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+      }
+    }
+    if (lane == 0) places[warp] = at;
   }
-  if (outside && !p.fill_rest) return;  // (of the whole block: the token is)
-  for (int i = threadIdx.x; i < p.half; i += AP_THREADS) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < tokens * p.half; i += AP_THREADS) {
+    const int t = i / p.half, f = i % p.half;
     // turns = position * f / (2 pi), less whole turns
-    double turns = double(position) * (double(p.frequencies[i]) * 0.15915494309189533577);
+    double turns = double(places[t].position) * (double(__ldg(p.frequencies + f)) * 0.15915494309189533577);
     turns -= rint(turns);
     float sn, cs;
     sincospif(float(2.0 * turns), &sn, &cs);
-    cos_s[i] = cs * p.factor;
-    sin_s[i] = sn * p.factor;
+    cos_s[t * AP_MAX_HALF + f] = cs * p.factor;
+    sin_s[t * AP_MAX_HALF + f] = sn * p.factor;
   }
   __syncthreads();
 
-  auto finish = [&](int r, const uint4& u, const bf16* src) {
+  auto finish = [&](int i, const uint4& u) {
+    const bool there = i < all;
+    const int t = there ? i / rows : 0, r = there ? i % rows : 0;
     const bool is_q = r < p.q_heads, is_v = r >= p.q_heads + p.kv_heads;
+    const AppendPlace at = places[t];
     bf16* dst = nullptr;
-    if (r < rows) {
+    if (there && on) {
       if (is_q)
-        dst = p.q_out + t * p.o_st + r * p.o_sh;
-      else if (!is_v && k_at >= 0)
-        dst = p.keys + k_at + (r - p.q_heads) * p.k_shead;
-      else if (is_v && v_at >= 0)
-        dst = p.values + v_at + (r - p.q_heads - p.kv_heads) * p.v_shead;
+        dst = at.inside || p.fill_rest ? p.q_out + (t0 + t) * p.o_st + r * p.o_sh : nullptr;
+      else if (!is_v && at.k_at >= 0)
+        dst = p.keys + at.k_at + (r - p.q_heads) * p.k_shead;
+      else if (is_v && at.v_at >= 0)
+        dst = p.values + at.v_at + (r - p.q_heads - p.kv_heads) * p.v_shead;
     }
-    if (outside) {
-      if (is_q && dst && on) *reinterpret_cast<uint4*>(dst + e0) = make_uint4(0, 0, 0, 0);
-      return;
-    }
+    const float *cs = cos_s + t * AP_MAX_HALF, *sn = sin_s + t * AP_MAX_HALF;
     float x[8] = {};
-    if (on && r < rows) unpack8(u, x);
+    if (on && there) unpack8(u, x);
     const bf16* weight = is_q ? p.q_norm : is_v ? nullptr : p.k_norm;
     float rstd = 1.f;
-    if (p.q_norm || p.k_norm) {  // (all lanes of the warp take part)
+    if (p.q_norm || p.k_norm) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+      for (int j = 0; j < 8; ++j) sum += x[j] * x[j];
 #pragma unroll
       for (int d = LANES / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       if (weight) {
@@ -140,68 +158,64 @@ paged_append_kernel(const AppendParams p) {
           float w[8];
           unpack8(__ldg(reinterpret_cast<const uint4*>(weight + e0)), w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= rstd * w[i];
+          for (int j = 0; j < 8; ++j) x[j] *= rstd * w[j];
         }
       }
     }
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i];
     if (p.half && p.interleaved) {
       if (!is_v) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int f = e0 / 2 + i;
+        for (int j = 0; j < 4; ++j) {
+          const int f = e0 / 2 + j;
           if (f < p.half) {
-            const float cs = cos_s[f], sn = sin_s[f];
-            y[2 * i] = x[2 * i] * cs - x[2 * i + 1] * sn;
-            y[2 * i + 1] = x[2 * i + 1] * cs + x[2 * i] * sn;
+            const float a = x[2 * j], b = x[2 * j + 1];
+            x[2 * j] = a * cs[f] - b * sn[f];
+            x[2 * j + 1] = b * cs[f] + a * sn[f];
           }
         }
       }
     } else if (p.half && p.half % 8 == 0) {
       const int step = p.half / 8;  // lanes between the elements of a pair
-      const bool second = e0 >= p.half;
-      const int from = second ? lane - step : lane + step;
+      const bool second = e0 >= p.half, turns = !is_v && e0 < 2 * p.half;
+      const int from = (second ? lane - step : lane + step) & 31, f0 = second ? e0 - p.half : e0;
+      // (a, b) -> (a cos - b sin, b cos + a sin): the second of a pair adds what the first subtracts
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float other = __shfl_sync(0xffffffffu, x[i], from & 31);
-        if (!is_v && e0 < 2 * p.half) {
-          const int f = second ? e0 - p.half + i : e0 + i;
-          y[i] = second ? x[i] * cos_s[f] + other * sin_s[f] : x[i] * cos_s[f] - other * sin_s[f];
+      for (int j = 0; j < 8; j += 4) {
+        const float4 c = turns ? *reinterpret_cast<const float4*>(cs + f0 + j) : make_float4(1.f, 1.f, 1.f, 1.f);
+        const float4 s = turns ? *reinterpret_cast<const float4*>(sn + f0 + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float cj[4] = {c.x, c.y, c.z, c.w}, sj[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float other = __shfl_sync(0xffffffffu, x[j + k], from);
+          if (turns) x[j + k] = x[j + k] * cj[k] + (second ? other : -other) * sj[k];
         }
       }
     } else if (p.half) {
       // pairs that do not lie a multiple of eight elements apart: the partners come from memory once more, before any lane of the warp stores
-      if (!is_v && on && r < rows) {
+      if (!is_v && on && there) {
+        const bf16* src = source(i);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int e = e0 + i;
+        for (int j = 0; j < 8; ++j) {
+          const int e = e0 + j;
           if (e < 2 * p.half) {
             const bool second = e >= p.half;
             const int other = second ? e - p.half : e + p.half, f = second ? other : e;
             float o = __bfloat162float(src[other]);
             if (weight) o *= rstd * __bfloat162float(weight[other]);
-            y[i] = second ? x[i] * cos_s[f] + o * sin_s[f] : x[i] * cos_s[f] - o * sin_s[f];
+            x[j] = second ? x[j] * cs[f] + o * sn[f] : x[j] * cs[f] - o * sn[f];
           }
         }
       }
       __syncwarp();
     }
-    if (dst && on) *reinterpret_cast<uint4*>(dst + e0) = pack8(y);
+    if (dst) *reinterpret_cast<uint4*>(dst + e0) = at.inside ? pack8(x) : make_uint4(0, 0, 0, 0);
   };
 
-  // (every lane makes the same rounds: the shuffles are the whole warp's)
-  const int first = blockIdx.y * GROUPS + (threadIdx.x & ~31) / LANES;  // row of the warp's first group
+  for (int base = 0; first + base < all; base += AHEAD * stride) {
+    if (base) fetch(i0 + base);
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i)
-    if (first + i * stride < rows) finish(r0 + i * stride, raw[i], r0 + i * stride < rows ? source(r0 + i * stride) : nullptr);
-  for (int i = AHEAD; first + i * stride < rows; ++i) {
-    const int r = r0 + i * stride;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    const bf16* src = r < rows ? source(r) : nullptr;
-    if (on && src) u = *reinterpret_cast<const uint4*>(src + e0);
-    finish(r, u, src);
+    for (int j = 0; j < AHEAD; ++j)
+      if (first + base + j * stride < all) finish(i0 + base + j * stride, raw[j]);
   }
 }
 
@@ -234,16 +248,15 @@ extern "C" int tpb_paged_append(const tpb_paged_append_t* a, void* stream_) {
   p.factor = a->factor, p.eps = a->eps;
   const int lanes = a->head_dim <= 64 ? 8 : a->head_dim <= 128 ? 16 : 32;
   const int rows = p.q_heads + 2 * p.kv_heads, groups = AP_THREADS / lanes;
-  const int rounds = (rows + groups - 1) / groups;
-  // few tokens: a token's rows over several blocks
-  const int split = a->tokens >= 148 * 4 ? 1 : rounds;
-  const dim3 grid(a->tokens, split);
+  // tokens to a block where that leaves four blocks to an SM and more, else a token's rows over several blocks
+  const int per_block = a->tokens >= 148 * 4 * AP_TOKENS ? AP_TOKENS : a->tokens >= 148 * 4 * 2 ? 2 : 1;
+  const dim3 grid((a->tokens + per_block - 1) / per_block, a->tokens >= 148 * 4 ? 1 : (rows + groups - 1) / groups);
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
   if (lanes == 8)
-    paged_append_kernel<8><<<grid, AP_THREADS, 0, s>>>(p);
+    paged_append_kernel<8><<<grid, AP_THREADS, 0, s>>>(p, per_block);
   else if (lanes == 16)
-    paged_append_kernel<16><<<grid, AP_THREADS, 0, s>>>(p);
+    paged_append_kernel<16><<<grid, AP_THREADS, 0, s>>>(p, per_block);
   else
-    paged_append_kernel<32><<<grid, AP_THREADS, 0, s>>>(p);
+    paged_append_kernel<32><<<grid, AP_THREADS, 0, s>>>(p, per_block);
   return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }

@@ -364,22 +364,25 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         cp_async16(smem_u32(q_s + t * Q_BYTES + (e >> 3) * (PW_M * 128) + r * 128 + (((e & 7) ^ (r & 7)) << 4)), src, 16);
       }
     };
+    auto announce_rows = [&]() {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[t]);
+    };
     int s_count = 0, o_count = 0;
-    bool fetched = false, ok = true;
+    bool announced = false, ok = true;
     for (int i = 0; ok; ++i) {
       ok = wait_all(&piece_full[i % PW_PIECES], (i / PW_PIECES) & 1);
       if (!ok) break;
       const WidePiece pc = pieces[i % PW_PIECES];
       if (max(pc.n[0], pc.n[1]) == 0) break;
       const int n = pc.n[t];
-      if (n > 0) {
-        if (!fetched) fetch_rows(pc);
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[t]);
+      if (n > 0 && !announced) {
+        fetch_rows(pc);
+        announce_rows();
       }
-      fetched = false;
+      announced = false;
       const int here = pc.row0 + t * PW_M + row;  // row of the sequence
       const int pos = pc.past + here / p.group;
       const int least_pos = pc.past + (pc.row0 + t * PW_M) / p.group, most_pos = pc.past + (pc.row0 + t * PW_M + PW_M - 1) / p.group;
@@ -466,7 +469,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const WidePiece& next = pieces[ni % PW_PIECES];
         if (next.n[t] > 0) {
           fetch_rows(next);
-          fetched = true;
+          announced = true;
         }
       }
       // ---- the result, or this piece of it ----
@@ -475,6 +478,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         if (!ok) break;
         tc_fence_after();
       }
+      if (announced) announce_rows();  // (their scores may come while the results leave: the products with them wait for the probabilities)
       const bool poisoned = reinterpret_cast<volatile int*>(lost)[i % PW_PIECES] == i + 1;
       if (m_run == -INFINITY) l_run = 0.f;
       if (poisoned) l_run = __uint_as_float(0x7fc00000u);
@@ -483,6 +487,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
         const int token = here / p.group, head = here % p.group;
         bf16* to = p.out + (long long)(pc.token0 + token) * p.o_st + (long long)(pc.kvh * p.group + head) * p.o_sh;
+        const bool sectors = (reinterpret_cast<uintptr_t>(to) & 31) == 0;  // (whole sectors leave at once)
         float* part = p.parts.o + ((long long)max(pc.slot, 0) * PW_ROWS + t * PW_M + row) * D;
 #pragma unroll
         for (int c = 0; c < D; c += W) {
@@ -496,7 +501,13 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           }
           if (mine && pc.slot >= 0) {
 #pragma unroll
-            for (int x = 0; x < W; x += 4) *reinterpret_cast<uint4*>(part + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+            for (int x = 0; x < W; x += 8) st_global_v8(part + c + x, o + x);
+          } else if (mine && sectors) {
+            uint32_t w[W / 2];
+#pragma unroll
+            for (int x = 0; x < W / 2; ++x) w[x] = pack_bf16x2(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv);
+#pragma unroll
+            for (int x = 0; x < W / 2; x += 8) st_global_v8(to + c + 2 * x, w + x);
           } else if (mine) {
 #pragma unroll
             for (int x = 0; x < W; x += 8)
