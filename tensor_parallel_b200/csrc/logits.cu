@@ -2,14 +2,17 @@
 //
 //   seen:  x = x > 0 ? x / repetition : x * repetition;   x -= frequency * count + presence * (count > 0);   x += bias;   not allowed: -inf
 //
-// Bound by memory: each logit is read once and written once.  A block has a slice of one row's vocabulary, up to eight 16-byte vectors per thread, which are on
-// their way to registers while it counts the tokens of that slice in shared memory (a 32-bit word per entry: the top bit for a token that was seen at all, the
-// rest for how often it was said) by walking the row's whole history, which the other slices of the row find in L2.  Integer atomics: the counts do not depend
-// on their order.  Long slices walk the history less often, short ones fill the GPU when there are few rows.
+// Bound by memory: each logit is read once and written once.  A block has a part of one row's vocabulary.  It counts the tokens of that part in shared memory (a
+// 32-bit word per entry: the top bit for a token that was seen at all, the rest for how often it was said) by walking the row's whole history, which the other
+// blocks of the row find in L2, and then streams its logits, four 16-byte vectors per thread on their way at a time, the first of them during the count.  Integer
+// atomics: the counts do not depend on their order.  Parts are as long as leaves three blocks to an SM: the walk, a chain of loads that nothing hides, is then
+// paid once (128 x 65024 fp32, 1000 tokens: parts of 1024 to 8192 entries in registers 28 to 33 us, 12 us without the walk).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <atomic>
 
 #include "ptx_sm100.cuh"
 #include "tpb_api.h"
@@ -30,7 +33,7 @@ struct LogitsParams {
   const uint32_t* allowed;
   uint32_t* status;
   long long logits_ld, out_ld, tokens_ld, bias_ld, allowed_ld;
-  int vocab, width, bias_fp32;
+  int vocab, width, bias_fp32, part;
   float repetition_all, frequency_all, presence_all;
 };
 
@@ -62,46 +65,39 @@ __device__ __forceinline__ void lg_numbers(const float* row, int at, int limit, 
   for (int i = 0; i < N; ++i) v[i] = at + i >= 0 && at + i < limit ? __ldg(row + at + i) : 0.f;
 }
 
-// WIDE: logits and results of a row lie alike to a 16-byte boundary, and go in 16-byte vectors of the row's own grid, of which the first may begin in front of a
-// slice's row and the last end behind it; else one by one.
-template <typename T, bool WIDE, int VECTORS>
+constexpr int LG_DEPTH = 4;         // vectors of a thread on their way
+constexpr int LG_MOST_ENTRIES = 16384;  // of a part: 64 KB of counts, three blocks per SM
+
+// WIDE: logits and results of a row lie alike to a 16-byte boundary, and go in 16-byte vectors of the row's own grid, of which the first may begin in front of the
+// row and the last end behind it; else one by one.
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(LG_THREADS)
 adjust_logits_kernel(const LogitsParams p) {
-  extern __shared__ uint32_t counts[];
-  constexpr int N = WIDE ? Vec<T>::N : 1, SLICE = LG_THREADS * N * VECTORS;
+  extern __shared__ __align__(16) uint32_t counts[];
+  constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * N;
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.logits) + row * p.logits_ld;
   T* y = static_cast<T*>(p.out) + row * p.out_ld;
   const int skew = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % N);
-  const int begin = blockIdx.y * SLICE - skew;  // (the first slice begins up to N - 1 in front of the row)
+  const int begin = blockIdx.y * p.part - skew, end = int(min((long long)p.vocab, (long long)begin + p.part));  // (the first part begins up to N - 1 in front of the row)
   const int mine = begin + int(threadIdx.x) * N;
-  uint4 raw[WIDE ? VECTORS : 1];
-  float single[WIDE ? 1 : VECTORS];
+  uint4 raw[LG_DEPTH];
+  auto fetch = [&](uint4& u, int at) {
+    T* v = reinterpret_cast<T*>(&u);
+    if (WIDE && at >= 0 && at + N <= p.vocab) {
+      u = __ldcs(reinterpret_cast<const uint4*>(x + at));
+    } else {
 #pragma unroll
-  for (int j = 0; j < VECTORS; ++j) {
-    const int at = mine + j * (LG_THREADS * N);
-    if (WIDE) {
-      T* v = reinterpret_cast<T*>(&raw[WIDE ? j : 0]);
-      if (at >= 0 && at + N <= p.vocab) {
-        raw[WIDE ? j : 0] = *reinterpret_cast<const uint4*>(x + at);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (at + i >= 0 && at + i < p.vocab) v[i] = x[at + i];
-      }
-    } else if (at < p.vocab) {
-      single[WIDE ? 0 : j] = lg_load(x + at);
+      for (int i = 0; i < N; ++i)
+        if (at + i >= 0 && at + i < p.vocab) v[i] = x[at + i];
     }
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < LG_DEPTH; ++j)
+    if (mine + j * ROUND < end) fetch(raw[j], mine + j * ROUND);
   const bool history = p.tokens != nullptr;
   if (history) {
-#pragma unroll
-    for (int i = 0; i < N * VECTORS; i += 4) {
-      if (N * VECTORS >= 4)
-        *reinterpret_cast<uint4*>(counts + (i * LG_THREADS + int(threadIdx.x) * 4)) = make_uint4(0, 0, 0, 0);
-    }
-    if (N * VECTORS < 4)
-      for (int i = threadIdx.x; i < SLICE; i += LG_THREADS) counts[i] = 0;
+    for (int i = threadIdx.x * 4; i < p.part; i += LG_THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
     int length = p.lengths ? __ldg(p.lengths + row) : p.width;
     const int prompt = p.prompts ? __ldg(p.prompts + row) : 0;
     if (length < 0 || length > p.width || prompt < 0) {
@@ -113,7 +109,7 @@ adjust_logits_kernel(const LogitsParams p) {
 #pragma unroll 4
     for (int i = threadIdx.x; i < p.width; i += LG_THREADS) {
       const long long token = __ldg(said + i);
-      if (i < length && token >= max(begin, 0) && token < min((long long)p.vocab, (long long)begin + SLICE)) {
+      if (i < length && token >= max(begin, 0) && token < end) {
         if (i < prompt)
           atomicOr(&counts[token - begin], 0x80000000u);
         else
@@ -128,14 +124,11 @@ adjust_logits_kernel(const LogitsParams p) {
   const uint32_t* allowed = p.allowed ? p.allowed + row * p.allowed_ld : nullptr;
   const int words = (p.vocab + 31) / 32;
 
-#pragma unroll
-  for (int j = 0; j < VECTORS; ++j) {
-    const int at = mine + j * (LG_THREADS * N);
-    if (at >= p.vocab) continue;
-    T* packed = reinterpret_cast<T*>(&raw[WIDE ? j : 0]);
+  auto adjust = [&](uint4 taken, int at) {
+    T* packed = reinterpret_cast<T*>(&taken);
     float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = WIDE ? lg_load(packed + i) : single[WIDE ? 0 : j];
+    for (int i = 0; i < N; ++i) v[i] = lg_load(packed + i);
     if (history) {
       uint32_t seen[N], any = 0;
 #pragma unroll
@@ -182,28 +175,45 @@ adjust_logits_kernel(const LogitsParams p) {
       for (int i = 0; i < N; ++i)
         if (!(bits >> i & 1u)) v[i] = -INFINITY;
     }
-    if (WIDE) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) lg_store(packed + i, v[i]);
-      if (at >= 0 && at + N <= p.vocab) {
-        *reinterpret_cast<uint4*>(y + at) = raw[WIDE ? j : 0];
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (at + i >= 0 && at + i < p.vocab) y[at + i] = packed[i];
-      }
+    for (int i = 0; i < N; ++i) lg_store(packed + i, v[i]);
+    if (WIDE && at >= 0 && at + N <= p.vocab) {
+      __stcs(reinterpret_cast<uint4*>(y + at), taken);
     } else {
-      lg_store(y + at, v[0]);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (at + i >= 0 && at + i < p.vocab) y[at + i] = packed[i];
+    }
+  };
+  for (int at = mine; at < end; at += LG_DEPTH * ROUND) {
+#pragma unroll
+    for (int j = 0; j < LG_DEPTH; ++j) {
+      const int now = at + j * ROUND, next = now + LG_DEPTH * ROUND;
+      if (now >= end) break;
+      const uint4 taken = raw[j];
+      if (next < end) fetch(raw[j], next);
+      adjust(taken, now);
     }
   }
 }
 
-template <typename T, bool WIDE, int VECTORS>
-static int lg_go(const LogitsParams& p, int rows, cudaStream_t stream) {
-  constexpr int SLICE = LG_THREADS * (WIDE ? Vec<T>::N : 1) * VECTORS;
-  const long long slices = ((long long)p.vocab + (WIDE ? Vec<T>::N - 1 : 0) + SLICE - 1) / SLICE;
-  if (slices > 65535) return TPB_ERR_SIZE;
-  adjust_logits_kernel<T, WIDE, VECTORS><<<dim3(rows, unsigned(slices)), LG_THREADS, p.tokens ? SLICE * 4 : 0, stream>>>(p);
+template <typename T, bool WIDE>
+static int lg_go(LogitsParams p, int rows, cudaStream_t stream) {
+  constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * (N < 4 ? 4 : N);
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TPB_ERR_CUDA;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(adjust_logits_kernel<T, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_MOST_ENTRIES * 4) != cudaSuccess) return TPB_ERR_CUDA;
+    ready[dev].store(true, std::memory_order_release);
+  }
+  // entries of a part: a row's over as many blocks as make three per SM of all rows, whole rounds of the block
+  const long long entries = (long long)p.vocab + N - 1, blocks = max(1LL, 148LL * 3 / rows);
+  const long long part = min((long long)LG_MOST_ENTRIES, ((entries + blocks - 1) / blocks + ROUND - 1) / ROUND * ROUND);
+  const long long parts = (entries + part - 1) / part;
+  if (parts > 65535) return TPB_ERR_SIZE;
+  p.part = int(part);
+  adjust_logits_kernel<T, WIDE><<<dim3(rows, unsigned(parts)), LG_THREADS, p.tokens ? size_t(part) * 4 : 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
@@ -212,10 +222,7 @@ static int lg_launch(const LogitsParams& p, int rows, cudaStream_t stream) {
   constexpr int N = Vec<T>::N;
   auto place = [](const void* t) { return reinterpret_cast<uintptr_t>(t) / sizeof(T) % N; };
   const bool wide = place(p.logits) == place(p.out) && (rows == 1 || (p.logits_ld - p.out_ld) % N == 0);
-  if (!wide) return lg_go<T, false, 8>(p, rows, stream);
-  const long long vectors = (long long)rows * ((p.vocab + N - 1) / N);
-  if (vectors >= 148LL * 4 * LG_THREADS * 4) return lg_go<T, true, 32 / N>(p, rows, stream);
-  return lg_go<T, true, 1>(p, rows, stream);
+  return wide ? lg_go<T, true>(p, rows, stream) : lg_go<T, false>(p, rows, stream);
 }
 
 }  // namespace tpb
@@ -225,7 +232,7 @@ using namespace tpb;
 extern "C" int tpb_adjust_logits(const tpb_adjust_logits_t* a, void* stream_) {
   if (!a || !a->logits || !a->out || !a->status || a->rows <= 0 || a->vocab <= 0 || a->width < 0 || a->dtype < 0 || a->dtype > 1) return TPB_ERR_ARG;
   LogitsParams p = {a->logits, a->out, a->tokens, a->lengths, a->prompts, a->repetition, a->frequency, a->presence, a->bias, reinterpret_cast<const uint32_t*>(a->allowed),
-                    static_cast<uint32_t*>(a->status), a->logits_ld, a->out_ld, a->tokens_ld, a->bias_ld, a->allowed_ld, a->vocab, a->width, a->bias_dtype,
+                    static_cast<uint32_t*>(a->status), a->logits_ld, a->out_ld, a->tokens_ld, a->bias_ld, a->allowed_ld, a->vocab, a->width, a->bias_dtype, 0,
                     a->repetition_all, a->frequency_all, a->presence_all};
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
   return a->dtype ? lg_launch<float>(p, a->rows, s) : lg_launch<bf16>(p, a->rows, s);

@@ -47,4 +47,17 @@ static int paged_tmap(CUtensorMap* map, const void* ptr, int head_dim, int page_
   return fa_tmap(map, ptr, head_dim, rows, page_size, kv_heads, pages, s_slot, s_head, s_page);
 }
 
+// Query rows [tokens][heads][head_dim] (strides positive where there are several); box: 64 elements, the heads of a group, `tokens_of_box` tokens.
+static int paged_rows_tmap(CUtensorMap* map, const void* ptr, int head_dim, int heads, int tokens, long long s_head, long long s_token, int group, int tokens_of_box) {
+  EncodeTiledFn fn = fa_encode_fn();
+  if (!fn) return TPB_ERR_DRIVER;
+  cuuint64_t dims[3] = {cuuint64_t(head_dim), cuuint64_t(heads), cuuint64_t(tokens)};
+  cuuint64_t strides[2] = {cuuint64_t(heads > 1 ? s_head : head_dim) * 2, cuuint64_t(tokens > 1 ? s_token : head_dim) * 2};
+  cuuint32_t box[3] = {64, cuuint32_t(group), cuuint32_t(tokens_of_box)}, estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? TPB_OK
+             : TPB_ERR_TMAP;
+}
+
 }  // namespace tpb

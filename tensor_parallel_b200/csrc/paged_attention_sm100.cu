@@ -6,10 +6,12 @@
 //
 //   work      : (sequence, row tile of 256, KV head, tile of keys) on one line, cut into equal ranges of the resident CTAs (share_out); what is cut goes by the
 //               workspace and the joining kernel.  Ranges balance ragged and causal work, and split long contexts with few rows.
-//   warp 0    : walks the range, one piece ahead of its own loads; announces pieces in a ring of four; keys and values by TMA boxes of a page
+//   warp 3    : walks the range and announces its pieces in a ring of four (64-bit divisions and lengths from memory: 2 us each in front of the loads)
+//   warp 0    : keys and values by TMA boxes of a page, table entries 32 at a time and 32 ahead
 //   warp 1    : issues the MMAs, and writes zeros over values of no key in reach
-//   warps 4-11: softmax, as there; they fetch the rows of the next piece themselves (cp.async, into the room of rows whose last scores are done), so that any
-//               strides and any number of heads in a group will do
+//   warp 2    : query rows, into the room of rows whose last scores are done: a TMA box of (64 elements, the heads of a group, tokens) where 128 rows are
+//               whole tokens, else (7, 12 or 71 heads to a group; rows that repeat) by cp.async.  (Fetched by the softmax warps themselves they were 3 us of theirs per piece)
+//   warps 4-11: softmax, as there; results leave through shared memory in whole lines
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -29,7 +31,8 @@ constexpr int PW_PIECE_COST = 1;  // in tiles: a piece's fill, drain and result
 constexpr int PW_MIN_SHARE = 5;   // a piece and four tiles
 constexpr float PW_RESCALE_LOG2 = 8.f;  // (see attention_sm100.cu: beyond the first 128 keys of a piece, the maximum follows large rises only)
 constexpr int PW_EXACT_KEYS = 128;
-constexpr int PW_PIECES = 4;
+constexpr int PW_PIECES = 4;  // announced at a time
+constexpr int PW_LOST = 8;    // (the loads are three pieces ahead of the results at most: two stages of one tile each)
 
 // D and keys per tile: 128 x 128, one CTA per SM; 64 x 64, two.
 template <int D, int N>
@@ -39,13 +42,15 @@ struct Wide {
   static constexpr int REGS_OTHER = N == 64 ? 32 : 56, REGS_SOFTMAX = N == 64 ? 104 : 224;
   static constexpr int DB = D / 64;
   static constexpr int Q_BYTES = DB * PW_M * 128, T_BYTES = DB * N * 128;
-  static constexpr int SMEM = 1024 + 2 * Q_BYTES + 4 * T_BYTES + 1024;
+  static constexpr int STAGE_BYTES = 4096;  // of a softmax warp: 32 rows of 128 bytes on their way to memory
+  static constexpr int SMEM = 1024 + 2 * Q_BYTES + 4 * T_BYTES + 8 * STAGE_BYTES + 1024;
   static_assert(4 * 32 * REGS_OTHER + 8 * 32 * REGS_SOFTMAX <= (N == 64 ? 80 : 168) * PW_THREADS, "registers of a CTA at its launch");
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 struct WidePiece {
   int token0, row0, rows, past, total, low, kvh, slot;
+  int seq;
   int tile0, n[2];  // first tile of keys, and how many each query tile takes of them; n both 0: no further piece
 };
 
@@ -65,7 +70,8 @@ __device__ __forceinline__ void tm_store(uint32_t at, const uint32_t (&r)[32]) {
 
 template <int D, int N>
 __global__ void __launch_bounds__(PW_THREADS, Wide<D, N>::CTAS)
-paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const PagedAttnParams p) {
+paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                       const PagedAttnParams p, const int boxed) {
   using C = Wide<D, N>;
   constexpr int DB = C::DB, W = C::W;
   constexpr uint32_t Q_BYTES = C::Q_BYTES, T_BYTES = C::T_BYTES;
@@ -79,7 +85,8 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   uint8_t* q_s = smem;                 // [2 tiles]
   uint8_t* k_s = q_s + 2 * Q_BYTES;    // [2 stages]
   uint8_t* v_s = k_s + 2 * T_BYTES;    // [2 stages]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + 2 * T_BYTES);
+  uint8_t* out_s = v_s + 2 * T_BYTES;  // [8 softmax warps]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(out_s + 8 * C::STAGE_BYTES);
   uint64_t* q_full = bars;             // [2 tiles]
   uint64_t* k_full = bars + 2;         // [2 stages]
   uint64_t* k_empty = bars + 4;
@@ -88,33 +95,36 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   uint64_t* s_full = bars + 10;        // [2 tiles]
   uint64_t* p_full = bars + 12;
   uint64_t* o_full = bars + 14;
-  uint64_t* piece_full = bars + 16;    // [PW_PIECES]
-  uint64_t* piece_empty = bars + 16 + PW_PIECES;
-  WidePiece* pieces = reinterpret_cast<WidePiece*>(bars + 16 + 2 * PW_PIECES);  // [PW_PIECES]
-  int* lost = reinterpret_cast<int*>(pieces + PW_PIECES);                       // [PW_PIECES] number (from 1) of a piece of which a page is not there
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(lost + PW_PIECES);
+  uint64_t* q_empty = bars + 16;
+  uint64_t* piece_full = bars + 18;    // [PW_PIECES]
+  uint64_t* piece_empty = bars + 18 + PW_PIECES;
+  WidePiece* pieces = reinterpret_cast<WidePiece*>(bars + 18 + 2 * PW_PIECES);  // [PW_PIECES]
+  int* lost = reinterpret_cast<int*>(pieces + PW_PIECES);                       // [PW_LOST] number (from 1) of a piece of which a page is not there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(lost + PW_LOST);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   __shared__ RangeSearch<PW_THREADS> range;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    if (boxed) prefetch_tmap(&tmap_q);
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&q_full[s], 4);  // one arrival per softmax warp of the tile
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[s], 4);  // one arrival per softmax warp of the tile
       mbar_init(&o_full[s], 1);
     }
     for (int s = 0; s < PW_PIECES; ++s) {
       mbar_init(&piece_full[s], 1);
-      mbar_init(&piece_empty[s], 9);  // MMA warp, softmax warps
-      lost[s] = 0;
+      mbar_init(&piece_empty[s], 11);  // warps 0 to 2, softmax warps
     }
+    for (int s = 0; s < PW_LOST; ++s) lost[s] = 0;
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -166,17 +176,12 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 
   if (warp < 4) {
     setmaxnreg_dec<C::REGS_OTHER>();
-    if (warp == 0) {
-      // ---------------- producer ----------------
-      const int page_size = 1 << p.b.page_shift;
-      const int per_tile = max(1, N >> p.b.page_shift), box_rows = min(page_size, N);
-      const int my_page = lane / DB, my_block = lane % DB;
-      int seq = range.seq, rt = 0, announced = 0, kt = 0;
+    if (warp == 3) {
+      // ---------------- planner: the pieces of the range, up to PW_PIECES ahead ----------------
+      int seq = range.seq, rt = 0;
       long long at = w0, unit_begin = range.begin;  // of the row tile rt of sequence seq
-      bool ok = true;
-      // the next piece of the range into the ring; its sequence, for the table
-      auto announce = [&]() {
-        int of = 0;
+      bool more = true;
+      for (int i = 0; more; ++i) {
         WidePiece o = {};
         while (at < w1 && seq < p.b.n) {
           PagedSequence s;
@@ -193,50 +198,55 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             ++rt;
             continue;
           }
-          const int kvh = int((at - unit_begin) / length), from = int((at - unit_begin) % length), to = int(min((long long)length, from + (w1 - at)));
+          const int into = int(at - unit_begin), kvh = into / length, from = into % length, to = int(min((long long)length, from + (w1 - at)));
           const int t0 = max(0, from - PW_PIECE_COST), t1 = max(0, to - PW_PIECE_COST);
           const long long unit_end = unit_begin + (long long)(kvh + 1) * length;
           at += to - from;
           if (t0 == t1) continue;
-          of = seq;
-          o.token0 = s.token0, o.row0 = rt * PW_ROWS, o.rows = min(PW_ROWS, rows - o.row0), o.past = s.past, o.total = s.past + s.fresh, o.low = low, o.kvh = kvh;
-          o.tile0 = first + t0;
+          o.seq = seq, o.token0 = s.token0, o.row0 = rt * PW_ROWS, o.rows = min(PW_ROWS, rows - o.row0), o.past = s.past, o.total = s.past + s.fresh, o.low = low;
+          o.kvh = kvh, o.tile0 = first + t0;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const int last = min(o.rows, (t + 1) * PW_M) - 1;  // row of the piece
             o.n[t] = last < t * PW_M ? 0 : max(0, min(first + t1, (s.past + (o.row0 + last) / p.group) / N + 1) - o.tile0);
           }
-          o.slot = t0 == 0 && t1 == end - first ? -1 : 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+          o.slot = t0 == 0 && t1 == end - first ? -1 : 2 * int(blockIdx.x) + (t0 == 0 ? 1 : 0);
           if (t0 == 0 && o.slot >= 0 && lane == 0) {
             p.parts.joins[2 * blockIdx.x] = make_int4(o.token0, o.row0, o.rows, kvh);
             p.parts.joins[2 * blockIdx.x + 1] = make_int4(int((unit_end - 1) / share), 0, 0, 0);
           }
           break;
         }
-        const int slot = announced % PW_PIECES;
-        ok = wait_all(&piece_empty[slot], ((announced / PW_PIECES) & 1) ^ 1);
-        if (ok && lane == 0) {
-          pieces[slot] = o;
-          mbar_arrive(&piece_full[slot]);
+        more = max(o.n[0], o.n[1]) > 0;
+        if (!wait_all(&piece_empty[i % PW_PIECES], ((i / PW_PIECES) & 1) ^ 1)) break;
+        if (lane == 0) {
+          pieces[i % PW_PIECES] = o;
+          mbar_arrive(&piece_full[i % PW_PIECES]);
         }
         __syncwarp();
-        ++announced;
-        return of;
-      };
-      int of = announce(), of_next = 0;
+      }
+    } else if (warp == 0) {
+      // ---------------- producer ----------------
+      const int page_size = 1 << p.b.page_shift;
+      const int per_tile = max(1, N >> p.b.page_shift), box_rows = min(page_size, N);
+      const int my_page = lane / DB, my_block = lane % DB;
+      int kt = 0;
+      bool ok = true;
       for (int i = 0; ok; ++i) {
-        const WidePiece pc = pieces[i % PW_PIECES];
-        const int n = max(pc.n[0], pc.n[1]);
+        ok = wait_all(&piece_full[i % PW_PIECES], (i / PW_PIECES) & 1);
+        if (!ok) break;
+        const WidePiece& pc = pieces[i % PW_PIECES];
+        const int n = max(pc.n[0], pc.n[1]), tile0 = pc.tile0, total = pc.total, low = pc.low, kvh = pc.kvh;
+        const int* row = p.b.table + (long long)pc.seq * p.b.table_ld;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&piece_empty[i % PW_PIECES]);
         if (n == 0) break;
-        of_next = announce();  // (before this piece's loads: the softmax warps want to know)
-        const int* row = p.b.table + (long long)of * p.b.table_ld;
-        of = of_next;
-        const int entries = ((pc.total - 1) >> p.b.page_shift) + 1;
-        int entry0 = pc.tile0 * N >> p.b.page_shift;
+        const int entries = ((total - 1) >> p.b.page_shift) + 1;
+        int entry0 = tile0 * N >> p.b.page_shift;
         auto fetch = [&](int e) { return e < entries ? __ldg(row + e) : -1; };
         int now = fetch(entry0 + lane), next = fetch(entry0 + 32 + lane);
         for (int j = 0; ok && j < n; ++j, ++kt) {
-          const int s = kt & 1, key0 = (pc.tile0 + j) * N;
+          const int s = kt & 1, key0 = (tile0 + j) * N;
           const uint32_t par = ((kt >> 1) & 1) ^ 1;
           int e = (key0 >> p.b.page_shift) - entry0;
           if (e >= 32) {
@@ -247,12 +257,12 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           }
           const int page = __shfl_sync(0xffffffffu, now, (e + my_page) & 31);
           const int first = key0 + my_page * page_size;
-          const bool wanted = lane < per_tile * DB && (per_tile == 1 || (first < pc.total && first + page_size > pc.low));
+          const bool wanted = lane < per_tile * DB && (per_tile == 1 || (first < total && first + page_size > low));
           const bool good = wanted && page >= 0 && page < p.b.pages;
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, good)) * box_rows * 128;
           if (__any_sync(0xffffffffu, wanted && !good) && lane == 0) {
             atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
-            lost[i % PW_PIECES] = i + 1;
+            lost[i % PW_LOST] = i + 1;
           }
           const uint32_t to = my_block * (N * 128) + my_page * box_rows * 128;
           const int slot = per_tile == 1 ? key0 & (page_size - 1) : 0;
@@ -260,12 +270,12 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(&k_full[s], bytes);
           __syncwarp();
-          if (good) tma_load_4d(k_s + s * T_BYTES + to, &tmap_k, &k_full[s], my_block * 64, slot, pc.kvh, page);
+          if (good) tma_load_4d(k_s + s * T_BYTES + to, &tmap_k, &k_full[s], my_block * 64, slot, kvh, page);
           ok = wait_all(&v_empty[s], par);
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(&v_full[s], bytes);
           __syncwarp();
-          if (good) tma_load_4d(v_s + s * T_BYTES + to, &tmap_v, &v_full[s], my_block * 64, slot, pc.kvh, page);
+          if (good) tma_load_4d(v_s + s * T_BYTES + to, &tmap_v, &v_full[s], my_block * 64, slot, kvh, page);
         }
       }
     } else if (warp == 1) {
@@ -308,7 +318,10 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         for (int t = 0; t < 2; ++t)
           if (ok && pc.n[t] > 0) {
             ok = arrived(&q_full[t], q_count[t]++ & 1);
-            if (ok) issue_qk(t, kt);
+            if (ok) {
+              issue_qk(t, kt);
+              if (pc.n[t] == 1) umma_commit_lead(leader, &q_empty[t]);
+            }
           }
         if (!ok) break;
         umma_commit_lead(leader, &k_empty[kt & 1]);
@@ -338,11 +351,61 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                   umma_commit_lead(leader, &o_full[t]);
                 else
                   issue_qk(t, kt + 1);
+                if (j == pc.n[t] - 2) umma_commit_lead(leader, &q_empty[t]);  // (those were its last scores)
               }
             }
           if (!ok) break;
           umma_commit_lead(leader, &v_empty[kt & 1]);                 // the values may be overwritten once these MMAs retire
           if (next) umma_commit_lead(leader, &k_empty[(kt + 1) & 1]);  // and the next keys
+        }
+      }
+    } else if (warp == 2) {
+      // ---------------- query rows of the next piece, as soon as the last scores of this one are done ----------------
+      int count[2] = {0, 0};
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        ok = wait_all(&piece_full[i % PW_PIECES], (i / PW_PIECES) & 1);
+        if (!ok) break;
+        const WidePiece& in_ring = pieces[i % PW_PIECES];
+        const int token0 = in_ring.token0, row0 = in_ring.row0, rows = in_ring.rows, kvh = in_ring.kvh, n[2] = {in_ring.n[0], in_ring.n[1]};
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&piece_empty[i % PW_PIECES]);
+        if (max(n[0], n[1]) == 0) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || n[t] == 0) continue;
+          ok = wait_all(&q_empty[t], (count[t]++ & 1) ^ 1);
+          if (!ok) continue;
+          if (boxed) {  // (rows of a box: the heads of a group, tokens)
+            if (lane == 0) {
+              mbar_expect_tx(&q_full[t], Q_BYTES);
+#pragma unroll
+              for (int d = 0; d < DB; ++d)
+                tma_load_3d(q_s + t * Q_BYTES + d * (PW_M * 128), &tmap_q, &q_full[t], d * 64, kvh * p.group, token0 + (row0 + t * PW_M) / p.group);
+            }
+            __syncwarp();
+            continue;
+          }
+          constexpr int STEP = 32 / (D / 8);  // rows at a time
+          const int e = lane % (D / 8), r0 = lane / (D / 8);
+          const int step_tokens = STEP / p.group, step_heads = STEP % p.group;
+          int token = (row0 + t * PW_M + r0) / p.group, head = (row0 + t * PW_M + r0) % p.group;
+          const bf16* base = p.q + (long long)token0 * p.q_st + (long long)kvh * p.group * p.q_sh + e * 8;
+          const uint32_t to = smem_u32(q_s + t * Q_BYTES + (e >> 3) * (PW_M * 128));
+#pragma unroll 4
+          for (int r = r0; r < PW_M; r += STEP) {
+            if (t * PW_M + r < rows) cp_async16(to + r * 128 + (((e & 7) ^ (r & 7)) << 4), base + token * p.q_st + head * p.q_sh, 16);  // (other rows' results go nowhere)
+            token += step_tokens;
+            head += step_heads;
+            if (head >= p.group) {
+              head -= p.group;
+              ++token;
+            }
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full[t]);
         }
       }
     }
@@ -354,35 +417,14 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     const int row = quarter * 32 + lane;
     const uint32_t s_addr = tmem_base + (uint32_t(quarter * 32) << 16) + t * N;  // scores, and in their first half the probabilities
     const uint32_t o_addr = tmem_base + (uint32_t(quarter * 32) << 16) + O_COL0 + t * D;
-    // this warp's 32 query rows of a piece on their way to shared memory
-    auto fetch_rows = [&](const WidePiece& pc) {
-#pragma unroll 4
-      for (int c = lane; c < 32 * (D / 8); c += 32) {
-        const int r = quarter * 32 + c / (D / 8), e = c % (D / 8), in = min(t * PW_M + r, pc.rows - 1);
-        const int token = (pc.row0 + in) / p.group, head = (pc.row0 + in) % p.group;
-        const bf16* src = p.q + (long long)(pc.token0 + token) * p.q_st + (long long)(pc.kvh * p.group + head) * p.q_sh + e * 8;
-        cp_async16(smem_u32(q_s + t * Q_BYTES + (e >> 3) * (PW_M * 128) + r * 128 + (((e & 7) ^ (r & 7)) << 4)), src, 16);
-      }
-    };
-    auto announce_rows = [&]() {
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[t]);
-    };
     int s_count = 0, o_count = 0;
-    bool announced = false, ok = true;
+    bool ok = true;
     for (int i = 0; ok; ++i) {
       ok = wait_all(&piece_full[i % PW_PIECES], (i / PW_PIECES) & 1);
       if (!ok) break;
       const WidePiece pc = pieces[i % PW_PIECES];
       if (max(pc.n[0], pc.n[1]) == 0) break;
       const int n = pc.n[t];
-      if (n > 0 && !announced) {
-        fetch_rows(pc);
-        announce_rows();
-      }
-      announced = false;
       const int here = pc.row0 + t * PW_M + row;  // row of the sequence
       const int pos = pc.past + here / p.group;
       const int least_pos = pc.past + (pc.row0 + t * PW_M) / p.group, most_pos = pc.past + (pc.row0 + t * PW_M + PW_M - 1) / p.group;
@@ -402,7 +444,12 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         if (!plain) {
 #pragma unroll
           for (int c = 0; c < N; ++c)
-            if (c >= visible || c < hidden) r[c] = 0xff800000u;
+            if (c >= visible) r[c] = 0xff800000u;
+          if (hidden > 0) {
+#pragma unroll
+            for (int c = 0; c < N; ++c)
+              if (c < hidden) r[c] = 0xff800000u;
+          }
         }
 #pragma unroll
         for (int c = 0; c < N; c += 4) {
@@ -463,35 +510,27 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
       if (!ok) break;
-      // the rows of the next piece, in the room of this one's: their last scores are done
-      const int ni = i + 1;
-      if (__all_sync(0xffffffffu, mbar_try_wait(&piece_full[ni % PW_PIECES], (ni / PW_PIECES) & 1))) {
-        const WidePiece& next = pieces[ni % PW_PIECES];
-        if (next.n[t] > 0) {
-          fetch_rows(next);
-          announced = true;
-        }
-      }
       // ---- the result, or this piece of it ----
       if (n > 0) {
         ok = wait_all(&o_full[t], o_count++ & 1);
         if (!ok) break;
         tc_fence_after();
       }
-      if (announced) announce_rows();  // (their scores may come while the results leave: the products with them wait for the probabilities)
-      const bool poisoned = reinterpret_cast<volatile int*>(lost)[i % PW_PIECES] == i + 1;
+      const bool poisoned = reinterpret_cast<volatile int*>(lost)[i % PW_LOST] == i + 1;
       if (m_run == -INFINITY) l_run = 0.f;
       if (poisoned) l_run = __uint_as_float(0x7fc00000u);
-      if (t * PW_M < pc.rows) {  // (warp-uniform: the loads from tensor memory are the whole warp's)
-        const bool mine = t * PW_M + row < pc.rows;
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-        const int token = here / p.group, head = here % p.group;
-        bf16* to = p.out + (long long)(pc.token0 + token) * p.o_st + (long long)(pc.kvh * p.group + head) * p.o_sh;
-        const bool sectors = (reinterpret_cast<uintptr_t>(to) & 31) == 0;  // (whole sectors leave at once)
-        float* part = p.parts.o + ((long long)max(pc.slot, 0) * PW_ROWS + t * PW_M + row) * D;
-#pragma unroll
-        for (int c = 0; c < D; c += W) {
-          uint32_t o[W];
+      const int left = pc.rows - t * PW_M - quarter * 32;  // of this warp's rows
+      if (left > 0) {
+        // through shared memory, 128 bytes of each row at a time in swizzled chunks of 16: a thread has a row, and eight threads store a line of one
+        const bool whole = pc.slot < 0;
+        const float inv = whole ? (l_run == 0.f ? 0.f : 1.f / l_run) : 1.f;
+        uint8_t* stage = out_s + (warp - 4) * C::STAGE_BYTES;
+        auto put = [&](int k, uint4 v) { *reinterpret_cast<uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) = v; };
+        auto get = [&](int i) {  // of row i * 4 + lane / 8
+          const int r = i * 4 + (lane >> 3);
+          return *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+        };
+        auto column = [&](int c, uint32_t (&o)[W]) {
           if (n > 0) {
             tm_load(o_addr + c, o);
             tmem_ld_wait();
@@ -499,30 +538,62 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 #pragma unroll
             for (int x = 0; x < W; ++x) o[x] = 0u;
           }
-          if (mine && pc.slot >= 0) {
+        };
+        if (whole) {
+          const int at = pc.row0 + t * PW_M + quarter * 32 + (lane >> 3), step_tokens = 4 / p.group, step_heads = 4 % p.group;
+          bf16* base = p.out + (long long)pc.token0 * p.o_st + (long long)pc.kvh * p.group * p.o_sh + (lane & 7) * 8;
 #pragma unroll
-            for (int x = 0; x < W; x += 8) st_global_v8(part + c + x, o + x);
-          } else if (mine && sectors) {
-            uint32_t w[W / 2];
+          for (int c = 0; c < D; c += 64) {
 #pragma unroll
-            for (int x = 0; x < W / 2; ++x) w[x] = pack_bf16x2(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv);
+            for (int w0 = 0; w0 < 64; w0 += W) {
+              uint32_t o[W];
+              column(c + w0, o);
 #pragma unroll
-            for (int x = 0; x < W / 2; x += 8) st_global_v8(to + c + 2 * x, w + x);
-          } else if (mine) {
+              for (int x = 0; x < W; x += 8)
+                put((w0 + x) / 8, make_uint4(pack_bf16x2(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv),
+                                             pack_bf16x2(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv),
+                                             pack_bf16x2(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv),
+                                             pack_bf16x2(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv)));
+            }
+            __syncwarp();
+            int token = at / p.group, head = at % p.group;
 #pragma unroll
-            for (int x = 0; x < W; x += 8)
-              *reinterpret_cast<uint4*>(to + c + x) =
-                  make_uint4(pack_bf16x2(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv), pack_bf16x2(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv),
-                             pack_bf16x2(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv), pack_bf16x2(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv));
+            for (int i = 0; i < 8; ++i) {
+              if (i * 4 + (lane >> 3) < left) *reinterpret_cast<uint4*>(base + token * p.o_st + head * p.o_sh + c) = get(i);
+              token += step_tokens;
+              head += step_heads;
+              if (head >= p.group) {
+                head -= p.group;
+                ++token;
+              }
+            }
+            __syncwarp();
+          }
+        } else {
+          const long long first = (long long)pc.slot * PW_ROWS + t * PW_M + quarter * 32;
+          float* part = p.parts.o + (first + (lane >> 3)) * D + (lane & 7) * 4;
+          if (lane < left) p.parts.ml[first + lane] = make_float2(poisoned ? 0.f : m_run, l_run);
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+#pragma unroll
+            for (int w0 = 0; w0 < 32; w0 += W) {
+              uint32_t o[W];
+              column(c + w0, o);
+#pragma unroll
+              for (int x = 0; x < W; x += 4) put((w0 + x) / 4, make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]));
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i * 4 + (lane >> 3) < left) *reinterpret_cast<uint4*>(part + i * 4 * D + c) = get(i);
+            __syncwarp();
           }
         }
-        if (mine && pc.slot >= 0) p.parts.ml[(long long)pc.slot * PW_ROWS + t * PW_M + row] = make_float2(poisoned ? 0.f : m_run, l_run);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&piece_empty[i % PW_PIECES]);
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 
   // ---------------- teardown ----------------
@@ -542,7 +613,11 @@ static int pw_go(const PagedAttnParams& p, const CUtensorMap& k, const CUtensorM
     if (cudaFuncSetAttribute(paged_attn_wide_kernel<D, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return TPB_ERR_CUDA;
     ready[dev].store(true, std::memory_order_release);
   }
-  return launch_dependent(paged_attn_wide_kernel<D, N>, dim3(grid), dim3(PW_THREADS), C::SMEM, stream, ahead, k, v, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  // query rows by boxes: whole tokens in 128 rows, and strides that TMA takes
+  CUtensorMap q = k;
+  bool boxed = PW_M % p.group == 0 && (p.b.tokens == 1 || p.q_st > 0) && (p.heads == 1 || p.q_sh > 0);
+  if (boxed) boxed = paged_rows_tmap(&q, p.q, D, p.heads, p.b.tokens, p.q_sh, p.q_st, p.group, PW_M / p.group) == TPB_OK;
+  return launch_dependent(paged_attn_wide_kernel<D, N>, dim3(grid), dim3(PW_THREADS), C::SMEM, stream, ahead, q, k, v, p, int(boxed)) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
 int pw_tile(int head_dim) { return head_dim; }
