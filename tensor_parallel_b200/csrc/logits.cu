@@ -2,11 +2,12 @@
 //
 //   seen:  x = x > 0 ? x / repetition : x * repetition;   x -= frequency * count + presence * (count > 0);   x += bias;   not allowed: -inf
 //
-// Bound by memory: each logit is read once and written once.  A block has a part of one row's vocabulary.  It counts the tokens of that part in shared memory (a
-// 32-bit word per entry: the top bit for a token that was seen at all, the rest for how often it was said) by walking the row's whole history, which the other
-// blocks of the row find in L2, and then streams its logits, four 16-byte vectors per thread on their way at a time, the first of them during the count.  Integer
-// atomics: the counts do not depend on their order.  Parts are as long as leaves three blocks to an SM: the walk, a chain of loads that nothing hides, is then
-// paid once (128 x 65024 fp32, 1000 tokens: parts of 1024 to 8192 entries in registers 28 to 33 us, 12 us without the walk).
+// Bound by memory: each logit is read once and written once.  Two kernels.  The first streams the logits with bias and mask, four 16-byte vectors per thread
+// on their way at a time.  The second deals with the few entries that a row has had; it is launched ahead and does all but its stores while the first one runs:
+// a block has a part of one row's vocabulary, counts the row's tokens of that part in shared memory (a 32-bit word per entry: the top bit for a token
+// that was seen at all, the rest for how often it was said), and whoever takes an entry's count computes its logit anew and stores it when the first kernel
+// has ended.  Integer atomics: the counts do not depend on their order.  In one kernel the walk over the history, a chain of loads, stood in front of every
+// block's stream, or its penalties in it (128 x 65024 fp32, 1000 tokens: 28 to 40 us; the stream alone takes 12).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -14,6 +15,7 @@
 
 #include <atomic>
 
+#include "launch.cuh"
 #include "ptx_sm100.cuh"
 #include "tpb_api.h"
 
@@ -33,7 +35,7 @@ struct LogitsParams {
   const uint32_t* allowed;
   uint32_t* status;
   long long logits_ld, out_ld, tokens_ld, bias_ld, allowed_ld;
-  int vocab, width, bias_fp32, part;
+  int vocab, width, bias_fp32;
   float repetition_all, frequency_all, presence_all;
 };
 
@@ -48,6 +50,9 @@ __device__ __forceinline__ float lg_load(const float* p) { return *p; }
 __device__ __forceinline__ float lg_load(const bf16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void lg_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void lg_store(bf16* p, float v) { *p = __float2bfloat16(v); }
+
+__device__ __forceinline__ void lg_wait_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void lg_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Elements at, at + 1, ... of a row of numbers, `n` of them in [0, limit); one vector where the address allows.
 template <int N>
@@ -65,94 +70,41 @@ __device__ __forceinline__ void lg_numbers(const float* row, int at, int limit, 
   for (int i = 0; i < N; ++i) v[i] = at + i >= 0 && at + i < limit ? __ldg(row + at + i) : 0.f;
 }
 
-constexpr int LG_DEPTH = 4;         // vectors of a thread on their way
-constexpr int LG_MOST_ENTRIES = 16384;  // of a part: 64 KB of counts, three blocks per SM
+constexpr int LG_DEPTH = 4;           // vectors of a thread on their way
+constexpr int LG_ENTRIES = 24576;     // of a part of the vocabulary at most: 96 KB of counts, two blocks per SM
+constexpr int LG_HELD = 8;            // results of a thread that wait for the first kernel
 
 // WIDE: logits and results of a row lie alike to a 16-byte boundary, and go in 16-byte vectors of the row's own grid, of which the first may begin in front of the
 // row and the last end behind it; else one by one.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(LG_THREADS)
-adjust_logits_kernel(const LogitsParams p) {
-  extern __shared__ __align__(16) uint32_t counts[];
+__global__ void __launch_bounds__(LG_THREADS, 5)
+adjust_stream_kernel(const LogitsParams p, int part) {
   constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * N;
+  lg_launch_next();
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.logits) + row * p.logits_ld;
   T* y = static_cast<T*>(p.out) + row * p.out_ld;
   const int skew = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % N);
-  const int begin = blockIdx.y * p.part - skew, end = int(min((long long)p.vocab, (long long)begin + p.part));  // (the first part begins up to N - 1 in front of the row)
+  const int begin = blockIdx.y * part - skew, end = int(min((long long)p.vocab, (long long)begin + part));  // (the first part begins up to N - 1 in front of the row)
   const int mine = begin + int(threadIdx.x) * N;
+  const uint32_t* allowed = p.allowed ? p.allowed + row * p.allowed_ld : nullptr;
+  const int words = (p.vocab + 31) / 32;
   uint4 raw[LG_DEPTH];
   auto fetch = [&](uint4& u, int at) {
     T* v = reinterpret_cast<T*>(&u);
     if (WIDE && at >= 0 && at + N <= p.vocab) {
-      u = __ldcs(reinterpret_cast<const uint4*>(x + at));
+      u = *reinterpret_cast<const uint4*>(x + at);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if (at + i >= 0 && at + i < p.vocab) v[i] = x[at + i];
     }
   };
-#pragma unroll
-  for (int j = 0; j < LG_DEPTH; ++j)
-    if (mine + j * ROUND < end) fetch(raw[j], mine + j * ROUND);
-  const bool history = p.tokens != nullptr;
-  if (history) {
-    for (int i = threadIdx.x * 4; i < p.part; i += LG_THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
-    int length = p.lengths ? __ldg(p.lengths + row) : p.width;
-    const int prompt = p.prompts ? __ldg(p.prompts + row) : 0;
-    if (length < 0 || length > p.width || prompt < 0) {
-      if (threadIdx.x == 0) atomicMax(p.status, uint32_t(STATUS_BAD_ARG));
-      length = min(max(length, 0), p.width);
-    }
-    __syncthreads();
-    const long long* said = p.tokens + row * p.tokens_ld;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < p.width; i += LG_THREADS) {
-      const long long token = __ldg(said + i);
-      if (i < length && token >= max(begin, 0) && token < end) {
-        if (i < prompt)
-          atomicOr(&counts[token - begin], 0x80000000u);
-        else
-          atomicAdd(&counts[token - begin], 1u);
-      }
-    }
-    __syncthreads();
-  }
-  const float repetition = p.repetition ? __ldg(p.repetition + row) : p.repetition_all;
-  const float frequency = p.frequency ? __ldg(p.frequency + row) : p.frequency_all;
-  const float presence = p.presence ? __ldg(p.presence + row) : p.presence_all;
-  const uint32_t* allowed = p.allowed ? p.allowed + row * p.allowed_ld : nullptr;
-  const int words = (p.vocab + 31) / 32;
-
   auto adjust = [&](uint4 taken, int at) {
     T* packed = reinterpret_cast<T*>(&taken);
     float v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = lg_load(packed + i);
-    if (history) {
-      uint32_t seen[N], any = 0;
-#pragma unroll
-      for (int i = 0; i < N; i += N < 4 ? 1 : 4) {
-        const uint32_t* from = counts + (at - begin) + i;
-        if (N < 4) {
-          seen[i] = *from;
-        } else {
-          const uint4 u = *reinterpret_cast<const uint4*>(from);
-          seen[i] = u.x, seen[i + (N > 1)] = u.y, seen[i + 2 * (N > 2)] = u.z, seen[i + 3 * (N > 3)] = u.w;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) any |= seen[i];
-      if (any) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (seen[i]) {
-            v[i] = v[i] > 0.f ? v[i] / repetition : v[i] * repetition;
-            const uint32_t count = seen[i] & 0x7fffffffu;
-            if (count) v[i] -= frequency * float(count) + presence;
-          }
-      }
-    }
     if (p.bias) {
       if (p.bias_fp32) {
         float b[N];
@@ -178,13 +130,16 @@ adjust_logits_kernel(const LogitsParams p) {
 #pragma unroll
     for (int i = 0; i < N; ++i) lg_store(packed + i, v[i]);
     if (WIDE && at >= 0 && at + N <= p.vocab) {
-      __stcs(reinterpret_cast<uint4*>(y + at), taken);
+      *reinterpret_cast<uint4*>(y + at) = taken;
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if (at + i >= 0 && at + i < p.vocab) y[at + i] = packed[i];
     }
   };
+#pragma unroll
+  for (int j = 0; j < LG_DEPTH; ++j)
+    if (mine + j * ROUND < end) fetch(raw[j], mine + j * ROUND);
   for (int at = mine; at < end; at += LG_DEPTH * ROUND) {
 #pragma unroll
     for (int j = 0; j < LG_DEPTH; ++j) {
@@ -197,24 +152,104 @@ adjust_logits_kernel(const LogitsParams p) {
   }
 }
 
+template <typename T>
+__global__ void __launch_bounds__(LG_THREADS)
+adjust_seen_kernel(const LogitsParams p, int part) {
+  extern __shared__ __align__(16) uint32_t counts[];
+  const long long row = blockIdx.x;
+  const long long begin = (long long)blockIdx.y * part, end = min((long long)p.vocab, begin + part);
+  const T* x = static_cast<const T*>(p.logits) + row * p.logits_ld;
+  T* y = static_cast<T*>(p.out) + row * p.out_ld;
+  for (int i = threadIdx.x * 4; i < part; i += LG_THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
+  int length = p.lengths ? __ldg(p.lengths + row) : p.width;
+  const int prompt = p.prompts ? __ldg(p.prompts + row) : 0;
+  if (length < 0 || length > p.width || prompt < 0) {
+    if (threadIdx.x == 0 && blockIdx.y == 0) atomicMax(p.status, uint32_t(STATUS_BAD_ARG));
+    length = min(max(length, 0), p.width);
+  }
+  const float repetition = p.repetition ? __ldg(p.repetition + row) : p.repetition_all;
+  const float frequency = p.frequency ? __ldg(p.frequency + row) : p.frequency_all;
+  const float presence = p.presence ? __ldg(p.presence + row) : p.presence_all;
+  const uint32_t* allowed = p.allowed ? p.allowed + row * p.allowed_ld : nullptr;
+  const long long* said = p.tokens + row * p.tokens_ld;
+  auto entry = [&](int i) {  // of token i in the counts, -1: not of this part
+    const long long token = __ldg(said + i);
+    return token >= begin && token < end ? int(token - begin) : -1;
+  };
+  auto count = [&](int at, int i) {
+    if (at < 0) return;
+    if (i < prompt)
+      atomicOr(&counts[at], 0x80000000u);
+    else
+      atomicAdd(&counts[at], 1u);
+  };
+  // the entry's logit, if nobody has taken it yet
+  auto take = [&](int at, float& v) {
+    const uint32_t seen = at < 0 ? 0u : atomicExch(&counts[at], 0u);
+    if (!seen) return false;
+    const long long token = begin + at;
+    v = lg_load(x + token);
+    v = v > 0.f ? v / repetition : v * repetition;
+    const uint32_t said_so_often = seen & 0x7fffffffu;
+    if (said_so_often) v -= frequency * float(said_so_often) + presence;
+    if (p.bias) v += p.bias_fp32 ? __ldg(static_cast<const float*>(p.bias) + row * p.bias_ld + token) : __bfloat162float(static_cast<const bf16*>(p.bias)[row * p.bias_ld + token]);
+    if (allowed && !(__ldg(allowed + (token >> 5)) >> (token & 31) & 1u)) v = -INFINITY;
+    return true;
+  };
+  int held[LG_HELD];
+#pragma unroll
+  for (int j = 0; j < LG_HELD; ++j) {
+    const int i = threadIdx.x + j * LG_THREADS;
+    held[j] = i < length ? entry(i) : -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < LG_HELD; ++j) count(held[j], threadIdx.x + j * LG_THREADS);
+#pragma unroll 4
+  for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_THREADS) count(entry(i), i);
+  __syncthreads();
+  float value[LG_HELD];
+#pragma unroll
+  for (int j = 0; j < LG_HELD; ++j)
+    if (!take(held[j], value[j])) held[j] = -1;
+  lg_wait_prior();
+#pragma unroll
+  for (int j = 0; j < LG_HELD; ++j)
+    if (held[j] >= 0) lg_store(y + begin + held[j], value[j]);
+  for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_THREADS) {
+    const int at = entry(i);
+    float v;
+    if (take(at, v)) lg_store(y + begin + at, v);
+  }
+}
+
 template <typename T, bool WIDE>
-static int lg_go(LogitsParams p, int rows, cudaStream_t stream) {
-  constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * (N < 4 ? 4 : N);
+static int lg_stream(const LogitsParams& p, int rows, cudaStream_t stream) {
+  constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * N;
+  // entries of a block: a row's over as many as make five blocks per SM of all rows, whole rounds
+  const long long entries = (long long)p.vocab + N - 1, blocks = max(1LL, 148LL * 5 / rows);
+  const long long part = min((1LL << 30) / ROUND * ROUND, ((entries + blocks - 1) / blocks + ROUND - 1) / ROUND * ROUND);
+  adjust_stream_kernel<T, WIDE><<<dim3(rows, unsigned((entries + part - 1) / part)), LG_THREADS, 0, stream>>>(p, int(part));
+  return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+}
+
+template <typename T>
+static int lg_seen(const LogitsParams& p, int rows, cudaStream_t stream) {
   static std::atomic<bool> ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TPB_ERR_CUDA;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(adjust_logits_kernel<T, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_MOST_ENTRIES * 4) != cudaSuccess) return TPB_ERR_CUDA;
+    if (cudaFuncSetAttribute(adjust_seen_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_ENTRIES * 4) != cudaSuccess) return TPB_ERR_CUDA;
     ready[dev].store(true, std::memory_order_release);
   }
-  // entries of a part: a row's over as many blocks as make three per SM of all rows, whole rounds of the block
-  const long long entries = (long long)p.vocab + N - 1, blocks = max(1LL, 148LL * 3 / rows);
-  const long long part = min((long long)LG_MOST_ENTRIES, ((entries + blocks - 1) / blocks + ROUND - 1) / ROUND * ROUND);
-  const long long parts = (entries + part - 1) / part;
+  // entries of a block: as few parts as fit where there are blocks enough for the SMs, shorter ones else
+  const long long least = (p.vocab + (long long)LG_ENTRIES - 1) / LG_ENTRIES, parts = max(least, min(148LL / rows, ((long long)p.vocab + 4095) / 4096));
   if (parts > 65535) return TPB_ERR_SIZE;
-  p.part = int(part);
-  adjust_logits_kernel<T, WIDE><<<dim3(rows, unsigned(parts)), LG_THREADS, p.tokens ? size_t(part) * 4 : 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  const int part = int((((p.vocab + parts - 1) / parts) + 3) / 4 * 4);
+  return launch_dependent(adjust_seen_kernel<T>, dim3(rows, unsigned((p.vocab + (long long)part - 1) / part)), dim3(LG_THREADS), size_t(part) * 4, stream, true, p, part) ==
+                 cudaSuccess
+             ? TPB_OK
+             : TPB_ERR_CUDA;
 }
 
 template <typename T>
@@ -222,7 +257,8 @@ static int lg_launch(const LogitsParams& p, int rows, cudaStream_t stream) {
   constexpr int N = Vec<T>::N;
   auto place = [](const void* t) { return reinterpret_cast<uintptr_t>(t) / sizeof(T) % N; };
   const bool wide = place(p.logits) == place(p.out) && (rows == 1 || (p.logits_ld - p.out_ld) % N == 0);
-  return wide ? lg_go<T, true>(p, rows, stream) : lg_go<T, false>(p, rows, stream);
+  const int rc = wide ? lg_stream<T, true>(p, rows, stream) : lg_stream<T, false>(p, rows, stream);
+  return rc != TPB_OK || !p.tokens || !p.width ? rc : lg_seen<T>(p, rows, stream);
 }
 
 }  // namespace tpb
@@ -232,7 +268,7 @@ using namespace tpb;
 extern "C" int tpb_adjust_logits(const tpb_adjust_logits_t* a, void* stream_) {
   if (!a || !a->logits || !a->out || !a->status || a->rows <= 0 || a->vocab <= 0 || a->width < 0 || a->dtype < 0 || a->dtype > 1) return TPB_ERR_ARG;
   LogitsParams p = {a->logits, a->out, a->tokens, a->lengths, a->prompts, a->repetition, a->frequency, a->presence, a->bias, reinterpret_cast<const uint32_t*>(a->allowed),
-                    static_cast<uint32_t*>(a->status), a->logits_ld, a->out_ld, a->tokens_ld, a->bias_ld, a->allowed_ld, a->vocab, a->width, a->bias_dtype, 0,
+                    static_cast<uint32_t*>(a->status), a->logits_ld, a->out_ld, a->tokens_ld, a->bias_ld, a->allowed_ld, a->vocab, a->width, a->bias_dtype,
                     a->repetition_all, a->frequency_all, a->presence_all};
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
   return a->dtype ? lg_launch<float>(p, a->rows, s) : lg_launch<bf16>(p, a->rows, s);

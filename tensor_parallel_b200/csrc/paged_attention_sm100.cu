@@ -443,12 +443,13 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tmem_ld_wait();
         if (!plain) {
 #pragma unroll
-          for (int c = 0; c < N; ++c)
-            if (c >= visible) r[c] = 0xff800000u;
-          if (hidden > 0) {
+          for (int c = 0; c < N; c += 32) {
+            // a bit for each of 32 keys: below `visible`, from `hidden` on
+            const int up = min(max(visible - c, 0), 32), down = min(max(hidden - c, 0), 32);
+            const uint32_t seen = (up == 32 ? 0xffffffffu : (1u << up) - 1u) & (down == 32 ? 0u : 0xffffffffu << down);
 #pragma unroll
-            for (int c = 0; c < N; ++c)
-              if (c < hidden) r[c] = 0xff800000u;
+            for (int x = 0; x < 32; ++x)
+              if (!(seen >> x & 1u)) r[c + x] = 0xff800000u;
           }
         }
 #pragma unroll
@@ -469,8 +470,8 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           rescale = true;
         }
         if (j > 0 && __any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-          for (int c = 0; c < D; c += W) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += W) {  // (rolled, as the result below: code that is not in the instruction cache costs more than its instructions)
             uint32_t o[W];
             tm_load(o_addr + c, o);
             tmem_ld_wait();
@@ -525,69 +526,49 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         const bool whole = pc.slot < 0;
         const float inv = whole ? (l_run == 0.f ? 0.f : 1.f / l_run) : 1.f;
         uint8_t* stage = out_s + (warp - 4) * C::STAGE_BYTES;
-        auto put = [&](int k, uint4 v) { *reinterpret_cast<uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) = v; };
-        auto get = [&](int i) {  // of row i * 4 + lane / 8
-          const int r = i * 4 + (lane >> 3);
-          return *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-        };
-        auto column = [&](int c, uint32_t (&o)[W]) {
+        if (!whole && lane < left) p.parts.ml[(long long)pc.slot * PW_ROWS + t * PW_M + quarter * 32 + lane] = make_float2(poisoned ? 0.f : m_run, l_run);
+        const int step_tokens = 4 / p.group, step_heads = 4 % p.group;
+        const int first_token = (pc.row0 + t * PW_M + quarter * 32 + (lane >> 3)) / p.group, first_head = (pc.row0 + t * PW_M + quarter * 32 + (lane >> 3)) % p.group;
+        char* base = whole ? reinterpret_cast<char*>(p.out + (long long)pc.token0 * p.o_st + (long long)pc.kvh * p.group * p.o_sh)
+                           : reinterpret_cast<char*>(p.parts.o + ((long long)pc.slot * PW_ROWS + t * PW_M + quarter * 32 + (lane >> 3)) * D);
+        base += (lane & 7) * 16;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
           if (n > 0) {
-            tm_load(o_addr + c, o);
+#pragma unroll
+            for (int w0 = 0; w0 < 32; w0 += W) tm_load(o_addr + c + w0, *reinterpret_cast<uint32_t(*)[W]>(o + w0));
             tmem_ld_wait();
           } else {
 #pragma unroll
-            for (int x = 0; x < W; ++x) o[x] = 0u;
+            for (int x = 0; x < 32; ++x) o[x] = 0u;
           }
-        };
-        if (whole) {
-          const int at = pc.row0 + t * PW_M + quarter * 32 + (lane >> 3), step_tokens = 4 / p.group, step_heads = 4 % p.group;
-          bf16* base = p.out + (long long)pc.token0 * p.o_st + (long long)pc.kvh * p.group * p.o_sh + (lane & 7) * 8;
+          const int k0 = whole ? (c >> 3) & 4 : 0;  // 32 columns are half of 128 bytes in bf16, all of them in fp32
+          if (whole) {
 #pragma unroll
-          for (int c = 0; c < D; c += 64) {
-#pragma unroll
-            for (int w0 = 0; w0 < 64; w0 += W) {
-              uint32_t o[W];
-              column(c + w0, o);
-#pragma unroll
-              for (int x = 0; x < W; x += 8)
-                put((w0 + x) / 8, make_uint4(pack_bf16x2(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv),
-                                             pack_bf16x2(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv),
-                                             pack_bf16x2(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv),
-                                             pack_bf16x2(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv)));
-            }
-            __syncwarp();
-            int token = at / p.group, head = at % p.group;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (i * 4 + (lane >> 3) < left) *reinterpret_cast<uint4*>(base + token * p.o_st + head * p.o_sh + c) = get(i);
-              token += step_tokens;
-              head += step_heads;
-              if (head >= p.group) {
-                head -= p.group;
-                ++token;
-              }
-            }
-            __syncwarp();
+            for (int x = 0; x < 16; ++x) o[x] = pack_bf16x2(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv);
           }
-        } else {
-          const long long first = (long long)pc.slot * PW_ROWS + t * PW_M + quarter * 32;
-          float* part = p.parts.o + (first + (lane >> 3)) * D + (lane & 7) * 4;
-          if (lane < left) p.parts.ml[first + lane] = make_float2(poisoned ? 0.f : m_run, l_run);
 #pragma unroll
-          for (int c = 0; c < D; c += 32) {
-#pragma unroll
-            for (int w0 = 0; w0 < 32; w0 += W) {
-              uint32_t o[W];
-              column(c + w0, o);
-#pragma unroll
-              for (int x = 0; x < W; x += 4) put((w0 + x) / 4, make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]));
+          for (int x = 0; x < 8; ++x)
+            if (x < 4 || !whole)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((k0 + x) ^ (lane & 7)) << 4)) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+          if (whole && !(c & 32)) continue;
+          __syncwarp();
+          int token = first_token, head = first_head;
+#pragma unroll 2
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            char* to = whole ? base + (token * p.o_st + head * p.o_sh + (c & ~63)) * 2 : base + (i * 4 * D + c) * 4;
+            if (r < left) *reinterpret_cast<uint4*>(to) = v;
+            token += step_tokens;
+            head += step_heads;
+            if (head >= p.group) {
+              head -= p.group;
+              ++token;
             }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i * 4 + (lane >> 3) < left) *reinterpret_cast<uint4*>(part + i * 4 * D + c) = get(i);
-            __syncwarp();
           }
+          __syncwarp();
         }
       }
       tc_fence_before();
