@@ -72,12 +72,13 @@ __device__ __forceinline__ void lg_numbers(const float* row, int at, int limit, 
 
 constexpr int LG_DEPTH = 4;           // vectors of a thread on their way
 constexpr int LG_ENTRIES = 24576;     // of a part of the vocabulary at most: 96 KB of counts, two blocks per SM
-constexpr int LG_HELD = 8;            // results of a thread that wait for the first kernel
+constexpr int LG_SEEN_THREADS = 512;
+constexpr int LG_HELD = 4;            // tokens of a thread at a time; the first of them wait for the first kernel with their results
 
 // WIDE: logits and results of a row lie alike to a 16-byte boundary, and go in 16-byte vectors of the row's own grid, of which the first may begin in front of the
 // row and the last end behind it; else one by one.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(LG_THREADS, 5)
+__global__ void __launch_bounds__(LG_THREADS, WIDE && sizeof(T) == 2 ? 4 : 5)
 adjust_stream_kernel(const LogitsParams p, int part) {
   constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * N;
   lg_launch_next();
@@ -153,14 +154,14 @@ adjust_stream_kernel(const LogitsParams p, int part) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LG_THREADS)
+__global__ void __launch_bounds__(LG_SEEN_THREADS)
 adjust_seen_kernel(const LogitsParams p, int part) {
   extern __shared__ __align__(16) uint32_t counts[];
   const long long row = blockIdx.x;
   const long long begin = (long long)blockIdx.y * part, end = min((long long)p.vocab, begin + part);
   const T* x = static_cast<const T*>(p.logits) + row * p.logits_ld;
   T* y = static_cast<T*>(p.out) + row * p.out_ld;
-  for (int i = threadIdx.x * 4; i < part; i += LG_THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x * 4; i < part; i += LG_SEEN_THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
   int length = p.lengths ? __ldg(p.lengths + row) : p.width;
   const int prompt = p.prompts ? __ldg(p.prompts + row) : 0;
   if (length < 0 || length > p.width || prompt < 0) {
@@ -183,43 +184,60 @@ adjust_seen_kernel(const LogitsParams p, int part) {
     else
       atomicAdd(&counts[at], 1u);
   };
-  // the entry's logit, if nobody has taken it yet
-  auto take = [&](int at, float& v) {
-    const uint32_t seen = at < 0 ? 0u : atomicExch(&counts[at], 0u);
-    if (!seen) return false;
-    const long long token = begin + at;
-    v = lg_load(x + token);
-    v = v > 0.f ? v / repetition : v * repetition;
-    const uint32_t said_so_often = seen & 0x7fffffffu;
-    if (said_so_often) v -= frequency * float(said_so_often) + presence;
-    if (p.bias) v += p.bias_fp32 ? __ldg(static_cast<const float*>(p.bias) + row * p.bias_ld + token) : __bfloat162float(static_cast<const bf16*>(p.bias)[row * p.bias_ld + token]);
-    if (allowed && !(__ldg(allowed + (token >> 5)) >> (token & 31) & 1u)) v = -INFINITY;
-    return true;
-  };
-  int held[LG_HELD];
-#pragma unroll
-  for (int j = 0; j < LG_HELD; ++j) {
-    const int i = threadIdx.x + j * LG_THREADS;
-    held[j] = i < length ? entry(i) : -1;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < LG_HELD; ++j) count(held[j], threadIdx.x + j * LG_THREADS);
-#pragma unroll 4
-  for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_THREADS) count(entry(i), i);
-  __syncthreads();
+  int at[LG_HELD];
   float value[LG_HELD];
+  auto entries = [&](int from) {
 #pragma unroll
-  for (int j = 0; j < LG_HELD; ++j)
-    if (!take(held[j], value[j])) held[j] = -1;
+    for (int j = 0; j < LG_HELD; ++j) at[j] = from + j * LG_SEEN_THREADS < length ? entry(from + j * LG_SEEN_THREADS) : -1;
+  };
+  // the logits of entries that nobody has taken yet; the others' places become -1.  (All loads of one kind behind one another, not a token's.)
+  auto take = [&]() {
+    uint32_t seen[LG_HELD];
+    float bias[LG_HELD];
+    uint32_t word[LG_HELD];
+#pragma unroll
+    for (int j = 0; j < LG_HELD; ++j) {
+      seen[j] = at[j] < 0 ? 0u : atomicExch(&counts[at[j]], 0u);
+      if (!seen[j]) at[j] = -1;
+    }
+#pragma unroll
+    for (int j = 0; j < LG_HELD; ++j) {
+      const long long token = begin + at[j];
+      value[j] = at[j] < 0 ? 0.f : lg_load(x + token);
+      bias[j] = at[j] < 0 || !p.bias ? 0.f
+                : p.bias_fp32        ? __ldg(static_cast<const float*>(p.bias) + row * p.bias_ld + token)
+                                     : __bfloat162float(static_cast<const bf16*>(p.bias)[row * p.bias_ld + token]);
+      word[j] = at[j] < 0 || !allowed ? ~0u : __ldg(allowed + (token >> 5));
+    }
+#pragma unroll
+    for (int j = 0; j < LG_HELD; ++j) {
+      float v = value[j];
+      if (at[j] >= 0) v = v > 0.f ? v / repetition : v * repetition;
+      const uint32_t often = seen[j] & 0x7fffffffu;
+      if (often) v -= frequency * float(often) + presence;
+      if (p.bias) v += bias[j];
+      value[j] = word[j] >> ((begin + at[j]) & 31) & 1u ? v : -INFINITY;
+    }
+  };
+  auto store = [&]() {
+#pragma unroll
+    for (int j = 0; j < LG_HELD; ++j)
+      if (at[j] >= 0) lg_store(y + begin + at[j], value[j]);
+  };
+  entries(threadIdx.x);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < LG_HELD; ++j) count(at[j], threadIdx.x + j * LG_SEEN_THREADS);
+#pragma unroll 4
+  for (int i = threadIdx.x + LG_HELD * LG_SEEN_THREADS; i < length; i += LG_SEEN_THREADS) count(entry(i), i);
+  __syncthreads();
+  take();
   lg_wait_prior();
-#pragma unroll
-  for (int j = 0; j < LG_HELD; ++j)
-    if (held[j] >= 0) lg_store(y + begin + held[j], value[j]);
-  for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_THREADS) {
-    const int at = entry(i);
-    float v;
-    if (take(at, v)) lg_store(y + begin + at, v);
+  store();
+  for (int i = threadIdx.x + LG_HELD * LG_SEEN_THREADS; i < length; i += LG_HELD * LG_SEEN_THREADS) {
+    entries(i);
+    take();
+    store();
   }
 }
 
@@ -246,7 +264,7 @@ static int lg_seen(const LogitsParams& p, int rows, cudaStream_t stream) {
   const long long least = (p.vocab + (long long)LG_ENTRIES - 1) / LG_ENTRIES, parts = max(least, min(148LL / rows, ((long long)p.vocab + 4095) / 4096));
   if (parts > 65535) return TPB_ERR_SIZE;
   const int part = int((((p.vocab + parts - 1) / parts) + 3) / 4 * 4);
-  return launch_dependent(adjust_seen_kernel<T>, dim3(rows, unsigned((p.vocab + (long long)part - 1) / part)), dim3(LG_THREADS), size_t(part) * 4, stream, true, p, part) ==
+  return launch_dependent(adjust_seen_kernel<T>, dim3(rows, unsigned((p.vocab + (long long)part - 1) / part)), dim3(LG_SEEN_THREADS), size_t(part) * 4, stream, true, p, part) ==
                  cudaSuccess
              ? TPB_OK
              : TPB_ERR_CUDA;

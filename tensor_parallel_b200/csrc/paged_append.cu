@@ -2,12 +2,13 @@
 //
 //   n = x * w / sqrt(mean(x^2) + eps)  (heads with a norm);   (a, b) -> (a cos - b sin, b cos + a sin) * factor  over the pairs of the first rotary_dim elements
 //
-// Bound by memory: every row is read once and written once, 4 bytes per element in all.  A row is a group of head_dim / 8 lanes (a power of two of them) with
-// eight elements each, so that the sum of squares and the partner of a pair come by shuffles; the rows (query, key and value heads) of a block's tokens are
-// dealt out to its groups.  A token's place (a search for its sequence, its lengths, its page: four loads behind one another) and its angles are common to its
-// heads: a warp per token looks the place up and a thread per frequency evaluates the angle, while the first rows are on their way.  Many tokens go eight to a
-// block, so that this chain is paid once for 8 x 48 rows; few tokens have several blocks each.  Angles are taken modulo a turn in 64 bits (position *
-// frequency in 32 bits is off by position * 2^-24 radians, 0.06 at a million), then by sincospif.  Rounded to bf16 once, at the end.
+// Bound by memory: every row is read once and written once, 4 bytes per element in all; next to it by instructions, so a lane has both elements of its pairs and
+// needs no exchange for them: a row is a group of head_dim / 16 lanes (a power of two of them) with two chunks of eight elements each, rotary_dim / 2 apart
+// (with one chunk per lane and shuffles, 16 k tokens of 48 heads of 128 took 168 us).  The rows (query, key and value heads) of a block's tokens are dealt out to its
+// groups.  A token's place (a search for its sequence, its lengths, its page: four loads behind one another) and its angles are common to its heads: a
+// warp per token looks the place up and a thread per frequency evaluates the angle, while the first rows are on their way.  Many tokens go eight to a block, so
+// that this chain is paid once for 8 x 48 rows; few tokens have several blocks each.  Angles are taken modulo a turn in 64 bits (position * frequency
+// in 32 bits is off by position * 2^-24 radians, 0.06 at a million), then by sincospif.  Rounded to bf16 once, at the end.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -64,159 +65,231 @@ struct AppendPlace {  // of a token
   long long k_at, v_at; // -1: not stored
 };
 
-template <int LANES>
-__global__ void __launch_bounds__(AP_THREADS, 4)
+// How the elements of a pair lie: none are turned; a multiple of eight apart; side by side; any other distance apart.
+enum { TURN_NONE, TURN_HALVES, TURN_PAIRS, TURN_ODD };
+
+template <int LANES, int TURN>
+__global__ void __launch_bounds__(AP_THREADS, 3)
 paged_append_kernel(const AppendParams p, int tokens_of_block) {
-  __shared__ float cos_s[AP_TOKENS * AP_MAX_HALF], sin_s[AP_TOKENS * AP_MAX_HALF];
+  __shared__ __align__(16) float cos_s[AP_TOKENS * AP_MAX_HALF], sin_s[AP_TOKENS * AP_MAX_HALF];
+  __shared__ __align__(16) float norm_s[2][2 * AP_MAX_HALF];  // weights of queries and keys
   __shared__ AppendPlace places[AP_TOKENS];
   constexpr int GROUPS = AP_THREADS / LANES;  // rows at a time
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = blockIdx.x * tokens_of_block, tokens = min(tokens_of_block, p.b.tokens - t0);
-  const int e0 = threadIdx.x % LANES * 8;
-  const bool on = e0 < p.head_dim;
-  const int rows = p.q_heads + 2 * p.kv_heads;
+  const int rows = p.q_heads + 2 * p.kv_heads, chunks = p.head_dim / 8;
+  // this lane's chunks: pairs of the turned part, then those that stay
+  const int l = threadIdx.x % LANES, turned = TURN == TURN_HALVES ? p.half / 8 : 0;
+  const bool pair = l < turned;
+  const int c0 = pair ? l : TURN == TURN_HALVES ? 2 * turned + 2 * (l - turned) : l, c1 = pair ? l + turned : TURN == TURN_HALVES ? c0 + 1 : l + LANES;
+  const bool on0 = c0 < chunks, on1 = c1 < chunks;
   // rows of the block: (token, head), heads fastest, one to a group and round; every lane makes its warp's rounds (the shuffles are the whole warp's)
-  const int all = tokens * rows, stride = gridDim.y * GROUPS;
+  const int all = tokens * rows, stride = gridDim.y * GROUPS, step_tokens = stride / rows, step_rows = stride % rows;
   const int i0 = blockIdx.y * GROUPS + threadIdx.x / LANES, first = blockIdx.y * GROUPS + (threadIdx.x & ~31) / LANES;
-
-  auto source = [&](int i) {
-    const long long t = t0 + i / rows;
-    const int r = i % rows;
-    return r < p.q_heads ? p.q + t * p.q_st + r * p.q_sh
-                         : r < p.q_heads + p.kv_heads ? p.k + t * p.k_st + (r - p.q_heads) * p.k_sh : p.v + t * p.v_st + (r - p.q_heads - p.kv_heads) * p.v_sh;
+  struct Cursor {
+    int t, r;
   };
-  constexpr int AHEAD = 4;
-  uint4 raw[AHEAD];
-  auto fetch = [&](int from) {
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int i = from + j * stride;
-      if (on && i < all) raw[j] = *reinterpret_cast<const uint4*>(source(i) + e0);
+  auto step = [&](Cursor& c) {
+    c.t += step_tokens;
+    c.r += step_rows;
+    if (c.r >= rows) {
+      c.r -= rows;
+      ++c.t;
     }
   };
-  fetch(i0);
+  auto source = [&](const Cursor& c) {
+    const long long t = t0 + c.t;
+    return c.r < p.q_heads                ? p.q + t * p.q_st + c.r * p.q_sh
+           : c.r < p.q_heads + p.kv_heads ? p.k + t * p.k_st + (c.r - p.q_heads) * p.k_sh
+                                          : p.v + t * p.v_st + (c.r - p.q_heads - p.kv_heads) * p.v_sh;
+  };
+  constexpr int AHEAD = 4;
+  uint4 raw[AHEAD][2];
+  Cursor next = {i0 / rows, i0 % rows};
+  auto fetch = [&]() {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (next.t < tokens) {
+        const bf16* src = source(next);
+        if (on0) raw[j][0] = *reinterpret_cast<const uint4*>(src + c0 * 8);
+        if (on1) raw[j][1] = *reinterpret_cast<const uint4*>(src + c1 * 8);
+      }
+      step(next);
+    }
+  };
+  Cursor at = next;
+  fetch();
 
   if (warp < tokens) {
     const int t = t0 + warp, seq = sequence_of(p.b, t, lane);
-    AppendPlace at = {0, seq >= 0 && seq < p.b.n, -1, -1};
-    if (at.inside) {
+    AppendPlace place = {0, seq >= 0 && seq < p.b.n, -1, -1};
+    if (place.inside) {
       const PagedSequence s = paged_sequence(p.b, seq);
-      at.position = s.past + (t - s.token0);
+      place.position = s.past + (t - s.token0);
       int page = -1;
-      if (!s.bad && t >= s.token0 && t < s.token0 + s.fresh) page = __ldg(p.b.table + seq * p.b.table_ld + (at.position >> p.b.page_shift));
+      if (!s.bad && t >= s.token0 && t < s.token0 + s.fresh) page = __ldg(p.b.table + seq * p.b.table_ld + (place.position >> p.b.page_shift));
       if (page >= 0 && page < p.b.pages) {
-        const int slot = at.position & ((1 << p.b.page_shift) - 1);
-        at.k_at = page * p.k_sp + slot * p.k_ss;
-        at.v_at = page * p.v_sp + slot * p.v_ss;
+        const int slot = place.position & ((1 << p.b.page_shift) - 1);
+        place.k_at = page * p.k_sp + slot * p.k_ss;
+        place.v_at = page * p.v_sp + slot * p.v_ss;
       } else if (lane == 0 && blockIdx.y == 0) {
         atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
       }
     }
-    if (lane == 0) places[warp] = at;
+    if (lane == 0) places[warp] = place;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < tokens * p.half; i += AP_THREADS) {
-    const int t = i / p.half, f = i % p.half;
-    // turns = position * f / (2 pi), less whole turns
-    double turns = double(places[t].position) * (double(__ldg(p.frequencies + f)) * 0.15915494309189533577);
-    turns -= rint(turns);
-    float sn, cs;
-    sincospif(float(2.0 * turns), &sn, &cs);
-    cos_s[t * AP_MAX_HALF + f] = cs * p.factor;
-    sin_s[t * AP_MAX_HALF + f] = sn * p.factor;
-  }
-  __syncthreads();
-
-  auto finish = [&](int i, const uint4& u) {
-    const bool there = i < all;
-    const int t = there ? i / rows : 0, r = there ? i % rows : 0;
-    const bool is_q = r < p.q_heads, is_v = r >= p.q_heads + p.kv_heads;
-    const AppendPlace at = places[t];
-    bf16* dst = nullptr;
-    if (there && on) {
-      if (is_q)
-        dst = at.inside || p.fill_rest ? p.q_out + (t0 + t) * p.o_st + r * p.o_sh : nullptr;
-      else if (!is_v && at.k_at >= 0)
-        dst = p.keys + at.k_at + (r - p.q_heads) * p.k_shead;
-      else if (is_v && at.v_at >= 0)
-        dst = p.values + at.v_at + (r - p.q_heads - p.kv_heads) * p.v_shead;
+  const bool norms = p.q_norm || p.k_norm;
+  if (norms)
+    for (int i = threadIdx.x; i < p.head_dim; i += AP_THREADS) {
+      norm_s[0][i] = p.q_norm ? __bfloat162float(p.q_norm[i]) : 1.f;
+      norm_s[1][i] = p.k_norm ? __bfloat162float(p.k_norm[i]) : 1.f;
     }
-    const float *cs = cos_s + t * AP_MAX_HALF, *sn = sin_s + t * AP_MAX_HALF;
-    float x[8] = {};
-    if (on && there) unpack8(u, x);
-    const bf16* weight = is_q ? p.q_norm : is_v ? nullptr : p.k_norm;
-    float rstd = 1.f;
-    if (p.q_norm || p.k_norm) {
-      float sum = 0.f;
+  __syncthreads();
+  if (TURN != TURN_NONE) {
+    for (int i = threadIdx.x; i < tokens * p.half; i += AP_THREADS) {
+      const int t = i / p.half, f = i % p.half;
+      // turns = position * f / (2 pi), less whole turns
+      double turns = double(places[t].position) * (double(__ldg(p.frequencies + f)) * 0.15915494309189533577);
+      turns -= rint(turns);
+      float sn, cs;
+      sincospif(float(2.0 * turns), &sn, &cs);
+      cos_s[t * AP_MAX_HALF + f] = cs * p.factor;
+      sin_s[t * AP_MAX_HALF + f] = sn * p.factor;
+    }
+    __syncthreads();
+  }
+
+  auto times = [](float (&x)[8], const float* w) {  // x *= w, eight of them from shared memory
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += x[j] * x[j];
+    for (int j = 0; j < 8; j += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(w + j);
+      ffma2(x[j], x[j + 1], x[j], x[j + 1], f.x, f.y, 0.f, 0.f);
+      ffma2(x[j + 2], x[j + 3], x[j + 2], x[j + 3], f.z, f.w, 0.f, 0.f);
+    }
+  };
+  auto finish = [&](const Cursor& c, const uint4 (&u)[2]) {
+    const bool there = c.t < tokens, is_q = c.r < p.q_heads, is_v = c.r >= p.q_heads + p.kv_heads;
+    const AppendPlace place = places[there ? c.t : 0];
+    bf16* dst = nullptr;
+    if (there) {
+      if (is_q)
+        dst = place.inside || p.fill_rest ? p.q_out + (long long)(t0 + c.t) * p.o_st + c.r * p.o_sh : nullptr;
+      else if (!is_v && place.k_at >= 0)
+        dst = p.keys + place.k_at + (c.r - p.q_heads) * p.k_shead;
+      else if (is_v && place.v_at >= 0)
+        dst = p.values + place.v_at + (c.r - p.q_heads - p.kv_heads) * p.v_shead;
+    }
+    uint4 y0 = u[0], y1 = u[1];
+    if (__any_sync(0xffffffffu, there && !is_v)) {
+      float x0[8] = {}, x1[8] = {};
+      if (on0 && there) unpack8(u[0], x0);
+      if (on1 && there) unpack8(u[1], x1);
+      const bool normed = !is_v && (is_q ? p.q_norm : p.k_norm);
+      float rstd = 1.f;
+      if (norms) {
+        float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int d = LANES / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (weight) {
-        rstd = rsqrtf(sum / p.head_dim + p.eps);
-        if (on) {
-          float w[8];
-          unpack8(__ldg(reinterpret_cast<const uint4*>(weight + e0)), w);
+        for (int j = 0; j < 8; j += 2) {
+          ffma2(s0, s1, x0[j], x0[j + 1], x0[j], x0[j + 1], s0, s1);
+          ffma2(s0, s1, x1[j], x1[j + 1], x1[j], x1[j + 1], s0, s1);
+        }
+        s0 += s1;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] *= rstd * w[j];
+        for (int d = LANES / 2; d > 0; d >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, d);
+        if (normed) {
+          rstd = rsqrtf(s0 / p.head_dim + p.eps);
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            ffma2(x0[j], x0[j + 1], x0[j], x0[j + 1], rstd, rstd, 0.f, 0.f);
+            ffma2(x1[j], x1[j + 1], x1[j], x1[j + 1], rstd, rstd, 0.f, 0.f);
+          }
+          const float* w = norm_s[is_q ? 0 : 1];
+          if (on0) times(x0, w + c0 * 8);
+          if (on1) times(x1, w + c1 * 8);
         }
       }
-    }
-    if (p.half && p.interleaved) {
-      if (!is_v) {
+      const float *cs = cos_s + (there ? c.t : 0) * AP_MAX_HALF, *sn = sin_s + (there ? c.t : 0) * AP_MAX_HALF;
+      if (TURN == TURN_HALVES && pair) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int f = e0 / 2 + j;
-          if (f < p.half) {
-            const float a = x[2 * j], b = x[2 * j + 1];
-            x[2 * j] = a * cs[f] - b * sn[f];
-            x[2 * j + 1] = b * cs[f] + a * sn[f];
+        for (int j = 0; j < 8; j += 4) {
+          const float4 cv = *reinterpret_cast<const float4*>(cs + c0 * 8 + j), sv = *reinterpret_cast<const float4*>(sn + c0 * 8 + j);
+          const float cj[4] = {cv.x, cv.y, cv.z, cv.w}, sj[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            float &a0 = x0[j + k], &a1 = x0[j + k + 1], &b0 = x1[j + k], &b1 = x1[j + k + 1];
+            float m0, m1, n0, n1;
+            ffma2(m0, m1, b0, b1, -sj[k], -sj[k + 1], 0.f, 0.f);
+            ffma2(n0, n1, a0, a1, sj[k], sj[k + 1], 0.f, 0.f);
+            ffma2(a0, a1, a0, a1, cj[k], cj[k + 1], m0, m1);
+            ffma2(b0, b1, b0, b1, cj[k], cj[k + 1], n0, n1);
           }
         }
-      }
-    } else if (p.half && p.half % 8 == 0) {
-      const int step = p.half / 8;  // lanes between the elements of a pair
-      const bool second = e0 >= p.half, turns = !is_v && e0 < 2 * p.half;
-      const int from = (second ? lane - step : lane + step) & 31, f0 = second ? e0 - p.half : e0;
-      // (a, b) -> (a cos - b sin, b cos + a sin): the second of a pair adds what the first subtracts
+      } else if (TURN == TURN_PAIRS) {
+        auto turn = [&](float (&x)[8], int chunk) {
 #pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        const float4 c = turns ? *reinterpret_cast<const float4*>(cs + f0 + j) : make_float4(1.f, 1.f, 1.f, 1.f);
-        const float4 s = turns ? *reinterpret_cast<const float4*>(sn + f0 + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float cj[4] = {c.x, c.y, c.z, c.w}, sj[4] = {s.x, s.y, s.z, s.w};
+          for (int j = 0; j < 4; ++j) {
+            const int f = chunk * 4 + j;
+            if (f < p.half) {
+              const float a = x[2 * j], b = x[2 * j + 1];
+              x[2 * j] = a * cs[f] - b * sn[f];
+              x[2 * j + 1] = b * cs[f] + a * sn[f];
+            }
+          }
+        };
+        turn(x0, c0);
+        turn(x1, c1);
+      } else if (TURN == TURN_ODD) {
+        // the partners come from memory once more, before any lane of the warp stores
+        auto turn = [&](float (&x)[8], int chunk, bool on) {
+          if (!on || !there || is_v) return;
+          const bf16* src = source(c);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float other = __shfl_sync(0xffffffffu, x[j + k], from);
-          if (turns) x[j + k] = x[j + k] * cj[k] + (second ? other : -other) * sj[k];
-        }
-      }
-    } else if (p.half) {
-      // pairs that do not lie a multiple of eight elements apart: the partners come from memory once more, before any lane of the warp stores
-      if (!is_v && on && there) {
-        const bf16* src = source(i);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int e = e0 + j;
-          if (e < 2 * p.half) {
+          for (int j = 0; j < 8; ++j) {
+            const int e = chunk * 8 + j;
+            if (e >= 2 * p.half) continue;
             const bool second = e >= p.half;
             const int other = second ? e - p.half : e + p.half, f = second ? other : e;
             float o = __bfloat162float(src[other]);
-            if (weight) o *= rstd * __bfloat162float(weight[other]);
+            if (normed) o = o * rstd * norm_s[is_q ? 0 : 1][other];
             x[j] = second ? x[j] * cs[f] + o * sn[f] : x[j] * cs[f] - o * sn[f];
           }
-        }
+        };
+        turn(x0, c0, on0);
+        turn(x1, c1, on1);
+        __syncwarp();
       }
-      __syncwarp();
+      if (!is_v) {
+        y0 = pack8(x0);
+        y1 = pack8(x1);
+      }
     }
-    if (dst) *reinterpret_cast<uint4*>(dst + e0) = at.inside ? pack8(x) : make_uint4(0, 0, 0, 0);
+    if (dst) {
+      if (!place.inside) y0 = y1 = make_uint4(0, 0, 0, 0);
+      if (on0) *reinterpret_cast<uint4*>(dst + c0 * 8) = y0;
+      if (on1) *reinterpret_cast<uint4*>(dst + c1 * 8) = y1;
+    }
   };
 
   for (int base = 0; first + base < all; base += AHEAD * stride) {
-    if (base) fetch(i0 + base);
+    if (base) fetch();
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      if (first + base + j * stride < all) finish(i0 + base + j * stride, raw[j]);
+    for (int j = 0; j < AHEAD; ++j) {
+      if (first + base + j * stride < all) finish(at, raw[j]);
+      step(at);
+    }
   }
+}
+
+template <int LANES>
+static void ap_launch(const AppendParams& p, dim3 grid, int per_block, cudaStream_t stream) {
+  if (!p.half)
+    paged_append_kernel<LANES, TURN_NONE><<<grid, AP_THREADS, 0, stream>>>(p, per_block);
+  else if (p.interleaved)
+    paged_append_kernel<LANES, TURN_PAIRS><<<grid, AP_THREADS, 0, stream>>>(p, per_block);
+  else if (p.half % 8 == 0)
+    paged_append_kernel<LANES, TURN_HALVES><<<grid, AP_THREADS, 0, stream>>>(p, per_block);
+  else
+    paged_append_kernel<LANES, TURN_ODD><<<grid, AP_THREADS, 0, stream>>>(p, per_block);
 }
 
 }  // namespace tpb
@@ -246,17 +319,17 @@ extern "C" int tpb_paged_append(const tpb_paged_append_t* a, void* stream_) {
   p.q_heads = a->q ? a->heads : 0;
   p.kv_heads = a->kv_heads, p.head_dim = a->head_dim, p.half = a->rotary_dim / 2, p.interleaved = a->interleaved, p.fill_rest = a->fill_rest;
   p.factor = a->factor, p.eps = a->eps;
-  const int lanes = a->head_dim <= 64 ? 8 : a->head_dim <= 128 ? 16 : 32;
+  const int lanes = a->head_dim <= 64 ? 4 : a->head_dim <= 128 ? 8 : 16;
   const int rows = p.q_heads + 2 * p.kv_heads, groups = AP_THREADS / lanes;
   // tokens to a block where that leaves four blocks to an SM and more, else a token's rows over several blocks
   const int per_block = a->tokens >= 148 * 4 * AP_TOKENS ? AP_TOKENS : a->tokens >= 148 * 4 * 2 ? 2 : 1;
   const dim3 grid((a->tokens + per_block - 1) / per_block, a->tokens >= 148 * 4 ? 1 : (rows + groups - 1) / groups);
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
-  if (lanes == 8)
-    paged_append_kernel<8><<<grid, AP_THREADS, 0, s>>>(p, per_block);
-  else if (lanes == 16)
-    paged_append_kernel<16><<<grid, AP_THREADS, 0, s>>>(p, per_block);
+  if (lanes == 4)
+    ap_launch<4>(p, grid, per_block, s);
+  else if (lanes == 8)
+    ap_launch<8>(p, grid, per_block, s);
   else
-    paged_append_kernel<32><<<grid, AP_THREADS, 0, s>>>(p, per_block);
+    ap_launch<16>(p, grid, per_block, s);
   return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
