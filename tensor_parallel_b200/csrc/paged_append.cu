@@ -103,22 +103,19 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
            : c.r < p.q_heads + p.kv_heads ? p.k + t * p.k_st + (c.r - p.q_heads) * p.k_sh
                                           : p.v + t * p.v_st + (c.r - p.q_heads - p.kv_heads) * p.v_sh;
   };
-  constexpr int AHEAD = 4;
+  constexpr int AHEAD = 3;  // rows on their way
   uint4 raw[AHEAD][2];
-  Cursor next = {i0 / rows, i0 % rows};
-  auto fetch = [&]() {
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      if (next.t < tokens) {
-        const bf16* src = source(next);
-        if (on0) raw[j][0] = *reinterpret_cast<const uint4*>(src + c0 * 8);
-        if (on1) raw[j][1] = *reinterpret_cast<const uint4*>(src + c1 * 8);
-      }
-      step(next);
+  Cursor next = {i0 / rows, i0 % rows}, at = next;
+  auto fetch = [&](uint4 (&u)[2]) {
+    if (next.t < tokens) {
+      const bf16* src = source(next);
+      if (on0) u[0] = *reinterpret_cast<const uint4*>(src + c0 * 8);
+      if (on1) u[1] = *reinterpret_cast<const uint4*>(src + c1 * 8);
     }
+    step(next);
   };
-  Cursor at = next;
-  fetch();
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) fetch(raw[j]);
 
   if (warp < tokens) {
     const int t = t0 + warp, seq = sequence_of(p.b, t, lane);
@@ -226,15 +223,17 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
         }
       } else if (TURN == TURN_PAIRS) {
         auto turn = [&](float (&x)[8], int chunk) {
+          const int f0 = chunk * 4;
+          if (f0 >= p.half) return;
+          const float4 cv = *reinterpret_cast<const float4*>(cs + f0), sv = *reinterpret_cast<const float4*>(sn + f0);  // (those beyond the turned part are not used)
+          const float cj[4] = {cv.x, cv.y, cv.z, cv.w}, sj[4] = {sv.x, sv.y, sv.z, sv.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int f = chunk * 4 + j;
-            if (f < p.half) {
+          for (int j = 0; j < 4; ++j)
+            if (f0 + j < p.half) {
               const float a = x[2 * j], b = x[2 * j + 1];
-              x[2 * j] = a * cs[f] - b * sn[f];
-              x[2 * j + 1] = b * cs[f] + a * sn[f];
+              x[2 * j] = a * cj[j] - b * sj[j];
+              x[2 * j + 1] = b * cj[j] + a * sj[j];
             }
-          }
         };
         turn(x0, c0);
         turn(x1, c1);
@@ -271,10 +270,12 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
   };
 
   for (int base = 0; first + base < all; base += AHEAD * stride) {
-    if (base) fetch();
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      if (first + base + j * stride < all) finish(at, raw[j]);
+      if (first + base + j * stride >= all) break;
+      const uint4 taken[2] = {raw[j][0], raw[j][1]};
+      fetch(raw[j]);
+      finish(at, taken);
       step(at);
     }
   }
