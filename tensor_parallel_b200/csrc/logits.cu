@@ -3,7 +3,7 @@
 //   seen:  x = x > 0 ? x / repetition : x * repetition;   x -= frequency * count + presence * (count > 0);   x += bias;   not allowed: -inf
 //
 // Bound by memory: each logit is read once and written once.  Two kernels.  The first streams the logits with bias and mask, four 16-byte vectors per thread
-// on their way at a time.  The second deals with the few entries that a row has had; it is launched ahead and does all but its stores while the first one runs:
+// on their way at a time with their biases.  The second deals with the few entries that a row has had; it is launched ahead and does all but its stores while the first one runs:
 // a block has a part of one row's vocabulary, counts the row's tokens of that part in shared memory (a 32-bit word per entry: the top bit for a token
 // that was seen at all, the rest for how often it was said), and whoever takes an entry's count computes its logit anew and stores it when the first kernel
 // has ended.  Integer atomics: the counts do not depend on their order.  In one kernel the walk over the history, a chain of loads, stood in front of every
@@ -54,101 +54,88 @@ __device__ __forceinline__ void lg_store(bf16* p, float v) { *p = __float2bfloat
 __device__ __forceinline__ void lg_wait_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void lg_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// Elements at, at + 1, ... of a row of numbers, `n` of them in [0, limit); one vector where the address allows.
-template <int N>
-__device__ __forceinline__ void lg_numbers(const float* row, int at, int limit, float (&v)[N]) {
-  if (N > 1 && at >= 0 && at + N <= limit && !(reinterpret_cast<uintptr_t>(row + at) & 15)) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(row + at + i));
-      v[i] = f.x;
-      if (N > 1) v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = at + i >= 0 && at + i < limit ? __ldg(row + at + i) : 0.f;
-}
-
-constexpr int LG_DEPTH = 4;           // vectors of a thread on their way
+constexpr int LG_DEPTH = 4;           // vectors of 16 bytes of fp32 of a thread on their way, half as many of bf16
 constexpr int LG_ENTRIES = 24576;     // of a part of the vocabulary at most: 96 KB of counts, two blocks per SM
-constexpr int LG_SEEN_THREADS = 512;
-constexpr int LG_HELD = 4;            // tokens of a thread at a time; the first of them wait for the first kernel with their results
+constexpr int LG_SEEN_THREADS = 256;  // (that many registers are left beside four blocks of the first kernel)
+constexpr int LG_HELD = 8;            // tokens of a thread at a time; the first of them wait for the first kernel with their results
 
 // WIDE: logits and results of a row lie alike to a 16-byte boundary, and go in 16-byte vectors of the row's own grid, of which the first may begin in front of the
 // row and the last end behind it; else one by one.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(LG_THREADS, WIDE && sizeof(T) == 2 ? 4 : 5)
+__global__ void __launch_bounds__(LG_THREADS, 4)
 adjust_stream_kernel(const LogitsParams p, int part) {
-  constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * N;
+  constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * N, DEPTH = LG_DEPTH * 4 / (N < 4 ? 4 : N);
   lg_launch_next();
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.logits) + row * p.logits_ld;
   T* y = static_cast<T*>(p.out) + row * p.out_ld;
   const int skew = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % N);
   const int begin = blockIdx.y * part - skew, end = int(min((long long)p.vocab, (long long)begin + part));  // (the first part begins up to N - 1 in front of the row)
-  const int mine = begin + int(threadIdx.x) * N;
   const uint32_t* allowed = p.allowed ? p.allowed + row * p.allowed_ld : nullptr;
+  const float* wide_bias = p.bias && p.bias_fp32 ? static_cast<const float*>(p.bias) + row * p.bias_ld : nullptr;
+  const bf16* narrow_bias = p.bias && !p.bias_fp32 ? static_cast<const bf16*>(p.bias) + row * p.bias_ld : nullptr;
+  const bool bias_vectors = N % 4 == 0 && !(reinterpret_cast<uintptr_t>(wide_bias - skew) & 15);
   const int words = (p.vocab + 31) / 32;
-  uint4 raw[LG_DEPTH];
-  auto fetch = [&](uint4& u, int at) {
-    T* v = reinterpret_cast<T*>(&u);
-    if (WIDE && at >= 0 && at + N <= p.vocab) {
-      u = *reinterpret_cast<const uint4*>(x + at);
-    } else {
+  for (int base = begin + int(threadIdx.x) * N; base < end; base += DEPTH * ROUND) {
+    uint4 raw[DEPTH];
+    float bias[DEPTH][N];
+    uint32_t low[DEPTH], high[DEPTH];
+    // all loads of a round in front of the first use
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (at + i >= 0 && at + i < p.vocab) v[i] = x[at + i];
-    }
-  };
-  auto adjust = [&](uint4 taken, int at) {
-    T* packed = reinterpret_cast<T*>(&taken);
-    float v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = lg_load(packed + i);
-    if (p.bias) {
-      if (p.bias_fp32) {
-        float b[N];
-        lg_numbers<N>(static_cast<const float*>(p.bias) + row * p.bias_ld, at, p.vocab, b);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += b[i];
+    for (int j = 0; j < DEPTH; ++j) {
+      const int at = base + j * ROUND;
+      if (at >= end) break;
+      T* v = reinterpret_cast<T*>(&raw[j]);
+      const bool inner = at >= 0 && at + N <= p.vocab;
+      if (WIDE && inner) {
+        raw[j] = *reinterpret_cast<const uint4*>(x + at);
       } else {
-        const bf16* b = static_cast<const bf16*>(p.bias) + row * p.bias_ld;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          if (at + i >= 0 && at + i < p.vocab) v[i] += __bfloat162float(b[at + i]);
+          if (at + i >= 0 && at + i < p.vocab) v[i] = x[at + i];
+      }
+      if (wide_bias) {
+        if (bias_vectors && inner) {
+#pragma unroll
+          for (int i = 0; i + 3 < N; i += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(wide_bias + at + i));
+            bias[j][i] = f.x, bias[j][i + 1] = f.y, bias[j][i + 2] = f.z, bias[j][i + 3] = f.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (at + i >= 0 && at + i < p.vocab) bias[j][i] = __ldg(wide_bias + at + i);
+        }
+      } else if (narrow_bias) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (at + i >= 0 && at + i < p.vocab) bias[j][i] = __bfloat162float(narrow_bias[at + i]);
+      }
+      if (allowed) {
+        // bits of tokens at, at + 1, ...: from two words (the vector may cross their border, and begin in front of the first)
+        const int word = at >> 5;
+        low[j] = word >= 0 ? __ldg(allowed + word) : 0u;
+        high[j] = word + 1 < words ? __ldg(allowed + word + 1) : 0u;
       }
     }
-    if (allowed) {
-      // bits of tokens at, at + 1, ...: from two words (the vector may cross their border, and begin in front of the first)
-      const int word = at >> 5;
-      const uint32_t low = word >= 0 ? __ldg(allowed + word) : 0u, high = word + 1 < words ? __ldg(allowed + word + 1) : 0u;
-      const uint32_t bits = __funnelshift_r(low, high, at & 31);
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (!(bits >> i & 1u)) v[i] = -INFINITY;
-    }
+    for (int j = 0; j < DEPTH; ++j) {
+      const int at = base + j * ROUND;
+      if (at >= end) break;
+      T* v = reinterpret_cast<T*>(&raw[j]);
+      const uint32_t bits = allowed ? __funnelshift_r(low[j], high[j], at & 31) : ~0u;
 #pragma unroll
-    for (int i = 0; i < N; ++i) lg_store(packed + i, v[i]);
-    if (WIDE && at >= 0 && at + N <= p.vocab) {
-      *reinterpret_cast<uint4*>(y + at) = taken;
-    } else {
+      for (int i = 0; i < N; ++i) {
+        const float f = p.bias ? lg_load(v + i) + bias[j][i] : lg_load(v + i);
+        lg_store(v + i, bits >> i & 1u ? f : -INFINITY);
+      }
+      if (WIDE && at >= 0 && at + N <= p.vocab) {
+        *reinterpret_cast<uint4*>(y + at) = raw[j];
+      } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (at + i >= 0 && at + i < p.vocab) y[at + i] = packed[i];
-    }
-  };
-#pragma unroll
-  for (int j = 0; j < LG_DEPTH; ++j)
-    if (mine + j * ROUND < end) fetch(raw[j], mine + j * ROUND);
-  for (int at = mine; at < end; at += LG_DEPTH * ROUND) {
-#pragma unroll
-    for (int j = 0; j < LG_DEPTH; ++j) {
-      const int now = at + j * ROUND, next = now + LG_DEPTH * ROUND;
-      if (now >= end) break;
-      const uint4 taken = raw[j];
-      if (next < end) fetch(raw[j], next);
-      adjust(taken, now);
+        for (int i = 0; i < N; ++i)
+          if (at + i >= 0 && at + i < p.vocab) y[at + i] = v[i];
+      }
     }
   }
 }
@@ -244,8 +231,8 @@ adjust_seen_kernel(const LogitsParams p, int part) {
 template <typename T, bool WIDE>
 static int lg_stream(const LogitsParams& p, int rows, cudaStream_t stream) {
   constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * N;
-  // entries of a block: a row's over as many as make five blocks per SM of all rows, whole rounds
-  const long long entries = (long long)p.vocab + N - 1, blocks = max(1LL, 148LL * 5 / rows);
+  // entries of a block: a row's over as many as make four blocks per SM of all rows, whole rounds
+  const long long entries = (long long)p.vocab + N - 1, blocks = max(1LL, 148LL * 4 / rows);
   const long long part = min((1LL << 30) / ROUND * ROUND, ((entries + blocks - 1) / blocks + ROUND - 1) / ROUND * ROUND);
   adjust_stream_kernel<T, WIDE><<<dim3(rows, unsigned((entries + part - 1) / part)), LG_THREADS, 0, stream>>>(p, int(part));
   return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;

@@ -10,22 +10,24 @@ def numbers(gen, *shape, dtype=BF16, scale=1.0):
     return (torch.randn(*shape, generator=gen, dtype=torch.float32) * scale).to(dtype)
 
 
-def batch(new, past, heads, kv_heads, dim, page, dtype=BF16, device="cpu", seed=0, spare=3, rest=0, front=0, junk=float("nan"), width=None, unused=-7):
+def batch(new, past, heads, kv_heads, dim, page, dtype=BF16, device="cpu", seed=0, spare=3, rest=0, front=0, junk=float("nan"), width=None, unused=-7, only_new=False):
     """A batch in which every slot that belongs to no sequence holds ``junk`` and every table entry beyond a sequence's pages ``unused``; ``front`` and ``rest`` rows of the
-    queries are in front of the first sequence and behind the last."""
+    queries are in front of the first sequence and behind the last.  ``only_new``: one page stands for all that no new token reaches."""
     gen = torch.Generator().manual_seed(seed)
     n = len(new)
     need = [-(-(p + m) // page) for p, m in zip(past, new)]
-    pages = sum(need) + spare
+    begin = [min(p // page, j) if only_new else 0 for p, j in zip(past, need)]
+    pages = sum(need) - sum(begin) + spare
     order = torch.randperm(pages, generator=gen)
     table = torch.full((n, width or max([1, *need])), unused, dtype=torch.int32)
     keys = torch.full((pages, kv_heads, page, dim), junk, dtype=dtype)
     values = torch.full((pages, kv_heads, page, dim), junk, dtype=dtype)
     at = 0
     for s in range(n):
-        table[s, :need[s]] = order[at:at + need[s]].int()
-        at += need[s]
-        for j in range(need[s]):
+        table[s, :begin[s]] = order[-1]
+        table[s, begin[s]:need[s]] = order[at:at + need[s] - begin[s]].int()
+        at += need[s] - begin[s]
+        for j in range(begin[s], need[s]):
             held = min(page, past[s] + new[s] - j * page)
             keys[table[s, j], :, :held] = numbers(gen, kv_heads, held, dim, dtype=dtype)
             values[table[s, j], :, :held] = numbers(gen, kv_heads, held, dim, dtype=dtype)

@@ -263,7 +263,7 @@ def test_append_of_lengths_that_do_not_fit(what):
 @pytest.mark.parametrize("turn", [None, (1.0, False, 1.0), (1.0, True, 1.3), (0.25, False, 0.8), (0.25, True, 1.0), (0.5, False, 1.0)])
 @pytest.mark.parametrize("norms", [False, True])
 def test_append(heads, kv_heads, dim, page, turn, norms):
-    b = batch([1, 3, 0, 40, 1], [255, 0, 9, 17, 131071], heads, kv_heads, dim, page, device="cuda", front=1, rest=2, junk=0.5)
+    b = batch([1, 3, 0, 40, 1], [255, 0, 9, 17, 131071], heads, kv_heads, dim, page, device="cuda", front=1, rest=2, junk=0.5, only_new=True)
     gen = torch.Generator().manual_seed(5)
     part = 0 if turn is None else max(2, int(dim * turn[0]) // 2 * 2)
     rotary = None if turn is None else OF.Rotary(OF.rotary(part, 10000.0, device="cuda").frequencies, turn[1], turn[2])

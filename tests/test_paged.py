@@ -31,7 +31,7 @@ def test_attention_of_ragged_batches(new, past, heads, kv_heads, dim, page, wind
 @pytest.mark.parametrize("norms", [False, True])
 @pytest.mark.parametrize("turn", [None, (8, False, 1.0), (8, True, 1.0), (4, False, 1.25), (6, True, 0.5), (2, False, 1.0)])
 def test_append_with_norms_and_rotation(turn, norms, dtype):
-    b = batch([1, 3, 0, 9], [5, 0, 2, 100003], 6, 2, 8, 4, dtype, front=1, rest=2)
+    b = batch([1, 3, 0, 9], [5, 0, 2, 100003], 6, 2, 8, 4, dtype, front=1, rest=2, only_new=True)
     gen = torch.Generator().manual_seed(5)
     rotary = None if turn is None else OF.Rotary(OF.rotary(turn[0], 1000.0).frequencies, turn[1], turn[2])
     q_norm, k_norm = (1 + numbers(gen, 8, dtype=dtype, scale=0.2) if norms else None for _ in range(2))
