@@ -56,21 +56,18 @@ __device__ __forceinline__ void lg_launch_next() { asm volatile("griddepcontrol.
 
 constexpr int LG_DEPTH = 4;           // vectors of 16 bytes of fp32 of a thread on their way, half as many of bf16
 constexpr int LG_ENTRIES = 24576;     // of a part of the vocabulary at most: 96 KB of counts, two blocks per SM
-constexpr int LG_SEEN_THREADS = 256;  // (that many registers are left beside four blocks of the first kernel)
+constexpr int LG_ALONE = 4096;        // entries of a part where one kernel does both
 constexpr int LG_HELD = 8;            // tokens of a thread at a time; the first of them wait for the first kernel with their results
 
 // WIDE: logits and results of a row lie alike to a 16-byte boundary, and go in 16-byte vectors of the row's own grid, of which the first may begin in front of the
 // row and the last end behind it; else one by one.
+// Bias and mask of the entries [begin, end) of a row; begin may lie up to N - 1 in front of it, on its grid.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(LG_THREADS, 4)
-adjust_stream_kernel(const LogitsParams p, int part) {
+__device__ __forceinline__ void stream_part(const LogitsParams& p, long long row, int begin, int end) {
   constexpr int N = WIDE ? Vec<T>::N : 1, ROUND = LG_THREADS * N, DEPTH = LG_DEPTH * 4 / (N < 4 ? 4 : N);
-  lg_launch_next();
-  const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.logits) + row * p.logits_ld;
   T* y = static_cast<T*>(p.out) + row * p.out_ld;
   const int skew = int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % N);
-  const int begin = blockIdx.y * part - skew, end = int(min((long long)p.vocab, (long long)begin + part));  // (the first part begins up to N - 1 in front of the row)
   const uint32_t* allowed = p.allowed ? p.allowed + row * p.allowed_ld : nullptr;
   const float* wide_bias = p.bias && p.bias_fp32 ? static_cast<const float*>(p.bias) + row * p.bias_ld : nullptr;
   const bf16* narrow_bias = p.bias && !p.bias_fp32 ? static_cast<const bf16*>(p.bias) + row * p.bias_ld : nullptr;
@@ -140,15 +137,29 @@ adjust_stream_kernel(const LogitsParams p, int part) {
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(LG_SEEN_THREADS)
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(LG_THREADS, 4)
+adjust_stream_kernel(const LogitsParams p, int part) {
+  constexpr int N = WIDE ? Vec<T>::N : 1;
+  lg_launch_next();
+  const long long row = blockIdx.x;
+  const int skew = int((reinterpret_cast<uintptr_t>(static_cast<const T*>(p.logits) + row * p.logits_ld) / sizeof(T)) % N);
+  const int begin = blockIdx.y * part - skew;
+  stream_part<T, WIDE>(p, row, begin, int(min((long long)p.vocab, (long long)begin + part)));
+}
+
+// FORM 0: behind the first kernel.  1 and 2: alone, with the stream of its own part in front (in vectors, one by one).
+template <typename T, int FORM>
+__global__ void __launch_bounds__(LG_THREADS, 4)
 adjust_seen_kernel(const LogitsParams p, int part) {
   extern __shared__ __align__(16) uint32_t counts[];
   const long long row = blockIdx.x;
-  const long long begin = (long long)blockIdx.y * part, end = min((long long)p.vocab, begin + part);
   const T* x = static_cast<const T*>(p.logits) + row * p.logits_ld;
   T* y = static_cast<T*>(p.out) + row * p.out_ld;
-  for (int i = threadIdx.x * 4; i < part; i += LG_SEEN_THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
+  // (alone, parts lie on the row's grid of vectors)
+  const long long begin = (long long)blockIdx.y * part - (FORM == 1 ? int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % Vec<T>::N) : 0);
+  const long long end = min((long long)p.vocab, begin + part);
+  for (int i = threadIdx.x * 4; i < part; i += LG_THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
   int length = p.lengths ? __ldg(p.lengths + row) : p.width;
   const int prompt = p.prompts ? __ldg(p.prompts + row) : 0;
   if (length < 0 || length > p.width || prompt < 0) {
@@ -162,7 +173,7 @@ adjust_seen_kernel(const LogitsParams p, int part) {
   const long long* said = p.tokens + row * p.tokens_ld;
   auto entry = [&](int i) {  // of token i in the counts, -1: not of this part
     const long long token = __ldg(said + i);
-    return token >= begin && token < end ? int(token - begin) : -1;
+    return token >= max(begin, 0LL) && token < end ? int(token - begin) : -1;
   };
   auto count = [&](int at, int i) {
     if (at < 0) return;
@@ -175,7 +186,7 @@ adjust_seen_kernel(const LogitsParams p, int part) {
   float value[LG_HELD];
   auto entries = [&](int from) {
 #pragma unroll
-    for (int j = 0; j < LG_HELD; ++j) at[j] = from + j * LG_SEEN_THREADS < length ? entry(from + j * LG_SEEN_THREADS) : -1;
+    for (int j = 0; j < LG_HELD; ++j) at[j] = from + j * LG_THREADS < length ? entry(from + j * LG_THREADS) : -1;
   };
   // the logits of entries that nobody has taken yet; the others' places become -1.  (All loads of one kind behind one another, not a token's.)
   auto take = [&]() {
@@ -212,16 +223,17 @@ adjust_seen_kernel(const LogitsParams p, int part) {
       if (at[j] >= 0) lg_store(y + begin + at[j], value[j]);
   };
   entries(threadIdx.x);
+  if (FORM) stream_part<T, FORM == 1>(p, row, int(begin), int(end));
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < LG_HELD; ++j) count(at[j], threadIdx.x + j * LG_SEEN_THREADS);
+  for (int j = 0; j < LG_HELD; ++j) count(at[j], threadIdx.x + j * LG_THREADS);
 #pragma unroll 4
-  for (int i = threadIdx.x + LG_HELD * LG_SEEN_THREADS; i < length; i += LG_SEEN_THREADS) count(entry(i), i);
+  for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_THREADS) count(entry(i), i);
   __syncthreads();
   take();
-  lg_wait_prior();
+  if (!FORM) lg_wait_prior();
   store();
-  for (int i = threadIdx.x + LG_HELD * LG_SEEN_THREADS; i < length; i += LG_HELD * LG_SEEN_THREADS) {
+  for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_HELD * LG_THREADS) {
     entries(i);
     take();
     store();
@@ -238,23 +250,18 @@ static int lg_stream(const LogitsParams& p, int rows, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
-template <typename T>
-static int lg_seen(const LogitsParams& p, int rows, cudaStream_t stream) {
+template <typename T, int FORM>
+static int lg_seen(const LogitsParams& p, int rows, int part, int parts, cudaStream_t stream) {
   static std::atomic<bool> ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TPB_ERR_CUDA;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(adjust_seen_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_ENTRIES * 4) != cudaSuccess) return TPB_ERR_CUDA;
+    if (cudaFuncSetAttribute(adjust_seen_kernel<T, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_ENTRIES * 4) != cudaSuccess) return TPB_ERR_CUDA;
     ready[dev].store(true, std::memory_order_release);
   }
-  // entries of a block: as few parts as fit where there are blocks enough for the SMs, shorter ones else
-  const long long least = (p.vocab + (long long)LG_ENTRIES - 1) / LG_ENTRIES, parts = max(least, min(148LL / rows, ((long long)p.vocab + 4095) / 4096));
   if (parts > 65535) return TPB_ERR_SIZE;
-  const int part = int((((p.vocab + parts - 1) / parts) + 3) / 4 * 4);
-  return launch_dependent(adjust_seen_kernel<T>, dim3(rows, unsigned((p.vocab + (long long)part - 1) / part)), dim3(LG_SEEN_THREADS), size_t(part) * 4, stream, true, p, part) ==
-                 cudaSuccess
-             ? TPB_OK
-             : TPB_ERR_CUDA;
+  return launch_dependent(adjust_seen_kernel<T, FORM>, dim3(rows, unsigned(parts)), dim3(LG_THREADS), size_t(part) * 4, stream, FORM == 0, p, part) == cudaSuccess ? TPB_OK
+                                                                                                                                                               : TPB_ERR_CUDA;
 }
 
 template <typename T>
@@ -262,8 +269,21 @@ static int lg_launch(const LogitsParams& p, int rows, cudaStream_t stream) {
   constexpr int N = Vec<T>::N;
   auto place = [](const void* t) { return reinterpret_cast<uintptr_t>(t) / sizeof(T) % N; };
   const bool wide = place(p.logits) == place(p.out) && (rows == 1 || (p.logits_ld - p.out_ld) % N == 0);
+  const bool history = p.tokens && p.width;
+  const long long entries = (long long)p.vocab + N - 1;
+  if (history && rows * entries <= 148LL * 4 * LG_ALONE) {
+    // short parts for each SM to have one, in whole vectors
+    const long long blocks = max(1LL, 148LL * 2 / rows);
+    const int part = int(min((long long)LG_ALONE, max(1024LL, ((entries + blocks - 1) / blocks + 31) / 32 * 32)));
+    const int parts = int((entries + part - 1) / part);
+    return wide ? lg_seen<T, 1>(p, rows, part, parts, stream) : lg_seen<T, 2>(p, rows, part, parts, stream);
+  }
   const int rc = wide ? lg_stream<T, true>(p, rows, stream) : lg_stream<T, false>(p, rows, stream);
-  return rc != TPB_OK || !p.tokens || !p.width ? rc : lg_seen<T>(p, rows, stream);
+  if (rc != TPB_OK || !history) return rc;
+  // as few parts as fit where there are blocks enough for the SMs, shorter ones else
+  const long long parts = max((p.vocab + (long long)LG_ENTRIES - 1) / LG_ENTRIES, min(148LL / rows, (p.vocab + 4095LL) / 4096));
+  const int part = int((((p.vocab + parts - 1) / parts) + 3) / 4 * 4);
+  return lg_seen<T, 0>(p, rows, part, int((p.vocab + (long long)part - 1) / part), stream);
 }
 
 }  // namespace tpb
