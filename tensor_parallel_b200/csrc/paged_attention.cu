@@ -86,10 +86,10 @@ struct Few {
   static constexpr int WARPS = R == 1 ? 4 : 8;
   static constexpr int KEY_GROUPS = WARPS / R;
   static constexpr int KEYS = PA_TILE / KEY_GROUPS;  // of a warp
-  static constexpr int CTAS = R == 1 ? 2 : 1;        // per SM
+  static constexpr int CTAS = R > 1 ? 1 : D == 64 ? 3 : 2;  // per SM
   static constexpr int DB = D / 64;
   static constexpr int STAGE_BYTES = 2 * DB * PA_BLOCK;
-  static constexpr int STAGES = (R == 1 ? 96 : 160) * 1024 / STAGE_BYTES;
+  static constexpr int STAGES = (R > 1 ? 160 : D == 64 ? 64 : 96) * 1024 / STAGE_BYTES;
   static constexpr int Q_BYTES = ROWS * D * 2;
   static constexpr int MERGE_COLS = STAGE_BYTES / (WARPS * 16 * 4) < D ? STAGE_BYTES / (WARPS * 16 * 4) : D;  // that the partial results of all warps fill a stage with
   static constexpr int THREADS = WARPS * 32 + 32;
@@ -282,9 +282,8 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     meet_phase ^= 1;
     return ok;
   };
-  for (int it = 0;; ++it) {
-    const int stage = it % STAGES;
-    ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait(&full[stage], (it / STAGES) & 1));
+  for (int stage = 0, phase = 0;; phase ^= stage == STAGES - 1, stage = stage == STAGES - 1 ? 0 : stage + 1) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase));
     if (!ok) break;
     const int2 info = stage_info[stage];
     if (info.y & RANGE_END) break;
@@ -313,32 +312,49 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       }
     }
     poisoned |= (info.y & PIECE_POISON) != 0;
-    // ---- scores ----
+    // ---- scores: all fragments of 16 keys in front of the products, which go in two chains (what bounds a tile is the length of its chain) ----
     float sc[NT][4];
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
     const uint32_t k_a = ring_a + stage * C::STAGE_BYTES, v_a = k_a + DB * PA_BLOCK;
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      uint32_t a[4];
-      if (R == 1) {
+    for (int np = 0; np < NT / 2; ++np) {
+      uint32_t kf[D / 16][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = qf[R == 1 ? kk : 0][j];
-      } else {
-        const int r = rg * 16 + (mi & 1) * 8 + mr, c = kk * 2 + (mi >> 1);
-        ldsm4(a, q_a + (piece & 1) * C::Q_BYTES + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const int r = key_off + np * 16 + (mi >> 1) * 8 + mr, c = kk * 2 + (mi & 1);
+        ldsm4(kf[kk], k_a + (c >> 3) * PA_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+      }
+      float odd[2][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[2 * np][j] = sc[2 * np + 1][j] = odd[0][j] = odd[1][j] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t a[4];
+        if (R == 1) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[j] = qf[R == 1 ? kk : 0][j];
+        } else {
+          const int r = rg * 16 + (mi & 1) * 8 + mr, c = kk * 2 + (mi >> 1);
+          ldsm4(a, q_a + (piece & 1) * C::Q_BYTES + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        }
+        mma16816(kk & 1 ? odd[0] : sc[2 * np], a, kf[kk][0], kf[kk][1]);
+        mma16816(kk & 1 ? odd[1] : sc[2 * np + 1], a, kf[kk][2], kf[kk][3]);
       }
 #pragma unroll
-      for (int np = 0; np < NT / 2; ++np) {
-        uint32_t b[4];
-        const int r = key_off + np * 16 + (mi >> 1) * 8 + mr, c = kk * 2 + (mi & 1);
-        ldsm4(b, k_a + (c >> 3) * PA_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-        mma16816(sc[2 * np], a, b[0], b[1]);
-        mma16816(sc[2 * np + 1], a, b[2], b[3]);
+      for (int j = 0; j < 4; ++j) {
+        sc[2 * np][j] += odd[0][j];
+        sc[2 * np + 1][j] += odd[1][j];
       }
     }
+    // the values of the first 16 keys come while the probabilities are made
+    uint32_t vf[D / 16][4];
+    auto load_values = [&](int ks) {
+#pragma unroll
+      for (int dn = 0; dn < D / 16; ++dn) {
+        const int r = key_off + ks * 16 + (mi & 1) * 8 + mr, c = dn * 2 + (mi >> 1);
+        ldsm4_t(vf[dn], v_a + (c >> 3) * PA_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+      }
+    };
+    load_values(0);
     // ---- mask, maximum, probabilities ----
     const int last_pos = pc.past + (pc.row0 + pc.rows - 1) / p.group;
     const bool plain = key0 + C::KEYS - 1 <= pc.past + pc.row0 / p.group && (!p.window || key0 > last_pos - p.window);
@@ -400,17 +416,15 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           keep[i] = (key >= pc.low && key < pc.total ? 0xffffu : 0u) | (key + 1 >= pc.low && key + 1 < pc.total ? 0xffff0000u : 0u);
         }
       }
+      if (ks) load_values(ks);
 #pragma unroll
       for (int dn = 0; dn < D / 16; ++dn) {
-        uint32_t b[4];
-        const int r = key_off + ks * 16 + (mi & 1) * 8 + mr, c = dn * 2 + (mi >> 1);
-        ldsm4_t(b, v_a + (c >> 3) * PA_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
         if (cut) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] &= keep[j & 1];
+          for (int j = 0; j < 4; ++j) vf[dn][j] &= keep[j & 1];
         }
-        mma16816(o[2 * dn], a, b[0], b[1]);
-        mma16816(o[2 * dn + 1], a, b[2], b[3]);
+        mma16816(o[2 * dn], a, vf[dn][0], vf[dn][1]);
+        mma16816(o[2 * dn + 1], a, vf[dn][2], vf[dn][3]);
       }
     }
     if (!(info.y & PIECE_LAST)) {
@@ -568,7 +582,7 @@ static PagedPlan pa_plan(int n, int tokens, int table_width, int page_shift, int
   if (few) {
     const long long tiles = min((long long)tokens * group / rows + n, (long long)n * ((min(most_rows, (long long)plan.few_high) + rows - 1) / rows)) * kv_heads;
     const long long most = tiles * ((keys + PA_TILE - 1) / PA_TILE + PA_PIECE_COST);
-    plan.few_grid = int(max(1LL, min((long long)pa_sms() * (plan.row_groups == 1 ? 2 : 1), (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE)));
+    plan.few_grid = int(max(1LL, min((long long)pa_sms() * (plan.row_groups > 1 ? 1 : head_dim == 64 ? Few<64, 1>::CTAS : Few<128, 1>::CTAS), (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE)));
     plan.few_floats = (long long)plan.few_grid * 2 * (rows * (head_dim + 2) + 4);
   }
   if (wide) {
