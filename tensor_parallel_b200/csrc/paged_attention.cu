@@ -33,6 +33,7 @@ constexpr int PA_BLOCK = PA_TILE * 128;     // bytes of a swizzled block of 64 k
 constexpr int PA_MIN_SHARE = 3;             // of a CTA's range, at least: a piece and two tiles
 // What a row tile costs beside its key tiles, in tiles: its query rows, the meeting of the key groups, its result.  It stands in front of them on the line.
 constexpr int PA_PIECE_COST = 1;
+constexpr float PA_RESCALE_LOG2 = 8.f;
 
 // A sequence as this launch deals with it.
 struct PagedUnits {
@@ -66,6 +67,12 @@ struct PagedPiece {  // of a row tile's keys, as the producer hands it to the co
   int bad;
 };
 
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const void* tmap, uint64_t* bar, int x, int y, int z, int w, int v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+      : "memory");
+}
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -156,7 +163,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     const int page_size = 1 << p.b.page_shift;
     const int per_tile = max(1, PA_TILE >> p.b.page_shift);  // pages of a tile
     const int box_rows = min(page_size, PA_TILE);
-    const int my_page = lane / (2 * DB), my_block = lane % (2 * DB);  // the box of this lane
+    const int my_page = lane / 2, box_bytes = box_rows * 128 * DB;  // the box of this lane: keys or values of a page
     int seq = range.seq, it = 0, piece = 0;
     long long at = w0, seq_begin = range.begin;
     bool ok = true;
@@ -170,12 +177,13 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         continue;
       }
       const int length = u.tiles + PA_PIECE_COST;
-      const long long unit = (at - seq_begin) / length;
-      const int from = int((at - seq_begin) - unit * length), to = int(min((long long)length, from + (w1 - at)));
+      const long long into = at - seq_begin;
+      const long long unit = into < INT_MAX ? int(into) / length : into / length;  // (64-bit divisions are long)
+      const int from = int(into - unit * length), to = int(min((long long)length, from + (w1 - at)));
       const int t0 = max(0, from - PA_PIECE_COST), t1 = max(0, to - PA_PIECE_COST);
       at += to - from;
       if (t0 == t1) continue;  // (the range ends in front of the first tile)
-      const int kvh = int(unit % p.kv_heads), row0 = int(unit / p.kv_heads) * ROWS;
+      const int kvh = int(unit) % p.kv_heads, row0 = int(unit) / p.kv_heads * ROWS;
       const int total = u.s.bad ? 0 : u.s.past + u.s.fresh;
       const int low = p.window && !u.s.bad ? max(0, u.s.past - p.window + 1) : 0;
       const int qb = piece & 1;
@@ -207,12 +215,21 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         }
       }
       {
-        const int chunks = ROWS * (D / 8), left = u.rows - row0;
-        for (int c = lane; c < chunks; c += 32) {
-          const int r = c / (D / 8), e = c % (D / 8);
-          const int t = (row0 + min(r, left - 1)) / p.group, g = (row0 + min(r, left - 1)) % p.group;
-          const bf16* src = p.q + (long long)(u.s.token0 + t) * p.q_st + (long long)(kvh * p.group + g) * p.q_sh + e * 8;
-          cp_async16(smem_u32(q_s + qb * C::Q_BYTES + (e >> 3) * (ROWS * 128) + r * 128 + (((e & 7) ^ (r & 7)) << 4)), src, r < left ? 16 : 0);
+        constexpr int STEP = 32 / (D / 8);  // rows at a time
+        const int e = lane % (D / 8), left = u.rows - row0;
+        const int step_tokens = STEP / p.group, step_heads = STEP % p.group;
+        int r = lane / (D / 8), t = (row0 + r) / p.group, g = (row0 + r) % p.group;
+        const bf16* base = p.q + (long long)u.s.token0 * p.q_st + (long long)kvh * p.group * p.q_sh + e * 8;
+        const uint32_t to = smem_u32(q_s + qb * C::Q_BYTES + (e >> 3) * (ROWS * 128));
+#pragma unroll
+        for (int i = 0; i < ROWS / STEP; ++i, r += STEP) {
+          cp_async16(to + r * 128 + (((e & 7) ^ (r & 7)) << 4), r < left ? base + t * p.q_st + g * p.q_sh : base, r < left ? 16 : 0);
+          t += step_tokens;
+          g += step_heads;
+          if (g >= p.group) {
+            g -= p.group;
+            ++t;
+          }
         }
         cp_async_arrive(&q_full[qb]);
         __syncwarp();
@@ -231,7 +248,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         }
         const int page = __shfl_sync(0xffffffffu, now, (e + my_page) & 31);
         const int first = key0 + my_page * page_size;  // (of pages shorter than a tile; longer ones have one box, with keys of use in it)
-        const bool wanted = lane < per_tile * 2 * DB && (per_tile == 1 || (first < total && first + page_size > low)) && total > 0;
+        const bool wanted = lane < per_tile * 2 && (per_tile == 1 || (first < total && first + page_size > low)) && total > 0;
         const bool good = wanted && page >= 0 && page < p.b.pages;
         const uint32_t boxes = __ballot_sync(0xffffffffu, good), lost = __ballot_sync(0xffffffffu, wanted && !good);
         ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait(&empty[stage], ((it / STAGES) & 1) ^ 1));
@@ -239,12 +256,12 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         if (lane == 0) {
           if (lost) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
           stage_info[stage] = make_int2(key0, (t == t0 ? PIECE_FIRST : 0) | (t == t1 - 1 ? PIECE_LAST : 0) | (lost ? PIECE_POISON : 0));
-          mbar_expect_tx(&full[stage], __popc(boxes) * box_rows * 128);
+          mbar_expect_tx(&full[stage], __popc(boxes) * box_bytes);
         }
         __syncwarp();
         if (good)
-          tma_load_4d(ring + stage * C::STAGE_BYTES + my_block * PA_BLOCK + my_page * box_rows * 128, my_block < DB ? &tmap_k : &tmap_v, &full[stage],
-                      (my_block % DB) * 64, per_tile == 1 ? key0 & (page_size - 1) : 0, kvh, page);
+          tma_load_5d(ring + stage * C::STAGE_BYTES + (lane & 1) * (DB * PA_BLOCK) + my_page * box_bytes, lane & 1 ? &tmap_v : &tmap_k, &full[stage], 0,
+                      per_tile == 1 ? key0 & (page_size - 1) : 0, 0, kvh, page);
       }
       if (!ok) break;
       ++piece;
@@ -267,11 +284,19 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   const int key_off = kg * C::KEYS;
   const int g8 = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;
   const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(q_s);
+  // a stage holds page by page, in each its blocks of 64 elements; 16 keys are always of one page
+  const int box_shift = min(p.b.page_shift, 6), block_step = 128 << box_shift;
+  uint32_t group_a[NT / 2];
+#pragma unroll
+  for (int i = 0; i < NT / 2; ++i) {
+    const int key = key_off + i * 16;
+    group_a[i] = (key >> box_shift) * (block_step * DB) + (key & ((1 << box_shift) - 1)) * 128;
+  }
   float o[D / 8][4];
   float m[2], l[2];
   uint32_t qf[R == 1 ? D / 16 : 1][4];
   PagedPiece pc = {};
-  int pos[2] = {0, 0}, piece = 0;
+  int pos[2] = {0, 0}, piece = 0, plain_from = 0, plain_to = 0;
   uint32_t meet_phase = 0;
   bool poisoned = false;
   bool ok = true;
@@ -299,6 +324,9 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         m[i] = -INFINITY;
         l[i] = 0.f;
       }
+      // the warp's keys of a tile need no mask if they begin in [plain_from, plain_to]
+      plain_from = p.window ? pc.past + (pc.row0 + pc.rows - 1) / p.group - p.window + 1 : 0;
+      plain_to = pc.past + pc.row0 / p.group + 1 - C::KEYS;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
 #pragma unroll
@@ -320,8 +348,8 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       uint32_t kf[D / 16][4];
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const int r = key_off + np * 16 + (mi >> 1) * 8 + mr, c = kk * 2 + (mi & 1);
-        ldsm4(kf[kk], k_a + (c >> 3) * PA_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        const int c = kk * 2 + (mi & 1);
+        ldsm4(kf[kk], k_a + group_a[np] + (kk >> 2) * block_step + ((mi >> 1) * 8 + mr) * 128 + (((c & 7) ^ mr) << 4));
       }
       float odd[2][4];
 #pragma unroll
@@ -350,39 +378,34 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     auto load_values = [&](int ks) {
 #pragma unroll
       for (int dn = 0; dn < D / 16; ++dn) {
-        const int r = key_off + ks * 16 + (mi & 1) * 8 + mr, c = dn * 2 + (mi >> 1);
-        ldsm4_t(vf[dn], v_a + (c >> 3) * PA_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        const int c = dn * 2 + (mi >> 1);
+        ldsm4_t(vf[dn], v_a + group_a[ks] + (dn >> 2) * block_step + ((mi & 1) * 8 + mr) * 128 + (((c & 7) ^ mr) << 4));
       }
     };
     load_values(0);
-    // ---- mask, maximum, probabilities ----
-    const int last_pos = pc.past + (pc.row0 + pc.rows - 1) / p.group;
-    const bool plain = key0 + C::KEYS - 1 <= pc.past + pc.row0 / p.group && (!p.window || key0 > last_pos - p.window);
+    // ---- mask, maximum, probabilities (2^(score - m), scores in powers of two) ----
+    if (key0 < plain_from || key0 > plain_to) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = key0 + i * 8 + t4 * 2 + (j & 1), at = pos[j >> 1];
+          if (key > at || (p.window && key <= at - p.window)) sc[i][j] = -INFINITY;
+        }
+    }
     float mt[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v = sc[i][j] * p.scale_log2e;
-        if (!plain) {
-          const int key = key0 + i * 8 + t4 * 2 + (j & 1), at = pos[j >> 1];
-          if (key > at || (p.window && key <= at - p.window)) v = -INFINITY;
-        }
-        sc[i][j] = v;
-        mt[j >> 1] = fmaxf(mt[j >> 1], v);
-      }
-    bool rises = false;
-    float base[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 1));
-      mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 2));
-      rises |= mt[i] > m[i];
-    }
-    if (__any_sync(0xffffffffu, rises)) {
+      for (int j = 0; j < 4; j += 2) mt[j >> 1] = fmax3(mt[j >> 1], sc[i][j], sc[i][j + 1]);
+    // the maximum is followed when it rises by more than 2^8, which is rare behind the first tiles (it cancels in the quotient; the scale is positive);
+    // only then do the four lanes of a row need to know each other's
+    if (__any_sync(0xffffffffu, mt[0] * p.scale_log2e > m[0] + PA_RESCALE_LOG2 || mt[1] * p.scale_log2e > m[1] + PA_RESCALE_LOG2)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float mn = fmaxf(m[i], mt[i]);
+        mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 1));
+        mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 2));
+        const float mn = fmaxf(m[i], mt[i] * p.scale_log2e);
         const float f = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - mn);
         m[i] = mn;
         l[i] *= f;
@@ -393,15 +416,16 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         }
       }
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i];
+    const float base[2] = {m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]};
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sc[i][j] = ex2_approx(sc[i][j] - base[j >> 1]);
-        l[j >> 1] += sc[i][j];
-      }
+      for (int j = 0; j < 4; ++j) sc[i][j] = ex2_approx(fmaf(sc[i][j], p.scale_log2e, base[j >> 1]));
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      l[0] += sc[i][0] + sc[i][1];
+      l[1] += sc[i][2] + sc[i][3];
+    }
     // ---- values ----
     const bool cut = key0 < pc.low || key0 + C::KEYS > pc.total;
 #pragma unroll
@@ -640,14 +664,14 @@ extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
   float* room = static_cast<float*>(a->workspace);
   const PagedParts few = pa_parts(room, plan.few_grid, 16 * plan.row_groups, a->head_dim), wide = pa_parts(room, plan.wide_grid, PW_ROWS, a->head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
-  auto maps = [&](CUtensorMap& k, CUtensorMap& v, int tile) {
+  auto maps = [&](auto paged_map, CUtensorMap& k, CUtensorMap& v, int tile) {
     const int box = min(a->page_size, tile);
-    const int r = paged_tmap(&k, a->keys, a->head_dim, a->page_size, a->kv_heads, a->pages, a->k_ss, a->k_sh, a->k_sp, box);
-    return r != TPB_OK ? r : paged_tmap(&v, a->values, a->head_dim, a->page_size, a->kv_heads, a->pages, a->v_ss, a->v_sh, a->v_sp, box);
+    const int r = paged_map(&k, a->keys, a->head_dim, a->page_size, a->kv_heads, a->pages, a->k_ss, a->k_sh, a->k_sp, box);
+    return r != TPB_OK ? r : paged_map(&v, a->values, a->head_dim, a->page_size, a->kv_heads, a->pages, a->v_ss, a->v_sh, a->v_sp, box);
   };
   CUtensorMap k, v;
   if (plan.few_grid) {
-    rc = maps(k, v, PA_TILE);
+    rc = maps(paged_blocks_tmap, k, v, PA_TILE);
     if (rc != TPB_OK) return rc;
     p.parts = few;
     p.rows_low = 1, p.rows_high = plan.few_high;
@@ -660,7 +684,7 @@ extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
     if (rc != TPB_OK) return rc;
   }
   if (plan.wide_grid) {
-    if (!plan.few_grid || a->page_size > PA_TILE) rc = maps(k, v, pw_tile(a->head_dim));
+    rc = maps(paged_tmap, k, v, pw_tile(a->head_dim));
     if (rc != TPB_OK) return rc;
     p.parts = wide;
     p.rows_low = plan.few_high + 1, p.rows_high = INT_MAX;
