@@ -141,6 +141,7 @@ template <typename T, bool WIDE>
 __global__ void __launch_bounds__(LG_THREADS, 4)
 adjust_stream_kernel(const LogitsParams p, int part) {
   constexpr int N = WIDE ? Vec<T>::N : 1;
+  lg_wait_prior();  // (launched ahead of the previous kernel's end: nothing is read or written before that)
   lg_launch_next();
   const long long row = blockIdx.x;
   const int skew = int((reinterpret_cast<uintptr_t>(static_cast<const T*>(p.logits) + row * p.logits_ld) / sizeof(T)) % N);
@@ -160,6 +161,10 @@ adjust_seen_kernel(const LogitsParams p, int part) {
   const long long begin = (long long)blockIdx.y * part - (FORM == 1 ? int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % Vec<T>::N) : 0);
   const long long end = min((long long)p.vocab, begin + part);
   for (int i = threadIdx.x * 4; i < part; i += LG_THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
+  if (FORM) {
+    lg_wait_prior();
+    lg_launch_next();
+  }
   int length = p.lengths ? __ldg(p.lengths + row) : p.width;
   const int prompt = p.prompts ? __ldg(p.prompts + row) : 0;
   if (length < 0 || length > p.width || prompt < 0) {
@@ -231,7 +236,10 @@ adjust_seen_kernel(const LogitsParams p, int part) {
   for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_THREADS) count(entry(i), i);
   __syncthreads();
   take();
-  if (!FORM) lg_wait_prior();
+  if (!FORM) {
+    lg_wait_prior();
+    lg_launch_next();
+  }
   store();
   for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_HELD * LG_THREADS) {
     entries(i);
@@ -246,8 +254,8 @@ static int lg_stream(const LogitsParams& p, int rows, cudaStream_t stream) {
   // entries of a block: a row's over as many as make four blocks per SM of all rows, whole rounds
   const long long entries = (long long)p.vocab + N - 1, blocks = max(1LL, 148LL * 4 / rows);
   const long long part = min((1LL << 30) / ROUND * ROUND, ((entries + blocks - 1) / blocks + ROUND - 1) / ROUND * ROUND);
-  adjust_stream_kernel<T, WIDE><<<dim3(rows, unsigned((entries + part - 1) / part)), LG_THREADS, 0, stream>>>(p, int(part));
-  return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  return launch_dependent(adjust_stream_kernel<T, WIDE>, dim3(rows, unsigned((entries + part - 1) / part)), dim3(LG_THREADS), 0, stream, true, p, int(part)) == cudaSuccess ? TPB_OK
+                                                                                                                                                                    : TPB_ERR_CUDA;
 }
 
 template <typename T, int FORM>
@@ -260,7 +268,7 @@ static int lg_seen(const LogitsParams& p, int rows, int part, int parts, cudaStr
     ready[dev].store(true, std::memory_order_release);
   }
   if (parts > 65535) return TPB_ERR_SIZE;
-  return launch_dependent(adjust_seen_kernel<T, FORM>, dim3(rows, unsigned(parts)), dim3(LG_THREADS), size_t(part) * 4, stream, FORM == 0, p, part) == cudaSuccess ? TPB_OK
+  return launch_dependent(adjust_seen_kernel<T, FORM>, dim3(rows, unsigned(parts)), dim3(LG_THREADS), size_t(part) * 4, stream, true, p, part) == cudaSuccess ? TPB_OK
                                                                                                                                                                : TPB_ERR_CUDA;
 }
 

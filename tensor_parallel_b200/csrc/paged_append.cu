@@ -114,6 +114,8 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
     }
     step(next);
   };
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched ahead of the previous kernel's end: nothing is read or written before that)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j) fetch(raw[j]);
 
@@ -282,15 +284,12 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
 }
 
 template <int LANES>
-static void ap_launch(const AppendParams& p, dim3 grid, int per_block, cudaStream_t stream) {
-  if (!p.half)
-    paged_append_kernel<LANES, TURN_NONE><<<grid, AP_THREADS, 0, stream>>>(p, per_block);
-  else if (p.interleaved)
-    paged_append_kernel<LANES, TURN_PAIRS><<<grid, AP_THREADS, 0, stream>>>(p, per_block);
-  else if (p.half % 8 == 0)
-    paged_append_kernel<LANES, TURN_HALVES><<<grid, AP_THREADS, 0, stream>>>(p, per_block);
-  else
-    paged_append_kernel<LANES, TURN_ODD><<<grid, AP_THREADS, 0, stream>>>(p, per_block);
+static cudaError_t ap_launch(const AppendParams& p, dim3 grid, int per_block, cudaStream_t stream) {
+  auto kernel = !p.half            ? paged_append_kernel<LANES, TURN_NONE>
+                : p.interleaved     ? paged_append_kernel<LANES, TURN_PAIRS>
+                : p.half % 8 == 0   ? paged_append_kernel<LANES, TURN_HALVES>
+                                    : paged_append_kernel<LANES, TURN_ODD>;
+  return launch_dependent(kernel, grid, dim3(AP_THREADS), 0, stream, true, p, per_block);
 }
 
 }  // namespace tpb
@@ -326,11 +325,6 @@ extern "C" int tpb_paged_append(const tpb_paged_append_t* a, void* stream_) {
   const int per_block = a->tokens >= 148 * 4 * AP_TOKENS ? AP_TOKENS : a->tokens >= 148 * 4 * 2 ? 2 : 1;
   const dim3 grid((a->tokens + per_block - 1) / per_block, a->tokens >= 148 * 4 ? 1 : (rows + groups - 1) / groups);
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
-  if (lanes == 4)
-    ap_launch<4>(p, grid, per_block, s);
-  else if (lanes == 8)
-    ap_launch<8>(p, grid, per_block, s);
-  else
-    ap_launch<16>(p, grid, per_block, s);
-  return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  const cudaError_t launched = lanes == 4 ? ap_launch<4>(p, grid, per_block, s) : lanes == 8 ? ap_launch<8>(p, grid, per_block, s) : ap_launch<16>(p, grid, per_block, s);
+  return launched == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }

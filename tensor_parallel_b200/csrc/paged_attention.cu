@@ -142,8 +142,9 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     *abort_flag = 0;
     fence_mbar_init();
   }
+  pa_wait_prior();  // (launched ahead of the previous kernel's end: nothing is read or written before that)
+  pa_launch_next();
   if (threadIdx.x < 2) p.parts.joins[2 * blockIdx.x + threadIdx.x] = make_int4(-1, 0, 0, 0);
-  pa_launch_next();  // (the whole grid is resident; the joining kernel waits for its end)
 
   long long share, w0, w1;
   share_out<C::THREADS>(p.b.n, PA_MIN_SHARE, range, [&](int i) {
@@ -208,11 +209,6 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         o.bad = u.s.bad;
         // keys that begin in this range and end in another's are joined by the block of this CTA; its other piece continues the range in front
         o.slot = t0 == 0 && t1 == u.tiles ? -1 : 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
-        if (t0 == 0 && t1 < u.tiles) {
-          const long long unit_end = seq_begin + (unit + 1) * length;
-          p.parts.joins[2 * blockIdx.x] = make_int4(o.token0, row0, o.rows, kvh);
-          p.parts.joins[2 * blockIdx.x + 1] = make_int4(int((unit_end - 1) / share), 0, 0, 0);
-        }
       }
       {
         constexpr int STEP = 32 / (D / 8);  // rows at a time
@@ -265,6 +261,11 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       }
       if (!ok) break;
       ++piece;
+      if (t0 == 0 && t1 < u.tiles && lane == 0) {
+        const long long unit_end = seq_begin + (unit + 1) * length;
+        p.parts.joins[2 * blockIdx.x] = make_int4(u.s.token0, row0, min(ROWS, u.rows - row0), kvh);
+        p.parts.joins[2 * blockIdx.x + 1] = make_int4(int((unit_end - 1) / share), 0, 0, 0);
+      }
     }
     if (ok) {
       const int stage = it % STAGES;
@@ -537,6 +538,7 @@ paged_attn_join_kernel(const PagedAttnParams p, const PagedParts few, int few_gr
   const PagedParts parts = is_wide ? wide : few;
   const int c = blockIdx.x - (is_wide ? few_grid : 0);
   pa_wait_prior();
+  pa_launch_next();
   const int4 unit = parts.joins[2 * c];
   const int last = parts.joins[2 * c + 1].x;
   if (unit.x < 0) return;
@@ -583,8 +585,7 @@ static int pa_few_launch(const PagedAttnParams& p, const CUtensorMap& k, const C
     if (cudaFuncSetAttribute(paged_attn_few_kernel<D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return TPB_ERR_CUDA;
     ready[dev].store(true, std::memory_order_release);
   }
-  paged_attn_few_kernel<D, R><<<grid, C::THREADS, C::SMEM, stream>>>(k, v, p);
-  return cudaGetLastError() == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  return launch_dependent(paged_attn_few_kernel<D, R>, dim3(grid), dim3(C::THREADS), C::SMEM, stream, true, k, v, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
 // What a call launches.  Sequences with few query rows (new tokens x query heads of a KV head) go by the kernel above, bound by memory; those with more by the one

@@ -71,7 +71,7 @@ __device__ __forceinline__ void tm_store(uint32_t at, const uint32_t (&r)[32]) {
 template <int D, int N>
 __global__ void __launch_bounds__(PW_THREADS, Wide<D, N>::CTAS)
 paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                       const PagedAttnParams p, const int boxed) {
+                       const PagedAttnParams p, const int boxed, const int ahead) {
   using C = Wide<D, N>;
   constexpr int DB = C::DB, W = C::W;
   constexpr uint32_t Q_BYTES = C::Q_BYTES, T_BYTES = C::T_BYTES;
@@ -128,12 +128,14 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     *abort_flag = 0;
     fence_mbar_init();
   }
+  // beside the launch for few rows, which has waited for what is in front of it, before this one was let in: its end is awaited at this one's
+  if (!ahead) pa_wait_prior();
+  pa_launch_next();
   if (threadIdx.x < 2) p.parts.joins[2 * blockIdx.x + threadIdx.x] = make_int4(-1, 0, 0, 0);
   if (warp == 1) {
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
-  pa_launch_next();
   auto units_of = [&](int i, PagedSequence& s, int& rows) {  // row tiles of a sequence that is this launch's
     s = paged_sequence(p.b, i);
     rows = s.fresh * p.group;
@@ -581,7 +583,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
-  pa_wait_prior();  // (launched ahead of the kernel in front: whoever waits for this one waits for both)
+  if (ahead) pa_wait_prior();  // (whoever waits for this launch waits for both)
 }
 
 template <int D, int N>
@@ -598,7 +600,7 @@ static int pw_go(const PagedAttnParams& p, const CUtensorMap& k, const CUtensorM
   CUtensorMap q = k;
   bool boxed = PW_M % p.group == 0 && (p.b.tokens == 1 || p.q_st > 0) && (p.heads == 1 || p.q_sh > 0);
   if (boxed) boxed = paged_rows_tmap(&q, p.q, D, p.heads, p.b.tokens, p.q_sh, p.q_st, p.group, PW_M / p.group) == TPB_OK;
-  return launch_dependent(paged_attn_wide_kernel<D, N>, dim3(grid), dim3(PW_THREADS), C::SMEM, stream, ahead, q, k, v, p, int(boxed)) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  return launch_dependent(paged_attn_wide_kernel<D, N>, dim3(grid), dim3(PW_THREADS), C::SMEM, stream, true, q, k, v, p, int(boxed), int(ahead)) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
 int pw_tile(int head_dim) { return head_dim; }
