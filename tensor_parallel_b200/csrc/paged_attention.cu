@@ -34,6 +34,9 @@ constexpr int PA_MIN_SHARE = 3;             // of a CTA's range, at least: a pie
 // What a row tile costs beside its key tiles, in tiles: its query rows, the meeting of the key groups, its result.  It stands in front of them on the line.
 constexpr int PA_PIECE_COST = 1;
 constexpr float PA_RESCALE_LOG2 = 8.f;
+// Tables with room for so few keys do without cut row tiles, and so without the second kernel (in a graph, both ways, us: one sequence of 256 keys, 32 heads of 128 8.8 / 10.5, 16
+// of 256, 32 / 8 heads 10.3 / 13.1, 16 of 512 13.9 / 16.0; one of 512 11.1 / 10.6, of 1024 18.9 / 13.6).
+constexpr int PA_WHOLE_TILES = 8;
 
 // A sequence as this launch deals with it.
 struct PagedUnits {
@@ -147,7 +150,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   if (threadIdx.x < 2) p.parts.joins[2 * blockIdx.x + threadIdx.x] = make_int4(-1, 0, 0, 0);
 
   long long share, w0, w1;
-  share_out<C::THREADS>(p.b.n, PA_MIN_SHARE, range, [&](int i) {
+  share_out<C::THREADS>(p.b.n, p.whole ? 1 : PA_MIN_SHARE, range, [&](int i) {
     const PagedUnits u = paged_units<ROWS>(p, i);
     if (u.s.bad && p.takes_bad && blockIdx.x == 0) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
     return u.cost;
@@ -180,7 +183,11 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       const int length = u.tiles + PA_PIECE_COST;
       const long long into = at - seq_begin;
       const long long unit = into < INT_MAX ? int(into) / length : into / length;  // (64-bit divisions are long)
-      const int from = int(into - unit * length), to = int(min((long long)length, from + (w1 - at)));
+      const int from = int(into - unit * length), to = p.whole ? length : int(min((long long)length, from + (w1 - at)));
+      if (p.whole && from) {  // (the CTA in whose range the row tile begins takes all of it)
+        at += length - from;
+        continue;
+      }
       const int t0 = max(0, from - PA_PIECE_COST), t1 = max(0, to - PA_PIECE_COST);
       at += to - from;
       if (t0 == t1) continue;  // (the range ends in front of the first tile)
@@ -599,6 +606,7 @@ static PagedPlan pa_plan(int n, int tokens, int table_width, int page_shift, int
   PagedPlan plan = {};
   const long long most_rows = (long long)min(most_new, tokens) * group, keys = (long long)table_width << page_shift;
   const bool wide = most_rows > 64, few = !wide || n > 1;
+  plan.joins = wide || keys > PA_WHOLE_TILES * PA_TILE;
   // rows of a tile of the first: all of a sequence's where there are no more than 64, else those of one token
   const long long usual = wide ? group : most_rows;
   plan.row_groups = usual <= 16 ? 1 : usual <= 32 ? 2 : 4;
@@ -606,15 +614,14 @@ static PagedPlan pa_plan(int n, int tokens, int table_width, int page_shift, int
   plan.few_high = !few ? 0 : wide ? rows : INT_MAX;
   if (few) {
     const long long tiles = min((long long)tokens * group / rows + n, (long long)n * ((min(most_rows, (long long)plan.few_high) + rows - 1) / rows)) * kv_heads;
-    const long long most = tiles * ((keys + PA_TILE - 1) / PA_TILE + PA_PIECE_COST);
-    plan.few_grid = int(max(1LL, min((long long)pa_sms() * (plan.row_groups > 1 ? 1 : head_dim == 64 ? Few<64, 1>::CTAS : Few<128, 1>::CTAS), (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE)));
+    const long long most = tiles * ((keys + PA_TILE - 1) / PA_TILE + PA_PIECE_COST), resident = pa_sms() * (plan.row_groups > 1 ? 1 : head_dim == 64 ? Few<64, 1>::CTAS : Few<128, 1>::CTAS);
+    plan.few_grid = int(max(1LL, min(resident, plan.joins ? (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE : tiles)));
     plan.few_floats = (long long)plan.few_grid * 2 * (rows * (head_dim + 2) + 4);
   }
   if (wide) {
     plan.wide_grid = pw_grid(head_dim);
     plan.wide_floats = (long long)plan.wide_grid * 2 * (PW_ROWS * (head_dim + 2) + 4);
   }
-  plan.joins = keys > PA_TILE;  // (a single tile of keys is never cut)
   return plan;
 }
 static PagedParts pa_parts(float*& room, int grid, int rows, int head_dim) {
@@ -662,6 +669,7 @@ extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
   p.q_st = a->q_st, p.q_sh = a->q_sh, p.o_st = a->o_st, p.o_sh = a->o_sh;
   p.heads = a->heads, p.kv_heads = a->kv_heads, p.group = group, p.window = a->window;
   p.scale_log2e = a->scale * 1.4426950408889634f;
+  p.whole = !plan.joins;
   float* room = static_cast<float*>(a->workspace);
   const PagedParts few = pa_parts(room, plan.few_grid, 16 * plan.row_groups, a->head_dim), wide = pa_parts(room, plan.wide_grid, PW_ROWS, a->head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream_);

@@ -24,6 +24,7 @@ struct PagedAttnParams {
   int rows_low, rows_high;  // sequences with rows (new tokens x group) in [rows_low, rows_high] are this launch's
   int takes_bad;            // and those whose lengths are not possible
   int fill_rest;            // rows outside all sequences become zeros
+  int whole;                // ranges end where row tiles do: nothing is cut, and nothing to join
   float scale_log2e;
   PagedParts parts;
 };
