@@ -300,6 +300,7 @@ using namespace tpb;
 
 extern "C" int tpb_adjust_logits(const tpb_adjust_logits_t* a, void* stream_) {
   if (!a || !a->logits || !a->out || !a->status || a->rows <= 0 || a->vocab <= 0 || a->width < 0 || a->dtype < 0 || a->dtype > 1) return TPB_ERR_ARG;
+  if (a->vocab > 1 << 30) return TPB_ERR_SIZE;
   LogitsParams p = {a->logits, a->out, a->tokens, a->lengths, a->prompts, a->repetition, a->frequency, a->presence, a->bias, reinterpret_cast<const uint32_t*>(a->allowed),
                     static_cast<uint32_t*>(a->status), a->logits_ld, a->out_ld, a->tokens_ld, a->bias_ld, a->allowed_ld, a->vocab, a->width, a->bias_dtype,
                     a->repetition_all, a->frequency_all, a->presence_all};

@@ -429,17 +429,21 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) sc[i][j] = ex2_approx(fmaf(sc[i][j], p.scale_log2e, base[j >> 1]));
+    // the sum is of the probabilities as the product takes them: where one key has nearly all of a row, its rounding cancels in the quotient (mean error of
+    // results of 256 keys 2.5e-3 -> 2.0e-3, 1.4e-3 of it their own rounding)
+    uint32_t pr[NT][2];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      l[0] += sc[i][0] + sc[i][1];
-      l[1] += sc[i][2] + sc[i][3];
-    }
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        pr[i][j] = pack_bf16x2(sc[i][2 * j], sc[i][2 * j + 1]);
+        l[j] += __uint_as_float(pr[i][j] << 16) + __uint_as_float(pr[i][j] & 0xFFFF0000u);
+      }
     // ---- values ----
     const bool cut = key0 < pc.low || key0 + C::KEYS > pc.total;
 #pragma unroll
     for (int ks = 0; ks < NT / 2; ++ks) {
-      uint32_t a[4] = {pack_bf16x2(sc[2 * ks][0], sc[2 * ks][1]), pack_bf16x2(sc[2 * ks][2], sc[2 * ks][3]),
-                       pack_bf16x2(sc[2 * ks + 1][0], sc[2 * ks + 1][1]), pack_bf16x2(sc[2 * ks + 1][2], sc[2 * ks + 1][3])};
+      const uint32_t a[4] = {pr[2 * ks][0], pr[2 * ks][1], pr[2 * ks + 1][0], pr[2 * ks + 1][1]};
       uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
       if (cut) {
 #pragma unroll
@@ -605,7 +609,7 @@ struct PagedPlan {
 static PagedPlan pa_plan(int n, int tokens, int table_width, int page_shift, int most_new, int kv_heads, int group, int head_dim) {
   PagedPlan plan = {};
   const long long most_rows = (long long)min(most_new, tokens) * group, keys = (long long)table_width << page_shift;
-  const bool wide = most_rows > 64, few = !wide || n > 1;
+  const bool wide = most_rows > 64, few = !wide || (n > 1 && group <= 64);
   plan.joins = wide || keys > PA_WHOLE_TILES * PA_TILE;
   // rows of a tile of the first: all of a sequence's where there are no more than 64, else those of one token
   const long long usual = wide ? group : most_rows;

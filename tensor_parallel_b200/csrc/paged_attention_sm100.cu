@@ -103,6 +103,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(lost + PW_LOST);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   __shared__ RangeSearch<PW_THREADS> range;
+  __shared__ int any_bad;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -126,16 +127,19 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     }
     for (int s = 0; s < PW_LOST; ++s) lost[s] = 0;
     *abort_flag = 0;
+    any_bad = 0;
     fence_mbar_init();
   }
+  __syncthreads();
   // beside the launch for few rows, which has waited for what is in front of it, before this one was let in: its end is awaited at this one's
   if (!ahead) pa_wait_prior();
-  pa_launch_next();
   if (threadIdx.x < 2) p.parts.joins[2 * blockIdx.x + threadIdx.x] = make_int4(-1, 0, 0, 0);
   if (warp == 1) {
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
+  __syncthreads();
+  pa_launch_next();  // (not before this CTA has its tensor memory: whoever comes next may want some while it waits)
   auto units_of = [&](int i, PagedSequence& s, int& rows) {  // row tiles of a sequence that is this launch's
     s = paged_sequence(p.b, i);
     rows = s.fresh * p.group;
@@ -146,7 +150,10 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     PagedSequence s;
     int rows, first, end, low;
     const int row_tiles = units_of(i, s, rows);
-    if (s.bad && p.takes_bad && blockIdx.x == 0) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+    if (s.bad && p.takes_bad) {
+      any_bad = 1;
+      if (blockIdx.x == 0) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+    }
     long long cost = 0;
     for (int rt = 0; rt < row_tiles; ++rt) {
       wide_span<N>(p, s, rows, rt, first, end, low);
@@ -154,7 +161,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     }
     return cost * p.kv_heads;
   }, share, w0, w1);
-  if (p.takes_bad)
+  if (any_bad)
     for (int i = 0; i < p.b.n; ++i) {
       const PagedSequence s = paged_sequence(p.b, i);
       if (s.bad) fill_rows<D, PW_THREADS>(p, s.token0, s.fresh, 0x7fc07fc0u);

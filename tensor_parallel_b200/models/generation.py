@@ -11,6 +11,7 @@ from typing import List, Optional
 
 import torch
 
+from tensor_parallel_b200.ops import functional as OF
 from tensor_parallel_b200.parallel.kv import PerDeviceTensors
 
 
@@ -37,20 +38,32 @@ def reorder_cache(past, beam_idx: torch.Tensor):
 @torch.no_grad()
 def generate(model, input_ids: Optional[torch.Tensor] = None, max_new_tokens: int = 20, num_beams: int = 1, do_sample: bool = False,
              top_p: float = 1.0, temperature: float = 1.0, eos_token_id: Optional[int] = None, output_scores: bool = False,
-             generator: Optional[torch.Generator] = None, inputs_embeds: Optional[torch.Tensor] = None, **model_kwargs):
+             generator: Optional[torch.Generator] = None, inputs_embeds: Optional[torch.Tensor] = None, repetition_penalty: Optional[float] = None,
+             frequency_penalty: Optional[float] = None, presence_penalty: Optional[float] = None, logit_bias: Optional[torch.Tensor] = None,
+             allowed_tokens=None, **model_kwargs):
     """Returns the generated ids ``[batch, prompt + new]`` (and the per-step score tensors when
     ``output_scores``: log-probabilities the next token was chosen from).  The prompt may be given as
     ``inputs_embeds [batch, prompt, hidden]`` instead of ids (the reference's ``test_generate_inputs_embeds`` case); the
-    result then holds the new tokens only."""
+    result then holds the new tokens only.
+
+    Greedy and sampled decoding adjust the logits in front of the pick (see :func:`~tensor_parallel_b200.ops.functional.adjust_logits`): ``repetition_penalty`` is for
+    the tokens of prompt and answer, ``frequency_penalty`` and ``presence_penalty`` for the answer's; ``logit_bias`` is ``[vocab]`` or ``[batch, vocab]``;
+    ``allowed_tokens``, the bits of the tokens that may come next (int32 ``[vocab / 32]`` or ``[batch, vocab / 32]``, rounded up), or a function that is given
+    the ids so far and returns them (a grammar), or None for all."""
     if (input_ids is None) == (inputs_embeds is None):
         raise ValueError("pass exactly one of input_ids / inputs_embeds")
+    adjusts = any(t is not None for t in (repetition_penalty, frequency_penalty, presence_penalty, logit_bias, allowed_tokens))
     if num_beams > 1:
+        if adjusts:
+            raise ValueError("penalties, biases and allowed tokens are for greedy and sampled decoding, not for beam search")
         return _beam_search(model, input_ids, max_new_tokens, num_beams, eos_token_id, output_scores, model_kwargs, inputs_embeds)
     prompt = input_ids if input_ids is not None else inputs_embeds
     ids = input_ids if input_ids is not None else torch.empty(prompt.shape[0], 0, dtype=torch.long, device=prompt.device)
     past, scores = None, []
     step_input = input_ids
     finished = torch.zeros(ids.shape[0], dtype=torch.bool, device=ids.device)
+    penalties = tuple(None if p is None else float(p) for p in (repetition_penalty, frequency_penalty, presence_penalty))
+    prompt_lengths = torch.full((ids.shape[0],), ids.shape[1], dtype=torch.int32, device=ids.device)
     for step in range(max_new_tokens):
         if step == 0 and inputs_embeds is not None:
             out = model(inputs_embeds=inputs_embeds, past_key_values=past, use_cache=True, **model_kwargs)
@@ -58,6 +71,11 @@ def generate(model, input_ids: Optional[torch.Tensor] = None, max_new_tokens: in
             out = model(input_ids=step_input, past_key_values=past, use_cache=True, **model_kwargs)
         past = out["past_key_values"]
         logits = out["logits"][:, -1].float().to(ids.device)
+        if adjusts:
+            allowed = allowed_tokens(ids) if callable(allowed_tokens) else allowed_tokens
+            history = (None, None) if all(p is None for p in penalties) else (ids, prompt_lengths)
+            logits = OF.adjust_logits(logits, history[0], None, history[1], *penalties, bias=None if logit_bias is None else logit_bias.to(logits.device),
+                                      allowed=None if allowed is None else allowed.to(logits.device))
         if do_sample:
             logits = logits / temperature
             if top_p < 1.0:

@@ -673,11 +673,12 @@ def paged_attention(q, cache: PagedCache, starts, past, scale: Optional[float] =
     ``q`` is ``[tokens, heads, head_dim]``; ``starts`` and ``past`` as for :func:`paged_append`, ``past`` not counting the new tokens: row ``starts[s] + i`` sees keys ``0`` to
     ``past[s] + i`` of sequence ``s``, or the last ``window`` of them.  One token of each sequence is a decode step, a whole prompt is a prefill, and
     sequences of both kinds may be in one batch.  ``most_new`` says how many new tokens any sequence has at most, where the caller knows (the launch is
-    chosen by it).  What lies in the cache outside of a token's keys has no influence, whatever it is; pages that have left the window are not read.
+    chosen by it).  What lies in the cache outside of a sequence's keys has no influence, whatever it is, and pages that have left every token's window are not
+    read; a sequence's own keys and values have to be finite (one that is not may reach any of its new tokens).
 
-    The result is a new tensor, zero in rows outside all sequences, or ``out`` (which may be ``q``), left as it is there.  A sequence whose rows, table or
-    pages do not fit, or with more than ``most_new`` new tokens, gives NaN, and the CUDA kernel records status 3 (see ``native.device_state``); the steps over tensors
-    raise.  Serving only: there is no gradient."""
+    The result is a new tensor, zero in rows outside all sequences, or ``out`` (which may be ``q``), left as it is there.  A sequence whose rows or table
+    do not fit, or with more than ``most_new`` new tokens, gives NaN, as rows do that reach a page outside the cache, and the CUDA kernel records status 3
+    (see ``native.device_state``); the steps over tensors raise.  Serving only: there is no gradient."""
     if _compiling():
         torch._dynamo.graph_break()
     done = paged_attention_directly(q, cache, starts, past, scale, window, most_new, out)

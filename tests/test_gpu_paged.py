@@ -454,3 +454,26 @@ def test_what_is_compiled_or_traced():
         torch.fx.experimental.proxy_tensor.make_fx(lambda q: OF.paged_attention(q, cache_of(b), b["starts"], b["past"]))(b["q"])
     with torch.utils.flop_counter.FlopCounterMode(display=False):
         within(attend(b), want, tol)
+    within(torch.compile(lambda q: OF.paged_attention(q * 1.0, cache_of(b), b["starts"], b["past"]) * 1.0, backend="eager")(b["q"]), want, tol)
+
+
+def test_negative_views_and_numbers_that_are_not_ordinary():
+    b = batch([1, 80], [30, 5], 4, 2, 64, 16, device="cuda", junk=0.0)
+    want, tol = attention64(b)
+    within(attend(dict(b, q=torch._neg_view(-b["q"]))), want, tol)
+    within(OF.paged_attention(b["q"], OF.PagedCache(torch._neg_view(-b["keys"]), torch._neg_view(-b["values"]), b["table"]), b["starts"], b["past"]), want, tol)
+    within(attend(b, scale=1 / 8, window=2 ** 40, most_new=2 ** 40), want, tol)
+    x, t = torch.randn(3, 100, device="cuda"), torch.randint(0, 100, (3, 9), device="cuda")
+    assert torch.equal(OF.adjust_logits(torch._neg_view(-x), t, None, None, 2), OF.adjust_logits(x, t, None, None, 2.0))
+
+
+def test_falcon_heads_and_bad_lengths_without_the_kernel_for_few_rows():
+    """71 query heads of one KV head are more rows than the kernel for few takes."""
+    b = batch([1, 1, 2, 1], [100, 40, 7, 300], 71, 1, 64, 16, device="cuda", front=1, rest=2)
+    want, tol = attention64(b)
+    within(attend(b, most_new=2), want, tol)
+    assert status_of() == 0
+    b["past"][1] = -5
+    out = attend(b, most_new=2)
+    assert status_of() == 3 and out[2].isnan().all()
+    within(out[[0, 1, 3, 4, 5, 6, 7]], want[[0, 1, 3, 4, 5, 6, 7]], tol[[0, 1, 3, 4, 5, 6, 7]])

@@ -209,3 +209,69 @@ def test_refused_logits():
             OF.adjust_logits(x, **bad)
     with pytest.raises(RuntimeError, match="gradient"):
         OF.adjust_logits(x.clone().requires_grad_())
+
+
+# -- in generate ---------------------------------------------------------------------------------
+
+
+def _tiny():
+    from tensor_parallel_b200.models.llama import LlamaConfig, LlamaForCausalLM
+
+    torch.manual_seed(0)
+    return LlamaForCausalLM(LlamaConfig(vocab_size=50, hidden_size=32, intermediate_size=48, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2)).eval()
+
+
+def test_generate_adjusts_its_logits():
+    model, prompt = _tiny(), torch.tensor([[3, 7, 9], [11, 3, 3]])
+    plain, scores = model.generate(prompt, max_new_tokens=6, output_scores=True)
+    same = model.generate(prompt, max_new_tokens=6, repetition_penalty=1.0, frequency_penalty=0.0, logit_bias=torch.zeros(50))
+    assert torch.equal(plain, same)
+    # a large presence penalty: no token of the answer comes twice; one of the prompt may
+    once = model.generate(prompt, max_new_tokens=12, presence_penalty=1e4)
+    assert all(len(set(row[3:].tolist())) == 12 for row in once)
+    # the repetition penalty is for the prompt too
+    with torch.no_grad():
+        first = model(input_ids=prompt)["logits"][:, -1].float()
+    want = OF.adjust_logits(first, prompt, None, None, 1.9).argmax(-1)
+    assert torch.equal(model.generate(prompt, max_new_tokens=1, repetition_penalty=1.9)[:, -1], want)
+    # a bias that decides, and bits that leave one token each
+    bias = torch.zeros(2, 50)
+    bias[0, 17] = bias[1, 23] = 1e4
+    assert model.generate(prompt, max_new_tokens=3, logit_bias=bias)[:, 3:].tolist() == [[17] * 3, [23] * 3]
+    steps = iter([5, 40, 33])
+
+    def grammar(ids):
+        bits = torch.zeros(2, dtype=torch.int64)
+        t = next(steps)
+        bits[t // 32] = 1 << (t % 32)
+        return torch.where(bits >= 2 ** 31, bits - 2 ** 32, bits).int()
+
+    assert model.generate(prompt, max_new_tokens=3, allowed_tokens=grammar)[:, 3:].tolist() == [[5, 40, 33]] * 2
+    sampled = model.generate(prompt, max_new_tokens=4, do_sample=True, allowed_tokens=torch.tensor([1 << 4, 1 << 1], dtype=torch.int32), generator=torch.Generator().manual_seed(0))
+    assert set(sampled[:, 3:].flatten().tolist()) <= {4, 33}
+    with pytest.raises(ValueError, match="beam"):
+        model.generate(prompt, max_new_tokens=2, num_beams=2, presence_penalty=1.0)
+
+
+def test_generate_of_a_wrapped_model_adjusts_too():
+    import tensor_parallel_b200 as tp
+
+    model, prompt = _tiny(), torch.tensor([[3, 7, 9]])
+    want = model.generate(prompt, max_new_tokens=5, presence_penalty=3.0, repetition_penalty=1.3)
+    wrapped = tp.tensor_parallel(model, ["cpu", "cpu"])
+    assert torch.equal(wrapped.generate(prompt, max_new_tokens=5, presence_penalty=3.0, repetition_penalty=1.3), want)
+
+
+def test_under_a_compiler():
+    b = batch([2, 1], [3, 0], 4, 2, 8, 4)
+    turn = OF.rotary(8)
+
+    def step(q, k, v):
+        q = OF.paged_append(cache_of(b), q * 1.0, k, v, b["starts"], b["past"], rotary=turn)
+        return OF.paged_attention(q, cache_of(b), b["starts"], b["past"]) + 1.0
+
+    want = step(b["q"], b["k"], b["v"])
+    assert torch.equal(torch.compile(step, backend="eager")(b["q"], b["k"], b["v"]), want)
+    x, t = torch.randn(2, 40), torch.randint(0, 40, (2, 6))
+    adjust = torch.compile(lambda x: OF.adjust_logits(x, t, presence=0.5), backend="eager", fullgraph=True)
+    assert torch.equal(adjust(x), OF.adjust_logits(x, t, presence=0.5))
