@@ -27,8 +27,11 @@ namespace tpb {
 
 constexpr int PW_M = 128;
 constexpr int PW_THREADS = 384;
-constexpr int PW_PIECE_COST = 1;  // in tiles: a piece's fill, drain and result
-constexpr int PW_MIN_SHARE = 5;   // a piece and four tiles
+// In tiles: a piece's fill, drain and result (whole calls at 1 / 2 / 3 / 5, in us: the prompts of 16.4 k tokens, 32 heads of 128 474 / 445 / 456 / 476, 16 x 1000, 32 / 8
+// heads 315 / 275 / 296 / 301, 8 x 2048, 32 heads of 64 319 / 317 / 303 / 305).
+template <int N>
+__device__ __forceinline__ constexpr int piece_cost() { return N == 64 ? 3 : 2; }
+constexpr int PW_MIN_SHARE = 6;   // a piece and four tiles
 constexpr float PW_RESCALE_LOG2 = 8.f;  // (see attention_sm100.cu: beyond the first 128 keys of a piece, the maximum follows large rises only)
 constexpr int PW_EXACT_KEYS = 128;
 constexpr int PW_PIECES = 4;  // announced at a time
@@ -157,7 +160,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     long long cost = 0;
     for (int rt = 0; rt < row_tiles; ++rt) {
       wide_span<N>(p, s, rows, rt, first, end, low);
-      cost += end - first + PW_PIECE_COST;
+      cost += end - first + piece_cost<N>();
     }
     return cost * p.kv_heads;
   }, share, w0, w1);
@@ -201,14 +204,14 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             continue;
           }
           wide_span<N>(p, s, rows, rt, first, end, low);
-          const int length = end - first + PW_PIECE_COST;
+          const int length = end - first + piece_cost<N>();
           if (at >= unit_begin + (long long)length * p.kv_heads) {
             unit_begin += (long long)length * p.kv_heads;
             ++rt;
             continue;
           }
           const int into = int(at - unit_begin), kvh = into / length, from = into % length, to = int(min((long long)length, from + (w1 - at)));
-          const int t0 = max(0, from - PW_PIECE_COST), t1 = max(0, to - PW_PIECE_COST);
+          const int t0 = max(0, from - piece_cost<N>()), t1 = max(0, to - piece_cost<N>());
           const long long unit_end = unit_begin + (long long)(kvh + 1) * length;
           at += to - from;
           if (t0 == t1) continue;
