@@ -77,7 +77,8 @@ __device__ __forceinline__ void share_out(int n, int least, RangeSearch<THREADS>
     mine_before = all + before;
     all += total;
   }
-  share = max((long long)least, (all + gridDim.x - 1) / gridDim.x);
+  // (64-bit divisions are long)
+  share = max((long long)least, all < INT_MAX / 2 ? (long long)((unsigned(all) + gridDim.x - 1) / gridDim.x) : (all + gridDim.x - 1) / gridDim.x);
   from = min(all, share * blockIdx.x);
   to = min(all, from + share);
   if (n <= THREADS) {
