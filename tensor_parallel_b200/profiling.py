@@ -15,7 +15,7 @@ import statistics
 
 import torch
 
-from tensor_parallel_b200.ops import native
+from tensor_parallel_b200.ops import functional as OF, native
 
 
 def _time(fn, iters: int):
@@ -189,6 +189,49 @@ def case_adamw(n, iters):
     return {"us": us, "tbps": n * (2 + 2 + 3 * 4 + 2 + 3 * 4) / us / 1e6}
 
 
+def _paged(new, past, heads, kv_heads, dim, page):
+    """Queries, keys and values of ``new`` tokens for each length in ``past``, and a paged cache that has room for them."""
+    pages = sum(-(-(p + new) // page) for p in past)
+    width = max(-(-(p + new) // page) for p in past)
+    table, at, order = torch.zeros(len(past), width, dtype=torch.int32), 0, torch.randperm(pages).int()
+    for s, p in enumerate(past):
+        need = -(-(p + new) // page)
+        table[s, :need], at = order[at:at + need], at + need
+    cache = OF.PagedCache(*(torch.randn(pages, kv_heads, page, dim, device="cuda", dtype=torch.bfloat16) for _ in range(2)), table.cuda())
+    starts = torch.arange(0, new * len(past) + 1, new, dtype=torch.int32, device="cuda")
+    qkv = torch.randn(new * len(past), heads + 2 * kv_heads, dim, device="cuda", dtype=torch.bfloat16)
+    return cache, qkv, starts, torch.tensor(past, dtype=torch.int32, device="cuda")
+
+
+def case_paged_attention(new, past, heads, kv_heads, dim, page, iters, ring=1):
+    sets = [_paged(new, past, heads, kv_heads, dim, page) for _ in range(ring)]
+
+    def call(i):
+        cache, qkv, starts, lengths = sets[i % ring]
+        OF.paged_attention(qkv[:, :heads], cache, starts, lengths, most_new=new)
+
+    res = _timed(call, iters)
+    us = res.get("graph_us", res["us"])
+    keys = sum(p + new for p in past)
+    pairs = sum(p + i + 1 for p in past for i in range(new))
+    return {**res, "tbps": 4.0 * dim * (keys * kv_heads + new * len(past) * heads) / us / 1e6, "tflops": 4.0 * dim * heads * pairs / us / 1e6}
+
+
+def case_paged_append(new, past, heads, kv_heads, dim, page, iters):
+    cache, qkv, starts, lengths = _paged(new, past, heads, kv_heads, dim, page)
+    q, k, v = qkv.split([heads, kv_heads, kv_heads], dim=1)
+    norm, turn = torch.ones(dim, device="cuda", dtype=torch.bfloat16), OF.rotary(dim, device="cuda")
+    res = _timed(lambda i: OF.paged_append(cache, q, k, v, starts, lengths, rotary=turn, q_norm=norm, k_norm=norm), iters)
+    return {**res, "tbps": 4.0 * qkv.numel() / res.get("graph_us", res["us"]) / 1e6}
+
+
+def case_adjust_logits(rows, vocab, width, iters):
+    sets = [(torch.randn(rows, vocab, device="cuda"), torch.randint(0, vocab, (rows, width), device="cuda"),
+             torch.randint(-2 ** 31, 2 ** 31, (rows, (vocab + 31) // 32), device="cuda").int()) for _ in range(5)]
+    res = _timed(lambda i: OF.adjust_logits(sets[i % 5][0], sets[i % 5][1], None, None, 1.2, 0.1, 0.1, None, sets[i % 5][2]), iters)
+    return {**res, "tbps": rows * vocab * 8.125 / res.get("graph_us", res["us"]) / 1e6}
+
+
 CASES = {
     "gemm_decode_qkv": lambda it: case_gemm(8, 12288, 4096, it),
     "gemm_decode_gate_up": lambda it: case_gemm(8, 22016, 4096, it),
@@ -210,6 +253,12 @@ CASES = {
     "int8_decode_gate_up": lambda it: case_int8_product(8, 22016, 4096, it, act="swiglu16"),
     "int8_short_down": lambda it: case_int8_product(100, 4096, 11008, it),
     "int8_prompt_up": lambda it: case_int8_product(2048, 11008, 4096, it),
+    "paged_append": lambda it: case_paged_append(2048, [0] * 8, 32, 8, 128, 64, it),
+    "paged_decode": lambda it: case_paged_attention(1, [2048] * 8, 32, 32, 128, 16, it, ring=2),
+    "paged_decode_grouped": lambda it: case_paged_attention(1, [2048] * 48, 128, 8, 64, 64, it, ring=2),
+    "paged_prompt": lambda it: case_paged_attention(2048, [0] * 4, 32, 32, 128, 64, it),
+    "paged_chunk": lambda it: case_paged_attention(512, [32000], 32, 8, 128, 16, it),
+    "adjust_logits": lambda it: case_adjust_logits(128, 65024, 1000, it),
     "swiglu": lambda it: case_swiglu(16384, 11008, it),
     "rope_append": lambda it: case_rope_append(8, 2048, 32, it),
     "adamw": lambda it: case_adamw(64 * 1024 * 1024, it),
