@@ -30,9 +30,10 @@ struct AppendParams {
   const bf16 *q, *k, *v, *q_norm, *k_norm;
   bf16 *q_out, *keys, *values;
   const float* frequencies;
-  long long q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, k_sp, k_shead, k_ss, v_sp, v_shead, v_ss;
+  long long k_sp, k_ss, v_sp, v_ss;
+  int q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, k_shead, v_shead;  // (pointers then are one 32 x 32 + 64 bit product away)
   int q_heads, kv_heads, head_dim, half, interleaved, fill_rest;  // q_heads 0: q is left alone
-  float factor, eps;
+  float factor, eps, inv_dim;
 };
 
 __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
@@ -98,10 +99,10 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
     }
   };
   auto source = [&](const Cursor& c) {
-    const long long t = t0 + c.t;
-    return c.r < p.q_heads                ? p.q + t * p.q_st + c.r * p.q_sh
-           : c.r < p.q_heads + p.kv_heads ? p.k + t * p.k_st + (c.r - p.q_heads) * p.k_sh
-                                          : p.v + t * p.v_st + (c.r - p.q_heads - p.kv_heads) * p.v_sh;
+    const bool is_q = c.r < p.q_heads, is_k = c.r < p.q_heads + p.kv_heads;
+    const bf16* base = is_q ? p.q : is_k ? p.k : p.v;
+    const int st = is_q ? p.q_st : is_k ? p.k_st : p.v_st, sh = is_q ? p.q_sh : is_k ? p.k_sh : p.v_sh, r = is_q ? c.r : is_k ? c.r - p.q_heads : c.r - p.q_heads - p.kv_heads;
+    return base + (long long)(t0 + c.t) * st + (long long)r * sh;
   };
   constexpr int AHEAD = 2;  // rows on their way (three, in three blocks per SM: 88 -> 90 us, 32 KV heads 151 -> 157)
   uint4 raw[AHEAD][2];
@@ -170,13 +171,12 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
     const bool there = c.t < tokens, is_q = c.r < p.q_heads, is_v = c.r >= p.q_heads + p.kv_heads;
     const AppendPlace place = places[there ? c.t : 0];
     bf16* dst = nullptr;
-    if (there) {
-      if (is_q)
-        dst = place.inside || p.fill_rest ? p.q_out + (long long)(t0 + c.t) * p.o_st + c.r * p.o_sh : nullptr;
-      else if (!is_v && place.k_at >= 0)
-        dst = p.keys + place.k_at + (c.r - p.q_heads) * p.k_shead;
-      else if (is_v && place.v_at >= 0)
-        dst = p.values + place.v_at + (c.r - p.q_heads - p.kv_heads) * p.v_shead;
+    if (is_q) {
+      if (there && (place.inside || p.fill_rest)) dst = p.q_out + (long long)(t0 + c.t) * p.o_st + (long long)c.r * p.o_sh;
+    } else {
+      const long long into = is_v ? place.v_at : place.k_at;
+      const int r = c.r - p.q_heads - (is_v ? p.kv_heads : 0);
+      if (there && into >= 0) dst = (is_v ? p.values : p.keys) + into + (long long)r * (is_v ? p.v_shead : p.k_shead);
     }
     uint4 y0 = u[0], y1 = u[1];
     if (__any_sync(0xffffffffu, there && !is_v)) {
@@ -196,7 +196,7 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
 #pragma unroll
         for (int d = LANES / 2; d > 0; d >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, d);
         if (normed) {
-          rstd = rsqrtf(s0 / p.head_dim + p.eps);
+          rstd = rsqrtf(s0 * p.inv_dim + p.eps);
 #pragma unroll
           for (int j = 0; j < 8; j += 2) {
             ffma2(x0[j], x0[j + 1], x0[j], x0[j + 1], rstd, rstd, 0.f, 0.f);
@@ -314,8 +314,12 @@ extern "C" int tpb_paged_append(const tpb_paged_append_t* a, void* stream_) {
   p.q_norm = static_cast<const bf16*>(a->q_norm), p.k_norm = static_cast<const bf16*>(a->k_norm);
   p.q_out = static_cast<bf16*>(a->q_out), p.keys = static_cast<bf16*>(a->keys), p.values = static_cast<bf16*>(a->values);
   p.frequencies = a->frequencies;
-  p.q_st = a->q_st, p.q_sh = a->q_sh, p.k_st = a->k_st, p.k_sh = a->k_sh, p.v_st = a->v_st, p.v_sh = a->v_sh, p.o_st = a->o_st, p.o_sh = a->o_sh;
-  p.k_sp = a->k_sp, p.k_shead = a->k_shead, p.k_ss = a->k_ss, p.v_sp = a->v_sp, p.v_shead = a->v_shead, p.v_ss = a->v_ss;
+  for (const long long t : {a->q_st, a->q_sh, a->k_st, a->k_sh, a->v_st, a->v_sh, a->o_st, a->o_sh, a->k_shead, a->v_shead})
+    if (t > INT_MAX || t < 0) return TPB_ERR_SIZE;
+  p.q_st = int(a->q_st), p.q_sh = int(a->q_sh), p.k_st = int(a->k_st), p.k_sh = int(a->k_sh), p.v_st = int(a->v_st), p.v_sh = int(a->v_sh);
+  p.o_st = int(a->o_st), p.o_sh = int(a->o_sh), p.k_shead = int(a->k_shead), p.v_shead = int(a->v_shead);
+  p.k_sp = a->k_sp, p.k_ss = a->k_ss, p.v_sp = a->v_sp, p.v_ss = a->v_ss;
+  p.inv_dim = 1.f / float(a->head_dim);
   p.q_heads = a->q ? a->heads : 0;
   p.kv_heads = a->kv_heads, p.head_dim = a->head_dim, p.half = a->rotary_dim / 2, p.interleaved = a->interleaved, p.fill_rest = a->fill_rest;
   p.factor = a->factor, p.eps = a->eps;

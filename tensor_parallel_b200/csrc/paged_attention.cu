@@ -539,37 +539,54 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 }
 
 // Joins the pieces of the row tile whose keys begin in a CTA's range and end in another's: blocks for each CTA, of which most have nothing to do, and a
-// thread for every four columns of a row.  `wide`: of a second launch, with larger tiles, behind those of the first.
+// thread for every four columns of a row or of several.  Behind those of the launch for few rows come those of the one for many.
 constexpr int PA_JOIN_THREADS = 128;
 
 template <int D>
 __global__ void __launch_bounds__(PA_JOIN_THREADS)
-paged_attn_join_kernel(const PagedAttnParams p, const PagedParts few, int few_grid, const PagedParts wide) {
-  const bool is_wide = int(blockIdx.x) >= few_grid;
+paged_attn_join_kernel(const PagedAttnParams p, const PagedParts few, const int few_blocks, const int blocks_of_few, const PagedParts wide, const int blocks_of_wide) {
+  const bool is_wide = int(blockIdx.x) >= few_blocks;
   const PagedParts parts = is_wide ? wide : few;
-  const int c = blockIdx.x - (is_wide ? few_grid : 0);
+  const int at = blockIdx.x - (is_wide ? few_blocks : 0), blocks = is_wide ? blocks_of_wide : blocks_of_few, c = at / blocks;
   pa_wait_prior();
   pa_launch_next();
   const int4 unit = parts.joins[2 * c];
   const int last = parts.joins[2 * c + 1].x;
   if (unit.x < 0) return;
-  for (int item = blockIdx.y * PA_JOIN_THREADS + threadIdx.x; item < unit.z * (D / 4); item += gridDim.y * PA_JOIN_THREADS) {
+  auto slot = [&](int i) { return (long long)(i == c ? 2 * c + 1 : 2 * i) * parts.rows; };
+  for (int item = at % blocks * PA_JOIN_THREADS + threadIdx.x; item < unit.z * (D / 4); item += blocks * PA_JOIN_THREADS) {
     const int r = item / (D / 4), col = item % (D / 4) * 4;
     const float2* ml = parts.ml + r;
     const float* part = parts.o + (long long)r * D + col;
-    auto slot = [&](int i) { return (long long)(i == c ? 2 * c + 1 : 2 * i) * parts.rows; };
     float top = -INFINITY, sum = 0.f;
-#pragma unroll 4
-    for (int i = c; i <= last; ++i) top = fmaxf(top, ml[slot(i)].x);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = c; i <= last; ++i) {
-      const float2 s = ml[slot(i)];
-      if (s.x == -INFINITY) continue;  // (no key of the piece is the row's)
-      const float4 w = *reinterpret_cast<const float4*>(part + slot(i) * D);
-      const float f = ex2_approx(s.x - top);
-      sum += s.y * f;
-      v.x += w.x * f, v.y += w.y * f, v.z += w.z * f, v.w += w.w * f;
+    // (several pieces at a time, all their loads in front of the first use; the sums so far are brought to a new maximum)
+    constexpr int AT_ONCE = 4;
+    for (int i0 = c; i0 <= last; i0 += AT_ONCE) {
+      float2 s[AT_ONCE];
+      float4 w[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        s[j] = make_float2(-INFINITY, 0.f);
+        if (i0 + j <= last) {
+          s[j] = ml[slot(i0 + j)];
+          w[j] = *reinterpret_cast<const float4*>(part + slot(i0 + j) * D);
+        }
+      }
+      float next = top;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) next = fmaxf(next, s[j].x);
+      const float down = top == -INFINITY ? 0.f : ex2_approx(top - next);
+      sum *= down;
+      v.x *= down, v.y *= down, v.z *= down, v.w *= down;
+      top = next;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        if (s[j].x == -INFINITY) continue;  // (no key of the piece is the row's)
+        const float f = ex2_approx(s[j].x - top);
+        sum += s[j].y * f;
+        v.x += w[j].x * f, v.y += w[j].y * f, v.z += w[j].z * f, v.w += w[j].w * f;
+      }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int t = (unit.y + r) / p.group, h = (unit.y + r) % p.group;
@@ -707,10 +724,12 @@ extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
     if (rc != TPB_OK) return rc;
   }
   if (!plan.joins) return TPB_OK;
-  const int rows = plan.wide_grid ? PW_ROWS : int(min((long long)few.rows, max(1LL, (long long)min(a->most_new, a->tokens) * group)));
-  const dim3 grid(plan.few_grid + plan.wide_grid, min(16, (rows * (a->head_dim / 4) + PA_JOIN_THREADS - 1) / PA_JOIN_THREADS));
-  const cudaError_t launched =
-      a->head_dim == 64 ? launch_dependent(paged_attn_join_kernel<64>, grid, dim3(PA_JOIN_THREADS), 0, s, true, p, few, plan.few_grid, wide)
-                        : launch_dependent(paged_attn_join_kernel<128>, grid, dim3(PA_JOIN_THREADS), 0, s, true, p, few, plan.few_grid, wide);
+  // a thread for each four columns of the first launch's tiles, for each eight of the second's
+  auto blocks = [&](int rows, int of_thread) { return (rows * (a->head_dim / 4) + of_thread * PA_JOIN_THREADS - 1) / (of_thread * PA_JOIN_THREADS); };
+  const int of_few = blocks(int(min((long long)few.rows, max(1LL, (long long)min(a->most_new, a->tokens) * group))), 1), of_wide = blocks(PW_ROWS, 2);
+  const int few_blocks = plan.few_grid * of_few;
+  const dim3 grid(few_blocks + plan.wide_grid * of_wide);
+  auto join = a->head_dim == 64 ? paged_attn_join_kernel<64> : paged_attn_join_kernel<128>;
+  const cudaError_t launched = launch_dependent(join, grid, dim3(PA_JOIN_THREADS), 0, s, true, p, few, few_blocks, of_few, wide, of_wide);
   return launched == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
