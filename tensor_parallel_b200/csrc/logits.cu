@@ -56,6 +56,7 @@ __device__ __forceinline__ void lg_launch_next() { asm volatile("griddepcontrol.
 
 constexpr int LG_DEPTH = 4;           // vectors of 16 bytes of fp32 of a thread on their way, half as many of bf16
 constexpr int LG_ENTRIES = 24576;     // of a part of the vocabulary at most: 96 KB of counts, two blocks per SM
+constexpr int LG_SEEN_THREADS = 512;  // of a block behind the first kernel: 4096 tokens at once
 constexpr int LG_ALONE = 4096;        // entries of a part where one kernel does both
 constexpr int LG_HELD = 8;            // tokens of a thread at a time; the first of them wait for the first kernel with their results
 
@@ -151,8 +152,9 @@ adjust_stream_kernel(const LogitsParams p, int part) {
 
 // FORM 0: behind the first kernel.  1 and 2: alone, with the stream of its own part in front (in vectors, one by one).
 template <typename T, int FORM>
-__global__ void __launch_bounds__(LG_THREADS, 4)
+__global__ void __launch_bounds__(FORM ? LG_THREADS : LG_SEEN_THREADS, FORM ? 4 : 2)
 adjust_seen_kernel(const LogitsParams p, int part) {
+  constexpr int THREADS = FORM ? LG_THREADS : LG_SEEN_THREADS;
   extern __shared__ __align__(16) uint32_t counts[];
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.logits) + row * p.logits_ld;
@@ -160,7 +162,7 @@ adjust_seen_kernel(const LogitsParams p, int part) {
   // (alone, parts lie on the row's grid of vectors)
   const long long begin = (long long)blockIdx.y * part - (FORM == 1 ? int((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % Vec<T>::N) : 0);
   const long long end = min((long long)p.vocab, begin + part);
-  for (int i = threadIdx.x * 4; i < part; i += LG_THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x * 4; i < part; i += THREADS * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
   if (FORM) {
     lg_wait_prior();
     lg_launch_next();
@@ -191,7 +193,7 @@ adjust_seen_kernel(const LogitsParams p, int part) {
   float value[LG_HELD];
   auto entries = [&](int from) {
 #pragma unroll
-    for (int j = 0; j < LG_HELD; ++j) at[j] = from + j * LG_THREADS < length ? entry(from + j * LG_THREADS) : -1;
+    for (int j = 0; j < LG_HELD; ++j) at[j] = from + j * THREADS < length ? entry(from + j * THREADS) : -1;
   };
   // the logits of entries that nobody has taken yet; the others' places become -1.  (All loads of one kind behind one another, not a token's.)
   auto take = [&]() {
@@ -231,9 +233,9 @@ adjust_seen_kernel(const LogitsParams p, int part) {
   if (FORM) stream_part<T, FORM == 1>(p, row, int(begin), int(end));
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < LG_HELD; ++j) count(at[j], threadIdx.x + j * LG_THREADS);
+  for (int j = 0; j < LG_HELD; ++j) count(at[j], threadIdx.x + j * THREADS);
 #pragma unroll 4
-  for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_THREADS) count(entry(i), i);
+  for (int i = threadIdx.x + LG_HELD * THREADS; i < length; i += THREADS) count(entry(i), i);
   __syncthreads();
   take();
   if (!FORM) {
@@ -241,7 +243,7 @@ adjust_seen_kernel(const LogitsParams p, int part) {
     lg_launch_next();
   }
   store();
-  for (int i = threadIdx.x + LG_HELD * LG_THREADS; i < length; i += LG_HELD * LG_THREADS) {
+  for (int i = threadIdx.x + LG_HELD * THREADS; i < length; i += LG_HELD * THREADS) {
     entries(i);
     take();
     store();
@@ -268,7 +270,7 @@ static int lg_seen(const LogitsParams& p, int rows, int part, int parts, cudaStr
     ready[dev].store(true, std::memory_order_release);
   }
   if (parts > 65535) return TPB_ERR_SIZE;
-  return launch_dependent(adjust_seen_kernel<T, FORM>, dim3(rows, unsigned(parts)), dim3(LG_THREADS), size_t(part) * 4, stream, true, p, part) == cudaSuccess ? TPB_OK
+  return launch_dependent(adjust_seen_kernel<T, FORM>, dim3(rows, unsigned(parts)), dim3(FORM ? LG_THREADS : LG_SEEN_THREADS), size_t(part) * 4, stream, true, p, part) == cudaSuccess ? TPB_OK
                                                                                                                                                                : TPB_ERR_CUDA;
 }
 
