@@ -595,14 +595,6 @@ paged_attn_join_kernel(const PagedAttnParams p, const PagedParts few, const int 
   }
 }
 
-static int pa_sms() {
-  static int sms[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 148;
-  if (!sms[dev]) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
-  return sms[dev];
-}
-
 template <int D, int R>
 static int pa_few_launch(const PagedAttnParams& p, const CUtensorMap& k, const CUtensorMap& v, int grid, cudaStream_t stream) {
   using C = Few<D, R>;

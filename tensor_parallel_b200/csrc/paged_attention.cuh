@@ -1,8 +1,22 @@
 // Shared by the two kernels that attend to a paged cache (paged_attention.cu, paged_attention_sm100.cu).
 #pragma once
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace tpb {
+
+inline int pa_sms() {
+  static std::atomic<int> sms[64];
+  int dev = 0, count = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return count;
+  count = sms[dev].load(std::memory_order_relaxed);
+  if (!count) {
+    if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || count <= 0) return 148;
+    sms[dev].store(count, std::memory_order_relaxed);
+  }
+  return count;
+}
 
 typedef __nv_bfloat16 bf16;
 

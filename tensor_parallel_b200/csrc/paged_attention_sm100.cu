@@ -615,11 +615,7 @@ static int pw_go(const PagedAttnParams& p, const CUtensorMap& k, const CUtensorM
 
 int pw_tile(int head_dim) { return head_dim; }
 
-int pw_grid(int head_dim) {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
-  return sms * (head_dim == 64 ? 2 : 1);
-}
+int pw_grid(int head_dim) { return pa_sms() * (head_dim == 64 ? 2 : 1); }
 
 int pw_launch(int head_dim, const PagedAttnParams& p, const CUtensorMap& k, const CUtensorMap& v, int grid, bool ahead, cudaStream_t stream) {
   return head_dim == 64 ? pw_go<64, 64>(p, k, v, grid, ahead, stream) : pw_go<128, 128>(p, k, v, grid, ahead, stream);

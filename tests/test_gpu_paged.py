@@ -220,6 +220,42 @@ def test_attention_of_lengths_that_do_not_fit(what, most_new):
             within(out[r], want[r], tol[r])
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,past,row0", [([200], [700], 0), ([1, 300, 1], [90, 100, 400], 1), ([1, 600], [3000, 2000], 1)])
+def test_attention_of_chunks_whose_pages_are_not_there(new, past, row0, dim):
+    b = batch(new, past, 4, 2, dim, 16, device="cuda")
+    want, tol = attention64(b)
+    chunk = max(range(len(new)), key=lambda s: new[s])
+    bad = dict(b, table=b["table"].clone())
+    bad["table"][chunk, 5] = 10 ** 9
+    out = attend(bad)
+    assert status_of() == 3 and out[row0:row0 + new[chunk]].isnan().all()
+    others = [r for r in range(sum(new)) if not row0 <= r < row0 + new[chunk]]
+    within(out[others], want[others], tol[others])
+    bad = dict(b, past=b["past"].clone())
+    bad["past"][chunk] = 2 ** 30
+    out = attend(bad)
+    assert status_of() == 3 and out[row0:row0 + new[chunk]].isnan().all()
+    within(out[others], want[others], tol[others])
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (14, 2), (71, 1), (8, 8)])
+def test_chunks_by_boxes_and_by_rows(heads, kv_heads):
+    """Query rows of whole tokens come by boxes, those of 7 or 71 heads and broadcast ones by rows."""
+    b = batch([130, 257, 1, 40], [300, 0, 60, 1000], heads, kv_heads, 128, 32, device="cuda", rest=5)
+    want, tol = attention64(b)
+    within(attend(b), want, tol)
+    one = b["q"][:, :1].expand(-1, heads, -1)
+    want, tol = attention64(dict(b, q=one.contiguous()))
+    within(OF.paged_attention(one, cache_of(b), b["starts"], b["past"]), want, tol)
+    q = b["q"].clone()
+    want, tol = attention64(b)
+    assert attend(dict(b, q=q), out=q) is q
+    used = int(b["starts"][-1])
+    within(q[:used], want[:used], tol[:used])
+    assert torch.equal(q[used:], b["q"][used:])
+
+
 def test_attention_of_more_new_tokens_than_said():
     b = batch([1, 5, 2], [100, 40, 7], 4, 2, 64, 16, device="cuda")
     want, tol = attention64(b)
