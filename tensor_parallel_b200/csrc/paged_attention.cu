@@ -90,19 +90,23 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// R groups of 16 rows.  Four warps and several CTAs per SM, which fill each other's gaps, where their registers fit; 64 rows of 128 elements take eight warps and the
+// SM (32 x 2049 keys, us, with 4 warps in 2 CTAs / 8 warps in one: 32 rows, 8 heads of 64 35.0 / 47.7, of 128 60.3 / 64.0; 64 rows, of 64 50.9 / 63.6, of 128 in one
+// CTA each 95.3 / 90.4; 16 rows of 64 in 2 / 3 / 4 CTAs, 48 ragged sequences 72.5 / 61.2 / 60.6).
 template <int D, int R>
 struct Few {
   static constexpr int ROWS = 16 * R;
-  static constexpr int WARPS = R == 1 ? 4 : 8;
+  static constexpr int WARPS = R == 4 && D == 128 ? 8 : 4;
   static constexpr int KEY_GROUPS = WARPS / R;
   static constexpr int KEYS = PA_TILE / KEY_GROUPS;  // of a warp
-  static constexpr int CTAS = R > 1 ? 1 : D == 64 ? 3 : 2;  // per SM
+  static constexpr int CTAS = WARPS == 8 ? 1 : R == 1 && D == 64 ? 3 : 2;  // per SM
   static constexpr int DB = D / 64;
   static constexpr int STAGE_BYTES = 2 * DB * PA_BLOCK;
-  static constexpr int STAGES = (R > 1 ? 160 : D == 64 ? 64 : 96) * 1024 / STAGE_BYTES;
+  static constexpr int STAGES = (WARPS == 8 ? 160 : R == 1 && D == 128 ? 96 : 64) * 1024 / STAGE_BYTES;
   static constexpr int Q_BYTES = ROWS * D * 2;
   static constexpr int MERGE_COLS = STAGE_BYTES / (WARPS * 16 * 4) < D ? STAGE_BYTES / (WARPS * 16 * 4) : D;  // that the partial results of all warps fill a stage with
   static constexpr int THREADS = WARPS * 32 + 32;
+  static_assert(PA_TILE % (16 * KEY_GROUPS) == 0 && MERGE_COLS >= 32, "a warp has whole groups of 16 keys");
   static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 2 * Q_BYTES + WARPS * 16 * 8 + STAGES * 8 + 2 * int(sizeof(PagedPiece)) +
                               (2 * STAGES + 6) * 8 + 256;
 };
@@ -608,6 +612,11 @@ static int pa_few_launch(const PagedAttnParams& p, const CUtensorMap& k, const C
   return launch_dependent(paged_attn_few_kernel<D, R>, dim3(grid), dim3(C::THREADS), C::SMEM, stream, true, k, v, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
+static int pa_few_ctas(int head_dim, int row_groups) {
+  if (head_dim == 64) return row_groups == 1 ? Few<64, 1>::CTAS : row_groups == 2 ? Few<64, 2>::CTAS : Few<64, 4>::CTAS;
+  return row_groups == 1 ? Few<128, 1>::CTAS : row_groups == 2 ? Few<128, 2>::CTAS : Few<128, 4>::CTAS;
+}
+
 // What a call launches.  Sequences with few query rows (new tokens x query heads of a KV head) go by the kernel above, bound by memory; those with more by the one
 // on the tensor cores of paged_attention_sm100.cu.  The host knows the rows of a sequence at most; where both kinds may be in the batch, both are launched.
 struct PagedPlan {
@@ -627,7 +636,7 @@ static PagedPlan pa_plan(int n, int tokens, int table_width, int page_shift, int
   plan.few_high = !few ? 0 : wide ? rows : INT_MAX;
   if (few) {
     const long long tiles = min((long long)tokens * group / rows + n, (long long)n * ((min(most_rows, (long long)plan.few_high) + rows - 1) / rows)) * kv_heads;
-    const long long most = tiles * ((keys + PA_TILE - 1) / PA_TILE + PA_PIECE_COST), resident = pa_sms() * (plan.row_groups > 1 ? 1 : head_dim == 64 ? Few<64, 1>::CTAS : Few<128, 1>::CTAS);
+    const long long most = tiles * ((keys + PA_TILE - 1) / PA_TILE + PA_PIECE_COST), resident = (long long)pa_sms() * pa_few_ctas(head_dim, plan.row_groups);
     plan.few_grid = int(max(1LL, min(resident, plan.joins ? (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE : tiles)));
     plan.few_floats = (long long)plan.few_grid * 2 * (rows * (head_dim + 2) + 4);
   }
