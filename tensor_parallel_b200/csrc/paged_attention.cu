@@ -4,10 +4,11 @@
 //
 // What bounds it is reading the pages once: 4 * head_dim bytes per key and KV head, and two products of 16 rows with each.  One launch deals with every
 // sequence of the batch, whatever their lengths: the work (sequence, row tile, KV head, tile of 64 keys) lies on one line, cut into as many equal
-// ranges as there are CTAs.  A range may begin and end inside a row tile's keys; such pieces leave unnormalised sums with their maximum in a workspace, and a
+// ranges as there are teams of warps (one to three in a CTA, a CTA per SM).  A range may begin and end inside a row tile's keys; such pieces leave unnormalised sums with their maximum in a workspace, and a
 // second kernel, launched ahead, joins them in the order of the keys (no counters, no atomics: the result does not depend on timing, and calls on
 // other streams or captured graphs share nothing).
 //
+// A team:
 //   producer warp : walks the range; TMA boxes of up to 64 slots per page into a ring of stages (keys and values of 64 keys), up to 32 table entries
 //                   fetched at a time and 32 ahead; query rows by cp.async into one of two buffers, so that the next piece's are there when its first keys are
 //   compute warps : a warp holds 16 query rows and a part of the stage's keys (ROW_GROUPS x key groups): mma.sync m16n8k16 (what there is to multiply
@@ -30,7 +31,7 @@ namespace tpb {
 
 constexpr int PA_TILE = 64;                 // keys of a stage
 constexpr int PA_BLOCK = PA_TILE * 128;     // bytes of a swizzled block of 64 keys x 64 elements
-constexpr int PA_MIN_SHARE = 3;             // of a CTA's range, at least: a piece and two tiles
+constexpr int PA_MIN_SHARE = 3;             // of a team's range, at least: a piece and two tiles
 // What a row tile costs beside its key tiles, in tiles: its query rows, the meeting of the key groups, its result.  It stands in front of them on the line.
 constexpr int PA_PIECE_COST = 1;
 constexpr float PA_RESCALE_LOG2 = 8.f;
@@ -90,16 +91,17 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// R groups of 16 rows.  Four warps and several CTAs per SM, which fill each other's gaps, where their registers fit; 64 rows of 128 elements take eight warps and the
-// SM (32 x 2049 keys, us, with 4 warps in 2 CTAs / 8 warps in one: 32 rows, 8 heads of 64 35.0 / 47.7, of 128 60.3 / 64.0; 64 rows, of 64 50.9 / 63.6, of 128 in one
-// CTA each 95.3 / 90.4; 16 rows of 64 in 2 / 3 / 4 CTAs, 48 ragged sequences 72.5 / 61.2 / 60.6).
+// R groups of 16 rows.  Teams of four warps, several per SM, fill each other's gaps where their registers fit; 64 rows of 128 elements take eight warps and the
+// SM (32 x 2049 keys, us, with 2 teams of 4 warps / one of 8: 32 rows, 8 heads of 64 35.0 / 47.7, of 128 60.3 / 64.0; 64 rows, of 64 50.9 / 63.6, of 128 one
+// team each 95.3 / 90.4; 16 rows of 64 by 2 / 3 / 4 teams, 48 ragged sequences 72.5 / 61.2 / 60.6).  Teams know nothing of each other; that they are one CTA and not
+// several costs nothing (within 2 % of those) and leaves the other launch whole SMs.
 template <int D, int R>
 struct Few {
   static constexpr int ROWS = 16 * R;
   static constexpr int WARPS = R == 4 && D == 128 ? 8 : 4;
   static constexpr int KEY_GROUPS = WARPS / R;
   static constexpr int KEYS = PA_TILE / KEY_GROUPS;  // of a warp
-  static constexpr int CTAS = WARPS == 8 ? 1 : R == 1 && D == 64 ? 3 : 2;  // per SM
+  static constexpr int TEAMS = WARPS == 8 ? 1 : R == 1 && D == 64 ? 3 : 2;  // of a CTA, each with a range of its own
   static constexpr int DB = D / 64;
   static constexpr int STAGE_BYTES = 2 * DB * PA_BLOCK;
   static constexpr int STAGES = (WARPS == 8 ? 160 : R == 1 && D == 128 ? 96 : 64) * 1024 / STAGE_BYTES;
@@ -107,18 +109,22 @@ struct Few {
   static constexpr int MERGE_COLS = STAGE_BYTES / (WARPS * 16 * 4) < D ? STAGE_BYTES / (WARPS * 16 * 4) : D;  // that the partial results of all warps fill a stage with
   static constexpr int THREADS = WARPS * 32 + 32;
   static_assert(PA_TILE % (16 * KEY_GROUPS) == 0 && MERGE_COLS >= 32, "a warp has whole groups of 16 keys");
-  static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 2 * Q_BYTES + WARPS * 16 * 8 + STAGES * 8 + 2 * int(sizeof(PagedPiece)) +
-                              (2 * STAGES + 6) * 8 + 256;
+  static constexpr int TEAM_SMEM = (STAGES * STAGE_BYTES + 2 * Q_BYTES + WARPS * 16 * 8 + STAGES * 8 + 2 * int(sizeof(PagedPiece)) + (2 * STAGES + 6) * 8 + 1279) / 1024 * 1024;
+  static constexpr int SMEM = 1024 + TEAMS * TEAM_SMEM;
+  static_assert(SMEM + 1024 <= 228 * 1024, "shared memory of an SM");
 };
 
 template <int D, int R>
-__global__ void __launch_bounds__(Few<D, R>::THREADS, Few<D, R>::CTAS)
+__global__ void __launch_bounds__(Few<D, R>::THREADS* Few<D, R>::TEAMS, 1)
 paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const PagedAttnParams p) {
   using C = Few<D, R>;
   constexpr int DB = C::DB, STAGES = C::STAGES, WARPS = C::WARPS, ROWS = C::ROWS;
 
   extern __shared__ uint8_t pa_smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023));
+  const int team = __shfl_sync(0xffffffffu, threadIdx.x / C::THREADS, 0), thread = threadIdx.x - team * C::THREADS;
+  // ranges that lie side by side on an SM when another launch has the SMs behind, else on all SMs first
+  const int range_no = p.split_sms ? int(blockIdx.x) * C::TEAMS + team : int(blockIdx.x) + team * int(gridDim.x);
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023)) + team * C::TEAM_SMEM;
   uint8_t* ring = smem;                                    // [STAGES][keys | values][DB][64 keys][128 bytes]
   uint8_t* q_s = ring + STAGES * C::STAGE_BYTES;           // [2][DB][ROWS][128 bytes], swizzled like the ring
   float2* stats = reinterpret_cast<float2*>(q_s + 2 * C::Q_BYTES);       // [WARPS][16 rows]
@@ -131,10 +137,11 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   uint64_t* q_empty = bars + 2 * STAGES + 2;  // [2]
   uint64_t* meet = bars + 2 * STAGES + 4;     // the compute warps, phase by phase
   volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
-  __shared__ RangeSearch<C::THREADS> range;
+  __shared__ RangeSearch<C::THREADS> ranges[C::TEAMS];
+  RangeSearch<C::THREADS>& range = ranges[team];
 
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
+  const int warp = __shfl_sync(0xffffffffu, thread >> 5, 0), lane = threadIdx.x & 31;
+  if (thread == 0) {
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
     for (int s = 0; s < STAGES; ++s) {
@@ -151,15 +158,22 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   }
   pa_wait_prior();  // (launched ahead of the previous kernel's end: nothing is read or written before that)
   pa_launch_next();
-  if (threadIdx.x < 2) p.parts.joins[2 * blockIdx.x + threadIdx.x] = make_int4(-1, 0, 0, 0);
+  if (thread < 2) p.parts.joins[2 * range_no + thread] = make_int4(-1, 0, 0, 0);
 
   long long share, w0, w1;
-  share_out<C::THREADS>(p.b.n, p.whole ? 1 : PA_MIN_SHARE, range, [&](int i) {
+  float few = 0.f, wide = 0.f;
+  auto meet_team = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(C::THREADS) : "memory"); };
+  share_out<C::THREADS>(p.b.n, p.whole ? 1 : PA_MIN_SHARE, thread, range_no, range, [&](int i) {
     const PagedUnits u = paged_units<ROWS>(p, i);
-    if (u.s.bad && p.takes_bad && blockIdx.x == 0) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+    if (u.s.bad && p.takes_bad && range_no == 0) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+    if (p.split_sms) pa_load(p, u.s, D, few, wide);
     return u.cost;
-  }, share, w0, w1);
-  if (p.fill_rest) fill_around<D, C::THREADS>(p);
+  }, [&]() {
+    if (!p.split_sms) return unsigned(p.ranges);
+    sum_loads<C::THREADS>(range, thread, meet_team, few, wide);
+    return unsigned(max(1, pa_few_sms(few, wide, p.split_sms)) * C::TEAMS);
+  }, meet_team, share, w0, w1);
+  if (p.fill_rest) fill_around<D, C::THREADS * C::TEAMS>(p);
 
   auto give_up = [&]() {
     atomicMax(p.b.status, uint32_t(STATUS_TIMEOUT_MBAR));
@@ -188,7 +202,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       const long long into = at - seq_begin;
       const long long unit = into < INT_MAX ? int(into) / length : into / length;  // (64-bit divisions are long)
       const int from = int(into - unit * length), to = p.whole ? length : int(min((long long)length, from + (w1 - at)));
-      if (p.whole && from) {  // (the CTA in whose range the row tile begins takes all of it)
+      if (p.whole && from) {  // (whoever has the beginning of the row tile in its range takes all of it)
         at += length - from;
         continue;
       }
@@ -218,8 +232,8 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         o.low = low;
         o.kvh = kvh;
         o.bad = u.s.bad;
-        // keys that begin in this range and end in another's are joined by the block of this CTA; its other piece continues the range in front
-        o.slot = t0 == 0 && t1 == u.tiles ? -1 : 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+        // keys that begin in this range and end in another's are joined by the blocks of this range; its other piece continues the range in front
+        o.slot = t0 == 0 && t1 == u.tiles ? -1 : 2 * range_no + (t0 == 0 ? 1 : 0);
       }
       {
         constexpr int STEP = 32 / (D / 8);  // rows at a time
@@ -274,8 +288,8 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       ++piece;
       if (t0 == 0 && t1 < u.tiles && lane == 0) {
         const long long unit_end = seq_begin + (unit + 1) * length;
-        p.parts.joins[2 * blockIdx.x] = make_int4(u.s.token0, row0, min(ROWS, u.rows - row0), kvh);
-        p.parts.joins[2 * blockIdx.x + 1] = make_int4(int((unit_end - 1) / share), 0, 0, 0);
+        p.parts.joins[2 * range_no] = make_int4(u.s.token0, row0, min(ROWS, u.rows - row0), kvh);
+        p.parts.joins[2 * range_no + 1] = make_int4(int((unit_end - 1) / share), 0, 0, 0);
       }
     }
     if (ok) {
@@ -512,7 +526,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           *reinterpret_cast<float2*>(merge + (warp * 16 + g8 + 8 * i) * COLS + ((d ^ (g8 & (COLS / 8 - 1))) * 8) + t4 * 2) =
               make_float2(o[c0 / 8 + d][2 * i] * f[i], o[c0 / 8 + d][2 * i + 1] * f[i]);
       if (!meet_all()) break;
-      for (int c = threadIdx.x; c < pc.rows * (COLS / 4); c += WARPS * 32) {
+      for (int c = thread; c < pc.rows * (COLS / 4); c += WARPS * 32) {
         const int r = c / (COLS / 4), col = (c % (COLS / 4)) * 4;
         const float* from = merge + ((r >> 4) * 16 + (r & 15)) * COLS + (((col >> 3) ^ (r & 7 & (COLS / 8 - 1))) * 8) + (col & 7);
         float4 v = *reinterpret_cast<const float4*>(from);
@@ -542,7 +556,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   if (!ok && lane == 0 && !*abort_flag) give_up();
 }
 
-// Joins the pieces of the row tile whose keys begin in a CTA's range and end in another's: blocks for each CTA, of which most have nothing to do, and a
+// Joins the pieces of the row tile whose keys begin in one range and end in another: blocks for each range, of which most have nothing to do, and a
 // thread for every four columns of a row or of several.  Behind those of the launch for few rows come those of the one for many.
 constexpr int PA_JOIN_THREADS = 128;
 
@@ -609,18 +623,18 @@ static int pa_few_launch(const PagedAttnParams& p, const CUtensorMap& k, const C
     if (cudaFuncSetAttribute(paged_attn_few_kernel<D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return TPB_ERR_CUDA;
     ready[dev].store(true, std::memory_order_release);
   }
-  return launch_dependent(paged_attn_few_kernel<D, R>, dim3(grid), dim3(C::THREADS), C::SMEM, stream, true, k, v, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
+  return launch_dependent(paged_attn_few_kernel<D, R>, dim3(grid), dim3(C::THREADS * C::TEAMS), C::SMEM, stream, true, k, v, p) == cudaSuccess ? TPB_OK : TPB_ERR_CUDA;
 }
 
-static int pa_few_ctas(int head_dim, int row_groups) {
-  if (head_dim == 64) return row_groups == 1 ? Few<64, 1>::CTAS : row_groups == 2 ? Few<64, 2>::CTAS : Few<64, 4>::CTAS;
-  return row_groups == 1 ? Few<128, 1>::CTAS : row_groups == 2 ? Few<128, 2>::CTAS : Few<128, 4>::CTAS;
+static int pa_few_teams(int head_dim, int row_groups) {
+  if (head_dim == 64) return row_groups == 1 ? Few<64, 1>::TEAMS : row_groups == 2 ? Few<64, 2>::TEAMS : Few<64, 4>::TEAMS;
+  return row_groups == 1 ? Few<128, 1>::TEAMS : row_groups == 2 ? Few<128, 2>::TEAMS : Few<128, 4>::TEAMS;
 }
 
 // What a call launches.  Sequences with few query rows (new tokens x query heads of a KV head) go by the kernel above, bound by memory; those with more by the one
 // on the tensor cores of paged_attention_sm100.cu.  The host knows the rows of a sequence at most; where both kinds may be in the batch, both are launched.
 struct PagedPlan {
-  int row_groups, few_grid, few_high, wide_grid;  // grid 0: not launched; sequences up to few_high rows are the first's
+  int row_groups, few_grid, few_slots, few_ranges, few_high, wide_grid;  // grid 0: not launched; sequences up to few_high rows are the first's
   bool joins;
   long long few_floats, wide_floats;
 };
@@ -636,9 +650,11 @@ static PagedPlan pa_plan(int n, int tokens, int table_width, int page_shift, int
   plan.few_high = !few ? 0 : wide ? rows : INT_MAX;
   if (few) {
     const long long tiles = min((long long)tokens * group / rows + n, (long long)n * ((min(most_rows, (long long)plan.few_high) + rows - 1) / rows)) * kv_heads;
-    const long long most = tiles * ((keys + PA_TILE - 1) / PA_TILE + PA_PIECE_COST), resident = (long long)pa_sms() * pa_few_ctas(head_dim, plan.row_groups);
-    plan.few_grid = int(max(1LL, min(resident, plan.joins ? (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE : tiles)));
-    plan.few_floats = (long long)plan.few_grid * 2 * (rows * (head_dim + 2) + 4);
+    const long long most = tiles * ((keys + PA_TILE - 1) / PA_TILE + PA_PIECE_COST), ranges = plan.joins ? (most + PA_MIN_SHARE - 1) / PA_MIN_SHARE : tiles;
+    plan.few_grid = wide ? pa_sms() : int(max(1LL, min((long long)pa_sms(), ranges)));
+    plan.few_slots = plan.few_grid * pa_few_teams(head_dim, plan.row_groups);
+    plan.few_ranges = wide ? plan.few_slots : int(max(1LL, min((long long)plan.few_slots, ranges)));
+    plan.few_floats = (long long)plan.few_slots * 2 * (rows * (head_dim + 2) + 4);
   }
   if (wide) {
     plan.wide_grid = pw_grid(head_dim);
@@ -692,8 +708,10 @@ extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
   p.heads = a->heads, p.kv_heads = a->kv_heads, p.group = group, p.window = a->window;
   p.scale_log2e = a->scale * 1.4426950408889634f;
   p.whole = !plan.joins;
+  p.few_high = plan.few_high;
+  p.split_sms = plan.few_grid && plan.wide_grid ? pa_sms() : 0;
   float* room = static_cast<float*>(a->workspace);
-  const PagedParts few = pa_parts(room, plan.few_grid, 16 * plan.row_groups, a->head_dim), wide = pa_parts(room, plan.wide_grid, PW_ROWS, a->head_dim);
+  const PagedParts few = pa_parts(room, plan.few_slots, 16 * plan.row_groups, a->head_dim), wide = pa_parts(room, plan.wide_grid, PW_ROWS, a->head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
   auto maps = [&](auto paged_map, CUtensorMap& k, CUtensorMap& v, int tile) {
     const int box = min(a->page_size, tile);
@@ -705,6 +723,7 @@ extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
     rc = maps(paged_blocks_tmap, k, v, PA_TILE);
     if (rc != TPB_OK) return rc;
     p.parts = few;
+    p.ranges = plan.few_ranges;
     p.rows_low = 1, p.rows_high = plan.few_high;
     p.takes_bad = 1;
     p.fill_rest = a->fill_rest;
@@ -728,7 +747,7 @@ extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
   // a thread for each four columns of the first launch's tiles, for each eight of the second's
   auto blocks = [&](int rows, int of_thread) { return (rows * (a->head_dim / 4) + of_thread * PA_JOIN_THREADS - 1) / (of_thread * PA_JOIN_THREADS); };
   const int of_few = blocks(int(min((long long)few.rows, max(1LL, (long long)min(a->most_new, a->tokens) * group))), 1), of_wide = blocks(PW_ROWS, 2);
-  const int few_blocks = plan.few_grid * of_few;
+  const int few_blocks = plan.few_ranges * of_few;
   const dim3 grid(few_blocks + plan.wide_grid * of_wide);
   auto join = a->head_dim == 64 ? paged_attn_join_kernel<64> : paged_attn_join_kernel<128>;
   const cudaError_t launched = launch_dependent(join, grid, dim3(PA_JOIN_THREADS), 0, s, true, p, few, few_blocks, of_few, wide, of_wide);

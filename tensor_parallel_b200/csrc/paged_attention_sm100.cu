@@ -149,10 +149,13 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     return s.bad || rows < p.rows_low || rows > p.rows_high ? 0 : (rows + PW_ROWS - 1) / PW_ROWS;
   };
   long long share, w0, w1;
-  share_out<PW_THREADS>(p.b.n, PW_MIN_SHARE, range, [&](int i) {
+  float few = 0.f, wide = 0.f;
+  auto meet = [&]() { __syncthreads(); };
+  share_out<PW_THREADS>(p.b.n, PW_MIN_SHARE, threadIdx.x, blockIdx.x, range, [&](int i) {
     PagedSequence s;
     int rows, first, end, low;
     const int row_tiles = units_of(i, s, rows);
+    if (p.split_sms) pa_load(p, s, D, few, wide);
     if (s.bad && p.takes_bad) {
       any_bad = 1;
       if (blockIdx.x == 0) atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
@@ -163,7 +166,11 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       cost += end - first + piece_cost<N>();
     }
     return cost * p.kv_heads;
-  }, share, w0, w1);
+  }, [&]() {
+    if (!p.split_sms) return gridDim.x;
+    sum_loads<PW_THREADS>(range, threadIdx.x, meet, few, wide);
+    return unsigned(max(1, p.split_sms - pa_few_sms(few, wide, p.split_sms)) * C::CTAS);
+  }, meet, share, w0, w1);
   if (any_bad)
     for (int i = 0; i < p.b.n; ++i) {
       const PagedSequence s = paged_sequence(p.b, i);
