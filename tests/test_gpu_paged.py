@@ -513,3 +513,41 @@ def test_falcon_heads_and_bad_lengths_without_the_kernel_for_few_rows():
     out = attend(b, most_new=2)
     assert status_of() == 3 and out[2].isnan().all()
     within(out[[0, 1, 3, 4, 5, 6, 7]], want[[0, 1, 3, 4, 5, 6, 7]], tol[[0, 1, 3, 4, 5, 6, 7]])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (8, 2, 64), (64, 2, 128), (20, 1, 64), (64, 1, 64)])
+@pytest.mark.parametrize("new,past,window", [([1] * 40 + [70], [900 + 37 * i for i in range(40)] + [0], None), ([1, 600], [0, 900], None), ([300, 1, 1, 128], [0, 2000, 5, 128], None),
+                                             ([1] * 400 + [65] * 3, [i % 50 for i in range(403)], 33), ([1, 0, 2], [300, 0, 70], None)])
+def test_decoding_sequences_beside_chunks(new, past, window, heads, kv_heads, dim):
+    """The SMs that either launch gets follow from the lengths: almost all for one, almost all for the other, all."""
+    b = batch(new, past, heads, kv_heads, dim, 16, device="cuda", rest=2)
+    want, tol = attention64(b, window=window)
+    out = attend(b, window=window)
+    within(out, want, tol)
+    assert torch.equal(out, attend(b, window=window)) and status_of() == 0
+
+
+def test_bad_lengths_beside_a_chunk():
+    b = batch([1, 200, 2, 1], [100, 40, 7, 300], 8, 2, 128, 16, device="cuda")
+    want, tol = attention64(b)
+    for s, rows in ((0, slice(0, 1)), (1, slice(1, 201)), (2, slice(201, 203))):
+        past = b["past"].clone()
+        past[s] = -5
+        out = attend(dict(b, past=past))
+        assert status_of() == 3 and out[rows].isnan().all()
+        keep = torch.ones(len(out), dtype=torch.bool)
+        keep[rows] = False
+        within(out[keep], want[keep], tol[keep])
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(8, 8), (8, 2), (64, 2), (12, 2)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_results_of_chunks_go_to_their_rows_only(heads, kv_heads, dim):
+    b = batch([260, 131, 160], [0, 70, 1000], heads, kv_heads, dim, 32, device="cuda", front=3, rest=5)
+    want, tol = attention64(b)
+    room = torch.full((len(b["q"]) + 2, heads + 3, dim + 16), 7.0, dtype=BF16, device="cuda")
+    out = room[1:-1, 2:-1, 8:-8]
+    attend(b, out=out)
+    within(out[3:-5], want[3:-5], tol[3:-5])
+    out[3:-5].fill_(7.0)  # (rows outside of all sequences are left as they were where the caller gives the result's place)
+    assert (room == 7.0).all()
