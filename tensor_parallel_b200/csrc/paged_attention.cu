@@ -161,7 +161,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   if (thread < 2) p.parts.joins[2 * range_no + thread] = make_int4(-1, 0, 0, 0);
 
   long long share, w0, w1;
-  float few = 0.f, wide = 0.f;
+  long long few = 0, wide = 0;
   auto meet_team = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(C::THREADS) : "memory"); };
   share_out<C::THREADS>(p.b.n, p.whole ? 1 : PA_MIN_SHARE, thread, range_no, range, [&](int i) {
     const PagedUnits u = paged_units<ROWS>(p, i);

@@ -53,25 +53,25 @@ __device__ __forceinline__ void pa_launch_next() { asm volatile("griddepcontrol.
 
 // The two launches of a batch with both kinds of sequences share out the SMs, so that one loads while the other multiplies: an SM alone reads about twice what
 // its part is when all of them read.  Both launches estimate from the lengths what either has to do, in the time that an SM needs for a tile of 64 keys
-// and up to 16 rows of the first.  (In a graph, one after the other on all SMs / side by side, us: 31 decoding, 777 tokens behind 3396, 32 / 8 heads of 128 143 / 119; 64 x 2001 keys
+// and up to 16 rows of the first; in whole numbers, whose sums are the same in both.  (In a graph, one after the other on all SMs / side by side, us: 31 decoding, 777 tokens behind 3396, 32 / 8 heads of 128 143 / 119; 64 x 2001 keys
 // and 512 behind 4000 145 / 121, of 64 99 / 80, 64 query heads per KV head 232 / 218; 64 x 2001 keys and four prompts of 512 128 / 110; 128 x 4001 keys and 100 334 / 331.)
 constexpr float PA_FEW_PIECE = 3.f, PA_WIDE_PIECE = 5.f;                // beside the tiles of a row tile
 constexpr float PA_FEW_32_ROWS = 2.f, PA_FEW_64_ROWS = 3.5f;           // a tile of as many rows
 constexpr float PA_WIDE_TILE_64 = 4.5f, PA_WIDE_TILE_128 = 5.5f;        // a tile of the second launch: 256 rows, as many keys as elements
-__device__ __forceinline__ void pa_load(const PagedAttnParams& p, const PagedSequence& s, int head_dim, float& few, float& wide) {
+__device__ __forceinline__ void pa_load(const PagedAttnParams& p, const PagedSequence& s, int head_dim, long long& few, long long& wide) {
   if (s.bad || s.fresh == 0) return;
   const int rows = s.fresh * p.group;
   const float keys = s.past + 0.5f * s.fresh, seen = p.window ? fminf(keys, p.window) : keys;  // of a row in the middle
   if (rows <= p.few_high)
-    few += p.kv_heads * (seen / 64.f + PA_FEW_PIECE) * (p.few_high > 32 ? PA_FEW_64_ROWS : p.few_high > 16 ? PA_FEW_32_ROWS : 1.f);
+    few += llrintf(p.kv_heads * (seen / 64.f + PA_FEW_PIECE) * (p.few_high > 32 ? PA_FEW_64_ROWS : p.few_high > 16 ? PA_FEW_32_ROWS : 1.f));
   else
-    wide += p.kv_heads * float((rows + 255) / 256) * (seen / head_dim + PA_WIDE_PIECE) * (head_dim == 64 ? PA_WIDE_TILE_64 : PA_WIDE_TILE_128);
+    wide += llrintf(p.kv_heads * float((rows + 255) / 256) * (seen / head_dim + PA_WIDE_PIECE) * (head_dim == 64 ? PA_WIDE_TILE_64 : PA_WIDE_TILE_128));
 }
 // SMs of the first launch.  The smaller part is rounded up, and then by half an SM more: one too few would weigh most there.
-__device__ __forceinline__ int pa_few_sms(float few, float wide, int sms) {
-  if (few == 0.f) return 0;
-  if (wide == 0.f) return sms;
-  const float want = sms * few / (few + wide);
+__device__ __forceinline__ int pa_few_sms(long long few, long long wide, int sms) {
+  if (few == 0) return 0;
+  if (wide == 0) return sms;
+  const float want = float(sms) * float(few) / float(few + wide);
   return max(1, min(sms - 1, int(2.f * want < sms ? ceilf(want + 0.5f) : floorf(want - 0.5f))));
 }
 
@@ -79,13 +79,13 @@ __device__ __forceinline__ int pa_few_sms(float few, float wide, int sms) {
 template <int THREADS>
 struct RangeSearch {
   long long scan[THREADS / 32];
-  float load[2][THREADS / 32];
+  long long load[2][THREADS / 32];
   long long begin;
   int seq;
 };
 // The sums of two numbers over THREADS threads.
 template <int THREADS, typename Meet>
-__device__ __forceinline__ void sum_loads(RangeSearch<THREADS>& at, int thread, Meet meet, float& a, float& b) {
+__device__ __forceinline__ void sum_loads(RangeSearch<THREADS>& at, int thread, Meet meet, long long& a, long long& b) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
     a += __shfl_xor_sync(0xffffffffu, a, d);
@@ -93,7 +93,7 @@ __device__ __forceinline__ void sum_loads(RangeSearch<THREADS>& at, int thread, 
   }
   if ((thread & 31) == 0) at.load[0][thread >> 5] = a, at.load[1][thread >> 5] = b;
   meet();
-  a = b = 0.f;
+  a = b = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) a += at.load[0][w], b += at.load[1][w];
 }

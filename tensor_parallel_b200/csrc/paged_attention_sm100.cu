@@ -158,7 +158,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     return s.bad || rows < p.rows_low || rows > p.rows_high ? 0 : (rows + PW_ROWS - 1) / PW_ROWS;
   };
   long long share, w0, w1;
-  float few = 0.f, wide = 0.f;
+  long long few = 0, wide = 0;
   auto meet = [&]() { __syncthreads(); };
   share_out<PW_THREADS>(p.b.n, PW_MIN_SHARE, threadIdx.x, blockIdx.x, range, [&](int i) {
     PagedSequence s;
