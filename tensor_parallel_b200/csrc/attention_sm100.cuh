@@ -51,10 +51,12 @@ __device__ __forceinline__ float fmax3_abs_nan(float a, float b, float c) {  // 
 // softmax of a 128 x 128 tile: as long as the tensor core needs for its two products).  x = n + f with n = round(x) taken
 // from the low mantissa bits of x + 1.5 * 2^23, a cubic for 2^f on [-0.5, 0.5] (relative error 7.5e-5, far below the bf16
 // rounding of the probabilities), n added into the exponent field.  x is clamped at -126: a masked score becomes 2^-126.
-__device__ __forceinline__ void ex2_poly2(float& x0, float& x1) {
+// `least`: what smaller exponents are taken for.  At EX2_NOTHING the polynomial is just above 1 and the exponent one below the least, which leaves 2^-140: zero in bf16.
+constexpr float EX2_NOTHING = -126.9998f;
+__device__ __forceinline__ void ex2_poly2(float& x0, float& x1, float least = -126.f) {
   constexpr float MAGIC = 12582912.f;
-  x0 = fmaxf(x0, -126.f);
-  x1 = fmaxf(x1, -126.f);
+  x0 = fmaxf(x0, least);
+  x1 = fmaxf(x1, least);
   float t0, t1, n0, n1, f0, f1, p0, p1;
   fadd2(t0, t1, x0, x1, MAGIC, MAGIC);
   fadd2(n0, n1, t0, t1, -MAGIC, -MAGIC);

@@ -490,7 +490,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         bool rescale = false;
         if (m_run == -INFINITY) {
           m_run = m_tile;  // nothing accumulated for this row yet
-          factor = 0.f;    // (but 2^-126 for each key of a tile in which it saw none)
+          factor = 0.f;    // (but 2^-140 in the sum for some keys of a tile in which it saw none)
           rescale = j > 0;
         } else if (m_tile > m_run + (j * N < PW_EXACT_KEYS ? 0.f : PW_RESCALE_LOG2)) {
           factor = ex2_approx(m_run - m_tile);
@@ -520,7 +520,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             ffma2(t0, t1, __uint_as_float(r[2 * (c + x)]), __uint_as_float(r[2 * (c + x) + 1]), p.scale_log2e, p.scale_log2e, nbase, nbase);
             float p0, p1;
             if ((x & 3) == 0) {  // (a quarter of the exponentials on the FMA pipe)
-              ex2_poly2(t0, t1);
+              ex2_poly2(t0, t1, EX2_NOTHING);  // (2^-126 of a value that a row does not see yet is not nothing: values go up to 2^128)
               p0 = t0;
               p1 = t1;
             } else {
