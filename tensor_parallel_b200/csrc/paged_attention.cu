@@ -511,7 +511,7 @@ paged_attn_few_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         top = 0.f;
         sum = __uint_as_float(0x7fc00000u);
       }
-      if (pc.slot < 0) f[i] = sum == 0.f ? 0.f : f[i] / sum;
+      if (pc.slot < 0) f[i] /= sum;  // (a row sees its own key at least: a sum of zero is of scores that are all -inf, and its result NaN)
       if (pc.slot >= 0 && kg == 0 && t4 == 0) p.parts.ml[(long long)pc.slot * ROWS + rg * 16 + g8 + 8 * i] = make_float2(top, sum);
     }
     float* merge = reinterpret_cast<float*>(ring + stage * C::STAGE_BYTES);
@@ -600,13 +600,13 @@ paged_attn_join_kernel(const PagedAttnParams p, const PagedParts few, const int 
       top = next;
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j) {
-        if (s[j].x == -INFINITY) continue;  // (no key of the piece is the row's)
+        if (s[j].x == -INFINITY && s[j].y == 0.f) continue;  // (no key of the piece is the row's; scores that are all NaN leave the sum NaN)
         const float f = ex2_approx(s[j].x - top);
         sum += s[j].y * f;
         v.x += w[j].x * f, v.y += w[j].y * f, v.z += w[j].z * f, v.w += w[j].w * f;
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = 1.f / sum;
     const int t = (unit.y + r) / p.group, h = (unit.y + r) % p.group;
     *reinterpret_cast<uint2*>(p.out + (long long)(unit.x + t) * p.o_st + (long long)(unit.w * p.group + h) * p.o_sh + col) =
         make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));

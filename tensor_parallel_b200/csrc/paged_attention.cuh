@@ -24,7 +24,7 @@ typedef __nv_bfloat16 bf16;
 // slot 2c + 1 of the range c in which the keys begin, those of the ranges behind it in their slots 2c'.
 struct PagedParts {
   float* o;    // [2 per range][rows of a tile][head_dim], not divided by the sum
-  float2* ml;  // [2 per range][rows of a tile] maximum (of scaled scores, in powers of two; -inf: the piece adds nothing) and sum
+  float2* ml;  // [2 per range][rows of a tile] maximum (of scaled scores, in powers of two) and sum; -inf and 0: the piece adds nothing
   int4* joins; // [2 per range]: (first row of the queries, first row of the tile, rows, KV head) and (last range); first -1: nothing to join
   int rows;    // of a tile
 };

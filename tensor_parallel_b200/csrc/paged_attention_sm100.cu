@@ -482,17 +482,19 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
 #pragma unroll
         for (int c = 0; c < N; c += 4) {
-          m0 = fmax3(m0, __uint_as_float(r[c]), __uint_as_float(r[c + 1]));
-          m1 = fmax3(m1, __uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
+          m0 = fmax3_nan(m0, __uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+          m1 = fmax3_nan(m1, __uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
         }
-        const float m_tile = fmaxf(m0, m1) * p.scale_log2e;  // (the scale is positive: the maximum commutes with it)
+        // (the scale is positive: the maximum commutes with it.  A score that is NaN makes the maximum NaN, and with it all that follows of the row: the
+        // exponentials on the FMA pipe would drop it)
+        const float m_tile = fmax3_nan(m0, m1, m1) * p.scale_log2e;
         float factor = 1.f;
         bool rescale = false;
         if (m_run == -INFINITY) {
           m_run = m_tile;  // nothing accumulated for this row yet
           factor = 0.f;    // (but 2^-140 in the sum for some keys of a tile in which it saw none)
           rescale = j > 0;
-        } else if (m_tile > m_run + (j * N < PW_EXACT_KEYS ? 0.f : PW_RESCALE_LOG2)) {
+        } else if (!(m_tile <= m_run + (j * N < PW_EXACT_KEYS ? 0.f : PW_RESCALE_LOG2))) {
           factor = ex2_approx(m_run - m_tile);
           m_run = m_tile;
           rescale = true;
@@ -547,7 +549,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       const bool poisoned = reinterpret_cast<volatile int*>(lost)[i % PW_LOST] == i + 1;
       if (m_run == -INFINITY) l_run = 0.f;
-      if (poisoned) l_run = __uint_as_float(0x7fc00000u);
+      if (poisoned || !(m_run < INFINITY)) l_run = __uint_as_float(0x7fc00000u);  // (scores that are NaN or infinite)
       const int left = pc.rows - t * PW_M - quarter * 32;  // of this warp's rows
       uint8_t* stage = out_s + (warp - 4) * C::STAGE_BYTES;
       if (lane == 0) tma_stores_read();  // (of the piece in front)
@@ -555,7 +557,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       if (boxed_out && left >= 32 && n > 0 && pc.slot < 0) {
         // whole tokens: 64 elements of 32 rows at a time by a box of their own (by loads and stores, as below, a piece's results hold both of its tiles up for 2.9 us:
         // us without / with boxes, 64 prompts of 256 tokens, 32 heads of 128 155 / 135, 16 of 1000, 32 / 8 heads 227 / 217, of 16.4 k tokens 453 / 441)
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        const float inv = 1.f / l_run;  // (a row sees its own key at least: a sum of zero is of scores that are all -inf, and its result NaN)
 #pragma unroll 1
         for (int c = 0; c < D; c += 64) {
           uint32_t o[64];
@@ -577,7 +579,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       } else if (left > 0) {
         // through shared memory, 128 bytes of each row at a time in swizzled chunks of 16: a thread has a row, and eight threads store a line of one
         const bool whole = pc.slot < 0;
-        const float inv = whole ? (l_run == 0.f ? 0.f : 1.f / l_run) : 1.f;
+        const float inv = whole ? 1.f / l_run : 1.f;
         if (!whole && lane < left) p.parts.ml[(long long)pc.slot * PW_ROWS + t * PW_M + quarter * 32 + lane] = make_float2(poisoned ? 0.f : m_run, l_run);
         const int step_tokens = 4 / p.group, step_heads = 4 % p.group;
         const int first_token = (pc.row0 + t * PW_M + quarter * 32 + (lane >> 3)) / p.group, first_head = (pc.row0 + t * PW_M + quarter * 32 + (lane >> 3)) % p.group;

@@ -1,5 +1,7 @@
 """Paged attention, append and adjusted logits where their kernels change form: rows that are not finite, pages that are not there, strides beyond 32 bits, sizes behind
 which a launch is made another way."""
+import math
+
 import pytest
 import torch
 
@@ -31,6 +33,26 @@ def attend(b, **kw):
     out = OF.paged_attention(b["q"], cache_of(b), b["starts"], b["past"], **kw)
     assert native().launch_count > before
     return out
+
+
+@pytest.mark.parametrize("number", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (8, 2, 128), (12, 4, 64)])
+@pytest.mark.parametrize("new,past,rows", [([1], [9999], [0]), ([1, 1, 1], [50, 4000, 9], [0, 1, 2]), ([3], [12000], [1]), ([600], [8000], [0, 333, 599]), ([300, 1], [0, 70], [0, 1, 2, 3, 130, 300]),
+                                           ([1, 200, 1], [900, 3000, 40], [0, 1, 70, 201])])
+def test_query_rows_that_are_not_finite(new, past, rows, heads, kv_heads, dim, number):
+    """A row of queries that is NaN, or infinite in an element, gives NaN wherever its keys are cut, and its neighbours what they give without it."""
+    b = batch(new, past, heads, kv_heads, dim, 16, device="cuda", seed=len(new) + past[0])
+    want, tol = attention64(b)
+    q = b["q"].clone()
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    for i, r in enumerate(rows):
+        q[r, (3 * i + 1) % heads, 5 if math.isinf(number) else slice(None)] = number
+        bad[r, (3 * i + 1) % heads] = True
+    for most_new in (None, max(new)):
+        out = attend(dict(b, q=q), most_new=most_new)
+        assert out[bad].isnan().all()
+        within(out[~bad], want[~bad], tol[~bad])
+    assert status_of() == 0
 
 
 @pytest.mark.parametrize("dim", [64, 128])
