@@ -111,7 +111,9 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   uint64_t* piece_full = bars + 18;    // [PW_PIECES]
   uint64_t* piece_empty = bars + 18 + PW_PIECES;
   WidePiece* pieces = reinterpret_cast<WidePiece*>(bars + 18 + 2 * PW_PIECES);  // [PW_PIECES]
-  int* lost = reinterpret_cast<int*>(pieces + PW_PIECES);                       // [PW_LOST] number (from 1) of a piece of which a page is not there
+  // [PW_LOST] (number (from 1) of a piece of which a page is not there) << 32 | its first tile with such a page.  A query tile that ends in front of that tile of keys
+  // may look while the producer writes: in one word, which it finds wrong either way
+  unsigned long long* lost = reinterpret_cast<unsigned long long*>(pieces + PW_PIECES);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(lost + PW_LOST);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   __shared__ RangeSearch<PW_THREADS> range;
@@ -273,6 +275,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         int entry0 = tile0 * N >> p.b.page_shift;
         auto fetch = [&](int e) { return e < entries ? __ldg(row + e) : -1; };
         int now = fetch(entry0 + lane), next = fetch(entry0 + 32 + lane);
+        bool whole = true;
         for (int j = 0; ok && j < n; ++j, ++kt) {
           const int s = kt & 1, key0 = (tile0 + j) * N;
           const uint32_t par = ((kt >> 1) & 1) ^ 1;
@@ -288,9 +291,12 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           const bool wanted = lane < per_tile * DB && (per_tile == 1 || (first < total && first + page_size > low));
           const bool good = wanted && page >= 0 && page < p.b.pages;
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, good)) * box_rows * 128;
-          if (__any_sync(0xffffffffu, wanted && !good) && lane == 0) {
-            atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
-            lost[i % PW_LOST] = i + 1;
+          if (whole && __any_sync(0xffffffffu, wanted && !good)) {
+            whole = false;
+            if (lane == 0) {
+              atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+              *reinterpret_cast<volatile unsigned long long*>(lost + i % PW_LOST) = static_cast<unsigned long long>(i + 1) << 32 | unsigned(j);
+            }
           }
           const uint32_t to = my_block * (N * 128) + my_page * box_rows * 128;
           const int slot = per_tile == 1 ? key0 & (page_size - 1) : 0;
@@ -547,7 +553,8 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (!ok) break;
         tc_fence_after();
       }
-      const bool poisoned = reinterpret_cast<volatile int*>(lost)[i % PW_LOST] == i + 1;
+      const unsigned long long gone = *reinterpret_cast<volatile unsigned long long*>(lost + i % PW_LOST);
+      const bool poisoned = int(gone >> 32) == i + 1 && int(unsigned(gone)) < n;
       if (m_run == -INFINITY) l_run = 0.f;
       if (poisoned || !(m_run < INFINITY)) l_run = __uint_as_float(0x7fc00000u);  // (scores that are NaN or infinite)
       const int left = pc.rows - t * PW_M - quarter * 32;  // of this warp's rows

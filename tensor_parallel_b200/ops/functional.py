@@ -677,7 +677,7 @@ def paged_attention(q, cache: PagedCache, starts, past, scale: Optional[float] =
     read; a sequence's own keys and values have to be finite (one that is not may reach any of its new tokens).  A row of queries with scores that are not finite gives NaN.
 
     The result is a new tensor, zero in rows outside all sequences, or ``out`` (which may be ``q``), left as it is there.  A sequence whose rows or table
-    do not fit, or with more than ``most_new`` new tokens, gives NaN, as rows do that reach a page outside the cache, and the CUDA kernel records status 3
+    do not fit, or with more than ``most_new`` new tokens, gives NaN, as rows do that reach a page outside the cache (and some of those in front of them in its sequence), and the CUDA kernel records status 3
     (see ``native.device_state``); the steps over tensors raise.  Serving only: there is no gradient."""
     if _compiling():
         torch._dynamo.graph_break()

@@ -66,3 +66,21 @@ def test_values_that_a_row_does_not_see_yet(dim):
     within(attend(b)[:60], want[:60], tol[:60])
     want, tol = attention64(b, window=30)
     within(attend(b, window=30)[:60], want[:60], tol[:60])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 128), (2, 2, 64), (4, 1, 128), (7, 1, 64)])
+def test_a_page_that_only_later_rows_reach(heads, kv_heads, dim):
+    """The first half of a row tile of 256 ends in front of the tile of keys with a page that is not there: its rows are right, call after call; those that reach the page are NaN."""
+    group = heads // kv_heads
+    tokens, half = 256 // group, -(-128 // group)
+    b = batch([tokens], [256 - half], heads, kv_heads, dim, 16, device="cuda")  # (the half's last key is the last of a tile)
+    want, tol = attention64(b)
+    bad = dict(b, table=b["table"].clone())
+    page = (256 - half + tokens - 1) // 16
+    bad["table"][0, page] = -1
+    outs = [attend(bad) for _ in range(20)]
+    assert status_of() == 3
+    within(outs[0][:128 // group], want[:128 // group], tol[:128 // group])
+    assert outs[0][page * 16 - (256 - half):].isnan().all()
+    for out in outs:
+        assert torch.equal(out.view(torch.int16), outs[0].view(torch.int16))
