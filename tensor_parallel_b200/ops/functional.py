@@ -210,16 +210,29 @@ class Rotary(NamedTuple):
     factor: float = 1.0
 
 
+# What a dictionary of scaled frequencies may name, by its kind.
+_SCALING_KEYS = {"default": (), "linear": ("factor",), "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+                 "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim")}
+
+
 def rotary(rotary_dim: int, theta: float = 10000.0, interleaved: bool = False, scaling: Optional[dict] = None, device=None) -> Rotary:
     """The usual frequencies ``theta ** (-2i / rotary_dim)``, for contexts longer than a model was trained on scaled as ``scaling`` says (the dictionary of
     a Hugging Face configuration): ``"linear"`` (all slower by ``factor``), ``"llama3"`` (slow ones slower by ``factor``, a ramp between) or ``"yarn"`` (a ramp over the
-    pairs, and a factor on cosine and sine)."""
+    pairs, from whole pairs unless ``truncate`` is false, and a factor on cosine and sine: ``attention_factor``, or by ``mscale`` and ``mscale_all_dim`` where both
+    are there).  A ``rope_theta`` in it has to be ``theta``, and a ``partial_rotary_factor`` is what ``rotary_dim`` says already; what else it names is refused."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"a rotation takes an even number of elements, got {rotary_dim}")
     f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
     kind, factor = "default", 1.0
     if scaling:
         kind = scaling.get("rope_type", scaling.get("type", "default"))
+        if kind not in _SCALING_KEYS:
+            raise ValueError(f"scaling of rotary frequencies: 'linear', 'llama3' or 'yarn', got {kind!r}")
+        strange = sorted(set(scaling) - {"rope_type", "type", "rope_theta", "partial_rotary_factor", *_SCALING_KEYS[kind]})
+        if strange:
+            raise ValueError(f"scaling of rotary frequencies: {kind!r} does not know {', '.join(map(repr, strange))}")
+        if scaling.get("rope_theta", theta) != theta:
+            raise ValueError(f"scaling of rotary frequencies: it says rope_theta={scaling['rope_theta']}, theta is {theta}")
     if kind == "linear":
         f = f / scaling["factor"]
     elif kind == "llama3":
@@ -228,16 +241,25 @@ def rotary(rotary_dim: int, theta: float = 10000.0, interleaved: bool = False, s
         keep = ((turns - low) / (high - low)).clamp(0, 1)
         f = f * keep + f / scaling["factor"] * (1 - keep)
     elif kind == "yarn":
+        by = scaling["factor"]
+
         def pair(turns):  # the pair that makes so many turns over the original context
             return rotary_dim * math.log(scaling["original_max_position_embeddings"] / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
-        low, high = max(math.floor(pair(scaling.get("beta_fast", 32))), 0), min(math.ceil(pair(scaling.get("beta_slow", 1))), rotary_dim - 1)
-        slow = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
-        f = f * (1 - slow) + f / scaling["factor"] * slow
-        factor = scaling.get("attention_factor") or (0.1 * math.log(scaling["factor"]) + 1.0 if scaling["factor"] > 1 else 1.0)
-    elif kind != "default":
-        raise ValueError(f"scaling of rotary frequencies: 'linear', 'llama3' or 'yarn', got {kind!r}")
-    return Rotary(f.float().to(device), interleaved, factor)
+        def temperature(weight):
+            return 0.1 * weight * math.log(by) + 1.0 if by > 1 else 1.0
+
+        low, high = pair(scaling.get("beta_fast") or 32), pair(scaling.get("beta_slow") or 1)
+        if scaling.get("truncate", True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rotary_dim - 1)
+        slow = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / (high - low if high != low else 0.001)).clamp(0, 1)
+        f = f * (1 - slow) + f / by * slow
+        factor = scaling.get("attention_factor")
+        if factor is None:
+            whole, part = scaling.get("mscale"), scaling.get("mscale_all_dim")
+            factor = temperature(whole) / temperature(part) if whole and part else temperature(1.0)
+    return Rotary(f.float().to(device), interleaved, float(factor))
 
 
 def _spans(what: str, cache: PagedCache, tokens: int, starts, past, most_new: Optional[int] = None):

@@ -1,0 +1,56 @@
+"""Ragged serving operators on the CPU: scaled frequencies pair by pair, what the C entries refuse, prompts of other types."""
+import math
+
+import pytest
+import torch
+
+from tensor_parallel_b200.ops import functional as OF
+
+
+def yarn64(dim, theta, d):
+    """Frequencies and factor by the published formulas, one pair at a time."""
+    original, by = d["original_max_position_embeddings"], d["factor"]
+    ends = [dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(theta)) for turns in (d.get("beta_fast") or 32, d.get("beta_slow") or 1)]
+    if d.get("truncate", True):
+        ends = [math.floor(ends[0]), math.ceil(ends[1])]
+    low, high = max(ends[0], 0), min(ends[1], dim - 1)
+    frequencies = []
+    for i in range(dim // 2):
+        f = theta ** (-2 * i / dim)
+        slow = min(max((i - low) / (high - low), 0.0), 1.0)
+        frequencies.append((1 - slow) * f + slow * f / by)
+    if d.get("attention_factor") is not None:
+        factor = d["attention_factor"]
+    elif d.get("mscale") and d.get("mscale_all_dim"):
+        factor = (0.1 * d["mscale"] * math.log(by) + 1) / (0.1 * d["mscale_all_dim"] * math.log(by) + 1) if by > 1 else 1.0
+    else:
+        factor = 0.1 * math.log(by) + 1 if by > 1 else 1.0
+    return torch.tensor(frequencies, dtype=torch.float64), factor
+
+
+@pytest.mark.parametrize("dim,theta,more", [
+    (64, 10000.0, dict(factor=4.0)), (128, 1000000.0, dict(factor=4.0, beta_fast=24, beta_slow=2)), (64, 150000.0, dict(factor=32.0, truncate=False)),
+    (64, 150000.0, dict(factor=32.0, truncate=True, beta_fast=None, beta_slow=None)), (64, 10000.0, dict(factor=40.0, mscale=1.0, mscale_all_dim=1.0)),
+    (64, 10000.0, dict(factor=40.0, mscale=0.707, mscale_all_dim=1.0)), (64, 10000.0, dict(factor=40.0, mscale=0.707)), (64, 10000.0, dict(factor=40.0, mscale_all_dim=0.707)),
+    (64, 10000.0, dict(factor=40.0, mscale=0.0, mscale_all_dim=0.0)), (64, 10000.0, dict(factor=1.0, mscale=0.5, mscale_all_dim=1.0)), (32, 10000.0, dict(factor=8.0, attention_factor=1.5)),
+    (32, 10000.0, dict(factor=8.0, attention_factor=0.0, mscale=1.0, mscale_all_dim=0.5)), (32, 10000.0, dict(factor=8.0, attention_factor=None))])
+@pytest.mark.parametrize("original", [4096, 32768])
+def test_yarn_pair_by_pair(dim, theta, more, original):
+    d = dict(rope_type="yarn", original_max_position_embeddings=original, **more)
+    want, factor = yarn64(dim, theta, d)
+    got = OF.rotary(dim, theta, scaling=d)
+    # a rounding to fp32, and some in 64 bits
+    assert ((got.frequencies.double() - want).abs() <= 2.0 ** -24 * 1.01 * want).all()
+    assert got.factor == pytest.approx(factor, rel=1e-14) and isinstance(got.factor, float)
+    assert torch.equal(OF.rotary(dim, theta, scaling=dict(d, rope_theta=theta, partial_rotary_factor=0.5)).frequencies, got.frequencies)
+
+
+def test_scaling_that_is_not_known_is_refused_by_name():
+    yarn = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096)
+    for scaling, name in ((dict(yarn, short_factor=[1.0]), "short_factor"), (dict(rope_type="default", mrope_section=[16, 24, 24]), "mrope_section"),
+                          (dict(type="linear", factor=2.0, mscale=1.0), "mscale"), (dict(yarn, rope_theta=500000.0), "rope_theta"), (dict(rope_type="longrope", factor=4.0), "longrope")):
+        with pytest.raises(ValueError, match=name):
+            OF.rotary(64, scaling=scaling)
+    plain = OF.rotary(64)
+    for scaling in (None, {}, dict(rope_type="default"), dict(rope_type="default", rope_theta=10000.0)):
+        assert torch.equal(OF.rotary(64, scaling=scaling).frequencies, plain.frequencies)
