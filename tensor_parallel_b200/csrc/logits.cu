@@ -296,6 +296,22 @@ static int lg_launch(const LogitsParams& p, int rows, cudaStream_t stream) {
   return lg_seen<T, 0>(p, rows, part, int((p.vocab + (long long)part - 1) / part), stream);
 }
 
+// Whether results may be written where they are: the logits of tokens that a row has had are read once more behind the stream's stores of their neighbours, or (two kernels) while
+// they are under way, so that nothing of the two may lie in one place.  Without a history a thread stores what it has read itself.
+static bool lg_places(const tpb_adjust_logits_t& a) {
+  const long long size = a.dtype ? 4 : 2, row = a.vocab * size, x_pitch = a.logits_ld * size, y_pitch = a.out_ld * size;
+  const intptr_t x = reinterpret_cast<intptr_t>(a.logits), y = reinterpret_cast<intptr_t>(a.out);
+  const bool one_pitch = a.rows == 1 || x_pitch == y_pitch;
+  if (x == y && one_pitch) return !(a.tokens && a.width);
+  const long long x_rest = (a.rows - 1) * x_pitch, y_rest = (a.rows - 1) * y_pitch;
+  const intptr_t x0 = x + min(0LL, x_rest), x1 = x + max(0LL, x_rest) + row, y0 = y + min(0LL, y_rest), y1 = y + max(0LL, y_rest) + row;
+  if (x1 <= y0 || y1 <= x0) return true;
+  // rows of one in the gaps of the other's
+  if (a.rows == 1 || !one_pitch || x_pitch <= 0) return false;
+  const long long apart = ((y - x) % x_pitch + x_pitch) % x_pitch;
+  return apart >= row && apart + row <= x_pitch;
+}
+
 }  // namespace tpb
 
 using namespace tpb;
@@ -303,6 +319,7 @@ using namespace tpb;
 extern "C" int tpb_adjust_logits(const tpb_adjust_logits_t* a, void* stream_) {
   if (!a || !a->logits || !a->out || !a->status || a->rows <= 0 || a->vocab <= 0 || a->width < 0 || a->dtype < 0 || a->dtype > 1) return TPB_ERR_ARG;
   if (a->vocab > 1 << 30) return TPB_ERR_SIZE;
+  if (!lg_places(*a)) return TPB_ERR_ARG;
   LogitsParams p = {a->logits, a->out, a->tokens, a->lengths, a->prompts, a->repetition, a->frequency, a->presence, a->bias, reinterpret_cast<const uint32_t*>(a->allowed),
                     static_cast<uint32_t*>(a->status), a->logits_ld, a->out_ld, a->tokens_ld, a->bias_ld, a->allowed_ld, a->vocab, a->width, a->bias_dtype,
                     a->repetition_all, a->frequency_all, a->presence_all};

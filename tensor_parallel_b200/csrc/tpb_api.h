@@ -201,7 +201,7 @@ int tpb_paged_append(const tpb_paged_append_t* args, void* stream);
 // Logits [rows][vocab] (bf16: dtype 0, fp32: 1) of sequences in front of the pick of a token: x of a token that is among the first `lengths` of its row's
 // tokens becomes x > 0 ? x / repetition : x * repetition; then frequency * count + presence * (count > 0) is subtracted, count being how often it is among those
 // behind the first `prompts`; bias is added; a token whose bit of `allowed` is clear becomes -inf.  Each of them may be null (per row: the number `*_all`
-// holds then).  out may be logits.
+// holds then).  out has no element in common with logits; without tokens it may be logits itself (one address, one pitch).
 typedef struct {
   const void* logits;
   void* out;

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from paged_cases import BF16, attention64, batch, within
+from paged_cases import BF16, attention64, batch, numbers, within
 from tensor_parallel_b200.ops import functional as OF
 
 pytestmark = pytest.mark.gpu
@@ -84,3 +84,35 @@ def test_a_page_that_only_later_rows_reach(heads, kv_heads, dim):
     assert outs[0][page * 16 - (256 - half):].isnan().all()
     for out in outs:
         assert torch.equal(out.view(torch.int16), outs[0].view(torch.int16))
+
+
+# -- logits ----------------------------------------------------------------------------------------
+
+
+def _adjust(x, out, tokens=None, bias=None):
+    status = native().device_state(x.device).status
+    a = native().AdjustLogits(logits=x.data_ptr(), out=out.data_ptr(), status=status.data_ptr(), logits_ld=x.stride(0), out_ld=out.stride(0), rows=x.shape[0], vocab=x.shape[1],
+                              dtype=int(x.dtype == torch.float32), repetition_all=1.25, presence_all=0.5)
+    if tokens is not None:
+        a.tokens, a.tokens_ld, a.width = tokens.data_ptr(), tokens.stride(0), tokens.shape[1]
+    if bias is not None:
+        a.bias, a.bias_dtype = bias.data_ptr(), 1
+    native().check(native().LIB.tpb_adjust_logits(a, torch.cuda.current_stream().cuda_stream), "tpb_adjust_logits")
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 1000), (40, 65000)])
+def test_where_the_c_entry_writes_results(rows, vocab):
+    gen = torch.Generator().manual_seed(2)
+    room = numbers(gen, rows, 2 * vocab + 8, dtype=torch.float32, scale=4.0).cuda()
+    bias, tokens = numbers(gen, vocab, dtype=torch.float32).cuda(), torch.randint(0, vocab, (rows, 50), generator=gen).cuda()
+    x, beside = room[:, :vocab], room[:, vocab + 4:2 * vocab + 4]
+    given, edges = x.clone(), room[:, vocab:vocab + 4].clone()
+    # in the gaps between the rows, with a history
+    _adjust(x, beside, tokens, bias)
+    torch.cuda.synchronize()
+    assert torch.equal(beside, OF.adjust_logits(given, tokens, None, None, 1.25, None, 0.5, bias=bias))
+    assert torch.equal(x, given) and torch.equal(room[:, vocab:vocab + 4], edges)
+    # in place, without one
+    _adjust(x, x, None, bias)
+    torch.cuda.synchronize()
+    assert torch.equal(x, given + bias)

@@ -54,3 +54,31 @@ def test_scaling_that_is_not_known_is_refused_by_name():
     plain = OF.rotary(64)
     for scaling in (None, {}, dict(rope_type="default"), dict(rope_type="default", rope_theta=10000.0)):
         assert torch.equal(OF.rotary(64, scaling=scaling).frequencies, plain.frequencies)
+
+
+def _adjust(x, out, tokens=None):
+    """The C entry's answer for ``x`` and ``out``, ``[rows, vocab]`` views (on a GPU where there is one: nothing here is launched with addresses that it cannot reach)."""
+    from tensor_parallel_b200.ops import native
+
+    status = torch.zeros(4, dtype=torch.int32, device=x.device)
+    a = native.AdjustLogits(logits=x.data_ptr(), out=out.data_ptr(), status=status.data_ptr(), logits_ld=x.stride(0), out_ld=out.stride(0), rows=x.shape[0], vocab=x.shape[1],
+                            dtype=int(x.dtype == torch.float32), repetition_all=1.0)
+    if tokens is not None:
+        a.tokens, a.tokens_ld, a.width = tokens.data_ptr(), tokens.stride(0), tokens.shape[1]
+    return native.LIB.tpb_adjust_logits(a, None)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_results_over_the_logits_are_refused_in_c(dtype):
+    device = "cuda" if torch.cuda.is_available() else "cpu"
+    room, tokens = torch.zeros(12, 128, dtype=dtype, device=device), torch.zeros(4, 3, dtype=torch.int64, device=device)
+    x = room[:4, :64]
+    err_arg = 1
+    assert _adjust(x, x, tokens) == err_arg                       # in place, and tokens to come back to
+    assert _adjust(x[:1], x[:1], tokens) == err_arg
+    for history in (None, tokens):
+        assert _adjust(x, room[1:5, :64], history) == err_arg     # a row further down
+        assert _adjust(x, room[:4, 8:72], history) == err_arg     # a few columns on
+        assert _adjust(x, room[:4, 72:].as_strided((4, 64), (128, 1), 72), history) == err_arg  # beyond the gap
+        assert _adjust(x, room.as_strided((4, 64), (64, 1)), history) == err_arg                # another pitch
+        assert _adjust(x[:1], room[:1, 63:127], history) == err_arg
