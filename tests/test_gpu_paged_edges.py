@@ -89,6 +89,57 @@ def test_a_page_that_only_later_rows_reach(heads, kv_heads, dim):
 # -- logits ----------------------------------------------------------------------------------------
 
 
+def logits64(x, tokens, lengths, prompts, repetition, frequency, presence, bias, allowed):
+    """``(want, tolerance)`` of long histories: a rounding to the type, and four in 32 bits of what goes into a result (logit, penalties, bias)."""
+    want, half = x.double().clone(), 2.0 ** -8 if x.dtype == BF16 else 2.0 ** -24
+    rows, vocab = x.shape
+    size = want.abs()
+    for r in range(rows):
+        history = tokens[r, :int(lengths[r])]
+        there = (history >= 0) & (history < vocab)
+        seen = torch.bincount(history[there], minlength=vocab) > 0
+        there[:int(prompts[r])] = False
+        count = torch.bincount(history[there], minlength=vocab)
+        rep, f, p = (float(t[r]) for t in (repetition, frequency, presence))
+        want[r] = torch.where(seen, torch.where(want[r] > 0, want[r] / rep, want[r] * rep), want[r])
+        size[r] = size[r] * max(rep, 1 / rep) + (f * count + p * (count > 0)).abs()
+        want[r] -= f * count + p * (count > 0)
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    if allowed is not None:
+        at = torch.arange(vocab, device=x.device)
+        want[(allowed.long()[:, at // 32] >> (at % 32)) % 2 == 0] = -math.inf
+    return want, half * 1.01 * want.abs().nan_to_num(posinf=0.0) + 4 * 2.0 ** -24 * size
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,width", [(3, 1000, 2048), (3, 1000, 2049), (2, 5003, 4097), (5, 300, 9000), (40, 65027, 9000), (128, 19000, 4096), (128, 19001, 4097), (1, 3000001, 5000),
+                                              (300, 8200, 300), (2, 1300000, 1)])
+@pytest.mark.parametrize("form", ["whole rows", "odd rows", "shared"])
+def test_adjusted_logits_of_long_histories(rows, vocab, width, dtype, form):
+    """Histories of several rounds of a block (2048 tokens, behind a stream 4096), and rows and vocabularies that go by two kernels."""
+    gen = torch.Generator(device="cuda").manual_seed(rows + vocab + width)
+    room = 4 * torch.randn(rows, vocab + 3, device="cuda", generator=gen)
+    x = room.to(dtype)[:, 3:] if form == "odd rows" else room[:, :vocab].to(dtype)
+    tokens = torch.randint(-2, vocab + 2, (rows, width), device="cuda", generator=gen)
+    tokens[:, 1::2] %= 7  # the same ones again and again, in every round
+    tokens[:, 2::5] = vocab - 1
+    lengths, prompts = (torch.randint(0, width + 1, (rows,), device="cuda", generator=gen, dtype=torch.int32) for _ in range(2))
+    lengths[0], prompts[0] = width, 0
+    lengths[-1], prompts[-1] = width, width // 2
+    r, f, p = (torch.rand(rows, device="cuda", generator=gen) + low for low in (0.6, 0.0, -0.5))
+    bias = None if form == "odd rows" else torch.randn(*(() if form == "shared" else (rows,)), vocab, device="cuda", generator=gen).to(BF16 if form == "shared" else torch.float32)
+    allowed = None if form == "shared" else torch.randint(-2 ** 31, 2 ** 31, (rows, (vocab + 31) // 32), device="cuda", generator=gen, dtype=torch.int64).int()
+    args = (x, tokens, lengths, prompts, r, f, p, bias, allowed)
+    want, tol = logits64(*args)
+    for _ in range(3):
+        got = OF.adjust_logits(*args)
+        off = (got.double() - want).abs()
+        bad = ~((off <= tol) | (got.double() == want))
+        assert not bad.any(), f"{int(bad.sum())} off, first at {bad.nonzero()[0].tolist()}: {got[bad][0].item()} for {want[bad][0].item()} +- {tol[bad][0].item():.3g}"
+    assert status_of() == 0
+
+
 def _adjust(x, out, tokens=None, bias=None):
     status = native().device_state(x.device).status
     a = native().AdjustLogits(logits=x.data_ptr(), out=out.data_ptr(), status=status.data_ptr(), logits_ld=x.stride(0), out_ld=out.stride(0), rows=x.shape[0], vocab=x.shape[1],
