@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from paged_cases import BF16, attention64, batch, numbers, within
+from paged_cases import BF16, attention64, batch, numbers, turned64, within
 from tensor_parallel_b200.ops import functional as OF
 
 pytestmark = pytest.mark.gpu
@@ -167,3 +167,59 @@ def test_where_the_c_entry_writes_results(rows, vocab):
     _adjust(x, x, None, bias)
     torch.cuda.synchronize()
     assert torch.equal(x, given + bias)
+
+
+# -- append ----------------------------------------------------------------------------------------
+
+
+def ragged(tokens, most, seed):
+    """Numbers of new tokens that add up to ``tokens``, up to ``most`` each, some of them none."""
+    gen = torch.Generator().manual_seed(seed)
+    new = []
+    while tokens:
+        new.append(min(tokens, int(torch.randint(0, most + 1, (), generator=gen))))
+        tokens -= new[-1]
+    return new
+
+
+@pytest.mark.parametrize("tokens", [591, 592, 1183, 1184, 1185, 4735, 4736, 4739])
+@pytest.mark.parametrize("heads,kv_heads,dim,turn,norms", [(8, 2, 64, None, True), (6, 2, 128, (128, False), True), (5, 1, 64, (32, True), False), (4, 4, 32, (20, False), True), (3, 1, 256, (256, True), False)])
+def test_append_of_several_tokens_to_a_block(tokens, heads, kv_heads, dim, turn, norms):
+    """A token's rows over several blocks, one, two and eight tokens to a block, the last block's fewer, sequences that begin and end inside of blocks, rows of no sequence."""
+    front, rest = 3, 6
+    new = ragged(tokens - front - rest, 211, tokens + dim)
+    gen = torch.Generator().manual_seed(dim)
+    past = torch.randint(0, 400, (len(new),), generator=gen).tolist()
+    past[1] = 100003
+    b = batch(new, past, heads, kv_heads, dim, 16, device="cuda", seed=tokens, front=front, rest=rest, junk=0.5, only_new=True)
+    assert b["q"].shape[0] == tokens
+    rotary = None if turn is None else OF.Rotary(OF.rotary(turn[0], device="cuda").frequencies, turn[1], 1.25)
+    norm = (1 + numbers(gen, dim, scale=0.2)).cuda() if norms else None
+    before = b["keys"].clone(), b["values"].clone()
+    for given in (None, torch.full_like(b["q"], 3.0)):
+        q = OF.paged_append(cache_of(b), b["q"], b["k"], b["v"], b["starts"], b["past"], rotary=rotary, q_norm=norm, k_norm=norm, out=given)
+        outside = torch.cat((q[:front], q[tokens - rest:]))
+        assert (outside == (0 if given is None else 3)).all()
+        check_append_at_once(b, q[front:tokens - rest], before, rotary, norm)
+        if given is not None:
+            assert torch.equal(q[front:tokens - rest], first)
+        first = q[front:tokens - rest]
+    assert status_of() == 0
+
+
+def check_append_at_once(b, q, before, rotary, norm, eps=1e-6):
+    """As ``check_append``, all tokens at a time: ``q`` holds those of the sequences."""
+    starts, past, page = b["starts"].long(), b["past"].long(), b["keys"].shape[2]
+    first, last = int(starts[0]), int(starts[-1])
+    of = torch.repeat_interleave(torch.arange(len(past), device=q.device), starts[1:] - starts[:-1])
+    at = past[of] + torch.arange(first, last, device=q.device) - starts[of]
+    want, tol = turned64(b["q"][first:last], norm, eps, at, rotary)
+    within(q, want, tol, "queries")
+    pages, slots = b["table"][of, at // page].long(), at % page
+    want, tol = turned64(b["k"][first:last], norm, eps, at, rotary)
+    within(b["keys"][pages, :, slots], want, tol, "keys")
+    assert torch.equal(b["values"][pages, :, slots], b["v"][first:last])
+    for now, then in zip((b["keys"], b["values"]), before):
+        then = then.clone()
+        then[pages, :, slots] = now[pages, :, slots]
+        assert torch.equal(now.view(torch.int16), then.view(torch.int16))
