@@ -684,7 +684,7 @@ def paged_append(cache: PagedCache, q, k, v, starts, past, rotary: Optional[Rota
     _serving_only("paged_append", cache[0], cache[1], q, k, v, q_norm, k_norm, out)
     _not_captured("paged_append")
     nat = _native(k)
-    if nat is not None and nat.paged_append_supported(cache, q, k, out):
+    if nat is not None and nat.paged_append_supported(cache, q, k, v, out):
         return nat.paged_append(cache, q, k, v, starts, past, rotary, q_norm, k_norm, eps, out)
     return paged_append_ref(PagedCache(*cache), q, k, v, starts, past, None if rotary is None else Rotary(*rotary), q_norm, k_norm, eps, out)
 

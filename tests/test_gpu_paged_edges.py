@@ -223,3 +223,24 @@ def check_append_at_once(b, q, before, rotary, norm, eps=1e-6):
         then = then.clone()
         then[pages, :, slots] = now[pages, :, slots]
         assert torch.equal(now.view(torch.int16), then.view(torch.int16))
+
+
+def test_a_cache_with_heads_outside_of_pages_beyond_32_bits():
+    """``[kv_heads, pages, page_size, head_dim]`` with 4 GB between heads, values behind the keys of each."""
+    if torch.cuda.get_device_properties(0).total_memory < 20 << 30:
+        pytest.skip("needs 5 GB")
+    small = batch([1, 70], [130, 40], 8, 2, 64, 16, device="cuda", junk=0.0)
+    pages, apart = small["keys"].shape[0], 2 ** 31 + 64 * 8
+    room = torch.zeros(apart + 2 * small["keys"].numel(), dtype=BF16, device="cuda")
+    far = dict(small)
+    for name, at in (("keys", 0), ("values", pages * 16 * 64)):
+        far[name] = room.as_strided(small["keys"].shape, (16 * 64, apart, 64, 1), at)
+        far[name].copy_(small[name])
+    want, tol = attention64(small)
+    within(attend(far), want, tol)
+    turn = OF.rotary(64, device="cuda")
+    before = far["keys"].clone(), far["values"].clone()
+    launches = native().launch_count
+    q = OF.paged_append(cache_of(far), far["q"], far["k"], far["v"], far["starts"], far["past"], rotary=turn)
+    assert native().launch_count == launches + 1
+    check_append_at_once(far, q, before, turn, None)

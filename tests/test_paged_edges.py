@@ -82,3 +82,22 @@ def test_results_over_the_logits_are_refused_in_c(dtype):
         assert _adjust(x, room[:4, 72:].as_strided((4, 64), (128, 1), 72), history) == err_arg  # beyond the gap
         assert _adjust(x, room.as_strided((4, 64), (64, 1)), history) == err_arg                # another pitch
         assert _adjust(x[:1], room[:1, 63:127], history) == err_arg
+
+
+def test_which_strides_the_append_kernel_takes():
+    """Up to 64 GB between tokens and between heads of the cache, any number between pages; what is further apart goes by its steps."""
+    from tensor_parallel_b200.ops import native
+
+    def held(shape, strides):
+        return torch.empty_strided(shape, strides, dtype=torch.bfloat16, device="meta")
+
+    limit = native.APPEND_STRIDE
+    rows, table = held((3, 2, 64), (128, 64, 1)), torch.zeros(1, 2, dtype=torch.int32)
+    near = held((2, 2, 16, 64), (2 * limit, limit - 8, 64, 1))
+    assert native.paged_append_supported((near, near, table), rows, rows, rows, None)
+    far = held((2, 2, 16, 64), (1024, limit, 64, 1))
+    assert not native.paged_append_supported((far, near, table), rows, rows, rows, None)
+    assert not native.paged_append_supported((near, far, table), rows, rows, rows, None)
+    wide = held((3, 2, 64), (limit, 64, 1))
+    for args in ((wide, rows, rows, None), (rows, wide, rows, None), (rows, rows, wide, None), (rows, rows, rows, wide)):
+        assert not native.paged_append_supported((near, near, table), *args)
