@@ -73,7 +73,7 @@ def generate(model, input_ids: Optional[torch.Tensor] = None, max_new_tokens: in
         logits = out["logits"][:, -1].float().to(ids.device)
         if adjusts:
             allowed = allowed_tokens(ids) if callable(allowed_tokens) else allowed_tokens
-            history = (None, None) if all(p is None for p in penalties) else (ids, prompt_lengths)
+            history = (None, None) if all(p is None for p in penalties) else (ids.long(), prompt_lengths)
             logits = OF.adjust_logits(logits, history[0], None, history[1], *penalties, bias=None if logit_bias is None else logit_bias.to(logits.device),
                                       allowed=None if allowed is None else allowed.to(logits.device))
         if do_sample:

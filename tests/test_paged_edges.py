@@ -101,3 +101,15 @@ def test_which_strides_the_append_kernel_takes():
     wide = held((3, 2, 64), (limit, 64, 1))
     for args in ((wide, rows, rows, None), (rows, wide, rows, None), (rows, rows, wide, None), (rows, rows, rows, wide)):
         assert not native.paged_append_supported((near, near, table), *args)
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_generate_with_penalties_takes_prompts_of_either_type(kind):
+    from tensor_parallel_b200.models.llama import LlamaConfig, LlamaForCausalLM
+
+    torch.manual_seed(0)
+    model = LlamaForCausalLM(LlamaConfig(vocab_size=50, hidden_size=32, intermediate_size=48, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2)).eval()
+    prompt = torch.tensor([[3, 7, 9], [11, 3, 3]])
+    want = model.generate(prompt, max_new_tokens=5, repetition_penalty=1.4, presence_penalty=0.5)
+    assert torch.equal(model.generate(prompt.to(kind), max_new_tokens=5, repetition_penalty=1.4, presence_penalty=0.5).long(), want)
+    assert model.generate(prompt.to(kind), max_new_tokens=5, repetition_penalty=1.4).dtype == model.generate(prompt.to(kind), max_new_tokens=5).dtype
