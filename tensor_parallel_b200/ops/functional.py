@@ -695,7 +695,7 @@ def paged_attention(q, cache: PagedCache, starts, past, scale: Optional[float] =
     ``q`` is ``[tokens, heads, head_dim]``; ``starts`` and ``past`` as for :func:`paged_append`, ``past`` not counting the new tokens: row ``starts[s] + i`` sees keys ``0`` to
     ``past[s] + i`` of sequence ``s``, or the last ``window`` of them.  One token of each sequence is a decode step, a whole prompt is a prefill, and
     sequences of both kinds may be in one batch.  ``most_new`` says how many new tokens any sequence has at most, where the caller knows (the launches
-    are chosen by it; without it those for prompts are made too).  A call has a workspace of up to 40 MB.  What lies in the cache outside of a sequence's keys has no influence, whatever it is, and pages that have left every token's window are not
+    are chosen by it; without it those for prompts are made too).  A call has a workspace of up to 51 MB.  What lies in the cache outside of a sequence's keys has no influence, whatever it is, and pages that have left every token's window are not
     read; a sequence's own keys and values have to be finite (one that is not may reach any of its new tokens).  A row of queries with scores that are not finite gives NaN.
 
     The result is a new tensor, zero in rows outside all sequences, or ``out`` (which may be ``q``), left as it is there.  A sequence whose rows or table

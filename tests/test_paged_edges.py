@@ -113,3 +113,17 @@ def test_generate_with_penalties_takes_prompts_of_either_type(kind):
     want = model.generate(prompt, max_new_tokens=5, repetition_penalty=1.4, presence_penalty=0.5)
     assert torch.equal(model.generate(prompt.to(kind), max_new_tokens=5, repetition_penalty=1.4, presence_penalty=0.5).long(), want)
     assert model.generate(prompt.to(kind), max_new_tokens=5, repetition_penalty=1.4).dtype == model.generate(prompt.to(kind), max_new_tokens=5).dtype
+
+
+def test_the_workspace_is_within_its_documented_bound():
+    from tensor_parallel_b200.ops import native
+
+    bound = int(OF.paged_attention.__doc__.split("a workspace of up to ")[1].split(" MB")[0]) * 10 ** 6
+    most = 0
+    for dim in (64, 128):
+        for group in (1, 2, 3, 4, 7, 8, 15, 16, 17, 31, 32, 33, 64, 65, 71, 128):
+            for kv_heads in (1, 8, 64):
+                for n, tokens, most_new in ((1, 1, 1), (1, 100000, 100000), (7, 64, 64), (256, 256, 1), (4096, 4096, 4096), (3, 300, 5), (50, 60, 16)):
+                    for width in (1, 2, 1000, 100000):
+                        most = max(most, native.LIB.tpb_paged_attention_workspace(n, tokens, width, 16, most_new, kv_heads, group, dim))
+    assert 0.9 * bound < most <= bound, most
