@@ -458,7 +458,7 @@ Tensor paged_attention(const Tensor& q, const Pages& p, double scale, int64_t wi
   a.page_size = int(p.keys->size(2)), a.table_width = int(p.table->size(1)), a.window = int(std::min<int64_t>(window, 1 << 30)), a.most_new = int(most);
   a.fill_rest = !given.defined(), a.scale = scale == 0. ? float(1. / std::sqrt(double(dim))) : float(scale);
   check(lib.paged_attention(&a, stream_of(q)), "tpb_paged_attention");
-  launched.fetch_add(2, std::memory_order_relaxed);
+  launched.fetch_add(a.launches, std::memory_order_relaxed);
   return out;
 }
 
@@ -555,7 +555,7 @@ Tensor adjust_logits(const Tensor& x, const Tensor& tokens, const Tensor& length
   if (bias.defined()) a.bias = bias.const_data_ptr(), a.bias_ld = bias.dim() == 2 ? bias.stride(0) : 0, a.bias_dtype = bias.scalar_type() == at::kFloat;
   if (allowed.defined()) a.allowed = allowed.const_data_ptr<int>(), a.allowed_ld = allowed.dim() == 2 ? allowed.stride(0) : 0;
   check(lib.adjust_logits(&a, stream_of(x)), "tpb_adjust_logits");
-  launched.fetch_add(1, std::memory_order_relaxed);
+  launched.fetch_add(a.launches, std::memory_order_relaxed);
   return out;
 }
 

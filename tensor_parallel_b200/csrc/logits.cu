@@ -275,12 +275,13 @@ static int lg_seen(const LogitsParams& p, int rows, int part, int parts, cudaStr
 }
 
 template <typename T>
-static int lg_launch(const LogitsParams& p, int rows, cudaStream_t stream) {
+static int lg_launch(const LogitsParams& p, int rows, cudaStream_t stream, int& launches) {
   constexpr int N = Vec<T>::N;
   auto place = [](const void* t) { return reinterpret_cast<uintptr_t>(t) / sizeof(T) % N; };
   const bool wide = place(p.logits) == place(p.out) && (rows == 1 || (p.logits_ld - p.out_ld) % N == 0);
   const bool history = p.tokens && p.width;
   const long long entries = (long long)p.vocab + N - 1;
+  launches = 1;
   if (history && rows * entries <= 148LL * 4 * LG_ALONE) {
     // short parts for each SM to have one, in whole vectors
     const long long blocks = max(1LL, 148LL * 2 / rows);
@@ -290,6 +291,7 @@ static int lg_launch(const LogitsParams& p, int rows, cudaStream_t stream) {
   }
   const int rc = wide ? lg_stream<T, true>(p, rows, stream) : lg_stream<T, false>(p, rows, stream);
   if (rc != TPB_OK || !history) return rc;
+  launches = 2;
   // as few parts as fit where there are blocks enough for the SMs, shorter ones else
   const long long parts = max((p.vocab + (long long)LG_ENTRIES - 1) / LG_ENTRIES, min(148LL / rows, (p.vocab + 4095LL) / 4096));
   const int part = int((((p.vocab + parts - 1) / parts) + 3) / 4 * 4);
@@ -316,7 +318,7 @@ static bool lg_places(const tpb_adjust_logits_t& a) {
 
 using namespace tpb;
 
-extern "C" int tpb_adjust_logits(const tpb_adjust_logits_t* a, void* stream_) {
+extern "C" int tpb_adjust_logits(tpb_adjust_logits_t* a, void* stream_) {
   if (!a || !a->logits || !a->out || !a->status || a->rows <= 0 || a->vocab <= 0 || a->width < 0 || a->dtype < 0 || a->dtype > 1) return TPB_ERR_ARG;
   if (a->vocab > 1 << 30) return TPB_ERR_SIZE;
   if (!lg_places(*a)) return TPB_ERR_ARG;
@@ -324,5 +326,5 @@ extern "C" int tpb_adjust_logits(const tpb_adjust_logits_t* a, void* stream_) {
                     static_cast<uint32_t*>(a->status), a->logits_ld, a->out_ld, a->tokens_ld, a->bias_ld, a->allowed_ld, a->vocab, a->width, a->bias_dtype,
                     a->repetition_all, a->frequency_all, a->presence_all};
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
-  return a->dtype ? lg_launch<float>(p, a->rows, s) : lg_launch<bf16>(p, a->rows, s);
+  return a->dtype ? lg_launch<float>(p, a->rows, s, a->launches) : lg_launch<bf16>(p, a->rows, s, a->launches);
 }

@@ -683,7 +683,7 @@ extern "C" long long tpb_paged_attention_workspace(int n, int tokens, int table_
   return (plan.few_floats + plan.wide_floats) * 4;
 }
 
-extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
+extern "C" int tpb_paged_attention(tpb_paged_attn_t* a, void* stream_) {
   if (!a || !a->q || !a->out || !a->keys || !a->values || !a->table || !a->starts || !a->past || !a->status || !a->workspace) return TPB_ERR_ARG;
   if (a->n <= 0 || a->tokens <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || a->pages <= 0 || a->table_width <= 0 || a->window < 0 ||
       a->most_new < 0)
@@ -700,6 +700,7 @@ extern "C" int tpb_paged_attention(const tpb_paged_attn_t* a, void* stream_) {
   const int group = a->heads / a->kv_heads;
   const PagedPlan plan = pa_plan(a->n, a->tokens, a->table_width, shift, a->most_new, a->kv_heads, group, a->head_dim);
   if (a->workspace_bytes < (plan.few_floats + plan.wide_floats) * 4) return TPB_ERR_WORKSPACE;
+  a->launches = (plan.few_grid != 0) + (plan.wide_grid != 0) + plan.joins;
   PagedAttnParams p = {};
   p.b = {a->starts, a->past, a->table, a->table_ld, a->n, a->tokens, a->table_width, a->pages, shift, a->most_new, static_cast<uint32_t*>(a->status)};
   p.q = static_cast<const bf16*>(a->q);

@@ -169,10 +169,11 @@ typedef struct {
   int most_new;   // new tokens of a sequence, at most
   int fill_rest;  // rows outside all sequences become zeros (else they stay as they are)
   float scale;    // positive
+  int launches;   // result: kernels launched
 } tpb_paged_attn_t;
 long long tpb_paged_attention_workspace(int n, int tokens, int table_width, int page_size, int most_new, int kv_heads, int group, int head_dim);
 // out[t, h] = softmax over the keys up to t's own, window of them at most.  head_dim 64 or 128.
-int tpb_paged_attention(const tpb_paged_attn_t* args, void* stream);
+int tpb_paged_attention(tpb_paged_attn_t* args, void* stream);
 
 // New tokens into a paged cache: k, after an RMSNorm of each head (k_norm, may be null) and the rotation of its position, and v are written to the slots past[s],
 // past[s] + 1, ... of sequence s; q_out gets q, normed and rotated (may be q itself).  Rotation: pairs (i, i + rotary_dim / 2), interleaved (2i, 2i + 1),
@@ -218,8 +219,9 @@ typedef struct {
   long long logits_ld, out_ld, tokens_ld, bias_ld, allowed_ld;
   int rows, vocab, width, dtype, bias_dtype;
   float repetition_all, frequency_all, presence_all;
+  int launches;  // result: kernels launched
 } tpb_adjust_logits_t;
-int tpb_adjust_logits(const tpb_adjust_logits_t* args, void* stream);
+int tpb_adjust_logits(tpb_adjust_logits_t* args, void* stream);
 
 // Sizes of the structures above as this library was built (plan, reduction context, options: one byte-count per 16 bits; the three of ragged batches in the
 // last, added up), and the version of the signatures that are called from elsewhere (1: tpb_rows_int8 takes `ahead`), for callers that are built apart from it.

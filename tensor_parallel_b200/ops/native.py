@@ -879,7 +879,7 @@ class PagedAttn(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("q", "out", "keys", "values", "table", "starts", "past", "status", "workspace")] + [("workspace_bytes", c_ll)]
                 + [(n, c_ll) for n in ("q_st", "q_sh", "o_st", "o_sh", "k_sp", "k_sh", "k_ss", "v_sp", "v_sh", "v_ss", "table_ld")]
                 + [(n, c_int) for n in ("n", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_size", "table_width", "window", "most_new", "fill_rest")]
-                + [("scale", c_float)])
+                + [("scale", c_float), ("launches", c_int)])
 
 
 class PagedAppend(ctypes.Structure):
@@ -893,7 +893,7 @@ class AdjustLogits(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("logits", "out", "tokens", "lengths", "prompts", "repetition", "frequency", "presence", "bias", "allowed", "status")]
                 + [(n, c_ll) for n in ("logits_ld", "out_ld", "tokens_ld", "bias_ld", "allowed_ld")]
                 + [(n, c_int) for n in ("rows", "vocab", "width", "dtype", "bias_dtype")]
-                + [(n, c_float) for n in ("repetition_all", "frequency_all", "presence_all")])
+                + [(n, c_float) for n in ("repetition_all", "frequency_all", "presence_all")] + [("launches", c_int)])
 
 
 LIB.tpb_paged_attention_workspace.argtypes = [c_int] * 8
@@ -992,7 +992,7 @@ def paged_attention(q, cache, starts, past, scale, window, most_new, out):
         (a.q_st, a.q_sh), (a.o_st, a.o_sh) = _strides(q, 2), _strides(out, 2)
         (a.k_sp, a.k_sh, a.k_ss), (a.v_sp, a.v_sh, a.v_ss) = _strides(keys, 3), _strides(values, 3)
         check(LIB.tpb_paged_attention(ctypes.byref(a), _stream()), "tpb_paged_attention")
-    _launches += 2
+    _launches += a.launches
     return out
 
 
@@ -1030,7 +1030,7 @@ def adjust_logits(logits, tokens, lengths, prompt_lengths, repetition, frequency
             t = dense(allowed)
             a.allowed, a.allowed_ld = _ptr(t), t.stride(0) if t.ndim == 2 else 0
         check(LIB.tpb_adjust_logits(ctypes.byref(a), _stream()), "tpb_adjust_logits")
-    _launches += 1
+    _launches += a.launches
     return out
 
 

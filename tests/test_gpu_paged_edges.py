@@ -244,3 +244,35 @@ def test_a_cache_with_heads_outside_of_pages_beyond_32_bits():
     q = OF.paged_append(cache_of(far), far["q"], far["k"], far["v"], far["starts"], far["past"], rotary=turn)
     assert native().launch_count == launches + 1
     check_append_at_once(far, q, before, turn, None)
+
+
+# -- launches --------------------------------------------------------------------------------------
+
+
+def launches_of(call):
+    """Kernels that ``launch_count`` adds for a call, and those that a profile of it shows."""
+    call()
+    torch.cuda.synchronize()
+    before = native().launch_count
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as seen:
+        call()
+        torch.cuda.synchronize()
+    return native().launch_count - before, sum(e.count for e in seen.key_averages() if "tpb::" in e.key)
+
+
+@pytest.mark.parametrize("new,past,heads,most_new,kernels", [([1], [100], 4, 1, 1), ([1], [5000], 4, 1, 2), ([1, 1], [5000, 3], 4, None, 2), ([70], [5], 4, 70, 2), ([70, 1], [5, 900], 4, None, 3),
+                                                             ([1, 1], [30, 40], 71, 1, 2)])
+@pytest.mark.parametrize("directly", [True, False])
+def test_launches_of_the_attention(new, past, heads, most_new, kernels, directly):
+    b = batch(new, past, heads, 1, 64, 16, device="cuda")
+    scale = 1.0 if directly else 1  # (a whole number goes on in Python)
+    counted, seen = launches_of(lambda: OF.paged_attention(b["q"], cache_of(b), b["starts"], b["past"], scale=scale, most_new=most_new))
+    assert counted == kernels and seen in (0, kernels)  # (0: no profiler on this machine)
+
+
+@pytest.mark.parametrize("rows,vocab,width,kernels", [(2, 1000, 9, 1), (128, 19000, 0, 1), (128, 19000, 9, 2)])
+@pytest.mark.parametrize("penalty", [1.25, 1])
+def test_launches_of_adjusted_logits(rows, vocab, width, kernels, penalty):
+    x, tokens = torch.zeros(rows, vocab, device="cuda"), torch.zeros(rows, width, dtype=torch.int64, device="cuda")
+    counted, seen = launches_of(lambda: OF.adjust_logits(x, tokens, repetition=penalty))  # (a whole number goes on in Python)
+    assert counted == kernels and seen in (0, kernels)
