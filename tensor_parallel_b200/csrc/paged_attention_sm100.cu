@@ -500,7 +500,7 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           m_run = m_tile;  // nothing accumulated for this row yet
           factor = 0.f;    // (but 2^-140 in the sum for some keys of a tile in which it saw none)
           rescale = j > 0;
-        } else if (!(m_tile <= m_run + (j * N < PW_EXACT_KEYS ? 0.f : PW_RESCALE_LOG2))) {
+        } else if (m_run == m_run && !(m_tile <= m_run + (j * N < PW_EXACT_KEYS ? 0.f : PW_RESCALE_LOG2))) {  // (a row that is NaN stays it, and calls for no more rescaling)
           factor = ex2_approx(m_run - m_tile);
           m_run = m_tile;
           rescale = true;
