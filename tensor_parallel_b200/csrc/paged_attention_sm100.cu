@@ -275,7 +275,6 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         int entry0 = tile0 * N >> p.b.page_shift;
         auto fetch = [&](int e) { return e < entries ? __ldg(row + e) : -1; };
         int now = fetch(entry0 + lane), next = fetch(entry0 + 32 + lane);
-        bool whole = true;
         for (int j = 0; ok && j < n; ++j, ++kt) {
           const int s = kt & 1, key0 = (tile0 + j) * N;
           const uint32_t par = ((kt >> 1) & 1) ^ 1;
@@ -291,12 +290,10 @@ paged_attn_wide_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           const bool wanted = lane < per_tile * DB && (per_tile == 1 || (first < total && first + page_size > low));
           const bool good = wanted && page >= 0 && page < p.b.pages;
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, good)) * box_rows * 128;
-          if (whole && __any_sync(0xffffffffu, wanted && !good)) {
-            whole = false;
-            if (lane == 0) {
-              atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
-              *reinterpret_cast<volatile unsigned long long*>(lost + i % PW_LOST) = static_cast<unsigned long long>(i + 1) << 32 | unsigned(j);
-            }
+          if (__any_sync(0xffffffffu, wanted && !good) && lane == 0) {
+            atomicMax(p.b.status, uint32_t(STATUS_BAD_ARG));
+            volatile unsigned long long* record = lost + i % PW_LOST;
+            if (int(*record >> 32) != i + 1) *record = static_cast<unsigned long long>(i + 1) << 32 | unsigned(j);
           }
           const uint32_t to = my_block * (N * 128) + my_page * box_rows * 128;
           const int slot = per_tile == 1 ? key0 & (page_size - 1) : 0;
