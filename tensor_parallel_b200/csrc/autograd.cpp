@@ -485,8 +485,8 @@ Queries paged_append(const Pages& p, const Tensor& q, const Tensor& k, const Ten
   if (q.defined() && (!rows_like(q, -1, p, tokens) || q.size(1) == 0)) return Queries::not_taken;
   if (given.defined() && (!q.defined() || !rows_like(given, q.size(1), p, tokens) || !written_once(given))) return Queries::not_taken;
   for (const Tensor* t : {&q, &k, &v, &given})
-    if (t->defined() && (step(*t, 0) >= TPB_APPEND_STRIDE || step(*t, 1) >= TPB_APPEND_STRIDE)) return Queries::not_taken;
-  if (step(*p.keys, 1) >= TPB_APPEND_STRIDE || step(*p.values, 1) >= TPB_APPEND_STRIDE) return Queries::not_taken;
+    if (t->defined() && (step(*t, 0) >= TPB_APPEND_ROW_STRIDE || step(*t, 1) >= TPB_APPEND_ROW_STRIDE)) return Queries::not_taken;
+  if (step(*p.keys, 1) >= TPB_APPEND_HEAD_STRIDE || step(*p.values, 1) >= TPB_APPEND_HEAD_STRIDE) return Queries::not_taken;
   const bool makes = q.defined() && (turn.frequencies.defined() || q_norm.defined() || given.defined());
   const py::gil_scoped_release unlocked;
   const c10::cuda::CUDAGuard guard(device);

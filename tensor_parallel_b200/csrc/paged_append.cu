@@ -27,13 +27,12 @@ constexpr int AP_TOKENS = 8;      // of a block, at most: one per warp
 
 struct AppendParams {
   PagedBatch b;
-  const uint4 *q, *k, *v;
-  const bf16 *q_norm, *k_norm;
-  uint4 *q_out, *keys, *values;
+  const bf16 *q, *k, *v, *q_norm, *k_norm;
+  bf16 *q_out, *keys, *values;
   const float* frequencies;
-  // strides in 16 bytes: pointers are one 32 x 32 + 64 bit product away, and 64 GB of a head of the cache or between tokens are within reach
   long long k_sp, k_ss, v_sp, v_ss;
-  unsigned q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, k_shead, v_shead;
+  int q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;  // (pointers then are one 32 x 32 + 64 bit product away)
+  unsigned k_shead, v_shead;                           // in 16 bytes, so that 64 GB between heads are within reach (those of the rows as well: 89 us for 87, more spills)
   int q_heads, kv_heads, head_dim, half, interleaved, fill_rest;  // q_heads 0: q is left alone
   float factor, eps, inv_dim;
 };
@@ -62,12 +61,10 @@ __device__ __forceinline__ int sequence_of(const PagedBatch& b, int t, int lane)
   return low - 1;
 }
 
-__device__ __forceinline__ unsigned long long ap_times(unsigned i, unsigned stride) { return static_cast<unsigned long long>(i) * stride; }
-
 struct AppendPlace {  // of a token
   int position;
   int inside;           // of a sequence
-  long long k_at, v_at; // in 16 bytes; -1: not stored
+  long long k_at, v_at; // -1: not stored
 };
 
 // How the elements of a pair lie: none are turned; a multiple of eight apart; side by side; any other distance apart.
@@ -104,19 +101,18 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
   };
   auto source = [&](const Cursor& c) {
     const bool is_q = c.r < p.q_heads, is_k = c.r < p.q_heads + p.kv_heads;
-    const uint4* base = is_q ? p.q : is_k ? p.k : p.v;
-    const unsigned st = is_q ? p.q_st : is_k ? p.k_st : p.v_st, sh = is_q ? p.q_sh : is_k ? p.k_sh : p.v_sh;
-    const unsigned r = is_q ? c.r : is_k ? c.r - p.q_heads : c.r - p.q_heads - p.kv_heads;
-    return base + ap_times(t0 + c.t, st) + ap_times(r, sh);
+    const bf16* base = is_q ? p.q : is_k ? p.k : p.v;
+    const int st = is_q ? p.q_st : is_k ? p.k_st : p.v_st, sh = is_q ? p.q_sh : is_k ? p.k_sh : p.v_sh, r = is_q ? c.r : is_k ? c.r - p.q_heads : c.r - p.q_heads - p.kv_heads;
+    return base + (long long)(t0 + c.t) * st + (long long)r * sh;
   };
   constexpr int AHEAD = 2;  // rows on their way (three, in three blocks per SM: 88 -> 90 us, 32 KV heads 151 -> 157)
   uint4 raw[AHEAD][2];
   Cursor next = {i0 / rows, i0 % rows}, at = next;
   auto fetch = [&](uint4 (&u)[2]) {
     if (next.t < tokens) {
-      const uint4* src = source(next);
-      if (on0) u[0] = src[c0];
-      if (on1) u[1] = src[c1];
+      const bf16* src = source(next);
+      if (on0) u[0] = *reinterpret_cast<const uint4*>(src + c0 * 8);
+      if (on1) u[1] = *reinterpret_cast<const uint4*>(src + c1 * 8);
     }
     step(next);
   };
@@ -175,13 +171,13 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
   auto finish = [&](const Cursor& c, const uint4 (&u)[2]) {
     const bool there = c.t < tokens, is_q = c.r < p.q_heads, is_v = c.r >= p.q_heads + p.kv_heads;
     const AppendPlace place = places[there ? c.t : 0];
-    uint4* dst = nullptr;
+    bf16* dst = nullptr;
     if (is_q) {
-      if (there && (place.inside || p.fill_rest)) dst = p.q_out + ap_times(t0 + c.t, p.o_st) + ap_times(c.r, p.o_sh);
+      if (there && (place.inside || p.fill_rest)) dst = p.q_out + (long long)(t0 + c.t) * p.o_st + (long long)c.r * p.o_sh;
     } else {
       const long long into = is_v ? place.v_at : place.k_at;
       const int r = c.r - p.q_heads - (is_v ? p.kv_heads : 0);
-      if (there && into >= 0) dst = (is_v ? p.values : p.keys) + into + ap_times(r, is_v ? p.v_shead : p.k_shead);
+      if (there && into >= 0) dst = (is_v ? p.values : p.keys) + into + (static_cast<unsigned long long>(unsigned(r)) * (is_v ? p.v_shead : p.k_shead) << 3);
     }
     uint4 y0 = u[0], y1 = u[1];
     if (__any_sync(0xffffffffu, there && !is_v)) {
@@ -248,7 +244,7 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
         // the partners come from memory once more, before any lane of the warp stores
         auto turn = [&](float (&x)[8], int chunk, bool on) {
           if (!on || !there || is_v) return;
-          const bf16* src = reinterpret_cast<const bf16*>(source(c));
+          const bf16* src = source(c);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int e = chunk * 8 + j;
@@ -271,8 +267,8 @@ paged_append_kernel(const AppendParams p, int tokens_of_block) {
     }
     if (dst) {
       if (!place.inside) y0 = y1 = make_uint4(0, 0, 0, 0);
-      if (on0) dst[c0] = y0;
-      if (on1) dst[c1] = y1;
+      if (on0) *reinterpret_cast<uint4*>(dst + c0 * 8) = y0;
+      if (on1) *reinterpret_cast<uint4*>(dst + c1 * 8) = y1;
     }
   };
 
@@ -315,16 +311,17 @@ extern "C" int tpb_paged_append(const tpb_paged_append_t* a, void* stream_) {
   int shift = 0;
   while ((1 << shift) < a->page_size) ++shift;
   p.b = {a->starts, a->past, a->table, a->table_ld, a->n, a->tokens, a->table_width, a->pages, shift, INT_MAX, static_cast<uint32_t*>(a->status)};
-  p.q = static_cast<const uint4*>(a->q), p.k = static_cast<const uint4*>(a->k), p.v = static_cast<const uint4*>(a->v);
+  p.q = static_cast<const bf16*>(a->q), p.k = static_cast<const bf16*>(a->k), p.v = static_cast<const bf16*>(a->v);
   p.q_norm = static_cast<const bf16*>(a->q_norm), p.k_norm = static_cast<const bf16*>(a->k_norm);
-  p.q_out = static_cast<uint4*>(a->q_out), p.keys = static_cast<uint4*>(a->keys), p.values = static_cast<uint4*>(a->values);
+  p.q_out = static_cast<bf16*>(a->q_out), p.keys = static_cast<bf16*>(a->keys), p.values = static_cast<bf16*>(a->values);
   p.frequencies = a->frequencies;
-  for (const long long t : {a->q_st, a->q_sh, a->k_st, a->k_sh, a->v_st, a->v_sh, a->o_st, a->o_sh, a->k_shead, a->v_shead})
-    if (t / 8 > UINT_MAX || t < 0) return TPB_ERR_SIZE;
-  auto units = [](long long t) { return unsigned(t / 8); };
-  p.q_st = units(a->q_st), p.q_sh = units(a->q_sh), p.k_st = units(a->k_st), p.k_sh = units(a->k_sh), p.v_st = units(a->v_st), p.v_sh = units(a->v_sh);
-  p.o_st = units(a->o_st), p.o_sh = units(a->o_sh), p.k_shead = units(a->k_shead), p.v_shead = units(a->v_shead);
-  p.k_sp = a->k_sp / 8, p.k_ss = a->k_ss / 8, p.v_sp = a->v_sp / 8, p.v_ss = a->v_ss / 8;
+  for (const long long t : {a->q_st, a->q_sh, a->k_st, a->k_sh, a->v_st, a->v_sh, a->o_st, a->o_sh})
+    if (t >= TPB_APPEND_ROW_STRIDE || t < 0) return TPB_ERR_SIZE;
+  for (const long long t : {a->k_shead, a->v_shead})
+    if (t >= TPB_APPEND_HEAD_STRIDE || t < 0) return TPB_ERR_SIZE;
+  p.q_st = int(a->q_st), p.q_sh = int(a->q_sh), p.k_st = int(a->k_st), p.k_sh = int(a->k_sh), p.v_st = int(a->v_st), p.v_sh = int(a->v_sh);
+  p.o_st = int(a->o_st), p.o_sh = int(a->o_sh), p.k_shead = unsigned(a->k_shead / 8), p.v_shead = unsigned(a->v_shead / 8);
+  p.k_sp = a->k_sp, p.k_ss = a->k_ss, p.v_sp = a->v_sp, p.v_ss = a->v_ss;
   p.inv_dim = 1.f / float(a->head_dim);
   p.q_heads = a->q ? a->heads : 0;
   p.kv_heads = a->kv_heads, p.head_dim = a->head_dim, p.half = a->rotary_dim / 2, p.interleaved = a->interleaved, p.fill_rest = a->fill_rest;

@@ -195,9 +195,11 @@ typedef struct {
   long long q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, k_sp, k_shead, k_ss, v_sp, v_shead, v_ss, table_ld;
   int n, tokens, heads, kv_heads, head_dim, pages, page_size, table_width, rotary_dim, interleaved;
   int fill_rest;  // rows of q_out outside all sequences become zeros (else they stay as they are)
-  float factor, eps;  // (strides below TPB_APPEND_STRIDE, but for those of pages and slots)
+  float factor, eps;
 } tpb_paged_append_t;
-#define TPB_APPEND_STRIDE (1ll << 35)
+// Strides of tokens and heads of q, k, v and q_out, and of the cache's heads, are below these numbers of elements.
+#define TPB_APPEND_ROW_STRIDE (1ll << 31)
+#define TPB_APPEND_HEAD_STRIDE (1ll << 35)
 int tpb_paged_append(const tpb_paged_append_t* args, void* stream);
 
 // Logits [rows][vocab] (bf16: dtype 0, fp32: 1) of sequences in front of the pick of a token: x of a token that is among the first `lengths` of its row's

@@ -929,12 +929,12 @@ def _pages_supported(cache, *written) -> bool:
             and all(s > 0 for t in (keys, values) for s, n in zip(t.stride(), t.shape) if n > 1))
 
 
-APPEND_STRIDE = 2 ** 35  # elements (TPB_APPEND_STRIDE)
+APPEND_ROW_STRIDE, APPEND_HEAD_STRIDE = 2 ** 31, 2 ** 35  # elements (TPB_APPEND_ROW_STRIDE, TPB_APPEND_HEAD_STRIDE)
 
 
 def paged_append_supported(cache, q, k, v, out) -> bool:
     page, d = cache[0].shape[2:]
-    near = all(t is None or max(_strides(t, 2)) < APPEND_STRIDE for t in (q, k, v, out)) and all(_strides(t, 2)[1] < APPEND_STRIDE for t in cache[:2])
+    near = all(t is None or max(_strides(t, 2)) < APPEND_ROW_STRIDE for t in (q, k, v, out)) and all(_strides(t, 2)[1] < APPEND_HEAD_STRIDE for t in cache[:2])
     return near and _pages_supported(cache, out) and page & (page - 1) == 0 and d % 8 == 0 and d <= 256 and k.shape[0] > 0 and cache[2].numel() > 0 and (out is None or _vector_rows(out))
 
 

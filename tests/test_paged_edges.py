@@ -85,20 +85,22 @@ def test_results_over_the_logits_are_refused_in_c(dtype):
 
 
 def test_which_strides_the_append_kernel_takes():
-    """Up to 64 GB between tokens and between heads of the cache, any number between pages; what is further apart goes by its steps."""
+    """Up to 64 GB between heads of the cache and 4 GB between rows, any number between pages; what is further apart goes by its steps."""
     from tensor_parallel_b200.ops import native
 
     def held(shape, strides):
         return torch.empty_strided(shape, strides, dtype=torch.bfloat16, device="meta")
 
-    limit = native.APPEND_STRIDE
+    limit = native.APPEND_HEAD_STRIDE
     rows, table = held((3, 2, 64), (128, 64, 1)), torch.zeros(1, 2, dtype=torch.int32)
     near = held((2, 2, 16, 64), (2 * limit, limit - 8, 64, 1))
     assert native.paged_append_supported((near, near, table), rows, rows, rows, None)
     far = held((2, 2, 16, 64), (1024, limit, 64, 1))
     assert not native.paged_append_supported((far, near, table), rows, rows, rows, None)
     assert not native.paged_append_supported((near, far, table), rows, rows, rows, None)
-    wide = held((3, 2, 64), (limit, 64, 1))
+    wide = held((3, 2, 64), (native.APPEND_ROW_STRIDE, 64, 1))
+    rows_apart = held((3, 2, 64), (native.APPEND_ROW_STRIDE - 8, 64, 1))
+    assert native.paged_append_supported((near, near, table), rows_apart, rows_apart, rows_apart, rows_apart)
     for args in ((wide, rows, rows, None), (rows, wide, rows, None), (rows, rows, wide, None), (rows, rows, rows, wide)):
         assert not native.paged_append_supported((near, near, table), *args)
 
