@@ -3,7 +3,7 @@
 // A cache holds keys and values as [pages][kv_heads][page_size][head_dim]; key j of a sequence is slot j % page_size of page table[sequence][j / page_size].
 // The batch is ragged: the new tokens of sequence s are the rows starts[s] .. starts[s + 1] of the queries, behind past[s] cached ones.  Lengths and
 // table live in device memory and change from step to step under a captured graph, so every kernel checks what it reads of them: a sequence that
-// does not fit the rows, the table or the cache is recorded as STATUS_BAD_ARG and answered with NaN, and nothing is read or written through its entries.
+// does not fit the rows, the table or the cache is recorded as STATUS_BAD_ARG and answered with NaN (append: its tokens are not stored), and nothing is read or written through its entries.
 #pragma once
 #include <cuda_bf16.h>
 #include <limits.h>

@@ -15,7 +15,10 @@
 //                   here leaves the tensor cores idle; tcgen05 would fill 128 rows for 1 to 64), its own running maximum and sum; key groups meet at the end of a piece
 //
 // Keys outside a sequence (the rest of its last page, slots that left the window) may hold anything: their scores are replaced, not added to, and
-// their values are cut out of the fragments, so that neither NaN nor infinities get through.
+// their values are cut out of the fragments, so that neither NaN nor infinities get through.  Scores of a row's own keys that are not finite make it NaN.
+//
+// Probabilities are rounded to bf16 for their product (a relative error of 1.6e-3 of ordinary rows beside the 1.65e-3 of the result's own rounding: 2.1 to 2.3e-3 in all), which one product of
+// two bf16 operands asks for.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -645,7 +648,10 @@ static PagedPlan pa_plan(int n, int tokens, int table_width, int page_shift, int
   const long long most_rows = (long long)min(most_new, tokens) * group, keys = (long long)table_width << page_shift;
   const bool wide = most_rows > 64, few = !wide || (n > 1 && group <= 64);
   plan.joins = wide || keys > PA_WHOLE_TILES * PA_TILE;
-  // rows of a tile of the first: all of a sequence's where there are no more than 64, else those of one token
+  // Rows of a tile of the first: all of a sequence's where there are no more than 64, else those of one token, since most sequences of such a batch decode and larger tiles cost
+  // them (32 x 2049 keys, 8 KV heads, 16 rows in tiles of 16 / 32, us: 30.8 / 35.7 at 64, 53.8 / 56.9 at 128).  Sequences with a few tokens more pay for it, in a batch with a chunk or
+  // without most_new: 20 rows, 32 x 2049 keys by this kernel / by the other 35.7 / 67.3 at 64, 56.9 / 90.0 at 128 (64 rows 52.4 / 68.6, 92.2 / 90.9); beside 777 tokens
+  // behind 3396 16 rows 83.8 and 110, 20 rows 109 and 144.
   const long long usual = wide ? group : most_rows;
   plan.row_groups = usual <= 16 ? 1 : usual <= 32 ? 2 : 4;
   const int rows = 16 * plan.row_groups;

@@ -659,6 +659,8 @@ def paged_append(cache: PagedCache, q, k, v, starts, past, rotary: Optional[Rota
 
     The queries come in a tensor of their own, in ``out`` (which may be ``q``), or as they are where nothing is done to them.  Rows in front of the first
     sequence and behind the last (a batch padded to a captured size) are not stored; ``out`` keeps what it has there, and a new tensor holds zeros.
+    The CUDA kernel takes bf16, heads of up to 256 elements in eights and pages of a power of two; other calls go by their steps, which read the lengths on the host (no CUDA graph).
+
     A sequence whose rows, table or pages do not fit is not stored: the CUDA kernel records status 3 (see ``native.device_state``), the steps over
     tensors raise.  Two tokens for one slot (sequences that share the page that they write to) leave either.  Serving only: there is no gradient."""
     if _compiling():
@@ -697,6 +699,8 @@ def paged_attention(q, cache: PagedCache, starts, past, scale: Optional[float] =
     sequences of both kinds may be in one batch.  ``most_new`` says how many new tokens any sequence has at most, where the caller knows (the launches
     are chosen by it; without it those for prompts are made too).  A call has a workspace of up to 51 MB.  What lies in the cache outside of a sequence's keys has no influence, whatever it is, and pages that have left every token's window are not
     read; a sequence's own keys and values have to be finite (one that is not may reach any of its new tokens).  A row of queries with scores that are not finite gives NaN.
+
+    The CUDA kernels take bf16, heads of 64 or 128 elements and pages of a power of two from 16 up; other calls go by their steps, which read the lengths on the host (no CUDA graph).
 
     The result is a new tensor, zero in rows outside all sequences, or ``out`` (which may be ``q``), left as it is there.  A sequence whose rows or table
     do not fit, or with more than ``most_new`` new tokens, gives NaN, as rows do that reach a page outside the cache (and some of those in front of them in its sequence), and the CUDA kernel records status 3

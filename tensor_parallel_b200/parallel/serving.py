@@ -98,7 +98,8 @@ class ServingMixin:
 
     @torch.no_grad()
     def generate(self, input_ids: Optional[torch.Tensor] = None, max_new_tokens: int = 20, quantize: Optional[str] = None, **kwargs):
-        """``quantize``: see :meth:`serving_engine`; ``"int8"`` is for greedy decoding on the engine only."""
+        """``quantize``: see :meth:`serving_engine`; ``"int8"`` is for greedy decoding on the engine only.  Calls with penalties, biases or allowed tokens go by the model's own steps,
+        not by the engine."""
         greedy = not kwargs.get("do_sample", False) and kwargs.get("num_beams", 1) == 1 and not kwargs.get("output_scores", False)
         if input_ids is not None and greedy and set(kwargs) <= {"do_sample", "num_beams", "output_scores"}:
             engine = self.serving_engine(input_ids.shape[0], input_ids.shape[1] + max_new_tokens + 4, quantize)
