@@ -649,7 +649,7 @@ static PagedPlan pa_plan(int n, int tokens, int table_width, int page_shift, int
   const bool wide = most_rows > 64, few = !wide || (n > 1 && group <= 64);
   plan.joins = wide || keys > PA_WHOLE_TILES * PA_TILE;
   // Rows of a tile of the first: all of a sequence's where there are no more than 64, else those of one token, since most sequences of such a batch decode and larger tiles cost
-  // them (32 x 2049 keys, 8 KV heads, 16 rows in tiles of 16 / 32, us: 30.8 / 35.7 at 64, 53.8 / 56.9 at 128).  Sequences with a few tokens more pay for it, in a batch with a chunk or
+  // them (32 x 2049 keys, 8 KV heads, 16 rows in tiles of 16 / 20 in tiles of 32, us: 30.8 / 35.7 at 64, 53.8 / 56.9 at 128).  Sequences with a few tokens more pay for it, in a batch with a chunk or
   // without most_new: 20 rows, 32 x 2049 keys by this kernel / by the other 35.7 / 67.3 at 64, 56.9 / 90.0 at 128 (64 rows 52.4 / 68.6, 92.2 / 90.9); beside 777 tokens
   // behind 3396 16 rows 83.8 and 110, 20 rows 109 and 144.
   const long long usual = wide ? group : most_rows;

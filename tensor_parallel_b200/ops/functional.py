@@ -219,7 +219,7 @@ def rotary(rotary_dim: int, theta: float = 10000.0, interleaved: bool = False, s
     """The usual frequencies ``theta ** (-2i / rotary_dim)``, for contexts longer than a model was trained on scaled as ``scaling`` says (the dictionary of
     a Hugging Face configuration): ``"linear"`` (all slower by ``factor``), ``"llama3"`` (slow ones slower by ``factor``, a ramp between) or ``"yarn"`` (a ramp over the
     pairs, from whole pairs unless ``truncate`` is false, and a factor on cosine and sine: ``attention_factor``, or by ``mscale`` and ``mscale_all_dim`` where both
-    are there).  A ``rope_theta`` in it has to be ``theta``, and a ``partial_rotary_factor`` is what ``rotary_dim`` says already; what else it names is refused."""
+    are there).  A ``rope_theta`` in it has to be ``theta``, a ``partial_rotary_factor`` is what ``rotary_dim`` says already and ``finetuned`` changes no number; what else it names is refused."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"a rotation takes an even number of elements, got {rotary_dim}")
     f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
@@ -228,10 +228,10 @@ def rotary(rotary_dim: int, theta: float = 10000.0, interleaved: bool = False, s
         kind = scaling.get("rope_type", scaling.get("type", "default"))
         if kind not in _SCALING_KEYS:
             raise ValueError(f"scaling of rotary frequencies: 'linear', 'llama3' or 'yarn', got {kind!r}")
-        strange = sorted(set(scaling) - {"rope_type", "type", "rope_theta", "partial_rotary_factor", *_SCALING_KEYS[kind]})
+        strange = sorted(set(scaling) - {"rope_type", "type", "rope_theta", "partial_rotary_factor", "finetuned", *_SCALING_KEYS[kind]})
         if strange:
             raise ValueError(f"scaling of rotary frequencies: {kind!r} does not know {', '.join(map(repr, strange))}")
-        if scaling.get("rope_theta", theta) != theta:
+        if scaling.get("rope_theta") not in (None, theta):
             raise ValueError(f"scaling of rotary frequencies: it says rope_theta={scaling['rope_theta']}, theta is {theta}")
     if kind == "linear":
         f = f / scaling["factor"]

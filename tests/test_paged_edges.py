@@ -42,7 +42,7 @@ def test_yarn_pair_by_pair(dim, theta, more, original):
     # a rounding to fp32, and some in 64 bits
     assert ((got.frequencies.double() - want).abs() <= 2.0 ** -24 * 1.01 * want).all()
     assert got.factor == pytest.approx(factor, rel=1e-14) and isinstance(got.factor, float)
-    assert torch.equal(OF.rotary(dim, theta, scaling=dict(d, rope_theta=theta, partial_rotary_factor=0.5)).frequencies, got.frequencies)
+    assert torch.equal(OF.rotary(dim, theta, scaling=dict(d, rope_theta=theta, partial_rotary_factor=0.5, finetuned=True)).frequencies, got.frequencies)
 
 
 def test_scaling_that_is_not_known_is_refused_by_name():
@@ -52,7 +52,7 @@ def test_scaling_that_is_not_known_is_refused_by_name():
         with pytest.raises(ValueError, match=name):
             OF.rotary(64, scaling=scaling)
     plain = OF.rotary(64)
-    for scaling in (None, {}, dict(rope_type="default"), dict(rope_type="default", rope_theta=10000.0)):
+    for scaling in (None, {}, dict(rope_type="default"), dict(rope_type="default", rope_theta=10000.0), dict(rope_type="default", rope_theta=None)):
         assert torch.equal(OF.rotary(64, scaling=scaling).frequencies, plain.frequencies)
 
 
