@@ -276,3 +276,76 @@ def test_launches_of_adjusted_logits(rows, vocab, width, kernels, penalty):
     x, tokens = torch.zeros(rows, vocab, device="cuda"), torch.zeros(rows, width, dtype=torch.int64, device="cuda")
     counted, seen = launches_of(lambda: OF.adjust_logits(x, tokens, repetition=penalty))  # (a whole number goes on in Python)
     assert counted == kernels and seen in (0, kernels)
+
+
+# -- long contexts, nothing new, graphs and streams ------------------------------------------------
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,new,past,window", [(4, 2, 64, 16, 1, 1000003, None), (8, 1, 128, 64, 1, 700001, None), (2, 2, 64, 256, 300, 200000, None), (2, 1, 128, 16, 70, 300000, 100000),
+                                                                     (8, 1, 64, 16, 1, 2000000, 2999)])
+def test_attention_of_a_million_keys(heads, kv_heads, dim, page, new, past, window):
+    """Pages of a few, again and again (a table may name a page as often as it likes)."""
+    gen = torch.Generator().manual_seed(1)
+    total, pages, group = past + new, 97, heads // kv_heads
+    b = dict(keys=numbers(gen, pages, kv_heads, page, dim).cuda(), values=numbers(gen, pages, kv_heads, page, dim).cuda(), table=torch.randint(0, pages, (1, -(-total // page)), generator=gen).int().cuda(),
+             starts=torch.tensor([0, new], dtype=torch.int32).cuda(), past=torch.tensor([past], dtype=torch.int32).cuda(), q=numbers(gen, new, heads, dim, scale=1.5).cuda())
+    low = 0 if window is None else max(0, past - window + 1) // page * page
+    k, v = (b[name][b["table"][0, low // page:].long(), 0].reshape(-1, dim)[:total - low].double() for name in ("keys", "values"))
+    q = b["q"][:, :group].double()
+    scores = torch.einsum("tgd,jd->gtj", q, k) / math.sqrt(dim)
+    size = (torch.einsum("tgd,jd->gtj", q.abs(), k.abs()) / math.sqrt(dim)).amax(-1).t()[..., None]
+    far = torch.arange(past, total, device="cuda")[:, None] - torch.arange(low, total, device="cuda")[None]
+    p = torch.softmax(scores.masked_fill((far < 0) | (far >= (window or 1 << 40)), -math.inf), -1)
+    want, a = torch.einsum("gtj,jd->tgd", p, v), torch.einsum("gtj,jd->tgd", p, v.abs())
+    # as attention64: probabilities and results to bf16, scores and sums in 32 bits
+    tol = (2.0 ** -8 + 2 * (dim + 4) * 2.0 ** -24 * size + len(k) * 2.0 ** -24) * a * 1.02 + 2.0 ** -8 * want.abs() * 1.02
+    for most_new in (None, new):
+        within(attend(b, window=window, most_new=most_new)[:, :group], want, tol)
+    assert status_of() == 0
+
+
+def test_no_new_tokens_at_all():
+    b = batch([0, 0, 0], [900, 5, 0], 4, 2, 64, 16, device="cuda", rest=5, front=2)
+    for most_new in (0, None):
+        assert not attend(b, most_new=most_new).any()
+        out = torch.full_like(b["q"], 2.0)
+        attend(b, most_new=most_new, out=out)
+        assert (out == 2).all()
+    before = b["keys"].clone()
+    q = OF.paged_append(cache_of(b), b["q"], b["k"], b["v"], b["starts"], b["past"], rotary=OF.rotary(64, device="cuda"))
+    assert not q.any() and torch.equal(b["keys"].view(torch.int16), before.view(torch.int16)) and status_of() == 0
+
+
+def test_captured_logits_of_two_kernels_at_once():
+    """Two graphs, each of a stream and its seen entries, replayed on two streams while histories change."""
+    rows, vocab, width = 130, 19001, 5000
+    gen = torch.Generator(device="cuda").manual_seed(4)
+
+    def make():
+        x, tokens = torch.randn(rows, vocab, device="cuda", generator=gen), torch.randint(-3, vocab + 3, (rows, width), device="cuda", generator=gen)
+        tokens[:, ::2] %= 11
+        lengths, prompts = (torch.randint(0, width + 1, (rows,), device="cuda", generator=gen, dtype=torch.int32) for _ in range(2))
+        args = [x, tokens, lengths, prompts, *(torch.rand(rows, device="cuda", generator=gen) + 0.6 for _ in range(3))]
+        OF.adjust_logits(*args)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = OF.adjust_logits(*args)
+        return args, graph, out, torch.cuda.Stream()
+
+    both = [make(), make()]
+    for _ in range(3):
+        for args, *_ in both:
+            args[0].normal_(generator=gen)
+            args[1].copy_(args[1].roll(7, 1))
+            args[2].copy_((args[2] + 613) % (width + 1))
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for _, graph, _, stream in both:
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for args, _, out, _ in both:
+            want, tol = logits64(*args, None, None)
+            within(out, want, tol)
+    assert status_of() == 0
